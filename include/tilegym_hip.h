@@ -333,6 +333,57 @@ int32_t tg_fp8_fused_moe(const tg_tensor* out, const tg_tensor* hidden, const tg
                          const tg_tensor* topk_ids, const tg_tensor* workspace, int32_t block_m, int32_t device_id,
                          uint64_t hip_stream);
 
+/*
+ * Root-mean-square norm with the residual's addition and an e4m3 output:
+ *   s = x + residual (fp32);  y = s / sqrt(mean(s^2) + eps) * weight;  q = e4m3(clamp(y / scale, -448, 448))
+ * with scale = amax(|y|) / 448 per group of group_size (16 / 32 / 64 / 128) consecutive elements (all-zero group -> 1), written to
+ * scales, or one given scale for the whole tensor.  q is rounded once, from the fp32 norm.
+ *   x (..., H) bf16 / f16 / f32, H % 16 == 0 and H % group_size == 0, H <= 32768; weight (H) of x's type or f32; q (..., H) e4m3fn
+ *   scales (..., H / group_size) f32 and scale NULL, or scale one f32 and scales NULL (group_size is then ignored)
+ *   residual, residual_out (s rounded to x's type), norm_out (y rounded to x's type): shape and type of x, or NULL.  residual_out may
+ *   be residual or x, norm_out may be x.
+ * All contiguous; x, weight and the optional tensors 16-byte aligned, q 8-byte.
+ */
+int32_t tg_fp8_rms_norm_quant(const tg_tensor* q, const tg_tensor* scales, const tg_tensor* norm_out, const tg_tensor* residual_out,
+                              const tg_tensor* x, const tg_tensor* weight, const tg_tensor* residual, const tg_tensor* scale, float eps,
+                              int32_t group_size, int32_t device_id, uint64_t hip_stream);
+
+/*
+ * A paged e4m3 cache of keys and values, with one scale per page and head:
+ *   k_cache (pages, heads, P, D), v_cache (pages, heads, D, P) e4m3fn: v is transposed inside a page; P 16, 32, 64 or 128, D 64, 128 or 256
+ *   k_scale, v_scale (pages, heads) f32: element = code * scale
+ *   block_table (B, W) int32: position p of sequence b is slot p % P of page block_table[b][p / P]
+ *   seq_lens (B) int32: tokens of each sequence, the new ones among them
+ *   indptr (B + 1) int32, ascending: rows indptr[b] .. indptr[b + 1] of the packed tensors belong to sequence b.  They are its last
+ *   indptr[b + 1] - indptr[b] positions (tg_fp8_kv_read: its first)
+ * What the int32 tensors hold is read on the device: positions below zero or beyond W * P, pages outside the pool and rows outside
+ * the packed tensors are left out.  Packed tensors are (tokens, heads, D), inputs with any row and head strides that are
+ * multiples of 8 elements and a contiguous last dimension, 16-byte aligned.  Outputs: rows of no sequence are left as they were.
+ *
+ * tg_fp8_kv_append: writes k and v (bf16 / f16) of the new tokens.  With rope (rows, R) f32, rows >= W * P, R a multiple of 16 up to
+ *   D, a row being cos of R / 2 angles, then sin: k's first R elements are turned by the row of the token's position, in pairs
+ *   (i, i + R / 2), or (2 i, 2 i + 1) if interleaved; and so are q's (tokens, any heads, D), into q_out (contiguous, not q), if given.
+ *   A page's scale is 2^e, e the smallest in [-40, 40] with amax <= 448 * 2^e; larger magnitudes (and infinities) saturate, NaN becomes
+ *   -448.  A write from a page's first slot on sets the scale anew; one behind earlier tokens keeps the larger of the page's and its own
+ *   and moves the earlier tokens' codes to it.  A page belongs to one sequence while it is written.
+ * tg_fp8_kv_read: the first indptr[b + 1] - indptr[b] tokens of each sequence as k, v (tokens, heads, D) bf16 / f16 / f32, contiguous.
+ * tg_fp8_kv_attention: out = softmax(sm_scale q k^T) v, causal: a token sees the positions up to its own, with window > 0 only the
+ *   last `window` of them and the positions below sink_tokens.  Pages no token sees need not exist.  q (tokens, H, D) bf16 / f16, H a
+ *   multiple of heads: query head h reads cache head h / (H / heads).  out: like q, contiguous, not q.  A token that sees nothing
+ *   gets zeros.  workspace: tg_fp8_kv_attention_workspace_bytes() bytes (0: NULL will do), 16-byte aligned, contents irrelevant; calls
+ *   that share one must not overlap in time.  The codes of live slots must be numbers (tg_fp8_kv_append writes no NaN).
+ */
+int32_t tg_fp8_kv_append(const tg_tensor* k_cache, const tg_tensor* v_cache, const tg_tensor* k_scale, const tg_tensor* v_scale, const tg_tensor* k,
+                         const tg_tensor* v, const tg_tensor* block_table, const tg_tensor* seq_lens, const tg_tensor* indptr, const tg_tensor* q_out,
+                         const tg_tensor* q, const tg_tensor* rope, int32_t interleaved, int32_t device_id, uint64_t hip_stream);
+int32_t tg_fp8_kv_read(const tg_tensor* k, const tg_tensor* v, const tg_tensor* k_cache, const tg_tensor* v_cache, const tg_tensor* k_scale,
+                       const tg_tensor* v_scale, const tg_tensor* block_table, const tg_tensor* indptr, int32_t device_id, uint64_t hip_stream);
+int64_t tg_fp8_kv_attention_workspace_bytes(int64_t tokens, int64_t q_heads, int64_t batch, int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                                            int64_t max_pages, int32_t window, int32_t sink_tokens);
+int32_t tg_fp8_kv_attention(const tg_tensor* out, const tg_tensor* q, const tg_tensor* k_cache, const tg_tensor* v_cache, const tg_tensor* k_scale,
+                            const tg_tensor* v_scale, const tg_tensor* block_table, const tg_tensor* seq_lens, const tg_tensor* indptr, float sm_scale,
+                            int32_t window, int32_t sink_tokens, const tg_tensor* workspace, int32_t device_id, uint64_t hip_stream);
+
 /* The schedule the most recent GEMM call on this host thread chose: fills out[0..n) with the
  * TG_CFG_* slots (kernel, BLOCK_M, BLOCK_N, SPLIT_K, ROW_GROUPS, WAVES).  Returns slots written. */
 int32_t tg_last_config(int32_t* out, int32_t n);

@@ -128,6 +128,16 @@ def load():
     L.tg_fp8_weight_dequant.argtypes = [P, P, P, ctypes.c_int32, ctypes.c_int32, ctypes.c_uint64]
     L.tg_silu_mul_quant_1x128.restype = ctypes.c_int32
     L.tg_silu_mul_quant_1x128.argtypes = [P, P, P, ctypes.c_int32, ctypes.c_uint64]
+    L.tg_fp8_rms_norm_quant.restype = ctypes.c_int32
+    L.tg_fp8_rms_norm_quant.argtypes = [P] * 8 + [ctypes.c_float, ctypes.c_int32, ctypes.c_int32, ctypes.c_uint64]
+    L.tg_fp8_kv_append.restype = ctypes.c_int32
+    L.tg_fp8_kv_append.argtypes = [P] * 12 + [ctypes.c_int32, ctypes.c_int32, ctypes.c_uint64]
+    L.tg_fp8_kv_read.restype = ctypes.c_int32
+    L.tg_fp8_kv_read.argtypes = [P] * 8 + [ctypes.c_int32, ctypes.c_uint64]
+    L.tg_fp8_kv_attention_workspace_bytes.restype = ctypes.c_int64
+    L.tg_fp8_kv_attention_workspace_bytes.argtypes = [ctypes.c_int64] * 7 + [ctypes.c_int32, ctypes.c_int32]
+    L.tg_fp8_kv_attention.restype = ctypes.c_int32
+    L.tg_fp8_kv_attention.argtypes = [P] * 9 + [ctypes.c_float, ctypes.c_int32, ctypes.c_int32, P, ctypes.c_int32, ctypes.c_uint64]
     L.tg_moe_sum.restype = ctypes.c_int32
     L.tg_moe_sum.argtypes = [P, P, ctypes.c_int32, ctypes.c_uint64]
     L.tg_moe_sum_routed.restype = ctypes.c_int32
@@ -569,6 +579,42 @@ def silu_mul_quant_1x128(x: torch.Tensor):
                                    _device_index(x), _stream_handle(x))
     check_rc(rc, "tg_silu_mul_quant_1x128")
     return q, scales
+
+
+def fp8_rms_norm_quant(q, scales, norm_out, residual_out, x, weight, residual, scale, eps: float, group_size: int) -> None:
+    L = _lib if _lib is not None else load()
+    rc = L.tg_fp8_rms_norm_quant(_desc(q), _desc(scales), _desc(norm_out), _desc(residual_out), _desc(x), _desc(weight), _desc(residual),
+                                 _desc(scale), float(eps), int(group_size), _device_index(x), _stream_handle(x))
+    check_rc(rc, "tg_fp8_rms_norm_quant")
+
+
+def fp8_kv_append(cache, k, v, block_table, seq_lens, indptr, q_out, q, rope, interleaved: bool) -> None:
+    """``cache``: (k_cache, v_cache, k_scale, v_scale)."""
+    L = _lib if _lib is not None else load()
+    rc = L.tg_fp8_kv_append(*[_desc(t) for t in cache], _desc(k), _desc(v), _desc(block_table), _desc(seq_lens), _desc(indptr), _desc(q_out),
+                            _desc(q), _desc(rope), int(bool(interleaved)), _device_index(k), _stream_handle(k))
+    check_rc(rc, "tg_fp8_kv_append")
+
+
+def fp8_kv_read(k, v, cache, block_table, indptr) -> None:
+    L = _lib if _lib is not None else load()
+    rc = L.tg_fp8_kv_read(_desc(k), _desc(v), *[_desc(t) for t in cache], _desc(block_table), _desc(indptr), _device_index(k), _stream_handle(k))
+    check_rc(rc, "tg_fp8_kv_read")
+
+
+def fp8_kv_attention(out, q, cache, block_table, seq_lens, indptr, sm_scale: float, window: int, sink_tokens: int) -> None:
+    """The scratch memory is the call's own (torch's allocator orders its reuse by stream, and gives each graph its own), not the
+    stream's: graphs captured on one stream may be replayed on several."""
+    L = _lib if _lib is not None else load()
+    dev, ws = _device_index(q), None
+    if q.dim() == 3 and cache[0].dim() == 4 and block_table.dim() == 2:
+        need = L.tg_fp8_kv_attention_workspace_bytes(q.shape[0], q.shape[1], block_table.shape[0], cache[0].shape[1], cache[0].shape[3],
+                                                     cache[0].shape[2], block_table.shape[1], int(window), int(sink_tokens))
+        if need > 0:
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    rc = L.tg_fp8_kv_attention(_desc(out), _desc(q), *[_desc(t) for t in cache], _desc(block_table), _desc(seq_lens), _desc(indptr),
+                               float(sm_scale), int(window), int(sink_tokens), _desc(ws), dev, _stream_handle(q))
+    check_rc(rc, "tg_fp8_kv_attention")
 
 
 def moe_sum(x: torch.Tensor, out: torch.Tensor) -> None:

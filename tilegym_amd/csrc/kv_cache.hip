@@ -1,0 +1,256 @@
+// Writing and reading the paged e4m3 cache (kv_device.h).
+//
+// Writing: rotary positions on the new tokens' q and k, then k and v in e4m3 with one scale per page and head.
+//   rotary: pairs (a, b) of the first R elements of a head, (x[i], x[i + R/2]) or (x[2i], x[2i + 1]), turn by the table's angle of
+//           the token's position: (a cos - b sin, a sin + b cos).  In fp32; k goes to e4m3 without a 16-bit rounding between.
+//   scale:  2^e with the smallest e in [-40, 40] that brings the page's largest magnitude within 448.  e4m3 is a floating-point type: a
+//           power of two costs its codes no precision, and moving stored codes from one power of two to a larger one only shifts their
+//           exponents, exact but for e4m3's subnormals.  So a page that fills token by token keeps max(old, new) as its scale,
+//           and its earlier codes move when the scale does: no token is rounded at more than one precision.
+// One workgroup writes the new tokens of one page, head and half of the cache: it alone reads and writes that scale, so no
+// atomics, and the result does not depend on the order of workgroups.  Bound by HBM at many tokens, by the launch and one chain
+// of dependent loads (sequence, page, scale) at few.
+#include "kv_device.h"
+#include "quant_device.h"
+
+namespace tg {
+namespace {
+
+constexpr int kMinExponent = -40, kMaxExponent = 40;
+
+// 2^e, the smallest with amax <= 448 * 2^e (448 = 1.75 * 2^8), from amax's bits
+__device__ __forceinline__ float page_scale(float amax) {
+    const uint32_t bits = __float_as_uint(amax);
+    const int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+    return __uint_as_float((uint32_t)(min(max(e, kMinExponent), kMaxExponent) + 127) << 23);
+}
+
+__device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d) {
+    int w = 0;  // (NaN: -448, as in the activation quantizer; a NaN code in v would reach rows that do not see its token)
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(__builtin_amdgcn_fmed3f(a, -448.f, 448.f), __builtin_amdgcn_fmed3f(b, -448.f, 448.f), w, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(__builtin_amdgcn_fmed3f(c, -448.f, 448.f), __builtin_amdgcn_fmed3f(d, -448.f, 448.f), w, true);
+    return (uint32_t)w;
+}
+
+// Elements 8 c .. 8 c + 7 of a head (x: its first element), turned by table row `row` (cos, then sin; rotary % 16 == 0).
+template <typename T>
+__device__ __forceinline__ v8f_q load_turned(const T* x, int c, const float* row, int rotary, int interleaved) {
+    v8f_q v = load8<T>(x + 8 * c);
+    if (8 * c >= rotary) return v;  // (rotary 0: no rotation)
+    const int half = rotary / 2;
+    if (interleaved) {
+        const v4f cs = *reinterpret_cast<const v4f*>(row + 4 * c), sn = *reinterpret_cast<const v4f*>(row + half + 4 * c);
+        v8f_q y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            y[2 * i] = v[2 * i] * cs[i] - v[2 * i + 1] * sn[i];
+            y[2 * i + 1] = v[2 * i] * sn[i] + v[2 * i + 1] * cs[i];
+        }
+        return y;
+    }
+    const bool upper = 8 * c >= half;
+    const int i0 = upper ? 8 * c - half : 8 * c;
+    const v8f_q o = load8<T>(x + (upper ? 8 * c - half : 8 * c + half));  // the other member of each pair
+    const v8f_q cs = load8<float>(row + i0), sn = load8<float>(row + half + i0);
+    v8f_q y;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = upper ? v[i] * cs[i] + o[i] * sn[i] : v[i] * cs[i] - o[i] * sn[i];
+    return y;
+}
+
+// Workgroups of the two kinds of work: first those that write the cache, (item, head, half) with the half fastest, then those that turn q.
+template <typename T>
+__global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendParams p, int items, int v_pad) {
+    const KvCache& c = p.c;
+    const int tid = (int)threadIdx.x, P = 1 << c.page_log2, D = c.dim, chunks = D / 8;
+    const int cache_blocks = items * c.heads * 2;
+    if ((int)blockIdx.x >= cache_blocks) {
+        // q: eight elements per lane
+        const int64_t at = (int64_t)((int)blockIdx.x - cache_blocks) * 256 + tid;
+        const int per_row = p.q_heads * chunks;
+        const int64_t row64 = at / per_row;
+        if (row64 >= c.rows) return;
+        const int row = (int)row64, rest = (int)(at - row64 * per_row), head = rest / chunks, ch = rest - head * chunks;
+        int lo = 0, hi = c.batch;  // the last sequence that begins at or before `row`
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (clamp_row(c.indptr[mid], c.rows) <= row) lo = mid;
+            else hi = mid;
+        }
+        const int first = clamp_row(c.indptr[lo], c.rows), end = clamp_row(c.indptr[lo + 1], c.rows);
+        if (row < first || row >= end) return;  // a row of no sequence: left as it was
+        const int64_t position = (int64_t)max(c.lens[lo], 0) - (end - row);
+        const float* angles = p.rope + (int64_t)min(max(position, (int64_t)0), (int64_t)p.rope_rows - 1) * p.rotary;
+        const v8f_q y = load_turned<T>((const T*)p.q + row * p.q_row + head * p.q_head, ch, angles, p.rotary, p.interleaved);
+        typedef T vecT __attribute__((ext_vector_type(8)));
+        *reinterpret_cast<vecT*>((T*)p.q_out + (row64 * p.q_heads + head) * D + 8 * ch) = __builtin_convertvector(y, vecT);
+        return;
+    }
+    extern __shared__ uint8_t lds[];  // v: the page's new codes, an element's tokens together, rows of v_pad bytes
+    __shared__ float part[4];
+    const int half = (int)blockIdx.x & 1, unit = (int)blockIdx.x >> 1, head = unit % c.heads;
+    const SeqItem f = find_sequence(c.indptr, c.batch, c.rows, unit / c.heads, 1, P, 2);
+    if (f.seq < 0) return;
+    const int64_t len = max(c.lens[f.seq], 0), start = len - f.n;  // position of the sequence's first new token
+    const int64_t first = start > 0 ? start : 0, page_index = (first >> c.page_log2) + f.item;
+    if (page_index >= c.width) return;
+    const int64_t page_begin = page_index << c.page_log2;
+    const int slot0 = (int)(first > page_begin ? first - page_begin : 0);
+    const int slot1 = (int)min(len - page_begin, (int64_t)P);
+    if (slot0 >= slot1) return;
+    const int page = c.table[(int64_t)f.seq * c.width + page_index];
+    if (page < 0 || page >= c.pages) return;
+    const int64_t block = (int64_t)page * c.heads + head;
+    float* scale_at = (half ? c.v_scale : c.k_scale) + block;
+    uint8_t* codes = (half ? c.v : c.k) + block * ((int64_t)P * D);
+    float old = 0.f;
+    if (slot0 > 0) old = *scale_at;
+    if (!(old > 0.f && old <= 0x1p100f)) old = 0.f;  // no scale that a write leaves: the earlier slots hold nothing
+    // rows of the packed input, and table rows, of the page's first slot on
+    const int64_t row0 = f.first + (page_begin - start);
+    const T* x = half ? (const T*)p.v + head * p.v_head : (const T*)p.k + head * p.k_head;
+    const int64_t x_row = half ? p.v_row : p.k_row;
+    const int rotary = half || !p.rope ? 0 : p.rotary;
+    const int count = (slot1 - slot0) * chunks;
+    auto element = [&](int i) {
+        const int slot = slot0 + i / chunks, ch = i % chunks;
+        const int64_t position = min(page_begin + slot, (int64_t)p.rope_rows - 1);
+        return load_turned<T>(x + (row0 + slot) * x_row, ch, rotary ? p.rope + position * p.rotary : nullptr, rotary, p.interleaved);
+    };
+    float amax = 0.f;
+    for (int i = tid; i < count; i += 256) {
+        const v8f_q v = element(i);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(v[k]));
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) amax = fmaxf(amax, __shfl_xor(amax, d));
+    if (tid % 64 == 0) part[tid / 64] = amax;
+    __syncthreads();  // (and every lane has read the old scale)
+    amax = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+    const float scale = fmaxf(page_scale(amax), old), inverse = 1.0f / scale;
+    if (tid == 0) *scale_at = scale;
+    if (slot0 > 0 && scale != old) {  // the earlier tokens' codes move to the new scale
+        const float move = old * inverse;
+        const int n = slot0 * D;
+        for (int i = tid; i < n; i += 256) {
+            uint8_t* at = half ? codes + (i / slot0) * P + i % slot0 : codes + i;
+            *at = old == 0.f ? 0 : (uint8_t)to_e4m3x4(e4m3_to_f32(*at) * move, 0.f, 0.f, 0.f);
+        }
+    }
+    for (int i = tid; i < count; i += 256) {
+        const v8f_q v = element(i) * inverse;
+        const uint32_t w0 = to_e4m3x4(v[0], v[1], v[2], v[3]), w1 = to_e4m3x4(v[4], v[5], v[6], v[7]);
+        const int slot = slot0 + i / chunks, ch = i % chunks;
+        if (!half) {
+            *reinterpret_cast<v2i*>(codes + slot * D + 8 * ch) = v2i{(int)w0, (int)w1};
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) lds[(8 * ch + k) * v_pad + slot] = (uint8_t)((k < 4 ? w0 : w1) >> (8 * (k & 3)));
+        }
+    }
+    if (half) {
+        __syncthreads();
+        const int words = P / 4;
+        for (int i = tid; i < D * words; i += 256) {
+            const int d = i / words, s = 4 * (i % words);
+            if (s + 4 <= slot0 || s >= slot1) continue;
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(lds + d * v_pad + s);
+            if (s >= slot0 && s + 4 <= slot1) {
+                *reinterpret_cast<uint32_t*>(codes + d * P + s) = w;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (s + k >= slot0 && s + k < slot1) codes[d * P + s + k] = (uint8_t)(w >> (8 * k));
+            }
+        }
+    }
+}
+
+// Reading: element = code * scale (one fp32 product, rounded once).  A workgroup per page, head and half; v is turned through LDS.
+template <typename T>
+__global__ void __launch_bounds__(256) kv_read_kernel(const KvReadParams p, int items, int v_pad) {
+    typedef T vecT __attribute__((ext_vector_type(8)));
+    extern __shared__ uint8_t lds[];
+    const KvCache& c = p.c;
+    const int tid = (int)threadIdx.x, P = 1 << c.page_log2, D = c.dim, chunks = D / 8;
+    const int half = (int)blockIdx.x & 1, unit = (int)blockIdx.x >> 1, head = unit % c.heads;
+    const SeqItem f = find_sequence(c.indptr, c.batch, c.rows, unit / c.heads, 1, P, 1);
+    if (f.seq < 0 || f.item >= c.width) return;
+    const int begin = f.item << c.page_log2, n = min(f.n - begin, P);
+    if (n <= 0) return;
+    const int page = c.table[(int64_t)f.seq * c.width + f.item];
+    if (page < 0 || page >= c.pages) return;
+    const int64_t block = (int64_t)page * c.heads + head;
+    const float scale = (half ? c.v_scale : c.k_scale)[block];
+    const uint8_t* codes = (half ? c.v : c.k) + block * ((int64_t)P * D);
+    T* out = (T*)(half ? p.v : p.k) + (((int64_t)f.first + begin) * c.heads + head) * D;
+    if (half) {
+        const int words = P / 4;
+        for (int i = tid; i < D * words; i += 256) {
+            const int d = i / words, s = 4 * (i % words);
+            *reinterpret_cast<uint32_t*>(lds + d * v_pad + s) = *reinterpret_cast<const uint32_t*>(codes + d * P + s);
+        }
+        __syncthreads();
+    }
+    for (int i = tid; i < n * chunks; i += 256) {
+        const int slot = i / chunks, ch = i % chunks;
+        v2i raw;
+        if (!half) {
+            raw = *reinterpret_cast<const v2i*>(codes + slot * D + 8 * ch);
+        } else {
+            uint32_t w[2] = {0, 0};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k / 4] |= (uint32_t)lds[(8 * ch + k) * v_pad + slot] << (8 * (k & 3));
+            raw = v2i{(int)w[0], (int)w[1]};
+        }
+        typedef float v2f __attribute__((ext_vector_type(2)));
+        v8f_q y;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const v2f lo = __builtin_amdgcn_cvt_pk_f32_fp8(raw[h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(raw[h], true);
+            y[4 * h] = lo[0] * scale, y[4 * h + 1] = lo[1] * scale, y[4 * h + 2] = hi[0] * scale, y[4 * h + 3] = hi[1] * scale;
+        }
+        T* at = out + (int64_t)slot * c.heads * D + 8 * ch;
+        if constexpr (sizeof(T) == 4) {
+            reinterpret_cast<v4f*>(at)[0] = __builtin_shufflevector(y, y, 0, 1, 2, 3);
+            reinterpret_cast<v4f*>(at)[1] = __builtin_shufflevector(y, y, 4, 5, 6, 7);
+        } else {
+            *reinterpret_cast<vecT*>(at) = __builtin_convertvector(y, vecT);
+        }
+    }
+}
+
+}  // namespace
+
+// Items that can begin: sum over sequences of ceil(n / P) (+ 1 where a run may begin inside a page), see find_sequence.
+hipError_t run_kv_append(const KvAppendParams& p, bool is_bf16, hipStream_t s) {
+    const KvCache& c = p.c;
+    if (c.rows <= 0 || c.batch <= 0) return hipSuccess;
+    const int64_t P = (int64_t)1 << c.page_log2, items = c.rows / P + 2 * (int64_t)c.batch;
+    const int64_t q_blocks = p.q ? ((int64_t)c.rows * p.q_heads * (c.dim / 8) + 255) / 256 : 0, blocks = items * c.heads * 2 + q_blocks;
+    if (blocks > INT32_MAX) return hipErrorInvalidValue;
+    const int v_pad = (int)P + 4;
+    const dim3 grid((unsigned)blocks), block(256);
+    const size_t lds = (size_t)c.dim * v_pad;
+    if (is_bf16) hipLaunchKernelGGL(kv_append_kernel<__bf16>, grid, block, lds, s, p, (int)items, v_pad);
+    else hipLaunchKernelGGL(kv_append_kernel<_Float16>, grid, block, lds, s, p, (int)items, v_pad);
+    return hipGetLastError();
+}
+
+hipError_t run_kv_read(const KvReadParams& p, int out_type, hipStream_t s) {
+    const KvCache& c = p.c;
+    if (c.rows <= 0 || c.batch <= 0) return hipSuccess;
+    const int64_t P = (int64_t)1 << c.page_log2, items = c.rows / P + c.batch, blocks = items * c.heads * 2;
+    if (blocks > INT32_MAX) return hipErrorInvalidValue;
+    const int v_pad = (int)P + 4;
+    const dim3 grid((unsigned)blocks), block(256);
+    const size_t lds = (size_t)c.dim * v_pad;
+    if (out_type == OUT_BF16) hipLaunchKernelGGL(kv_read_kernel<__bf16>, grid, block, lds, s, p, (int)items, v_pad);
+    else if (out_type == OUT_F16) hipLaunchKernelGGL(kv_read_kernel<_Float16>, grid, block, lds, s, p, (int)items, v_pad);
+    else if (out_type == OUT_F32) hipLaunchKernelGGL(kv_read_kernel<float>, grid, block, lds, s, p, (int)items, v_pad);
+    else return hipErrorInvalidValue;
+    return hipGetLastError();
+}
+
+}  // namespace tg

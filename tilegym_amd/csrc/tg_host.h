@@ -119,6 +119,71 @@ hipError_t run_silu_mul_quant(const void* x, int x_type, uint8_t* q, float* scal
 // out (tokens, H) <- sum over the top_k axis of x (tokens, top_k, H); bf16/f16, H % 8 == 0
 // ids: null, or (tokens, top_k) expert ids; slots whose id is outside [0, E) then count as zeros
 hipError_t run_moe_sum(const void* x, void* out, int x_type, int64_t tokens, int top_k, int H, const void* ids, bool ids_are_i64, int E, hipStream_t s);
+// Root-mean-square norm with the residual's addition and an e4m3 output (rms_norm_quant.hip)
+struct NormQuantParams {
+    const void* x;           // (rows, hidden)
+    const void* weight;      // (hidden)
+    const void* residual;    // (rows, hidden) or null
+    void* residual_out;      // (rows, hidden) or null: x + residual; may be x or residual
+    void* norm_out;          // (rows, hidden) or null: the norm before quantization; may be x
+    uint8_t* q;              // (rows, hidden)
+    float* scales;           // (rows, hidden / group), or null with
+    const float* scale;      // the given scale of the whole tensor
+    int64_t rows;
+    int hidden;              // a multiple of 16 and of the group, at most kNormMaxHidden
+    int lanes_per_group, group_shift;  // group / 8: 2, 4, 8 or 16, and its logarithm
+    float eps;
+};
+constexpr int kNormMaxHidden = 32768;
+hipError_t run_rms_norm_quant(const NormQuantParams& p, int x_type, bool weight_f32, hipStream_t s);
+
+// The paged e4m3 cache (kv_device.h) and the calls over it
+struct KvCache {
+    uint8_t* k;          // (pages, heads, P, dim)
+    uint8_t* v;          // (pages, heads, dim, P)
+    float* k_scale;      // (pages, heads)
+    float* v_scale;
+    const int* table;    // (batch, width)
+    const int* lens;     // (batch); null for reading
+    const int* indptr;   // (batch + 1)
+    int pages, heads, dim, page_log2, batch, width;
+    int rows;            // of the packed tensors
+};
+struct KvAppendParams {
+    KvCache c;
+    const void *k, *v;                 // (rows, heads, dim), element strides below, the last dimension contiguous
+    int64_t k_row, k_head, v_row, v_head;
+    const void* q;                     // (rows, q_heads, dim) or null
+    void* q_out;                       // contiguous
+    int64_t q_row, q_head;
+    int q_heads;
+    const float* rope;                 // (rope_rows, rotary): cos, then sin; null: no rotation
+    int rope_rows, rotary, interleaved;
+};
+hipError_t run_kv_append(const KvAppendParams& p, bool is_bf16, hipStream_t s);
+struct KvReadParams {
+    KvCache c;
+    void *k, *v;                       // (rows, heads, dim), contiguous
+};
+hipError_t run_kv_read(const KvReadParams& p, int out_type, hipStream_t s);
+struct KvAttentionParams {
+    KvCache c;
+    const void* q;                     // (rows, q_heads, dim), element strides below
+    void* out;                         // (rows, q_heads, dim), contiguous
+    int64_t q_row, q_head;
+    int q_heads, group;                // group = q_heads / heads
+    float scale_log2;                  // softmax scale * log2(e)
+    int window, sinks;                 // window 0: all earlier positions
+    int splits;                        // > 1: partial results below, joined by a second launch
+    float* part_o;                     // (splits, rows * q_heads, dim)
+    float* part_ml;                    // (splits, rows * q_heads, 2): running maximum and sum
+};
+// splits the launch should use for these sizes (p.c.rows, batch, heads, width, page_log2, dim, group, window, sinks)
+int kv_attention_splits(const KvAttentionParams& p);
+inline int64_t kv_attention_part_bytes(int64_t splits, int64_t rows, int64_t q_heads, int64_t dim) {
+    return splits > 1 ? splits * rows * q_heads * (dim + 2) * 4 : 0;
+}
+hipError_t run_kv_attention(const KvAttentionParams& p, bool is_bf16, hipStream_t s);
 // dst (cols, rows) <- transpose of src (rows, cols), one byte per element
 // dst (cols x ld) = transpose of src (rows x cols), zero beyond `rows` in every dst row
 hipError_t run_transpose_u8(const uint8_t* src, uint8_t* dst, int rows, int cols, int ld, hipStream_t s);

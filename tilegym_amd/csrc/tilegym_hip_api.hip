@@ -1966,6 +1966,252 @@ int32_t tg_fp8_weight_dequant(const tg_tensor* y, const tg_tensor* x, const tg_t
     return TG_OK;
 }
 
+int32_t tg_fp8_rms_norm_quant(const tg_tensor* q, const tg_tensor* scales, const tg_tensor* norm_out, const tg_tensor* residual_out,
+                              const tg_tensor* x, const tg_tensor* weight, const tg_tensor* residual, const tg_tensor* scale, float eps,
+                              int32_t group_size, int32_t device_id, uint64_t hip_stream) {
+    g_err[0] = 0;
+    int32_t rc;
+    if ((rc = check_tensor(x, "x", -1)) || (rc = check_tensor(weight, "weight", 1)) || (rc = check_tensor(q, "q", -1))) return rc;
+    const int x_type = io_type_of(x->dtype);
+    if (x_type < 0) return fail(TG_ERR_DTYPE, "x must be bf16, f16 or f32");
+    if (weight->dtype != x->dtype && weight->dtype != TG_F32) return fail(TG_ERR_DTYPE, "weight must have x's dtype or f32");
+    if (q->dtype != TG_F8E4M3FN) return fail(TG_ERR_DTYPE, "q must be float8_e4m3fn (dtype code 7)");
+    if (x->ndim < 1) return fail(TG_ERR_INVALID, "x needs at least one dimension");
+    const int64_t n = numel(x), H = x->shape[x->ndim - 1];
+    if (H < 16 || H % 16 != 0 || H > tg::kNormMaxHidden)
+        return fail(TG_ERR_INVALID, "the last dimension (%lld) must be a multiple of 16 and at most %d", (long long)H, tg::kNormMaxHidden);
+    if (weight->shape[0] != H) return fail(TG_ERR_INVALID, "weight must have %lld elements", (long long)H);
+    if (numel(q) != n) return fail(TG_ERR_INVALID, "q must have the shape of x");
+    const tg_tensor* like[3] = {residual, residual_out, norm_out};
+    const char* names[3] = {"residual", "residual_out", "norm_out"};
+    for (int i = 0; i < 3; ++i) {
+        if (!like[i]) continue;
+        if ((rc = check_tensor(like[i], names[i], -1))) return rc;
+        if (like[i]->dtype != x->dtype) return fail(TG_ERR_DTYPE, "%s must have x's dtype", names[i]);
+        if (numel(like[i]) != n) return fail(TG_ERR_INVALID, "%s must have the shape of x", names[i]);
+        if (!aligned16(like[i]->ptr)) return fail(TG_ERR_INVALID, "%s must be 16-byte aligned", names[i]);
+    }
+    if (residual_out && !residual) return fail(TG_ERR_INVALID, "residual_out without residual");
+    if (!(eps >= 0.f)) return fail(TG_ERR_INVALID, "eps must not be negative");
+    if (scale) {
+        if (scales) return fail(TG_ERR_INVALID, "scales and a given scale exclude each other");
+        if ((rc = check_tensor(scale, "scale", -1))) return rc;
+        if (scale->dtype != TG_F32) return fail(TG_ERR_DTYPE, "scale must be f32");
+        if (numel(scale) != 1) return fail(TG_ERR_INVALID, "scale must have one element");
+    } else {
+        if ((rc = check_tensor(scales, "scales", -1))) return rc;
+        if (scales->dtype != TG_F32) return fail(TG_ERR_DTYPE, "scales must be f32");
+        if (group_size != 16 && group_size != 32 && group_size != 64 && group_size != 128)
+            return fail(TG_ERR_INVALID, "group_size must be 16, 32, 64 or 128, got %d", group_size);
+        if (H % group_size != 0) return fail(TG_ERR_INVALID, "the last dimension (%lld) must be a multiple of %d", (long long)H, group_size);
+        if (numel(scales) != n / group_size) return fail(TG_ERR_INVALID, "scales must have %lld elements", (long long)(n / group_size));
+    }
+    if (n == 0) return TG_OK;
+    if (!aligned16(x->ptr) || !aligned16(weight->ptr) || (q->ptr & 7) != 0) return fail(TG_ERR_INVALID, "x and weight must be 16-byte and q 8-byte aligned");
+    if (n / H > INT32_MAX) return fail(TG_ERR_INVALID, "too many rows");
+    DeviceGuard guard(device_id);
+    if (!guard.ok) return fail(TG_ERR_DEVICE, "cannot use HIP device %d", device_id);
+    auto at = [](const tg_tensor* t) { return t ? reinterpret_cast<void*>(t->ptr) : nullptr; };
+    tg::NormQuantParams p{};
+    p.x = at(x), p.weight = at(weight), p.residual = at(residual), p.residual_out = at(residual_out), p.norm_out = at(norm_out);
+    p.q = static_cast<uint8_t*>(at(q)), p.scales = static_cast<float*>(at(scales)), p.scale = static_cast<const float*>(at(scale));
+    p.rows = n / H, p.hidden = (int)H, p.eps = eps;
+    p.lanes_per_group = scale ? 16 : group_size / 8;
+    for (p.group_shift = 0; (1 << p.group_shift) < p.lanes_per_group;) ++p.group_shift;
+    const hipError_t e = tg::run_rms_norm_quant(p, x_type, weight->dtype == TG_F32, reinterpret_cast<hipStream_t>(hip_stream));
+    if (e != hipSuccess) return fail(TG_ERR_LAUNCH, "rms_norm_quant launch failed: %s", hipGetErrorString(e));
+    return TG_OK;
+}
+
+// A packed (rows, heads, dim) tensor whose last dimension is contiguous and whose rows and heads lie on 16-byte boundaries.
+static int32_t check_packed(const tg_tensor* t, const char* name) {
+    if (!t) return fail(TG_ERR_NULL, "%s: null tensor descriptor", name);
+    if (t->ndim != 3) return fail(TG_ERR_INVALID, "%s: expected 3 dims (tokens, heads, elements), got %d", name, t->ndim);
+    for (int i = 0; i < 3; ++i)
+        if (t->shape[i] < 0) return fail(TG_ERR_INVALID, "%s: negative extent", name);
+    if (t->dtype != TG_BF16 && t->dtype != TG_F16) return fail(TG_ERR_DTYPE, "%s must be bf16 or f16", name);
+    if (numel(t) == 0) return TG_OK;
+    if (t->ptr == 0) return fail(TG_ERR_NULL, "%s: null data pointer", name);
+    if (t->shape[2] > 1 && t->strides[2] != 1) return fail(TG_ERR_INVALID, "%s: the last dimension must be contiguous", name);
+    for (int i = 0; i < 2; ++i)
+        if (t->shape[i] > 1 && (t->strides[i] < 0 || t->strides[i] % 8 != 0)) return fail(TG_ERR_INVALID, "%s: strides must be multiples of 8 elements", name);
+    if (!aligned16(t->ptr)) return fail(TG_ERR_INVALID, "%s must be 16-byte aligned", name);
+    return TG_OK;
+}
+
+// The cache's tensors, the page table and the sequences' tensors; lens may be null (reading).  On success c is filled, c.rows aside.
+static int32_t check_kv_cache(const tg_tensor* k_cache, const tg_tensor* v_cache, const tg_tensor* k_scale, const tg_tensor* v_scale,
+                              const tg_tensor* block_table, const tg_tensor* seq_lens, bool with_lens, const tg_tensor* indptr, int64_t rows, tg::KvCache& c) {
+    int32_t rc;
+    if ((rc = check_tensor(k_cache, "k_cache", 4)) || (rc = check_tensor(v_cache, "v_cache", 4)) || (rc = check_tensor(k_scale, "k_scale", 2)) ||
+        (rc = check_tensor(v_scale, "v_scale", 2)) || (rc = check_tensor(block_table, "block_table", 2)) || (rc = check_tensor(indptr, "indptr", 1)) ||
+        (with_lens && (rc = check_tensor(seq_lens, "seq_lens", 1))))
+        return rc;
+    if (k_cache->dtype != TG_F8E4M3FN || v_cache->dtype != TG_F8E4M3FN) return fail(TG_ERR_DTYPE, "k_cache and v_cache must be float8_e4m3fn (dtype code 7)");
+    if (k_scale->dtype != TG_F32 || v_scale->dtype != TG_F32) return fail(TG_ERR_DTYPE, "k_scale and v_scale must be f32");
+    if (block_table->dtype != TG_I32 || indptr->dtype != TG_I32 || (with_lens && seq_lens->dtype != TG_I32))
+        return fail(TG_ERR_DTYPE, "block_table, indptr and seq_lens must be int32");
+    const int64_t pages = k_cache->shape[0], heads = k_cache->shape[1], P = k_cache->shape[2], D = k_cache->shape[3], B = block_table->shape[0],
+                  W = block_table->shape[1];
+    if (P != 16 && P != 32 && P != 64 && P != 128) return fail(TG_ERR_INVALID, "pages must hold 16, 32, 64 or 128 tokens, got %lld", (long long)P);
+    if (D != 64 && D != 128 && D != 256) return fail(TG_ERR_INVALID, "heads must have 64, 128 or 256 elements, got %lld", (long long)D);
+    if (v_cache->shape[0] != pages || v_cache->shape[1] != heads || v_cache->shape[2] != D || v_cache->shape[3] != P)
+        return fail(TG_ERR_INVALID, "v_cache must be (%lld, %lld, %lld, %lld)", (long long)pages, (long long)heads, (long long)D, (long long)P);
+    const tg_tensor* scales[2] = {k_scale, v_scale};
+    for (const tg_tensor* t : scales)
+        if (t->shape[0] != pages || t->shape[1] != heads) return fail(TG_ERR_INVALID, "k_scale and v_scale must be (%lld, %lld)", (long long)pages, (long long)heads);
+    if (indptr->shape[0] != B + 1) return fail(TG_ERR_INVALID, "indptr must have %lld elements", (long long)(B + 1));
+    if (with_lens && seq_lens->shape[0] != B) return fail(TG_ERR_INVALID, "seq_lens must have %lld elements", (long long)B);
+    if (pages < 1 || pages > INT32_MAX || heads < 1 || heads > 65536) return fail(TG_ERR_INVALID, "the cache needs between 1 and 2^31 - 1 pages and 1 to 65536 heads");
+    if (B > (1 << 24) || W > (1 << 24) || (B > 0 && W < 1)) return fail(TG_ERR_INVALID, "block_table must have 1 to 2^24 columns and at most 2^24 rows");
+    if (rows > (1 << 28)) return fail(TG_ERR_INVALID, "too many tokens");
+    if (!aligned16(k_cache->ptr) || !aligned16(v_cache->ptr)) return fail(TG_ERR_INVALID, "k_cache and v_cache must be 16-byte aligned");
+    c = tg::KvCache{};
+    c.k = reinterpret_cast<uint8_t*>(k_cache->ptr), c.v = reinterpret_cast<uint8_t*>(v_cache->ptr);
+    c.k_scale = reinterpret_cast<float*>(k_scale->ptr), c.v_scale = reinterpret_cast<float*>(v_scale->ptr);
+    c.table = reinterpret_cast<const int*>(block_table->ptr), c.indptr = reinterpret_cast<const int*>(indptr->ptr);
+    c.lens = with_lens ? reinterpret_cast<const int*>(seq_lens->ptr) : nullptr;
+    c.pages = (int)pages, c.heads = (int)heads, c.dim = (int)D, c.batch = (int)B, c.width = (int)W, c.rows = (int)rows;
+    for (c.page_log2 = 4; (1 << c.page_log2) < P;) ++c.page_log2;
+    return TG_OK;
+}
+
+int32_t tg_fp8_kv_append(const tg_tensor* k_cache, const tg_tensor* v_cache, const tg_tensor* k_scale, const tg_tensor* v_scale, const tg_tensor* k,
+                         const tg_tensor* v, const tg_tensor* block_table, const tg_tensor* seq_lens, const tg_tensor* indptr, const tg_tensor* q_out,
+                         const tg_tensor* q, const tg_tensor* rope, int32_t interleaved, int32_t device_id, uint64_t hip_stream) {
+    g_err[0] = 0;
+    int32_t rc;
+    if ((rc = check_packed(k, "k")) || (rc = check_packed(v, "v"))) return rc;
+    tg::KvAppendParams p{};
+    const int64_t T = k->shape[0];
+    if ((rc = check_kv_cache(k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, true, indptr, T, p.c))) return rc;
+    const int64_t D = p.c.dim;
+    if (v->dtype != k->dtype) return fail(TG_ERR_DTYPE, "k and v must have one dtype");
+    const tg_tensor* kv[2] = {k, v};
+    for (const tg_tensor* t : kv)
+        if (t->shape[0] != T || t->shape[1] != p.c.heads || t->shape[2] != D) return fail(TG_ERR_INVALID, "k and v must be (tokens, %d, %lld)", p.c.heads, (long long)D);
+    if ((q != nullptr) != (q_out != nullptr)) return fail(TG_ERR_NULL, "q and q_out come together");
+    if (rope) {
+        if ((rc = check_tensor(rope, "rope", 2))) return rc;
+        if (rope->dtype != TG_F32) return fail(TG_ERR_DTYPE, "rope must be f32");
+        const int64_t R = rope->shape[1], capacity = (int64_t)p.c.width << p.c.page_log2;
+        if (R < 16 || R % 16 != 0 || R > D) return fail(TG_ERR_INVALID, "rope must turn a multiple of 16 elements, at most %lld", (long long)D);
+        if (rope->shape[0] > INT32_MAX || rope->shape[0] < 1 || (p.c.batch > 0 && rope->shape[0] < capacity))
+            return fail(TG_ERR_INVALID, "rope must cover the %lld positions of block_table", (long long)capacity);
+        if (!aligned16(rope->ptr)) return fail(TG_ERR_INVALID, "rope must be 16-byte aligned");
+        p.rope = reinterpret_cast<const float*>(rope->ptr), p.rope_rows = (int)rope->shape[0], p.rotary = (int)R, p.interleaved = interleaved != 0;
+    }
+    if (q) {
+        if (!rope) return fail(TG_ERR_NULL, "q needs rope");
+        if ((rc = check_packed(q, "q")) || (rc = check_tensor(q_out, "q_out", 3))) return rc;
+        if (q->dtype != k->dtype || q_out->dtype != k->dtype) return fail(TG_ERR_DTYPE, "q and q_out must have k's dtype");
+        for (int i = 0; i < 3; ++i)
+            if (q_out->shape[i] != q->shape[i]) return fail(TG_ERR_INVALID, "q_out must have the shape of q");
+        if (q->shape[0] != T || q->shape[2] != D) return fail(TG_ERR_INVALID, "q must be (%lld, heads, %lld)", (long long)T, (long long)D);
+        if (q->shape[1] > 65536) return fail(TG_ERR_INVALID, "q has too many heads");
+        if (!aligned16(q_out->ptr)) return fail(TG_ERR_INVALID, "q_out must be 16-byte aligned");
+        if (numel(q) > 0) {
+            if (q_out->ptr == q->ptr) return fail(TG_ERR_INVALID, "q_out must not be q");
+            p.q = reinterpret_cast<const void*>(q->ptr), p.q_out = reinterpret_cast<void*>(q_out->ptr);
+            p.q_row = q->strides[0], p.q_head = q->strides[1], p.q_heads = (int)q->shape[1];
+        }
+    }
+    if (T == 0 || p.c.batch == 0) return TG_OK;
+    p.k = reinterpret_cast<const void*>(k->ptr), p.v = reinterpret_cast<const void*>(v->ptr);
+    p.k_row = k->strides[0], p.k_head = k->strides[1], p.v_row = v->strides[0], p.v_head = v->strides[1];
+    DeviceGuard guard(device_id);
+    if (!guard.ok) return fail(TG_ERR_DEVICE, "cannot use HIP device %d", device_id);
+    const hipError_t e = tg::run_kv_append(p, k->dtype == TG_BF16, reinterpret_cast<hipStream_t>(hip_stream));
+    if (e != hipSuccess) return fail(TG_ERR_LAUNCH, "kv_append launch failed: %s", hipGetErrorString(e));
+    return TG_OK;
+}
+
+int32_t tg_fp8_kv_read(const tg_tensor* k, const tg_tensor* v, const tg_tensor* k_cache, const tg_tensor* v_cache, const tg_tensor* k_scale,
+                       const tg_tensor* v_scale, const tg_tensor* block_table, const tg_tensor* indptr, int32_t device_id, uint64_t hip_stream) {
+    g_err[0] = 0;
+    int32_t rc;
+    if ((rc = check_tensor(k, "k", 3)) || (rc = check_tensor(v, "v", 3))) return rc;
+    tg::KvReadParams p{};
+    if ((rc = check_kv_cache(k_cache, v_cache, k_scale, v_scale, block_table, nullptr, false, indptr, k->shape[0], p.c))) return rc;
+    const int out_type = io_type_of(k->dtype);
+    if (out_type < 0 || v->dtype != k->dtype) return fail(TG_ERR_DTYPE, "k and v must both be bf16, f16 or f32");
+    const tg_tensor* kv[2] = {k, v};
+    for (const tg_tensor* t : kv) {
+        if (t->shape[0] != k->shape[0] || t->shape[1] != p.c.heads || t->shape[2] != p.c.dim)
+            return fail(TG_ERR_INVALID, "k and v must be (tokens, %d, %d)", p.c.heads, p.c.dim);
+        if (!aligned16(t->ptr)) return fail(TG_ERR_INVALID, "k and v must be 16-byte aligned");
+    }
+    if (p.c.rows == 0 || p.c.batch == 0) return TG_OK;
+    p.k = reinterpret_cast<void*>(k->ptr), p.v = reinterpret_cast<void*>(v->ptr);
+    DeviceGuard guard(device_id);
+    if (!guard.ok) return fail(TG_ERR_DEVICE, "cannot use HIP device %d", device_id);
+    const hipError_t e = tg::run_kv_read(p, out_type, reinterpret_cast<hipStream_t>(hip_stream));
+    if (e != hipSuccess) return fail(TG_ERR_LAUNCH, "kv_read launch failed: %s", hipGetErrorString(e));
+    return TG_OK;
+}
+
+// What the launch of an attention call goes by; the sizes are in range (check_kv_cache's limits).
+static tg::KvAttentionParams attention_sizes(int64_t tokens, int64_t q_heads, int64_t batch, int64_t heads, int64_t dim, int64_t page_size, int64_t width,
+                                             int32_t window, int32_t sinks) {
+    tg::KvAttentionParams p{};
+    p.c.rows = (int)tokens, p.c.batch = (int)batch, p.c.heads = (int)heads, p.c.dim = (int)dim, p.c.width = (int)width;
+    for (p.c.page_log2 = 4; ((int64_t)1 << p.c.page_log2) < page_size;) ++p.c.page_log2;
+    p.q_heads = (int)q_heads, p.group = (int)(q_heads / heads), p.window = window, p.sinks = sinks;
+    p.splits = tg::kv_attention_splits(p);
+    return p;
+}
+
+int64_t tg_fp8_kv_attention_workspace_bytes(int64_t tokens, int64_t q_heads, int64_t batch, int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                                            int64_t max_pages, int32_t window, int32_t sink_tokens) {
+    if (tokens < 1 || batch < 1 || kv_heads < 1 || kv_heads > 65536 || q_heads < kv_heads || q_heads % kv_heads != 0 || q_heads > 65536 || head_dim < 1 ||
+        head_dim > 256 || page_size < 16 || page_size > 128 || max_pages < 1 || max_pages > (1 << 24) || batch > (1 << 24) || window < 0 || sink_tokens < 0 ||
+        tokens * q_heads > INT32_MAX)
+        return 0;
+    const tg::KvAttentionParams p = attention_sizes(tokens, q_heads, batch, kv_heads, head_dim, page_size, max_pages, window, sink_tokens);
+    return tg::kv_attention_part_bytes(p.splits, tokens, q_heads, head_dim);
+}
+
+int32_t tg_fp8_kv_attention(const tg_tensor* out, const tg_tensor* q, const tg_tensor* k_cache, const tg_tensor* v_cache, const tg_tensor* k_scale,
+                            const tg_tensor* v_scale, const tg_tensor* block_table, const tg_tensor* seq_lens, const tg_tensor* indptr, float sm_scale,
+                            int32_t window, int32_t sink_tokens, const tg_tensor* workspace, int32_t device_id, uint64_t hip_stream) {
+    g_err[0] = 0;
+    int32_t rc;
+    if ((rc = check_packed(q, "q")) || (rc = check_tensor(out, "out", 3))) return rc;
+    tg::KvCache c;
+    const int64_t T = q->shape[0], QH = q->shape[1];
+    if ((rc = check_kv_cache(k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, true, indptr, T, c))) return rc;
+    if (out->dtype != q->dtype) return fail(TG_ERR_DTYPE, "out must have q's dtype");
+    if (q->shape[2] != c.dim) return fail(TG_ERR_INVALID, "q must be (tokens, heads, %d)", c.dim);
+    for (int i = 0; i < 3; ++i)
+        if (out->shape[i] != q->shape[i]) return fail(TG_ERR_INVALID, "out must have the shape of q");
+    if (QH < 1 || QH > 65536 || QH % c.heads != 0) return fail(TG_ERR_INVALID, "q's heads (%lld) must be a multiple of the cache's (%d)", (long long)QH, c.heads);
+    if (T * QH > INT32_MAX) return fail(TG_ERR_INVALID, "too many rows");
+    if (!std::isfinite(sm_scale)) return fail(TG_ERR_INVALID, "sm_scale must be finite");
+    if (window < 0 || sink_tokens < 0) return fail(TG_ERR_INVALID, "window and sink_tokens must not be negative");
+    if (window == 0 && sink_tokens != 0) return fail(TG_ERR_INVALID, "sink_tokens need a window");
+    if (!aligned16(out->ptr)) return fail(TG_ERR_INVALID, "out must be 16-byte aligned");
+    if (T == 0 || c.batch == 0) return TG_OK;
+    if (out->ptr == q->ptr) return fail(TG_ERR_INVALID, "out must not be q");
+    tg::KvAttentionParams p = attention_sizes(T, QH, c.batch, c.heads, c.dim, (int64_t)1 << c.page_log2, c.width, window, sink_tokens);
+    p.c = c;
+    const int64_t need = tg::kv_attention_part_bytes(p.splits, T, QH, c.dim);
+    if (need > 0) {
+        if ((rc = check_tensor(workspace, "workspace", -1))) return rc;
+        if (numel(workspace) * elem_size(workspace->dtype) < need || !aligned16(workspace->ptr))
+            return fail(TG_ERR_INVALID, "workspace must be 16-byte aligned and hold %lld bytes", (long long)need);
+        p.part_o = reinterpret_cast<float*>(workspace->ptr);
+        p.part_ml = p.part_o + (int64_t)p.splits * T * QH * c.dim;
+    }
+    p.q = reinterpret_cast<const void*>(q->ptr), p.out = reinterpret_cast<void*>(out->ptr);
+    p.q_row = q->strides[0], p.q_head = q->strides[1];
+    p.scale_log2 = sm_scale * 1.44269504088896341f;
+    DeviceGuard guard(device_id);
+    if (!guard.ok) return fail(TG_ERR_DEVICE, "cannot use HIP device %d", device_id);
+    const hipError_t e = tg::run_kv_attention(p, q->dtype == TG_BF16, reinterpret_cast<hipStream_t>(hip_stream));
+    if (e != hipSuccess) return fail(TG_ERR_LAUNCH, "kv_attention launch failed: %s", hipGetErrorString(e));
+    return TG_OK;
+}
+
 int32_t tg_silu_mul_quant_1x128(const tg_tensor* q, const tg_tensor* scales, const tg_tensor* x,
                                 int32_t device_id, uint64_t hip_stream) {
     g_err[0] = 0;

@@ -10,11 +10,12 @@ boundaries, and the row-major form here follows the oracle's division, not that 
 
 from __future__ import annotations
 
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
+from .backend import register_impl
 
 FP8 = torch.float8_e4m3fn
 _GROUPS = (16, 32, 64, 128)
@@ -83,3 +84,32 @@ def weight_dequant(x: torch.Tensor, s: torch.Tensor, block_size: int = 128,
     if x.dtype != FP8 or dtype not in _ACT_DTYPES:
         raise NotImplementedError(f"weight_dequant: {x.dtype} -> {dtype} is not implemented (e4m3fn -> bf16 / f16 / f32)")
     return _lib.fp8_weight_dequant(x, s.float(), block_size, dtype)
+
+
+@register_impl("rms_norm_quant", backend="hip")
+def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None,
+                   group_size: Optional[int] = 128, scale: Optional[torch.Tensor] = None, residual_out: Optional[torch.Tensor] = None,
+                   return_norm: bool = False) -> Tuple[torch.Tensor, ...]:
+    """Norm with the residual's addition and an e4m3 output: see ``tilegym_amd.ops.rms_norm_quant``."""
+    _require_device(x, "rms_norm_quant", 128 if scale is not None else group_size)
+    for name, t in (("weight", weight), ("residual", residual), ("scale", scale), ("residual_out", residual_out)):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"rms_norm_quant: {name} is on {t.device}, x on {x.device}")
+    if residual_out is not None and residual is None:
+        raise ValueError("rms_norm_quant: residual_out without residual")
+    for name, t in (("residual", residual), ("residual_out", residual_out)):
+        if t is not None and t.shape != x.shape:
+            raise ValueError(f"rms_norm_quant: {name} must have x's shape {tuple(x.shape)}, got {tuple(t.shape)}")
+    q = torch.empty(x.shape, dtype=FP8, device=x.device)
+    scales = None
+    if scale is None:
+        assert x.shape[-1] % group_size == 0, "the last dimension of `x` must be divisible by `group_size`"
+        scales = torch.empty(x.shape[:-1] + (x.shape[-1] // group_size,), dtype=torch.float32, device=x.device)
+    if residual is not None and residual_out is None:
+        residual_out = torch.empty_like(x)
+    norm = torch.empty_like(x) if return_norm else None
+    _lib.fp8_rms_norm_quant(q, scales, norm, residual_out, x, weight, residual, scale, eps, group_size or 0)
+    out = (q, scales if scale is None else scale)
+    if residual is not None:
+        out += (residual_out,)
+    return out + (norm,) if return_norm else out
