@@ -69,7 +69,8 @@ class TileGymHipError(RuntimeError):
 _lib = None
 native = None  # the extension module, once load() has run (still None where it cannot be imported)
 _NATIVE_ENTRY_POINTS = ("tg_fp8_gemm", "tg_fp8_gemm_workspace_bytes", "tg_fp8_ragged_gemm", "tg_fp8_quant_group", "tg_fp8_fused_moe",
-                        "tg_fp8_fused_moe_block_m", "tg_fp8_fused_moe_workspace_bytes")
+                        "tg_fp8_fused_moe_block_m", "tg_fp8_fused_moe_workspace_bytes", "tg_fp8_rms_norm_quant", "tg_fp8_kv_append",
+                        "tg_fp8_kv_read", "tg_fp8_kv_attention", "tg_fp8_kv_attention_workspace_bytes")
 
 
 def lib_path() -> str:

@@ -28,6 +28,11 @@ decltype(&tg_fp8_quant_group) g_quant_group = nullptr;
 decltype(&tg_fp8_fused_moe) g_fused_moe = nullptr;
 decltype(&tg_fp8_fused_moe_block_m) g_fused_moe_block_m = nullptr;
 decltype(&tg_fp8_fused_moe_workspace_bytes) g_fused_moe_workspace_bytes = nullptr;
+decltype(&tg_fp8_rms_norm_quant) g_rms_norm_quant = nullptr;
+decltype(&tg_fp8_kv_append) g_kv_append = nullptr;
+decltype(&tg_fp8_kv_read) g_kv_read = nullptr;
+decltype(&tg_fp8_kv_attention) g_kv_attention = nullptr;
+decltype(&tg_fp8_kv_attention_workspace_bytes) g_kv_attention_workspace_bytes = nullptr;
 PyObject* g_workspaces = nullptr;     // {(device, stream, under capture): [scratch tensors, newest last]}
 PyObject* g_workspace_for = nullptr;  // callable(device, bytes, index, stream) -> tensor, for a new or larger one
 PyObject* g_check_rc = nullptr;       // callable(rc, where): raises
@@ -328,6 +333,198 @@ PyObject* py_fused_moe(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// An optional tensor of the first tensor's device: described into *d and *p set; a None leaves *p null.  False: not plain.
+bool optional_tensor(PyObject* o, const at::Tensor& like, tg_tensor* d, const tg_tensor** p) {
+    *p = nullptr;
+    if (o == Py_None) return true;
+    const at::Tensor* t = tensor_of(o);
+    if (!on_gpu(t) || t->device() != like.device() || !describe(*t, d)) return false;
+    *p = d;
+    return true;
+}
+
+// rms_norm_quant(x, weight, eps, residual, group_size, scale, residual_out, return_norm) -> tuple, or None.  group_size 0 with a scale
+PyObject* py_rms_norm_quant(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 8) { PyErr_SetString(PyExc_TypeError, "rms_norm_quant takes 8 arguments"); return nullptr; }
+    const at::Tensor* x = tensor_of(args[0]);
+    const double eps = PyFloat_AsDouble(args[2]);
+    const long group = PyLong_AsLong(args[4]);
+    if (PyErr_Occurred()) return nullptr;
+    const bool given = args[5] != Py_None;
+    if (!on_gpu(x) || !io_type(x->scalar_type()) || !x->is_contiguous() || x->dim() < 1 || x->dim() > TG_MAX_DIMS ||
+        (!given && (group <= 0 || x->size(x->dim() - 1) % group != 0)))
+        Py_RETURN_NONE;
+    tg_tensor dx, dw, dr, dro, dsc, dq, ds, dn;
+    const tg_tensor *w, *r, *ro, *sc;
+    if (!describe(*x, &dx) || !optional_tensor(args[1], *x, &dw, &w) || !w || !optional_tensor(args[3], *x, &dr, &r) || !optional_tensor(args[6], *x, &dro, &ro) ||
+        !optional_tensor(args[5], *x, &dsc, &sc))
+        Py_RETURN_NONE;
+    if ((r && tensor_of(args[3])->sizes() != x->sizes()) || (ro && (!r || tensor_of(args[6])->sizes() != x->sizes()))) Py_RETURN_NONE;
+    at::Tensor q = new_tensor(x->sizes(), at::kFloat8_e4m3fn, *x), scales, made_residual, norm;
+    if (!describe(q, &dq)) Py_RETURN_NONE;
+    if (!given) {
+        c10::SmallVector<int64_t, 4> sizes(x->sizes().begin(), x->sizes().end());
+        sizes.back() /= group;
+        scales = new_tensor(sizes, at::kFloat, *x);
+        if (!describe(scales, &ds)) Py_RETURN_NONE;
+    }
+    if (r && !ro) {
+        made_residual = new_tensor(x->sizes(), x->scalar_type(), *x);
+        if (!describe(made_residual, &dro)) Py_RETURN_NONE;
+        ro = &dro;
+    }
+    const bool with_norm = args[7] == Py_True;
+    if (with_norm) {
+        norm = new_tensor(x->sizes(), x->scalar_type(), *x);
+        if (!describe(norm, &dn)) Py_RETURN_NONE;
+    }
+    const int index = x->get_device();
+    const hipStream_t stream = c10::hip::getCurrentHIPStream(index).stream();
+    int32_t rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_rms_norm_quant(&dq, given ? nullptr : &ds, with_norm ? &dn : nullptr, ro, &dx, w, r, sc, (float)eps, (int32_t)group, index,
+                          (uint64_t)(uintptr_t)stream);
+    Py_END_ALLOW_THREADS
+    if (!succeeded(rc, "tg_fp8_rms_norm_quant")) return nullptr;
+    PyObject* tuple = PyTuple_New(2 + (r != nullptr) + with_norm);
+    if (!tuple) return nullptr;
+    int at = 0;
+    auto borrowed = [](PyObject* o) { Py_INCREF(o); return o; };
+    PyTuple_SET_ITEM(tuple, at++, THPVariable_Wrap(std::move(q)));
+    PyTuple_SET_ITEM(tuple, at++, given ? borrowed(args[5]) : THPVariable_Wrap(std::move(scales)));
+    if (r) PyTuple_SET_ITEM(tuple, at++, made_residual.defined() ? THPVariable_Wrap(std::move(made_residual)) : borrowed(args[6]));
+    if (with_norm) PyTuple_SET_ITEM(tuple, at++, THPVariable_Wrap(std::move(norm)));
+    return tuple;
+    END_HANDLE_TH_ERRORS
+}
+
+// A paged cache's four tensors, described; null: not four tensors of one device.
+const at::Tensor* describe_cache(PyObject* o, tg_tensor d[4]) {
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) return nullptr;
+    const at::Tensor* first = nullptr;
+    for (int i = 0; i < 4; ++i) {
+        const at::Tensor* t = tensor_of(PyTuple_GET_ITEM(o, i));
+        if (!on_gpu(t) || (first && t->device() != first->device()) || !describe(*t, &d[i])) return nullptr;
+        if (!first) first = t;
+    }
+    return first->dim() == 4 ? first : nullptr;
+}
+
+// kv_append(cache, k, v, block_table, seq_lens, indptr, q, rope, interleaved) -> (q turned or None,), or None
+PyObject* py_kv_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 9) { PyErr_SetString(PyExc_TypeError, "kv_append takes 9 arguments"); return nullptr; }
+    tg_tensor dc[4], d[7], dq_out;
+    const tg_tensor* p[7];
+    const at::Tensor* first = describe_cache(args[0], dc);
+    if (!first) Py_RETURN_NONE;
+    for (int i = 0; i < 7; ++i)
+        if (!optional_tensor(args[1 + i], *first, &d[i], &p[i]) || (i < 5 && !p[i])) Py_RETURN_NONE;
+    const tg_tensor *q = p[5], *rope = p[6];
+    if (q && !rope) Py_RETURN_NONE;
+    at::Tensor q_out;
+    if (q) {
+        const at::Tensor* t = tensor_of(args[6]);
+        q_out = new_tensor(t->sizes(), t->scalar_type(), *t);
+        if (!describe(q_out, &dq_out)) Py_RETURN_NONE;
+    }
+    const int index = first->get_device();
+    const hipStream_t stream = c10::hip::getCurrentHIPStream(index).stream();
+    const int interleaved = PyObject_IsTrue(args[8]);
+    if (interleaved < 0) return nullptr;
+    int32_t rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_kv_append(&dc[0], &dc[1], &dc[2], &dc[3], p[0], p[1], p[2], p[3], p[4], q ? &dq_out : nullptr, q, rope, interleaved, index,
+                     (uint64_t)(uintptr_t)stream);
+    Py_END_ALLOW_THREADS
+    if (!succeeded(rc, "tg_fp8_kv_append")) return nullptr;
+    PyObject* tuple = PyTuple_New(1);
+    if (!tuple) return nullptr;
+    if (q) {
+        PyTuple_SET_ITEM(tuple, 0, THPVariable_Wrap(std::move(q_out)));
+    } else {
+        Py_INCREF(Py_None);
+        PyTuple_SET_ITEM(tuple, 0, Py_None);
+    }
+    return tuple;
+    END_HANDLE_TH_ERRORS
+}
+
+// kv_read(cache, block_table, indptr, total_tokens, out_dtype) -> (k, v), or None
+PyObject* py_kv_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 5) { PyErr_SetString(PyExc_TypeError, "kv_read takes 5 arguments"); return nullptr; }
+    tg_tensor dc[4], dt, di, dk, dv;
+    const tg_tensor *table, *indptr;
+    const at::Tensor* first = describe_cache(args[0], dc);
+    const long long total = PyLong_AsLongLong(args[3]);
+    if (total == -1 && PyErr_Occurred()) return nullptr;
+    if (!first || !optional_tensor(args[1], *first, &dt, &table) || !table || !optional_tensor(args[2], *first, &di, &indptr) || !indptr || total < 0 ||
+        !THPDtype_Check(args[4]))
+        Py_RETURN_NONE;
+    const at::ScalarType type = reinterpret_cast<THPDtype*>(args[4])->scalar_type;
+    if (!io_type(type)) Py_RETURN_NONE;
+    at::Tensor k = new_tensor({total, first->size(1), first->size(3)}, type, *first), v = new_tensor({total, first->size(1), first->size(3)}, type, *first);
+    if (!describe(k, &dk) || !describe(v, &dv)) Py_RETURN_NONE;
+    const int index = first->get_device();
+    const hipStream_t stream = c10::hip::getCurrentHIPStream(index).stream();
+    int32_t rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_kv_read(&dk, &dv, &dc[0], &dc[1], &dc[2], &dc[3], table, indptr, index, (uint64_t)(uintptr_t)stream);
+    Py_END_ALLOW_THREADS
+    if (!succeeded(rc, "tg_fp8_kv_read")) return nullptr;
+    PyObject* tuple = PyTuple_New(2);
+    if (!tuple) return nullptr;
+    PyTuple_SET_ITEM(tuple, 0, THPVariable_Wrap(std::move(k)));
+    PyTuple_SET_ITEM(tuple, 1, THPVariable_Wrap(std::move(v)));
+    return tuple;
+    END_HANDLE_TH_ERRORS
+}
+
+// kv_attention(q, cache, block_table, seq_lens, indptr, sm_scale, window, sink_tokens, out) -> out, or None.  The scratch memory
+// is the call's own: torch's allocator orders its reuse by stream and keeps a graph's apart
+PyObject* py_kv_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 9) { PyErr_SetString(PyExc_TypeError, "kv_attention takes 9 arguments"); return nullptr; }
+    const at::Tensor* q = tensor_of(args[0]);
+    tg_tensor dc[4], dq, dout, dt, dl, di, dws;
+    const tg_tensor *table, *lens, *indptr, *given;
+    const at::Tensor* first = describe_cache(args[1], dc);
+    const double scale = PyFloat_AsDouble(args[5]);
+    const long window = PyLong_AsLong(args[6]), sinks = PyLong_AsLong(args[7]);
+    if (PyErr_Occurred()) return nullptr;
+    if (!on_gpu(q) || !first || q->dim() != 3 || q->device() != first->device() || !describe(*q, &dq) || !optional_tensor(args[2], *q, &dt, &table) || !table ||
+        !optional_tensor(args[3], *q, &dl, &lens) || !lens || !optional_tensor(args[4], *q, &di, &indptr) || !indptr ||
+        !optional_tensor(args[8], *q, &dout, &given) || dt.ndim != 2 || window < 0 || window > INT32_MAX || sinks < 0 || sinks > INT32_MAX)
+        Py_RETURN_NONE;
+    at::Tensor out, ws;
+    if (!given) {
+        out = new_tensor(q->sizes(), q->scalar_type(), *q);
+        if (!describe(out, &dout)) Py_RETURN_NONE;
+    }
+    const int64_t need = g_kv_attention_workspace_bytes(q->size(0), q->size(1), dt.shape[0], first->size(1), first->size(3), first->size(2), dt.shape[1],
+                                                        (int32_t)window, (int32_t)sinks);
+    if (need > 0) {
+        ws = new_tensor({need}, at::kByte, *q);
+        if (!describe(ws, &dws)) Py_RETURN_NONE;
+    }
+    const int index = q->get_device();
+    const hipStream_t stream = c10::hip::getCurrentHIPStream(index).stream();
+    int32_t rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = g_kv_attention(&dout, &dq, &dc[0], &dc[1], &dc[2], &dc[3], table, lens, indptr, (float)scale, (int32_t)window, (int32_t)sinks,
+                        need > 0 ? &dws : nullptr, index, (uint64_t)(uintptr_t)stream);
+    Py_END_ALLOW_THREADS
+    if (!succeeded(rc, "tg_fp8_kv_attention")) return nullptr;
+    if (given) {
+        Py_INCREF(args[8]);
+        return args[8];
+    }
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
 // set_up({name: address}, workspaces, workspace_for, check_rc)
 PyObject* py_set_up(PyObject*, PyObject* args) {
     PyObject *table, *workspaces, *workspace_for, *check_rc;
@@ -341,6 +538,8 @@ PyObject* py_set_up(PyObject*, PyObject* args) {
     };
     if (!find("tg_fp8_gemm", &g_gemm) || !find("tg_fp8_gemm_workspace_bytes", &g_gemm_workspace_bytes) || !find("tg_fp8_ragged_gemm", &g_ragged_gemm) ||
         !find("tg_fp8_quant_group", &g_quant_group) || !find("tg_fp8_fused_moe", &g_fused_moe) ||
+        !find("tg_fp8_rms_norm_quant", &g_rms_norm_quant) || !find("tg_fp8_kv_append", &g_kv_append) || !find("tg_fp8_kv_read", &g_kv_read) ||
+        !find("tg_fp8_kv_attention", &g_kv_attention) || !find("tg_fp8_kv_attention_workspace_bytes", &g_kv_attention_workspace_bytes) ||
         !find("tg_fp8_fused_moe_block_m", &g_fused_moe_block_m) || !find("tg_fp8_fused_moe_workspace_bytes", &g_fused_moe_workspace_bytes))
         return nullptr;
     for (auto [slot, o] : {std::pair{&g_workspaces, workspaces}, std::pair{&g_workspace_for, workspace_for}, std::pair{&g_check_rc, check_rc}}) {
@@ -358,6 +557,10 @@ PyMethodDef kMethods[] = {TG_FAST("matmul", py_matmul),
                           TG_FAST("act_quant", py_act_quant),
                           TG_FAST("ragged_matmul", py_ragged_matmul),
                           TG_FAST("fused_moe", py_fused_moe),
+                          TG_FAST("rms_norm_quant", py_rms_norm_quant),
+                          TG_FAST("kv_append", py_kv_append),
+                          TG_FAST("kv_read", py_kv_read),
+                          TG_FAST("kv_attention", py_kv_attention),
                           {"set_up", py_set_up, METH_VARARGS, nullptr},
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

@@ -20,6 +20,10 @@ def _one_device(where: str, *tensors) -> None:
 
 @register_impl("kv_cache_append", backend="hip")
 def kv_cache_append(cache, k, v, block_table, seq_lens, indptr, q=None, rope=None, interleaved=False):
+    if _lib.native_path():
+        done = _lib.native.kv_append(cache, k, v, block_table, seq_lens, indptr, q, rope, interleaved)
+        if done is not None:
+            return done[0]
     _one_device("kv_cache_append", k, v, *cache, block_table, seq_lens, indptr, q, rope)
     q_out = None
     if q is not None:
@@ -32,6 +36,10 @@ def kv_cache_append(cache, k, v, block_table, seq_lens, indptr, q=None, rope=Non
 
 @register_impl("kv_cache_read", backend="hip")
 def kv_cache_read(cache, block_table, indptr, total_tokens, out_dtype=torch.bfloat16, k_out=None, v_out=None):
+    if k_out is None and v_out is None and _lib.native_path():
+        out = _lib.native.kv_read(cache, block_table, indptr, total_tokens, out_dtype)
+        if out is not None:
+            return out
     _one_device("kv_cache_read", *cache, block_table, indptr, k_out, v_out)
     if cache[0].dim() != 4:
         raise ValueError("kv_cache_read: the cache's k must be (pages, heads, page size, head dim)")
@@ -46,10 +54,17 @@ def kv_cache_read(cache, block_table, indptr, total_tokens, out_dtype=torch.bflo
 
 @register_impl("kv_cache_attention", backend="hip")
 def kv_cache_attention(q, cache, block_table, seq_lens, indptr, sm_scale=None, window=0, sink_tokens=0, out=None):
+    for name, value in (("window", window), ("sink_tokens", sink_tokens)):
+        if not 0 <= value < 2 ** 31:
+            raise ValueError(f"kv_cache_attention: {name} must be in [0, 2^31), got {value}")
+    if sm_scale is None:
+        sm_scale = q.shape[-1] ** -0.5 if q.dim() and q.shape[-1] else 1.0
+    if _lib.native_path():
+        done = _lib.native.kv_attention(q, cache, block_table, seq_lens, indptr, sm_scale, window, sink_tokens, out)
+        if done is not None:
+            return done
     _one_device("kv_cache_attention", q, *cache, block_table, seq_lens, indptr, out)
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if sm_scale is None:
-        sm_scale = q.shape[-1] ** -0.5 if q.dim() and q.shape[-1] else 1.0
     _lib.fp8_kv_attention(out, q, cache, block_table, seq_lens, indptr, sm_scale, window, sink_tokens)
     return out

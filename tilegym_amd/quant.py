@@ -91,6 +91,10 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, res
                    group_size: Optional[int] = 128, scale: Optional[torch.Tensor] = None, residual_out: Optional[torch.Tensor] = None,
                    return_norm: bool = False) -> Tuple[torch.Tensor, ...]:
     """Norm with the residual's addition and an e4m3 output: see ``tilegym_amd.ops.rms_norm_quant``."""
+    if (scale is not None or group_size in _GROUPS) and _lib.native_path():
+        out = _lib.native.rms_norm_quant(x, weight, eps, residual, group_size or 0, scale, residual_out, return_norm)
+        if out is not None:
+            return out
     _require_device(x, "rms_norm_quant", 128 if scale is not None else group_size)
     for name, t in (("weight", weight), ("residual", residual), ("scale", scale), ("residual_out", residual_out)):
         if t is not None and t.device != x.device:
