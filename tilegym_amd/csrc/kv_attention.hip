@@ -53,6 +53,9 @@ __device__ __forceinline__ typename Types<T>::v8 widen(int lo, int hi) {
 
 constexpr float kMinusInf = -__builtin_inff();
 constexpr float kSmallestUnit = 0x1p-126f;
+// The maximum that scores are taken against moves only when it has grown by more than this (in powers of two): weights are then at most
+// 2^8, which costs no precision in floating point, and O is rescaled a few times in all instead of in most steps.
+constexpr float kSlack = 8.f;
 
 // The rows of one workgroup and the steps of 64 keys that any of them sees.
 struct RowTile {
@@ -260,6 +263,229 @@ __global__ void __launch_bounds__(256) kv_attention_kernel(const KvAttentionPara
     }
 }
 
+// Many rows: 128 of them per workgroup, 32 per wave, and every wave runs over the same keys, whose codes are staged in LDS for all
+// four: 16 bytes per lane and load through registers, the next step's while this one's products run, in two buffers with one
+// barrier a step.  Codes stay e4m3 in LDS (half the reads that 16 bits would cost) and are widened behind each read for 32 rows.
+// 16-byte chunks are placed so that the 16 lanes that read together (16 rows of one fragment, one chunk each) cover all banks:
+//   k, chunks of row `key`: chunk ^ f, rows of a fragment being 16 a + 4 i + b;  v, 4 chunks a row: chunk ^ (row / 4) % 4
+template <int D>
+__device__ __forceinline__ int k_swizzle(int row) {
+    const int a = (row >> 4) & 3, b = row & 3;
+    return D == 64 ? a : D == 128 ? 2 * a + (b >> 1) : 4 * a + b;
+}
+__device__ __forceinline__ int v_swizzle(int row) { return (row >> 2) & 3; }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_rows_kernel(const KvAttentionParams p, int items) {
+    typedef typename Types<T>::v8 v8;
+    constexpr int CH = D / 64, DT = D / 16, LOADS = D / 64, KCH = D / 16;
+    __shared__ __align__(16) uint8_t lds_k[2][64 * D], lds_v[2][64 * D];
+    const KvCache& c = p.c;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
+    const int head = (int)blockIdx.x % c.heads, rest = (int)blockIdx.x / c.heads, split = rest % p.splits;
+    RowTile t;
+    if (!find_tile(p, 128, items - 1 - rest / p.splits, head, t)) return;  // (the last rows of a sequence, which see most, first)
+    const int share = max((t.steps + p.splits - 1) / p.splits, 4);
+    const int begin = min(split * share, t.steps), end = min(begin + share, t.steps);
+
+    // this lane's two rows
+    int64_t position[2];
+    v8 q[2][CH][2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const int row = wave * 32 + n * 16 + col, r = t.r0 + row, token = r / p.group, q_head = head * p.group + r % p.group;
+        position[n] = row < t.rows ? t.start + token : -1;
+#pragma unroll
+        for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (row < t.rows) q[n][ch][h] = *reinterpret_cast<const v8*>((const T*)p.q + (int64_t)(t.first + token) * p.q_row + (int64_t)q_head * p.q_head + ch * 64 + g * 16 + h * 8);
+                else q[n][ch][h] = v8{};
+            }
+    }
+    const int wave_rows = min(t.rows - wave * 32, 32);
+    const int64_t wave_low = t.start + (t.r0 + wave * 32) / p.group, wave_high = t.start + (t.r0 + wave * 32 + wave_rows - 1) / p.group;
+
+    const int P = 1 << c.page_log2, in_page = P - 1;
+    const int64_t block_bytes = (int64_t)P * D;
+    v4f o[2][DT];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[n][d] = v4f{0.f, 0.f, 0.f, 0.f};
+    float m[2] = {kMinusInf, kMinusInf}, l[2] = {0.f, 0.f}, u = kSmallestUnit;
+
+    // a step's pages, one per group of 16 lanes, then its codes and scales on their way to LDS
+    v4i k_reg[LOADS], v_reg[LOADS];
+    float k_scale, v_scale;
+    Granule page{0, false}, there{0, false};
+    auto load_page = [&](int step) { if (step < end) page = granule_of(c, t.seq, t.key_of(step) + 16 * g); };
+    auto load_codes = [&](int step) {
+        there = page;
+        const int64_t key = t.key_of(step), at = (int64_t)page.page * c.heads + head;
+        k_scale = c.k_scale[at], v_scale = c.v_scale[at];
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            const int ci = tid + 256 * j, row = ci / KCH, chunk = (ci % KCH) ^ k_swizzle<D>(row);
+            const int64_t block = (int64_t)__shfl(page.page, (row >> 4) * 16) * c.heads + head;
+            k_reg[j] = *reinterpret_cast<const v4i*>(c.k + block * block_bytes + (int64_t)((key + row) & in_page) * D + chunk * 16);
+        }
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            const int ci = tid + 256 * j, row = ci / 4, chunk = (ci & 3) ^ v_swizzle(row);
+            const int64_t block = (int64_t)__shfl(page.page, chunk * 16) * c.heads + head;
+            v_reg[j] = *reinterpret_cast<const v4i*>(c.v + block * block_bytes + (int64_t)row * P + ((key + 16 * chunk) & in_page));
+        }
+    };
+    auto store_codes = [&](int step, int buffer) {
+        const int64_t key = t.key_of(step);
+        const bool whole = key + 64 <= t.key1 && key >= t.key0 && __ballot(!there.there) == 0;
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) *reinterpret_cast<v4i*>(&lds_k[buffer][(tid + 256 * j) * 16]) = k_reg[j];
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            const int ci = tid + 256 * j, chunk = (ci & 3) ^ v_swizzle(ci / 4);
+            if (!whole) {  // codes that no row sees: behind the last key, before the window, in no page
+                const int64_t first = key + 16 * chunk;
+                const bool any = __shfl((int)there.there, chunk * 16) && first < t.key1 && (first + 16 > t.key0 || first < p.sinks);
+                const int live = any ? (int)min(t.key1 - first, (int64_t)16) : 0;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const int bytes = min(max(live - 4 * w, 0), 4);
+                    v_reg[j][w] &= bytes == 4 ? -1 : (1 << (8 * bytes)) - 1;
+                }
+            }
+            *reinterpret_cast<v4i*>(&lds_v[buffer][ci * 16]) = v_reg[j];
+        }
+    };
+
+    if (begin < end) {
+        load_page(begin);
+        load_codes(begin);
+        load_page(begin + 1);
+        store_codes(begin, 0);
+    }
+    __syncthreads();
+    for (int step = begin; step < end; ++step) {
+        const int buffer = (step - begin) & 1;
+        const int64_t key = t.key_of(step), mine = key + 16 * g;
+        const float factor = k_scale * p.scale_log2;
+        float v_unit = v_scale;
+        const bool page_there = there.there;
+        if (step + 1 < end) {
+            load_codes(step + 1);
+            load_page(step + 2);
+        }
+        if (wave_rows > 0 && key <= wave_high) {
+            v4f s[2][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[0][i] = s[1][i] = v4f{0.f, 0.f, 0.f, 0.f};
+                const int row = 16 * (col >> 2) + 4 * i + (col & 3);
+#pragma unroll
+                for (int ch = 0; ch < CH; ++ch) {
+                    const v4i kc = *reinterpret_cast<const v4i*>(&lds_k[buffer][row * D + ((ch * 4 + g) ^ k_swizzle<D>(row)) * 16]);
+                    const v8 a = widen<T>(kc[0], kc[1]), b = widen<T>(kc[2], kc[3]);
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        s[n][i] = mfma16(a, q[n][ch][0], s[n][i]);
+                        s[n][i] = mfma16(b, q[n][ch][1], s[n][i]);
+                    }
+                }
+            }
+            const bool whole = key + 63 <= wave_low && (!p.window || key > wave_high - p.window) && __ballot(!page_there) == 0;
+            if (!whole && !(page_there && mine < t.key1 && (mine + 16 > t.key0 || mine < p.sinks))) v_unit = 0.f;
+            float unit = fmaxf(v_unit, __shfl_xor(v_unit, 16));
+            unit = fmaxf(fmaxf(unit, __shfl_xor(unit, 32)), u);
+            const float ratio = v_unit / unit;
+            float rescale[2];
+            v8 pt[2][2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[n][i] *= factor;
+                if (!whole) {
+                    const int64_t first_seen = p.window ? position[n] - p.window + 1 : 0;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int64_t j = mine + i;
+                        const bool seen = page_there && j <= position[n] && (j >= first_seen || j < p.sinks);
+                        s[n][i / 4][i % 4] = seen ? s[n][i / 4][i % 4] : kMinusInf;
+                    }
+                }
+                float top = fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3]));
+#pragma unroll
+                for (int i = 1; i < 4; ++i) top = fmaxf(top, fmaxf(fmaxf(s[n][i][0], s[n][i][1]), fmaxf(s[n][i][2], s[n][i][3])));
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float m_new = top > m[n] + kSlack ? top : m[n], base = m_new == kMinusInf ? 0.f : m_new;
+                const float shrink = __builtin_amdgcn_exp2f(m[n] - base);
+                rescale[n] = m_new == m[n] ? u / unit : shrink * (u / unit);
+                l[n] = m_new == m[n] ? l[n] : l[n] * shrink;
+                m[n] = m_new;
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        s[n][i][j] = __builtin_amdgcn_exp2f(s[n][i][j] - base);
+                        sum += s[n][i][j];
+                    }
+                l[n] += sum;
+                if (__ballot(ratio != 1.f)) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[n][i] *= ratio;
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    pt[n][h] = __builtin_convertvector(__builtin_shufflevector(s[n][2 * h], s[n][2 * h + 1], 0, 1, 2, 3, 4, 5, 6, 7), v8);
+            }
+            u = unit;
+            if (__ballot(rescale[0] != 1.f || rescale[1] != 1.f)) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) o[n][d] *= rescale[n];
+            }
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const int row = d * 16 + col;
+                const v4i vc = *reinterpret_cast<const v4i*>(&lds_v[buffer][row * 64 + (g ^ v_swizzle(row)) * 16]);
+                const v8 a = widen<T>(vc[0], vc[1]), b = widen<T>(vc[2], vc[3]);
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    o[n][d] = mfma16(a, pt[n][0], o[n][d]);
+                    o[n][d] = mfma16(b, pt[n][1], o[n][d]);
+                }
+            }
+        }
+        if (step + 1 < end) store_codes(step + 1, buffer ^ 1);
+        __syncthreads();
+    }
+
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        float sum = l[n] + __shfl_xor(l[n], 16);
+        sum += __shfl_xor(sum, 32);
+        const int row = wave * 32 + n * 16 + col, r = t.r0 + row;
+        if (row >= t.rows) continue;
+        const int64_t out_row = (int64_t)(t.first + r / p.group) * p.q_heads + head * p.group + r % p.group;
+        if (p.splits > 1) {
+            const int64_t at = (int64_t)split * c.rows * p.q_heads + out_row;
+            if (g == 0) p.part_ml[2 * at] = m[n], p.part_ml[2 * at + 1] = sum;
+            if (sum > 0.f) {
+#pragma unroll
+                for (int d = 0; d < DT; ++d) *reinterpret_cast<v4f*>(p.part_o + at * D + d * 16 + 4 * g) = o[n][d] * u;
+            }
+        } else {
+            typedef T v4t __attribute__((ext_vector_type(4)));
+            const float f = sum > 0.f ? u / sum : 0.f;  // a row that sees nothing is zero
+#pragma unroll
+            for (int d = 0; d < DT; ++d) *reinterpret_cast<v4t*>((T*)p.out + out_row * D + d * 16 + 4 * g) = __builtin_convertvector(o[n][d] * f, v4t);
+        }
+    }
+}
+
 // out = sum over splits of exp2(m_s - m) O_s, over the sum of exp2(m_s - m) l_s: D / 4 lanes per row of q, in the order of the splits.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv_attention_join_kernel(const KvAttentionParams p) {
@@ -287,12 +513,18 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const KvAttentio
     *reinterpret_cast<v4t*>((T*)p.out + row * D + e) = __builtin_convertvector(x, v4t);
 }
 
+// Tiles that can begin: sum over sequences of ceil(n * group / tile_rows), see find_sequence.
+int64_t row_tiles(const KvAttentionParams& p, int64_t tile_rows) { return (int64_t)p.c.rows * p.group / tile_rows + p.c.batch; }
+// The form for many rows: by the rows that a sequence's key/value head has on average, as the host does not read the tensors.
+bool many_rows(const KvAttentionParams& p) { return (int64_t)p.c.rows * p.group > 32 * (int64_t)p.c.batch; }
+
 template <typename T, int D>
 hipError_t launch(const KvAttentionParams& p, hipStream_t s) {
-    const int64_t tiles = (int64_t)p.c.rows * p.group / 16 + p.c.batch, blocks = tiles * p.c.heads * p.splits;
+    const int64_t tile_rows = many_rows(p) ? 128 : 16, tiles = row_tiles(p, tile_rows), blocks = tiles * p.c.heads * p.splits;
     const int64_t join = ((int64_t)p.c.rows * p.q_heads * (D / 4) + 255) / 256;
     if (blocks > INT32_MAX || join > INT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((kv_attention_kernel<T, D>), dim3((unsigned)blocks), dim3(256), 0, s, p);
+    if (many_rows(p)) hipLaunchKernelGGL((kv_attention_rows_kernel<T, D>), dim3((unsigned)blocks), dim3(256), 0, s, p, (int)tiles);
+    else hipLaunchKernelGGL((kv_attention_kernel<T, D>), dim3((unsigned)blocks), dim3(256), 0, s, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
     hipLaunchKernelGGL((kv_attention_join_kernel<T, D>), dim3((unsigned)join), dim3(256), 0, s, p);
@@ -302,7 +534,7 @@ hipError_t launch(const KvAttentionParams& p, hipStream_t s) {
 }  // namespace
 
 int kv_attention_splits(const KvAttentionParams& p) {
-    const int64_t tiles = (int64_t)p.c.rows * p.group / 16 + p.c.batch, units = tiles * p.c.heads;
+    const int64_t units = row_tiles(p, many_rows(p) ? 128 : 16) * p.c.heads;
     int64_t keys = (int64_t)p.c.width << p.c.page_log2;
     if (p.window) keys = std::min<int64_t>(keys, (int64_t)p.window + 128 + (p.sinks + 63) / 64 * 64);
     const int64_t steps = (keys + 63) / 64;
