@@ -22,6 +22,9 @@
 #include <algorithm>
 #include <type_traits>
 
+#ifndef TG_WANT
+#define TG_WANT 512
+#endif
 namespace tg {
 namespace {
 
@@ -51,21 +54,26 @@ __device__ __forceinline__ typename Types<T>::v8 widen(int lo, int hi) {
     return __builtin_shufflevector(__builtin_shufflevector(a, b, 0, 1, 2, 3), __builtin_shufflevector(c, d, 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+constexpr int kMostSplits = 64;
+constexpr int kLeastSteps = 4;  // of a split
 constexpr float kMinusInf = -__builtin_inff();
 constexpr float kSmallestUnit = 0x1p-126f;
-// The maximum that scores are taken against moves only when it has grown by more than this (in powers of two): weights are then at most
-// 2^8, which costs no precision in floating point, and O is rescaled a few times in all instead of in most steps.
-constexpr float kSlack = 8.f;
+// The maximum that a row's scores are taken against is looked for only when 16 weights against the old one add up to more than this: floating
+// point loses no precision in weights above 1 (f16 holds 16 times as much, and sums and O are fp32).  A row's first keys find a maximum of
+// -inf and so a sum that is not a number, and take the same path.  In the other steps there is no search, no exchange between lanes
+// and no rescaling of O.
+constexpr float kLargeSum = 4096.f;
 
-// The rows of one workgroup and the steps of 64 keys that any of them sees.
+// The rows of one workgroup and the steps of 64 keys that any of them sees.  Positions and keys are below 2^30 (the table's capacity)
+// or a sequence's length.
 struct RowTile {
     int seq, head;          // sequence, key/value head
     int first, r0, rows;    // sequence's first packed row; the tile's first row of the sequence, and how many it has
-    int64_t start;          // position of the sequence's first new token
-    int64_t low, high;      // positions of the tile's first and last row
-    int64_t key0, key1;     // keys [key0, key1) and, below key0, [0, sinks)
+    int start;              // position of the sequence's first new token
+    int low, high;          // positions of the tile's first and last row
+    int key0, key1;         // keys [key0, key1) and, below key0, [0, sinks)
     int steps, sink_steps;  // steps of 64 keys: sink_steps from 0 on, then from key0 / 64 on
-    __device__ __forceinline__ int64_t key_of(int step) const { return step < sink_steps ? (int64_t)step * 64 : ((key0 >> 6) + step - sink_steps) * 64; }
+    __device__ __forceinline__ int key_of(int step) const { return (step < sink_steps ? step : (key0 >> 6) + step - sink_steps) * 64; }
 };
 
 __device__ __forceinline__ bool find_tile(const KvAttentionParams& p, int tile_rows, int item, int head, RowTile& t) {
@@ -76,189 +84,308 @@ __device__ __forceinline__ bool find_tile(const KvAttentionParams& p, int tile_r
     if (r0 >= total) return false;
     t.seq = f.seq, t.head = head, t.first = f.first;
     t.r0 = (int)r0, t.rows = (int)min((int64_t)tile_rows, total - r0);
-    t.start = (int64_t)max(c.lens[f.seq], 0) - f.n;
+    t.start = max(c.lens[f.seq], 0) - f.n;
     t.low = t.start + t.r0 / p.group, t.high = t.start + (t.r0 + t.rows - 1) / p.group;
-    const int64_t capacity = (int64_t)c.width << c.page_log2;
-    t.key1 = max(min(t.high + 1, capacity), (int64_t)0);
-    t.key0 = p.window ? min(max(t.low - p.window + 1, (int64_t)0), t.key1) : 0;
-    const int64_t sinks = min((int64_t)p.sinks, t.key0);
-    t.sink_steps = (int)min((sinks + 63) >> 6, t.key0 >> 6);
-    t.steps = t.key1 > 0 ? t.sink_steps + (int)(((t.key1 + 63) >> 6) - (t.key0 >> 6)) : 0;
+    const int capacity = c.width << c.page_log2;
+    t.key1 = t.high < 0 ? 0 : t.high < capacity ? t.high + 1 : capacity;
+    t.key0 = p.window ? min(max(t.low - (p.window - 1), 0), t.key1) : 0;
+    const int sinks = min(p.sinks, t.key0);
+    t.sink_steps = min((sinks + 63) >> 6, t.key0 >> 6);
+    t.steps = t.key1 > 0 ? t.sink_steps + (((t.key1 + 63) >> 6) - (t.key0 >> 6)) : 0;
     return true;
 }
 
-// A page for lane's 16 keys from `key` on, or one that may be read in its place (its keys are then not seen).
+// The table's entry for the page of 16 keys, as it is: looked at a step later (page_of), so that the load is not waited for.
+__device__ __forceinline__ int table_entry(const KvCache& c, const int* row, int key) { return row[min(key >> c.page_log2, c.width - 1)]; }
+// A page, or one that may be read in its place (its keys are then not seen).
 struct Granule {
     int page;
     bool there;
 };
-__device__ __forceinline__ Granule granule_of(const KvCache& c, int seq, int64_t key) {
-    const int64_t index = min(key >> c.page_log2, (int64_t)c.width - 1);
-    const int page = c.table[(int64_t)seq * c.width + index];
+__device__ __forceinline__ Granule page_of(const KvCache& c, int entry) {
     Granule g;
-    g.there = page >= 0 && page < c.pages;
-    g.page = g.there ? page : 0;
+    g.there = entry >= 0 && entry < c.pages;
+    g.page = g.there ? entry : 0;
     return g;
 }
 
-// Four waves, 16 rows; the waves take the steps of the workgroup's share in turn and join at the end.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) kv_attention_kernel(const KvAttentionParams p) {
-    typedef typename Types<T>::v8 v8;
-    constexpr int CH = D / 64, DT = D / 16;  // 64-element chunks of a key, 16-element tiles of a value
-    const KvCache& c = p.c;
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
-    const int split = (int)blockIdx.x % p.splits, rest = (int)blockIdx.x / p.splits;
-    RowTile t;
-    if (!find_tile(p, 16, rest / c.heads, rest % c.heads, t)) return;
-    const int share = max((t.steps + p.splits - 1) / p.splits, 4);
-    const int begin = min(split * share, t.steps), end = min(begin + share, t.steps);
+// Bytes of 16 codes of v that some row sees: those of keys first .. first + 15 that lie in [key0, key1) or among the sinks, all or none
+// towards the lower end (earlier keys of the same page are numbers), and exactly towards the upper (later slots may hold anything).
+__device__ __forceinline__ v4i seen_codes(v4i codes, const RowTile& t, int sinks, int first, bool there) {
+    const bool any = there && first < t.key1 && (first + 16 > t.key0 || first < sinks);
+    const int live = any ? t.key1 - first : 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const int bytes = min(max(live - 4 * w, 0), 4);
+        codes[w] &= bytes == 4 ? -1 : (1 << (8 * bytes)) - 1;
+    }
+    return codes;
+}
 
-    // this lane's row
-    const int r = t.r0 + col, token = r / p.group, q_head = t.head * p.group + r % p.group;
-    const bool row_live = col < t.rows;
-    const int64_t position = row_live ? t.start + token : -1;
-    v8 q[CH][2];
+__device__ __forceinline__ void select_seen(v4f (&s)[4], int key, int position, int window, int sinks, bool there) {
+    const int first_seen = window ? position - (window - 1) : 0;
 #pragma unroll
-    for (int ch = 0; ch < CH; ++ch)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if (row_live) q[ch][h] = *reinterpret_cast<const v8*>((const T*)p.q + (int64_t)(t.first + token) * p.q_row + (int64_t)q_head * p.q_head + ch * 64 + g * 16 + h * 8);
-            else q[ch][h] = v8{};
+    for (int i = 0; i < 16; ++i) {
+        const int j = key + i;
+        const bool seen = there && j <= position && (j >= first_seen || j < sinks);
+        s[i / 4][i % 4] = seen ? s[i / 4][i % 4] : kMinusInf;
+    }
+}
+
+// v's scale against the unit u that O is held in; lanes hold the scales of their own 16 keys.
+struct Unit {
+    float u = kSmallestUnit, inverse = 0x1p126f;
+    float grown = 1.f;                 // this step: u before / u now
+    float lift, back;                  // this step: log2(v_scale / u), u / v_scale
+    // seen: whether any key of the lane's 16 is seen (the scale of the others may be anything)
+    __device__ __forceinline__ void step(float v_scale, bool seen) {
+        grown = 1.f;
+        float s = seen ? v_scale : 0.f;
+        if (__ballot(s > u)) {
+            float top = fmaxf(s, __shfl_xor(s, 16));
+            top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), u);
+            grown = u / top;
+            u = top, inverse = 1.f / top;
         }
+        s = fmaxf(s * inverse, 0x1p-100f);  // (no keys, or a scale of zero: any finite logarithm will do)
+        lift = __builtin_amdgcn_logf(s), back = __builtin_amdgcn_rcpf(s);
+    }
+};
 
-    const int P = 1 << c.page_log2, in_page = P - 1;
-    const int64_t block_bytes = (int64_t)P * D;
-    v4f o[DT];
+// One row's 16 scores of a step -> its weights, against the running maximum m and in units of u, and its sum l.  Returns what O has to
+// be multiplied by on m's account.  factor > 0.
+template <typename T>
+__device__ __forceinline__ float weigh(v4f (&s)[4], float factor, const Unit& unit, float& m, float& l, typename Types<T>::v8 (&pt)[2]) {
+    v4f w[4];
+    float shrink = 1.f, base = unit.lift - m, sum = 0.f;
 #pragma unroll
-    for (int d = 0; d < DT; ++d) o[d] = v4f{0.f, 0.f, 0.f, 0.f};
-    float m = kMinusInf, l = 0.f, u = kSmallestUnit;
-
-    for (int step = begin + wave; step < end; step += 4) {
-        const int64_t key = t.key_of(step);
-        const int64_t mine = key + 16 * g;  // this lane's 16 keys, as columns of V^T
-        const Granule kg = granule_of(c, t.seq, key + 16 * (col >> 2)), vg = granule_of(c, t.seq, mine);
-        const uint8_t* kp = c.k + ((int64_t)kg.page * c.heads + t.head) * block_bytes + (int64_t)((key + 16 * (col >> 2) + (col & 3)) & in_page) * D + g * 16;
-        const uint8_t* vp = c.v + ((int64_t)vg.page * c.heads + t.head) * block_bytes + col * P + (mine & in_page);
-        v4i kc[4][CH], vc[DT];
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            w[i][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j], factor, base));
+            sum = i + j == 0 ? w[i][j] : sum + w[i][j];
+        }
+    if (__ballot(!(sum <= kLargeSum))) {
+        float top = kMinusInf;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int ch = 0; ch < CH; ++ch) kc[i][ch] = *reinterpret_cast<const v4i*>(kp + i * 4 * D + ch * 64);
-#pragma unroll
-        for (int d = 0; d < DT; ++d) vc[d] = *reinterpret_cast<const v4i*>(vp + d * 16 * P);
-        const int64_t at = (int64_t)vg.page * c.heads + t.head;
-        const float k_scale = c.k_scale[at];
-        float v_scale = c.v_scale[at];
-
-        v4f s[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            s[i] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int ch = 0; ch < CH; ++ch) {
-                s[i] = mfma16(widen<T>(kc[i][ch][0], kc[i][ch][1]), q[ch][0], s[i]);
-                s[i] = mfma16(widen<T>(kc[i][ch][2], kc[i][ch][3]), q[ch][1], s[i]);
-            }
-        }
-        const float factor = k_scale * p.scale_log2;
-        // every key of the step seen by every row: nothing to select
-        const bool whole = key + 63 <= t.low && (!p.window || key > t.high - p.window) && __ballot(!vg.there) == 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[i] *= factor;
-        if (!whole) {
-            const int64_t first_seen = p.window ? position - p.window + 1 : 0;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int64_t j = mine + i;
-                const bool seen = vg.there && j <= position && (j >= first_seen || j < p.sinks);
-                s[i / 4][i % 4] = seen ? s[i / 4][i % 4] : kMinusInf;
-            }
-            // codes that no row sees: behind the last key, before the window, in no page
-            const bool any = vg.there && mine < t.key1 && (mine + 16 > t.key0 || mine < p.sinks);
-            const int live = any ? (int)min(t.key1 - mine, (int64_t)16) : 0;
-            if (!any) v_scale = 0.f;
-            v4i mask;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const int bytes = min(max(live - 4 * w, 0), 4);
-                mask[w] = bytes == 4 ? -1 : (1 << (8 * bytes)) - 1;
-            }
-#pragma unroll
-            for (int d = 0; d < DT; ++d) vc[d] &= mask;
-        }
-        float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
-#pragma unroll
-        for (int i = 1; i < 4; ++i) top = fmaxf(top, fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3])));
+            for (int j = 0; j < 4; ++j) top = fmaxf(top, s[i][j] * factor);
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float m_new = fmaxf(m, top), base = m_new == kMinusInf ? 0.f : m_new;
-        const float shrink = __builtin_amdgcn_exp2f(m - base);
-        float unit = fmaxf(v_scale, __shfl_xor(v_scale, 16));
-        unit = fmaxf(fmaxf(unit, __shfl_xor(unit, 32)), u);
-        const float ratio = v_scale / unit, rescale = shrink * (u / unit);
-        m = m_new, u = unit;
-        float sum = 0.f;
+        top = fmaxf(m, top);
+        const float finite = top == kMinusInf ? 0.f : top;
+        shrink = __builtin_amdgcn_exp2f(m - finite);
+        l *= shrink;
+        m = top;
+        base = unit.lift - finite;
+        sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                s[i][j] = __builtin_amdgcn_exp2f(s[i][j] - base);
-                sum += s[i][j];
-                s[i][j] *= ratio;
+                w[i][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j], factor, base));
+                sum += w[i][j];
             }
-        l = l * shrink + sum;
-        typename Types<T>::v8 pt[2];
+    }
+    l = __builtin_fmaf(sum, unit.back, l);
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-            pt[h] = __builtin_convertvector(__builtin_shufflevector(s[2 * h], s[2 * h + 1], 0, 1, 2, 3, 4, 5, 6, 7), v8);
+    for (int h = 0; h < 2; ++h)
+        pt[h] = __builtin_convertvector(__builtin_shufflevector(w[2 * h], w[2 * h + 1], 0, 1, 2, 3, 4, 5, 6, 7), typename Types<T>::v8);
+    return shrink;
+}
+
+// q's eight elements with the softmax factor's sign, which the scores then need not have
+template <typename T>
+__device__ __forceinline__ typename Types<T>::v8 load_q(const T* at, bool negative) {
+    v4i x = *reinterpret_cast<const v4i*>(at);
+    if (negative) x ^= (int)0x80008000;
+    return __builtin_bit_cast(typename Types<T>::v8, x);
+}
+
+// k's scale and the softmax factor; never zero, so that what is not seen stays at -inf
+__device__ __forceinline__ float score_factor(float k_scale, float scale_log2) { return fmaxf(fabsf(k_scale * scale_log2), 0x1p-126f); }
+
+// Few rows: four waves, 16 NT rows; the waves take the steps of the workgroup's share in turn and join at the end.  Codes come straight
+// from memory into registers, k's of the next step being asked for when this step's are used up, v's likewise.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_kernel(const KvAttentionParams p) {
+    typedef typename Types<T>::v8 v8;
+    constexpr int CH = D / 64, DT = D / 16, ROWS = 16 * NT;  // 64-element chunks of a key, 16-element tiles of a value
+    const KvCache& c = p.c;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, g = lane >> 4;
+    const int split = (int)blockIdx.x % p.splits, rest = (int)blockIdx.x / p.splits;
+    RowTile t;
+    if (!find_tile(p, ROWS, rest / c.heads, rest % c.heads, t)) return;
+    const int share = max((t.steps + p.splits - 1) / p.splits, kLeastSteps);
+    const int begin = min(split * share, t.steps), end = min(begin + share, t.steps);
+
+    const int P = 1 << c.page_log2, in_page = P - 1, head_bytes = P * D;
+    const int64_t page_bytes = (int64_t)c.heads * head_bytes;
+    const uint8_t *k_head = c.k + (int64_t)t.head * head_bytes + g * 16, *v_head = c.v + (int64_t)t.head * head_bytes + col * P;
+    const int* table = c.table + (int64_t)t.seq * c.width;
+    const int k_key = 16 * (col >> 2) + (col & 3);  // this lane's first key of a step as a row of K, and 16 g its first as a column of V^T
+
+    v4i kc[4][CH], vc[DT];
+    int k_entry = 0, v_entry = 0;
+    Granule v_page{0, false}, there{0, false};
+    float k_scale = 0.f, v_scale = 0.f;
+    auto load_pages = [&](int step) {
+        if (step >= end) return;
+        const int key = t.key_of(step);
+        k_entry = table_entry(c, table, key + 16 * (col >> 2)), v_entry = table_entry(c, table, key + 16 * g);
+    };
+    auto load_k = [&](int step) {
+        v_page = page_of(c, v_entry);
+        const uint8_t* at = k_head + page_of(c, k_entry).page * page_bytes + ((t.key_of(step) + k_key) & in_page) * D;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int ch = 0; ch < CH; ++ch) kc[i][ch] = *reinterpret_cast<const v4i*>(at + i * 4 * D + ch * 64);
+        k_scale = c.k_scale[(int64_t)v_page.page * c.heads + t.head];
+    };
+    auto load_v = [&](int step) {
+        there = v_page;
+        const uint8_t* at = v_head + v_page.page * page_bytes + ((t.key_of(step) + 16 * g) & in_page);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) vc[d] = *reinterpret_cast<const v4i*>(at + d * 16 * P);
+        v_scale = c.v_scale[(int64_t)v_page.page * c.heads + t.head];
+    };
+    const int mine = begin + wave;
+    if (mine < end) {
+        load_pages(mine);
+        load_k(mine);
+        load_v(mine);
+        load_pages(mine + 4);
+    }
+
+    // this lane's rows
+    int position[NT];
+    v8 q[NT][CH][2];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int row = n * 16 + col, r = t.r0 + row, token = r / p.group, q_head = t.head * p.group + r % p.group;
+        position[n] = row < t.rows ? t.start + token : -1;
+        m[n] = row < t.rows ? kMinusInf : 0.f, l[n] = 0.f;
+#pragma unroll
+        for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                q[n][ch][h] = v8{};
+                if (row < t.rows) q[n][ch][h] = load_q<T>((const T*)p.q + (int64_t)(t.first + token) * p.q_row + (int64_t)q_head * p.q_head + ch * 64 + g * 16 + h * 8, p.scale_log2 < 0.f);
+            }
+    }
+    v4f o[NT][DT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[n][d] = v4f{0.f, 0.f, 0.f, 0.f};
+    Unit unit;
+
+    for (int step = mine; step < end; step += 4) {
+        const int key = t.key_of(step), first = key + 16 * g;
+        v4f s[NT][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) s[n][i] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ch = 0; ch < CH; ++ch) {
+                const v8 a = widen<T>(kc[i][ch][0], kc[i][ch][1]), b = widen<T>(kc[i][ch][2], kc[i][ch][3]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    s[n][i] = mfma16(a, q[n][ch][0], s[n][i]);
+                    s[n][i] = mfma16(b, q[n][ch][1], s[n][i]);
+                }
+            }
+        }
+        const float factor = score_factor(k_scale, p.scale_log2);
+        if (step + 4 < end) load_k(step + 4);
+        // every key of the step seen by every row: nothing to select
+        const bool whole = key + 63 <= t.low && (!p.window || key > t.high - p.window) && __ballot(!there.there) == 0;
+        unit.step(v_scale, whole || (there.there && first < t.key1 && (first + 16 > t.key0 || first < p.sinks)));
+        if (!whole) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) select_seen(s[n], first, position[n], p.window, p.sinks, there.there);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) vc[d] = seen_codes(vc[d], t, p.sinks, first, there.there);
+        }
+        v8 pt[NT][2];
+        float rescale[NT];
+        bool any = unit.grown != 1.f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            rescale[n] = weigh<T>(s[n], factor, unit, m[n], l[n], pt[n]) * unit.grown;
+            any = any || rescale[n] != 1.f;
+        }
+        if (__ballot(any)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[n][d] *= rescale[n];
+        }
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-            o[d] *= rescale;
-            o[d] = mfma16(widen<T>(vc[d][0], vc[d][1]), pt[0], o[d]);
-            o[d] = mfma16(widen<T>(vc[d][2], vc[d][3]), pt[1], o[d]);
+            const v8 a = widen<T>(vc[d][0], vc[d][1]), b = widen<T>(vc[d][2], vc[d][3]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                o[n][d] = mfma16(a, pt[n][0], o[n][d]);
+                o[n][d] = mfma16(b, pt[n][1], o[n][d]);
+            }
+        }
+        if (step + 4 < end) {
+            load_v(step + 4);
+            load_pages(step + 8);
         }
     }
 
     // the four waves' results: m, l and u, then O, each in units of the largest
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-    __shared__ float part_m[4][16], part_l[4][16], part_u[4];
+    __shared__ float part_m[4][ROWS], part_l[4][ROWS], part_u[4];
     __shared__ float part_o[4][16][D + 4];
-    if (lane < 16) part_m[wave][col] = m, part_l[wave][col] = l;
-    if (lane == 0) part_u[wave] = u;
-    __syncthreads();
-    float top = part_m[0][col], unit = part_u[0];
+    if (lane == 0) part_u[wave] = unit.u;
 #pragma unroll
-    for (int w = 1; w < 4; ++w) top = fmaxf(top, part_m[w][col]), unit = fmaxf(unit, part_u[w]);
-    const float base = top == kMinusInf ? 0.f : top, mine = __builtin_amdgcn_exp2f(m - base) * (u / unit);
+    for (int n = 0; n < NT; ++n) {
+        l[n] += __shfl_xor(l[n], 16);
+        l[n] += __shfl_xor(l[n], 32);
+        if (lane < 16) part_m[wave][n * 16 + col] = m[n], part_l[wave][n * 16 + col] = l[n];
+    }
 #pragma unroll
-    for (int d = 0; d < DT; ++d) *reinterpret_cast<v4f*>(&part_o[wave][col][d * 16 + 4 * g]) = o[d] * mine;
-    __syncthreads();
-    constexpr int QUADS = D / 4;
-    for (int i = tid; i < t.rows * QUADS; i += 256) {
-        const int row = i / QUADS, e = 4 * (i % QUADS), rr = t.r0 + row;
-        float row_top = part_m[0][row];
+    for (int n = 0; n < NT; ++n) {
+        __syncthreads();
+        float top = part_m[0][n * 16 + col], u = part_u[0];
 #pragma unroll
-        for (int w = 1; w < 4; ++w) row_top = fmaxf(row_top, part_m[w][row]);
-        const float row_base = row_top == kMinusInf ? 0.f : row_top;
-        float sum = 0.f;
-        v4f x = {0.f, 0.f, 0.f, 0.f};
+        for (int w = 1; w < 4; ++w) top = fmaxf(top, part_m[w][n * 16 + col]), u = fmaxf(u, part_u[w]);
+        const float base = top == kMinusInf ? 0.f : top, f = __builtin_amdgcn_exp2f(m[n] - base) * (unit.u / u);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            sum += part_l[w][row] * __builtin_amdgcn_exp2f(part_m[w][row] - row_base);
-            x += *reinterpret_cast<const v4f*>(&part_o[w][row][e]);
-        }
-        x *= unit;
-        const int64_t out_row = (int64_t)(t.first + rr / p.group) * p.q_heads + t.head * p.group + rr % p.group;
-        if (p.splits > 1) {
-            const int64_t at = (int64_t)split * c.rows * p.q_heads + out_row;
-            if (e == 0) p.part_ml[2 * at] = row_top, p.part_ml[2 * at + 1] = sum;
-            if (sum > 0.f) *reinterpret_cast<v4f*>(p.part_o + at * D + e) = x;
-        } else {
-            typedef T v4t __attribute__((ext_vector_type(4)));
-            x *= sum > 0.f ? 1.0f / sum : 0.f;  // a row that sees nothing is zero
-            *reinterpret_cast<v4t*>((T*)p.out + out_row * D + e) = __builtin_convertvector(x, v4t);
+        for (int d = 0; d < DT; ++d) *reinterpret_cast<v4f*>(&part_o[wave][col][d * 16 + 4 * g]) = o[n][d] * f;
+        __syncthreads();
+        constexpr int QUADS = D / 4;
+        const int rows = min(t.rows - n * 16, 16);
+        for (int i = tid; i < rows * QUADS; i += 256) {
+            const int row = i / QUADS, e = 4 * (i % QUADS), rr = t.r0 + n * 16 + row;
+            float row_top = part_m[0][n * 16 + row];
+#pragma unroll
+            for (int w = 1; w < 4; ++w) row_top = fmaxf(row_top, part_m[w][n * 16 + row]);
+            const float row_base = row_top == kMinusInf ? 0.f : row_top;
+            float sum = 0.f;
+            v4f x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                sum += part_l[w][n * 16 + row] * __builtin_amdgcn_exp2f(part_m[w][n * 16 + row] - row_base);
+                x += *reinterpret_cast<const v4f*>(&part_o[w][row][e]);
+            }
+            x *= u;
+            const int64_t out_row = (int64_t)(t.first + rr / p.group) * p.q_heads + t.head * p.group + rr % p.group;
+            if (p.splits > 1) {
+                const int64_t at = (int64_t)split * c.rows * p.q_heads + out_row;
+                if (e == 0) p.part_ml[2 * at] = row_top, p.part_ml[2 * at + 1] = sum;
+                if (sum > 0.f) *reinterpret_cast<v4f*>(p.part_o + at * D + e) = x;
+            } else {
+                typedef T v4t __attribute__((ext_vector_type(4)));
+                x *= sum > 0.f ? 1.0f / sum : 0.f;  // a row that sees nothing is zero
+                *reinterpret_cast<v4t*>((T*)p.out + out_row * D + e) = __builtin_convertvector(x, v4t);
+            }
         }
     }
 }
@@ -279,83 +406,85 @@ template <typename T, int D>
 __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_rows_kernel(const KvAttentionParams p, int items) {
     typedef typename Types<T>::v8 v8;
     constexpr int CH = D / 64, DT = D / 16, LOADS = D / 64, KCH = D / 16;
+    constexpr bool EARLY = D < 256;  // (registers)
     __shared__ __align__(16) uint8_t lds_k[2][64 * D], lds_v[2][64 * D];
     const KvCache& c = p.c;
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, g = lane >> 4;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, g = lane >> 4;
     const int head = (int)blockIdx.x % c.heads, rest = (int)blockIdx.x / c.heads, split = rest % p.splits;
     RowTile t;
     if (!find_tile(p, 128, items - 1 - rest / p.splits, head, t)) return;  // (the last rows of a sequence, which see most, first)
-    const int share = max((t.steps + p.splits - 1) / p.splits, 4);
+    const int share = max((t.steps + p.splits - 1) / p.splits, kLeastSteps);
     const int begin = min(split * share, t.steps), end = min(begin + share, t.steps);
 
     // this lane's two rows
-    int64_t position[2];
+    int position[2];
     v8 q[2][CH][2];
+    float m[2], l[2];
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
         const int row = wave * 32 + n * 16 + col, r = t.r0 + row, token = r / p.group, q_head = head * p.group + r % p.group;
         position[n] = row < t.rows ? t.start + token : -1;
+        m[n] = row < t.rows ? kMinusInf : 0.f, l[n] = 0.f;
 #pragma unroll
         for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                if (row < t.rows) q[n][ch][h] = *reinterpret_cast<const v8*>((const T*)p.q + (int64_t)(t.first + token) * p.q_row + (int64_t)q_head * p.q_head + ch * 64 + g * 16 + h * 8);
-                else q[n][ch][h] = v8{};
+                q[n][ch][h] = v8{};
+                if (row < t.rows) q[n][ch][h] = load_q<T>((const T*)p.q + (int64_t)(t.first + token) * p.q_row + (int64_t)q_head * p.q_head + ch * 64 + g * 16 + h * 8, p.scale_log2 < 0.f);
             }
     }
     const int wave_rows = min(t.rows - wave * 32, 32);
-    const int64_t wave_low = t.start + (t.r0 + wave * 32) / p.group, wave_high = t.start + (t.r0 + wave * 32 + wave_rows - 1) / p.group;
+    const int wave_low = t.start + (t.r0 + wave * 32) / p.group, wave_high = t.start + (t.r0 + wave * 32 + wave_rows - 1) / p.group;
 
-    const int P = 1 << c.page_log2, in_page = P - 1;
-    const int64_t block_bytes = (int64_t)P * D;
+    const int P = 1 << c.page_log2, in_page = P - 1, head_bytes = P * D;
+    const int64_t page_bytes = (int64_t)c.heads * head_bytes;
+    const uint8_t *k_head = c.k + (int64_t)head * head_bytes, *v_head = c.v + (int64_t)head * head_bytes;
+    const int* table = c.table + (int64_t)t.seq * c.width;
     v4f o[2][DT];
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[n][d] = v4f{0.f, 0.f, 0.f, 0.f};
-    float m[2] = {kMinusInf, kMinusInf}, l[2] = {0.f, 0.f}, u = kSmallestUnit;
+    Unit unit;
 
-    // a step's pages, one per group of 16 lanes, then its codes and scales on their way to LDS
+    // a step's pages, one per group of 16 lanes, then its codes and scales on their way to LDS.  A thread's loads: rows and chunks
+    // of its own, the same in every step
+    int k_row[LOADS], k_chunk[LOADS], v_row[LOADS], v_chunk;
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+        const int ci = tid + 256 * j;
+        k_row[j] = ci / KCH, k_chunk[j] = ((ci % KCH) ^ k_swizzle<D>(k_row[j])) * 16;
+        v_row[j] = (ci / 4) * P;
+    }
+    v_chunk = (tid & 3) ^ v_swizzle(tid / 4);  // (256 threads on, the row is 64 further: the same swizzle)
     v4i k_reg[LOADS], v_reg[LOADS];
-    float k_scale, v_scale;
-    Granule page{0, false}, there{0, false};
-    auto load_page = [&](int step) { if (step < end) page = granule_of(c, t.seq, t.key_of(step) + 16 * g); };
+    float k_scale = 0.f, v_scale = 0.f;
+    int entry = 0;
+    Granule there{0, false};
+    auto load_page = [&](int step) { if (step < end) entry = table_entry(c, table, t.key_of(step) + 16 * g); };
     auto load_codes = [&](int step) {
-        there = page;
-        const int64_t key = t.key_of(step), at = (int64_t)page.page * c.heads + head;
+        const Granule page = there = page_of(c, entry);
+        const int key = t.key_of(step);
+        const int64_t at = (int64_t)page.page * c.heads + head;
         k_scale = c.k_scale[at], v_scale = c.v_scale[at];
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j) {
-            const int ci = tid + 256 * j, row = ci / KCH, chunk = (ci % KCH) ^ k_swizzle<D>(row);
-            const int64_t block = (int64_t)__shfl(page.page, (row >> 4) * 16) * c.heads + head;
-            k_reg[j] = *reinterpret_cast<const v4i*>(c.k + block * block_bytes + (int64_t)((key + row) & in_page) * D + chunk * 16);
-        }
+        for (int j = 0; j < LOADS; ++j)
+            k_reg[j] = *reinterpret_cast<const v4i*>(k_head + __shfl(page.page, k_row[j] & 48) * page_bytes + (((key + k_row[j]) & in_page) * D + k_chunk[j]));
+        const uint8_t* v_at = v_head + __shfl(page.page, v_chunk * 16) * page_bytes + ((key + 16 * v_chunk) & in_page);
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j) {
-            const int ci = tid + 256 * j, row = ci / 4, chunk = (ci & 3) ^ v_swizzle(row);
-            const int64_t block = (int64_t)__shfl(page.page, chunk * 16) * c.heads + head;
-            v_reg[j] = *reinterpret_cast<const v4i*>(c.v + block * block_bytes + (int64_t)row * P + ((key + 16 * chunk) & in_page));
-        }
+        for (int j = 0; j < LOADS; ++j) v_reg[j] = *reinterpret_cast<const v4i*>(v_at + v_row[j]);
     };
     auto store_codes = [&](int step, int buffer) {
-        const int64_t key = t.key_of(step);
-        const bool whole = key + 64 <= t.key1 && key >= t.key0 && __ballot(!there.there) == 0;
+        const int key = t.key_of(step);
+        if (key + 64 > t.key1 || key < t.key0 || __ballot(!there.there)) {
+            const bool chunk_there = __shfl((int)there.there, v_chunk * 16) != 0;
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j) *reinterpret_cast<v4i*>(&lds_k[buffer][(tid + 256 * j) * 16]) = k_reg[j];
+            for (int j = 0; j < LOADS; ++j) v_reg[j] = seen_codes(v_reg[j], t, p.sinks, key + 16 * v_chunk, chunk_there);
+        }
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) {
-            const int ci = tid + 256 * j, chunk = (ci & 3) ^ v_swizzle(ci / 4);
-            if (!whole) {  // codes that no row sees: behind the last key, before the window, in no page
-                const int64_t first = key + 16 * chunk;
-                const bool any = __shfl((int)there.there, chunk * 16) && first < t.key1 && (first + 16 > t.key0 || first < p.sinks);
-                const int live = any ? (int)min(t.key1 - first, (int64_t)16) : 0;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const int bytes = min(max(live - 4 * w, 0), 4);
-                    v_reg[j][w] &= bytes == 4 ? -1 : (1 << (8 * bytes)) - 1;
-                }
-            }
-            *reinterpret_cast<v4i*>(&lds_v[buffer][ci * 16]) = v_reg[j];
+            *reinterpret_cast<v4i*>(&lds_k[buffer][(tid + 256 * j) * 16]) = k_reg[j];
+            *reinterpret_cast<v4i*>(&lds_v[buffer][(tid + 256 * j) * 16]) = v_reg[j];
         }
     };
 
@@ -368,24 +497,31 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_rows_kerne
     __syncthreads();
     for (int step = begin; step < end; ++step) {
         const int buffer = (step - begin) & 1;
-        const int64_t key = t.key_of(step), mine = key + 16 * g;
-        const float factor = k_scale * p.scale_log2;
-        float v_unit = v_scale;
+        const int key = t.key_of(step), first = key + 16 * g;
+        const float factor = score_factor(k_scale, p.scale_log2), this_v_scale = v_scale;
         const bool page_there = there.there;
         if (step + 1 < end) {
             load_codes(step + 1);
             load_page(step + 2);
         }
         if (wave_rows > 0 && key <= wave_high) {
+            // fragments of k, and then of v in front of the softmax, are all asked for before the first is used
             v4f s[2][4];
+            v4i kc[4][CH], vc[DT];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int ch = 0; ch < CH; ++ch) {
+                    const int row = 16 * (col >> 2) + 4 * i + (col & 3);
+                    kc[i][ch] = *reinterpret_cast<const v4i*>(&lds_k[buffer][row * D + ((ch * 4 + g) ^ k_swizzle<D>(row)) * 16]);
+                }
+            if constexpr (EARLY) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 s[0][i] = s[1][i] = v4f{0.f, 0.f, 0.f, 0.f};
-                const int row = 16 * (col >> 2) + 4 * i + (col & 3);
 #pragma unroll
                 for (int ch = 0; ch < CH; ++ch) {
-                    const v4i kc = *reinterpret_cast<const v4i*>(&lds_k[buffer][row * D + ((ch * 4 + g) ^ k_swizzle<D>(row)) * 16]);
-                    const v8 a = widen<T>(kc[0], kc[1]), b = widen<T>(kc[2], kc[3]);
+                    const v8 a = widen<T>(kc[i][ch][0], kc[i][ch][1]), b = widen<T>(kc[i][ch][2], kc[i][ch][3]);
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
                         s[n][i] = mfma16(a, q[n][ch][0], s[n][i]);
@@ -393,54 +529,25 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_rows_kerne
                     }
                 }
             }
-            const bool whole = key + 63 <= wave_low && (!p.window || key > wave_high - p.window) && __ballot(!page_there) == 0;
-            if (!whole && !(page_there && mine < t.key1 && (mine + 16 > t.key0 || mine < p.sinks))) v_unit = 0.f;
-            float unit = fmaxf(v_unit, __shfl_xor(v_unit, 16));
-            unit = fmaxf(fmaxf(unit, __shfl_xor(unit, 32)), u);
-            const float ratio = v_unit / unit;
-            float rescale[2];
-            v8 pt[2][2];
+            auto read_v = [&](int d) {
+                const int row = d * 16 + col;
+                vc[d] = *reinterpret_cast<const v4i*>(&lds_v[buffer][row * 64 + (g ^ v_swizzle(row)) * 16]);
+            };
+            if constexpr (EARLY) {
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[n][i] *= factor;
-                if (!whole) {
-                    const int64_t first_seen = p.window ? position[n] - p.window + 1 : 0;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int64_t j = mine + i;
-                        const bool seen = page_there && j <= position[n] && (j >= first_seen || j < p.sinks);
-                        s[n][i / 4][i % 4] = seen ? s[n][i / 4][i % 4] : kMinusInf;
-                    }
-                }
-                float top = fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3]));
-#pragma unroll
-                for (int i = 1; i < 4; ++i) top = fmaxf(top, fmaxf(fmaxf(s[n][i][0], s[n][i][1]), fmaxf(s[n][i][2], s[n][i][3])));
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                const float m_new = top > m[n] + kSlack ? top : m[n], base = m_new == kMinusInf ? 0.f : m_new;
-                const float shrink = __builtin_amdgcn_exp2f(m[n] - base);
-                rescale[n] = m_new == m[n] ? u / unit : shrink * (u / unit);
-                l[n] = m_new == m[n] ? l[n] : l[n] * shrink;
-                m[n] = m_new;
-                float sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        s[n][i][j] = __builtin_amdgcn_exp2f(s[n][i][j] - base);
-                        sum += s[n][i][j];
-                    }
-                l[n] += sum;
-                if (__ballot(ratio != 1.f)) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[n][i] *= ratio;
-                }
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    pt[n][h] = __builtin_convertvector(__builtin_shufflevector(s[n][2 * h], s[n][2 * h + 1], 0, 1, 2, 3, 4, 5, 6, 7), v8);
+                for (int d = 0; d < DT; ++d) read_v(d);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            u = unit;
+            const bool whole = key + 63 <= wave_low && (!p.window || key > wave_high - p.window) && __ballot(!page_there) == 0;
+            unit.step(this_v_scale, whole || (page_there && first < t.key1 && (first + 16 > t.key0 || first < p.sinks)));
+            if (!whole) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n) select_seen(s[n], first, position[n], p.window, p.sinks, page_there);
+            }
+            v8 pt[2][2];
+            float rescale[2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) rescale[n] = weigh<T>(s[n], factor, unit, m[n], l[n], pt[n]) * unit.grown;
             if (__ballot(rescale[0] != 1.f || rescale[1] != 1.f)) {
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
@@ -449,9 +556,8 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_rows_kerne
             }
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const int row = d * 16 + col;
-                const v4i vc = *reinterpret_cast<const v4i*>(&lds_v[buffer][row * 64 + (g ^ v_swizzle(row)) * 16]);
-                const v8 a = widen<T>(vc[0], vc[1]), b = widen<T>(vc[2], vc[3]);
+                if constexpr (!EARLY) read_v(d);
+                const v8 a = widen<T>(vc[d][0], vc[d][1]), b = widen<T>(vc[d][2], vc[d][3]);
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
                     o[n][d] = mfma16(a, pt[n][0], o[n][d]);
@@ -475,71 +581,100 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_rows_kerne
             if (g == 0) p.part_ml[2 * at] = m[n], p.part_ml[2 * at + 1] = sum;
             if (sum > 0.f) {
 #pragma unroll
-                for (int d = 0; d < DT; ++d) *reinterpret_cast<v4f*>(p.part_o + at * D + d * 16 + 4 * g) = o[n][d] * u;
+                for (int d = 0; d < DT; ++d) *reinterpret_cast<v4f*>(p.part_o + at * D + d * 16 + 4 * g) = o[n][d] * unit.u;
             }
         } else {
             typedef T v4t __attribute__((ext_vector_type(4)));
-            const float f = sum > 0.f ? u / sum : 0.f;  // a row that sees nothing is zero
+            const float f = sum > 0.f ? unit.u / sum : 0.f;  // a row that sees nothing is zero
 #pragma unroll
             for (int d = 0; d < DT; ++d) *reinterpret_cast<v4t*>((T*)p.out + out_row * D + d * 16 + 4 * g) = __builtin_convertvector(o[n][d] * f, v4t);
         }
     }
 }
 
-// out = sum over splits of exp2(m_s - m) O_s, over the sum of exp2(m_s - m) l_s: D / 4 lanes per row of q, in the order of the splits.
+// out = sum over splits of exp2(m_s - m) O_s, over the sum of exp2(m_s - m) l_s, in the order of the splits: D / 4 lanes per row of q.  The factors first,
+// all splits' m and l asked for at once; then O, four splits in flight.  Parts with no weight were not written.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv_attention_join_kernel(const KvAttentionParams p) {
-    constexpr int QUADS = D / 4;
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)p.c.rows * p.q_heads, row = at / QUADS;
-    if (row >= rows) return;
+    constexpr int QUADS = D / 4, ROWS = 256 / QUADS;
+    __shared__ float weight[ROWS][kMostSplits];
+    const int tid = (int)threadIdx.x, lane = tid % QUADS;
+    const int64_t rows = (int64_t)p.c.rows * p.q_heads, row = (int64_t)blockIdx.x * ROWS + tid / QUADS;
+    const int token = (int)(min(row, rows - 1) / p.q_heads);
     // rows of no sequence are left as they were
-    const int token = (int)(row / p.q_heads), e = 4 * (int)(at % QUADS);
-    if (token < clamp_row(p.c.indptr[0], p.c.rows) || token >= clamp_row(p.c.indptr[p.c.batch], p.c.rows)) return;
-    float top = kMinusInf;
-    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.part_ml[2 * (s * rows + row)]);
+    const bool live = row < rows && token >= clamp_row(p.c.indptr[0], p.c.rows) && token < clamp_row(p.c.indptr[p.c.batch], p.c.rows);
+    constexpr int EACH = kMostSplits / QUADS > 0 ? kMostSplits / QUADS : 1;
+    float m[EACH], l[EACH], top = kMinusInf, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const int s = lane + i * QUADS;
+        m[i] = kMinusInf, l[i] = 0.f;
+        if (live && s < p.splits) m[i] = p.part_ml[2 * (s * rows + row)], l[i] = p.part_ml[2 * (s * rows + row) + 1];
+        top = fmaxf(top, m[i]);
+    }
+#pragma unroll
+    for (int d = 1; d < QUADS; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
     const float base = top == kMinusInf ? 0.f : top;
-    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const float f = l[i] > 0.f ? __builtin_amdgcn_exp2f(m[i] - base) : 0.f;
+        if (lane + i * QUADS < kMostSplits) weight[tid / QUADS][lane + i * QUADS] = f;
+        sum += f * l[i];
+    }
+#pragma unroll
+    for (int d = 1; d < QUADS; d <<= 1) sum += __shfl_xor(sum, d);
+    __syncthreads();
+    if (!live) return;
     v4f x = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < p.splits; ++s) {
-        const float l = p.part_ml[2 * (s * rows + row) + 1];
-        if (l > 0.f) {
-            const float f = __builtin_amdgcn_exp2f(p.part_ml[2 * (s * rows + row)] - base);
-            sum += f * l;
-            x += f * *reinterpret_cast<const v4f*>(p.part_o + (s * rows + row) * D + e);
+    for (int s0 = 0; s0 < p.splits; s0 += 4) {
+        v4f part[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            part[i] = v4f{0.f, 0.f, 0.f, 0.f};
+            if (s0 + i < p.splits && weight[tid / QUADS][s0 + i] > 0.f) part[i] = *reinterpret_cast<const v4f*>(p.part_o + ((s0 + i) * rows + row) * D + 4 * lane);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x += (s0 + i < p.splits ? weight[tid / QUADS][s0 + i] : 0.f) * part[i];
     }
     typedef T v4t __attribute__((ext_vector_type(4)));
     x *= sum > 0.f ? 1.0f / sum : 0.f;
-    *reinterpret_cast<v4t*>((T*)p.out + row * D + e) = __builtin_convertvector(x, v4t);
+    *reinterpret_cast<v4t*>((T*)p.out + row * D + 4 * lane) = __builtin_convertvector(x, v4t);
 }
 
 // Tiles that can begin: sum over sequences of ceil(n * group / tile_rows), see find_sequence.
 int64_t row_tiles(const KvAttentionParams& p, int64_t tile_rows) { return (int64_t)p.c.rows * p.group / tile_rows + p.c.batch; }
-// The form for many rows: by the rows that a sequence's key/value head has on average, as the host does not read the tensors.
-bool many_rows(const KvAttentionParams& p) { return (int64_t)p.c.rows * p.group > 32 * (int64_t)p.c.batch; }
+// Rows of a tile, by the rows that a sequence's key/value head has on average, as the host does not read the tensors: 16 or 32 in the form
+// for few rows, 128 in the one for many.
+int tile_rows_of(const KvAttentionParams& p) {
+    const int64_t rows = (int64_t)p.c.rows * p.group, batch = p.c.batch;
+    return rows <= 16 * batch || (p.c.dim == 256 && rows <= 32 * batch) ? 16 : rows <= 32 * batch ? 32 : 128;
+}
 
 template <typename T, int D>
 hipError_t launch(const KvAttentionParams& p, hipStream_t s) {
-    const int64_t tile_rows = many_rows(p) ? 128 : 16, tiles = row_tiles(p, tile_rows), blocks = tiles * p.c.heads * p.splits;
+    const int tile_rows = tile_rows_of(p);
+    const int64_t tiles = row_tiles(p, tile_rows), blocks = tiles * p.c.heads * p.splits;
     const int64_t join = ((int64_t)p.c.rows * p.q_heads * (D / 4) + 255) / 256;
     if (blocks > INT32_MAX || join > INT32_MAX) return hipErrorInvalidValue;
-    if (many_rows(p)) hipLaunchKernelGGL((kv_attention_rows_kernel<T, D>), dim3((unsigned)blocks), dim3(256), 0, s, p, (int)tiles);
-    else hipLaunchKernelGGL((kv_attention_kernel<T, D>), dim3((unsigned)blocks), dim3(256), 0, s, p);
+    const dim3 grid((unsigned)blocks), block(256);
+    if (tile_rows == 128) hipLaunchKernelGGL((kv_attention_rows_kernel<T, D>), grid, block, 0, s, p, (int)tiles);
+    else if (tile_rows == 16) hipLaunchKernelGGL((kv_attention_kernel<T, D, 1>), grid, block, 0, s, p);
+    else if constexpr (D != 256) hipLaunchKernelGGL((kv_attention_kernel<T, D, 2>), grid, block, 0, s, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
-    hipLaunchKernelGGL((kv_attention_join_kernel<T, D>), dim3((unsigned)join), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((kv_attention_join_kernel<T, D>), dim3((unsigned)join), block, 0, s, p);
     return hipGetLastError();
 }
 
 }  // namespace
 
 int kv_attention_splits(const KvAttentionParams& p) {
-    const int64_t units = row_tiles(p, many_rows(p) ? 128 : 16) * p.c.heads;
+    const int64_t units = row_tiles(p, tile_rows_of(p)) * p.c.heads;
     int64_t keys = (int64_t)p.c.width << p.c.page_log2;
     if (p.window) keys = std::min<int64_t>(keys, (int64_t)p.window + 128 + (p.sinks + 63) / 64 * 64);
     const int64_t steps = (keys + 63) / 64;
-    const int64_t wanted = (512 + units - 1) / units, most = (steps + 3) / 4;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(wanted, most), 64));
+    const int64_t wanted = (TG_WANT + units - 1) / units, most = (steps + kLeastSteps - 1) / kLeastSteps;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(wanted, most), kMostSplits));
 }
 
 hipError_t run_kv_attention(const KvAttentionParams& p, bool is_bf16, hipStream_t s) {

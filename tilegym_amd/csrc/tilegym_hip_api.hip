@@ -2064,6 +2064,7 @@ static int32_t check_kv_cache(const tg_tensor* k_cache, const tg_tensor* v_cache
     if (with_lens && seq_lens->shape[0] != B) return fail(TG_ERR_INVALID, "seq_lens must have %lld elements", (long long)B);
     if (pages < 1 || pages > INT32_MAX || heads < 1 || heads > 65536) return fail(TG_ERR_INVALID, "the cache needs between 1 and 2^31 - 1 pages and 1 to 65536 heads");
     if (B > (1 << 24) || W > (1 << 24) || (B > 0 && W < 1)) return fail(TG_ERR_INVALID, "block_table must have 1 to 2^24 columns and at most 2^24 rows");
+    if ((W * P) > (1 << 30)) return fail(TG_ERR_INVALID, "block_table must cover at most 2^30 positions");
     if (rows > (1 << 28)) return fail(TG_ERR_INVALID, "too many tokens");
     if (!aligned16(k_cache->ptr) || !aligned16(v_cache->ptr)) return fail(TG_ERR_INVALID, "k_cache and v_cache must be 16-byte aligned");
     c = tg::KvCache{};
