@@ -78,13 +78,13 @@ struct RowTile {
 
 __device__ __forceinline__ bool find_tile(const KvAttentionParams& p, int tile_rows, int item, int head, RowTile& t) {
     const KvCache& c = p.c;
-    const SeqItem f = find_sequence(c.indptr, c.batch, c.rows, item, p.group, tile_rows, 1);
+    const SeqItem f = find_sequence(c, item, p.group, tile_rows, 1);
     if (f.seq < 0) return false;
     const int64_t r0 = (int64_t)f.item * tile_rows, total = (int64_t)f.n * p.group;
     if (r0 >= total) return false;
     t.seq = f.seq, t.head = head, t.first = f.first;
     t.r0 = (int)r0, t.rows = (int)min((int64_t)tile_rows, total - r0);
-    t.start = max(c.lens[f.seq], 0) - f.n;
+    t.start = f.len - f.n;
     t.low = t.start + t.r0 / p.group, t.high = t.start + (t.r0 + t.rows - 1) / p.group;
     const int capacity = c.width << c.page_log2;
     t.key1 = t.high < 0 ? 0 : t.high < capacity ? t.high + 1 : capacity;
@@ -208,7 +208,8 @@ __device__ __forceinline__ float score_factor(float k_scale, float scale_log2) {
 
 // Few rows: four waves, 16 NT rows; the waves take the steps of the workgroup's share in turn and join at the end.  Codes come straight
 // from memory into registers, k's of the next step being asked for when this step's are used up, v's likewise.
-template <typename T, int D, int NT>
+// ONE: pages hold whole steps (64 or 128 tokens), so a step's page, its scales and its address are scalars.
+template <typename T, int D, int NT, bool ONE>
 __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_kernel(const KvAttentionParams p) {
     typedef typename Types<T>::v8 v8;
     constexpr int CH = D / 64, DT = D / 16, ROWS = 16 * NT;  // 64-element chunks of a key, 16-element tiles of a value
@@ -221,8 +222,6 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_kernel(con
     const int begin = min(split * share, t.steps), end = min(begin + share, t.steps);
 
     const int P = 1 << c.page_log2, in_page = P - 1, head_bytes = P * D;
-    const int64_t page_bytes = (int64_t)c.heads * head_bytes;
-    const uint8_t *k_head = c.k + (int64_t)t.head * head_bytes + g * 16, *v_head = c.v + (int64_t)t.head * head_bytes + col * P;
     const int* table = c.table + (int64_t)t.seq * c.width;
     const int k_key = 16 * (col >> 2) + (col & 3);  // this lane's first key of a step as a row of K, and 16 g its first as a column of V^T
 
@@ -233,31 +232,51 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_kernel(con
     auto load_pages = [&](int step) {
         if (step >= end) return;
         const int key = t.key_of(step);
-        k_entry = table_entry(c, table, key + 16 * (col >> 2)), v_entry = table_entry(c, table, key + 16 * g);
+        if constexpr (ONE) {
+            v_entry = uniform_load(table + min(key >> c.page_log2, c.width - 1));
+        } else {
+            k_entry = table_entry(c, table, key + 16 * (col >> 2)), v_entry = table_entry(c, table, key + 16 * g);
+        }
     };
+    const int k_lane = k_key * D + g * 16, v_lane = col * P + 16 * g;
     auto load_k = [&](int step) {
         v_page = page_of(c, v_entry);
-        const uint8_t* at = k_head + page_of(c, k_entry).page * page_bytes + ((t.key_of(step) + k_key) & in_page) * D;
+        const int key = t.key_of(step);
+        const int64_t at = (int64_t)v_page.page * c.heads + t.head;
+        if constexpr (ONE) {
+            const uint8_t* base = c.k + at * head_bytes + (key & in_page) * D;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int ch = 0; ch < CH; ++ch) kc[i][ch] = *reinterpret_cast<const v4i*>(at + i * 4 * D + ch * 64);
-        k_scale = c.k_scale[(int64_t)v_page.page * c.heads + t.head];
+                for (int ch = 0; ch < CH; ++ch) kc[i][ch] = *reinterpret_cast<const v4i*>(base + (uint32_t)k_lane + (i * 4 * D + ch * 64));
+            k_scale = uniform_load(c.k_scale + at);
+        } else {
+            const uint8_t* base = c.k + ((int64_t)page_of(c, k_entry).page * c.heads + t.head) * head_bytes + ((key + k_key) & in_page) * D + g * 16;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int ch = 0; ch < CH; ++ch) kc[i][ch] = *reinterpret_cast<const v4i*>(base + i * 4 * D + ch * 64);
+            k_scale = c.k_scale[at];
+        }
     };
     auto load_v = [&](int step) {
         there = v_page;
-        const uint8_t* at = v_head + v_page.page * page_bytes + ((t.key_of(step) + 16 * g) & in_page);
+        const int key = t.key_of(step);
+        const int64_t at = (int64_t)v_page.page * c.heads + t.head;
+        if constexpr (ONE) {
+            const uint8_t* base = c.v + at * head_bytes + (key & in_page);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) vc[d] = *reinterpret_cast<const v4i*>(at + d * 16 * P);
-        v_scale = c.v_scale[(int64_t)v_page.page * c.heads + t.head];
+            for (int d = 0; d < DT; ++d) vc[d] = *reinterpret_cast<const v4i*>(base + d * 16 * P + (uint32_t)v_lane);
+            v_scale = uniform_load(c.v_scale + at);
+        } else {
+            const uint8_t* base = c.v + at * head_bytes + col * P + ((key + 16 * g) & in_page);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) vc[d] = *reinterpret_cast<const v4i*>(base + d * 16 * P);
+            v_scale = c.v_scale[at];
+        }
     };
     const int mine = begin + wave;
-    if (mine < end) {
-        load_pages(mine);
-        load_k(mine);
-        load_v(mine);
-        load_pages(mine + 4);
-    }
+    load_pages(mine);
 
     // this lane's rows
     int position[NT];
@@ -275,6 +294,11 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_kernel(con
                 q[n][ch][h] = v8{};
                 if (row < t.rows) q[n][ch][h] = load_q<T>((const T*)p.q + (int64_t)(t.first + token) * p.q_row + (int64_t)q_head * p.q_head + ch * 64 + g * 16 + h * 8, p.scale_log2 < 0.f);
             }
+    }
+    if (mine < end) {
+        load_k(mine);
+        load_v(mine);
+        load_pages(mine + 4);
     }
     v4f o[NT][DT];
 #pragma unroll
@@ -402,7 +426,7 @@ __device__ __forceinline__ int k_swizzle(int row) {
 }
 __device__ __forceinline__ int v_swizzle(int row) { return (row >> 2) & 3; }
 
-template <typename T, int D>
+template <typename T, int D, bool ONE>
 __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_rows_kernel(const KvAttentionParams p, int items) {
     typedef typename Types<T>::v8 v8;
     constexpr int CH = D / 64, DT = D / 16, LOADS = D / 64, KCH = D / 16;
@@ -461,18 +485,32 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_rows_kerne
     float k_scale = 0.f, v_scale = 0.f;
     int entry = 0;
     Granule there{0, false};
-    auto load_page = [&](int step) { if (step < end) entry = table_entry(c, table, t.key_of(step) + 16 * g); };
+    auto load_page = [&](int step) {
+        if (step >= end) return;
+        if constexpr (ONE) entry = uniform_load(table + min(t.key_of(step) >> c.page_log2, c.width - 1));
+        else entry = table_entry(c, table, t.key_of(step) + 16 * g);
+    };
     auto load_codes = [&](int step) {
         const Granule page = there = page_of(c, entry);
         const int key = t.key_of(step);
         const int64_t at = (int64_t)page.page * c.heads + head;
-        k_scale = c.k_scale[at], v_scale = c.v_scale[at];
+        if constexpr (ONE) {
+            k_scale = uniform_load(c.k_scale + at), v_scale = uniform_load(c.v_scale + at);
+            const uint8_t *k_at = c.k + at * head_bytes + (key & in_page) * D, *v_at = c.v + at * head_bytes + (key & in_page);
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j)
-            k_reg[j] = *reinterpret_cast<const v4i*>(k_head + __shfl(page.page, k_row[j] & 48) * page_bytes + (((key + k_row[j]) & in_page) * D + k_chunk[j]));
-        const uint8_t* v_at = v_head + __shfl(page.page, v_chunk * 16) * page_bytes + ((key + 16 * v_chunk) & in_page);
+            for (int j = 0; j < LOADS; ++j) {
+                k_reg[j] = *reinterpret_cast<const v4i*>(k_at + (uint32_t)(k_row[j] * D + k_chunk[j]));
+                v_reg[j] = *reinterpret_cast<const v4i*>(v_at + (uint32_t)(v_row[j] + v_chunk * 16));
+            }
+        } else {
+            k_scale = c.k_scale[at], v_scale = c.v_scale[at];
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j) v_reg[j] = *reinterpret_cast<const v4i*>(v_at + v_row[j]);
+            for (int j = 0; j < LOADS; ++j)
+                k_reg[j] = *reinterpret_cast<const v4i*>(k_head + __shfl(page.page, k_row[j] & 48) * page_bytes + (((key + k_row[j]) & in_page) * D + k_chunk[j]));
+            const uint8_t* v_at = v_head + __shfl(page.page, v_chunk * 16) * page_bytes + ((key + 16 * v_chunk) & in_page);
+#pragma unroll
+            for (int j = 0; j < LOADS; ++j) v_reg[j] = *reinterpret_cast<const v4i*>(v_at + v_row[j]);
+        }
     };
     auto store_codes = [&](int step, int buffer) {
         const int key = t.key_of(step);
@@ -657,9 +695,17 @@ hipError_t launch(const KvAttentionParams& p, hipStream_t s) {
     const int64_t join = ((int64_t)p.c.rows * p.q_heads * (D / 4) + 255) / 256;
     if (blocks > INT32_MAX || join > INT32_MAX) return hipErrorInvalidValue;
     const dim3 grid((unsigned)blocks), block(256);
-    if (tile_rows == 128) hipLaunchKernelGGL((kv_attention_rows_kernel<T, D>), grid, block, 0, s, p, (int)tiles);
-    else if (tile_rows == 16) hipLaunchKernelGGL((kv_attention_kernel<T, D, 1>), grid, block, 0, s, p);
-    else if constexpr (D != 256) hipLaunchKernelGGL((kv_attention_kernel<T, D, 2>), grid, block, 0, s, p);
+    const bool one = p.c.page_log2 >= 6;
+    if (tile_rows == 128) {
+        if (one) hipLaunchKernelGGL((kv_attention_rows_kernel<T, D, true>), grid, block, 0, s, p, (int)tiles);
+        else hipLaunchKernelGGL((kv_attention_rows_kernel<T, D, false>), grid, block, 0, s, p, (int)tiles);
+    } else if (tile_rows == 16) {
+        if (one) hipLaunchKernelGGL((kv_attention_kernel<T, D, 1, true>), grid, block, 0, s, p);
+        else hipLaunchKernelGGL((kv_attention_kernel<T, D, 1, false>), grid, block, 0, s, p);
+    } else if constexpr (D != 256) {
+        if (one) hipLaunchKernelGGL((kv_attention_kernel<T, D, 2, true>), grid, block, 0, s, p);
+        else hipLaunchKernelGGL((kv_attention_kernel<T, D, 2, false>), grid, block, 0, s, p);
+    }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
     hipLaunchKernelGGL((kv_attention_join_kernel<T, D>), dim3((unsigned)join), block, 0, s, p);

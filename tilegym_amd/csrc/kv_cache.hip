@@ -89,9 +89,9 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendParams p, 
     extern __shared__ uint8_t lds[];  // v: the page's new codes, an element's tokens together, rows of v_pad bytes
     __shared__ float part[4];
     const int half = (int)blockIdx.x & 1, unit = (int)blockIdx.x >> 1, head = unit % c.heads;
-    const SeqItem f = find_sequence(c.indptr, c.batch, c.rows, unit / c.heads, 1, P, 2);
+    const SeqItem f = find_sequence(c, unit / c.heads, 1, P, 2);
     if (f.seq < 0) return;
-    const int64_t len = max(c.lens[f.seq], 0), start = len - f.n;  // position of the sequence's first new token
+    const int64_t len = f.len, start = len - f.n;  // position of the sequence's first new token
     const int64_t first = start > 0 ? start : 0, page_index = (first >> c.page_log2) + f.item;
     if (page_index >= c.width) return;
     const int64_t page_begin = page_index << c.page_log2;
@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvReadParams p, int 
     const KvCache& c = p.c;
     const int tid = (int)threadIdx.x, P = 1 << c.page_log2, D = c.dim, chunks = D / 8;
     const int half = (int)blockIdx.x & 1, unit = (int)blockIdx.x >> 1, head = unit % c.heads;
-    const SeqItem f = find_sequence(c.indptr, c.batch, c.rows, unit / c.heads, 1, P, 1);
+    const SeqItem f = find_sequence(c, unit / c.heads, 1, P, 1);
     if (f.seq < 0 || f.item >= c.width) return;
     const int begin = f.item << c.page_log2, n = min(f.n - begin, P);
     if (n <= 0) return;

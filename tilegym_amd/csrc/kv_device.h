@@ -23,27 +23,33 @@ struct SeqItem {
     int seq;        // -1: none
     int first, n;   // rows of the packed inputs
     int item;       // item of the sequence
+    int len;        // its length, not below zero (0 without lens)
 };
-__device__ __forceinline__ SeqItem find_sequence(const int* __restrict__ indptr, int batch, int rows, int item, int num, int den, int more) {
+// All that is asked for comes in one round of loads: the neighbouring entry and the length by the lane that then turns out to have them.
+__device__ __forceinline__ SeqItem find_sequence(const KvCache& c, int item, int num, int den, int more) {
     const int lane = (int)threadIdx.x & 63;
-    int seq = -1;
-    for (int base = 0; base < batch; base += 64) {
-        const int b = base + lane;
-        bool begun = false;
-        if (b < batch) begun = (int)((int64_t)clamp_row(indptr[b], rows) * num / den) + more * b <= item;
-        const int count = __popcll(__ballot(begun));
-        seq += count;
+    SeqItem f;
+    f.seq = -1, f.first = f.n = f.item = f.len = 0;
+    for (int base = 0; base < c.batch; base += 64) {
+        const int b = base + lane, at = min(b, c.batch - 1);
+        const int first = clamp_row(c.indptr[at], c.rows), end = clamp_row(c.indptr[at + 1], c.rows), len = c.lens ? c.lens[at] : 0;
+        const int begin = (int)((int64_t)first * num / den) + more * b;
+        const int count = __popcll(__ballot(b < c.batch && begin <= item));
+        if (count > 0) {
+            f.seq = base + count - 1;
+            f.first = __builtin_amdgcn_readlane(first, count - 1);
+            f.n = __builtin_amdgcn_readlane(end, count - 1) - f.first;
+            f.item = item - __builtin_amdgcn_readlane(begin, count - 1);
+            f.len = max(__builtin_amdgcn_readlane(len, count - 1), 0);
+        }
         if (count < 64) break;
     }
-    SeqItem f;
-    f.seq = seq;
-    f.first = f.n = f.item = 0;
-    if (seq < 0) return f;
-    f.first = clamp_row(indptr[seq], rows);
-    f.n = clamp_row(indptr[seq + 1], rows) - f.first;
-    f.item = item - ((int)((int64_t)f.first * num / den) + more * seq);
     if (f.n <= 0 || f.item < 0) f.seq = -1;
     return f;
 }
+
+// A value that all lanes have alike, through the scalar cache: it is then not counted among the vector loads in flight
+__device__ __forceinline__ int uniform_load(const int* at) { return *(const __attribute__((address_space(4))) int*)(uintptr_t)at; }
+__device__ __forceinline__ float uniform_load(const float* at) { return *(const __attribute__((address_space(4))) float*)(uintptr_t)at; }
 
 }  // namespace tg
