@@ -22,6 +22,14 @@
 #include <algorithm>
 #include <type_traits>
 
+#ifdef TG_NOFENCE
+#define TG_FENCE
+#else
+#define TG_FENCE __builtin_amdgcn_sched_barrier(0)
+#endif
+#ifndef TG_OCC
+#define TG_OCC 2
+#endif
 #ifndef TG_WANT
 #define TG_WANT 512
 #endif
@@ -33,12 +41,17 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
+typedef float v16f __attribute__((ext_vector_type(16)));
+
 template <typename T> struct Types;
 template <> struct Types<__bf16> { typedef bf16x8 v8; typedef bf16x2 v2; };
 template <> struct Types<_Float16> { typedef f16x8 v8; typedef f16x2 v2; };
 
 __device__ __forceinline__ v4f mfma16(bf16x8 a, bf16x8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ v4f mfma16(f16x8 a, f16x8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+__device__ __forceinline__ v16f mfma32(bf16x8 a, bf16x8 b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ v16f mfma32(f16x8 a, f16x8 b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
 // eight e4m3 codes -> T, exact
 template <typename T>
@@ -56,6 +69,14 @@ __device__ __forceinline__ typename Types<T>::v8 widen(int lo, int hi) {
 
 constexpr int kMostSplits = 64;
 constexpr int kLeastSteps = 4;  // of a split
+// A load through the vector path whatever the address is
+template <typename X>
+__device__ __forceinline__ X vector_load(const X* at) {
+    int zero = 0;
+    asm("" : "+v"(zero));
+    return at[zero];
+}
+
 constexpr float kMinusInf = -__builtin_inff();
 constexpr float kSmallestUnit = 0x1p-126f;
 // The maximum that a row's scores are taken against is looked for only when 16 weights against the old one add up to more than this: floating
@@ -63,6 +84,19 @@ constexpr float kSmallestUnit = 0x1p-126f;
 // -inf and so a sum that is not a number, and take the same path.  In the other steps there is no search, no exchange between lanes
 // and no rescaling of O.
 constexpr float kLargeSum = 4096.f;
+
+// 16 bytes per lane from memory to LDS without a register between: lane i's go to lds_addr + 16 i.  Inline assembly, as the compiler would have every
+// later LDS read wait for a direct load in flight; the kernel waits itself, in front of the barrier after which they are read.  The
+// write of M0 and the s_nop are the five wait states that a scalar operand written by a vector instruction needs.
+__device__ __forceinline__ void load_to_lds(uint32_t lds_addr, const uint8_t* base, uint32_t offset) {  // base: a scalar
+    lds_addr = __builtin_amdgcn_readfirstlane(lds_addr);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds_addr), "v"(offset), "s"(base) : "memory");
+}
+__device__ __forceinline__ void load_to_lds(uint32_t lds_addr, const uint8_t* at) {
+    lds_addr = __builtin_amdgcn_readfirstlane(lds_addr);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds_addr), "v"(at) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p; }
 
 // The rows of one workgroup and the steps of 64 keys that any of them sees.  Positions and keys are below 2^30 (the table's capacity)
 // or a sequence's length.
@@ -96,7 +130,7 @@ __device__ __forceinline__ bool find_tile(const KvAttentionParams& p, int tile_r
 }
 
 // The table's entry for the page of 16 keys, as it is: looked at a step later (page_of), so that the load is not waited for.
-__device__ __forceinline__ int table_entry(const KvCache& c, const int* row, int key) { return row[min(key >> c.page_log2, c.width - 1)]; }
+__device__ __forceinline__ int table_entry(const KvCache& c, const int* row, int key) { return vector_load(row + min(key >> c.page_log2, c.width - 1)); }
 // A page, or one that may be read in its place (its keys are then not seen).
 struct Granule {
     int page;
@@ -122,13 +156,28 @@ __device__ __forceinline__ v4i seen_codes(v4i codes, const RowTile& t, int sinks
     return codes;
 }
 
-__device__ __forceinline__ void select_seen(v4f (&s)[4], int key, int position, int window, int sinks, bool there) {
+// A lane's 16 scores: four results of a 16 x 16 product, or one of a 32 x 32
+struct Scores16 {
+    v4f x[4];
+    __device__ __forceinline__ float operator[](int i) const { return x[i / 4][i % 4]; }
+    __device__ __forceinline__ void set(int i, float f) { x[i / 4][i % 4] = f; }
+    static constexpr int kFirstLane = 16;  // lanes this far apart, and the further powers of two, share a row
+};
+struct Scores32 {
+    v16f x;
+    __device__ __forceinline__ float operator[](int i) const { return x[i]; }
+    __device__ __forceinline__ void set(int i, float f) { x[i] = f; }
+    static constexpr int kFirstLane = 32;
+};
+
+template <typename S>
+__device__ __forceinline__ void select_seen(S& s, int key, int position, int window, int sinks, bool there) {
     const int first_seen = window ? position - (window - 1) : 0;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const int j = key + i;
         const bool seen = there && j <= position && (j >= first_seen || j < sinks);
-        s[i / 4][i % 4] = seen ? s[i / 4][i % 4] : kMinusInf;
+        s.set(i, seen ? s[i] : kMinusInf);
     }
 }
 
@@ -144,6 +193,7 @@ struct Unit {
         if (__ballot(s > u)) {
             float top = fmaxf(s, __shfl_xor(s, 16));
             top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), u);
+            top = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(top)));  // (the same in all lanes)
             grown = u / top;
             u = top, inverse = 1.f / top;
         }
@@ -154,25 +204,21 @@ struct Unit {
 
 // One row's 16 scores of a step -> its weights, against the running maximum m and in units of u, and its sum l.  Returns what O has to
 // be multiplied by on m's account.  factor > 0.
-template <typename T>
-__device__ __forceinline__ float weigh(v4f (&s)[4], float factor, const Unit& unit, float& m, float& l, typename Types<T>::v8 (&pt)[2]) {
-    v4f w[4];
+template <typename T, typename S>
+__device__ __forceinline__ float weigh(const S& s, float factor, const Unit& unit, float& m, float& l, typename Types<T>::v8 (&pt)[2]) {
+    v16f w;
     float shrink = 1.f, base = unit.lift - m, sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            w[i][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j], factor, base));
-            sum = i + j == 0 ? w[i][j] : sum + w[i][j];
-        }
+    for (int i = 0; i < 16; ++i) {
+        w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], factor, base));
+        sum = i == 0 ? w[i] : sum + w[i];
+    }
     if (__ballot(!(sum <= kLargeSum))) {
         float top = kMinusInf;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i] * factor);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) top = fmaxf(top, s[i][j] * factor);
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
+        for (int d = S::kFirstLane; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
         top = fmaxf(m, top);
         const float finite = top == kMinusInf ? 0.f : top;
         shrink = __builtin_amdgcn_exp2f(m - finite);
@@ -181,17 +227,14 @@ __device__ __forceinline__ float weigh(v4f (&s)[4], float factor, const Unit& un
         base = unit.lift - finite;
         sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                w[i][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j], factor, base));
-                sum += w[i][j];
-            }
+        for (int i = 0; i < 16; ++i) {
+            w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], factor, base));
+            sum += w[i];
+        }
     }
     l = __builtin_fmaf(sum, unit.back, l);
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-        pt[h] = __builtin_convertvector(__builtin_shufflevector(w[2 * h], w[2 * h + 1], 0, 1, 2, 3, 4, 5, 6, 7), typename Types<T>::v8);
+    pt[0] = __builtin_convertvector(__builtin_shufflevector(w, w, 0, 1, 2, 3, 4, 5, 6, 7), typename Types<T>::v8);
+    pt[1] = __builtin_convertvector(__builtin_shufflevector(w, w, 8, 9, 10, 11, 12, 13, 14, 15), typename Types<T>::v8);
     return shrink;
 }
 
@@ -309,18 +352,18 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_kernel(con
 
     for (int step = mine; step < end; step += 4) {
         const int key = t.key_of(step), first = key + 16 * g;
-        v4f s[NT][4];
+        Scores16 s[NT];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) s[n][i] = v4f{0.f, 0.f, 0.f, 0.f};
+            for (int n = 0; n < NT; ++n) s[n].x[i] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int ch = 0; ch < CH; ++ch) {
                 const v8 a = widen<T>(kc[i][ch][0], kc[i][ch][1]), b = widen<T>(kc[i][ch][2], kc[i][ch][3]);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    s[n][i] = mfma16(a, q[n][ch][0], s[n][i]);
-                    s[n][i] = mfma16(b, q[n][ch][1], s[n][i]);
+                    s[n].x[i] = mfma16(a, q[n][ch][0], s[n].x[i]);
+                    s[n].x[i] = mfma16(b, q[n][ch][1], s[n].x[i]);
                 }
             }
         }
@@ -416,217 +459,215 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_kernel(con
 
 // Many rows: 128 of them per workgroup, 32 per wave, and every wave runs over the same keys, whose codes are staged in LDS for all
 // four: 16 bytes per lane and load through registers, the next step's while this one's products run, in two buffers with one
-// barrier a step.  Codes stay e4m3 in LDS (half the reads that 16 bits would cost) and are widened behind each read for 32 rows.
-// 16-byte chunks are placed so that the 16 lanes that read together (16 rows of one fragment, one chunk each) cover all banks:
-//   k, chunks of row `key`: chunk ^ f, rows of a fragment being 16 a + 4 i + b;  v, 4 chunks a row: chunk ^ (row / 4) % 4
+// barrier a step.  Codes stay e4m3 in LDS (half the reads that 16 bits would cost) and are widened behind each read, for 32 rows.
+// The products are 32x32x16 instructions on 32 keys at a time, the same way round: S^T row 8 a + 4 h + b stands for key 16 h + 4 a + b, so a
+// lane (row lane % 32, h = lane / 32) has 16 consecutive keys of its one row.
+// 16-byte chunks lie in LDS so that the 8, and the 16, neighbouring lanes that read together cover different banks: chunk ^ f,
+// f of bits 0, 1, 2 and 4 of k's row (its key), and of bits 1, 2 and 3 of v's row (its element).
 template <int D>
-__device__ __forceinline__ int k_swizzle(int row) {
-    const int a = (row >> 4) & 3, b = row & 3;
-    return D == 64 ? a : D == 128 ? 2 * a + (b >> 1) : 4 * a + b;
+__device__ __forceinline__ int k_swizzle(int key) {
+    const int b0 = key & 1, b1 = (key >> 1) & 1, b2 = (key >> 2) & 1, b4 = (key >> 4) & 1;
+    return D == 64 ? (b1 ^ b2) + 2 * b4 : D == 128 ? b1 + 2 * b4 + 4 * (b0 ^ b2) : b0 + 2 * b1 + 4 * b4 + 8 * b2;
 }
-__device__ __forceinline__ int v_swizzle(int row) { return (row >> 2) & 3; }
+__device__ __forceinline__ int v_swizzle(int row) { return (((row >> 1) ^ (row >> 3)) & 1) + 2 * ((row >> 2) & 1); }
 
 template <typename T, int D, bool ONE>
-__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_rows_kernel(const KvAttentionParams p, int items) {
+__global__ void __launch_bounds__(256, D == 256 ? 1 : TG_OCC) kv_attention_rows_kernel(const KvAttentionParams p, int items) {
     typedef typename Types<T>::v8 v8;
-    constexpr int CH = D / 64, DT = D / 16, LOADS = D / 64, KCH = D / 16;
-    constexpr bool EARLY = D < 256;  // (registers)
+    constexpr int CH = D / 32, DT = D / 32, LOADS = D / 64, KCH = D / 16;  // 32-element chunks of a key, 32-element tiles of a value
     __shared__ __align__(16) uint8_t lds_k[2][64 * D], lds_v[2][64 * D];
     const KvCache& c = p.c;
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, g = lane >> 4;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, h = lane >> 5;
     const int head = (int)blockIdx.x % c.heads, rest = (int)blockIdx.x / c.heads, split = rest % p.splits;
     RowTile t;
     if (!find_tile(p, 128, items - 1 - rest / p.splits, head, t)) return;  // (the last rows of a sequence, which see most, first)
     const int share = max((t.steps + p.splits - 1) / p.splits, kLeastSteps);
     const int begin = min(split * share, t.steps), end = min(begin + share, t.steps);
 
-    // this lane's two rows
-    int position[2];
-    v8 q[2][CH][2];
-    float m[2], l[2];
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-        const int row = wave * 32 + n * 16 + col, r = t.r0 + row, token = r / p.group, q_head = head * p.group + r % p.group;
-        position[n] = row < t.rows ? t.start + token : -1;
-        m[n] = row < t.rows ? kMinusInf : 0.f, l[n] = 0.f;
-#pragma unroll
-        for (int ch = 0; ch < CH; ++ch)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                q[n][ch][h] = v8{};
-                if (row < t.rows) q[n][ch][h] = load_q<T>((const T*)p.q + (int64_t)(t.first + token) * p.q_row + (int64_t)q_head * p.q_head + ch * 64 + g * 16 + h * 8, p.scale_log2 < 0.f);
-            }
-    }
-    const int wave_rows = min(t.rows - wave * 32, 32);
-    const int wave_low = t.start + (t.r0 + wave * 32) / p.group, wave_high = t.start + (t.r0 + wave * 32 + wave_rows - 1) / p.group;
-
     const int P = 1 << c.page_log2, in_page = P - 1, head_bytes = P * D;
+    const int* table = c.table + (int64_t)t.seq * c.width;
+    // a step's pages (one for each 16 of a lane's keys, in each half of the step; with ONE one scalar), then its codes and scales on
+    // their way to LDS.  A thread's loads: rows and chunks of its own, the same in every step
+    // (256 threads on, v's row is 64 further, k's 4096 / D: the swizzle is the same, for k if that is a multiple of 32)
+    constexpr int K_ROWS = 4096 / D;
+    const int k_row = tid / KCH, v_chunk = (tid & 3) ^ v_swizzle(tid / 4), v_at0 = (tid / 4) * P + v_chunk * 16;
+    int k_at[K_ROWS % 32 == 0 ? 1 : LOADS];
+#pragma unroll
+    for (int j = 0; j < (K_ROWS % 32 == 0 ? 1 : LOADS); ++j) k_at[j] = (k_row + j * K_ROWS) * D + ((tid % KCH) ^ k_swizzle<D>(k_row + j * K_ROWS)) * 16;
+    auto k_offset = [&](int j) { return K_ROWS % 32 == 0 ? k_at[0] + j * K_ROWS * D : k_at[j]; };
+    constexpr int HALVES = ONE ? 1 : 2;
+    float k_scale[HALVES], v_scale[HALVES];
+    int entry[HALVES];
+    Granule there[HALVES];
+    // (entries are asked for past the last step too: the index is kept inside the table's row)
+    auto load_page = [&](int key) {
+        entry[0] = table_entry(c, table, key + (ONE ? 0 : 16 * h));
+        if constexpr (!ONE) entry[HALVES - 1] = table_entry(c, table, key + 32 + 16 * h);
+    };
     const int64_t page_bytes = (int64_t)c.heads * head_bytes;
     const uint8_t *k_head = c.k + (int64_t)head * head_bytes, *v_head = c.v + (int64_t)head * head_bytes;
-    const int* table = c.table + (int64_t)t.seq * c.width;
-    v4f o[2][DT];
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[n][d] = v4f{0.f, 0.f, 0.f, 0.f};
-    Unit unit;
-
-    // a step's pages, one per group of 16 lanes, then its codes and scales on their way to LDS.  A thread's loads: rows and chunks
-    // of its own, the same in every step
-    int k_row[LOADS], k_chunk[LOADS], v_row[LOADS], v_chunk;
-#pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-        const int ci = tid + 256 * j;
-        k_row[j] = ci / KCH, k_chunk[j] = ((ci % KCH) ^ k_swizzle<D>(k_row[j])) * 16;
-        v_row[j] = (ci / 4) * P;
-    }
-    v_chunk = (tid & 3) ^ v_swizzle(tid / 4);  // (256 threads on, the row is 64 further: the same swizzle)
-    v4i k_reg[LOADS], v_reg[LOADS];
-    float k_scale = 0.f, v_scale = 0.f;
-    int entry = 0;
-    Granule there{0, false};
-    auto load_page = [&](int step) {
-        if (step >= end) return;
-        if constexpr (ONE) entry = uniform_load(table + min(t.key_of(step) >> c.page_log2, c.width - 1));
-        else entry = table_entry(c, table, t.key_of(step) + 16 * g);
-    };
-    auto load_codes = [&](int step) {
-        const Granule page = there = page_of(c, entry);
-        const int key = t.key_of(step);
-        const int64_t at = (int64_t)page.page * c.heads + head;
+    auto load_codes = [&](int key, int buffer) {
+        const uint32_t k_to = lds_address(&lds_k[0][0]) + buffer * (64 * D) + wave * 1024, v_to = lds_address(&lds_v[0][0]) + buffer * (64 * D) + wave * 1024;
         if constexpr (ONE) {
-            k_scale = uniform_load(c.k_scale + at), v_scale = uniform_load(c.v_scale + at);
-            const uint8_t *k_at = c.k + at * head_bytes + (key & in_page) * D, *v_at = c.v + at * head_bytes + (key & in_page);
+            // (vector loads, made scalar where they are used: scalar ones would be waited for by every LDS read)
+            there[0] = page_of(c, __builtin_amdgcn_readfirstlane(entry[0]));
+            const int64_t at = (int64_t)there[0].page * c.heads + head, offset = there[0].page * page_bytes;
+            k_scale[0] = vector_load(c.k_scale + at), v_scale[0] = vector_load(c.v_scale + at);
+            const uint8_t *k_base = k_head + (offset + (key & in_page) * D), *v_base = v_head + (offset + (key & in_page));
 #pragma unroll
             for (int j = 0; j < LOADS; ++j) {
-                k_reg[j] = *reinterpret_cast<const v4i*>(k_at + (uint32_t)(k_row[j] * D + k_chunk[j]));
-                v_reg[j] = *reinterpret_cast<const v4i*>(v_at + (uint32_t)(v_row[j] + v_chunk * 16));
+                if constexpr (K_ROWS % 32 == 0) load_to_lds(k_to + 4096 * j, k_base + j * K_ROWS * D, (uint32_t)k_at[0]);
+                else load_to_lds(k_to + 4096 * j, k_base, (uint32_t)k_at[j]);
+                load_to_lds(v_to + 4096 * j, v_base + j * 64 * P, (uint32_t)v_at0);
             }
         } else {
-            k_scale = c.k_scale[at], v_scale = c.v_scale[at];
+#pragma unroll
+            for (int i = 0; i < HALVES; ++i) {
+                there[i] = page_of(c, entry[i]);
+                const int64_t at = (int64_t)there[i].page * c.heads + head;
+                k_scale[i] = c.k_scale[at], v_scale[i] = c.v_scale[at];
+            }
+            auto block = [&](int sixteenth) {  // of 16 keys: held by the lanes of one h, as entry of one half
+                const int lo = __shfl(there[0].page, (sixteenth & 1) * 32), hi = __shfl(there[HALVES - 1].page, (sixteenth & 1) * 32);
+                return (sixteenth < 2 ? lo : hi) * page_bytes;
+            };
 #pragma unroll
             for (int j = 0; j < LOADS; ++j)
-                k_reg[j] = *reinterpret_cast<const v4i*>(k_head + __shfl(page.page, k_row[j] & 48) * page_bytes + (((key + k_row[j]) & in_page) * D + k_chunk[j]));
-            const uint8_t* v_at = v_head + __shfl(page.page, v_chunk * 16) * page_bytes + ((key + 16 * v_chunk) & in_page);
+                load_to_lds(k_to + 4096 * j, k_head + block((k_row + j * K_ROWS) >> 4) + (((key + k_row + j * K_ROWS) & in_page) * D + (k_offset(j) & (D - 1))));
+            const uint8_t* v_from = v_head + block(v_chunk) + ((tid / 4) * P + ((key + 16 * v_chunk) & in_page));
 #pragma unroll
-            for (int j = 0; j < LOADS; ++j) v_reg[j] = *reinterpret_cast<const v4i*>(v_at + v_row[j]);
+            for (int j = 0; j < LOADS; ++j) load_to_lds(v_to + 4096 * j, v_from + j * 64 * P);
         }
     };
-    auto store_codes = [&](int step, int buffer) {
-        const int key = t.key_of(step);
-        if (key + 64 > t.key1 || key < t.key0 || __ballot(!there.there)) {
-            const bool chunk_there = __shfl((int)there.there, v_chunk * 16) != 0;
-#pragma unroll
-            for (int j = 0; j < LOADS; ++j) v_reg[j] = seen_codes(v_reg[j], t, p.sinks, key + 16 * v_chunk, chunk_there);
-        }
-#pragma unroll
-        for (int j = 0; j < LOADS; ++j) {
-            *reinterpret_cast<v4i*>(&lds_k[buffer][(tid + 256 * j) * 16]) = k_reg[j];
-            *reinterpret_cast<v4i*>(&lds_v[buffer][(tid + 256 * j) * 16]) = v_reg[j];
-        }
-    };
+    // the keys of this step, the next and the one after it
+    auto key_behind = [&](int key, int step) { return step == t.sink_steps ? t.key0 & ~63 : key + 64; };  // step: the one behind
+    int key = t.key_of(begin), key1 = key_behind(key, begin + 1), key2 = key_behind(key1, begin + 2);
+    load_page(key);
 
-    if (begin < end) {
-        load_page(begin);
-        load_codes(begin);
-        load_page(begin + 1);
-        store_codes(begin, 0);
-    }
-    __syncthreads();
-    for (int step = begin; step < end; ++step) {
-        const int buffer = (step - begin) & 1;
-        const int key = t.key_of(step), first = key + 16 * g;
-        const float factor = score_factor(k_scale, p.scale_log2), this_v_scale = v_scale;
-        const bool page_there = there.there;
-        if (step + 1 < end) {
-            load_codes(step + 1);
-            load_page(step + 2);
+    // this lane's row
+    const int row = wave * 32 + col, r = t.r0 + row, token = r / p.group, q_head = head * p.group + r % p.group;
+    const bool live = row < t.rows;
+    const int position = live ? t.start + token : -1;
+    v8 q[CH][2];
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            q[ch][j] = v8{};
+            if (live) q[ch][j] = load_q<T>((const T*)p.q + (int64_t)(t.first + token) * p.q_row + (int64_t)q_head * p.q_head + ch * 32 + h * 16 + j * 8, p.scale_log2 < 0.f);
         }
-        if (wave_rows > 0 && key <= wave_high) {
-            // fragments of k, and then of v in front of the softmax, are all asked for before the first is used
-            v4f s[2][4];
-            v4i kc[4][CH], vc[DT];
+    // the first 32 keys from `none` on are seen by no row of the wave; those at `last_whole` and before, and behind `first_whole`, by all
+    const int wave_rows = min(t.rows - wave * 32, 32);
+    const int none = wave_rows > 0 ? t.start + (t.r0 + wave * 32 + wave_rows - 1) / p.group + 1 : 0;
+    const int last_whole = t.start + (t.r0 + wave * 32) / p.group - 31, first_whole = p.window ? none - 1 - p.window : -1;
+    if (begin < end) {
+        load_codes(key, 0);
+        load_page(key1);
+    }
+    v16f o[DT];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+    for (int d = 0; d < DT; ++d) o[d] = v16f{};
+    float m = live ? kMinusInf : 0.f, l = 0.f;
+    Unit unit;
+    const int s_key = 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3);  // the key that this lane reads as a row of K, of 32
+    const int k_lane = s_key * D + (h ^ k_swizzle<D>(s_key)) * 16, v_lane = col * 64 + (h ^ v_swizzle(col)) * 16;
+    for (int step = begin; step < end; ++step, key = key1, key1 = key2) {
+        const int buffer = (step - begin) & 1;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();  // this step's codes are there for all, and all are done with the other buffer
+        float factor[HALVES], this_v_scale[HALVES];
+        bool page_there[HALVES];
 #pragma unroll
-                for (int ch = 0; ch < CH; ++ch) {
-                    const int row = 16 * (col >> 2) + 4 * i + (col & 3);
-                    kc[i][ch] = *reinterpret_cast<const v4i*>(&lds_k[buffer][row * D + ((ch * 4 + g) ^ k_swizzle<D>(row)) * 16]);
-                }
-            if constexpr (EARLY) __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < HALVES; ++i) factor[i] = score_factor(k_scale[i], p.scale_log2), this_v_scale[i] = v_scale[i], page_there[i] = there[i].there;
+        key2 = key_behind(key1, step + 2);
+        if (step + 1 < end) {
+            load_codes(key1, buffer ^ 1);
+            load_page(key2);
+        }
+        if (key >= none) continue;
+        // (with ONE, a scalar: whether any key of the step's page is seen by the tile)
+        if constexpr (ONE) unit.step(this_v_scale[0], page_there[0] && key < t.key1 && (key + 64 > t.key0 || key < p.sinks));
+        // fragments are asked for a phase ahead (k's of the second half in front of the first half's second product, v's in front of
+        // the softmax), pinned by fences: behind each other, a read's latency and its use would add up 16 times a step
+        // (the chunks of a fragment's rows differ from the first one's in an exclusive or of their number, which the swizzle leaves alone)
+        v4i kc[CH], vc[DT];
+        const int k_first = k_lane + buffer * (64 * D), v_first = v_lane + buffer * (64 * D);
+        auto read_k = [&](int half) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                s[0][i] = s[1][i] = v4f{0.f, 0.f, 0.f, 0.f};
+            for (int ch = 0; ch < CH; ++ch) kc[ch] = *reinterpret_cast<const v4i*>(&lds_k[0][0] + (k_first ^ (ch * 32)) + half * 32 * D);
+            if constexpr (D < 256) TG_FENCE;
+        };
+        read_k(0);
 #pragma unroll
-                for (int ch = 0; ch < CH; ++ch) {
-                    const v8 a = widen<T>(kc[i][ch][0], kc[i][ch][1]), b = widen<T>(kc[i][ch][2], kc[i][ch][3]);
+        for (int half = 0; half < 2; ++half) {
+            const int key_h = key + 32 * half, first = key_h + 16 * h, i_h = ONE ? 0 : half;
+            if (half == 1 && key_h >= none) continue;
+            Scores32 s;
+            s.x = v16f{};
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        s[n][i] = mfma16(a, q[n][ch][0], s[n][i]);
-                        s[n][i] = mfma16(b, q[n][ch][1], s[n][i]);
-                    }
-                }
-            }
-            auto read_v = [&](int d) {
-                const int row = d * 16 + col;
-                vc[d] = *reinterpret_cast<const v4i*>(&lds_v[buffer][row * 64 + (g ^ v_swizzle(row)) * 16]);
-            };
-            if constexpr (EARLY) {
-#pragma unroll
-                for (int d = 0; d < DT; ++d) read_v(d);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            const bool whole = key + 63 <= wave_low && (!p.window || key > wave_high - p.window) && __ballot(!page_there) == 0;
-            unit.step(this_v_scale, whole || (page_there && first < t.key1 && (first + 16 > t.key0 || first < p.sinks)));
-            if (!whole) {
-#pragma unroll
-                for (int n = 0; n < 2; ++n) select_seen(s[n], first, position[n], p.window, p.sinks, page_there);
-            }
-            v8 pt[2][2];
-            float rescale[2];
-#pragma unroll
-            for (int n = 0; n < 2; ++n) rescale[n] = weigh<T>(s[n], factor, unit, m[n], l[n], pt[n]) * unit.grown;
-            if (__ballot(rescale[0] != 1.f || rescale[1] != 1.f)) {
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) o[n][d] *= rescale[n];
+            for (int ch = 0; ch < CH; ++ch) {
+                s.x = mfma32(widen<T>(kc[ch][0], kc[ch][1]), q[ch][0], s.x);
+                s.x = mfma32(widen<T>(kc[ch][2], kc[ch][3]), q[ch][1], s.x);
             }
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                if constexpr (!EARLY) read_v(d);
-                const v8 a = widen<T>(vc[d][0], vc[d][1]), b = widen<T>(vc[d][2], vc[d][3]);
+                vc[d] = *reinterpret_cast<const v4i*>(&lds_v[0][0] + (v_first ^ (half * 32)) + d * 32 * 64);
+            }
+            if constexpr (D < 256) TG_FENCE;
+            bool whole = key_h <= last_whole && key_h > first_whole;
+            if constexpr (ONE) {
+                whole = whole && page_there[0];
+            } else {
+                whole = whole && __ballot(!page_there[i_h]) == 0;
+                unit.step(this_v_scale[i_h], whole || (page_there[i_h] && first < t.key1 && (first + 16 > t.key0 || first < p.sinks)));
+            }
+            if (!whole) {
+                asm volatile("");  // (keeps the selection a branch)
+                select_seen(s, first, position, p.window, p.sinks, page_there[i_h]);
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    o[n][d] = mfma16(a, pt[n][0], o[n][d]);
-                    o[n][d] = mfma16(b, pt[n][1], o[n][d]);
-                }
+                for (int d = 0; d < DT; ++d) vc[d] = seen_codes(vc[d], t, p.sinks, first, page_there[i_h]);
+            }
+            v8 pt[2];
+            float rescale = weigh<T>(s, factor[i_h], unit, m, l, pt);
+            if (!ONE || half == 0) rescale *= unit.grown;
+            if (__ballot(rescale != 1.f)) {
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[d] *= rescale;
+            }
+            if (half == 0) read_k(1);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                o[d] = mfma32(widen<T>(vc[d][0], vc[d][1]), pt[0], o[d]);
+                o[d] = mfma32(widen<T>(vc[d][2], vc[d][3]), pt[1], o[d]);
             }
         }
-        if (step + 1 < end) store_codes(step + 1, buffer ^ 1);
-        __syncthreads();
     }
 
+    const float sum = l + __shfl_xor(l, 32);
+    int last = t.r0 + row;
+    asm("" : "+v"(last));  // (worked out again, not held through the loop)
+    if (row >= t.rows) return;
+    const int64_t out_row = (int64_t)(t.first + last / p.group) * p.q_heads + head * p.group + last % p.group;
+    if (p.splits > 1) {
+        const int64_t at = (int64_t)split * c.rows * p.q_heads + out_row;
+        if (h == 0) p.part_ml[2 * at] = m, p.part_ml[2 * at + 1] = sum;
+        if (sum > 0.f) {
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-        float sum = l[n] + __shfl_xor(l[n], 16);
-        sum += __shfl_xor(sum, 32);
-        const int row = wave * 32 + n * 16 + col, r = t.r0 + row;
-        if (row >= t.rows) continue;
-        const int64_t out_row = (int64_t)(t.first + r / p.group) * p.q_heads + head * p.group + r % p.group;
-        if (p.splits > 1) {
-            const int64_t at = (int64_t)split * c.rows * p.q_heads + out_row;
-            if (g == 0) p.part_ml[2 * at] = m[n], p.part_ml[2 * at + 1] = sum;
-            if (sum > 0.f) {
+            for (int d = 0; d < DT; ++d)
 #pragma unroll
-                for (int d = 0; d < DT; ++d) *reinterpret_cast<v4f*>(p.part_o + at * D + d * 16 + 4 * g) = o[n][d] * unit.u;
-            }
-        } else {
-            typedef T v4t __attribute__((ext_vector_type(4)));
-            const float f = sum > 0.f ? unit.u / sum : 0.f;  // a row that sees nothing is zero
-#pragma unroll
-            for (int d = 0; d < DT; ++d) *reinterpret_cast<v4t*>((T*)p.out + out_row * D + d * 16 + 4 * g) = __builtin_convertvector(o[n][d] * f, v4t);
+                for (int a = 0; a < 4; ++a)
+                    *reinterpret_cast<v4f*>(p.part_o + at * D + d * 32 + 8 * a + 4 * h) = v4f{o[d][4 * a], o[d][4 * a + 1], o[d][4 * a + 2], o[d][4 * a + 3]} * unit.u;
         }
+    } else {
+        typedef T v4t __attribute__((ext_vector_type(4)));
+        const float f = sum > 0.f ? unit.u / sum : 0.f;  // a row that sees nothing is zero
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                const v4f x = v4f{o[d][4 * a], o[d][4 * a + 1], o[d][4 * a + 2], o[d][4 * a + 3]} * f;
+                *reinterpret_cast<v4t*>((T*)p.out + out_row * D + d * 32 + 8 * a + 4 * h) = __builtin_convertvector(x, v4t);
+            }
     }
 }
 
