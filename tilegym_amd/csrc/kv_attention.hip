@@ -27,11 +27,17 @@
 #else
 #define TG_FENCE __builtin_amdgcn_sched_barrier(0)
 #endif
+#ifndef TG_DOCC
+#define TG_DOCC 3
+#endif
 #ifndef TG_OCC
 #define TG_OCC 2
 #endif
 #ifndef TG_WANT
-#define TG_WANT 512
+#define TG_WANT 2304
+#endif
+#ifndef TG_WANT2
+#define TG_WANT2 768
 #endif
 namespace tg {
 namespace {
@@ -253,7 +259,7 @@ __device__ __forceinline__ float score_factor(float k_scale, float scale_log2) {
 // from memory into registers, k's of the next step being asked for when this step's are used up, v's likewise.
 // ONE: pages hold whole steps (64 or 128 tokens), so a step's page, its scales and its address are scalars.
 template <typename T, int D, int NT, bool ONE>
-__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_kernel(const KvAttentionParams p) {
+__global__ void __launch_bounds__(256, D == 256 ? 1 : NT == 1 && ONE ? TG_DOCC : 2) kv_attention_kernel(const KvAttentionParams p) {
     typedef typename Types<T>::v8 v8;
     constexpr int CH = D / 64, DT = D / 16, ROWS = 16 * NT;  // 64-element chunks of a key, 16-element tiles of a value
     const KvCache& c = p.c;
@@ -307,9 +313,11 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_kernel(con
         const int key = t.key_of(step);
         const int64_t at = (int64_t)v_page.page * c.heads + t.head;
         if constexpr (ONE) {
-            const uint8_t* base = c.v + at * head_bytes + (key & in_page);
+            // (one scalar base: eight would not fit the scalar registers)
+            const uint8_t* base = c.v + at * head_bytes;
+            const int offset = v_lane + (key & in_page);
 #pragma unroll
-            for (int d = 0; d < DT; ++d) vc[d] = *reinterpret_cast<const v4i*>(base + d * 16 * P + (uint32_t)v_lane);
+            for (int d = 0; d < DT; ++d) vc[d] = *reinterpret_cast<const v4i*>(base + (uint32_t)(offset + d * 16 * P));
             v_scale = uniform_load(c.v_scale + at);
         } else {
             const uint8_t* base = c.v + at * head_bytes + col * P + ((key + 16 * g) & in_page);
@@ -755,12 +763,17 @@ hipError_t launch(const KvAttentionParams& p, hipStream_t s) {
 
 }  // namespace
 
+// Workgroups to spread the keys of a call over.  Few rows (768 at a time on the chip): three rounds, so that sequences of uneven length fill it
+// (64 sequences of 100 to 8000 tokens, 8 heads of 128: 116 us with 768, 115 with 1536, 112 with 2304, 112 with 4096, without splits 124).
+// The other forms: a round and a half; their results are larger against their keys (5 new tokens in 16 sequences of 500 to 4000: 36 us with 256, 30
+// with 512, 29 with 768, 35 with 1536, 40 with 2304).
 int kv_attention_splits(const KvAttentionParams& p) {
-    const int64_t units = row_tiles(p, tile_rows_of(p)) * p.c.heads;
+    const int tile_rows = tile_rows_of(p);
+    const int64_t units = row_tiles(p, tile_rows) * p.c.heads;
     int64_t keys = (int64_t)p.c.width << p.c.page_log2;
     if (p.window) keys = std::min<int64_t>(keys, (int64_t)p.window + 128 + (p.sinks + 63) / 64 * 64);
-    const int64_t steps = (keys + 63) / 64;
-    const int64_t wanted = (TG_WANT + units - 1) / units, most = (steps + kLeastSteps - 1) / kLeastSteps;
+    const int64_t steps = (keys + 63) / 64, workgroups = tile_rows == 16 ? TG_WANT : TG_WANT2;
+    const int64_t wanted = (workgroups + units - 1) / units, most = (steps + kLeastSteps - 1) / kLeastSteps;
     return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(wanted, most), kMostSplits));
 }
 

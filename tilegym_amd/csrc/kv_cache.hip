@@ -167,56 +167,105 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendParams p, 
     }
 }
 
-// Reading: element = code * scale (one fp32 product, rounded once).  A workgroup per page, head and half; v is turned through LDS.
+// Reading: element = code * scale (one fp32 product, rounded once).  A workgroup per 64 tokens of a sequence, head and half, whatever the
+// page: 16-token pages one by one would make workgroups that are all latency.  k's rows are widened straight away; v's are turned in
+// 4 x 4 blocks of bytes in registers, then through LDS.
+// 16 bytes of output: four or eight elements, from one or two dwords of codes.
 template <typename T>
-__global__ void __launch_bounds__(256) kv_read_kernel(const KvReadParams p, int items, int v_pad) {
-    typedef T vecT __attribute__((ext_vector_type(8)));
-    extern __shared__ uint8_t lds[];
+__device__ __forceinline__ void store_widened(T* at, v2i codes, float scale) {
+    typedef float v2f __attribute__((ext_vector_type(2)));
+    typedef T vecT __attribute__((ext_vector_type(16 / sizeof(T))));
+    v8f_q y;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const v2f lo = __builtin_amdgcn_cvt_pk_f32_fp8(codes[h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(codes[h], true);
+        y[4 * h] = lo[0] * scale, y[4 * h + 1] = lo[1] * scale, y[4 * h + 2] = hi[0] * scale, y[4 * h + 3] = hi[1] * scale;
+    }
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<v4f*>(at) = __builtin_shufflevector(y, y, 0, 1, 2, 3);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {  // the product is rounded on its own, then converted (no single-rounding mixed-precision multiplication)
+            float t = y[i];
+            asm("" : "+v"(t));
+            y[i] = t;
+        }
+        *reinterpret_cast<vecT*>(at) = __builtin_convertvector(y, vecT);
+    }
+}
+
+// The place of 16-byte chunk `chunk` of a token's row in LDS: what neighbouring lanes write, four tokens 16 apart, goes to different banks.
+__device__ __forceinline__ int turned_chunk(int token, int chunk, int chunks) { return chunk ^ ((2 * (token >> 4)) & (chunks - 1)); }
+
+template <typename T>
+__global__ void __launch_bounds__(256) kv_read_kernel(const KvReadParams p) {
+    extern __shared__ __align__(16) uint8_t lds[];  // v: 64 tokens' rows of D codes
     const KvCache& c = p.c;
-    const int tid = (int)threadIdx.x, P = 1 << c.page_log2, D = c.dim, chunks = D / 8;
+    const int tid = (int)threadIdx.x, P = 1 << c.page_log2, D = c.dim, chunks = D / 16;
     const int half = (int)blockIdx.x & 1, unit = (int)blockIdx.x >> 1, head = unit % c.heads;
-    const SeqItem f = find_sequence(c, unit / c.heads, 1, P, 1);
-    if (f.seq < 0 || f.item >= c.width) return;
-    const int begin = f.item << c.page_log2, n = min(f.n - begin, P);
+    const SeqItem f = find_sequence(c, unit / c.heads, 1, 64, 1);
+    if (f.seq < 0) return;
+    const int64_t begin = (int64_t)f.item * 64, capacity = (int64_t)c.width << c.page_log2;
+    const int n = (int)min(min((int64_t)f.n, capacity) - begin, (int64_t)64);
     if (n <= 0) return;
-    const int page = c.table[(int64_t)f.seq * c.width + f.item];
-    if (page < 0 || page >= c.pages) return;
-    const int64_t block = (int64_t)page * c.heads + head;
-    const float scale = (half ? c.v_scale : c.k_scale)[block];
-    const uint8_t* codes = (half ? c.v : c.k) + block * ((int64_t)P * D);
+    const int* row = c.table + (int64_t)f.seq * c.width;
+    const uint8_t* codes = half ? c.v : c.k;
+    const float* scales = half ? c.v_scale : c.k_scale;
     T* out = (T*)(half ? p.v : p.k) + (((int64_t)f.first + begin) * c.heads + head) * D;
+    // the page of a token, or -1 (its row is then left as it was)
+    auto page_at = [&](int token) {
+        const int page = row[(begin + token) >> c.page_log2];
+        return page >= 0 && page < c.pages ? page : -1;
+    };
     if (half) {
-        const int words = P / 4;
-        for (int i = tid; i < D * words; i += 256) {
-            const int d = i / words, s = 4 * (i % words);
-            *reinterpret_cast<uint32_t*>(lds + d * v_pad + s) = *reinterpret_cast<const uint32_t*>(codes + d * P + s);
+        for (int i = tid; i < D; i += 256) {  // (a block of four elements, 16 tokens)
+            const int four = i >> 2, token = 16 * (i & 3);
+            if (token >= n) continue;
+            const int page = page_at(token);
+            if (page < 0) continue;
+            const uint8_t* from = codes + ((int64_t)page * c.heads + head) * ((int64_t)P * D) + 4 * four * P + (int)((begin + token) & (P - 1));
+            v4i x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = *reinterpret_cast<const v4i*>(from + e * P);
+#pragma unroll
+            for (int t4 = 0; t4 < 4; ++t4) {
+                const uint32_t a = x[0][t4], b = x[1][t4], d = x[2][t4], e = x[3][t4];  // four tokens of one element each
+                const uint32_t ab = __builtin_amdgcn_perm(b, a, 0x05010400), de = __builtin_amdgcn_perm(e, d, 0x05010400),
+                               ab2 = __builtin_amdgcn_perm(b, a, 0x07030602), de2 = __builtin_amdgcn_perm(e, d, 0x07030602);
+                const uint32_t w[4] = {__builtin_amdgcn_perm(de, ab, 0x05040100), __builtin_amdgcn_perm(de, ab, 0x07060302),
+                                       __builtin_amdgcn_perm(de2, ab2, 0x05040100), __builtin_amdgcn_perm(de2, ab2, 0x07060302)};
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const int to = token + 4 * t4 + t;
+                    *reinterpret_cast<uint32_t*>(lds + to * D + turned_chunk(to, four >> 2, chunks) * 16 + 4 * (four & 3)) = w[t];
+                }
+            }
         }
         __syncthreads();
     }
-    for (int i = tid; i < n * chunks; i += 256) {
-        const int slot = i / chunks, ch = i % chunks;
-        v2i raw;
-        if (!half) {
-            raw = *reinterpret_cast<const v2i*>(codes + slot * D + 8 * ch);
-        } else {
-            uint32_t w[2] = {0, 0};
+    // 16 bytes of output per lane and store, neighbouring lanes side by side, four loads ahead of their stores.  A wave's lanes are in the same 16
+    // tokens (64 E / D of them are 16 at most), so page and scale are scalars.
+    constexpr int E = 16 / sizeof(T);
+    const int shift = 31 - __clz(D / E), count = n << shift;  // (D / E: a power of two)
+    for (int i0 = tid; i0 < count; i0 += 1024) {
+        v2i x[4];
+        float scale[4];
+        int page[4];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) w[k / 4] |= (uint32_t)lds[(8 * ch + k) * v_pad + slot] << (8 * (k & 3));
-            raw = v2i{(int)w[0], (int)w[1]};
+        for (int u = 0; u < 4; ++u) {
+            const int i = min(i0 + 256 * u, count - 1), token = i >> shift, e = (i - (token << shift)) * E;
+            page[u] = uniform_load(row + ((begin + __builtin_amdgcn_readfirstlane(token)) >> c.page_log2));
+            if (page[u] >= c.pages) page[u] = -1;
+            const int64_t block = (int64_t)max(page[u], 0) * c.heads + head;
+            scale[u] = uniform_load(scales + block);
+            auto load = [&](const uint8_t* at) { return E == 8 ? *reinterpret_cast<const v2i*>(at) : v2i{*reinterpret_cast<const int*>(at), 0}; };
+            if (half) x[u] = load(lds + token * D + turned_chunk(token, e >> 4, chunks) * 16 + (e & 15));
+            else x[u] = load(codes + block * ((int64_t)P * D) + (int)((begin + token) & (P - 1)) * D + e);
         }
-        typedef float v2f __attribute__((ext_vector_type(2)));
-        v8f_q y;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const v2f lo = __builtin_amdgcn_cvt_pk_f32_fp8(raw[h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(raw[h], true);
-            y[4 * h] = lo[0] * scale, y[4 * h + 1] = lo[1] * scale, y[4 * h + 2] = hi[0] * scale, y[4 * h + 3] = hi[1] * scale;
-        }
-        T* at = out + (int64_t)slot * c.heads * D + 8 * ch;
-        if constexpr (sizeof(T) == 4) {
-            reinterpret_cast<v4f*>(at)[0] = __builtin_shufflevector(y, y, 0, 1, 2, 3);
-            reinterpret_cast<v4f*>(at)[1] = __builtin_shufflevector(y, y, 4, 5, 6, 7);
-        } else {
-            *reinterpret_cast<vecT*>(at) = __builtin_convertvector(y, vecT);
+        for (int u = 0; u < 4; ++u) {
+            const int i = i0 + 256 * u, token = i >> shift;
+            if (i < count && page[u] >= 0) store_widened<T>(out + (int64_t)token * c.heads * D + (i - (token << shift)) * E, x[u], scale[u]);
         }
     }
 }
@@ -241,14 +290,13 @@ hipError_t run_kv_append(const KvAppendParams& p, bool is_bf16, hipStream_t s) {
 hipError_t run_kv_read(const KvReadParams& p, int out_type, hipStream_t s) {
     const KvCache& c = p.c;
     if (c.rows <= 0 || c.batch <= 0) return hipSuccess;
-    const int64_t P = (int64_t)1 << c.page_log2, items = c.rows / P + c.batch, blocks = items * c.heads * 2;
+    const int64_t blocks = ((int64_t)c.rows / 64 + c.batch) * c.heads * 2;
     if (blocks > INT32_MAX) return hipErrorInvalidValue;
-    const int v_pad = (int)P + 4;
     const dim3 grid((unsigned)blocks), block(256);
-    const size_t lds = (size_t)c.dim * v_pad;
-    if (out_type == OUT_BF16) hipLaunchKernelGGL(kv_read_kernel<__bf16>, grid, block, lds, s, p, (int)items, v_pad);
-    else if (out_type == OUT_F16) hipLaunchKernelGGL(kv_read_kernel<_Float16>, grid, block, lds, s, p, (int)items, v_pad);
-    else if (out_type == OUT_F32) hipLaunchKernelGGL(kv_read_kernel<float>, grid, block, lds, s, p, (int)items, v_pad);
+    const size_t lds = (size_t)c.dim * 64;
+    if (out_type == OUT_BF16) hipLaunchKernelGGL(kv_read_kernel<__bf16>, grid, block, lds, s, p);
+    else if (out_type == OUT_F16) hipLaunchKernelGGL(kv_read_kernel<_Float16>, grid, block, lds, s, p);
+    else if (out_type == OUT_F32) hipLaunchKernelGGL(kv_read_kernel<float>, grid, block, lds, s, p);
     else return hipErrorInvalidValue;
     return hipGetLastError();
 }

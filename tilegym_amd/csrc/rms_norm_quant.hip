@@ -7,7 +7,7 @@
 // The norm is taken of the fp32 sum and y goes to e4m3 without a 16-bit rounding between: one rounding in place of three
 // launches' three.
 //
-// Bound by HBM (at most 3 x 16 bits + 1 byte per element): a row is read once and stays in the registers of the lanes that
+// Bound by HBM (at most 3 x 16 bits + 1 byte per element), few rows by latency: a row is read once and stays in the registers of the lanes that
 // share it, V vectors of 8 elements each; the two reductions are the sum of squares over the row and the maximum over the 2 to
 // 16 neighbouring lanes of a group.
 #include "quant_device.h"
@@ -28,7 +28,7 @@ __device__ __forceinline__ void store8<float>(float* p, v8f_q v) {
     reinterpret_cast<v4f*>(p)[1] = __builtin_shufflevector(v, v, 4, 5, 6, 7);
 }
 
-// TPR lanes share a row (64: one wave, four rows per workgroup; else the workgroup has one row), V vectors of 8 elements per lane.
+// TPR lanes share a row (64 or 128: four or two rows per workgroup; else the workgroup has one), V vectors of 8 elements per lane.
 // x, r and their outputs may be the same memory (element by element): no __restrict__ on them.
 template <typename T, typename W, int TPR, int V>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) rms_norm_quant_kernel(const NormQuantParams p) {
@@ -66,12 +66,12 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) rms_norm_quant_kernel(c
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
     if constexpr (WAVES > 1) {
-        __shared__ float part[WAVES];
+        __shared__ float part[ROWS * WAVES];
         if (tid % 64 == 0) part[tid / 64] = sum;
         __syncthreads();
         sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < WAVES; ++i) sum += part[i];
+        for (int i = 0; i < WAVES; ++i) sum += part[tid / TPR * WAVES + i];
     }
     if (!live) return;
     const float norm = 1.0f / sqrtf(sum / (float)p.hidden + p.eps);
@@ -99,10 +99,11 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) rms_norm_quant_kernel(c
                 s = amax == 0.f ? 1.0f : amax / 448.0f;
                 if ((at & (p.lanes_per_group - 1)) == 0) p.scales[row * (vectors >> p.group_shift) + (at >> p.group_shift)] = s;
             }
-            const ScaleDivider div(s);
+            // y carries the norm's own 2^-22; a reciprocal's half unit in the last place moves a code only where y / s lies that near a border
+            const float inverse = 1.0f / s;
             v8f_q c;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) c[k] = __builtin_amdgcn_fmed3f(div.fast ? div.quotient(y[k]) : y[k] / s, -448.0f, 448.0f);
+            for (int k = 0; k < 8; ++k) c[k] = __builtin_amdgcn_fmed3f(y[k] * inverse, -448.0f, 448.0f);
             int packed[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -117,6 +118,11 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) rms_norm_quant_kernel(c
     }
 }
 
+// As many lanes as a row has vectors, one each: a row's chain of load, sum, exchange, store is shortest, and few registers let many rows share
+// a compute unit (kernel and launch, bf16 with residual, one vector per lane against up to four on 256 lanes: 1 x 4096 3.5 / 4.3 us,
+// 777 x 5120 9.7 / 13.5, 4096 x 8192 49.3 / 85.0, 1000 x 16384 with two on 1024 24.8 / 39.8).  Rows of 4097 to 8192 elements leave lanes of 1024 idle:
+// with enough rows to fill the chip two vectors on 512 are ahead (777 x 5120 9.0 / 9.7 us, 2000 x 8192 24.2 / 25.7; one row of 8192 4.1 / 3.9).
+// 8192 x 4096: 47.8 us, 4.9 TB/s (a copy: 5.2).
 template <typename T, typename W>
 hipError_t launch(const NormQuantParams& p, hipStream_t s) {
     const int vectors = p.hidden / 8;
@@ -127,11 +133,14 @@ hipError_t launch(const NormQuantParams& p, hipStream_t s) {
         return hipGetLastError();                                                                                                \
     }
     TG_NORM(64, 1)
-    TG_NORM(64, 2)
+    TG_NORM(128, 1)
     TG_NORM(256, 1)
-    TG_NORM(256, 2)
-    TG_NORM(256, 4)
-    TG_NORM(512, 4)
+    TG_NORM(512, 1)
+    if (p.rows >= 512) {
+        TG_NORM(512, 2)
+    }
+    TG_NORM(1024, 1)
+    TG_NORM(1024, 2)
     TG_NORM(512, 8)
 #undef TG_NORM
     return hipErrorInvalidValue;
