@@ -7,9 +7,11 @@
 //           power of two costs its codes no precision, and moving stored codes from one power of two to a larger one only shifts their
 //           exponents, exact but for e4m3's subnormals.  So a page that fills token by token keeps max(old, new) as its scale,
 //           and its earlier codes move when the scale does: no token is rounded at more than one precision.
-// One workgroup writes the new tokens of one page, head and half of the cache: it alone reads and writes that scale, so no
-// atomics, and the result does not depend on the order of workgroups.  Bound by HBM at many tokens, by the launch and one chain
+// One workgroup, or wave, writes the new tokens of one page, head and half of the cache: it alone reads and writes that scale, so no
+// atomics, and the result does not depend on any order.  Bound by HBM at many tokens, by the launch and one chain
 // of dependent loads (sequence, page, scale) at few.
+#include <algorithm>
+
 #include "kv_device.h"
 #include "quant_device.h"
 
@@ -58,38 +60,50 @@ __device__ __forceinline__ v8f_q load_turned(const T* x, int c, const float* row
     return y;
 }
 
-// Workgroups of the two kinds of work: first those that write the cache, (item, head, half) with the half fastest, then those that turn q.
-template <typename T>
-__global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendParams p, int items, int v_pad) {
+// What lanes of one wave, or of the workgroup, have written to LDS is there for the others of them.
+template <int WAVES>
+__device__ __forceinline__ void lds_written() {
+    if constexpr (WAVES > 1) {
+        __syncthreads();
+    } else {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+}
+
+// Workgroups of the two kinds of work: first those that write the cache, then those that turn q.  A page, head and half is the work of WAVES
+// waves: four where sequences have many new tokens, one where they have few (16 lanes of 8 elements have a token's 128).
+template <typename T, int WAVES>
+__global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendParams p, int items, int cache_blocks, int v_pad, int q_waves) {
+    constexpr int LANES = 64 * WAVES;
+    typedef T vecT __attribute__((ext_vector_type(8)));
     const KvCache& c = p.c;
-    const int tid = (int)threadIdx.x, P = 1 << c.page_log2, D = c.dim, chunks = D / 8;
-    const int cache_blocks = items * c.heads * 2;
+    const int P = 1 << c.page_log2, D = c.dim, chunks = D / 8, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     if ((int)blockIdx.x >= cache_blocks) {
-        // q: eight elements per lane
-        const int64_t at = (int64_t)((int)blockIdx.x - cache_blocks) * 256 + tid;
-        const int per_row = p.q_heads * chunks;
-        const int64_t row64 = at / per_row;
-        if (row64 >= c.rows) return;
-        const int row = (int)row64, rest = (int)(at - row64 * per_row), head = rest / chunks, ch = rest - head * chunks;
-        int lo = 0, hi = c.batch;  // the last sequence that begins at or before `row`
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (clamp_row(c.indptr[mid], c.rows) <= row) lo = mid;
-            else hi = mid;
+        // q: a wave has one token, and every q_waves-th 64 vectors of 8 elements of it
+        const int64_t job = (int64_t)((int)blockIdx.x - cache_blocks) * 4 + wave;
+        const int64_t row = job / q_waves;
+        if (row >= c.rows) return;
+        const SeqItem f = find_sequence(c, (int)row, 1, 1, 0);
+        if (f.seq < 0 || f.item >= f.n) return;  // a row of no sequence: left as it was
+        const int64_t position = (int64_t)f.len - f.n + f.item;
+        const float* angles = p.rope + min(max(position, (int64_t)0), (int64_t)p.rope_rows - 1) * p.rotary;
+        const int vectors = p.q_heads * chunks;
+        for (int i = (int)(job % q_waves) * 64 + ((int)threadIdx.x & 63); i < vectors; i += q_waves * 64) {
+            const int head = i / chunks, ch = i - head * chunks;
+            const v8f_q y = load_turned<T>((const T*)p.q + row * p.q_row + head * p.q_head, ch, angles, p.rotary, p.interleaved);
+            *reinterpret_cast<vecT*>((T*)p.q_out + (row * p.q_heads + head) * D + 8 * ch) = __builtin_convertvector(y, vecT);
         }
-        const int first = clamp_row(c.indptr[lo], c.rows), end = clamp_row(c.indptr[lo + 1], c.rows);
-        if (row < first || row >= end) return;  // a row of no sequence: left as it was
-        const int64_t position = (int64_t)max(c.lens[lo], 0) - (end - row);
-        const float* angles = p.rope + (int64_t)min(max(position, (int64_t)0), (int64_t)p.rope_rows - 1) * p.rotary;
-        const v8f_q y = load_turned<T>((const T*)p.q + row * p.q_row + head * p.q_head, ch, angles, p.rotary, p.interleaved);
-        typedef T vecT __attribute__((ext_vector_type(8)));
-        *reinterpret_cast<vecT*>((T*)p.q_out + (row64 * p.q_heads + head) * D + 8 * ch) = __builtin_convertvector(y, vecT);
         return;
     }
-    extern __shared__ uint8_t lds[];  // v: the page's new codes, an element's tokens together, rows of v_pad bytes
+    extern __shared__ uint8_t all_lds[];  // v: the page's new codes, an element's tokens together, rows of v_pad bytes
     __shared__ float part[4];
-    const int half = (int)blockIdx.x & 1, unit = (int)blockIdx.x >> 1, head = unit % c.heads;
-    const SeqItem f = find_sequence(c, unit / c.heads, 1, P, 2);
+    const int unit = WAVES == 1 ? (int)blockIdx.x * 4 + wave : (int)blockIdx.x, tid = (int)threadIdx.x & (LANES - 1);
+    uint8_t* lds = all_lds + (WAVES == 1 ? wave * D * v_pad : 0);
+    const int half = unit & 1, head = (unit >> 1) % c.heads, item = (unit >> 1) / c.heads;
+    if (item >= items) return;
+    const SeqItem f = find_sequence(c, item, 1, P, 2);
     if (f.seq < 0) return;
     const int64_t len = f.len, start = len - f.n;  // position of the sequence's first new token
     const int64_t first = start > 0 ? start : 0, page_index = (first >> c.page_log2) + f.item;
@@ -98,62 +112,77 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendParams p, 
     const int slot0 = (int)(first > page_begin ? first - page_begin : 0);
     const int slot1 = (int)min(len - page_begin, (int64_t)P);
     if (slot0 >= slot1) return;
-    const int page = c.table[(int64_t)f.seq * c.width + page_index];
+    const int page = uniform_load(c.table + (int64_t)f.seq * c.width + page_index);
     if (page < 0 || page >= c.pages) return;
     const int64_t block = (int64_t)page * c.heads + head;
     float* scale_at = (half ? c.v_scale : c.k_scale) + block;
     uint8_t* codes = (half ? c.v : c.k) + block * ((int64_t)P * D);
     float old = 0.f;
     if (slot0 > 0) old = *scale_at;
-    if (!(old > 0.f && old <= 0x1p100f)) old = 0.f;  // no scale that a write leaves: the earlier slots hold nothing
     // rows of the packed input, and table rows, of the page's first slot on
     const int64_t row0 = f.first + (page_begin - start);
     const T* x = half ? (const T*)p.v + head * p.v_head : (const T*)p.k + head * p.k_head;
     const int64_t x_row = half ? p.v_row : p.k_row;
     const int rotary = half || !p.rope ? 0 : p.rotary;
-    const int count = (slot1 - slot0) * chunks;
+    const int chunks_log2 = 31 - __clz(chunks), count = (slot1 - slot0) << chunks_log2;
     auto element = [&](int i) {
-        const int slot = slot0 + i / chunks, ch = i % chunks;
+        const int slot = slot0 + (i >> chunks_log2), ch = i & (chunks - 1);
         const int64_t position = min(page_begin + slot, (int64_t)p.rope_rows - 1);
         return load_turned<T>(x + (row0 + slot) * x_row, ch, rotary ? p.rope + position * p.rotary : nullptr, rotary, p.interleaved);
     };
+    // a lane's first vector stays in a register, the others are loaded again (held too, they cost more in waves per compute unit
+    // than the second, cached, load: 4096 tokens 25 us, with two held 24.5 to 28, with four 33)
+    v8f_q held = {};
+    if (tid < count) held = element(tid);
     float amax = 0.f;
-    for (int i = tid; i < count; i += 256) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(held[k]));
+    for (int i = tid + LANES; i < count; i += LANES) {
         const v8f_q v = element(i);
 #pragma unroll
         for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(v[k]));
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) amax = fmaxf(amax, __shfl_xor(amax, d));
-    if (tid % 64 == 0) part[tid / 64] = amax;
-    __syncthreads();  // (and every lane has read the old scale)
-    amax = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+    if constexpr (WAVES > 1) {
+        if (tid % 64 == 0) part[wave] = amax;
+        __syncthreads();  // (and every lane has read the old scale)
+        amax = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+    }
+    if (!(old > 0.f && old <= 0x1p100f)) old = 0.f;  // no scale that a write leaves: the earlier slots hold nothing
     const float scale = fmaxf(page_scale(amax), old), inverse = 1.0f / scale;
     if (tid == 0) *scale_at = scale;
     if (slot0 > 0 && scale != old) {  // the earlier tokens' codes move to the new scale
         const float move = old * inverse;
         const int n = slot0 * D;
-        for (int i = tid; i < n; i += 256) {
+        for (int i = tid; i < n; i += LANES) {
             uint8_t* at = half ? codes + (i / slot0) * P + i % slot0 : codes + i;
             *at = old == 0.f ? 0 : (uint8_t)to_e4m3x4(e4m3_to_f32(*at) * move, 0.f, 0.f, 0.f);
         }
     }
-    for (int i = tid; i < count; i += 256) {
-        const v8f_q v = element(i) * inverse;
+    // v: a few tokens byte by byte, many turned through LDS
+    const bool few = slot1 - slot0 <= 8;
+    auto write = [&](int i, v8f_q v) {
+        v *= inverse;
         const uint32_t w0 = to_e4m3x4(v[0], v[1], v[2], v[3]), w1 = to_e4m3x4(v[4], v[5], v[6], v[7]);
-        const int slot = slot0 + i / chunks, ch = i % chunks;
+        const int slot = slot0 + (i >> chunks_log2), ch = i & (chunks - 1);
         if (!half) {
             *reinterpret_cast<v2i*>(codes + slot * D + 8 * ch) = v2i{(int)w0, (int)w1};
+        } else if (few) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) codes[(8 * ch + k) * P + slot] = (uint8_t)((k < 4 ? w0 : w1) >> (8 * (k & 3)));
         } else {
 #pragma unroll
             for (int k = 0; k < 8; ++k) lds[(8 * ch + k) * v_pad + slot] = (uint8_t)((k < 4 ? w0 : w1) >> (8 * (k & 3)));
         }
-    }
-    if (half) {
-        __syncthreads();
-        const int words = P / 4;
-        for (int i = tid; i < D * words; i += 256) {
-            const int d = i / words, s = 4 * (i % words);
+    };
+    if (tid < count) write(tid, held);
+    for (int i = tid + LANES; i < count; i += LANES) write(i, element(i));
+    if (half && !few) {
+        lds_written<WAVES>();
+        const int words_log2 = c.page_log2 - 2;
+        for (int i = tid; i < D << words_log2; i += LANES) {
+            const int d = i >> words_log2, s = 4 * (i & (P / 4 - 1));
             if (s + 4 <= slot0 || s >= slot1) continue;
             const uint32_t w = *reinterpret_cast<const uint32_t*>(lds + d * v_pad + s);
             if (s >= slot0 && s + 4 <= slot1) {
@@ -272,19 +301,30 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvReadParams p) {
 
 }  // namespace
 
-// Items that can begin: sum over sequences of ceil(n / P) (+ 1 where a run may begin inside a page), see find_sequence.
-hipError_t run_kv_append(const KvAppendParams& p, bool is_bf16, hipStream_t s) {
+template <typename T>
+static hipError_t launch_kv_append(const KvAppendParams& p, hipStream_t s) {
     const KvCache& c = p.c;
-    if (c.rows <= 0 || c.batch <= 0) return hipSuccess;
-    const int64_t P = (int64_t)1 << c.page_log2, items = c.rows / P + 2 * (int64_t)c.batch;
-    const int64_t q_blocks = p.q ? ((int64_t)c.rows * p.q_heads * (c.dim / 8) + 255) / 256 : 0, blocks = items * c.heads * 2 + q_blocks;
-    if (blocks > INT32_MAX) return hipErrorInvalidValue;
+    const int64_t P = (int64_t)1 << c.page_log2, items = c.rows / P + 2 * (int64_t)c.batch, units = items * c.heads * 2;
+    // one wave per page where sequences have up to four new tokens on average
+    const bool single = c.rows <= 4 * (int64_t)c.batch;
+    const int64_t cache_blocks = single ? (units + 3) / 4 : units;
+    // q: as many waves for a token as it has 64 vectors, fewer once that makes 8192 in all
+    const int64_t vectors = (int64_t)p.q_heads * (c.dim / 8);
+    const int64_t q_waves = p.q ? std::max<int64_t>(1, std::min<int64_t>((vectors + 63) / 64, 8192 / c.rows)) : 1;
+    const int64_t blocks = cache_blocks + (p.q ? (c.rows * q_waves + 3) / 4 : 0);
+    if (blocks > INT32_MAX || items > INT32_MAX) return hipErrorInvalidValue;
     const int v_pad = (int)P + 4;
     const dim3 grid((unsigned)blocks), block(256);
-    const size_t lds = (size_t)c.dim * v_pad;
-    if (is_bf16) hipLaunchKernelGGL(kv_append_kernel<__bf16>, grid, block, lds, s, p, (int)items, v_pad);
-    else hipLaunchKernelGGL(kv_append_kernel<_Float16>, grid, block, lds, s, p, (int)items, v_pad);
+    const size_t lds = (size_t)c.dim * v_pad * (single ? 4 : 1);
+    if (single) hipLaunchKernelGGL((kv_append_kernel<T, 1>), grid, block, lds, s, p, (int)items, (int)cache_blocks, v_pad, (int)q_waves);
+    else hipLaunchKernelGGL((kv_append_kernel<T, 4>), grid, block, lds, s, p, (int)items, (int)cache_blocks, v_pad, (int)q_waves);
     return hipGetLastError();
+}
+
+// Items that can begin: sum over sequences of ceil(n / P) (+ 1 where a run may begin inside a page), see find_sequence.
+hipError_t run_kv_append(const KvAppendParams& p, bool is_bf16, hipStream_t s) {
+    if (p.c.rows <= 0 || p.c.batch <= 0) return hipSuccess;
+    return is_bf16 ? launch_kv_append<__bf16>(p, s) : launch_kv_append<_Float16>(p, s);
 }
 
 hipError_t run_kv_read(const KvReadParams& p, int out_type, hipStream_t s) {
