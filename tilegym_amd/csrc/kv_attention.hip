@@ -22,22 +22,14 @@
 #include <algorithm>
 #include <type_traits>
 
-#ifdef TG_NOFENCE
-#define TG_FENCE
-#else
-#define TG_FENCE __builtin_amdgcn_sched_barrier(0)
-#endif
-#ifndef TG_DOCC
-#define TG_DOCC 3
-#endif
-#ifndef TG_OCC
-#define TG_OCC 2
-#endif
 #ifndef TG_WANT
-#define TG_WANT 2304
+#define TG_WANT 256
 #endif
 #ifndef TG_WANT2
-#define TG_WANT2 768
+#define TG_WANT2 512
+#endif
+#ifndef TG_LF
+#define TG_LF
 #endif
 namespace tg {
 namespace {
@@ -74,7 +66,7 @@ __device__ __forceinline__ typename Types<T>::v8 widen(int lo, int hi) {
 }
 
 constexpr int kMostSplits = 64;
-constexpr int kLeastSteps = 4;  // of a split
+constexpr int kLeastSteps = 8;  // of a split
 // A load through the vector path whatever the address is
 template <typename X>
 __device__ __forceinline__ X vector_load(const X* at) {
@@ -116,9 +108,8 @@ struct RowTile {
     __device__ __forceinline__ int key_of(int step) const { return (step < sink_steps ? step : (key0 >> 6) + step - sink_steps) * 64; }
 };
 
-__device__ __forceinline__ bool find_tile(const KvAttentionParams& p, int tile_rows, int item, int head, RowTile& t) {
+__device__ __forceinline__ bool set_tile(const KvAttentionParams& p, const SeqItem& f, int tile_rows, int head, RowTile& t) {
     const KvCache& c = p.c;
-    const SeqItem f = find_sequence(c, item, p.group, tile_rows, 1);
     if (f.seq < 0) return false;
     const int64_t r0 = (int64_t)f.item * tile_rows, total = (int64_t)f.n * p.group;
     if (r0 >= total) return false;
@@ -255,19 +246,28 @@ __device__ __forceinline__ typename Types<T>::v8 load_q(const T* at, bool negati
 // k's scale and the softmax factor; never zero, so that what is not seen stays at -inf
 __device__ __forceinline__ float score_factor(float k_scale, float scale_log2) { return fmaxf(fabsf(k_scale * scale_log2), 0x1p-126f); }
 
-// Few rows: four waves, 16 NT rows; the waves take the steps of the workgroup's share in turn and join at the end.  Codes come straight
+// Few rows: eight waves (four with 256 elements, which take the registers of two), 16 NT rows; the waves take the steps of the workgroup's share in turn and join at the end.  Codes come straight
 // from memory into registers, k's of the next step being asked for when this step's are used up, v's likewise.
+template <int D>
+constexpr int kFewWaves = D == 256 ? 4 : 8;
 // ONE: pages hold whole steps (64 or 128 tokens), so a step's page, its scales and its address are scalars.
 template <typename T, int D, int NT, bool ONE>
-__global__ void __launch_bounds__(256, D == 256 ? 1 : NT == 1 && ONE ? TG_DOCC : 2) kv_attention_kernel(const KvAttentionParams p) {
+__global__ void __launch_bounds__(64 * kFewWaves<D>, D == 256 ? 1 : 2) kv_attention_kernel(const KvAttentionParams p) {
     typedef typename Types<T>::v8 v8;
-    constexpr int CH = D / 64, DT = D / 16, ROWS = 16 * NT;  // 64-element chunks of a key, 16-element tiles of a value
+    constexpr int WAVES = kFewWaves<D>, CH = D / 64, DT = D / 16, ROWS = 16 * NT;  // 64-element chunks of a key, 16-element tiles of a value
     const KvCache& c = p.c;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, g = lane >> 4;
     const int split = (int)blockIdx.x % p.splits, rest = (int)blockIdx.x / p.splits;
     RowTile t;
-    if (!find_tile(p, ROWS, rest / c.heads, rest % c.heads, t)) return;
-    const int share = max((t.steps + p.splits - 1) / p.splits, kLeastSteps);
+    {
+        __shared__ int ranks[WAVES][64];
+        SeqItem f;
+        f.item = -1;
+        if (p.longest_first) f = find_longest<WAVES>(c, rest / c.heads, p.group, ROWS, ranks);
+        if (f.item < 0) f = find_sequence(c, rest / c.heads, p.group, ROWS, 1);
+        if (!set_tile(p, f, ROWS, rest % c.heads, t)) return;
+    }
+    const int share = p.splits == 1 ? t.steps : max((t.steps + p.splits - 1) / p.splits, kLeastSteps);
     const int begin = min(split * share, t.steps), end = min(begin + share, t.steps);
 
     const int P = 1 << c.page_log2, in_page = P - 1, head_bytes = P * D;
@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : NT == 1 && ONE ? TG_DOCC :
     if (mine < end) {
         load_k(mine);
         load_v(mine);
-        load_pages(mine + 4);
+        load_pages(mine + WAVES);
     }
     v4f o[NT][DT];
 #pragma unroll
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : NT == 1 && ONE ? TG_DOCC :
         for (int d = 0; d < DT; ++d) o[n][d] = v4f{0.f, 0.f, 0.f, 0.f};
     Unit unit;
 
-    for (int step = mine; step < end; step += 4) {
+    for (int step = mine; step < end; step += WAVES) {
         const int key = t.key_of(step), first = key + 16 * g;
         Scores16 s[NT];
 #pragma unroll
@@ -376,7 +376,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : NT == 1 && ONE ? TG_DOCC :
             }
         }
         const float factor = score_factor(k_scale, p.scale_log2);
-        if (step + 4 < end) load_k(step + 4);
+        if (step + WAVES < end) load_k(step + WAVES);
         // every key of the step seen by every row: nothing to select
         const bool whole = key + 63 <= t.low && (!p.window || key > t.high - p.window) && __ballot(!there.there) == 0;
         unit.step(v_scale, whole || (there.there && first < t.key1 && (first + 16 > t.key0 || first < p.sinks)));
@@ -409,15 +409,15 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : NT == 1 && ONE ? TG_DOCC :
                 o[n][d] = mfma16(b, pt[n][1], o[n][d]);
             }
         }
-        if (step + 4 < end) {
-            load_v(step + 4);
-            load_pages(step + 8);
+        if (step + WAVES < end) {
+            load_v(step + WAVES);
+            load_pages(step + 2 * WAVES);
         }
     }
 
-    // the four waves' results: m, l and u, then O, each in units of the largest
-    __shared__ float part_m[4][ROWS], part_l[4][ROWS], part_u[4];
-    __shared__ float part_o[4][16][D + 4];
+    // the waves' results: m, l and u, then O, each in units of the largest
+    __shared__ float part_m[WAVES][ROWS], part_l[WAVES][ROWS], part_u[WAVES];
+    __shared__ float part_o[WAVES][16][D + 4];
     if (lane == 0) part_u[wave] = unit.u;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -430,23 +430,23 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : NT == 1 && ONE ? TG_DOCC :
         __syncthreads();
         float top = part_m[0][n * 16 + col], u = part_u[0];
 #pragma unroll
-        for (int w = 1; w < 4; ++w) top = fmaxf(top, part_m[w][n * 16 + col]), u = fmaxf(u, part_u[w]);
+        for (int w = 1; w < WAVES; ++w) top = fmaxf(top, part_m[w][n * 16 + col]), u = fmaxf(u, part_u[w]);
         const float base = top == kMinusInf ? 0.f : top, f = __builtin_amdgcn_exp2f(m[n] - base) * (unit.u / u);
 #pragma unroll
         for (int d = 0; d < DT; ++d) *reinterpret_cast<v4f*>(&part_o[wave][col][d * 16 + 4 * g]) = o[n][d] * f;
         __syncthreads();
         constexpr int QUADS = D / 4;
         const int rows = min(t.rows - n * 16, 16);
-        for (int i = tid; i < rows * QUADS; i += 256) {
+        for (int i = tid; i < rows * QUADS; i += 64 * WAVES) {
             const int row = i / QUADS, e = 4 * (i % QUADS), rr = t.r0 + n * 16 + row;
             float row_top = part_m[0][n * 16 + row];
 #pragma unroll
-            for (int w = 1; w < 4; ++w) row_top = fmaxf(row_top, part_m[w][n * 16 + row]);
+            for (int w = 1; w < WAVES; ++w) row_top = fmaxf(row_top, part_m[w][n * 16 + row]);
             const float row_base = row_top == kMinusInf ? 0.f : row_top;
             float sum = 0.f;
             v4f x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
+            for (int w = 0; w < WAVES; ++w) {
                 sum += part_l[w][n * 16 + row] * __builtin_amdgcn_exp2f(part_m[w][n * 16 + row] - row_base);
                 x += *reinterpret_cast<const v4f*>(&part_o[w][row][e]);
             }
@@ -480,7 +480,7 @@ __device__ __forceinline__ int k_swizzle(int key) {
 __device__ __forceinline__ int v_swizzle(int row) { return (((row >> 1) ^ (row >> 3)) & 1) + 2 * ((row >> 2) & 1); }
 
 template <typename T, int D, bool ONE>
-__global__ void __launch_bounds__(256, D == 256 ? 1 : TG_OCC) kv_attention_rows_kernel(const KvAttentionParams p, int items) {
+__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_rows_kernel(const KvAttentionParams p, int items) {
     typedef typename Types<T>::v8 v8;
     constexpr int CH = D / 32, DT = D / 32, LOADS = D / 64, KCH = D / 16;  // 32-element chunks of a key, 32-element tiles of a value
     __shared__ __align__(16) uint8_t lds_k[2][64 * D], lds_v[2][64 * D];
@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : TG_OCC) kv_attention_rows_
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, h = lane >> 5;
     const int head = (int)blockIdx.x % c.heads, rest = (int)blockIdx.x / c.heads, split = rest % p.splits;
     RowTile t;
-    if (!find_tile(p, 128, items - 1 - rest / p.splits, head, t)) return;  // (the last rows of a sequence, which see most, first)
+    if (!set_tile(p, find_sequence(c, items - 1 - rest / p.splits, p.group, 128, 1), 128, head, t)) return;  // (the last rows of a sequence, which see most, first)
     const int share = max((t.steps + p.splits - 1) / p.splits, kLeastSteps);
     const int begin = min(split * share, t.steps), end = min(begin + share, t.steps);
 
@@ -603,7 +603,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : TG_OCC) kv_attention_rows_
         auto read_k = [&](int half) {
 #pragma unroll
             for (int ch = 0; ch < CH; ++ch) kc[ch] = *reinterpret_cast<const v4i*>(&lds_k[0][0] + (k_first ^ (ch * 32)) + half * 32 * D);
-            if constexpr (D < 256) TG_FENCE;
+            if constexpr (D < 256) __builtin_amdgcn_sched_barrier(0);
         };
         read_k(0);
 #pragma unroll
@@ -621,7 +621,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : TG_OCC) kv_attention_rows_
             for (int d = 0; d < DT; ++d) {
                 vc[d] = *reinterpret_cast<const v4i*>(&lds_v[0][0] + (v_first ^ (half * 32)) + d * 32 * 64);
             }
-            if constexpr (D < 256) TG_FENCE;
+            if constexpr (D < 256) __builtin_amdgcn_sched_barrier(0);
             bool whole = key_h <= last_whole && key_h > first_whole;
             if constexpr (ONE) {
                 whole = whole && page_there[0];
@@ -679,8 +679,8 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : TG_OCC) kv_attention_rows_
     }
 }
 
-// out = sum over splits of exp2(m_s - m) O_s, over the sum of exp2(m_s - m) l_s, in the order of the splits: D / 4 lanes per row of q.  The factors first,
-// all splits' m and l asked for at once; then O, four splits in flight.  Parts with no weight were not written.
+// out = sum over splits of exp2(m_s - m) O_s, over the sum of exp2(m_s - m) l_s, in the order of the splits: D / 4 lanes per row of q.  All
+// splits' m and l, and the first four parts of O, are asked for at once; then O, four in flight.  Parts with no weight were not written.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv_attention_join_kernel(const KvAttentionParams p) {
     constexpr int QUADS = D / 4, ROWS = 256 / QUADS;
@@ -690,6 +690,14 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const KvAttentio
     const int token = (int)(min(row, rows - 1) / p.q_heads);
     // rows of no sequence are left as they were
     const bool live = row < rows && token >= clamp_row(p.c.indptr[0], p.c.rows) && token < clamp_row(p.c.indptr[p.c.batch], p.c.rows);
+    const float* part_at = p.part_o + row * D + 4 * lane;
+    const int64_t part_step = rows * D;
+    v4f part[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        part[i] = v4f{0.f, 0.f, 0.f, 0.f};
+        if (live && i < p.splits) part[i] = *reinterpret_cast<const v4f*>(part_at + i * part_step);
+    }
     constexpr int EACH = kMostSplits / QUADS > 0 ? kMostSplits / QUADS : 1;
     float m[EACH], l[EACH], top = kMinusInf, sum = 0.f;
 #pragma unroll
@@ -714,14 +722,13 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const KvAttentio
     if (!live) return;
     v4f x = {0.f, 0.f, 0.f, 0.f};
     for (int s0 = 0; s0 < p.splits; s0 += 4) {
-        v4f part[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            part[i] = v4f{0.f, 0.f, 0.f, 0.f};
-            if (s0 + i < p.splits && weight[tid / QUADS][s0 + i] > 0.f) part[i] = *reinterpret_cast<const v4f*>(p.part_o + ((s0 + i) * rows + row) * D + 4 * lane);
+            const float f = s0 + i < p.splits ? weight[tid / QUADS][s0 + i] : 0.f;
+            if (f > 0.f) x += f * part[i];
+            // the next four: a part without weight may hold anything and is left out by selection
+            if (s0 + 4 + i < p.splits) part[i] = *reinterpret_cast<const v4f*>(part_at + (s0 + 4 + i) * part_step);
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x += (s0 + i < p.splits ? weight[tid / QUADS][s0 + i] : 0.f) * part[i];
     }
     typedef T v4t __attribute__((ext_vector_type(4)));
     x *= sum > 0.f ? 1.0f / sum : 0.f;
@@ -738,23 +745,27 @@ int tile_rows_of(const KvAttentionParams& p) {
 }
 
 template <typename T, int D>
-hipError_t launch(const KvAttentionParams& p, hipStream_t s) {
+hipError_t launch(KvAttentionParams p, hipStream_t s) {
     const int tile_rows = tile_rows_of(p);
     const int64_t tiles = row_tiles(p, tile_rows), blocks = tiles * p.c.heads * p.splits;
     const int64_t join = ((int64_t)p.c.rows * p.q_heads * (D / 4) + 255) / 256;
     if (blocks > INT32_MAX || join > INT32_MAX) return hipErrorInvalidValue;
     const dim3 grid((unsigned)blocks), block(256);
+    // more workgroups than compute units, whole sequences each: the long ones first, and the short ones fill in behind them
+    p.longest_first = tile_rows == 16 && p.splits == 1 && p.c.batch <= 64 && p.c.batch > 1 && blocks > 256 TG_LF;
     const bool one = p.c.page_log2 >= 6;
+#define TG_FEW(NT, ONE) hipLaunchKernelGGL((kv_attention_kernel<T, D, NT, ONE>), grid, dim3(64 * kFewWaves<D>), 0, s, p)
     if (tile_rows == 128) {
         if (one) hipLaunchKernelGGL((kv_attention_rows_kernel<T, D, true>), grid, block, 0, s, p, (int)tiles);
         else hipLaunchKernelGGL((kv_attention_rows_kernel<T, D, false>), grid, block, 0, s, p, (int)tiles);
     } else if (tile_rows == 16) {
-        if (one) hipLaunchKernelGGL((kv_attention_kernel<T, D, 1, true>), grid, block, 0, s, p);
-        else hipLaunchKernelGGL((kv_attention_kernel<T, D, 1, false>), grid, block, 0, s, p);
+        if (one) TG_FEW(1, true);
+        else TG_FEW(1, false);
     } else if constexpr (D != 256) {
-        if (one) hipLaunchKernelGGL((kv_attention_kernel<T, D, 2, true>), grid, block, 0, s, p);
-        else hipLaunchKernelGGL((kv_attention_kernel<T, D, 2, false>), grid, block, 0, s, p);
+        if (one) TG_FEW(2, true);
+        else TG_FEW(2, false);
     }
+#undef TG_FEW
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
     hipLaunchKernelGGL((kv_attention_join_kernel<T, D>), dim3((unsigned)join), block, 0, s, p);
@@ -763,17 +774,13 @@ hipError_t launch(const KvAttentionParams& p, hipStream_t s) {
 
 }  // namespace
 
-// Workgroups to spread the keys of a call over.  Few rows (768 at a time on the chip): three rounds, so that sequences of uneven length fill it
-// (64 sequences of 100 to 8000 tokens, 8 heads of 128: 116 us with 768, 115 with 1536, 112 with 2304, 112 with 4096, without splits 124).
-// The other forms: a round and a half; their results are larger against their keys (5 new tokens in 16 sequences of 500 to 4000: 36 us with 256, 30
-// with 512, 29 with 768, 35 with 1536, 40 with 2304).
 int kv_attention_splits(const KvAttentionParams& p) {
     const int tile_rows = tile_rows_of(p);
     const int64_t units = row_tiles(p, tile_rows) * p.c.heads;
     int64_t keys = (int64_t)p.c.width << p.c.page_log2;
     if (p.window) keys = std::min<int64_t>(keys, (int64_t)p.window + 128 + (p.sinks + 63) / 64 * 64);
-    const int64_t steps = (keys + 63) / 64, workgroups = tile_rows == 16 ? TG_WANT : TG_WANT2;
-    const int64_t wanted = (workgroups + units - 1) / units, most = (steps + kLeastSteps - 1) / kLeastSteps;
+    const int64_t steps = (keys + 63) / 64, workgroups = tile_rows != 128 ? TG_WANT : TG_WANT2;
+    const int64_t wanted = (workgroups + units / 2) / units, most = (steps + kLeastSteps - 1) / kLeastSteps;
     return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(wanted, most), kMostSplits));
 }
 

@@ -48,6 +48,38 @@ __device__ __forceinline__ SeqItem find_sequence(const KvCache& c, int item, int
     return f;
 }
 
+// find_sequence for at most 64 sequences of at most one item each, the longest sequence first (of equal ones the first): item -1 where
+// some sequence has more than one.  A lane's sequence is ranked by comparison with all others, a share of them in each of the
+// workgroup's waves (WAVES; all of them call this).  part: LDS.
+template <int WAVES>
+__device__ __forceinline__ SeqItem find_longest(const KvCache& c, int item, int num, int den, int (*part)[64]) {
+    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), at = min(lane, c.batch - 1);
+    const int first = clamp_row(c.indptr[at], c.rows), n = clamp_row(c.indptr[at + 1], c.rows) - first, len = max(c.lens[at], 0);
+    int rank = 0;
+#pragma unroll
+    for (int i = 0; i < 64 / WAVES; ++i) {
+        const int b = wave * (64 / WAVES) + i, other = __builtin_amdgcn_readlane(len, b);
+        rank += b < c.batch && (other > len || (other == len && b < lane)) ? 1 : 0;
+    }
+    part[wave][lane] = rank;
+    __syncthreads();
+    rank = 0;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) rank += part[i][lane];
+    SeqItem f;
+    f.seq = -1, f.first = f.n = f.item = f.len = 0;
+    if (__ballot((int64_t)n * num > den)) {
+        f.item = -1;
+        return f;
+    }
+    const uint64_t found = __ballot(lane < c.batch && rank == item);
+    if (!found) return f;
+    f.seq = __ffsll((unsigned long long)found) - 1;
+    f.first = __builtin_amdgcn_readlane(first, f.seq), f.n = __builtin_amdgcn_readlane(n, f.seq), f.len = __builtin_amdgcn_readlane(len, f.seq);
+    if (f.n <= 0) f.seq = -1;
+    return f;
+}
+
 // A value that all lanes have alike, through the scalar cache: it is then not counted among the vector loads in flight
 __device__ __forceinline__ int uniform_load(const int* at) { return *(const __attribute__((address_space(4))) int*)(uintptr_t)at; }
 __device__ __forceinline__ float uniform_load(const float* at) { return *(const __attribute__((address_space(4))) float*)(uintptr_t)at; }

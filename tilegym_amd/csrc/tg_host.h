@@ -174,6 +174,7 @@ struct KvAttentionParams {
     int q_heads, group;                // group = q_heads / heads
     float scale_log2;                  // softmax scale * log2(e)
     int window, sinks;                 // window 0: all earlier positions
+    int longest_first;                 // up to 64 sequences: workgroups in the order of their lengths
     int splits;                        // > 1: partial results below, joined by a second launch
     float* part_o;                     // (splits, rows * q_heads, dim)
     float* part_ml;                    // (splits, rows * q_heads, 2): running maximum and sum
