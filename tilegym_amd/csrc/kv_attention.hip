@@ -780,7 +780,7 @@ int kv_attention_splits(const KvAttentionParams& p) {
     int64_t keys = (int64_t)p.c.width << p.c.page_log2;
     if (p.window) keys = std::min<int64_t>(keys, (int64_t)p.window + 128 + (p.sinks + 63) / 64 * 64);
     const int64_t steps = (keys + 63) / 64, workgroups = tile_rows != 128 ? TG_WANT : TG_WANT2;
-    const int64_t wanted = (workgroups + units / 2) / units, most = (steps + kLeastSteps - 1) / kLeastSteps;
+    const int64_t wanted = (workgroups + units / 2) / units, most = steps <= 2 * kLeastSteps ? 1 : (steps + kLeastSteps - 1) / kLeastSteps;
     return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(wanted, most), kMostSplits));
 }
 
