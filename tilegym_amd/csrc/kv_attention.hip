@@ -22,15 +22,6 @@
 #include <algorithm>
 #include <type_traits>
 
-#ifndef TG_WANT
-#define TG_WANT 256
-#endif
-#ifndef TG_WANT2
-#define TG_WANT2 512
-#endif
-#ifndef TG_LF
-#define TG_LF
-#endif
 namespace tg {
 namespace {
 
@@ -65,8 +56,10 @@ __device__ __forceinline__ typename Types<T>::v8 widen(int lo, int hi) {
     return __builtin_shufflevector(__builtin_shufflevector(a, b, 0, 1, 2, 3), __builtin_shufflevector(c, d, 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+constexpr int kComputeUnits = 256;
 constexpr int kMostSplits = 64;
 constexpr int kLeastSteps = 8;  // of a split
+
 // A load through the vector path whatever the address is
 template <typename X>
 __device__ __forceinline__ X vector_load(const X* at) {
@@ -107,6 +100,12 @@ struct RowTile {
     int steps, sink_steps;  // steps of 64 keys: sink_steps from 0 on, then from key0 / 64 on
     __device__ __forceinline__ int key_of(int step) const { return (step < sink_steps ? step : (key0 >> 6) + step - sink_steps) * 64; }
 };
+
+// Tiles of ROWS rows of a sequence with n new tokens.
+template <int ROWS>
+__device__ __forceinline__ auto tiles_of(int group) {
+    return [group](int n, int) { return (int)(((int64_t)n * group + ROWS - 1) / ROWS); };
+}
 
 __device__ __forceinline__ bool set_tile(const KvAttentionParams& p, const SeqItem& f, int tile_rows, int head, RowTile& t) {
     const KvCache& c = p.c;
@@ -264,7 +263,7 @@ __global__ void __launch_bounds__(64 * kFewWaves<D>, D == 256 ? 1 : 2) kv_attent
         SeqItem f;
         f.item = -1;
         if (p.longest_first) f = find_longest<WAVES>(c, rest / c.heads, p.group, ROWS, ranks);
-        if (f.item < 0) f = find_sequence(c, rest / c.heads, p.group, ROWS, 1);
+        if (f.item < 0) f = find_sequence(c, rest / c.heads, tiles_of<ROWS>(p.group));
         if (!set_tile(p, f, ROWS, rest % c.heads, t)) return;
     }
     const int share = p.splits == 1 ? t.steps : max((t.steps + p.splits - 1) / p.splits, kLeastSteps);
@@ -465,9 +464,9 @@ __global__ void __launch_bounds__(64 * kFewWaves<D>, D == 256 ? 1 : 2) kv_attent
     }
 }
 
-// Many rows: 128 of them per workgroup, 32 per wave, and every wave runs over the same keys, whose codes are staged in LDS for all
-// four: 16 bytes per lane and load through registers, the next step's while this one's products run, in two buffers with one
-// barrier a step.  Codes stay e4m3 in LDS (half the reads that 16 bits would cost) and are widened behind each read, for 32 rows.
+// Many rows: 128 of them per workgroup, 32 per wave, and every wave runs over the same keys, whose codes go to LDS for all four
+// without a register between, the next step's while this one's products run, in two buffers with one barrier a step.  Codes stay
+// e4m3 in LDS (half the reads that 16 bits would cost, 193 against 200 us) and are widened behind each read, for 32 rows.
 // The products are 32x32x16 instructions on 32 keys at a time, the same way round: S^T row 8 a + 4 h + b stands for key 16 h + 4 a + b, so a
 // lane (row lane % 32, h = lane / 32) has 16 consecutive keys of its one row.
 // 16-byte chunks lie in LDS so that the 8, and the 16, neighbouring lanes that read together cover different banks: chunk ^ f,
@@ -480,7 +479,7 @@ __device__ __forceinline__ int k_swizzle(int key) {
 __device__ __forceinline__ int v_swizzle(int row) { return (((row >> 1) ^ (row >> 3)) & 1) + 2 * ((row >> 2) & 1); }
 
 template <typename T, int D, bool ONE>
-__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_rows_kernel(const KvAttentionParams p, int items) {
+__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_rows_kernel(const KvAttentionParams p) {
     typedef typename Types<T>::v8 v8;
     constexpr int CH = D / 32, DT = D / 32, LOADS = D / 64, KCH = D / 16;  // 32-element chunks of a key, 32-element tiles of a value
     __shared__ __align__(16) uint8_t lds_k[2][64 * D], lds_v[2][64 * D];
@@ -488,7 +487,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_rows_kerne
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, h = lane >> 5;
     const int head = (int)blockIdx.x % c.heads, rest = (int)blockIdx.x / c.heads, split = rest % p.splits;
     RowTile t;
-    if (!set_tile(p, find_sequence(c, items - 1 - rest / p.splits, p.group, 128, 1), 128, head, t)) return;  // (the last rows of a sequence, which see most, first)
+    if (!set_tile(p, find_sequence(c, rest / p.splits, tiles_of<128>(p.group), true), 128, head, t)) return;  // (the last rows of a sequence, which see most, first)
     const int share = max((t.steps + p.splits - 1) / p.splits, kLeastSteps);
     const int begin = min(split * share, t.steps), end = min(begin + share, t.steps);
 
@@ -735,7 +734,7 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const KvAttentio
     *reinterpret_cast<v4t*>((T*)p.out + row * D + 4 * lane) = __builtin_convertvector(x, v4t);
 }
 
-// Tiles that can begin: sum over sequences of ceil(n * group / tile_rows), see find_sequence.
+// Tiles there can be: sum over sequences of ceil(n * group / tile_rows) at most.
 int64_t row_tiles(const KvAttentionParams& p, int64_t tile_rows) { return (int64_t)p.c.rows * p.group / tile_rows + p.c.batch; }
 // Rows of a tile, by the rows that a sequence's key/value head has on average, as the host does not read the tensors: 16 or 32 in the form
 // for few rows, 128 in the one for many.
@@ -751,13 +750,14 @@ hipError_t launch(KvAttentionParams p, hipStream_t s) {
     const int64_t join = ((int64_t)p.c.rows * p.q_heads * (D / 4) + 255) / 256;
     if (blocks > INT32_MAX || join > INT32_MAX) return hipErrorInvalidValue;
     const dim3 grid((unsigned)blocks), block(256);
-    // more workgroups than compute units, whole sequences each: the long ones first, and the short ones fill in behind them
-    p.longest_first = tile_rows == 16 && p.splits == 1 && p.c.batch <= 64 && p.c.batch > 1 && blocks > 256 TG_LF;
+    // more workgroups than compute units, whole sequences each: the long ones first, and the short ones fill in behind them (64 sequences of 1
+    // to 8000 keys 98 us, in their own order 119)
+    p.longest_first = tile_rows == 16 && p.splits == 1 && p.c.batch <= 64 && p.c.batch > 1 && blocks > kComputeUnits;
     const bool one = p.c.page_log2 >= 6;
 #define TG_FEW(NT, ONE) hipLaunchKernelGGL((kv_attention_kernel<T, D, NT, ONE>), grid, dim3(64 * kFewWaves<D>), 0, s, p)
     if (tile_rows == 128) {
-        if (one) hipLaunchKernelGGL((kv_attention_rows_kernel<T, D, true>), grid, block, 0, s, p, (int)tiles);
-        else hipLaunchKernelGGL((kv_attention_rows_kernel<T, D, false>), grid, block, 0, s, p, (int)tiles);
+        if (one) hipLaunchKernelGGL((kv_attention_rows_kernel<T, D, true>), grid, block, 0, s, p);
+        else hipLaunchKernelGGL((kv_attention_rows_kernel<T, D, false>), grid, block, 0, s, p);
     } else if (tile_rows == 16) {
         if (one) TG_FEW(1, true);
         else TG_FEW(1, false);
@@ -776,10 +776,14 @@ hipError_t launch(KvAttentionParams p, hipStream_t s) {
 
 int kv_attention_splits(const KvAttentionParams& p) {
     const int tile_rows = tile_rows_of(p);
-    const int64_t units = row_tiles(p, tile_rows) * p.c.heads;
+    // Few rows: a tile for each sequence, as far as the host can tell, and a workgroup per compute unit (two do not fit its registers).
+    // Shares are cut only where compute units would be left over: 8 sequences of 8000 keys x 8 heads 27.6 us, uncut 48.6; 24 such 71,
+    // cut in two 78.  Many rows: two workgroups per compute unit.  No share below 8 steps, and none up to 1024 keys (8 x 1000 keys 11.5 us in
+    // one launch, 12.0 cut and joined).
+    const int64_t units = (tile_rows != 128 ? (int64_t)p.c.batch : row_tiles(p, tile_rows)) * p.c.heads;
     int64_t keys = (int64_t)p.c.width << p.c.page_log2;
-    if (p.window) keys = std::min<int64_t>(keys, (int64_t)p.window + 128 + (p.sinks + 63) / 64 * 64);
-    const int64_t steps = (keys + 63) / 64, workgroups = tile_rows != 128 ? TG_WANT : TG_WANT2;
+    if (p.window) keys = std::min<int64_t>(keys, (int64_t)p.window + 128 + ((int64_t)p.sinks + 63) / 64 * 64);
+    const int64_t steps = (keys + 63) / 64, workgroups = tile_rows != 128 ? kComputeUnits : 2 * kComputeUnits;
     const int64_t wanted = (workgroups + units / 2) / units, most = steps <= 2 * kLeastSteps ? 1 : (steps + kLeastSteps - 1) / kLeastSteps;
     return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(wanted, most), kMostSplits));
 }

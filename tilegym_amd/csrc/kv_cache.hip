@@ -83,11 +83,11 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendParams p, 
     if ((int)blockIdx.x >= cache_blocks) {
         // q: a wave has one token, and every q_waves-th 64 vectors of 8 elements of it
         const int64_t job = (int64_t)((int)blockIdx.x - cache_blocks) * 4 + wave;
-        const int64_t row = job / q_waves;
-        if (row >= c.rows) return;
-        const SeqItem f = find_sequence(c, (int)row, 1, 1, 0);
-        if (f.seq < 0 || f.item >= f.n) return;  // a row of no sequence: left as it was
-        const int64_t position = (int64_t)f.len - f.n + f.item;
+        // (the items are the rows that sequences have, in order; rows of no sequence are left as they were)
+        if (job / q_waves >= c.rows) return;
+        const SeqItem f = find_sequence(c, (int)(job / q_waves), [](int n, int) { return n; });
+        if (f.seq < 0 || f.item >= f.n) return;
+        const int64_t row = f.first + f.item, position = (int64_t)f.len - f.n + f.item;
         const float* angles = p.rope + min(max(position, (int64_t)0), (int64_t)p.rope_rows - 1) * p.rotary;
         const int vectors = p.q_heads * chunks;
         for (int i = (int)(job % q_waves) * 64 + ((int)threadIdx.x & 63); i < vectors; i += q_waves * 64) {
@@ -103,7 +103,8 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendParams p, 
     uint8_t* lds = all_lds + (WAVES == 1 ? wave * D * v_pad : 0);
     const int half = unit & 1, head = (unit >> 1) % c.heads, item = (unit >> 1) / c.heads;
     if (item >= items) return;
-    const SeqItem f = find_sequence(c, item, 1, P, 2);
+    // pages from the one of the first new token's position (or of the sequence's beginning) to the last's
+    const SeqItem f = find_sequence(c, item, [&](int n, int len) { return len > 0 ? ((len - 1) >> c.page_log2) - (max(len - n, 0) >> c.page_log2) + 1 : 0; });
     if (f.seq < 0) return;
     const int64_t len = f.len, start = len - f.n;  // position of the sequence's first new token
     const int64_t first = start > 0 ? start : 0, page_index = (first >> c.page_log2) + f.item;
@@ -232,7 +233,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvReadParams p) {
     const KvCache& c = p.c;
     const int tid = (int)threadIdx.x, P = 1 << c.page_log2, D = c.dim, chunks = D / 16;
     const int half = (int)blockIdx.x & 1, unit = (int)blockIdx.x >> 1, head = unit % c.heads;
-    const SeqItem f = find_sequence(c, unit / c.heads, 1, 64, 1);
+    const SeqItem f = find_sequence(c, unit / c.heads, [](int n, int) { return (n + 63) >> 6; });
     if (f.seq < 0) return;
     const int64_t begin = (int64_t)f.item * 64, capacity = (int64_t)c.width << c.page_log2;
     const int n = (int)min(min((int64_t)f.n, capacity) - begin, (int64_t)64);
@@ -304,7 +305,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvReadParams p) {
 template <typename T>
 static hipError_t launch_kv_append(const KvAppendParams& p, hipStream_t s) {
     const KvCache& c = p.c;
-    const int64_t P = (int64_t)1 << c.page_log2, items = c.rows / P + 2 * (int64_t)c.batch, units = items * c.heads * 2;
+    const int64_t P = (int64_t)1 << c.page_log2, items = c.rows / P + 2 * (int64_t)c.batch /* at most: ceil(n / P) + 1 each */, units = items * c.heads * 2;
     // one wave per page where sequences have up to four new tokens on average
     const bool single = c.rows <= 4 * (int64_t)c.batch;
     const int64_t cache_blocks = single ? (units + 3) / 4 : units;
@@ -321,7 +322,6 @@ static hipError_t launch_kv_append(const KvAppendParams& p, hipStream_t s) {
     return hipGetLastError();
 }
 
-// Items that can begin: sum over sequences of ceil(n / P) (+ 1 where a run may begin inside a page), see find_sequence.
 hipError_t run_kv_append(const KvAppendParams& p, bool is_bf16, hipStream_t s) {
     if (p.c.rows <= 0 || p.c.batch <= 0) return hipSuccess;
     return is_bf16 ? launch_kv_append<__bf16>(p, s) : launch_kv_append<_Float16>(p, s);

@@ -15,37 +15,62 @@ namespace tg {
 
 __device__ __forceinline__ int clamp_row(int x, int rows) { return min(max(x, 0), rows); }
 
-// Which sequence work item `item` belongs to.  Sequence b's items begin at floor(indptr[b] * num / den) + more * b; the caller
-// chooses num, den and more so that a sequence has at most as many items as lie between that and the next one's beginning, so no
-// prefix sum over the sequences is needed: the last beginning that is not above `item`, by a ballot over 64 sequences at a
-// time.  All lanes of a wave return the same.
 struct SeqItem {
     int seq;        // -1: none
     int first, n;   // rows of the packed inputs
     int item;       // item of the sequence
     int len;        // its length, not below zero (0 without lens)
 };
-// All that is asked for comes in one round of loads: the neighbouring entry and the length by the lane that then turns out to have them.
-__device__ __forceinline__ SeqItem find_sequence(const KvCache& c, int item, int num, int den, int more) {
+
+// Inclusive prefix sum over the lanes of a wave, by lane permutations inside the vector instructions.
+__device__ __forceinline__ int wave_prefix(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8: inside rows of 16
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast 15: a row's sum to the next, in rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast 31: the lower half's to the upper
+    return x;
+}
+
+// Which sequence work item `item` belongs to, where sequence b has count(n, len) items (n new rows of it, length len): 64 sequences at a time by a
+// prefix sum over the lanes.  Items are numbered without gaps: workgroups without work in between would keep later ones waiting for
+// the compute unit that they were dealt (256 workgroups of a compute unit each among 416: 29 us, without gaps 18).  from_end: item 0 is
+// the last.  All that is asked for comes in one round of loads.  All lanes of a wave return the same.
+template <typename Count>
+__device__ __forceinline__ SeqItem find_sequence(const KvCache& c, int item, Count count, bool from_end = false) {
     const int lane = (int)threadIdx.x & 63;
     SeqItem f;
     f.seq = -1, f.first = f.n = f.item = f.len = 0;
-    for (int base = 0; base < c.batch; base += 64) {
+    int first, n, len, items, prefix;
+    auto load = [&](int base, int before) {
         const int b = base + lane, at = min(b, c.batch - 1);
-        const int first = clamp_row(c.indptr[at], c.rows), end = clamp_row(c.indptr[at + 1], c.rows), len = c.lens ? c.lens[at] : 0;
-        const int begin = (int)((int64_t)first * num / den) + more * b;
-        const int count = __popcll(__ballot(b < c.batch && begin <= item));
-        if (count > 0) {
-            f.seq = base + count - 1;
-            f.first = __builtin_amdgcn_readlane(first, count - 1);
-            f.n = __builtin_amdgcn_readlane(end, count - 1) - f.first;
-            f.item = item - __builtin_amdgcn_readlane(begin, count - 1);
-            f.len = max(__builtin_amdgcn_readlane(len, count - 1), 0);
-        }
-        if (count < 64) break;
+        first = clamp_row(c.indptr[at], c.rows), n = clamp_row(c.indptr[at + 1], c.rows) - first, len = c.lens ? max(c.lens[at], 0) : 0;
+        items = b < c.batch && n > 0 ? count(n, len) : 0;
+        prefix = wave_prefix(items) + before;
+        return __builtin_amdgcn_readlane(prefix, 63);
+    };
+    int total = load(0, 0);
+    if (from_end) {
+        for (int base = 64; base < c.batch; base += 64) total = load(base, total);
+        item = total - 1 - item;
+        if (item < 0) return f;
+        if (c.batch > 64) total = load(0, 0);
     }
-    if (f.n <= 0 || f.item < 0) f.seq = -1;
-    return f;
+    for (int base = 0;;) {
+        if (item < total) {
+            const int found = __popcll(__ballot(prefix <= item));
+            f.item = item - (__builtin_amdgcn_readlane(prefix, found & 63) - __builtin_amdgcn_readlane(items, found & 63));
+            f.first = __builtin_amdgcn_readlane(first, found & 63), f.n = __builtin_amdgcn_readlane(n, found & 63);
+            f.len = __builtin_amdgcn_readlane(len, found & 63);
+            // (where indptr is no prefix sum, found may be anything: what it names is then checked against the tensors like the rest)
+            if (found < 64 && base + found < c.batch && f.item >= 0 && f.n > 0) f.seq = base + found;
+            return f;
+        }
+        base += 64;
+        if (base >= c.batch) return f;
+        total = load(base, total);
+    }
 }
 
 // find_sequence for at most 64 sequences of at most one item each, the longest sequence first (of equal ones the first): item -1 where
