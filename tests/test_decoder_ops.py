@@ -749,3 +749,144 @@ def test_two_graphs_share_no_scratch_memory(device):
                 graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+
+
+# ---------------------------------------------------------------------------- the forms that a call's sizes choose between
+def test_table_beyond_the_positions_is_refused_without_a_device():
+    a = {**_cache_args(page=128, batch=1), "table": torch.zeros(1, (1 << 23) + 1, dtype=torch.int32)}
+    assert _attention_rc(a) == -6 and _read_rc(a) == -6 and _append_rc({**a, "rope": None, "q": None, "out": None}) == -6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch", [33, 64, 70])
+@pytest.mark.parametrize("dim,heads", [(128, 8), (64, 9), (256, 10)])
+def test_attention_more_sequences_than_compute_units(device, batch, dim, heads):
+    """Whole sequences of very different lengths, some of them equal, empty or without new tokens; then one with many more rows than a tile."""
+    g = torch.Generator().manual_seed(batch)
+    lens = torch.randint(0, 150, (batch,), generator=g).tolist()
+    lens[3] = lens[4] = lens[-1] = 77
+    lens[5] = 0
+    news = [0 if n == 0 or b % 9 == 8 else 1 for b, n in enumerate(lens)]
+    pool = Pool(device, batch * 3, heads, 64, dim, batch, 3)
+    pool.fill(lens, lens)
+    _attend(pool, lens, news, 2, BF16)
+    lens[7], news[7] = 90, 21
+    pool.fill([90 if b == 7 else 0 for b in range(batch)], [90 if b == 7 else 0 for b in range(batch)])
+    _attend(pool, lens, news, 2, BF16)
+    _attend(pool, lens, news, 2, BF16, window=30, sinks=2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page,dim", [(16, 64), (32, 128), (64, 128), (128, 64), (64, 256), (128, 256), (16, 256)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("group,news", [(1, [1, 1]), (4, [4, 4]), (5, [5, 4]), (2, [70, 0]), (3, [150, 100])])
+def test_attention_split_contexts(device, page, dim, dtype, group, news):
+    """Every form of tile with its keys split over workgroups and joined."""
+    lens = [1700, 1100]
+    width = -(-2048 // page)
+    pool = Pool(device, 2 * width, 1, page, dim, 2, width)
+    pool.fill(lens, lens, dtype)
+    assert _lib.load().tg_fp8_kv_attention_workspace_bytes(sum(news), group, 2, 1, dim, page, width, 0, 0) > 0
+    _attend(pool, lens, news, group, dtype)
+    _attend(pool, lens, news, group, dtype, window=1100, sinks=130)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [16, 64])
+def test_attention_many_sequences_of_many_rows(device, page):
+    """More sequences than one prefix sum covers, each with more rows than a tile, a few with none."""
+    batch = 140
+    lens = [(7 * b) % 61 for b in range(batch)]
+    news = [max(0, n - 5) for n in lens]
+    width = -(-61 // page)
+    pool = Pool(device, batch * width, 1, page, 64, batch, width)
+    pool.fill(lens, lens)
+    _attend(pool, lens, news, 6, BF16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page,dim,heads", CACHES)
+def test_append_single_tokens_beside_a_chunk(device, page, dim, heads):
+    """Mostly one token a sequence, and one sequence with a chunk over a page's border: a wave writes each page."""
+    batch, chunk = 24, page + 19
+    pool = Pool(device, batch * 3, heads, page, dim, batch, 3)
+    rope = ops.rope_table(3 * page, dim, device="cpu")
+    lens = [(5 * b) % page for b in range(batch)]
+    pool.fill(lens, lens)
+    news = [1] * batch
+    news[2], news[11] = min(chunk, 4 * batch - 2 * batch), 0
+    lens = [a + b for a, b in zip(lens, news)]
+    assert sum(news) <= 4 * batch
+    pool.fill(lens, news, BF16, rope)
+    pool.check(True)
+
+
+@pytest.mark.gpu
+def test_call_paths_agree_and_refuse_alike(device, monkeypatch):
+    """The native and the ctypes path: the same bits, the same refusals of tensors elsewhere and of values out of range."""
+    lens, news = [100, 40], [3, 2]
+    pool = Pool(device, 8, 2, 64, 128, 2, 2)
+    pool.fill(lens, lens)
+    qkv = torch.randn(5, 8, 128, generator=pool.g).to(BF16).to(device)
+    q, k, v = qkv.split([4, 2, 2], 1)
+    rope = ops.rope_table(128, 64, device=device)
+    table, lens, indptr = pool.i32(pool.table), pool.i32(lens), pool.i32([0, 3, 5])
+    x, w = torch.randn(5, 256, generator=pool.g).to(BF16).to(device), torch.ones(256, dtype=BF16, device=device)
+
+    def run():
+        cache = ops.KVCache(*(t.clone() for t in pool.cache))
+        out = [ops.kv_cache_append(cache, k, v, table, lens, indptr, q=q, rope=rope), *cache]
+        out += [ops.kv_cache_attention(q, cache, table, lens, indptr), *ops.kv_cache_read(cache, table, indptr, 5), *ops.rms_norm_quant(x, w)]
+        errors = []
+        for call in (lambda: ops.kv_cache_append(cache, k, v.cpu(), table, lens, indptr), lambda: ops.kv_cache_append(cache, k, v, table, lens, indptr.cpu()),
+                     lambda: ops.kv_cache_append(cache, k, v, table, lens, indptr, q=q), lambda: ops.kv_cache_attention(q, cache, table.cpu(), lens, indptr),
+                     lambda: ops.kv_cache_attention(q, cache, table, lens, indptr, window=2 ** 31),
+                     lambda: ops.kv_cache_attention(q, cache, table, lens, indptr, window=4, sink_tokens=2 ** 31),
+                     lambda: ops.kv_cache_attention(q, cache, table, lens, indptr, sink_tokens=-1),
+                     lambda: ops.kv_cache_attention(q, cache, table, lens, indptr, out=torch.empty(5, 4, 128, dtype=BF16)),
+                     lambda: ops.kv_cache_read(cache, table.cpu(), indptr, 5), lambda: ops.rms_norm_quant(x, w.cpu())):
+            with pytest.raises(ValueError) as info:
+                call()
+            errors.append(str(info.value))
+        for call in (lambda: ops.kv_cache_attention(q[:, :3], cache, table, lens, indptr), lambda: ops.kv_cache_attention(q, cache, table.long(), lens, indptr),
+                     lambda: ops.kv_cache_append(cache, k[..., ::2], v, table, lens, indptr), lambda: ops.kv_cache_attention(q, cache, table, lens, indptr, sink_tokens=3),
+                     lambda: ops.kv_cache_append(cache, k, v, table, lens, indptr, rope=rope[:127])):
+            with pytest.raises(_lib.TileGymHipError) as info:
+                call()
+            errors.append(str(info.value))
+        return out, errors
+
+    native, said = run()
+    monkeypatch.setattr(_lib, "native_path", lambda: False)
+    plain, said_too = run()
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(native, plain))
+    assert said == said_too
+
+
+@pytest.mark.gpu
+def test_calls_at_once_on_two_streams(device):
+    """Split contexts, appends to caches of their own and norms on two streams, each twenty times over: the bits of the calls one by one."""
+    pool = Pool(device, 130, 2, 64, 128, 2, 64)
+    pool.fill([4000, 3900], [4000, 3900])
+    table, lens, indptr = pool.i32(pool.table), pool.i32([4000, 3900]), pool.i32([0, 1, 2])
+    qkv = [torch.randn(2, 12, 128, generator=pool.g).to(BF16).to(device) for _ in range(2)]
+    x = [torch.randn(600, 1040, generator=pool.g).to(BF16).to(device) for _ in range(2)]
+    w = torch.ones(1040, dtype=BF16, device=device)
+    caches = [ops.KVCache(*(t.clone() for t in pool.cache)) for _ in range(2)]
+
+    def step(i):
+        q, k, v = qkv[i].split([8, 2, 2], 1)
+        ops.kv_cache_append(caches[i], k, v, table, lens, indptr)
+        return (ops.kv_cache_attention(q, caches[i], table, lens, indptr), *ops.rms_norm_quant(x[i], w, group_size=16))
+
+    want = [step(i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for outs in got[i]:
+            assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(outs, want[i]))
