@@ -776,15 +776,16 @@ hipError_t launch(KvAttentionParams p, hipStream_t s) {
 
 int kv_attention_splits(const KvAttentionParams& p) {
     const int tile_rows = tile_rows_of(p);
-    // Few rows: a tile for each sequence, as far as the host can tell, and a workgroup per compute unit (two do not fit its registers).
-    // Shares are cut only where compute units would be left over: 8 sequences of 8000 keys x 8 heads 27.6 us, uncut 48.6; 24 such 71,
-    // cut in two 78.  Many rows: two workgroups per compute unit.  No share below 8 steps, and none up to 1024 keys (8 x 1000 keys 11.5 us in
-    // one launch, 12.0 cut and joined).
+    // Few rows: a tile for each sequence, as far as the host can tell, and a workgroup per compute unit (two do not fit its registers), never
+    // more: 12 sequences of 4000 keys x 8 heads 23.4 us cut in two, 32.5 cut in three (288 workgroups); 20 such uncut 29.6, cut in two 41.2;
+    // 8 of 8000 cut in four 27.6, uncut 48.6.  Shares of one size for long and short sequences, counted on the device, were no faster: the
+    // memory is shared by those that still run.  Many rows: two workgroups per compute unit.  No share below 8 steps, and none up to 1024 keys
+    // (8 x 1000 keys 11.5 us in one launch, 12.0 cut and joined).
     const int64_t units = (tile_rows != 128 ? (int64_t)p.c.batch : row_tiles(p, tile_rows)) * p.c.heads;
     int64_t keys = (int64_t)p.c.width << p.c.page_log2;
     if (p.window) keys = std::min<int64_t>(keys, (int64_t)p.window + 128 + ((int64_t)p.sinks + 63) / 64 * 64);
     const int64_t steps = (keys + 63) / 64, workgroups = tile_rows != 128 ? kComputeUnits : 2 * kComputeUnits;
-    const int64_t wanted = (workgroups + units / 2) / units, most = steps <= 2 * kLeastSteps ? 1 : (steps + kLeastSteps - 1) / kLeastSteps;
+    const int64_t wanted = tile_rows != 128 ? workgroups / units : (workgroups + units / 2) / units, most = steps <= 2 * kLeastSteps ? 1 : (steps + kLeastSteps - 1) / kLeastSteps;
     return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(wanted, most), kMostSplits));
 }
 
