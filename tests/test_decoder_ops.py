@@ -890,3 +890,20 @@ def test_calls_at_once_on_two_streams(device):
     for i in range(2):
         for outs in got[i]:
             assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(outs, want[i]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page,dim", [(64, 128), (128, 64), (32, 256), (128, 256)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_append_long_runs_into_few_pages(device, page, dim, dtype):
+    """Few pages and many new tokens of each: from a page's beginning, then from the middle of one."""
+    pool = Pool(device, 12, 2, page, dim, 2, 5)
+    rope = ops.rope_table(5 * page, dim, device="cpu")
+    lens = [2 * page + 5, page - 3]
+    pool.fill(lens, lens, dtype, rope, True)
+    pool.check(True)
+    news = [2 * page + 1, 3 * page + 3]
+    q, out, want, _ = pool.fill([a + b for a, b in zip(lens, news)], news, dtype, rope, True, q_heads=3)
+    pool.check(True)
+    slack = 2.0 ** -22 * 2 * want.abs().amax()  # two products and a difference in fp32
+    assert bool(((out.cpu().double() - want).abs() <= HALF[dtype] * want.abs() * (1 + 2.0 ** -10) + slack + 2.0 ** -26).all())

@@ -73,16 +73,16 @@ __device__ __forceinline__ void lds_written() {
 }
 
 // Workgroups of the two kinds of work: first those that write the cache, then those that turn q.  A page, head and half is the work of WAVES
-// waves: four where sequences have many new tokens, one where they have few (16 lanes of 8 elements have a token's 128).
+// waves: one where sequences have few new tokens (16 lanes of 8 elements have 128 of a token), else 4 or 16.
 template <typename T, int WAVES>
-__global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendParams p, int items, int cache_blocks, int v_pad, int q_waves) {
-    constexpr int LANES = 64 * WAVES;
+__global__ void __launch_bounds__(64 * (WAVES > 4 ? WAVES : 4)) kv_append_kernel(const KvAppendParams p, int items, int cache_blocks, int v_pad, int q_waves) {
+    constexpr int LANES = 64 * WAVES, BLOCK_WAVES = WAVES > 4 ? WAVES : 4;
     typedef T vecT __attribute__((ext_vector_type(8)));
     const KvCache& c = p.c;
     const int P = 1 << c.page_log2, D = c.dim, chunks = D / 8, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     if ((int)blockIdx.x >= cache_blocks) {
         // q: a wave has one token, and every q_waves-th 64 vectors of 8 elements of it
-        const int64_t job = (int64_t)((int)blockIdx.x - cache_blocks) * 4 + wave;
+        const int64_t job = (int64_t)((int)blockIdx.x - cache_blocks) * BLOCK_WAVES + wave;
         // (the items are the rows that sequences have, in order; rows of no sequence are left as they were)
         if (job / q_waves >= c.rows) return;
         const SeqItem f = find_sequence(c, (int)(job / q_waves), [](int n, int) { return n; });
@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendParams p, 
         return;
     }
     extern __shared__ uint8_t all_lds[];  // v: the page's new codes, an element's tokens together, rows of v_pad bytes
-    __shared__ float part[4];
+    __shared__ float part[BLOCK_WAVES];
     const int unit = WAVES == 1 ? (int)blockIdx.x * 4 + wave : (int)blockIdx.x, tid = (int)threadIdx.x & (LANES - 1);
     uint8_t* lds = all_lds + (WAVES == 1 ? wave * D * v_pad : 0);
     const int half = unit & 1, head = (unit >> 1) % c.heads, item = (unit >> 1) / c.heads;
@@ -148,7 +148,8 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendParams p, 
     if constexpr (WAVES > 1) {
         if (tid % 64 == 0) part[wave] = amax;
         __syncthreads();  // (and every lane has read the old scale)
-        amax = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) amax = fmaxf(amax, part[w]);
     }
     if (!(old > 0.f && old <= 0x1p100f)) old = 0.f;  // no scale that a write leaves: the earlier slots hold nothing
     const float scale = fmaxf(page_scale(amax), old), inverse = 1.0f / scale;
@@ -306,18 +307,22 @@ template <typename T>
 static hipError_t launch_kv_append(const KvAppendParams& p, hipStream_t s) {
     const KvCache& c = p.c;
     const int64_t P = (int64_t)1 << c.page_log2, items = c.rows / P + 2 * (int64_t)c.batch /* at most: ceil(n / P) + 1 each */, units = items * c.heads * 2;
-    // one wave per page where sequences have up to four new tokens on average
+    // One wave per page where sequences have up to four new tokens on average, else four, or 16 where that leaves compute units without work
+    // and pages and runs are long: a lane's vectors come one after the other.  512 tokens of 8 heads of 128 in pages of 128: 11.8 us with four, 7.7
+    // with 16, of 256 20.5 and 11.8; but 2048 of 64 in pages of 64 8.5 and 11.1, runs of 16 tokens 5.0 and 5.9.
     const bool single = c.rows <= 4 * (int64_t)c.batch;
-    const int64_t cache_blocks = single ? (units + 3) / 4 : units;
+    const bool many = !single && units <= 512 && P * c.dim >= 8192 && (int64_t)c.rows * c.dim >= 4096 * (int64_t)c.batch;
+    const int64_t cache_blocks = single ? (units + 3) / 4 : units, block_waves = many ? 16 : 4;
     // q: as many waves for a token as it has 64 vectors, fewer once that makes 8192 in all
     const int64_t vectors = (int64_t)p.q_heads * (c.dim / 8);
     const int64_t q_waves = p.q ? std::max<int64_t>(1, std::min<int64_t>((vectors + 63) / 64, 8192 / c.rows)) : 1;
-    const int64_t blocks = cache_blocks + (p.q ? (c.rows * q_waves + 3) / 4 : 0);
+    const int64_t blocks = cache_blocks + (p.q ? (c.rows * q_waves + block_waves - 1) / block_waves : 0);
     if (blocks > INT32_MAX || items > INT32_MAX) return hipErrorInvalidValue;
     const int v_pad = (int)P + 4;
-    const dim3 grid((unsigned)blocks), block(256);
+    const dim3 grid((unsigned)blocks), block((unsigned)(64 * block_waves));
     const size_t lds = (size_t)c.dim * v_pad * (single ? 4 : 1);
     if (single) hipLaunchKernelGGL((kv_append_kernel<T, 1>), grid, block, lds, s, p, (int)items, (int)cache_blocks, v_pad, (int)q_waves);
+    else if (many) hipLaunchKernelGGL((kv_append_kernel<T, 16>), grid, block, lds, s, p, (int)items, (int)cache_blocks, v_pad, (int)q_waves);
     else hipLaunchKernelGGL((kv_append_kernel<T, 4>), grid, block, lds, s, p, (int)items, (int)cache_blocks, v_pad, (int)q_waves);
     return hipGetLastError();
 }
