@@ -736,11 +736,31 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const KvAttentio
 
 // Tiles there can be: sum over sequences of ceil(n * group / tile_rows) at most.
 int64_t row_tiles(const KvAttentionParams& p, int64_t tile_rows) { return (int64_t)p.c.rows * p.group / tile_rows + p.c.batch; }
-// Rows of a tile, by the rows that a sequence's key/value head has on average, as the host does not read the tensors: 16 or 32 in the form
-// for few rows, 128 in the one for many.
+// Rows that a sequence's key/value head has on average, and tiles of so many in all sequences and heads: the host does not read the tensors.
+int64_t rows_each(const KvAttentionParams& p) { return ((int64_t)p.c.rows * p.group + p.c.batch - 1) / p.c.batch; }
+int64_t tiles_in_all(const KvAttentionParams& p, int64_t tile_rows) { return p.c.batch * ((rows_each(p) + tile_rows - 1) / tile_rows) * p.c.heads; }
+
+// Keys that a tile can see, as far as the host can tell.
+int64_t keys_at_most(const KvAttentionParams& p) {
+    const int64_t keys = (int64_t)p.c.width << p.c.page_log2;
+    return p.window ? std::min<int64_t>(keys, (int64_t)p.window + 128 + ((int64_t)p.sinks + 63) / 64 * 64) : keys;
+}
+
+// Rows of a tile: 16 or 32 in the form for few rows, 128 in the one for many.  A workgroup of the first runs through its steps fastest with 16 rows,
+// but every tile reads the keys, and a compute unit holds one workgroup.  So (128 elements, 8 heads; us with tiles of 16 / 32 / 128 rows):
+//   16 while the compute units hold all tiles, up to two a sequence, which share an XCD's cache if workgroups 8 apart have the same head (4
+//   sequences of 20 rows and 3000 keys 14.6 / 18.0 / 23; 32 of 20 rows 48 / 38 / 44; 64 of 20 rows and 2 heads 35 / 27 / 32), and
+//   more of them only up to a quarter of the compute units (1 of 64 rows 13.8 / 16.9 / 20.6; 8 of 80 rows and 8000 keys 96 / 54 / 64);
+//   32 while the compute units hold all tiles (2 of 512 rows 45 / 27 / 39), or twice as many if the keys are read twice at most and not so few that the
+//   workgroups' beginnings and ends count (32 of 48 rows: 3000 keys 67 / 53 / 65, 500 keys 29 / 26 / 18; 16 of 96 rows 67 / 51 / 46);
+//   of 256 elements there is no form of 32 rows, and 128 of them spill: 16 up to 32 rows each (64 of 20 rows 185 / - / 254) and
+//   up to twice the compute units (16 of 48 rows 80 / - / 105, of 96 rows 120 / - / 85).
 int tile_rows_of(const KvAttentionParams& p) {
-    const int64_t rows = (int64_t)p.c.rows * p.group, batch = p.c.batch;
-    return rows <= 16 * batch || (p.c.dim == 256 && rows <= 32 * batch) ? 16 : rows <= 32 * batch ? 32 : 128;
+    const int64_t each = rows_each(p), by16 = tiles_in_all(p, 16), by32 = tiles_in_all(p, 32);
+    if (each <= 16 || by16 <= (each <= 32 && p.c.heads % 8 == 0 ? kComputeUnits : kComputeUnits / 4)) return 16;
+    if (p.c.dim == 256) return each <= 32 || by16 <= 2 * kComputeUnits ? 16 : 128;
+    if (by32 <= kComputeUnits) return 32;
+    return keys_at_most(p) > 1024 && (each <= 32 || (each <= 64 && by32 <= 2 * kComputeUnits)) ? 32 : 128;
 }
 
 template <typename T, int D>
@@ -776,15 +796,13 @@ hipError_t launch(KvAttentionParams p, hipStream_t s) {
 
 int kv_attention_splits(const KvAttentionParams& p) {
     const int tile_rows = tile_rows_of(p);
-    // Few rows: a tile for each sequence, as far as the host can tell, and a workgroup per compute unit (two do not fit its registers), never
+    // Few rows: tiles as far as the host can tell, and a workgroup per compute unit (of 128 elements, two do not fit its registers), never
     // more: 12 sequences of 4000 keys x 8 heads 23.4 us cut in two, 32.5 cut in three (288 workgroups); 20 such uncut 29.6, cut in two 41.2;
     // 8 of 8000 cut in four 27.6, uncut 48.6.  Shares of one size for long and short sequences, counted on the device, were no faster: the
     // memory is shared by those that still run.  Many rows: two workgroups per compute unit.  No share below 8 steps, and none up to 1024 keys
     // (8 x 1000 keys 11.5 us in one launch, 12.0 cut and joined).
-    const int64_t units = (tile_rows != 128 ? (int64_t)p.c.batch : row_tiles(p, tile_rows)) * p.c.heads;
-    int64_t keys = (int64_t)p.c.width << p.c.page_log2;
-    if (p.window) keys = std::min<int64_t>(keys, (int64_t)p.window + 128 + ((int64_t)p.sinks + 63) / 64 * 64);
-    const int64_t steps = (keys + 63) / 64, workgroups = tile_rows != 128 ? kComputeUnits : 2 * kComputeUnits;
+    const int64_t units = tile_rows != 128 ? tiles_in_all(p, tile_rows) : row_tiles(p, tile_rows) * p.c.heads;
+    const int64_t steps = (keys_at_most(p) + 63) / 64, workgroups = tile_rows != 128 ? kComputeUnits : 2 * kComputeUnits;
     const int64_t wanted = tile_rows != 128 ? workgroups / units : (workgroups + units / 2) / units, most = steps <= 2 * kLeastSteps ? 1 : (steps + kLeastSteps - 1) / kLeastSteps;
     return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(wanted, most), kMostSplits));
 }
