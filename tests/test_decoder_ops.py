@@ -907,3 +907,71 @@ def test_append_long_runs_into_few_pages(device, page, dim, dtype):
     pool.check(True)
     slack = 2.0 ** -22 * 2 * want.abs().amax()  # two products and a difference in fp32
     assert bool(((out.cpu().double() - want).abs() <= HALF[dtype] * want.abs() * (1 + 2.0 ** -10) + slack + 2.0 ** -26).all())
+
+
+# ---------------------------------------------------------------------------- values and arguments at the edges
+@pytest.mark.gpu
+@pytest.mark.parametrize("given", [False, True])
+def test_norm_of_rows_next_to_nothing(device, given):
+    """Scales below the smallest normal number: zeros stay zeros, the others are rounded as ever."""
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(6, 512, generator=g) * 1e-36
+    x[:, ::3] = 0
+    w = torch.full((512,), 1e-4)
+    scale = torch.tensor([3e-40], device=device) if given else None
+    q, s = ops.rms_norm_quant(x.to(device), w.to(device), 1e-6, group_size=128, scale=scale)
+    y = x.double() * 1e3 * 1e-4  # (the mean square is nothing beside eps)
+    step = (s.cpu().double() if not given else torch.full((6, 4), float(scale))).repeat_interleave(128, 1)
+    got = q.cpu().float().double() * step
+    assert bool((step < 2.0 ** -126).all()) and bool((got[:, ::3] == 0).all())
+    # half an e4m3 step, and the fp32 steps below 2^-126: 2^-150 off for y, and as much relative to a scale of 2^-150 / scale
+    y = torch.minimum(torch.maximum(y, -448 * step), 448 * step)
+    assert bool(((got - y).abs() <= 2.0 ** -4 * y.abs() * (1 + 2.0 ** -10) + 2 * step * 2.0 ** -10 + 2.0 ** -149 + y.abs() * 2.0 ** -149 / step).all())
+
+
+@pytest.mark.gpu
+def test_norm_flags_that_are_not_bools(device):
+    x, w = torch.randn(3, 128, device=device).to(BF16), torch.ones(128, dtype=BF16, device=device)
+    want = ops.rms_norm_quant(x, w, return_norm=True)
+    got = ops.rms_norm_quant(x, w, return_norm=1)
+    assert len(got) == 3 and torch.equal(got[2], want[2]) and len(ops.rms_norm_quant(x, w, return_norm=0)) == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("news", [1, 24])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_attention_many_faint_keys(device, dtype, news):
+    """One strong key with value zero beside twenty thousand faint ones with value one, each 2^-25.2 of it."""
+    n, dim, strong = 20000, 64, 20.0
+    cache = ops.alloc_kv_cache(-(-n // 64), 1, dim, 64, device=device)
+    k, v = torch.zeros(n, 1, dim), torch.ones(n, 1, dim)
+    k[:, 0, 0] = 2.5
+    k[0, 0, 0], v[0] = strong, 0
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    table = torch.arange(-(-n // 64), dtype=torch.int32, device=device)[None]
+    ops.kv_cache_append(cache, k.to(dtype).to(device), v.to(dtype).to(device), table, i32(n), i32(0, n))
+    q = torch.zeros(news, 4, dim)
+    q[..., 0] = 1
+    out = ops.kv_cache_attention(q.to(dtype).to(device), cache, table, i32(n), i32(0, news), sm_scale=1.0).cpu().double()
+    weight = math.exp(2.5 - strong)
+    for t in range(news):
+        faint = n - news + t
+        want = faint * weight / (1 + faint * weight)
+        # a weight is rounded to 16 bits, or by half of f16's smallest step, a 128th of 2^-25 against the maximum; the scores' 20 are 2^-23 off, the
+        # exponentials and the sum of 20000 fp32 terms a few units of 2^-24 each
+        tol = want * (2 * HALF[dtype] + 20 * 2.0 ** -22 + 20000 / 16 * 2.0 ** -24) + (faint * 2.0 ** -32 if dtype == F16 else 0)
+        assert bool(((out[t] - want).abs() <= tol).all()), (float(out[t, 0, 0]), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("news", [6, 40])
+def test_attention_of_more_new_tokens_than_there_are_in_the_widest_window(device, news):
+    """Positions below zero see nothing, whatever the window; those from zero on see all before them."""
+    pool = Pool(device, 2, 1, 64, 64, 1, 1)
+    pool.fill([3], [3])
+    q = torch.randn(news, 4, 64, generator=pool.g).to(BF16).to(device)
+    args = (q, pool.cache, pool.i32(pool.table), pool.i32([3]), pool.i32([0, news]))
+    want = ops.kv_cache_attention(*args)
+    assert bool((want[:news - 3] == 0).all()) and bool((want[news - 3:] != 0).any(-1).all())
+    for window in (2 ** 31 - 1, 2 ** 31 - 3, 2 ** 30, 3):
+        assert torch.equal(ops.kv_cache_attention(*args, window=window, sink_tokens=0), want)

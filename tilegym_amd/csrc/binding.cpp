@@ -350,6 +350,7 @@ PyObject* py_rms_norm_quant(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor* x = tensor_of(args[0]);
     const double eps = PyFloat_AsDouble(args[2]);
     const long group = PyLong_AsLong(args[4]);
+    const int with_norm = PyObject_IsTrue(args[7]);
     if (PyErr_Occurred()) return nullptr;
     const bool given = args[5] != Py_None;
     if (!on_gpu(x) || !io_type(x->scalar_type()) || !x->is_contiguous() || x->dim() < 1 || x->dim() > TG_MAX_DIMS ||
@@ -374,7 +375,6 @@ PyObject* py_rms_norm_quant(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (!describe(made_residual, &dro)) Py_RETURN_NONE;
         ro = &dro;
     }
-    const bool with_norm = args[7] == Py_True;
     if (with_norm) {
         norm = new_tensor(x->sizes(), x->scalar_type(), *x);
         if (!describe(norm, &dn)) Py_RETURN_NONE;
@@ -387,7 +387,7 @@ PyObject* py_rms_norm_quant(PyObject*, PyObject* const* args, Py_ssize_t n) {
                           (uint64_t)(uintptr_t)stream);
     Py_END_ALLOW_THREADS
     if (!succeeded(rc, "tg_fp8_rms_norm_quant")) return nullptr;
-    PyObject* tuple = PyTuple_New(2 + (r != nullptr) + with_norm);
+    PyObject* tuple = PyTuple_New(2 + (r != nullptr) + (with_norm != 0));
     if (!tuple) return nullptr;
     int at = 0;
     auto borrowed = [](PyObject* o) { Py_INCREF(o); return o; };

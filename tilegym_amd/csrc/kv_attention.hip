@@ -12,7 +12,7 @@
 // the cache's transposed v has them in 16 consecutive bytes.  They lie in one page (P is a multiple of 16), so scales are
 // one value per lane.
 // Codes become the 16-bit type of q exactly (e4m3 has 4 significant bits).  k's scale joins the softmax's factor.  v's scale: O is
-// held in units of the largest one seen, u; P is multiplied by v_scale / u <= 1 before it is rounded to 16 bits (2^-9 relative in
+// held in units of the largest one seen, u (or a 128th of it); P is multiplied by v_scale / u before it is rounded to 16 bits (2^-9 relative in
 // bf16, 2^-12 in f16, of its own value), where a page differs from that.  S, m, l and O are fp32.
 //
 // What is not seen is taken out by selection, never by arithmetic: scores before the maximum, and v's codes, since 0 x NaN is NaN
@@ -71,7 +71,7 @@ __device__ __forceinline__ X vector_load(const X* at) {
 constexpr float kMinusInf = -__builtin_inff();
 constexpr float kSmallestUnit = 0x1p-126f;
 // The maximum that a row's scores are taken against is looked for only when 16 weights against the old one add up to more than this: floating
-// point loses no precision in weights above 1 (f16 holds 16 times as much, and sums and O are fp32).  A row's first keys find a maximum of
+// point loses no precision in weights above 1 (f16 holds 16 times as much, and sums and O are fp32; a maximum's 16 weights are 2048 at most).  A row's first keys find a maximum of
 // -inf and so a sum that is not a number, and take the same path.  In the other steps there is no search, no exchange between lanes
 // and no rescaling of O.
 constexpr float kLargeSum = 4096.f;
@@ -118,7 +118,7 @@ __device__ __forceinline__ bool set_tile(const KvAttentionParams& p, const SeqIt
     t.low = t.start + t.r0 / p.group, t.high = t.start + (t.r0 + t.rows - 1) / p.group;
     const int capacity = c.width << c.page_log2;
     t.key1 = t.high < 0 ? 0 : t.high < capacity ? t.high + 1 : capacity;
-    t.key0 = p.window ? min(max(t.low - (p.window - 1), 0), t.key1) : 0;
+    t.key0 = p.window ? (int)min(max((int64_t)t.low - (p.window - 1), (int64_t)0), (int64_t)t.key1) : 0;  // (positions may lie below zero)
     const int sinks = min(p.sinks, t.key0);
     t.sink_steps = min((sinks + 63) >> 6, t.key0 >> 6);
     t.steps = t.key1 > 0 ? t.sink_steps + (((t.key1 + 63) >> 6) - (t.key0 >> 6)) : 0;
@@ -177,15 +177,20 @@ __device__ __forceinline__ void select_seen(S& s, int key, int position, int win
     }
 }
 
-// v's scale against the unit u that O is held in; lanes hold the scales of their own 16 keys.
+// v's scale against the unit u that O is held in; lanes hold the scales of their own 16 keys.  u is the largest scale seen, in f16 a 128th of it: weights
+// against the maximum are then 128 times as large, and one that f16's smallest step swallows is below 2^-32 of the maximum's and not 2^-25, which tens
+// of thousands of faint keys beside one strong one would add up to more than a rounding of the result.
+template <typename T>
 struct Unit {
+    static constexpr int kUp = std::is_same_v<T, __bf16> ? 0 : 7;
+    static constexpr float kDown = 1.f / (1 << kUp);
     float u = kSmallestUnit, inverse = 0x1p126f;
     float grown = 1.f;                 // this step: u before / u now
     float lift, back;                  // this step: log2(v_scale / u), u / v_scale
     // seen: whether any key of the lane's 16 is seen (the scale of the others may be anything)
     __device__ __forceinline__ void step(float v_scale, bool seen) {
         grown = 1.f;
-        float s = seen ? v_scale : 0.f;
+        float s = seen ? v_scale * kDown : 0.f;
         if (__ballot(s > u)) {
             float top = fmaxf(s, __shfl_xor(s, 16));
             top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), u);
@@ -194,14 +199,14 @@ struct Unit {
             u = top, inverse = 1.f / top;
         }
         s = fmaxf(s * inverse, 0x1p-100f);  // (no keys, or a scale of zero: any finite logarithm will do)
-        lift = __builtin_amdgcn_logf(s), back = __builtin_amdgcn_rcpf(s);
+        lift = __builtin_amdgcn_logf(s) + (float)kUp, back = __builtin_amdgcn_rcpf(s) * kDown;
     }
 };
 
 // One row's 16 scores of a step -> its weights, against the running maximum m and in units of u, and its sum l.  Returns what O has to
 // be multiplied by on m's account.  factor > 0.
 template <typename T, typename S>
-__device__ __forceinline__ float weigh(const S& s, float factor, const Unit& unit, float& m, float& l, typename Types<T>::v8 (&pt)[2]) {
+__device__ __forceinline__ float weigh(const S& s, float factor, const Unit<T>& unit, float& m, float& l, typename Types<T>::v8 (&pt)[2]) {
     v16f w;
     float shrink = 1.f, base = unit.lift - m, sum = 0.f;
 #pragma unroll
@@ -355,7 +360,7 @@ __global__ void __launch_bounds__(64 * kFewWaves<D>, D == 256 ? 1 : 2) kv_attent
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[n][d] = v4f{0.f, 0.f, 0.f, 0.f};
-    Unit unit;
+    Unit<T> unit;
 
     for (int step = mine; step < end; step += WAVES) {
         const int key = t.key_of(step), first = key + 16 * g;
@@ -575,7 +580,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_rows_kerne
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = v16f{};
     float m = live ? kMinusInf : 0.f, l = 0.f;
-    Unit unit;
+    Unit<T> unit;
     const int s_key = 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3);  // the key that this lane reads as a row of K, of 32
     const int k_lane = s_key * D + (h ^ k_swizzle<D>(s_key)) * 16, v_lane = col * 64 + (h ^ v_swizzle(col)) * 16;
     for (int step = begin; step < end; ++step, key = key1, key1 = key2) {

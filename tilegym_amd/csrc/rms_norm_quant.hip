@@ -100,7 +100,11 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) rms_norm_quant_kernel(c
                 if ((at & (p.lanes_per_group - 1)) == 0) p.scales[row * (vectors >> p.group_shift) + (at >> p.group_shift)] = s;
             }
             // y carries the norm's own 2^-22; a reciprocal's half unit in the last place moves a code only where y / s lies that near a border
-            const float inverse = 1.0f / s;
+            float inverse = 1.0f / s;
+            if (s < 0x1p-100f) {  // (the reciprocal of a subnormal scale may be infinite, and zero times that no number)
+                y *= 0x1p60f;
+                inverse = 1.0f / (s * 0x1p60f);
+            }
             v8f_q c;
 #pragma unroll
             for (int k = 0; k < 8; ++k) c[k] = __builtin_amdgcn_fmed3f(y[k] * inverse, -448.0f, 448.0f);
