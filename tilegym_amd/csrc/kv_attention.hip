@@ -250,8 +250,11 @@ __device__ __forceinline__ typename Types<T>::v8 load_q(const T* at, bool negati
 // k's scale and the softmax factor; never zero, so that what is not seen stays at -inf
 __device__ __forceinline__ float score_factor(float k_scale, float scale_log2) { return fmaxf(fabsf(k_scale * scale_log2), 0x1p-126f); }
 
-// Few rows: eight waves (four with 256 elements, which take the registers of two), 16 NT rows; the waves take the steps of the workgroup's share in turn and join at the end.  Codes come straight
-// from memory into registers, k's of the next step being asked for when this step's are used up, v's likewise.
+// Few rows: eight waves (four with 256 elements, which take the registers of two), 16 NT rows; the waves take the steps of the workgroup's share in
+// turn and join at the end.  Codes come straight from memory into registers, k's of the next step being asked for when this step's are used
+// up, v's likewise.  Bound by HBM once some 150 compute units have work (64 sequences of 100 to 8000 keys x 8 heads: 5.5 TB/s), by latency below
+// that.  Eight waves and one workgroup to a compute unit against four and two: those 64 sequences, long ones first, 98 and 110 us; 64 of 4000 keys each
+// 101 and 98, 8 of them 19.5 and 19.2, one of 777 11.4 and 10.3.
 template <int D>
 constexpr int kFewWaves = D == 256 ? 4 : 8;
 // ONE: pages hold whole steps (64 or 128 tokens), so a step's page, its scales and its address are scalars.
@@ -471,7 +474,9 @@ __global__ void __launch_bounds__(64 * kFewWaves<D>, D == 256 ? 1 : 2) kv_attent
 
 // Many rows: 128 of them per workgroup, 32 per wave, and every wave runs over the same keys, whose codes go to LDS for all four
 // without a register between, the next step's while this one's products run, in two buffers with one barrier a step.  Codes stay
-// e4m3 in LDS (half the reads that 16 bits would cost, 193 against 200 us) and are widened behind each read, for 32 rows.
+// e4m3 in LDS (half the reads that 16 bits would cost) and are widened behind each read, for 32 rows.  Bound by the SIMDs' issue, products and the
+// softmax's and widening's vector instructions sharing them, two waves each: 4096 tokens of 3 sequences x 32 heads over 1500 to 4500 keys 180 us, 860
+// TFLOP/s (a large 16-bit product: 1205); with 16 bits in LDS 4 % more, with three waves per SIMD spills.
 // The products are 32x32x16 instructions on 32 keys at a time, the same way round: S^T row 8 a + 4 h + b stands for key 16 h + 4 a + b, so a
 // lane (row lane % 32, h = lane / 32) has 16 consecutive keys of its one row.
 // 16-byte chunks lie in LDS so that the 8, and the 16, neighbouring lanes that read together cover different banks: chunk ^ f,
@@ -775,8 +780,8 @@ hipError_t launch(KvAttentionParams p, hipStream_t s) {
     const int64_t join = ((int64_t)p.c.rows * p.q_heads * (D / 4) + 255) / 256;
     if (blocks > INT32_MAX || join > INT32_MAX) return hipErrorInvalidValue;
     const dim3 grid((unsigned)blocks), block(256);
-    // more workgroups than compute units, whole sequences each: the long ones first, and the short ones fill in behind them (64 sequences of 1
-    // to 8000 keys 98 us, in their own order 119)
+    // more workgroups than compute units, whole sequences each: the long ones first, and the short ones fill in behind them (64 sequences of 100
+    // to 8000 keys 98 us, in their own order 110; 40 of them 74 and 83; of 4000 each 101 and 100)
     p.longest_first = tile_rows == 16 && p.splits == 1 && p.c.batch <= 64 && p.c.batch > 1 && blocks > kComputeUnits;
     const bool one = p.c.page_log2 >= 6;
 #define TG_FEW(NT, ONE) hipLaunchKernelGGL((kv_attention_kernel<T, D, NT, ONE>), grid, dim3(64 * kFewWaves<D>), 0, s, p)
