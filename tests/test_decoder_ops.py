@@ -975,3 +975,20 @@ def test_attention_of_more_new_tokens_than_there_are_in_the_widest_window(device
     assert bool((want[:news - 3] == 0).all()) and bool((want[news - 3:] != 0).any(-1).all())
     for window in (2 ** 31 - 1, 2 ** 31 - 3, 2 ** 30, 3):
         assert torch.equal(ops.kv_cache_attention(*args, window=window, sink_tokens=0), want)
+
+
+@pytest.mark.gpu
+def test_launches_too_large_for_the_device_are_refused(device):
+    """Small tensors whose sequences and heads would make more work items than a launch can have."""
+    heads = 65536
+    cache = ops.alloc_kv_cache(1, heads, 64, 16, device=device)
+    table, lens = torch.full((256, 1), -1, dtype=torch.int32, device=device), torch.zeros(256, dtype=torch.int32, device=device)
+    indptr = torch.zeros(257, dtype=torch.int32, device=device)
+    x = torch.zeros(1, heads, 64, dtype=BF16, device=device)
+    for call in (lambda: ops.kv_cache_read(cache, table, indptr, 1), lambda: ops.kv_cache_append(cache, x, x, table, lens, indptr),
+                 lambda: ops.kv_cache_attention(x, cache, table, lens, indptr)):
+        with pytest.raises(_lib.TileGymHipError):
+            call()
+    # nothing is left behind: a smaller call of the same kind runs
+    out = ops.kv_cache_attention(x, cache, table[:1], lens[:1], indptr[:2], out=torch.full_like(x, 3.0))
+    assert bool((out == 3).all())

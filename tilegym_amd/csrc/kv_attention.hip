@@ -778,7 +778,7 @@ hipError_t launch(KvAttentionParams p, hipStream_t s) {
     const int tile_rows = tile_rows_of(p);
     const int64_t tiles = row_tiles(p, tile_rows), blocks = tiles * p.c.heads * p.splits;
     const int64_t join = ((int64_t)p.c.rows * p.q_heads * (D / 4) + 255) / 256;
-    if (blocks > INT32_MAX || join > INT32_MAX) return hipErrorInvalidValue;
+    if (blocks * 64 * kFewWaves<D> > kMostThreads || join * 256 > kMostThreads) return hipErrorInvalidValue;
     const dim3 grid((unsigned)blocks), block(256);
     // more workgroups than compute units, whole sequences each: the long ones first, and the short ones fill in behind them (64 sequences of 100
     // to 8000 keys 98 us, in their own order 110; 40 of them 74 and 83; of 4000 each 101 and 100)

@@ -317,7 +317,7 @@ static hipError_t launch_kv_append(const KvAppendParams& p, hipStream_t s) {
     const int64_t vectors = (int64_t)p.q_heads * (c.dim / 8);
     const int64_t q_waves = p.q ? std::max<int64_t>(1, std::min<int64_t>((vectors + 63) / 64, 8192 / c.rows)) : 1;
     const int64_t blocks = cache_blocks + (p.q ? (c.rows * q_waves + block_waves - 1) / block_waves : 0);
-    if (blocks > INT32_MAX || items > INT32_MAX) return hipErrorInvalidValue;
+    if (blocks * 64 * block_waves > kMostThreads || items > INT32_MAX) return hipErrorInvalidValue;
     const int v_pad = (int)P + 4;
     const dim3 grid((unsigned)blocks), block((unsigned)(64 * block_waves));
     const size_t lds = (size_t)c.dim * v_pad * (single ? 4 : 1);
@@ -336,7 +336,7 @@ hipError_t run_kv_read(const KvReadParams& p, int out_type, hipStream_t s) {
     const KvCache& c = p.c;
     if (c.rows <= 0 || c.batch <= 0) return hipSuccess;
     const int64_t blocks = ((int64_t)c.rows / 64 + c.batch) * c.heads * 2;
-    if (blocks > INT32_MAX) return hipErrorInvalidValue;
+    if (blocks * 256 > kMostThreads) return hipErrorInvalidValue;
     const dim3 grid((unsigned)blocks), block(256);
     const size_t lds = (size_t)c.dim * 64;
     if (out_type == OUT_BF16) hipLaunchKernelGGL(kv_read_kernel<__bf16>, grid, block, lds, s, p);

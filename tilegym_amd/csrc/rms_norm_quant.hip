@@ -133,6 +133,7 @@ hipError_t launch(const NormQuantParams& p, hipStream_t s) {
 #define TG_NORM(TPR, V)                                                                                                          \
     if (vectors <= TPR * V) {                                                                                                    \
         const int rows = TPR < 256 ? 256 / TPR : 1;                                                                              \
+        if ((p.rows + rows - 1) / rows * (TPR < 256 ? 256 : TPR) > kMostThreads) return hipErrorInvalidValue;                    \
         hipLaunchKernelGGL((rms_norm_quant_kernel<T, W, TPR, V>), dim3((unsigned)((p.rows + rows - 1) / rows)), dim3(TPR < 256 ? 256 : TPR), 0, s, p); \
         return hipGetLastError();                                                                                                \
     }

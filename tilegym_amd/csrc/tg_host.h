@@ -149,6 +149,7 @@ struct KvCache {
     int pages, heads, dim, page_log2, batch, width;
     int rows;            // of the packed tensors
 };
+constexpr int64_t kMostThreads = ((int64_t)1 << 32) - 1;  // of a launch: larger ones are refused
 struct KvAppendParams {
     KvCache c;
     const void *k, *v;                 // (rows, heads, dim), element strides below, the last dimension contiguous
