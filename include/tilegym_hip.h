@@ -416,6 +416,11 @@ int32_t tg_diag_mfma(int32_t fmas, int32_t iters, int32_t workgroups, const tg_t
  * form (few rows per expert); 0 when it does not.  Host arithmetic, no GPU needed.  Never more than a compute unit's 160 KiB. */
 int64_t tg_diag_moe_lds_bytes(int64_t tokens, int64_t top_k, int64_t experts, int64_t hidden, int64_t inter);
 
+/* The form that tg_fp8_kv_attention takes for these sizes: form[0] rows of a tile (16, 32 or 128), form[1] parts that contexts are cut
+ * into (1: uncut, one launch).  The arguments are those of tg_fp8_kv_attention_workspace_bytes.  Host arithmetic, no GPU needed. */
+int32_t tg_diag_kv_attention_form(int64_t tokens, int64_t q_heads, int64_t batch, int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                                  int64_t max_pages, int32_t window, int32_t sink_tokens, int32_t* form);
+
 #ifdef __cplusplus
 }
 #endif

@@ -106,3 +106,41 @@ def ref_attention(q, k: List[torch.Tensor], v: List[torch.Tensor], lens, indptr,
                 if half_step < 2.0 ** -9:
                     tol[row, h] += len(seen) * 2.0 ** -25 * 448 * v_unit
     return out, tol + 1e-30
+
+
+def ref_attention_by_head(q, k: List[torch.Tensor], v: List[torch.Tensor], lens, indptr, scale: float, window: int = 0, sinks: int = 0,
+                          half_step: float = 0.0, v_scale: Optional[List[torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """ref_attention with a head's rows of a sequence in one product, on the tensors' device; v_scale[b] (positions, heads): the scale that
+    each value's code is multiplied by.
+
+    Two terms of the bound are its own.  A weight times its value's scale is an exponential whose argument holds the scale's logarithm: off by
+    2^-24 of that twice.  And in f16 a weight is off by up to half of the smallest step, 2^-25, where the row's largest product of weight and scale stands
+    at 2^7 at least: 2^-32 of that product, times a code of up to 448, for each key; a result is off by 2^-25 below 2^-14."""
+    out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    tol = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    group, f16 = q.shape[1] // (k[0].shape[1] if k else 1), 0 < half_step < 2.0 ** -9
+    for b, length in enumerate(lens):
+        n = indptr[b + 1] - indptr[b]
+        if n == 0 or k[b].shape[0] == 0:
+            continue
+        p = torch.arange(length - n, length, device=q.device)[:, None]
+        j = torch.arange(k[b].shape[0], device=q.device)[None, :]
+        seen = j <= p
+        if window:
+            seen = seen & ((p - j < window) | (j < sinks))
+        some = seen.any(1, keepdim=True)
+        count = seen.sum(1, keepdim=True).double()
+        rows = slice(indptr[b], indptr[b] + n)
+        for h in range(q.shape[1]):
+            kk, vv, qq = k[b][:, h // group].double(), v[b][:, h // group].double(), q[rows, h].double()
+            s = (qq @ kk.t()) * scale
+            w = torch.where(some, torch.softmax(s.masked_fill(~seen & some, -math.inf), 1) * seen, torch.zeros_like(s))
+            out[rows, h] = w @ vv
+            spread = ((qq.abs() @ kk.abs().t()) * seen).amax(1, keepdim=True) * abs(scale)
+            units = torch.ones(kk.shape[0], dtype=torch.float64, device=q.device) if v_scale is None else v_scale[b][:, h // group].double()
+            binades = float(units.log2().abs().max())
+            fp32 = 2 * (q.shape[2] + 8) * 2.0 ** -24 * spread + (8 + count / 16 + binades) * 2.0 ** -23
+            tol[rows, h] = (half_step + fp32) * (w @ vv.abs()) * 1.01 + half_step * out[rows, h].abs()
+            if f16:
+                tol[rows, h] += count * 2.0 ** -32 * 448 * (w * units).amax(1, keepdim=True) + 2.0 ** -25
+    return out, tol + 1e-30

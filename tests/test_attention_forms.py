@@ -1,0 +1,126 @@
+"""kv_cache_attention in each of its forms (tiles of 16, 32 and 128 rows, contexts whole and cut), every test saying which form it runs."""
+
+import ctypes
+import itertools
+import math
+
+import pytest
+import torch
+
+from oracle import decoder_reference as R
+from tilegym_amd import _lib, ops
+
+from .test_decoder_ops import BF16, F16, HALF, Pool
+
+
+def form_of(tokens, q_heads, batch, kv_heads, dim, page, width, window=0, sinks=0):
+    """(rows of a tile, parts that contexts are cut into)."""
+    out = (ctypes.c_int32 * 2)()
+    assert _lib.load().tg_diag_kv_attention_form(tokens, q_heads, batch, kv_heads, dim, page, width, window, sinks, out) == 0
+    return tuple(out)
+
+
+def test_form_query_needs_no_device():
+    out = (ctypes.c_int32 * 2)()
+    query = _lib.load().tg_diag_kv_attention_form
+    assert query(0, 4, 1, 1, 64, 16, 1, 0, 0, out) == -6 and query(1, 4, 1, 3, 64, 16, 1, 0, 0, out) == -6 and query(1, 4, 1, 1, 64, 16, 1, -1, 0, out) == -6
+    assert query(2 ** 62, 4, 1, 1, 64, 16, 1, 0, 0, out) == -6
+    assert query(1, 4, 1, 1, 64, 16, 1, 0, 0, None) == -5
+    assert form_of(1, 4, 1, 1, 64, 16, 1) == (16, 1)
+    # cut exactly where there is scratch memory to be had
+    need = _lib.load().tg_fp8_kv_attention_workspace_bytes
+    for sizes in itertools.product((1, 40, 600), (8, 32), (1, 9), (8,), (64, 128, 256), (16, 128), (1, 30), (0, 500), (0,)):
+        assert (form_of(*sizes)[1] > 1) == (need(*sizes) > 0), sizes
+
+
+def test_oracle_by_head_agrees():
+    g = torch.Generator().manual_seed(2)
+    lens, indptr = [9, 3, 40], [0, 4, 9, 11]  # (sequence 1 has fewer tokens than new ones)
+    k, v = ([torch.randn(n, 2, 64, generator=g, dtype=torch.float64) for n in lens] for _ in range(2))
+    q = torch.randn(11, 6, 64, generator=g)
+    for window, sinks in ((0, 0), (3, 0), (5, 2)):
+        a, tol = R.ref_attention(q, k, v, lens, indptr, 0.2, window, sinks, 2.0 ** -8)
+        b, tol2 = R.ref_attention_by_head(q, k, v, lens, indptr, 0.2, window, sinks, 2.0 ** -8)
+        assert bool(((a - b).abs() <= 1e-12).all()) and bool(((tol - tol2).abs() <= 1e-3 * tol + 1e-12).all())
+
+
+class Forms(Pool):
+    """A pool whose tables list pages in turn, with the scale of every position."""
+
+    def scales(self, lens):
+        s = self.cache.v_scale.double()
+        return [torch.cat([s[p][None].expand(self.page, -1) if 0 <= p < s.shape[0] else torch.ones(self.page, s.shape[1], dtype=torch.float64, device=s.device)
+                           for p in self.table[b]])[:n] for b, n in enumerate(lens)]
+
+    def rows(self, name, lens):
+        """Of the positions that the table has; pages that are not there are zeros (no token sees them)."""
+        return [x.nan_to_num(0.0).to(self.device) for x in super().rows(name, lens)]
+
+    def queries(self, tokens, heads, dtype, factor=1.0):
+        wide = torch.randn(tokens, heads + 3, self.dim, generator=self.g) * factor
+        return wide.to(dtype).to(self.device)[:, 2:2 + heads]
+
+    def attend(self, q, lens, news, window=0, sinks=0, sm_scale=None, table=None):
+        indptr = [0] + list(itertools.accumulate(news))
+        got = ops.kv_cache_attention(q, self.cache, self.i32(table or self.table), self.i32(lens), self.i32(indptr), sm_scale=sm_scale, window=window,
+                                     sink_tokens=sinks)
+        return got, indptr
+
+    def check(self, q, lens, news, window=0, sinks=0, sm_scale=None, table=None):
+        got, indptr = self.attend(q, lens, news, window, sinks, sm_scale, table)
+        scale = self.dim ** -0.5 if sm_scale is None else sm_scale
+        want, tol = R.ref_attention_by_head(q, self.rows("k", lens), self.rows("v", lens), lens, indptr, scale, window, sinks, HALF[q.dtype], self.scales(lens))
+        err = (got.double() - want).abs()
+        assert bool((err <= tol).all()), (float((err / tol).nan_to_num(math.inf).max()), lens, news, window, sinks)
+        return got
+
+
+# (rows of a tile, whether contexts are cut): heads, query heads to each, head dims, (lengths, new tokens)
+FORMS = {
+    (16, False): (2, 4, (64, 128, 256), ([1000, 90, 700], [3, 5, 1])),
+    (16, True): (2, 4, (64, 128, 256), ([1900, 90, 700], [3, 5, 1])),
+    (32, False): (2, 5, (64, 128), ([1000, 130], [150, 30])),
+    (32, True): (2, 5, (64, 128), ([1900, 130], [150, 30])),
+    (128, False): (8, 4, (64, 128, 256), ([1000, 90], [281, 40])),
+    (128, True): (8, 4, (64, 128, 256), ([1900, 90], [281, 40])),
+}
+CASES = [(form, dim) for form, (_, _, dims, _) in FORMS.items() for dim in dims]
+
+
+def _pool_of(device, form, dim, page, dtype):
+    heads, group, _, (lens, news) = FORMS[form]
+    width = -(-max(lens) // page)
+    pool = Forms(device, width * len(lens), heads, page, dim, len(lens), width, seed=dim + page)
+    pool.fill(lens, lens, dtype)
+    return pool, group, lens, news, width
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form,dim", CASES)
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_form(device, form, dim, page, dtype):
+    """Many steps of keys; then a window with first tokens, whose unseen pages are not there."""
+    pool, group, lens, news, width = _pool_of(device, form, dim, page, dtype)
+    heads = pool.heads * group
+    q = pool.queries(sum(news), heads, dtype, 3.0)
+    for window, sinks in ((0, 0), (950 if form[1] else 300, 70), (33, 0)):
+        rows, parts = form_of(sum(news), heads, len(lens), pool.heads, dim, page, width, window, sinks)
+        assert rows == form[0] and (parts > 1) == (form[1] and window != 33)
+        table = [row[:] for row in pool.table]
+        if window:
+            for b, (length, n) in enumerate(zip(lens, news)):
+                first = max(0, length - n - window + 1)
+                for i in range(width):
+                    if i * page >= length or (i * page >= sinks and (i + 1) * page <= first):
+                        table[b][i] = -1 if i % 2 else 10 ** 6
+        pool.check(q, lens, news, window, sinks, table=table)
+    pool.check(q, lens, news, sm_scale=-0.2)
+
+
+def test_sizes_reach_the_forms():
+    for form, dim in CASES:
+        heads, group, _, (lens, news) = FORMS[form]
+        for page in (16, 32, 64, 128):
+            sizes = (sum(news), heads * group, len(lens), heads, dim, page, -(-max(lens) // page))
+            assert form_of(*sizes)[0] == form[0] and (form_of(*sizes)[1] > 1) == form[1], (form, dim, page)

@@ -992,3 +992,38 @@ def test_launches_too_large_for_the_device_are_refused(device):
     # nothing is left behind: a smaller call of the same kind runs
     out = ops.kv_cache_attention(x, cache, table[:1], lens[:1], indptr[:2], out=torch.full_like(x, 3.0))
     assert bool((out == 3).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,hidden", [(600, 4112), (513, 5120), (777, 8192)])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_norm_of_many_rows_of_two_vectors_a_lane(device, rows, hidden, dtype):
+    """512 rows and more of 4097 to 8192 elements have a form of their own."""
+    x, r, w = _norm_case(rows, hidden, dtype, device)
+    *out, norm = ops.rms_norm_quant(x, w, 1e-5, residual=r, group_size=16, return_norm=True)
+    _check_norm(out, x, w, 1e-5, r, 16, None, dtype)
+    _, y = R.ref_rms_norm(x.cpu(), w.cpu(), 1e-5, r.cpu())
+    # f16's numbers below 2^-14 are 2^-24 apart, so a rounding there is off by up to 2^-25, more than 2^-11 of the value; some of these 2.5 to 6
+    # million elements are that small.  (bf16 and fp32 have nothing as coarse near zero.)
+    smallest = 2.0 ** -25 if dtype == F16 else 0.0
+    assert bool(((norm.cpu().double() - y).abs() <= (HALF[dtype] + 2.0 ** -18) * y.abs() + smallest + 2.0 ** -126).all())
+    scale = torch.tensor([0.02], device=device)
+    _check_norm(ops.rms_norm_quant(x, w, 1e-5, group_size=None, scale=scale), x, w, 1e-5, None, None, scale, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page,dim,heads", CACHES)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_append_a_wave_per_page_over_a_border(device, page, dim, heads, dtype):
+    """Mostly one token a sequence, and one sequence with a chunk that ends in a later page than it begins in; a wave writes each page."""
+    batch, chunk = 24, 48
+    pool = Pool(device, batch * 5, heads, page, dim, batch, 5)
+    rope = ops.rope_table(5 * page, dim, device="cpu")
+    lens = [(5 * b) % page for b in range(batch)]
+    lens[2] = page - 5
+    pool.fill(lens, lens, dtype)
+    news = [1] * batch
+    news[2], news[11] = chunk, 0
+    assert sum(news) <= 4 * batch and (lens[2] + chunk - 1) // page > lens[2] // page
+    pool.fill([a + b for a, b in zip(lens, news)], news, dtype, rope)
+    pool.check(True)

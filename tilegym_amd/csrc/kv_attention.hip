@@ -756,6 +756,8 @@ int64_t keys_at_most(const KvAttentionParams& p) {
     return p.window ? std::min<int64_t>(keys, (int64_t)p.window + 128 + ((int64_t)p.sinks + 63) / 64 * 64) : keys;
 }
 
+}  // namespace
+
 // Rows of a tile: 16 or 32 in the form for few rows, 128 in the one for many.  A workgroup of the first runs through its steps fastest with 16 rows,
 // but every tile reads the keys, and a compute unit holds one workgroup.  So (128 elements, 8 heads; us with tiles of 16 / 32 / 128 rows):
 //   16 while the compute units hold all tiles, up to two a sequence, which share an XCD's cache if workgroups 8 apart have the same head (4
@@ -765,7 +767,7 @@ int64_t keys_at_most(const KvAttentionParams& p) {
 //   workgroups' beginnings and ends count (32 of 48 rows: 3000 keys 67 / 53 / 65, 500 keys 29 / 26 / 18; 16 of 96 rows 67 / 51 / 46);
 //   of 256 elements there is no form of 32 rows, and 128 of them spill: 16 up to 32 rows each (64 of 20 rows 185 / - / 254) and
 //   up to twice the compute units (16 of 48 rows 80 / - / 105, of 96 rows 120 / - / 85).
-int tile_rows_of(const KvAttentionParams& p) {
+int kv_attention_tile_rows(const KvAttentionParams& p) {
     const int64_t each = rows_each(p), by16 = tiles_in_all(p, 16), by32 = tiles_in_all(p, 32);
     if (each <= 16 || by16 <= (each <= 32 && p.c.heads % 8 == 0 ? kComputeUnits : kComputeUnits / 4)) return 16;
     if (p.c.dim == 256) return each <= 32 || by16 <= 2 * kComputeUnits ? 16 : 128;
@@ -773,9 +775,11 @@ int tile_rows_of(const KvAttentionParams& p) {
     return keys_at_most(p) > 1024 && (each <= 32 || (each <= 64 && by32 <= 2 * kComputeUnits)) ? 32 : 128;
 }
 
+namespace {
+
 template <typename T, int D>
 hipError_t launch(KvAttentionParams p, hipStream_t s) {
-    const int tile_rows = tile_rows_of(p);
+    const int tile_rows = kv_attention_tile_rows(p);
     const int64_t tiles = row_tiles(p, tile_rows), blocks = tiles * p.c.heads * p.splits;
     const int64_t join = ((int64_t)p.c.rows * p.q_heads * (D / 4) + 255) / 256;
     if (blocks * 64 * kFewWaves<D> > kMostThreads || join * 256 > kMostThreads) return hipErrorInvalidValue;
@@ -805,7 +809,7 @@ hipError_t launch(KvAttentionParams p, hipStream_t s) {
 }  // namespace
 
 int kv_attention_splits(const KvAttentionParams& p) {
-    const int tile_rows = tile_rows_of(p);
+    const int tile_rows = kv_attention_tile_rows(p);
     // Few rows: tiles as far as the host can tell, and a workgroup per compute unit (of 128 elements, two do not fit its registers), never
     // more: 12 sequences of 4000 keys x 8 heads 23.4 us cut in two, 32.5 cut in three (288 workgroups); 20 such uncut 29.6, cut in two 41.2;
     // 8 of 8000 cut in four 27.6, uncut 48.6.  Shares of one size for long and short sequences, counted on the device, were no faster: the

@@ -180,7 +180,8 @@ struct KvAttentionParams {
     float* part_o;                     // (splits, rows * q_heads, dim)
     float* part_ml;                    // (splits, rows * q_heads, 2): running maximum and sum
 };
-// splits the launch should use for these sizes (p.c.rows, batch, heads, width, page_log2, dim, group, window, sinks)
+// rows of a tile, and splits, the launch should use for these sizes (p.c.rows, batch, heads, width, page_log2, dim, group, window, sinks)
+int kv_attention_tile_rows(const KvAttentionParams& p);
 int kv_attention_splits(const KvAttentionParams& p);
 inline int64_t kv_attention_part_bytes(int64_t splits, int64_t rows, int64_t q_heads, int64_t dim) {
     return splits > 1 ? splits * rows * q_heads * (dim + 2) * 4 : 0;

@@ -2162,12 +2162,27 @@ static tg::KvAttentionParams attention_sizes(int64_t tokens, int64_t q_heads, in
     return p;
 }
 
+static bool attention_sizes_in_range(int64_t tokens, int64_t q_heads, int64_t batch, int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                                     int64_t max_pages, int32_t window, int32_t sink_tokens) {
+    return !(tokens < 1 || batch < 1 || kv_heads < 1 || kv_heads > 65536 || q_heads < kv_heads || q_heads % kv_heads != 0 || q_heads > 65536 || head_dim < 1 ||
+             head_dim > 256 || page_size < 16 || page_size > 128 || max_pages < 1 || max_pages > (1 << 24) || batch > (1 << 24) || window < 0 ||
+             sink_tokens < 0 || tokens > INT32_MAX || tokens * q_heads > INT32_MAX);
+}
+
+int32_t tg_diag_kv_attention_form(int64_t tokens, int64_t q_heads, int64_t batch, int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                                  int64_t max_pages, int32_t window, int32_t sink_tokens, int32_t* form) {
+    g_err[0] = 0;
+    if (!form) return fail(TG_ERR_NULL, "form: null pointer");
+    if (!attention_sizes_in_range(tokens, q_heads, batch, kv_heads, head_dim, page_size, max_pages, window, sink_tokens))
+        return fail(TG_ERR_INVALID, "sizes out of range");
+    const tg::KvAttentionParams p = attention_sizes(tokens, q_heads, batch, kv_heads, head_dim, page_size, max_pages, window, sink_tokens);
+    form[0] = tg::kv_attention_tile_rows(p), form[1] = p.splits;
+    return TG_OK;
+}
+
 int64_t tg_fp8_kv_attention_workspace_bytes(int64_t tokens, int64_t q_heads, int64_t batch, int64_t kv_heads, int64_t head_dim, int64_t page_size,
                                             int64_t max_pages, int32_t window, int32_t sink_tokens) {
-    if (tokens < 1 || batch < 1 || kv_heads < 1 || kv_heads > 65536 || q_heads < kv_heads || q_heads % kv_heads != 0 || q_heads > 65536 || head_dim < 1 ||
-        head_dim > 256 || page_size < 16 || page_size > 128 || max_pages < 1 || max_pages > (1 << 24) || batch > (1 << 24) || window < 0 || sink_tokens < 0 ||
-        tokens * q_heads > INT32_MAX)
-        return 0;
+    if (!attention_sizes_in_range(tokens, q_heads, batch, kv_heads, head_dim, page_size, max_pages, window, sink_tokens)) return 0;
     const tg::KvAttentionParams p = attention_sizes(tokens, q_heads, batch, kv_heads, head_dim, page_size, max_pages, window, sink_tokens);
     return tg::kv_attention_part_bytes(p.splits, tokens, q_heads, head_dim);
 }
