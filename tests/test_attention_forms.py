@@ -124,3 +124,36 @@ def test_sizes_reach_the_forms():
         for page in (16, 32, 64, 128):
             sizes = (sum(news), heads * group, len(lens), heads, dim, page, -(-max(lens) // page))
             assert form_of(*sizes)[0] == form[0] and (form_of(*sizes)[1] > 1) == form[1], (form, dim, page)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form,dim", CASES)
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_rows_that_are_no_numbers_show_it(device, form, dim, page, dtype):
+    """A NaN in q, an infinity, and (bf16) one key whose score overflows: those rows come out as no numbers whether contexts are cut or
+    not, and the other rows as ever."""
+    pool, group, lens, news, width = _pool_of(device, form, dim, page, dtype)
+    heads, total = pool.heads * group, sum(news)
+    assert form_of(total, heads, len(lens), pool.heads, dim, page, width)[0] == form[0]
+    key = 700 if form[1] else 70  # (in one part of a cut context)
+    pool.cache.k.view(torch.uint8)[:, :, :, 0] = 0
+    pool.cache.k.view(torch.uint8)[pool.table[0][key // page], :, key % page, 0] = 0x7E  # 448
+    q = pool.queries(total, heads, dtype)
+    clean = q.clone()
+    last = news[0] - 1
+    bad = [(0, 1, math.nan), (last, heads - 1, math.inf), (total - 1, 0, math.nan)]
+    for row, head, x in bad:
+        q[row, head, 3] = x
+    if dtype == BF16:
+        q[last, 2] = 0
+        q[last, 2, 0] = 3e38
+        bad.append((last, 2, 0))
+    got, indptr = pool.attend(q, lens, news)
+    want, tol = R.ref_attention_by_head(clean, pool.rows("k", lens), pool.rows("v", lens), lens, indptr, dim ** -0.5, half_step=HALF[dtype],
+                                        v_scale=pool.scales(lens))
+    spoilt = torch.zeros(total, heads, dtype=torch.bool, device=device)
+    for row, head, _ in bad:
+        spoilt[row, head] = True
+    assert not bool(torch.isfinite(got[spoilt]).any())
+    assert bool(((got[~spoilt].double() - want[~spoilt]).abs() <= tol[~spoilt]).all())

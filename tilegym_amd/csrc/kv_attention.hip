@@ -462,10 +462,10 @@ __global__ void __launch_bounds__(64 * kFewWaves<D>, D == 256 ? 1 : 2) kv_attent
             if (p.splits > 1) {
                 const int64_t at = (int64_t)split * c.rows * p.q_heads + out_row;
                 if (e == 0) p.part_ml[2 * at] = row_top, p.part_ml[2 * at + 1] = sum;
-                if (sum > 0.f) *reinterpret_cast<v4f*>(p.part_o + at * D + e) = x;
+                if (!(sum == 0.f)) *reinterpret_cast<v4f*>(p.part_o + at * D + e) = x;
             } else {
                 typedef T v4t __attribute__((ext_vector_type(4)));
-                x *= sum > 0.f ? 1.0f / sum : 0.f;  // a row that sees nothing is zero
+                x *= sum == 0.f ? 0.f : 1.0f / sum;  // a row that sees nothing is zero; a sum that is no number shows
                 *reinterpret_cast<v4t*>((T*)p.out + out_row * D + e) = __builtin_convertvector(x, v4t);
             }
         }
@@ -668,7 +668,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_rows_kerne
     if (p.splits > 1) {
         const int64_t at = (int64_t)split * c.rows * p.q_heads + out_row;
         if (h == 0) p.part_ml[2 * at] = m, p.part_ml[2 * at + 1] = sum;
-        if (sum > 0.f) {
+        if (!(sum == 0.f)) {
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -677,7 +677,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_rows_kerne
         }
     } else {
         typedef T v4t __attribute__((ext_vector_type(4)));
-        const float f = sum > 0.f ? unit.u / sum : 0.f;  // a row that sees nothing is zero
+        const float f = sum == 0.f ? 0.f : unit.u / sum;  // a row that sees nothing is zero
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -689,7 +689,8 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_rows_kerne
 }
 
 // out = sum over splits of exp2(m_s - m) O_s, over the sum of exp2(m_s - m) l_s, in the order of the splits: D / 4 lanes per row of q.  All
-// splits' m and l, and the first four parts of O, are asked for at once; then O, four in flight.  Parts with no weight were not written.
+// splits' m and l, and the first four parts of O, are asked for at once; then O, four in flight.  Parts with no weight were not written.  Empty is what has a sum of
+// zero and nothing else: a sum that is no number (NaN in q, a score that overflowed) makes the row's sum, and so the row, no number.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv_attention_join_kernel(const KvAttentionParams p) {
     constexpr int QUADS = D / 4, ROWS = 256 / QUADS;
@@ -721,7 +722,7 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const KvAttentio
     const float base = top == kMinusInf ? 0.f : top;
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
-        const float f = l[i] > 0.f ? __builtin_amdgcn_exp2f(m[i] - base) : 0.f;
+        const float f = l[i] == 0.f ? 0.f : __builtin_amdgcn_exp2f(m[i] - base);
         if (lane + i * QUADS < kMostSplits) weight[tid / QUADS][lane + i * QUADS] = f;
         sum += f * l[i];
     }
@@ -740,7 +741,7 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const KvAttentio
         }
     }
     typedef T v4t __attribute__((ext_vector_type(4)));
-    x *= sum > 0.f ? 1.0f / sum : 0.f;
+    x *= sum == 0.f ? 0.f : 1.0f / sum;
     *reinterpret_cast<v4t*>((T*)p.out + row * D + 4 * lane) = __builtin_convertvector(x, v4t);
 }
 
