@@ -370,7 +370,8 @@ int32_t tg_fp8_rms_norm_quant(const tg_tensor* q, const tg_tensor* scales, const
  * tg_fp8_kv_attention: out = softmax(sm_scale q k^T) v, causal: a token sees the positions up to its own, with window > 0 only the
  *   last `window` of them and the positions below sink_tokens.  Pages no token sees need not exist.  q (tokens, H, D) bf16 / f16, H a
  *   multiple of heads: query head h reads cache head h / (H / heads).  out: like q, contiguous, not q.  A token that sees nothing
- *   gets zeros; one whose scores are no numbers (NaN or infinities in q, an fp32 overflow) gets no numbers.  workspace: tg_fp8_kv_attention_workspace_bytes() bytes (0: NULL will do), 16-byte aligned, contents irrelevant; calls
+ *   gets zeros; one whose scores are no numbers (NaN or infinities in q, an fp32 overflow) gets no numbers; one behind
+ *   the table's end sees the positions that the table has.  workspace: tg_fp8_kv_attention_workspace_bytes() bytes (0: NULL will do), 16-byte aligned, contents irrelevant; calls
  *   that share one must not overlap in time.  The codes of live slots must be numbers (tg_fp8_kv_append writes no NaN).
  */
 int32_t tg_fp8_kv_append(const tg_tensor* k_cache, const tg_tensor* v_cache, const tg_tensor* k_scale, const tg_tensor* v_scale, const tg_tensor* k,

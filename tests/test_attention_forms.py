@@ -157,3 +157,20 @@ def test_rows_that_are_no_numbers_show_it(device, form, dim, page, dtype):
         spoilt[row, head] = True
     assert not bool(torch.isfinite(got[spoilt]).any())
     assert bool(((got[~spoilt].double() - want[~spoilt]).abs() <= tol[~spoilt]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form,dim", CASES)
+@pytest.mark.parametrize("page", [16, 32, 64])
+def test_lengths_beyond_the_table_see_what_the_table_has(device, form, dim, page):
+    """Tables that end inside a step of 64 keys, lengths behind their end."""
+    heads, group, _, (lens, news) = FORMS[form]
+    width = (max(lens) // page - 1) // 2 * 2 + 1
+    capacity = width * page
+    assert form_of(sum(news), heads * group, len(lens), heads, dim, page, width)[0] == form[0]
+    pool = Forms(device, width * len(lens), heads, page, dim, len(lens), width)
+    pool.fill([capacity] + lens[1:], [capacity] + lens[1:])
+    q = pool.queries(sum(news), heads * group, BF16)
+    for beyond in (1, 40, 64, 1000):
+        pool.check(q, [capacity + beyond] + lens[1:], news)
+        pool.check(q, [capacity + beyond] + lens[1:], news, window=500, sinks=20)

@@ -138,6 +138,13 @@ __device__ __forceinline__ Granule page_of(const KvCache& c, int entry) {
     g.page = g.there ? entry : 0;
     return g;
 }
+// The same for 16 keys from `key` on, which may lie behind the table's end: a table of pages of 16 or 32 can end inside a step of 64 keys, and
+// table_entry then gives its last page.  (Positions behind the end are possible too: they see what the table has.)
+__device__ __forceinline__ Granule page_of(const KvCache& c, int entry, int key) {
+    Granule g = page_of(c, entry);
+    g.there = g.there && (key >> c.page_log2) < c.width;
+    return g;
+}
 
 // Bytes of 16 codes of v that some row sees: those of keys first .. first + 15 that lie in [key0, key1) or among the sinks, all or none
 // towards the lower end (earlier keys of the same page are numbers), and exactly towards the upper (later slots may hold anything).
@@ -296,8 +303,8 @@ __global__ void __launch_bounds__(64 * kFewWaves<D>, D == 256 ? 1 : 2) kv_attent
     };
     const int k_lane = k_key * D + g * 16, v_lane = col * P + 16 * g;
     auto load_k = [&](int step) {
-        v_page = page_of(c, v_entry);
         const int key = t.key_of(step);
+        v_page = ONE ? page_of(c, v_entry) : page_of(c, v_entry, key + 16 * g);
         const int64_t at = (int64_t)v_page.page * c.heads + t.head;
         if constexpr (ONE) {
             const uint8_t* base = c.k + at * head_bytes + (key & in_page) * D;
@@ -540,7 +547,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_rows_kerne
         } else {
 #pragma unroll
             for (int i = 0; i < HALVES; ++i) {
-                there[i] = page_of(c, entry[i]);
+                there[i] = page_of(c, entry[i], key + 32 * i + 16 * h);
                 const int64_t at = (int64_t)there[i].page * c.heads + head;
                 k_scale[i] = c.k_scale[at], v_scale[i] = c.v_scale[at];
             }

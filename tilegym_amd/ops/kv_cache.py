@@ -127,7 +127,8 @@ def kv_cache_attention(
 
     A token sees the positions up to its own; with ``window`` > 0 only the last ``window`` of them (its own included) and the
     first ``sink_tokens`` of the sequence.  Pages that no token sees need not exist (their table entries may be -1).  A
-    token that sees nothing gets zeros; one whose scores are no numbers (NaN or infinities in q) gets no numbers.  Results do not depend on what unwritten slots hold, and a call gives the same bits every time.
+    token that sees nothing gets zeros; one whose scores are no numbers (NaN or infinities in q) gets no numbers; one behind the table's
+    end sees the positions that the table has.  Results do not depend on what unwritten slots hold, and a call gives the same bits every time.
 
     Returns (tokens, heads, D) of q's type; ``out`` (contiguous, not q) is written if given.  Rows of no sequence are left as they were
     in ``out``, and unset without it."""
