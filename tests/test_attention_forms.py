@@ -174,3 +174,29 @@ def test_lengths_beyond_the_table_see_what_the_table_has(device, form, dim, page
     for beyond in (1, 40, 64, 1000):
         pool.check(q, [capacity + beyond] + lens[1:], news)
         pool.check(q, [capacity + beyond] + lens[1:], news, window=500, sinks=20)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form,dim", CASES)
+@pytest.mark.parametrize("page,run", [(16, 1), (64, 1), (64, 9)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("small", [0.003, 0.0])
+def test_rows_on_pages_of_very_different_sizes(device, form, dim, page, run, dtype, small):
+    """Values of 30000 in every other page (or run of pages, so that a wave that takes every eighth step meets both) and of 0.003 or
+    zero between them, scales 2^23 or 2^48 apart: rows whose weight lies on the small ones, beside rows on the large ones and rows on both."""
+    heads, group, _, (lens, news) = FORMS[form]
+    width = -(-max(lens) // page)
+    assert form_of(sum(news), heads * group, len(lens), heads, dim, page, width)[0] == form[0]
+    pool = Forms(device, width * len(lens), heads, page, dim, len(lens), width)
+    indptr = [0] + list(itertools.accumulate(lens))
+    k, v = (torch.randn(indptr[-1], heads, dim, generator=pool.g) for _ in range(2))
+    odd = torch.cat([torch.arange(n) // page // run % 2 for n in lens])[:, None]
+    k[..., 0] = 8.0 * odd - 4.0
+    v = v.clamp(-2, 2) * torch.where(odd == 1, small, 30000.0)[..., None]
+    i32 = pool.i32
+    ops.kv_cache_append(pool.cache, k.to(dtype).to(device), v.to(dtype).to(device), i32(pool.table), i32(lens), i32(indptr))
+    assert float(pool.cache.v_scale[pool.table[0][0], 0] / pool.cache.v_scale[pool.table[0][run], 0]) >= 2.0 ** 22
+    q = torch.randn(sum(news), heads * group, dim, generator=pool.g) * 0.1
+    q[..., 0] = torch.randint(-1, 2, q.shape[:2], generator=pool.g) * 10.0
+    q[0, :, 0] = 10.0
+    pool.check(q.to(dtype).to(device), lens, news, sm_scale=1.0)

@@ -11,9 +11,9 @@
 // that lane group g ends up with the 16 consecutive keys 16 g ... of its row.  Those are, in order, the second product's operand, and
 // the cache's transposed v has them in 16 consecutive bytes.  They lie in one page (P is a multiple of 16), so scales are
 // one value per lane.
-// Codes become the 16-bit type of q exactly (e4m3 has 4 significant bits).  k's scale joins the softmax's factor.  v's scale: O is
-// held in units of the largest one seen, u (or a 128th of it); P is multiplied by v_scale / u before it is rounded to 16 bits (2^-9 relative in
-// bf16, 2^-12 in f16, of its own value), where a page differs from that.  S, m, l and O are fp32.
+// Codes become the 16-bit type of q exactly (e4m3 has 4 significant bits).  k's scale joins the softmax's factor.  v's scale joins the softmax's
+// exponent: m is the maximum of a row's c q.k + log2 v_scale, and P, rounded to 16 bits, is exp2 of that less m (off by 2^-9 relative in bf16, 2^-12 in f16, of its own value,
+// in f16 by no more than 2^-32 of the row's largest where that is more).  S, m, l and O are fp32.
 //
 // What is not seen is taken out by selection, never by arithmetic: scores before the maximum, and v's codes, since 0 x NaN is NaN
 // and a page's unwritten slots may hold anything.
@@ -69,7 +69,6 @@ __device__ __forceinline__ X vector_load(const X* at) {
 }
 
 constexpr float kMinusInf = -__builtin_inff();
-constexpr float kSmallestUnit = 0x1p-126f;
 // The maximum that a row's scores are taken against is looked for only when 16 weights against the old one add up to more than this: floating
 // point loses no precision in weights above 1 (f16 holds 16 times as much, and sums and O are fp32; a maximum's 16 weights are 2048 at most).  A row's first keys find a maximum of
 // -inf and so a sum that is not a number, and take the same path.  In the other steps there is no search, no exchange between lanes
@@ -184,38 +183,31 @@ __device__ __forceinline__ void select_seen(S& s, int key, int position, int win
     }
 }
 
-// v's scale against the unit u that O is held in; lanes hold the scales of their own 16 keys.  u is the largest scale seen, in f16 a 128th of it: weights
-// against the maximum are then 128 times as large, and one that f16's smallest step swallows is below 2^-32 of the maximum's and not 2^-25, which tens
-// of thousands of faint keys beside one strong one would add up to more than a rounding of the result.
+// v's scale in a lane's 16 keys of a step: it joins the weight's exponent, so that P is p v_scale against the row's largest such product so far (2^m), and
+// is taken out of the sum again.  What 16 bits lose of a weight is then measured by what the row itself adds up, whatever scales other rows and
+// pages without weight have.  In f16 weights stand 128 times as high: one that f16's smallest step swallows is below 2^-32 of the row's largest
+// product and not 2^-25, which tens of thousands of faint keys beside one strong one would add up to more than a rounding of the result.  Times a
+// code it is at most 2^-23 of the largest product; e4m3 itself rounds that key's value by up to 2^-10 of it, or more.
 template <typename T>
-struct Unit {
+struct ValueScale {
     static constexpr int kUp = std::is_same_v<T, __bf16> ? 0 : 7;
-    static constexpr float kDown = 1.f / (1 << kUp);
-    float u = kSmallestUnit, inverse = 0x1p126f;
-    float grown = 1.f;                 // this step: u before / u now
-    float lift, back;                  // this step: log2(v_scale / u), u / v_scale
-    // seen: whether any key of the lane's 16 is seen (the scale of the others may be anything)
-    __device__ __forceinline__ void step(float v_scale, bool seen) {
-        grown = 1.f;
-        float s = seen ? v_scale * kDown : 0.f;
-        if (__ballot(s > u)) {
-            float top = fmaxf(s, __shfl_xor(s, 16));
-            top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), u);
-            top = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(top)));  // (the same in all lanes)
-            grown = u / top;
-            u = top, inverse = 1.f / top;
-        }
-        s = fmaxf(s * inverse, 0x1p-100f);  // (no keys, or a scale of zero: any finite logarithm will do)
-        lift = __builtin_amdgcn_logf(s) + (float)kUp, back = __builtin_amdgcn_rcpf(s) * kDown;
+    static constexpr float kDown = 1.f / (1 << kUp);  // O is held in units of 2^m kDown
+    float log, back;
+    // seen: whether any key of the lane's 16 is seen (the scale of the others may be anything).  Scales are 2^-40 to 2^40 as written; others are held
+    // within what fp32 sums of 1 / scale can take
+    __device__ __forceinline__ void set(float v_scale, bool seen) {
+        const float s = __builtin_amdgcn_fmed3f(seen ? v_scale : 1.f, 0x1p-64f, 0x1p100f);
+        log = __builtin_amdgcn_logf(s), back = __builtin_amdgcn_rcpf(s) * kDown;
     }
 };
 
-// One row's 16 scores of a step -> its weights, against the running maximum m and in units of u, and its sum l.  Returns what O has to
+// One row's 16 scores of a step -> its weights against the running maximum m, and its sum l of exp2(score - m).  Returns what O has to
 // be multiplied by on m's account.  factor > 0.
 template <typename T, typename S>
-__device__ __forceinline__ float weigh(const S& s, float factor, const Unit<T>& unit, float& m, float& l, typename Types<T>::v8 (&pt)[2]) {
+__device__ __forceinline__ float weigh(const S& s, float factor, const ValueScale<T>& v, float& m, float& l, typename Types<T>::v8 (&pt)[2]) {
     v16f w;
-    float shrink = 1.f, base = unit.lift - m, sum = 0.f;
+    const float lift = v.log + (float)ValueScale<T>::kUp;
+    float shrink = 1.f, base = lift - m, sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], factor, base));
@@ -225,6 +217,7 @@ __device__ __forceinline__ float weigh(const S& s, float factor, const Unit<T>& 
         float top = kMinusInf;
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i] * factor);
+        top += v.log;
 #pragma unroll
         for (int d = S::kFirstLane; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
         top = fmaxf(m, top);
@@ -232,7 +225,7 @@ __device__ __forceinline__ float weigh(const S& s, float factor, const Unit<T>& 
         shrink = __builtin_amdgcn_exp2f(m - finite);
         l *= shrink;
         m = top;
-        base = unit.lift - finite;
+        base = lift - finite;
         sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -240,7 +233,7 @@ __device__ __forceinline__ float weigh(const S& s, float factor, const Unit<T>& 
             sum += w[i];
         }
     }
-    l = __builtin_fmaf(sum, unit.back, l);
+    l = __builtin_fmaf(sum, v.back, l);
     pt[0] = __builtin_convertvector(__builtin_shufflevector(w, w, 0, 1, 2, 3, 4, 5, 6, 7), typename Types<T>::v8);
     pt[1] = __builtin_convertvector(__builtin_shufflevector(w, w, 8, 9, 10, 11, 12, 13, 14, 15), typename Types<T>::v8);
     return shrink;
@@ -370,7 +363,6 @@ __global__ void __launch_bounds__(64 * kFewWaves<D>, D == 256 ? 1 : 2) kv_attent
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[n][d] = v4f{0.f, 0.f, 0.f, 0.f};
-    Unit<T> unit;
 
     for (int step = mine; step < end; step += WAVES) {
         const int key = t.key_of(step), first = key + 16 * g;
@@ -393,7 +385,8 @@ __global__ void __launch_bounds__(64 * kFewWaves<D>, D == 256 ? 1 : 2) kv_attent
         if (step + WAVES < end) load_k(step + WAVES);
         // every key of the step seen by every row: nothing to select
         const bool whole = key + 63 <= t.low && (!p.window || key > t.high - p.window) && __ballot(!there.there) == 0;
-        unit.step(v_scale, whole || (there.there && first < t.key1 && (first + 16 > t.key0 || first < p.sinks)));
+        ValueScale<T> value;
+        value.set(v_scale, whole || (there.there && first < t.key1 && (first + 16 > t.key0 || first < p.sinks)));
         if (!whole) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) select_seen(s[n], first, position[n], p.window, p.sinks, there.there);
@@ -402,10 +395,10 @@ __global__ void __launch_bounds__(64 * kFewWaves<D>, D == 256 ? 1 : 2) kv_attent
         }
         v8 pt[NT][2];
         float rescale[NT];
-        bool any = unit.grown != 1.f;
+        bool any = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            rescale[n] = weigh<T>(s[n], factor, unit, m[n], l[n], pt[n]) * unit.grown;
+            rescale[n] = weigh<T>(s[n], factor, value, m[n], l[n], pt[n]);
             any = any || rescale[n] != 1.f;
         }
         if (__ballot(any)) {
@@ -429,10 +422,9 @@ __global__ void __launch_bounds__(64 * kFewWaves<D>, D == 256 ? 1 : 2) kv_attent
         }
     }
 
-    // the waves' results: m, l and u, then O, each in units of the largest
-    __shared__ float part_m[WAVES][ROWS], part_l[WAVES][ROWS], part_u[WAVES];
+    // the waves' results: m and l, then O, each in units of the largest
+    __shared__ float part_m[WAVES][ROWS], part_l[WAVES][ROWS];
     __shared__ float part_o[WAVES][16][D + 4];
-    if (lane == 0) part_u[wave] = unit.u;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         l[n] += __shfl_xor(l[n], 16);
@@ -442,10 +434,10 @@ __global__ void __launch_bounds__(64 * kFewWaves<D>, D == 256 ? 1 : 2) kv_attent
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         __syncthreads();
-        float top = part_m[0][n * 16 + col], u = part_u[0];
+        float top = part_m[0][n * 16 + col];
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) top = fmaxf(top, part_m[w][n * 16 + col]), u = fmaxf(u, part_u[w]);
-        const float base = top == kMinusInf ? 0.f : top, f = __builtin_amdgcn_exp2f(m[n] - base) * (unit.u / u);
+        for (int w = 1; w < WAVES; ++w) top = fmaxf(top, part_m[w][n * 16 + col]);
+        const float base = top == kMinusInf ? 0.f : top, f = __builtin_amdgcn_exp2f(m[n] - base) * ValueScale<T>::kDown;
 #pragma unroll
         for (int d = 0; d < DT; ++d) *reinterpret_cast<v4f*>(&part_o[wave][col][d * 16 + 4 * g]) = o[n][d] * f;
         __syncthreads();
@@ -464,7 +456,6 @@ __global__ void __launch_bounds__(64 * kFewWaves<D>, D == 256 ? 1 : 2) kv_attent
                 sum += part_l[w][n * 16 + row] * __builtin_amdgcn_exp2f(part_m[w][n * 16 + row] - row_base);
                 x += *reinterpret_cast<const v4f*>(&part_o[w][row][e]);
             }
-            x *= u;
             const int64_t out_row = (int64_t)(t.first + rr / p.group) * p.q_heads + t.head * p.group + rr % p.group;
             if (p.splits > 1) {
                 const int64_t at = (int64_t)split * c.rows * p.q_heads + out_row;
@@ -482,7 +473,7 @@ __global__ void __launch_bounds__(64 * kFewWaves<D>, D == 256 ? 1 : 2) kv_attent
 // Many rows: 128 of them per workgroup, 32 per wave, and every wave runs over the same keys, whose codes go to LDS for all four
 // without a register between, the next step's while this one's products run, in two buffers with one barrier a step.  Codes stay
 // e4m3 in LDS (half the reads that 16 bits would cost) and are widened behind each read, for 32 rows.  Bound by the SIMDs' issue, products and the
-// softmax's and widening's vector instructions sharing them, two waves each: 4096 tokens of 3 sequences x 32 heads over 1500 to 4500 keys 180 us, 860
+// softmax's and widening's vector instructions sharing them, two waves each: 4096 tokens of 3 sequences x 32 heads over 1500 to 4500 keys 176 us, 880
 // TFLOP/s (a large 16-bit product: 1205); with 16 bits in LDS 4 % more, with three waves per SIMD spills.
 // The products are 32x32x16 instructions on 32 keys at a time, the same way round: S^T row 8 a + 4 h + b stands for key 16 h + 4 a + b, so a
 // lane (row lane % 32, h = lane / 32) has 16 consecutive keys of its one row.
@@ -592,7 +583,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_rows_kerne
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = v16f{};
     float m = live ? kMinusInf : 0.f, l = 0.f;
-    Unit<T> unit;
+    ValueScale<T> value;
     const int s_key = 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3);  // the key that this lane reads as a row of K, of 32
     const int k_lane = s_key * D + (h ^ k_swizzle<D>(s_key)) * 16, v_lane = col * 64 + (h ^ v_swizzle(col)) * 16;
     for (int step = begin; step < end; ++step, key = key1, key1 = key2) {
@@ -610,7 +601,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_rows_kerne
         }
         if (key >= none) continue;
         // (with ONE, a scalar: whether any key of the step's page is seen by the tile)
-        if constexpr (ONE) unit.step(this_v_scale[0], page_there[0] && key < t.key1 && (key + 64 > t.key0 || key < p.sinks));
+        if constexpr (ONE) value.set(this_v_scale[0], page_there[0] && key < t.key1 && (key + 64 > t.key0 || key < p.sinks));
         // fragments are asked for a phase ahead (k's of the second half in front of the first half's second product, v's in front of
         // the softmax), pinned by fences: behind each other, a read's latency and its use would add up 16 times a step
         // (the chunks of a fragment's rows differ from the first one's in an exclusive or of their number, which the swizzle leaves alone)
@@ -643,7 +634,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_rows_kerne
                 whole = whole && page_there[0];
             } else {
                 whole = whole && __ballot(!page_there[i_h]) == 0;
-                unit.step(this_v_scale[i_h], whole || (page_there[i_h] && first < t.key1 && (first + 16 > t.key0 || first < p.sinks)));
+                value.set(this_v_scale[i_h], whole || (page_there[i_h] && first < t.key1 && (first + 16 > t.key0 || first < p.sinks)));
             }
             if (!whole) {
                 asm volatile("");  // (keeps the selection a branch)
@@ -652,8 +643,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_rows_kerne
                 for (int d = 0; d < DT; ++d) vc[d] = seen_codes(vc[d], t, p.sinks, first, page_there[i_h]);
             }
             v8 pt[2];
-            float rescale = weigh<T>(s, factor[i_h], unit, m, l, pt);
-            if (!ONE || half == 0) rescale *= unit.grown;
+            const float rescale = weigh<T>(s, factor[i_h], value, m, l, pt);
             if (__ballot(rescale != 1.f)) {
 #pragma unroll
                 for (int d = 0; d < DT; ++d) o[d] *= rescale;
@@ -680,11 +670,11 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) kv_attention_rows_kerne
             for (int d = 0; d < DT; ++d)
 #pragma unroll
                 for (int a = 0; a < 4; ++a)
-                    *reinterpret_cast<v4f*>(p.part_o + at * D + d * 32 + 8 * a + 4 * h) = v4f{o[d][4 * a], o[d][4 * a + 1], o[d][4 * a + 2], o[d][4 * a + 3]} * unit.u;
+                    *reinterpret_cast<v4f*>(p.part_o + at * D + d * 32 + 8 * a + 4 * h) = v4f{o[d][4 * a], o[d][4 * a + 1], o[d][4 * a + 2], o[d][4 * a + 3]} * ValueScale<T>::kDown;
         }
     } else {
         typedef T v4t __attribute__((ext_vector_type(4)));
-        const float f = sum == 0.f ? 0.f : unit.u / sum;  // a row that sees nothing is zero
+        const float f = sum == 0.f ? 0.f : ValueScale<T>::kDown / sum;  // a row that sees nothing is zero
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
