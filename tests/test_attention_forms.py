@@ -200,3 +200,57 @@ def test_rows_on_pages_of_very_different_sizes(device, form, dim, page, run, dty
     q[..., 0] = torch.randint(-1, 2, q.shape[:2], generator=pool.g) * 10.0
     q[0, :, 0] = 10.0
     pool.check(q.to(dtype).to(device), lens, news, sm_scale=1.0)
+
+
+def _described(ptr, shape, strides, dtype):
+    """A descriptor of a tensor that does not exist (for refusals, which look at nothing else)."""
+    d = _lib.TgTensor()
+    d.ptr, d.ndim, d.dtype = ptr, len(shape), dtype
+    for i, (n, s) in enumerate(zip(shape, strides)):
+        d.shape[i], d.strides[i] = n, s
+    return ctypes.byref(d)
+
+
+def _rc_of_sizes(tokens, q_heads, kv_heads, dim, batch=1, width=1, page=16):
+    """What attention over sizes that no memory holds returns: -4 (there is no device 999) where it would have gone on to launch."""
+    dense = lambda *s: (s, [math.prod(s[i + 1:]) for i in range(len(s))])  # noqa: E731
+    t = lambda dtype, *s: _described(1 << 20, *dense(*s), dtype)  # noqa: E731
+    codes = {d: _lib.make_tensor_desc(torch.zeros(1, dtype=d)).dtype for d in (BF16, torch.float8_e4m3fn, torch.float32, torch.int32)}
+    e4m3, f32, i32 = codes[torch.float8_e4m3fn], codes[torch.float32], codes[torch.int32]
+    x = t(codes[BF16], tokens, q_heads, dim)
+    out = _described(1 << 21, *dense(tokens, q_heads, dim), codes[BF16])
+    rc = _lib.load().tg_fp8_kv_attention(out, x, t(e4m3, 1, kv_heads, page, dim), t(e4m3, 1, kv_heads, dim, page), t(f32, 1, kv_heads), t(f32, 1, kv_heads),
+                                         t(i32, batch, width), t(i32, batch), t(i32, batch + 1), 1.0, 0, 0, None, 999, 0)
+    return rc, _lib.load().tg_last_error().decode()
+
+
+def test_launches_are_refused_by_the_threads_that_they_have():
+    # no join where contexts are whole: 2^34 elements and more of a result are no reason
+    for dim in (64, 128, 256):
+        assert form_of(1 << 20, 128, 1, 128, dim, 16, 1) == (128, 1)
+        assert _rc_of_sizes(1 << 20, 128, 128, dim)[0] == -4
+    # 128-row tiles have 256 threads: 2^23 + 2^22 of them can be launched
+    for dim in (64, 128, 256):
+        assert _rc_of_sizes(3 << 22, 128, 128, dim)[0] == -4
+    tokens = (1 << 28) - 129  # (2^21 - 1 tiles for each of 7 heads)
+    assert tokens * 7 <= 2 ** 31 - 1 and form_of(tokens, 7, 1, 7, 64, 16, 1) == (128, 1) and _rc_of_sizes(tokens, 7, 7, 64)[0] == -4
+    batch = 1 << 15
+    assert form_of(batch, 1024, batch, 1024, 128, 16, 1) == (16, 1)
+    rc, said = _rc_of_sizes(batch, 1024, 1024, 128, batch=batch)
+    assert rc == -6 and "threads" in said and "kv_cache_attention" in said
+
+
+@pytest.mark.gpu
+def test_a_result_of_more_than_2_to_the_34_elements(device):
+    """Contexts that are whole need no join, whose launch would be too large."""
+    tokens, heads, dim = 1 << 20, 64, 256
+    assert tokens * heads * dim >= 2 ** 34 and form_of(tokens, heads, 1, heads, dim, 16, 1) == (128, 1)
+    pool = Forms(device, 1, heads, 16, dim, 1, 1)
+    pool.fill([16], [16])
+    one = pool.queries(1, heads, BF16)
+    got = ops.kv_cache_attention(one.expand(tokens, heads, dim), pool.cache, pool.i32(pool.table), pool.i32([tokens]), pool.i32([0, tokens]))
+    want = ops.kv_cache_attention(one.expand(150, heads, dim), pool.cache, pool.i32(pool.table), pool.i32([150]), pool.i32([0, 150]))
+    assert form_of(150, heads, 1, heads, dim, 16, 1) == (128, 1)
+    assert torch.equal(got[:150], want)
+    for at in (1 << 15, (1 << 19) - 3, 1 << 19, tokens - 5):
+        assert torch.equal(got[at:at + 5], want[20:21].expand(5, heads, dim))

@@ -746,6 +746,8 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const KvAttentio
 int64_t row_tiles(const KvAttentionParams& p, int64_t tile_rows) { return (int64_t)p.c.rows * p.group / tile_rows + p.c.batch; }
 // Rows that a sequence's key/value head has on average, and tiles of so many in all sequences and heads: the host does not read the tensors.
 int64_t rows_each(const KvAttentionParams& p) { return ((int64_t)p.c.rows * p.group + p.c.batch - 1) / p.c.batch; }
+int64_t attention_blocks(const KvAttentionParams& p, int64_t tile_rows) { return row_tiles(p, tile_rows) * p.c.heads * p.splits; }
+int64_t join_blocks(const KvAttentionParams& p) { return ((int64_t)p.c.rows * p.q_heads * (p.c.dim / 4) + 255) / 256; }
 int64_t tiles_in_all(const KvAttentionParams& p, int64_t tile_rows) { return p.c.batch * ((rows_each(p) + tile_rows - 1) / tile_rows) * p.c.heads; }
 
 // Keys that a tile can see, as far as the host can tell.
@@ -778,9 +780,7 @@ namespace {
 template <typename T, int D>
 hipError_t launch(KvAttentionParams p, hipStream_t s) {
     const int tile_rows = kv_attention_tile_rows(p);
-    const int64_t tiles = row_tiles(p, tile_rows), blocks = tiles * p.c.heads * p.splits;
-    const int64_t join = ((int64_t)p.c.rows * p.q_heads * (D / 4) + 255) / 256;
-    if (blocks * 64 * kFewWaves<D> > kMostThreads || join * 256 > kMostThreads) return hipErrorInvalidValue;
+    const int64_t blocks = attention_blocks(p, tile_rows);
     const dim3 grid((unsigned)blocks), block(256);
     // more workgroups than compute units, whole sequences each: the long ones first, and the short ones fill in behind them (64 sequences of 100
     // to 8000 keys 98 us, in their own order 110; 40 of them 74 and 83; of 4000 each 101 and 100)
@@ -800,7 +800,7 @@ hipError_t launch(KvAttentionParams p, hipStream_t s) {
 #undef TG_FEW
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
-    hipLaunchKernelGGL((kv_attention_join_kernel<T, D>), dim3((unsigned)join), block, 0, s, p);
+    hipLaunchKernelGGL((kv_attention_join_kernel<T, D>), dim3((unsigned)join_blocks(p)), block, 0, s, p);
     return hipGetLastError();
 }
 
@@ -817,6 +817,11 @@ int kv_attention_splits(const KvAttentionParams& p) {
     const int64_t steps = (keys_at_most(p) + 63) / 64, workgroups = tile_rows != 128 ? kComputeUnits : 2 * kComputeUnits;
     const int64_t wanted = tile_rows != 128 ? workgroups / units : (workgroups + units / 2) / units, most = steps <= 2 * kLeastSteps ? 1 : (steps + kLeastSteps - 1) / kLeastSteps;
     return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(wanted, most), kMostSplits));
+}
+
+int64_t kv_attention_threads(const KvAttentionParams& p) {
+    const int tile_rows = kv_attention_tile_rows(p), waves = tile_rows == 128 ? 4 : p.c.dim == 256 ? kFewWaves<256> : kFewWaves<128>;
+    return std::max(attention_blocks(p, tile_rows) * 64 * waves, p.splits > 1 ? join_blocks(p) * 256 : 0);
 }
 
 hipError_t run_kv_attention(const KvAttentionParams& p, bool is_bf16, hipStream_t s) {

@@ -303,29 +303,51 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvReadParams p) {
 
 }  // namespace
 
-template <typename T>
-static hipError_t launch_kv_append(const KvAppendParams& p, hipStream_t s) {
+namespace {
+struct AppendPlan {
+    int64_t items, cache_blocks, blocks, block_waves, q_waves;
+    bool single, many;
+};
+AppendPlan append_plan(const KvAppendParams& p) {
     const KvCache& c = p.c;
-    const int64_t P = (int64_t)1 << c.page_log2, items = c.rows / P + 2 * (int64_t)c.batch /* at most: ceil(n / P) + 1 each */, units = items * c.heads * 2;
+    AppendPlan a;
+    const int64_t P = (int64_t)1 << c.page_log2;
+    a.items = c.rows / P + 2 * (int64_t)c.batch;  // at most: ceil(n / P) + 1 each
+    const int64_t units = a.items * c.heads * 2;
     // One wave per page where sequences have up to four new tokens on average, else four, or 16 where that leaves compute units without work
     // and pages and runs are long: a lane's vectors come one after the other.  512 tokens of 8 heads of 128 in pages of 128: 11.8 us with four, 7.7
     // with 16, of 256 20.5 and 11.8; but 2048 of 64 in pages of 64 8.5 and 11.1, runs of 16 tokens 5.0 and 5.9.
-    const bool single = c.rows <= 4 * (int64_t)c.batch;
-    const bool many = !single && units <= 512 && P * c.dim >= 8192 && (int64_t)c.rows * c.dim >= 4096 * (int64_t)c.batch;
-    const int64_t cache_blocks = single ? (units + 3) / 4 : units, block_waves = many ? 16 : 4;
+    a.single = c.rows <= 4 * (int64_t)c.batch;
+    a.many = !a.single && units <= 512 && P * c.dim >= 8192 && (int64_t)c.rows * c.dim >= 4096 * (int64_t)c.batch;
+    a.cache_blocks = a.single ? (units + 3) / 4 : units, a.block_waves = a.many ? 16 : 4;
     // q: as many waves for a token as it has 64 vectors, fewer once that makes 8192 in all
     const int64_t vectors = (int64_t)p.q_heads * (c.dim / 8);
-    const int64_t q_waves = p.q ? std::max<int64_t>(1, std::min<int64_t>((vectors + 63) / 64, 8192 / c.rows)) : 1;
-    const int64_t blocks = cache_blocks + (p.q ? (c.rows * q_waves + block_waves - 1) / block_waves : 0);
-    if (blocks * 64 * block_waves > kMostThreads || items > INT32_MAX) return hipErrorInvalidValue;
-    const int v_pad = (int)P + 4;
-    const dim3 grid((unsigned)blocks), block((unsigned)(64 * block_waves));
-    const size_t lds = (size_t)c.dim * v_pad * (single ? 4 : 1);
-    if (single) hipLaunchKernelGGL((kv_append_kernel<T, 1>), grid, block, lds, s, p, (int)items, (int)cache_blocks, v_pad, (int)q_waves);
-    else if (many) hipLaunchKernelGGL((kv_append_kernel<T, 16>), grid, block, lds, s, p, (int)items, (int)cache_blocks, v_pad, (int)q_waves);
-    else hipLaunchKernelGGL((kv_append_kernel<T, 4>), grid, block, lds, s, p, (int)items, (int)cache_blocks, v_pad, (int)q_waves);
+    a.q_waves = p.q ? std::max<int64_t>(1, std::min<int64_t>((vectors + 63) / 64, 8192 / c.rows)) : 1;
+    a.blocks = a.cache_blocks + (p.q ? (c.rows * a.q_waves + a.block_waves - 1) / a.block_waves : 0);
+    return a;
+}
+int64_t read_blocks(const KvCache& c) { return ((int64_t)c.rows / 64 + c.batch) * c.heads * 2; }
+
+template <typename T>
+hipError_t launch_kv_append(const KvAppendParams& p, hipStream_t s) {
+    const AppendPlan a = append_plan(p);
+    const int v_pad = (1 << p.c.page_log2) + 4;
+    const dim3 grid((unsigned)a.blocks), block((unsigned)(64 * a.block_waves));
+    const size_t lds = (size_t)p.c.dim * v_pad * (a.single ? 4 : 1);
+#define TG_APPEND(WAVES) hipLaunchKernelGGL((kv_append_kernel<T, WAVES>), grid, block, lds, s, p, (int)a.items, (int)a.cache_blocks, v_pad, (int)a.q_waves)
+    if (a.single) TG_APPEND(1);
+    else if (a.many) TG_APPEND(16);
+    else TG_APPEND(4);
+#undef TG_APPEND
     return hipGetLastError();
 }
+}  // namespace
+
+int64_t kv_append_threads(const KvAppendParams& p) {
+    const AppendPlan a = append_plan(p);
+    return a.blocks * 64 * a.block_waves;
+}
+int64_t kv_read_threads(const KvReadParams& p) { return read_blocks(p.c) * 256; }
 
 hipError_t run_kv_append(const KvAppendParams& p, bool is_bf16, hipStream_t s) {
     if (p.c.rows <= 0 || p.c.batch <= 0) return hipSuccess;
@@ -335,9 +357,7 @@ hipError_t run_kv_append(const KvAppendParams& p, bool is_bf16, hipStream_t s) {
 hipError_t run_kv_read(const KvReadParams& p, int out_type, hipStream_t s) {
     const KvCache& c = p.c;
     if (c.rows <= 0 || c.batch <= 0) return hipSuccess;
-    const int64_t blocks = ((int64_t)c.rows / 64 + c.batch) * c.heads * 2;
-    if (blocks * 256 > kMostThreads) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)blocks), block(256);
+    const dim3 grid((unsigned)read_blocks(c)), block(256);
     const size_t lds = (size_t)c.dim * 64;
     if (out_type == OUT_BF16) hipLaunchKernelGGL(kv_read_kernel<__bf16>, grid, block, lds, s, p);
     else if (out_type == OUT_F16) hipLaunchKernelGGL(kv_read_kernel<_Float16>, grid, block, lds, s, p);

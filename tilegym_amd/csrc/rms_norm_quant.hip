@@ -127,23 +127,30 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) rms_norm_quant_kernel(c
 // 777 x 5120 9.7 / 13.5, 4096 x 8192 49.3 / 85.0, 1000 x 16384 with two on 1024 24.8 / 39.8).  Rows of 4097 to 8192 elements leave lanes of 1024 idle:
 // with enough rows to fill the chip two vectors on 512 are ahead (777 x 5120 9.0 / 9.7 us, 2000 x 8192 24.2 / 25.7; one row of 8192 4.1 / 3.9).
 // 8192 x 4096: 47.8 us, 4.9 TB/s (a copy: 5.2).
+int lanes_of(const NormQuantParams& p) {
+    const int vectors = p.hidden / 8;
+    if (vectors <= 512) return vectors <= 64 ? 64 : vectors <= 128 ? 128 : vectors <= 256 ? 256 : 512;
+    return vectors > 2048 || (vectors <= 1024 && p.rows >= 512) ? 512 : 1024;
+}
+int64_t blocks_of(const NormQuantParams& p, int lanes) {
+    const int rows = lanes < 256 ? 256 / lanes : 1;
+    return (p.rows + rows - 1) / rows;
+}
+
 template <typename T, typename W>
 hipError_t launch(const NormQuantParams& p, hipStream_t s) {
-    const int vectors = p.hidden / 8;
-#define TG_NORM(TPR, V)                                                                                                          \
-    if (vectors <= TPR * V) {                                                                                                    \
-        const int rows = TPR < 256 ? 256 / TPR : 1;                                                                              \
-        if ((p.rows + rows - 1) / rows * (TPR < 256 ? 256 : TPR) > kMostThreads) return hipErrorInvalidValue;                    \
-        hipLaunchKernelGGL((rms_norm_quant_kernel<T, W, TPR, V>), dim3((unsigned)((p.rows + rows - 1) / rows)), dim3(TPR < 256 ? 256 : TPR), 0, s, p); \
-        return hipGetLastError();                                                                                                \
+    const int vectors = p.hidden / 8, lanes = lanes_of(p);
+    const dim3 grid((unsigned)blocks_of(p, lanes)), block(lanes < 256 ? 256 : lanes);
+#define TG_NORM(TPR, V)                                                                            \
+    if (lanes == TPR && vectors <= TPR * V) {                                                      \
+        hipLaunchKernelGGL((rms_norm_quant_kernel<T, W, TPR, V>), grid, block, 0, s, p);           \
+        return hipGetLastError();                                                                  \
     }
     TG_NORM(64, 1)
     TG_NORM(128, 1)
     TG_NORM(256, 1)
     TG_NORM(512, 1)
-    if (p.rows >= 512) {
-        TG_NORM(512, 2)
-    }
+    TG_NORM(512, 2)
     TG_NORM(1024, 1)
     TG_NORM(1024, 2)
     TG_NORM(512, 8)
@@ -152,6 +159,11 @@ hipError_t launch(const NormQuantParams& p, hipStream_t s) {
 }
 
 }  // namespace
+
+int64_t rms_norm_quant_threads(const NormQuantParams& p) {
+    const int lanes = lanes_of(p);
+    return blocks_of(p, lanes) * (lanes < 256 ? 256 : lanes);
+}
 
 hipError_t run_rms_norm_quant(const NormQuantParams& p, int x_type, bool weight_f32, hipStream_t s) {
     if (p.rows <= 0) return hipSuccess;

@@ -119,6 +119,8 @@ hipError_t run_silu_mul_quant(const void* x, int x_type, uint8_t* q, float* scal
 // out (tokens, H) <- sum over the top_k axis of x (tokens, top_k, H); bf16/f16, H % 8 == 0
 // ids: null, or (tokens, top_k) expert ids; slots whose id is outside [0, E) then count as zeros
 hipError_t run_moe_sum(const void* x, void* out, int x_type, int64_t tokens, int top_k, int H, const void* ids, bool ids_are_i64, int E, hipStream_t s);
+// Threads that a launch can have.  The *_threads functions below give what the largest launch of a call has, for the refusal of larger ones.
+constexpr int64_t kMostThreads = ((int64_t)1 << 32) - 1;
 // Root-mean-square norm with the residual's addition and an e4m3 output (rms_norm_quant.hip)
 struct NormQuantParams {
     const void* x;           // (rows, hidden)
@@ -135,6 +137,7 @@ struct NormQuantParams {
     float eps;
 };
 constexpr int kNormMaxHidden = 32768;
+int64_t rms_norm_quant_threads(const NormQuantParams& p);
 hipError_t run_rms_norm_quant(const NormQuantParams& p, int x_type, bool weight_f32, hipStream_t s);
 
 // The paged e4m3 cache (kv_device.h) and the calls over it
@@ -149,7 +152,6 @@ struct KvCache {
     int pages, heads, dim, page_log2, batch, width;
     int rows;            // of the packed tensors
 };
-constexpr int64_t kMostThreads = ((int64_t)1 << 32) - 1;  // of a launch: larger ones are refused
 struct KvAppendParams {
     KvCache c;
     const void *k, *v;                 // (rows, heads, dim), element strides below, the last dimension contiguous
@@ -161,11 +163,13 @@ struct KvAppendParams {
     const float* rope;                 // (rope_rows, rotary): cos, then sin; null: no rotation
     int rope_rows, rotary, interleaved;
 };
+int64_t kv_append_threads(const KvAppendParams& p);
 hipError_t run_kv_append(const KvAppendParams& p, bool is_bf16, hipStream_t s);
 struct KvReadParams {
     KvCache c;
     void *k, *v;                       // (rows, heads, dim), contiguous
 };
+int64_t kv_read_threads(const KvReadParams& p);
 hipError_t run_kv_read(const KvReadParams& p, int out_type, hipStream_t s);
 struct KvAttentionParams {
     KvCache c;
@@ -186,6 +190,7 @@ int kv_attention_splits(const KvAttentionParams& p);
 inline int64_t kv_attention_part_bytes(int64_t splits, int64_t rows, int64_t q_heads, int64_t dim) {
     return splits > 1 ? splits * rows * q_heads * (dim + 2) * 4 : 0;
 }
+int64_t kv_attention_threads(const KvAttentionParams& p);
 hipError_t run_kv_attention(const KvAttentionParams& p, bool is_bf16, hipStream_t s);
 // dst (cols, rows) <- transpose of src (rows, cols), one byte per element
 // dst (cols x ld) = transpose of src (rows x cols), zero beyond `rows` in every dst row

@@ -1966,6 +1966,12 @@ int32_t tg_fp8_weight_dequant(const tg_tensor* y, const tg_tensor* x, const tg_t
     return TG_OK;
 }
 
+// A launch that the device cannot have is refused before anything is asked of the device.
+static int32_t check_threads(int64_t threads, const char* what) {
+    if (threads <= tg::kMostThreads) return TG_OK;
+    return fail(TG_ERR_INVALID, "%s: these sizes make a launch of %lld threads, at most %lld are possible", what, (long long)threads, (long long)tg::kMostThreads);
+}
+
 int32_t tg_fp8_rms_norm_quant(const tg_tensor* q, const tg_tensor* scales, const tg_tensor* norm_out, const tg_tensor* residual_out,
                               const tg_tensor* x, const tg_tensor* weight, const tg_tensor* residual, const tg_tensor* scale, float eps,
                               int32_t group_size, int32_t device_id, uint64_t hip_stream) {
@@ -2009,8 +2015,6 @@ int32_t tg_fp8_rms_norm_quant(const tg_tensor* q, const tg_tensor* scales, const
     if (n == 0) return TG_OK;
     if (!aligned16(x->ptr) || !aligned16(weight->ptr) || (q->ptr & 7) != 0) return fail(TG_ERR_INVALID, "x and weight must be 16-byte and q 8-byte aligned");
     if (n / H > INT32_MAX) return fail(TG_ERR_INVALID, "too many rows");
-    DeviceGuard guard(device_id);
-    if (!guard.ok) return fail(TG_ERR_DEVICE, "cannot use HIP device %d", device_id);
     auto at = [](const tg_tensor* t) { return t ? reinterpret_cast<void*>(t->ptr) : nullptr; };
     tg::NormQuantParams p{};
     p.x = at(x), p.weight = at(weight), p.residual = at(residual), p.residual_out = at(residual_out), p.norm_out = at(norm_out);
@@ -2018,6 +2022,9 @@ int32_t tg_fp8_rms_norm_quant(const tg_tensor* q, const tg_tensor* scales, const
     p.rows = n / H, p.hidden = (int)H, p.eps = eps;
     p.lanes_per_group = scale ? 16 : group_size / 8;
     for (p.group_shift = 0; (1 << p.group_shift) < p.lanes_per_group;) ++p.group_shift;
+    if ((rc = check_threads(tg::rms_norm_quant_threads(p), "rms_norm_quant"))) return rc;
+    DeviceGuard guard(device_id);
+    if (!guard.ok) return fail(TG_ERR_DEVICE, "cannot use HIP device %d", device_id);
     const hipError_t e = tg::run_rms_norm_quant(p, x_type, weight->dtype == TG_F32, reinterpret_cast<hipStream_t>(hip_stream));
     if (e != hipSuccess) return fail(TG_ERR_LAUNCH, "rms_norm_quant launch failed: %s", hipGetErrorString(e));
     return TG_OK;
@@ -2120,6 +2127,7 @@ int32_t tg_fp8_kv_append(const tg_tensor* k_cache, const tg_tensor* v_cache, con
     if (T == 0 || p.c.batch == 0) return TG_OK;
     p.k = reinterpret_cast<const void*>(k->ptr), p.v = reinterpret_cast<const void*>(v->ptr);
     p.k_row = k->strides[0], p.k_head = k->strides[1], p.v_row = v->strides[0], p.v_head = v->strides[1];
+    if ((rc = check_threads(tg::kv_append_threads(p), "kv_cache_append"))) return rc;
     DeviceGuard guard(device_id);
     if (!guard.ok) return fail(TG_ERR_DEVICE, "cannot use HIP device %d", device_id);
     const hipError_t e = tg::run_kv_append(p, k->dtype == TG_BF16, reinterpret_cast<hipStream_t>(hip_stream));
@@ -2144,6 +2152,7 @@ int32_t tg_fp8_kv_read(const tg_tensor* k, const tg_tensor* v, const tg_tensor* 
     }
     if (p.c.rows == 0 || p.c.batch == 0) return TG_OK;
     p.k = reinterpret_cast<void*>(k->ptr), p.v = reinterpret_cast<void*>(v->ptr);
+    if ((rc = check_threads(tg::kv_read_threads(p), "kv_cache_read"))) return rc;
     DeviceGuard guard(device_id);
     if (!guard.ok) return fail(TG_ERR_DEVICE, "cannot use HIP device %d", device_id);
     const hipError_t e = tg::run_kv_read(p, out_type, reinterpret_cast<hipStream_t>(hip_stream));
@@ -2210,6 +2219,7 @@ int32_t tg_fp8_kv_attention(const tg_tensor* out, const tg_tensor* q, const tg_t
     if (out->ptr == q->ptr) return fail(TG_ERR_INVALID, "out must not be q");
     tg::KvAttentionParams p = attention_sizes(T, QH, c.batch, c.heads, c.dim, (int64_t)1 << c.page_log2, c.width, window, sink_tokens);
     p.c = c;
+    if ((rc = check_threads(tg::kv_attention_threads(p), "kv_cache_attention"))) return rc;
     const int64_t need = tg::kv_attention_part_bytes(p.splits, T, QH, c.dim);
     if (need > 0) {
         if ((rc = check_tensor(workspace, "workspace", -1))) return rc;
