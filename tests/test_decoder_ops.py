@@ -1027,3 +1027,73 @@ def test_append_a_wave_per_page_over_a_border(device, page, dim, heads, dtype):
     assert sum(news) <= 4 * batch and (lens[2] + chunk - 1) // page > lens[2] // page
     pool.fill([a + b for a, b in zip(lens, news)], news, dtype, rope)
     pool.check(True)
+
+
+# ---------------------------------------------------------------------------- torch's dispatcher
+def test_operators_infer_shapes_through_torchs_dispatcher():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from tilegym_amd import torch_ops
+    names = ("fp8_rms_norm_quant", "fp8_kv_append", "fp8_kv_append_turn", "fp8_kv_read", "fp8_kv_attention")
+    assert {f"tilegym_hip::{n}" for n in names} <= set(torch_ops.registered_ops())
+    t = torch.ops.tilegym_hip
+    for op in (t.fp8_kv_append, t.fp8_kv_append_turn):  # the cache's four tensors are written, nothing else is
+        assert [a.name for a in op.default._schema.arguments if a.alias_info is not None and a.alias_info.is_write] == ["k_cache", "v_cache", "k_scale", "v_scale"]
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        e = lambda *s, dtype=BF16: torch.empty(*s, dtype=dtype, device="cuda")  # noqa: E731
+        got = t.fp8_rms_norm_quant(e(4, 3, 256), e(256), 1e-6, e(4, 3, 256), 64, None, True)
+        assert [(tuple(x.shape), x.dtype) for x in got] == [((4, 3, 256), FP8), ((4, 3, 4), F32), ((4, 3, 256), BF16), ((4, 3, 256), BF16)]
+        assert len(t.fp8_rms_norm_quant(e(4, 256), e(256), 1e-6, None, 0, e(1, dtype=F32), False)) == 1
+        with pytest.raises(ValueError):
+            t.fp8_rms_norm_quant(e(4, 240), e(240), 1e-6, None, 128, None, False)
+        i32 = lambda *s: e(*s, dtype=torch.int32)  # noqa: E731
+        cache = (e(9, 2, 64, 128, dtype=FP8), e(9, 2, 128, 64, dtype=FP8), e(9, 2, dtype=F32), e(9, 2, dtype=F32))
+        batch, rope = (i32(3, 4), i32(3), i32(4)), e(256, 64, dtype=F32)
+        assert t.fp8_kv_append(*cache, e(5, 2, 128), e(5, 2, 128), *batch, rope, False) is None
+        q = t.fp8_kv_append_turn(*cache, e(5, 2, 128), e(5, 2, 128), *batch, e(5, 12, 128)[:, :8], rope, True)
+        assert q.shape == (5, 8, 128) and q.is_contiguous()
+        k, v = t.fp8_kv_read(*cache, batch[0], batch[2], 77, F32)
+        assert k.shape == v.shape == (77, 2, 128) and k.dtype == F32
+        out = t.fp8_kv_attention(e(5, 12, 128)[:, :8], *cache, *batch, None, 0, 0)
+        assert out.shape == (5, 8, 128) and out.is_contiguous() and out.dtype == BF16
+        with pytest.raises(ValueError):
+            t.fp8_kv_attention(e(5, 8, 64), *cache, *batch, None, 0, 0)
+    x = torch.zeros(2, 128)
+    with pytest.raises(NotImplementedError):
+        t.fp8_rms_norm_quant(x, x[0], 1e-6, None, 128, None, False)
+
+
+@pytest.mark.gpu
+def test_operators_through_torchs_dispatcher(device):
+    """The bits of the direct calls, one by one and in a graph traced whole, caches written in place."""
+    lens, news = [100, 40], [3, 2]
+    pool = Pool(device, 8, 2, 64, 128, 2, 2)
+    pool.fill(lens, lens)
+    x, r = (torch.randn(5, 1024, generator=pool.g).to(BF16).to(device) for _ in range(2))
+    w, rope, scale = torch.ones(1024, dtype=BF16, device=device), ops.rope_table(128, 64, device=device), torch.tensor([0.02], device=device)
+    batch = (pool.i32(pool.table), pool.i32(lens), pool.i32([0, 3, 5]))
+    bits = lambda ts: [t.view(torch.uint8).clone() for t in ts]  # noqa: E731
+
+    def direct(cache):
+        norm = ops.rms_norm_quant(x, w, 1e-5, residual=r, return_norm=True)
+        q, k, v = norm[3].view(5, 8, 128).split([4, 2, 2], 1)
+        turned = ops.kv_cache_append(cache, k, v, *batch, q=q, rope=rope)
+        ops.kv_cache_append(cache, k, v, *batch)
+        out = ops.kv_cache_attention(turned, cache, *batch, window=50, sink_tokens=2)
+        return [*norm, *ops.rms_norm_quant(x, w, 1e-5, scale=scale)[:1], turned, out, *ops.kv_cache_read(cache, batch[0], batch[2], 5, F32)]
+
+    def through(c0, c1, c2, c3, x, w, r, scale, table, lens, indptr, rope):
+        t, c, b = torch.ops.tilegym_hip, (c0, c1, c2, c3), (table, lens, indptr)
+        norm = t.fp8_rms_norm_quant(x, w, 1e-5, r, 128, None, True)
+        q, k, v = norm[3].view(5, 8, 128).split([4, 2, 2], 1)
+        turned = t.fp8_kv_append_turn(*c, k, v, *b, q, rope, False)
+        t.fp8_kv_append(*c, k, v, *b, None, False)
+        out = t.fp8_kv_attention(turned, *c, *b, None, 50, 2)
+        return [*norm, *t.fp8_rms_norm_quant(x, w, 1e-5, None, 0, scale, False), turned, out, *t.fp8_kv_read(c[0], c[1], c[2], c[3], b[0], b[2], 5, F32)]
+
+    cache = ops.KVCache(*(t.clone() for t in pool.cache))
+    want = bits(direct(cache)) + bits(cache)
+    for call in (through, torch.compile(through, backend="aot_eager", fullgraph=True)):
+        cache = ops.KVCache(*(t.clone() for t in pool.cache))
+        got = bits(call(*cache, x, w, r, scale, *batch, rope)) + bits(cache)
+        assert len(got) == len(want) and all(torch.equal(a, b) for a, b in zip(got, want))

@@ -7,7 +7,7 @@ Import paths mirror the reference package (src/tilegym/__init__.py:34-49):
 ``tilegym_amd.suites.flashinfer.ops.{ragged_block_scaled_bmm,gemm_alpha_beta}``,
 ``tilegym_amd.ops.{rms_norm_quant,kv_cache_append,kv_cache_read,kv_cache_attention}`` (between FP8 projections),
 ``tilegym_amd.set_backend`` / ``is_backend_available``.  ``install_as_tilegym()`` makes the same
-modules importable under the name ``tilegym``.  Importing the package also registers the GEMM entry points with
+modules importable under the name ``tilegym``.  Importing the package also registers the entry points with
 torch's dispatcher as ``torch.ops.tilegym_hip.*`` (``tilegym_amd.torch_ops``).
 """
 
