@@ -371,7 +371,8 @@ int32_t tg_fp8_rms_norm_quant(const tg_tensor* q, const tg_tensor* scales, const
  *   last `window` of them and the positions below sink_tokens.  Pages no token sees need not exist.  q (tokens, H, D) bf16 / f16, H a
  *   multiple of heads: query head h reads cache head h / (H / heads).  out: like q, contiguous, not q.  A token that sees nothing
  *   gets zeros; one whose scores are no numbers (NaN or infinities in q, an fp32 overflow) gets no numbers; one behind
- *   the table's end sees the positions that the table has.  workspace: tg_fp8_kv_attention_workspace_bytes() bytes (0: NULL will do), 16-byte aligned, contents irrelevant; calls
+ *   the table's end sees the positions that the table has.  Scores, softmax statistics and sums are fp32; the weights (times v's page scale) are
+ *   rounded to q's 16-bit type for the product with v's codes.  workspace: tg_fp8_kv_attention_workspace_bytes() bytes (0: NULL will do), 16-byte aligned, contents irrelevant; calls
  *   that share one must not overlap in time.  The codes of live slots must be numbers (tg_fp8_kv_append writes no NaN).
  */
 int32_t tg_fp8_kv_append(const tg_tensor* k_cache, const tg_tensor* v_cache, const tg_tensor* k_scale, const tg_tensor* v_scale, const tg_tensor* k,

@@ -12,7 +12,7 @@
 // the cache's transposed v has them in 16 consecutive bytes.  They lie in one page (P is a multiple of 16), so scales are
 // one value per lane.
 // Codes become the 16-bit type of q exactly (e4m3 has 4 significant bits).  k's scale joins the softmax's factor.  v's scale joins the softmax's
-// exponent: m is the maximum of a row's c q.k + log2 v_scale, and P, rounded to 16 bits, is exp2 of that less m (off by 2^-9 relative in bf16, 2^-12 in f16, of its own value,
+// exponent: m is the maximum of a row's c q.k + log2 v_scale, and P, rounded to 16 bits, is exp2 of that less m (off by 2^-8 relative in bf16, 2^-11 in f16, of its own value,
 // in f16 by no more than 2^-32 of the row's largest where that is more).  S, m, l and O are fp32.
 //
 // What is not seen is taken out by selection, never by arithmetic: scores before the maximum, and v's codes, since 0 x NaN is NaN

@@ -128,7 +128,9 @@ def kv_cache_attention(
     A token sees the positions up to its own; with ``window`` > 0 only the last ``window`` of them (its own included) and the
     first ``sink_tokens`` of the sequence.  Pages that no token sees need not exist (their table entries may be -1).  A
     token that sees nothing gets zeros; one whose scores are no numbers (NaN or infinities in q) gets no numbers; one behind the table's
-    end sees the positions that the table has.  Results do not depend on what unwritten slots hold, and a call gives the same bits every time.
+    end sees the positions that the table has.  Scores, the softmax's maximum and sum and the results are held in fp32; the softmax's weights times
+    their values' page scales are rounded to q's 16-bit type in front of the product with v's codes, by up to 2^-8 of their own size in bf16, 2^-11 in f16
+    (there by up to 2^-32 of the row's largest where that is more), and the result once more.  Results do not depend on what unwritten slots hold, and a call gives the same bits every time.
 
     Returns (tokens, heads, D) of q's type; ``out`` (contiguous, not q) is written if given.  Rows of no sequence are left as they were
     in ``out``, and unset without it."""
