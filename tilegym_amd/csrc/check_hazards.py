@@ -48,7 +48,7 @@ VGPR_SPILL_LIMITS = {"fp8_gemm_tile256_kernel": 0, "fp8_gemm_tile_ring_kernel": 
                      "fp8_gemm_pair_kernel": 0, "fp8_gemm_bs320_kernel": 0,
                      "fp8_gemm_bs256_kernelILi0ELb0E": 52, "fp8_gemm_bs256_kernelILi0ELb1E": 0,
                      "fp8_gemm_bs256_kernelILi1ELb0E": 17, "fp8_gemm_bs256_kernelILi1ELb1E": 0,
-                     "kv_attention_rows_kernelIDF16bLi128E": 0, "kv_attention_rows_kernelIDF16bLi64E": 0}
+                     "kv_attention_rows_kernel": 0, "kv_attention_kernel": 0}
 # Kernels that are launched with as much dynamic LDS as a compute unit has: no static LDS beside it (the dynamic array is
 # 1024-byte aligned, so one static variable would take 1 KiB).
 NO_STATIC_LDS = ("moe_decode_kernel", "moe_decode_sum_kernel")

@@ -188,6 +188,8 @@ __device__ __forceinline__ void select_seen(S& s, int key, int position, int win
 // pages without weight have.  In f16 weights stand 128 times as high: one that f16's smallest step swallows is below 2^-32 of the row's largest
 // product and not 2^-25, which tens of thousands of faint keys beside one strong one would add up to more than a rounding of the result.  Times a
 // code it is at most 2^-23 of the largest product; e4m3 itself rounds that key's value by up to 2^-10 of it, or more.
+// With q in bf16 P is bf16, which has no such end: where the heaviest keys' values are zero in an element, the faint keys' are still held to 2^-8.  f16 weights there
+// lose those, though they are nearer to 64 bits elsewhere (4096 tokens over 1500 to 4500 keys: relative error 0.0016 and 0.0022; 182 and 174 us).
 template <typename T>
 struct ValueScale {
     static constexpr int kUp = std::is_same_v<T, __bf16> ? 0 : 7;
@@ -254,7 +256,8 @@ __device__ __forceinline__ float score_factor(float k_scale, float scale_log2) {
 // turn and join at the end.  Codes come straight from memory into registers, k's of the next step being asked for when this step's are used
 // up, v's likewise.  Bound by HBM once some 150 compute units have work (64 sequences of 100 to 8000 keys x 8 heads: 5.5 TB/s), by latency below
 // that.  Eight waves and one workgroup to a compute unit against four and two: those 64 sequences, long ones first, 98 and 110 us; 64 of 4000 keys each
-// 101 and 98, 8 of them 19.5 and 19.2, one of 777 11.4 and 10.3.
+// 101 and 98, 8 of them 19.5 and 19.2, one of 777 11.4 and 10.3.  The forms of 16 rows keep 43 to 77 of their scalars in lanes of vector registers (the compiler's
+// scalar spills); no vector register spills.
 template <int D>
 constexpr int kFewWaves = D == 256 ? 4 : 8;
 // ONE: pages hold whole steps (64 or 128 tokens), so a step's page, its scales and its address are scalars.
@@ -765,7 +768,7 @@ int64_t keys_at_most(const KvAttentionParams& p) {
 //   more of them only up to a quarter of the compute units (1 of 64 rows 13.8 / 16.9 / 20.6; 8 of 80 rows and 8000 keys 96 / 54 / 64);
 //   32 while the compute units hold all tiles (2 of 512 rows 45 / 27 / 39), or twice as many if the keys are read twice at most and not so few that the
 //   workgroups' beginnings and ends count (32 of 48 rows: 3000 keys 67 / 53 / 65, 500 keys 29 / 26 / 18; 16 of 96 rows 67 / 51 / 46);
-//   of 256 elements there is no form of 32 rows, and 128 of them spill: 16 up to 32 rows each (64 of 20 rows 185 / - / 254) and
+//   of 256 elements there is no form of 32 rows, and 128 of them take all registers, one wave per SIMD: 16 up to 32 rows each (64 of 20 rows 185 / - / 254) and
 //   up to twice the compute units (16 of 48 rows 80 / - / 105, of 96 rows 120 / - / 85).
 int kv_attention_tile_rows(const KvAttentionParams& p) {
     const int64_t each = rows_each(p), by16 = tiles_in_all(p, 16), by32 = tiles_in_all(p, 32);
