@@ -337,7 +337,7 @@ int32_t tg_fp8_fused_moe(const tg_tensor* out, const tg_tensor* hidden, const tg
  * Root-mean-square norm with the residual's addition and an e4m3 output:
  *   s = x + residual (fp32);  y = s / sqrt(mean(s^2) + eps) * weight;  q = e4m3(clamp(y / scale, -448, 448))
  * with scale = amax(|y|) / 448 per group of group_size (16 / 32 / 64 / 128) consecutive elements (all-zero group -> 1), written to
- * scales, or one given scale for the whole tensor.  q is rounded once, from the fp32 norm.
+ * scales, or one given scale for the whole tensor.  q is rounded once, from the IEEE quotient of the fp32 norm.
  *   x (..., H) bf16 / f16 / f32, H % 16 == 0 and H % group_size == 0, H <= 32768; weight (H) of x's type or f32; q (..., H) e4m3fn
  *   scales (..., H / group_size) f32 and scale NULL, or scale one f32 and scales NULL (group_size is then ignored)
  *   residual, residual_out (s rounded to x's type), norm_out (y rounded to x's type): shape and type of x, or NULL.  residual_out may

@@ -1097,3 +1097,36 @@ def test_operators_through_torchs_dispatcher(device):
         cache = ops.KVCache(*(t.clone() for t in pool.cache))
         got = bits(call(*cache, x, w, r, scale, *batch, rope)) + bits(cache)
         assert len(got) == len(want) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hidden", [512, 4096, 8192, 16384])
+def test_norm_codes_are_those_of_the_quantizer(device, hidden):
+    """With fp32 rows, which come out unrounded: scales and codes are the bits of act_quant on them, every division included."""
+    from tilegym_amd.suites.unsloth.ops import act_quant
+    g = torch.Generator(device=device).manual_seed(hidden)
+    x = torch.randn((1 << 25) // hidden, hidden, generator=g, device=device)
+    w = 1 + 0.2 * torch.randn(hidden, generator=g, device=device)
+    for group in (16, 128):
+        q, scales, norm = ops.rms_norm_quant(x, w, 1e-5, group_size=group, return_norm=True)
+        want, want_scales = act_quant(norm, group)
+        assert torch.equal(scales, want_scales) and torch.equal(q.view(torch.uint8), want.view(torch.uint8))
+    # a given scale: the IEEE quotient, cut and rounded
+    for s in (0.03, 0.0123):
+        scale = torch.tensor([s], device=device)
+        q, _, norm = ops.rms_norm_quant(x, w, 1e-5, scale=scale, return_norm=True)
+        assert torch.equal(q.view(torch.uint8), (norm / scale).clamp(-448, 448).to(FP8).view(torch.uint8))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("given", [1e-30, 1e-17, 0.02, 3e18, 1e30])
+def test_norm_with_a_given_scale_saturates(device, given):
+    """Infinite and very large elements against small, ordinary and large scales: +-448 by their sign, NaN -448, zeros zero."""
+    x = torch.tensor([1.0, -1.0, 0.0, -0.0] * 128).repeat(4, 1)
+    w = torch.tensor([math.inf, 3e38, 1e30, 1.0, 1e-30, 0.0, math.nan, -math.inf]).repeat_interleave(64)
+    scale = torch.tensor([given], device=device)
+    q, _, norm = ops.rms_norm_quant(x.to(device), w.to(device), 0.0, scale=scale, return_norm=True)
+    y = norm.cpu()
+    want = (y / given).clamp(-448, 448)
+    want = torch.where(torch.isnan(want), torch.full_like(want, -448.0), want).to(FP8)
+    assert torch.equal(q.cpu().float(), want.float())

@@ -5,7 +5,8 @@
 //   scale = amax(|y|) / 448 over groups of 16, 32, 64 or 128 consecutive elements (all-zero group -> 1), the rule of act_quant,
 //           or one given scale for the whole tensor
 // The norm is taken of the fp32 sum and y goes to e4m3 without a 16-bit rounding between: one rounding in place of three
-// launches' three.
+// launches' three.  Both divisions are IEEE quotients, so codes and scales are the bits of act_quant on the fp32 norm (with a product by the reciprocal in
+// their place one code in a million is another: 777 x 5120 8.15 us, 8.4 with quotients; 8192 x 4096 43.1 and 43.3).
 //
 // Bound by HBM (at most 3 x 16 bits + 1 byte per element), few rows by latency: a row is read once and stays in the registers of the lanes that
 // share it, V vectors of 8 elements each; the two reductions are the sum of squares over the row and the maximum over the 2 to
@@ -26,6 +27,13 @@ template <>
 __device__ __forceinline__ void store8<float>(float* p, v8f_q v) {
     reinterpret_cast<v4f*>(p)[0] = __builtin_shufflevector(v, v, 0, 1, 2, 3);
     reinterpret_cast<v4f*>(p)[1] = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+}
+
+// ScaleDivider's quotient, with residuals s t - a that are subtracted: a zero keeps its sign by itself.
+__device__ __forceinline__ float quotient(float a, const ScaleDivider& d) {
+    float t = a * d.r;
+    t = __builtin_fmaf(-__builtin_fmaf(d.s, t, -a), d.r, t);
+    return __builtin_fmaf(-__builtin_fmaf(d.s, t, -a), d.r, t);
 }
 
 // TPR lanes share a row (64 or 128: four or two rows per workgroup; else the workgroup has one), V vectors of 8 elements per lane.
@@ -99,15 +107,21 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) rms_norm_quant_kernel(c
                 s = amax == 0.f ? 1.0f : amax / 448.0f;
                 if ((at & (p.lanes_per_group - 1)) == 0) p.scales[row * (vectors >> p.group_shift) + (at >> p.group_shift)] = s;
             }
-            // y carries the norm's own 2^-22; a reciprocal's half unit in the last place moves a code only where y / s lies that near a border
-            float inverse = 1.0f / s;
-            if (s < 0x1p-100f) {  // (the reciprocal of a subnormal scale may be infinite, and zero times that no number)
-                y *= 0x1p60f;
-                inverse = 1.0f / (s * 0x1p60f);
-            }
             v8f_q c;
+            const ScaleDivider div(s);
+            if (div.fast) {
+                if (p.scale) {  // infinite and very large y are cut where the code saturates anyway, before their residuals are no numbers
 #pragma unroll
-            for (int k = 0; k < 8; ++k) c[k] = __builtin_amdgcn_fmed3f(y[k] * inverse, -448.0f, 448.0f);
+                    for (int k = 0; k < 8; ++k) y[k] = __builtin_amdgcn_fmed3f(y[k], -512.0f * s, 512.0f * s);
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) c[k] = quotient(y[k], div);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) c[k] = y[k] / s;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) c[k] = __builtin_amdgcn_fmed3f(c[k], -448.0f, 448.0f);
             int packed[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -126,7 +140,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) rms_norm_quant_kernel(c
 // a compute unit (kernel and launch, bf16 with residual, one vector per lane against up to four on 256 lanes: 1 x 4096 3.5 / 4.3 us,
 // 777 x 5120 9.7 / 13.5, 4096 x 8192 49.3 / 85.0, 1000 x 16384 with two on 1024 24.8 / 39.8).  Rows of 4097 to 8192 elements leave lanes of 1024 idle:
 // with enough rows to fill the chip two vectors on 512 are ahead (777 x 5120 9.0 / 9.7 us, 2000 x 8192 24.2 / 25.7; one row of 8192 4.1 / 3.9).
-// 8192 x 4096 with one given scale, call after call: 42.8 us, 5.5 TB/s, as part of the 235 MB stays in the caches (a copy: 5.2 TB/s, 45 us).
+// 8192 x 4096 with one given scale, call after call: 43.3 us, 5.4 TB/s, as part of the 235 MB stays in the caches (a copy: 5.2 TB/s, 45 us).
 int lanes_of(const NormQuantParams& p) {
     const int vectors = p.hidden / 8;
     if (vectors <= 512) return vectors <= 64 ? 64 : vectors <= 128 ? 128 : vectors <= 256 ? 256 : 512;

@@ -61,7 +61,8 @@ def rms_norm_quant(
     """Root-mean-square norm with the residual's addition and an e4m3 output, in front of an FP8 projection, in one launch
     (in the reference: ``rms_norm``, src/tilegym/ops/ops.py, and a quantizer behind it).
 
-    s = x + residual;  y = s / sqrt(mean(s^2) + eps) * weight;  q = e4m3(y / scale), clamped to +-448, rounded once from fp32.
+    s = x + residual;  y = s / sqrt(mean(s^2) + eps) * weight;  q = e4m3(y / scale), clamped to +-448, rounded once from the IEEE quotient of
+    fp32 y: scales and codes are those of ``act_quant`` on it.
     x (..., H) bf16 / f16 / f32, contiguous, H % 16 == 0, H <= 32768; weight (H), x's type or fp32; residual like x.
     ``scale`` None: 1 x group_size scales amax / 448 as ``act_quant``'s (all-zero group -> 1), H % group_size == 0, group_size 16 /
     32 / 64 / 128: what ``w8a8_block_fp8_matmul`` takes.  Else one fp32 element on the device, for ``matmul(scale_a=scale)``.
