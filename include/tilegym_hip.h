@@ -362,7 +362,8 @@ int32_t tg_fp8_rms_norm_quant(const tg_tensor* q, const tg_tensor* scales, const
  *
  * tg_fp8_kv_append: writes k and v (bf16 / f16) of the new tokens.  With rope (rows, R) f32, rows >= W * P, R a multiple of 16 up to
  *   D, a row being cos of R / 2 angles, then sin: k's first R elements are turned by the row of the token's position, in pairs
- *   (i, i + R / 2), or (2 i, 2 i + 1) if interleaved; and so are q's (tokens, any heads, D), into q_out (contiguous, not q), if given.
+ *   (i, i + R / 2), or (2 i, 2 i + 1) if interleaved; and so are q's (tokens, any heads, D), into q_out (contiguous, not q), if given
+ *   (positions below zero and beyond rope: by its first and last row).
  *   A page's scale is 2^e, e the smallest in [-40, 40] with amax <= 448 * 2^e; larger magnitudes (and infinities) saturate, NaN becomes
  *   -448.  A write from a page's first slot on sets the scale anew; one behind earlier tokens keeps the larger of the page's and its own
  *   and moves the earlier tokens' codes to it.  A page belongs to one sequence while it is written.

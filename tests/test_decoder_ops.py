@@ -1130,3 +1130,16 @@ def test_norm_with_a_given_scale_saturates(device, given):
     want = (y / given).clamp(-448, 448)
     want = torch.where(torch.isnan(want), torch.full_like(want, -448.0), want).to(FP8)
     assert torch.equal(q.cpu().float(), want.float())
+
+
+@pytest.mark.gpu
+def test_append_turns_q_of_positions_outside_the_table_by_its_ends(device):
+    """More new tokens than the sequence has, and a length beyond the table: finite rows, by the first and the last angles."""
+    pool = Pool(device, 4, 1, 16, 64, 2, 2)
+    rope = ops.rope_table(32, 64, base=50.0, device="cpu")
+    k = torch.randn(9, 1, 64, generator=pool.g).to(BF16).to(device)
+    q = torch.randn(9, 3, 64, generator=pool.g).to(BF16)
+    out = ops.kv_cache_append(pool.cache, k, k, pool.i32(pool.table), pool.i32([2, 34]), pool.i32([0, 5, 9]), q=q.to(device), rope=rope.to(device))
+    want = R.ref_rope(q, [0, 0, 0, 0, 1, 30, 31, 31, 31], rope, False)
+    # one rounding to bf16, and two products and a difference in fp32
+    assert bool(((out.cpu().double() - want).abs() <= 2.0 ** -8 * (1 + 2.0 ** -10) * want.abs() + 2.0 ** -21 * want.abs().amax()).all())

@@ -87,7 +87,8 @@ def kv_cache_append(
     earlier codes to it, which is exact except where they become subnormal.
 
     Pages are written by one sequence at a time: no page twice in what a call writes.  Positions beyond the table's width and pages outside
-    the pool (such as -1) are not written.  Rows of no sequence: their q is left unwritten."""
+    the pool (such as -1) are not written; q of positions below zero or beyond ``rope`` is turned by its first or last row.  Rows of no sequence:
+    their q is left unwritten."""
     raise NotImplementedError(f"kv_cache_append is not implemented for this backend: {get_current_backend()}")
 
 
