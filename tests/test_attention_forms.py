@@ -254,3 +254,71 @@ def test_a_result_of_more_than_2_to_the_34_elements(device):
     assert torch.equal(got[:150], want)
     for at in (1 << 15, (1 << 19) - 3, 1 << 19, tokens - 5):
         assert torch.equal(got[at:at + 5], want[20:21].expand(5, heads, dim))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form,dim", CASES)
+@pytest.mark.parametrize("page", [16, 128])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_scales_that_are_no_powers_of_two(device, form, dim, page, dtype):
+    """A cache that something else than kv_cache_append has filled: any scales, some of them zero."""
+    pool, group, lens, news, width = _pool_of(device, form, dim, page, dtype)
+    assert form_of(sum(news), pool.heads * group, len(lens), pool.heads, dim, page, width)[0] == form[0]
+    for t in (pool.cache.k_scale, pool.cache.v_scale):
+        t.mul_((torch.rand(t.shape, generator=pool.g) * 3 + 0.3).to(device))
+    pool.cache.v_scale[pool.table[0][1]] = 0
+    q = pool.queries(sum(news), pool.heads * group, dtype)
+    indptr = [0] + list(itertools.accumulate(news))
+    got = ops.kv_cache_attention(q, pool.cache, pool.i32(pool.table), pool.i32(lens), pool.i32(indptr))
+    scales = [s.clamp(min=2.0 ** -64) for s in pool.scales(lens)]  # (a scale of zero counts as the least)
+    want, tol = R.ref_attention_by_head(q, pool.rows("k", lens), pool.rows("v", lens), lens, indptr, dim ** -0.5, half_step=HALF[dtype], v_scale=scales)
+    assert bool(((got.double() - want).abs() <= tol + 448 * 2.0 ** -64).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page,longest", [(32, 1000), (64, 1000), (64, 1500)])
+def test_a_prompt_among_decoding_sequences(device, dim, page, longest):
+    """The 128-row form with tiles of one token's rows: single tokens, drafted ones, nothing new and no tokens at all beside a prompt."""
+    g = torch.Generator().manual_seed(dim + page)
+    batch, heads, group = 70, 8, 4
+    lens = torch.randint(1, 200, (batch,), generator=g).tolist()
+    lens[3], lens[11], lens[20], lens[69] = longest, 0, longest - 1, 70
+    news = [1] * batch
+    news[3], news[11], news[30], news[31], news[69] = 1000, 0, 0, min(5, lens[31]), 70
+    width = -(-longest // page)
+    assert form_of(sum(news), heads * group, batch, heads, dim, page, width) == (128, 1)
+    pool = Forms(device, sum(-(-n // page) for n in lens) + 1, heads, page, dim, batch, 1)
+    pages = iter(torch.randperm(pool.cache.k.shape[0], generator=g).tolist())
+    pool.table = [[next(pages) if i * page < n else -1 for i in range(width)] for n in lens]
+    pool.fill(lens, lens)
+    q = pool.queries(sum(news), heads * group, BF16, 2.0)
+    pool.check(q, lens, news)
+    pool.check(q, lens, news, window=100, sinks=5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,heads,group,news", [(16, 2, 4, 3), (32, 2, 5, 180), (128, 8, 4, 281)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_many_faint_keys(device, rows, heads, group, news, dtype):
+    """One strong key with value zero beside twenty thousand faint ones with value one, each 2^-25.2 of it, in every form."""
+    n, dim, strong = 20000, 64, 20.0
+    width = -(-n // 64)
+    assert form_of(news, heads * group, 1, heads, dim, 64, width)[0] == rows
+    cache = ops.alloc_kv_cache(width, heads, dim, 64, device=device)
+    k, v = torch.zeros(n, heads, dim, device=device), torch.ones(n, heads, dim, device=device)
+    k[..., 0] = 2.5
+    k[0, :, 0], v[0] = strong, 0
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    table = torch.arange(width, dtype=torch.int32, device=device)[None]
+    ops.kv_cache_append(cache, k.to(dtype), v.to(dtype), table, i32(n), i32(0, n))
+    q = torch.zeros(news, heads * group, dim, dtype=dtype, device=device)
+    q[..., 0] = 1
+    out = ops.kv_cache_attention(q, cache, table, i32(n), i32(0, news), sm_scale=1.0).cpu().double()
+    weight = math.exp(2.5 - strong)
+    faint = torch.arange(n - news, n, dtype=torch.float64)[:, None, None]
+    want = faint * weight / (1 + faint * weight)
+    # a weight is rounded to 16 bits, or by half of f16's smallest step, a 128th of 2^-25 against the maximum; the scores' 20 are 2^-23 off, the
+    # exponentials and the sum of 20000 fp32 terms a few units of 2^-24 each
+    tol = want * (2 * HALF[dtype] + 20 * 2.0 ** -22 + 20000 / 16 * 2.0 ** -24) + (faint * 2.0 ** -32 if dtype == F16 else 0)
+    assert bool(((out - want).abs() <= tol).all())
