@@ -387,6 +387,55 @@ int32_t tg_fp8_kv_attention(const tg_tensor* out, const tg_tensor* q, const tg_t
                             const tg_tensor* v_scale, const tg_tensor* block_table, const tg_tensor* seq_lens, const tg_tensor* indptr, float sm_scale,
                             int32_t window, int32_t sink_tokens, const tg_tensor* workspace, int32_t device_id, uint64_t hip_stream);
 
+/*
+ * Products in 8-bit integers, a scale per token and per output channel:
+ *   C[m,n] = scale_a[m] * scale_b[n] * sum_k A[m,k] * B[n,k] + bias[n]
+ * The sums are int32 and exact (K at most 131071); the rest is fp32: float(sum) * scale_a[m], then one multiply-add with scale_b[n] and the bias,
+ * rounded once to c's type.  Every kernel and every split returns the same bits.
+ *   a (M, K), b (N, K) int8, contiguous; c (M, N) bf16 / f16 / f32, contiguous; scale_a f32, M elements or one; scale_b f32, N elements or one;
+ *   bias (N) bf16 / f16 / f32, or NULL.  Rows of a multiple of 16 bytes on 16-byte addresses take the fast kernels.
+ *   workspace: NULL, or a 16-byte aligned buffer of tg_int8_gemm_workspace_bytes() bytes, contents irrelevant: it holds the partial sums of split K
+ *   (without it K is not split).  Calls that share one must not overlap in time.
+ * cfg: TG_CFG_KERNEL (0, 1 or 3), TG_CFG_BLOCK_M, TG_CFG_BLOCK_N, TG_CFG_SPLIT_K as for tg_fp8_gemm; what does not exist is ignored.
+ *
+ * tg_int8_ragged_gemm: rows m_indptr[e] .. m_indptr[e + 1] of a with b[e] (E, N, K) and scale_b (E, N) (or one element); m_indptr (E + 1) int32 DEVICE
+ * memory, non-decreasing.  Rows that belong to no expert are not written.
+ */
+int32_t tg_int8_gemm(const tg_tensor* c, const tg_tensor* a, const tg_tensor* b, const tg_tensor* scale_a, const tg_tensor* scale_b, const tg_tensor* bias,
+                     const tg_tensor* workspace, const int32_t* cfg, int32_t ncfg, int32_t device_id, uint64_t hip_stream);
+int64_t tg_int8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int32_t tg_int8_ragged_gemm(const tg_tensor* c, const tg_tensor* a, const tg_tensor* b, const tg_tensor* scale_a, const tg_tensor* scale_b,
+                            const tg_tensor* m_indptr, const int32_t* cfg, int32_t ncfg, int32_t device_id, uint64_t hip_stream);
+
+/*
+ * Rows in int8 with a scale each: scale = max|y| * fp32(1 / 127) (0: 1), q = round-half-even(y / scale), an IEEE quotient, within +-127, y = x, or with
+ * silu_mul y = silu(x[:K]) * x[K:] in fp32.  A row that holds a NaN or an infinity gets the scale NaN and codes of zero.
+ * x (..., K) or (..., 2 K) bf16 / f16 / f32; q int8 and scales f32, a scale per row; all contiguous.
+ * place (rows, copies) int32, or NULL: row r goes to the rows place[r][j] of q (rows * copies, K) and scales; where that is below zero, zeros and a
+ * scale of 1 go to row -1 - place[r][j].  Excludes silu_mul.
+ */
+int32_t tg_int8_quant(const tg_tensor* q, const tg_tensor* scales, const tg_tensor* x, const tg_tensor* place, int32_t silu_mul, int32_t device_id,
+                      uint64_t hip_stream);
+
+/*
+ * Tokens sorted by expert and back.
+ * tg_moe_sort: the (token, slot) pairs of topk_ids (int32 / int64, any shape, n pairs) in the order of their experts, stable; pairs whose id is outside
+ *   [0, num_experts) behind the last expert.  indptr (num_experts + 1) int32: rows indptr[e] .. indptr[e + 1] are expert e's; rows (n) int32: the
+ *   row of each pair, or -1 - row for the pairs behind the last expert; slots (n) int32: the pair of each row.  num_experts at most 512.
+ * tg_moe_permute: out[rows[t][j]] = x[t]; zeros in the rows behind the last expert.  x (T, H), rows (T, k), out (T * k, H).
+ * tg_moe_unpermute: out[t] = sum_j weights[t][j] * x[rows[t][j]] over the pairs that have an expert, in fp32, in the order of j, rounded once.
+ *   weights (T, k) bf16 / f16 / f32, or NULL (ones).  Without weights it is the gradient of tg_moe_permute.
+ * tg_moe_unpermute_backward: grad_x[rows[t][j]] = weights[t][j] * grad_out[t] (zeros in the rows behind the last expert), grad_weights[t][j] = <grad_out[t],
+ *   x[rows[t][j]]> in fp32, rounded to the weights' type (zero for pairs without an expert).
+ * Rows of bf16 / f16 / f32 (one type per call), contiguous, any H.  What `rows` names outside the T * k rows is left out.
+ */
+int32_t tg_moe_sort(const tg_tensor* topk_ids, int32_t num_experts, const tg_tensor* indptr, const tg_tensor* rows, const tg_tensor* slots, int32_t device_id,
+                    uint64_t hip_stream);
+int32_t tg_moe_permute(const tg_tensor* out, const tg_tensor* x, const tg_tensor* rows, int32_t device_id, uint64_t hip_stream);
+int32_t tg_moe_unpermute(const tg_tensor* out, const tg_tensor* x, const tg_tensor* rows, const tg_tensor* weights, int32_t device_id, uint64_t hip_stream);
+int32_t tg_moe_unpermute_backward(const tg_tensor* grad_x, const tg_tensor* grad_weights, const tg_tensor* grad_out, const tg_tensor* x, const tg_tensor* rows,
+                                  const tg_tensor* weights, int32_t device_id, uint64_t hip_stream);
+
 /* The schedule the most recent GEMM call on this host thread chose: fills out[0..n) with the
  * TG_CFG_* slots (kernel, BLOCK_M, BLOCK_N, SPLIT_K, ROW_GROUPS, WAVES).  Returns slots written. */
 int32_t tg_last_config(int32_t* out, int32_t n);

@@ -1,0 +1,593 @@
+"""Products in 8-bit integers, their quantizers, and tokens sorted by expert and back: refusals and the oracle on the CPU, the kernels against
+float64 (and, where every step is defined, bit by bit) on a GPU.
+
+Tolerances count roundings: half a step of a type is eps / 2 of the value (bf16 2^-8, f16 2^-11, fp32 2^-24), and where a value is smaller than
+the type's normal numbers half of its smallest step."""
+
+import pytest
+import torch
+
+from oracle import int8_reference as R
+from tilegym_amd import _lib, ops
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+HALF = {BF16: 2.0 ** -8, F16: 2.0 ** -11, F32: 2.0 ** -24}
+TINY = {BF16: 2.0 ** -134, F16: 2.0 ** -25, F32: 2.0 ** -150}
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def codes(shape, seed):
+    return torch.randint(-128, 128, shape, generator=gen(seed), dtype=torch.int16).to(torch.int8)
+
+
+def scales(shape, seed):
+    return 0.01 * torch.exp(torch.randn(shape, generator=gen(seed)))
+
+
+def near(out, exact, size, t, roundings, what=""):
+    """`roundings` fp32 ones of `size`, and the store's of the result."""
+    tol = roundings * 2.0 ** -24 * size + HALF[t] * (exact.abs() + roundings * 2.0 ** -24 * size) + TINY[t]
+    off = (out.cpu().double() - exact).abs()
+    assert bool((off <= tol).all()), (what, float((off / tol).max()))
+
+
+def bits(t):
+    return t.contiguous().view(torch.int16 if t.element_size() == 2 else torch.int32 if t.element_size() == 4 else torch.int8).cpu()
+
+
+# ---------------------------------------------------------------------------- CPU: the oracle, refusals
+def test_oracle_of_the_order():
+    ids = torch.tensor([[1, 0], [5, 1], [-1, 1]])
+    indptr, rows, slots = R.ref_sort(ids, 2)
+    assert indptr == [0, 1, 4] and slots == [1, 0, 3, 5, 2, 4] and rows == [1, 0, -5, 2, -6, 3]
+    x = torch.arange(3.0)[:, None] + 1
+    rows = torch.tensor(rows).view(3, 2)
+    p = R.ref_permute(x, rows)
+    assert p.flatten().tolist() == [1, 1, 2, 3, 0, 0]
+    assert R.ref_unpermute(p, rows)[0].flatten().tolist() == [2, 2, 3]
+
+
+def test_operators_have_no_host_path():
+    a, b, s = torch.zeros(2, 64, dtype=torch.int8), torch.zeros(3, 64, dtype=torch.int8), torch.ones(1)
+    i32 = torch.zeros(2, 1, dtype=torch.int32)
+    order = ops.MoeOrder(torch.zeros(2, dtype=torch.int32), i32, i32.flatten())
+    x = torch.zeros(2, 8)
+    for call in (lambda: ops.int8_matmul(a, b, s, s), lambda: ops.ragged_int8_matmul(a, b[None], s, s, i32.flatten()), lambda: ops.quant_int8(x),
+                 lambda: ops.silu_mul_quant_int8(x), lambda: ops.moe_sort(i32, 1), lambda: ops.moe_permute(x, order), lambda: ops.moe_unpermute(x, order),
+                 lambda: ops.moe_permute_quant_int8(x, order), lambda: ops.moe_permute_backward(x, order),
+                 lambda: ops.moe_unpermute_backward(x, x, order, torch.ones(2, 1))):
+        with pytest.raises(RuntimeError, match="HIP device"):
+            call()
+
+
+def _matmul_rc(a=None, b=None, c=None, sa=None, sb=None, bias=None, ws=None):
+    a = torch.zeros(4, 64, dtype=torch.int8) if a is None else a
+    b = torch.zeros(8, 64, dtype=torch.int8) if b is None else b
+    c = torch.zeros(4, 8, dtype=BF16) if c is None else c
+    sa, sb = torch.ones(4) if sa is None else sa, torch.ones(8) if sb is None else sb
+    d, (cfg, n) = _lib._desc, _lib.make_cfg(None)
+    return _lib.load().tg_int8_gemm(d(c), d(a), d(b), d(sa), d(sb), d(bias), d(ws), cfg, n, 9999, 0)
+
+
+def _error():
+    return _lib.load().tg_last_error().decode()
+
+
+def test_matmul_refusals():
+    i8 = torch.int8
+    assert _matmul_rc() == -4  # everything is in order up to the device
+    assert _matmul_rc(a=torch.zeros(4, 64)) == -2
+    assert _matmul_rc(b=torch.zeros(8, 64, dtype=torch.uint8)) == -2
+    assert _matmul_rc(c=torch.zeros(4, 8, dtype=i8)) == -2
+    assert _matmul_rc(sa=torch.ones(4, dtype=BF16)) == -2
+    assert _matmul_rc(bias=torch.ones(8, dtype=torch.int32)) == -2
+    assert _matmul_rc(b=torch.zeros(8, 32, dtype=i8)) == -6
+    assert _matmul_rc(c=torch.zeros(8, 4, dtype=BF16)) == -6
+    assert _matmul_rc(sa=torch.ones(3)) == -6 and "scale_a" in _error()
+    assert _matmul_rc(sb=torch.ones(4)) == -6 and "scale_b" in _error()
+    assert _matmul_rc(bias=torch.ones(7)) == -6
+    assert _matmul_rc(a=torch.zeros(64, 4, dtype=i8).t()) == -6 and "contiguous" in _error()
+    assert _matmul_rc(a=torch.zeros(4, 0, dtype=i8), b=torch.zeros(8, 0, dtype=i8)) == -6
+    wide = torch.zeros(1, dtype=i8).expand(1, 131072).contiguous()
+    assert _matmul_rc(a=wide, b=wide, c=torch.zeros(1, 1), sa=torch.ones(1), sb=torch.ones(1)) == -6 and "131071" in _error()
+    assert _matmul_rc(a=torch.zeros(0, 64, dtype=i8), c=torch.zeros(0, 8, dtype=BF16), sa=torch.ones(0)) == 0
+    assert _matmul_rc(sa=torch.ones(1), sb=torch.ones(1)) == -4
+
+
+def test_ragged_refusals():
+    i8, i32 = torch.int8, torch.int32
+    d, (cfg, n) = _lib._desc, _lib.make_cfg(None)
+
+    def rc(a=torch.zeros(4, 64, dtype=i8), b=torch.zeros(2, 8, 64, dtype=i8), c=torch.zeros(4, 8, dtype=BF16), sa=torch.ones(4), sb=torch.ones(2, 8),
+           ptr=torch.zeros(3, dtype=i32)):
+        return _lib.load().tg_int8_ragged_gemm(d(c), d(a), d(b), d(sa), d(sb), d(ptr), cfg, n, 9999, 0)
+
+    assert rc() == -4
+    assert rc(ptr=torch.zeros(3, dtype=torch.int64)) == -2
+    assert rc(ptr=torch.zeros(4, dtype=i32)) == -6
+    assert rc(sb=torch.ones(8)) == -6
+    assert rc(b=torch.zeros(8, 64, dtype=i8)) == -6
+    assert rc(b=torch.zeros(2, 8, 32, dtype=i8)) == -6
+
+
+def test_quant_refusals():
+    d = _lib._desc
+
+    def rc(x=torch.zeros(3, 16), q=torch.zeros(3, 16, dtype=torch.int8), s=torch.zeros(3), place=None, silu=0):
+        return _lib.load().tg_int8_quant(d(q), d(s), d(x), d(place), silu, 9999, 0)
+
+    assert rc() == -4
+    assert rc(x=torch.zeros(3, 16, dtype=torch.int32)) == -2
+    assert rc(q=torch.zeros(3, 16, dtype=torch.uint8)) == -2
+    assert rc(s=torch.zeros(3, dtype=BF16)) == -2
+    assert rc(s=torch.zeros(2)) == -6
+    assert rc(silu=1) == -6
+    assert rc(x=torch.zeros(3, 31), silu=1) == -6
+    assert rc(x=torch.zeros(3, 32), silu=1) == -4
+    place = torch.zeros(3, 2, dtype=torch.int32)
+    assert rc(place=place) == -6
+    assert rc(place=place, q=torch.zeros(6, 16, dtype=torch.int8), s=torch.zeros(6)) == -4
+    assert rc(place=place, x=torch.zeros(3, 32), q=torch.zeros(6, 16, dtype=torch.int8), s=torch.zeros(6), silu=1) == -6
+    assert rc(place=place.long(), q=torch.zeros(6, 16, dtype=torch.int8), s=torch.zeros(6)) == -2
+    assert rc(x=torch.zeros(0, 16), q=torch.zeros(0, 16, dtype=torch.int8), s=torch.zeros(0)) == 0
+
+
+def test_route_refusals():
+    d, L, i32 = _lib._desc, _lib.load(), torch.int32
+    ids = torch.zeros(3, 2, dtype=i32)
+
+    def sort(ids=ids, E=4, ptr=torch.zeros(5, dtype=i32), rows=torch.zeros(3, 2, dtype=i32), slots=torch.zeros(6, dtype=i32)):
+        return L.tg_moe_sort(d(ids), E, d(ptr), d(rows), d(slots), 9999, 0)
+
+    assert sort() == -4 and sort(ids=ids.long()) == -4
+    assert sort(ids=ids.to(torch.uint8)) == -2
+    assert sort(slots=torch.zeros(6, dtype=torch.int64)) == -2
+    assert sort(E=3) == -6 and sort(E=0, ptr=torch.zeros(1, dtype=i32)) == -6 and sort(E=513, ptr=torch.zeros(514, dtype=i32)) == -6
+    assert sort(rows=torch.zeros(5, dtype=i32)) == -6
+
+    x, y, w = torch.zeros(3, 8), torch.zeros(6, 8), torch.zeros(3, 2)
+    for by_token, by_row, rows, want in ((x, y, ids, -4), (x, y.to(BF16), ids, -2), (x.int(), y.int(), ids, -2), (x, y[:5], ids, -6), (x, y, ids.long(), -2),
+                                         (x, y, ids[:2].contiguous(), -6), (x, torch.zeros(6, 7), ids, -6), (x, y, ids.flatten(), -6)):
+        assert L.tg_moe_permute(d(by_row), d(by_token), d(rows), 9999, 0) == want
+        assert L.tg_moe_unpermute(d(by_token), d(by_row), d(rows), None, 9999, 0) == want
+        assert L.tg_moe_unpermute_backward(d(by_row), d(w), d(by_token), d(by_row), d(rows), d(w), 9999, 0) == want
+    assert L.tg_moe_unpermute(d(x), d(y), d(ids), d(w[:, :1].contiguous()), 9999, 0) == -6
+    assert L.tg_moe_unpermute(d(x), d(y), d(ids), d(w.int()), 9999, 0) == -2
+    assert L.tg_moe_unpermute_backward(d(y), d(w.to(BF16)), d(x), d(y), d(ids), d(w), 9999, 0) == -2
+    assert L.tg_moe_unpermute_backward(d(y), None, d(x), d(y), d(ids), d(w), 9999, 0) == -5
+    assert L.tg_moe_unpermute_backward(d(y), d(w), d(x), None, d(ids), d(w), 9999, 0) == -5
+    assert L.tg_moe_unpermute_backward(d(y), d(w), d(x), d(y), d(ids), None, 9999, 0) == -5
+
+
+# ---------------------------------------------------------------------------- GPU: products
+def _check_matmul(dev, m, n, k, t, bias=None, per_token=True, per_channel=True, seed=0, **more):
+    a, b = codes((m, k), seed), codes((n, k), seed + 1)
+    sa, sb = scales(m if per_token else 1, seed + 2), scales(n if per_channel else 1, seed + 3)
+    bv = None if bias is None else (10 * torch.randn(n, generator=gen(seed + 4))).to(bias)
+    out = ops.int8_matmul(a.to(dev), b.to(dev), sa.to(dev), sb.to(dev), bias=None if bv is None else bv.to(dev), out_dtype=t, **more)
+    assert out.shape == (m, n) and out.dtype == t
+    exact, size = R.ref_int8_matmul(a, b, sa, sb, bv)
+    # the sum's conversion, its product with scale_a, the multiply-add
+    near(out, exact, torch.maximum(size, exact.abs()), t, 3.01, (m, n, k, more))
+    if bv is None:
+        assert torch.equal(bits(out), bits(R.ref_int8_matmul_f32(a, b, sa, sb).to(t))), (m, n, k, more)
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [BF16, F16, F32])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 64, 16), (3, 5, 7), (16, 48, 64), (17, 65, 63), (65, 100, 130), (64, 64, 1000), (130, 200, 257), (200, 70, 15)])
+def test_matmul_odd_sizes(device, m, n, k, t):
+    _check_matmul(device, m, n, k, t)
+    _check_matmul(device, m, n, k, t, bias=t, per_token=False)
+    _check_matmul(device, m, n, k, t, bias=F32, per_channel=False)
+
+
+MATMUL_SIZES = [(1, 256, 256), (8, 1000, 512), (16, 640, 1152), (24, 512, 2048), (33, 2112, 1024), (64, 512, 4096), (100, 1032, 640), (129, 384, 1280), (256, 512, 512),
+                (257, 776, 384), (300, 520, 2064), (513, 1024, 400), (777, 640, 1408)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", MATMUL_SIZES)
+def test_matmul_aligned_sizes(device, m, n, k):
+    for t in (BF16, F16, F32):
+        _check_matmul(device, m, n, k, t)
+    _check_matmul(device, m, n, k, F16, bias=F16, per_token=False)
+    _check_matmul(device, m, n, k, BF16, bias=F32, per_channel=False)
+
+
+@pytest.mark.gpu
+def test_matmul_largest_sums(device):
+    """The largest sum that 32 bits hold: 131071 products of -128 * -128."""
+    k = 131071
+    a = torch.full((2, k), -128, dtype=torch.int8, device=device)
+    out = ops.int8_matmul(a, a, torch.ones(1, device=device), torch.ones(1, device=device), out_dtype=F32)
+    assert out.tolist() == [[float(torch.tensor(k * 16384).float())] * 2] * 2
+    out = ops.int8_matmul(a[:, :131056].contiguous(), a[:, :131056].contiguous(), torch.ones(1, device=device), torch.ones(1, device=device), out_dtype=F32)
+    assert out.tolist() == [[131056.0 * 16384.0] * 2] * 2
+
+
+@pytest.mark.gpu
+def test_matmul_takes_any_rank_views_and_out(device):
+    a, b = codes((6, 64), 1).to(device), codes((10, 64), 2).to(device)
+    sa, sb = scales((2, 3), 3).to(device), scales(10, 4).to(device)
+    want = ops.int8_matmul(a, b, sa.flatten(), sb)
+    assert torch.equal(ops.int8_matmul(a.view(2, 3, 64), b, sa, sb), want.view(2, 3, 10))
+    out = torch.empty(6, 10, dtype=F32, device=device)
+    assert ops.int8_matmul(a, b, sa, sb, out_dtype=F32, out=out) is out and torch.equal(out.to(BF16), want)
+    assert ops.int8_matmul(a[0], b, sa[0, :1], sb).shape == (10,)
+    assert ops.int8_matmul(a[:0], b, sa.flatten()[:0], sb).shape == (0, 10)
+    # operands that start at odd addresses
+    odd = torch.empty(6 * 64 + 1, dtype=torch.int8, device=device)[1:].view(6, 64).copy_(a)
+    assert torch.equal(ops.int8_matmul(odd, b, sa, sb), want)
+    for bad in (dict(a=a.t()), dict(out=torch.empty(6, 10, device=device)), dict(out=torch.empty(6, 9, dtype=BF16, device=device)), dict(b=b[None])):
+        with pytest.raises(ValueError):
+            ops.int8_matmul(**{**dict(a=a, b=b, scale_a=sa, scale_b=sb), **bad})
+    with pytest.raises(ValueError, match="cpu"):
+        ops.int8_matmul(a, b, sa.cpu(), sb)
+
+
+@pytest.mark.gpu
+def test_matmul_nan_scales_show_where_they_are(device):
+    a, b = codes((40, 256), 1).to(device), codes((96, 256), 2).to(device)
+    sa, sb = scales(40, 3).to(device), scales(96, 4).to(device)
+    want = ops.int8_matmul(a, b, sa, sb)
+    sa[7], sb[33] = float("nan"), float("inf")
+    got = ops.int8_matmul(a, b, sa, sb)
+    assert bool(got[7].isnan().all()) and not bool(got[:, 33].isfinite().any())
+    keep = [i for i in range(40) if i != 7], [i for i in range(96) if i != 33]
+    assert torch.equal(got[keep[0]][:, keep[1]], want[keep[0]][:, keep[1]])
+
+
+# ---------------------------------------------------------------------------- GPU: products over experts
+def _check_ragged(dev, counts, n, k, t, seed=0, tail=0, start=0, **more):
+    E = len(counts)
+    indptr = torch.tensor([start] + counts).cumsum(0).to(torch.int32)
+    m = int(indptr[-1]) + tail
+    a, b = codes((m, k), seed), codes((E, n, k), seed + 1)
+    sa, sb = scales(m, seed + 2), scales((E, n), seed + 3)
+    out = torch.full((m, n), 77.0, dtype=t, device=dev)
+    got = ops.ragged_int8_matmul(a.to(dev), b.to(dev), sa.to(dev), sb.to(dev), indptr.to(dev), out_dtype=t, out=out, **more)
+    assert got is out
+    want = R.ref_ragged(a, b, sa, sb, indptr, R.ref_int8_matmul_f32)
+    live = ~want[:, 0].isnan() if n else None
+    assert torch.equal(bits(out[live.to(dev)]), bits(want[live].to(t))), (counts, n, k, more)
+    assert bool((out[~live.to(dev)] == 77.0).all())  # rows of no expert are left as they were
+    return out
+
+
+RAGGED = [([3], 40, 64), ([0, 5, 0, 1], 72, 96), ([1] * 9, 256, 128), ([70, 0, 130, 3, 64], 200, 384), ([16, 17, 15, 0, 33], 130, 1408), ([300, 5], 512, 640),
+          ([0, 0, 0], 64, 64), ([2] * 70, 96, 256), ([0] * 300 + [7] + [0] * 10 + [500], 64, 192), ([4, 9, 2], 33, 31), ([260, 512, 31, 0, 700], 776, 896)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("counts,n,k", RAGGED)
+def test_ragged(device, counts, n, k):
+    for t in (BF16, F16, F32):
+        _check_ragged(device, counts, n, k, t)
+    _check_ragged(device, counts, n, k, BF16, tail=37, start=5)
+
+
+@pytest.mark.gpu
+def test_ragged_offsets_beyond_the_rows_are_cut(device):
+    """Whatever indptr holds, nothing outside the rows is read or written."""
+    a, b = codes((50, 128), 1).to(device), codes((3, 64, 128), 2).to(device)
+    sa, sb = scales(50, 3).to(device), scales((3, 64), 4).to(device)
+    want = ops.ragged_int8_matmul(a, b, sa, sb, torch.tensor([0, 20, 40, 50], dtype=torch.int32, device=device))
+    got = torch.zeros(50, 64, dtype=BF16, device=device)
+    ops.ragged_int8_matmul(a, b, sa, sb, torch.tensor([0, 20, 40, 5000], dtype=torch.int32, device=device), out=got)
+    assert torch.equal(got[:40], want[:40])
+    ops.ragged_int8_matmul(a, b, sa, sb, torch.tensor([-5, 20, 10, 40], dtype=torch.int32, device=device), out=got)
+
+
+# ---------------------------------------------------------------------------- GPU: quantizers
+QUANT_ROWS = [(1, 1), (3, 7), (5, 8), (2, 64), (9, 100), (4, 512), (3, 1000), (2, 2048), (5, 4096), (3, 4104), (2, 11000), (3, 16384), (1, 32768), (2, 32776), (1, 70001)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,k", QUANT_ROWS)
+@pytest.mark.parametrize("t", [BF16, F16, F32])
+def test_quant_is_its_fp32_steps(device, rows, k, t):
+    x = torch.randn(rows, k, generator=gen(rows * k)).to(t)
+    x[0, k // 2] = 0
+    q, s = ops.quant_int8(x.to(device))
+    wq, ws = R.ref_quant(x)
+    assert q.shape == x.shape and s.shape == x.shape[:-1]
+    assert torch.equal(q.cpu(), wq) and torch.equal(bits(s), bits(ws))
+
+
+@pytest.mark.gpu
+def test_quant_extremes(device):
+    x = torch.zeros(12, 24)
+    x[1] = 3.0
+    x[2, 5] = float("nan")
+    x[3, 0] = float("-inf")
+    x[4] = torch.linspace(-1, 1, 24) * 3.4e38
+    x[5] = 1e-45                                   # amax times 1 / 127 is zero
+    x[6] = torch.arange(24) * 2.0 ** -149 * 1000   # a subnormal scale
+    x[7] = torch.arange(24) * 1e-30
+    x[8] = torch.arange(24) * 1e25
+    x[9] = torch.tensor([127.0, 0.5, 1.5, 2.5, -0.5, -1.5, 126.5, -126.5] * 3)  # ties go to even
+    x[10, 3] = -5.0
+    x[11] = -x[9]
+    q, s = ops.quant_int8(x.to(device))
+    wq, ws = R.ref_quant(x)
+    assert torch.equal(q.cpu(), wq) and torch.equal(bits(s.nan_to_num(-1)), bits(ws.nan_to_num(-1))) and torch.equal(s.isnan().cpu(), ws.isnan())
+    assert q.cpu()[9].tolist() == [127, 0, 2, 2, 0, -2, 126, -126] * 3
+    assert s.cpu()[0] == 1 and s.cpu()[5] == 1 and int(q.cpu()[5].abs().max()) == 0
+    a = ops.int8_matmul(q, torch.ones(8, 24, dtype=torch.int8, device=device), s, torch.ones(1, device=device))
+    assert bool(a[2:4].isnan().all()) and bool(a[:2].isfinite().all())
+
+
+@pytest.mark.gpu
+def test_quant_any_rank_and_address(device):
+    x = torch.randn(2, 3, 40, generator=gen(1)).to(BF16).to(device)
+    q, s = ops.quant_int8(x)
+    assert q.shape == (2, 3, 40) and s.shape == (2, 3)
+    assert torch.equal(ops.quant_int8(x.view(6, 40))[0].view(2, 3, 40), q)
+    odd = torch.empty(241, dtype=BF16, device=device)[1:].view(6, 40).copy_(x.view(6, 40))
+    assert torch.equal(ops.quant_int8(odd)[0], q.view(6, 40))
+    assert ops.quant_int8(x[0, 0])[1].shape == ()
+    assert ops.quant_int8(x[:0])[0].shape == (0, 3, 40)
+    with pytest.raises(_lib.TileGymHipError, match="contiguous"):
+        ops.quant_int8(x.transpose(0, 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,i", [(1, 1), (3, 9), (4, 64), (7, 1408), (3, 4100), (2, 14336), (1, 33000)])
+@pytest.mark.parametrize("t", [BF16, F16, F32])
+def test_silu_mul_quant(device, rows, i, t):
+    x = (2 * torch.randn(rows, 2 * i, generator=gen(rows + i))).to(t)
+    q, s = ops.silu_mul_quant_int8(x.to(device))
+    gate, up = x.double()[:, :i], x.double()[:, i:]
+    y = gate / (1 + torch.exp(-gate)) * up
+    # The hardware's exponential of gate * log2(e): its argument is off by 2^-24 of itself and the result by a few units, the reciprocal by one, the products by
+    # half each: |gate| + 8 roundings of 2^-23 are more than all of these.
+    err = (gate.abs() + 8) * 2.0 ** -23 * y.abs()
+    top = y.abs().amax(1)
+    worst = (err.amax(1) + 2.0 ** -24 * top) / 127
+    # (the scale: 1 / 127 is rounded, and the product with it)
+    assert bool(((s.cpu().double() - top / 127).abs() <= worst + 2.0 ** -23 * top / 127 + 2.0 ** -150).all())
+    off = (q.cpu().double() * s.cpu().double()[:, None] - y).abs()
+    # half a step; y's own error; the quotient's and the scale's rounding over up to 127 steps; the clamp
+    tol = s.cpu().double()[:, None] * (0.5 + 127 * 2.0 ** -22) + err + worst[:, None] * 127
+    assert bool((off <= tol).all()), float((off / tol).max())
+
+
+@pytest.mark.gpu
+def test_silu_mul_quant_extremes(device):
+    x = torch.zeros(5, 16)
+    x[0, :8], x[0, 8:] = -200.0, 5.0       # the sigmoid is zero
+    x[1, :8], x[1, 8:] = 200.0, -3.0
+    x[2, 3] = float("nan")
+    x[3, :8], x[3, 8] = 1.0, float("inf")
+    x[4, :8], x[4, 8:] = 1.0, 2.0
+    q, s = ops.silu_mul_quant_int8(x.to(device))
+    assert int(q[0].abs().max()) == 0 and q[1].tolist() == [-127] * 8 and abs(float(s[1]) - 600 / 127) < 1e-4
+    assert bool(s[2:4].isnan().all()) and int(q[2:4].abs().max()) == 0 and q[4].tolist() == [127] * 8
+
+
+# ---------------------------------------------------------------------------- GPU: sorted by expert and back
+def routing(tokens, experts, k, seed, absent=False, skew=False, dtype=torch.int32):
+    ids = torch.stack([torch.randperm(max(experts, k), generator=gen(seed + t))[:k] for t in range(tokens)]) if tokens else torch.zeros(0, k, dtype=torch.long)
+    if skew:
+        ids = torch.where(ids % 3 == 0, ids, torch.zeros_like(ids))
+    if absent:
+        ids = ids * 2 - 1
+    return ids.to(dtype)
+
+
+def _order(dev, ids, experts):
+    order = ops.moe_sort(ids.to(dev), experts)
+    indptr, rows, slots = R.ref_sort(ids, experts)
+    assert order.indptr.tolist() == indptr and order.rows.flatten().tolist() == rows and order.slots.tolist() == slots
+    assert order.rows.shape == ids.shape and all(t.dtype == torch.int32 for t in order)
+    return order
+
+
+ROUTES = [(0, 4, 2), (1, 1, 1), (1, 8, 8), (5, 4, 2), (16, 64, 6), (33, 300, 8), (64, 512, 2), (200, 7, 3), (1000, 64, 6), (3000, 128, 8), (9000, 16, 4)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,experts,k", ROUTES)
+def test_sort(device, tokens, experts, k):
+    for absent, skew, dtype in ((False, False, torch.int32), (True, False, torch.int64), (False, True, torch.int32)):
+        _order(device, routing(tokens, experts, k, 7, absent, skew, dtype), experts)
+    same = torch.full((tokens, k), experts - 1, dtype=torch.int32)
+    _order(device, same, experts)
+    _order(device, torch.full_like(same, -1), experts)
+
+
+@pytest.mark.gpu
+def test_sort_refuses(device):
+    ids = torch.zeros(3, 2, dtype=torch.int32, device=device)
+    with pytest.raises(_lib.TileGymHipError):
+        ops.moe_sort(ids, 513)
+    with pytest.raises(_lib.TileGymHipError):
+        ops.moe_sort(ids, 0)
+    with pytest.raises(ValueError):
+        ops.moe_sort(ids.flatten(), 4)
+    assert ops.moe_sort(torch.zeros(2, 3, dtype=torch.int32, device=device).t(), 4).rows.shape == (3, 2)
+
+
+WIDTHS = [1, 7, 8, 64, 100, 2048, 2056, 4100, 7168]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("h", WIDTHS)
+@pytest.mark.parametrize("t", [BF16, F16, F32])
+def test_there_and_back(device, h, t):
+    for tokens, experts, k, absent in ((1, 4, 2, False), (37, 16, 3, True), (20, 64, 8, False), (9, 32, 11, True)):
+        order = _order(device, routing(tokens, experts, k, h, absent), experts)
+        rows = order.rows.cpu()
+        x = torch.randn(tokens, h, generator=gen(h)).to(t)
+        there = ops.moe_permute(x.to(device), order)
+        assert torch.equal(bits(there), bits(R.ref_permute(x, rows).to(t)))
+        q, s = ops.moe_permute_quant_int8(x.to(device), order)
+        wq, ws = R.ref_quant(x)
+        live = (rows >= 0).flatten()
+        where = rows.flatten()[live].long()
+        token = torch.arange(tokens)[:, None].expand(-1, k).flatten()[live]
+        assert torch.equal(q.cpu()[where], wq[token]) and torch.equal(s.cpu()[where], ws[token])
+        dead = int(order.indptr[-1])
+        assert int(q[dead:].abs().sum()) == 0 and bool((s[dead:] == 1).all())
+
+        y = torch.randn(tokens * k, h, generator=gen(h + 1)).to(t)
+        y[dead:] = float("nan")  # (rows behind the last expert are not read)
+        back = ops.moe_unpermute(y.to(device), order)
+        exact, size = R.ref_unpermute(y, rows)
+        near(back, exact, size, t, k)
+        for wt in (F32, BF16, F16):
+            w = torch.rand(tokens, k, generator=gen(h + 2)).to(wt)
+            exact, size = R.ref_unpermute(y, rows, w)
+            near(ops.moe_unpermute(y.to(device), order, w.to(device)), exact, size, t, k)
+
+            g = torch.randn(tokens, h, generator=gen(h + 3)).to(t)
+            gx, gw = ops.moe_unpermute_backward(g.to(device), y.to(device), order, w.to(device))
+            ex, ew, size = R.ref_unpermute_backward(g, y, rows, w)
+            near(gx, ex, ex.abs(), t, 1)
+            assert gw.dtype == wt
+            near(gw, ew, size, wt, h / 64 + 16)  # (a lane's sum, then the lanes': far fewer additions in a row than this)
+        gp = torch.randn(tokens * k, h, generator=gen(h + 4)).to(t)
+        exact, size = R.ref_unpermute(gp, rows)
+        near(ops.moe_permute_backward(gp.to(device), order), exact, size, t, k)
+
+
+@pytest.mark.gpu
+def test_places_beyond_the_rows_are_left_out(device):
+    rows = torch.tensor([[0, 99], [-99, 1]], dtype=torch.int32, device=device)
+    order = ops.MoeOrder(torch.zeros(2, dtype=torch.int32, device=device), rows, rows.flatten())
+    x = torch.randn(2, 16, device=device)
+    there = ops.moe_permute(x, order)
+    assert torch.equal(there[:2], x)
+    q, s = ops.moe_permute_quant_int8(x, order)
+    assert torch.equal(q[:2], ops.quant_int8(x)[0])
+    y = torch.randn(4, 16, device=device)
+    assert torch.equal(ops.moe_unpermute(y, order), y[:2])
+    gx, gw = ops.moe_unpermute_backward(x, y, order, torch.ones(2, 2, device=device))
+    assert torch.equal(gx[:2], x) and gw[0, 1] == 0 and gw[1, 0] == 0
+
+
+@pytest.mark.gpu
+def test_gradients(device):
+    """autograd's gradients are the formula's, and agree with differences: both ways are linear in each argument."""
+    tokens, experts, k, h = 50, 16, 3, 264
+    order = ops.moe_sort(routing(tokens, experts, k, 3, absent=True).to(device), experts)
+    x = torch.randn(tokens, h, device=device, requires_grad=True)
+    w = torch.rand(tokens, k, device=device, requires_grad=True)
+    g = torch.randn(tokens, h, device=device)
+    c = torch.randn(tokens * k, h, device=device)
+
+    def run(x, w):
+        return (ops.moe_unpermute(ops.moe_permute(x, order) * c, order, w) * g).sum()
+
+    gx, gw = torch.autograd.grad(run(x, w), (x, w))
+    grad_made, want_w = ops.moe_unpermute_backward(g, ops.moe_permute(x.detach(), order) * c, order, w.detach())
+    assert torch.equal(gw, want_w) and torch.equal(gx, ops.moe_permute_backward(grad_made * c, order))
+    with torch.no_grad():
+        for value, grad, name in ((x, gx, "x"), (w, gw, "w")):
+            d = torch.randn_like(value)
+            plus, minus = (run(*((value + s * d, w) if name == "x" else (x, value + s * d))) for s in (1.0, -1.0))
+            want, got = float((plus.double() - minus.double()) / 2), float((grad.double() * d.double()).sum())
+            # both sides are sums of tokens * k * h products of values of a few units, each rounded a few times and added in fp32 trees
+            assert abs(want - got) <= 2.0 ** -24 * 40 * float((gx.abs().sum() + gw.abs().sum()) * 10), (name, want, got)
+    # a gradient that is an expanded scalar, and weights left out
+    x2 = torch.randn(tokens, h, device=device, requires_grad=True)
+    ops.moe_unpermute(ops.moe_permute(x2, order), order).sum().backward()
+    here = (order.rows >= 0).sum(1, keepdim=True).float()
+    assert torch.equal(x2.grad, here.expand_as(x2.grad))
+    # inputs of which only one takes a gradient
+    y = torch.randn(tokens * k, h, device=device)
+    (only,) = torch.autograd.grad((ops.moe_unpermute(y, order, w) * g).sum(), w)
+    assert torch.equal(only, ops.moe_unpermute_backward(g, y, order, w.detach())[1])
+
+
+# ---------------------------------------------------------------------------- GPU: together
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,experts,k,h,i,absent", [(1, 8, 2, 256, 128, False), (40, 16, 4, 512, 192, False), (300, 8, 2, 256, 320, True), (7, 64, 6, 1024, 96, True)])
+def test_layer(device, tokens, experts, k, h, i, absent):
+    """The layer out of its operators, against the same steps in float64 from the int8 rows on."""
+    x = torch.randn(tokens, h, generator=gen(1)).to(BF16)
+    w1, s1 = R.ref_quant(torch.randn(experts * 2 * i, h, generator=gen(2)) / h ** 0.5)
+    w2, s2 = R.ref_quant(torch.randn(experts * h, i, generator=gen(3)) / i ** 0.5)
+    w1, s1, w2, s2 = w1.view(experts, 2 * i, h), s1.view(experts, 2 * i), w2.view(experts, h, i), s2.view(experts, h)
+    ids, w = routing(tokens, experts, k, 4, absent), torch.rand(tokens, k, generator=gen(5))
+    out = ops.int8_moe(*(t.to(device) for t in (x, w1, w2, s1, s2, w, ids)))
+    assert out.shape == x.shape and out.dtype == BF16
+    q, s = R.ref_quant(x)
+    want = torch.zeros(tokens, h, dtype=torch.float64)
+    for t in range(tokens):
+        for j in range(k):
+            e = int(ids[t, j])
+            if not 0 <= e < experts:
+                continue
+            hid = R.ref_int8_matmul_f32(q[t:t + 1], w1[e], s[t:t + 1], s1[e]).to(BF16)
+            act = hid[:, :i].double() * torch.sigmoid(hid[:, :i].double()) * hid[:, i:].double()
+            aq, asc = R.ref_quant(act)
+            want[t] += float(w[t, j]) * R.ref_int8_matmul_f32(aq, w2[e], asc, s2[e]).to(BF16).double()[0]
+    # A code of the activation may fall on the other side of a tie, by one step in rows of i codes; all else is the rounding of the result.
+    step = 2.0 ** -8 * want.abs() + 2.0 ** -7 * want.abs().amax(1, keepdim=True)
+    assert bool(((out.cpu().double() - want).abs() <= step + 1e-30).all())
+
+
+@pytest.mark.gpu
+def test_captured_and_replayed(device):
+    """A routing, a layer and both gradients in one graph: replayed over new inputs, with eager work between, every replay is the eager result."""
+    tokens, experts, k, h, i = 24, 16, 3, 256, 128
+    w1, w2 = codes((experts, 2 * i, h), 1).to(device), codes((experts, h, i), 2).to(device)
+    s1, s2 = scales((experts, 2 * i), 3).to(device) / 100, scales((experts, h), 4).to(device) / 100
+    x, g = torch.zeros(tokens, h, dtype=BF16, device=device), torch.zeros(tokens, h, dtype=BF16, device=device)
+    w, ids = torch.zeros(tokens, k, device=device), torch.zeros(tokens, k, dtype=torch.int32, device=device)
+
+    def run():
+        order = ops.moe_sort(ids, experts)
+        rows = ops.moe_permute(x, order)
+        made = ops.int8_moe(x, w1, w2, s1, s2, w, ids)
+        grad_rows, gw = ops.moe_unpermute_backward(g, rows, order, w)
+        return (*order, rows, made, ops.moe_unpermute(rows, order, w), grad_rows, gw, ops.moe_permute_backward(grad_rows, order))
+
+    def fill(seed):
+        x.copy_(torch.randn(tokens, h, generator=gen(seed)))
+        g.copy_(torch.randn(tokens, h, generator=gen(seed + 1)))
+        w.copy_(torch.rand(tokens, k, generator=gen(seed + 2)))
+        ids.copy_(routing(tokens, experts, k, seed, absent=seed % 2 == 1))
+
+    fill(0)
+    run()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        run()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = run()
+    for seed in range(1, 6):
+        fill(seed)
+        graph.replay()
+        got = [t.clone() for t in held]
+        want = run()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(bits(a), bits(b))
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(device):
+    """Calls on two streams share nothing."""
+    a = [codes((300, 512), s).to(device) for s in (1, 2)]
+    b = [codes((1024, 512), s).to(device) for s in (3, 4)]
+    one = torch.full((1,), 0.01, device=device)
+    want = [ops.int8_matmul(x, y, one, one) for x, y in zip(a, b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(5):
+        for s, x, y, to in zip(streams, a, b, got):
+            with torch.cuda.stream(s):
+                to.append(ops.int8_matmul(x, y, one, one))
+    torch.cuda.synchronize()
+    assert all(torch.equal(bits(o), bits(w)) for to, w in zip(got, want) for o in to)

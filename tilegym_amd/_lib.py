@@ -139,6 +139,22 @@ def load():
     L.tg_fp8_kv_attention_workspace_bytes.argtypes = [ctypes.c_int64] * 7 + [ctypes.c_int32, ctypes.c_int32]
     L.tg_fp8_kv_attention.restype = ctypes.c_int32
     L.tg_fp8_kv_attention.argtypes = [P] * 9 + [ctypes.c_float, ctypes.c_int32, ctypes.c_int32, P, ctypes.c_int32, ctypes.c_uint64]
+    L.tg_int8_gemm.restype = ctypes.c_int32
+    L.tg_int8_gemm.argtypes = [P] * 7 + [I32P, ctypes.c_int32, ctypes.c_int32, ctypes.c_uint64]
+    L.tg_int8_gemm_workspace_bytes.restype = ctypes.c_int64
+    L.tg_int8_gemm_workspace_bytes.argtypes = [ctypes.c_int64] * 3
+    L.tg_int8_ragged_gemm.restype = ctypes.c_int32
+    L.tg_int8_ragged_gemm.argtypes = [P] * 6 + [I32P, ctypes.c_int32, ctypes.c_int32, ctypes.c_uint64]
+    L.tg_int8_quant.restype = ctypes.c_int32
+    L.tg_int8_quant.argtypes = [P] * 4 + [ctypes.c_int32, ctypes.c_int32, ctypes.c_uint64]
+    L.tg_moe_sort.restype = ctypes.c_int32
+    L.tg_moe_sort.argtypes = [P, ctypes.c_int32, P, P, P, ctypes.c_int32, ctypes.c_uint64]
+    L.tg_moe_permute.restype = ctypes.c_int32
+    L.tg_moe_permute.argtypes = [P] * 3 + [ctypes.c_int32, ctypes.c_uint64]
+    L.tg_moe_unpermute.restype = ctypes.c_int32
+    L.tg_moe_unpermute.argtypes = [P] * 4 + [ctypes.c_int32, ctypes.c_uint64]
+    L.tg_moe_unpermute_backward.restype = ctypes.c_int32
+    L.tg_moe_unpermute_backward.argtypes = [P] * 6 + [ctypes.c_int32, ctypes.c_uint64]
     L.tg_moe_sum.restype = ctypes.c_int32
     L.tg_moe_sum.argtypes = [P, P, ctypes.c_int32, ctypes.c_uint64]
     L.tg_moe_sum_routed.restype = ctypes.c_int32
@@ -618,6 +634,57 @@ def fp8_kv_attention(out, q, cache, block_table, seq_lens, indptr, sm_scale: flo
     rc = L.tg_fp8_kv_attention(_desc(out), _desc(q), *[_desc(t) for t in cache], _desc(block_table), _desc(seq_lens), _desc(indptr),
                                float(sm_scale), int(window), int(sink_tokens), _desc(ws), dev, _stream_handle(q))
     check_rc(rc, "tg_fp8_kv_attention")
+
+
+def int8_gemm(c, a, b, scale_a, scale_b, bias=None, kernel_configs=None) -> None:
+    """The scratch memory of a split K is the call's own, as fp8_kv_attention's."""
+    L = _lib if _lib is not None else load()
+    dev, ws = _device_index(a), None
+    cfg, ncfg = _cfg(kernel_configs)
+    if a.dim() == 2 and b.dim() == 2:
+        need = L.tg_int8_gemm_workspace_bytes(a.shape[0], b.shape[0], a.shape[1])
+        if need > 0:
+            ws = torch.empty(need, dtype=torch.uint8, device=a.device)
+    rc = L.tg_int8_gemm(_desc(c), _desc(a), _desc(b), _desc(scale_a), _desc(scale_b), _desc(bias), _desc(ws), cfg, ncfg, dev, _stream_handle(a))
+    check_rc(rc, "tg_int8_gemm")
+
+
+def int8_ragged_gemm(c, a, b, scale_a, scale_b, m_indptr, kernel_configs=None) -> None:
+    L = _lib if _lib is not None else load()
+    cfg, ncfg = _cfg(kernel_configs)
+    rc = L.tg_int8_ragged_gemm(_desc(c), _desc(a), _desc(b), _desc(scale_a), _desc(scale_b), _desc(m_indptr), cfg, ncfg, _device_index(a), _stream_handle(a))
+    check_rc(rc, "tg_int8_ragged_gemm")
+
+
+def int8_quant(q, scales, x, place=None, silu_mul: bool = False) -> None:
+    L = _lib if _lib is not None else load()
+    rc = L.tg_int8_quant(_desc(q), _desc(scales), _desc(x), _desc(place), int(bool(silu_mul)), _device_index(x), _stream_handle(x))
+    check_rc(rc, "tg_int8_quant")
+
+
+def moe_sort(topk_ids, num_experts: int, indptr, rows, slots) -> None:
+    L = _lib if _lib is not None else load()
+    rc = L.tg_moe_sort(_desc(topk_ids), int(num_experts), _desc(indptr), _desc(rows), _desc(slots), _device_index(topk_ids), _stream_handle(topk_ids))
+    check_rc(rc, "tg_moe_sort")
+
+
+def moe_permute(out, x, rows) -> None:
+    L = _lib if _lib is not None else load()
+    rc = L.tg_moe_permute(_desc(out), _desc(x), _desc(rows), _device_index(x), _stream_handle(x))
+    check_rc(rc, "tg_moe_permute")
+
+
+def moe_unpermute(out, x, rows, weights=None) -> None:
+    L = _lib if _lib is not None else load()
+    rc = L.tg_moe_unpermute(_desc(out), _desc(x), _desc(rows), _desc(weights), _device_index(x), _stream_handle(x))
+    check_rc(rc, "tg_moe_unpermute")
+
+
+def moe_unpermute_backward(grad_x, grad_weights, grad_out, x, rows, weights) -> None:
+    L = _lib if _lib is not None else load()
+    rc = L.tg_moe_unpermute_backward(_desc(grad_x), _desc(grad_weights), _desc(grad_out), _desc(x), _desc(rows), _desc(weights), _device_index(x),
+                                     _stream_handle(x))
+    check_rc(rc, "tg_moe_unpermute_backward")
 
 
 def moe_sum(x: torch.Tensor, out: torch.Tensor) -> None:

@@ -1,0 +1,259 @@
+// Tokens sorted by expert, carried there and back with the router's weights, and the gradients of both ways.
+//
+// sort: a stable counting sort of the (token, slot) pairs by expert.  Pairs whose expert is not here (an id outside [0, E)) are sorted behind the
+// last expert: every pair has a row, and every row a pair.  Every workgroup counts all ids in LDS (those in front of its slice, those behind),
+// ranks its own slice in order, and needs nothing from the others: one launch, no workspace, no order that atomics could change.
+//
+// permute, unpermute and their gradients go by tokens, not by rows: a token's element is read once and written to its top_k rows, or
+// gathered from them, summed in fp32 in the order of the slots and rounded once.  No atomics.  Bound by HBM.
+#include "quant_device.h"
+
+namespace tg {
+namespace {
+
+constexpr int kSortWaves = 16;
+
+// Lanes that hold the same key (keys below 1024), as a mask.
+__device__ __forceinline__ unsigned long long same_key(int key, bool in) {
+    unsigned long long m = __ballot(in);
+#pragma unroll
+    for (int b = 0; b < 10; ++b) {
+        const bool set = (key >> b) & 1;
+        const unsigned long long with = __ballot(set);
+        m &= set ? with : ~with;
+    }
+    return m;
+}
+
+template <typename IdT>
+__global__ void __launch_bounds__(64 * kSortWaves) moe_sort_kernel(const IdT* __restrict__ ids, int n, int E, int per_wave, int* __restrict__ indptr,
+                                                                   int* __restrict__ rows, int* __restrict__ slots) {
+    extern __shared__ int lds[];
+    const int B = E + 1;                   // experts, and the pairs without one
+    int* const mine = lds;                 // [kSortWaves][B]: counts of this workgroup's waves, then their next rows
+    int* const before = mine + kSortWaves * B;  // [B]: pairs in front of this workgroup's slice
+    int* const behind = before + B;        // [B]
+    int* const waves = behind + B;         // [kSortWaves]
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    constexpr int NT = 64 * kSortWaves;
+    for (int i = tid; i < (kSortWaves + 2) * B; i += NT) lds[i] = 0;
+    __syncthreads();
+    const int64_t lo = (int64_t)blockIdx.x * kSortWaves * per_wave, hi = min(lo + (int64_t)kSortWaves * per_wave, (int64_t)n);
+    auto key_of = [&](int64_t i) {
+        const IdT id = ids[i];
+        return id >= 0 && id < E ? (int)id : E;
+    };
+    constexpr int BATCH = 8;  // loads in flight together
+    for (int64_t i0 = tid; i0 < n; i0 += NT * BATCH) {
+        int key[BATCH];
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) key[u] = i0 + u * NT < n ? key_of(i0 + u * NT) : -1;
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) {
+            const int64_t i = i0 + u * NT;
+            if (key[u] < 0) continue;
+            if (i < lo) atomicAdd(&before[key[u]], 1);
+            else if (i >= hi) atomicAdd(&behind[key[u]], 1);
+            else atomicAdd(&mine[(int)((i - lo) / per_wave) * B + key[u]], 1);
+        }
+    }
+    __syncthreads();
+    // thread e: expert e's pairs, and the rows in front of them
+    int total = 0;
+    if (tid < B) {
+        total = before[tid] + behind[tid];
+        for (int w = 0; w < kSortWaves; ++w) total += mine[w * B + tid];
+    }
+    int upto = total;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int t = __shfl_up(upto, d);
+        if (lane >= d) upto += t;
+    }
+    if (lane == 63) waves[wave] = upto;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) upto += waves[w];
+    if (tid < B) {
+        const int first = upto - total;
+        if (blockIdx.x == 0) indptr[tid] = first;
+        int next = first + before[tid];
+        for (int w = 0; w < kSortWaves; ++w) {
+            const int c = mine[w * B + tid];
+            mine[w * B + tid] = next;
+            next += c;
+        }
+    }
+    __syncthreads();
+    volatile int* const cursor = mine + wave * B;  // (written by one lane, read by others of its wave)
+    const int64_t first = lo + (int64_t)wave * per_wave, last = min(first + per_wave, (int64_t)n);
+    for (int64_t i0 = first; i0 < last; i0 += 64) {
+        const int64_t i = i0 + lane;
+        const bool in = i < last;
+        const int key = in ? key_of(i) : 0;
+        const unsigned long long same = same_key(key, in);
+        const int rank = __popcll(same & ((1ull << lane) - 1));
+        int row = 0;
+        if (in) {
+            row = cursor[key] + rank;
+            rows[i] = key < E ? row : -1 - row;
+            slots[row] = (int)i;
+        }
+        __builtin_amdgcn_wave_barrier();
+        if (in && rank == 0) cursor[key] = row + __popcll(same);  // (LDS serves a wave's accesses in their order)
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// ---------------------------------------------------------------------------- there and back
+template <typename T, bool VEC>
+__device__ __forceinline__ v8f_q get8(const T* p, int at, int H) {
+    if constexpr (VEC) return load8<T>(p + at);
+    v8f_q v;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = at + k < H ? (float)p[at + k] : 0.f;
+    return v;
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void set8(T* p, int at, int H, v8f_q v) {
+    if constexpr (VEC) {
+        if constexpr (sizeof(T) == 4) {
+            reinterpret_cast<v4f*>(p + at)[0] = __builtin_shufflevector(v, v, 0, 1, 2, 3);
+            reinterpret_cast<v4f*>(p + at)[1] = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+        } else {
+            typedef T t8 __attribute__((ext_vector_type(8)));
+            *reinterpret_cast<t8*>(p + at) = __builtin_convertvector(v, t8);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (at + k < H) p[at + k] = (T)v[k];
+    }
+}
+
+__device__ __forceinline__ float weight_of(const void* w, int type, int64_t i) {
+    return !w ? 1.f : type == OUT_F32 ? ((const float*)w)[i] : type == OUT_BF16 ? (float)((const __bf16*)w)[i] : (float)((const _Float16*)w)[i];
+}
+
+constexpr int kRouteLanes = 256;
+
+// rows[place] = x[token] for each of a token's places; zeros where it has no expert.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kRouteLanes) moe_permute_kernel(const MoeRouteParams p) {
+    const int64_t token = blockIdx.x, places = p.tokens * p.top_k;
+    const T* x = (const T*)p.x + token * p.H;
+    const int* rows = p.rows + token * p.top_k;
+    for (int at = (int)threadIdx.x * 8; at < p.H; at += kRouteLanes * 8) {
+        const v8f_q v = get8<T, VEC>(x, at, p.H);
+        v8f_q zero = v;
+        zero = 0.f;
+        for (int j = 0; j < p.top_k; ++j) {
+            const int r = rows[j];
+            const int64_t to = r < 0 ? -1 - (int64_t)r : r;
+            if (to < places) set8<T, VEC>((T*)p.out + to * p.H, at, p.H, r < 0 ? zero : v);
+        }
+    }
+}
+
+// out[token] = the sum over its slots of weight * x[place]
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kRouteLanes) moe_unpermute_kernel(const MoeRouteParams p) {
+    const int64_t token = blockIdx.x, places = p.tokens * p.top_k;
+    const int* rows = p.rows + token * p.top_k;
+    for (int at = (int)threadIdx.x * 8; at < p.H; at += kRouteLanes * 8) {
+        v8f_q sum;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum[k] = 0.f;
+        for (int j = 0; j < p.top_k; ++j) {
+            const int64_t r = rows[j];
+            if (r < 0 || r >= places) continue;
+            const v8f_q v = get8<T, VEC>((const T*)p.x + r * p.H, at, p.H);
+            const float w = weight_of(p.weights, p.weights_type, token * p.top_k + j);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sum[k] = __builtin_fmaf(w, v[k], sum[k]);
+        }
+        set8<T, VEC>((T*)p.out + token * p.H, at, p.H, sum);
+    }
+}
+
+// out[place] = weight * x[token]; grad_weights[slot] = <x[token], made[place]>
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kRouteLanes) moe_unpermute_backward_kernel(const MoeRouteParams p) {
+    __shared__ float part[kRouteLanes / 64];
+    const int64_t token = blockIdx.x, places = p.tokens * p.top_k;
+    const int tid = threadIdx.x;
+    const T* x = (const T*)p.x + token * p.H;
+    const int* rows = p.rows + token * p.top_k;
+    for (int j = 0; j < p.top_k; ++j) {
+        const int r = rows[j];
+        const int64_t to = r < 0 ? -1 - (int64_t)r : r;
+        const bool here = r >= 0 && to < places;
+        const float w = weight_of(p.weights, p.weights_type, token * p.top_k + j);
+        float dot = 0.f;
+        if (to < places) {
+            for (int at = tid * 8; at < p.H; at += kRouteLanes * 8) {
+                v8f_q g = get8<T, VEC>(x, at, p.H);
+                if (here) {
+                    const v8f_q m = get8<T, VEC>((const T*)p.made + to * p.H, at, p.H);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) dot = __builtin_fmaf(g[k], m[k], dot);
+                    g *= w;
+                } else {
+                    g = 0.f;
+                }
+                set8<T, VEC>((T*)p.out + to * p.H, at, p.H, g);
+            }
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) dot += __shfl_xor(dot, d);
+        if (tid % 64 == 0) part[tid / 64] = dot;
+        __syncthreads();
+        if (tid == 0) {
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < kRouteLanes / 64; ++i) sum += part[i];
+            const int64_t at = token * p.top_k + j;
+            if (p.weights_type == OUT_F32) ((float*)p.grad_weights)[at] = sum;
+            else if (p.weights_type == OUT_BF16) ((__bf16*)p.grad_weights)[at] = (__bf16)sum;
+            else ((_Float16*)p.grad_weights)[at] = (_Float16)sum;
+        }
+        __syncthreads();
+    }
+}
+
+template <typename T, bool VEC>
+hipError_t launch(int which, const MoeRouteParams& p, hipStream_t s) {
+    const dim3 grid((unsigned)p.tokens), block(kRouteLanes);
+    if (which == 0) hipLaunchKernelGGL((moe_permute_kernel<T, VEC>), grid, block, 0, s, p);
+    else if (which == 1) hipLaunchKernelGGL((moe_unpermute_kernel<T, VEC>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((moe_unpermute_backward_kernel<T, VEC>), grid, block, 0, s, p);
+    return hipGetLastError();
+}
+hipError_t launch_type(int which, const MoeRouteParams& p, int type, hipStream_t s) {
+    if (p.tokens <= 0) return hipSuccess;
+    if (type == OUT_F32) return p.vec ? launch<float, true>(which, p, s) : launch<float, false>(which, p, s);
+    if (type == OUT_BF16) return p.vec ? launch<__bf16, true>(which, p, s) : launch<__bf16, false>(which, p, s);
+    if (type == OUT_F16) return p.vec ? launch<_Float16, true>(which, p, s) : launch<_Float16, false>(which, p, s);
+    return hipErrorInvalidValue;
+}
+
+}  // namespace
+
+hipError_t run_moe_sort(const void* ids, bool ids_are_i64, int n, int E, int* indptr, int* rows, int* slots, hipStream_t s) {
+    if (E < 1 || E > kSortMaxExperts) return hipErrorInvalidValue;
+    // up to 32 workgroups; a wave's slice is a multiple of 64 pairs
+    int groups = (n + 1023) / 1024;
+    groups = groups < 1 ? 1 : groups > 32 ? 32 : groups;
+    const int64_t waves = (int64_t)groups * kSortWaves;
+    const int per_wave = (int)((((int64_t)n + waves - 1) / waves + 63) / 64 * 64);
+    const int bytes = ((kSortWaves + 2) * (E + 1) + kSortWaves) * 4;
+    if (ids_are_i64) hipLaunchKernelGGL(moe_sort_kernel<int64_t>, dim3(groups), dim3(64 * kSortWaves), bytes, s, (const int64_t*)ids, n, E, per_wave > 0 ? per_wave : 64, indptr, rows, slots);
+    else hipLaunchKernelGGL(moe_sort_kernel<int>, dim3(groups), dim3(64 * kSortWaves), bytes, s, (const int*)ids, n, E, per_wave > 0 ? per_wave : 64, indptr, rows, slots);
+    return hipGetLastError();
+}
+
+int64_t moe_route_threads(const MoeRouteParams& p) { return p.tokens * kRouteLanes; }
+hipError_t run_moe_permute(const MoeRouteParams& p, int type, hipStream_t s) { return launch_type(0, p, type, s); }
+hipError_t run_moe_unpermute(const MoeRouteParams& p, int type, hipStream_t s) { return launch_type(1, p, type, s); }
+hipError_t run_moe_unpermute_backward(const MoeRouteParams& p, int type, hipStream_t s) { return launch_type(2, p, type, s); }
+
+}  // namespace tg

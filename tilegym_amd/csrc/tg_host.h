@@ -192,6 +192,60 @@ inline int64_t kv_attention_part_bytes(int64_t splits, int64_t rows, int64_t q_h
 }
 int64_t kv_attention_threads(const KvAttentionParams& p);
 hipError_t run_kv_attention(const KvAttentionParams& p, bool is_bf16, hipStream_t s);
+// Products in 8-bit integers (int8_device.h)
+struct Int8GemmParams {
+    const int8_t* A;         // (M, K)
+    const int8_t* B;         // (N, K), or (E, N, K)
+    void* C;                 // rows of ldc elements of out_type
+    const float *sa, *sb;    // a scale per row of A and per row of B; with a step of 0 one for all
+    const void* bias;        // (N) of bias_type, or null
+    int sa_step, sb_step, bias_type, out_type;
+    int M, N, K;
+    int64_t ldc;
+    int vec_store;           // 16-byte stores of 8 outputs are aligned
+    int split_k, ksteps_per_split;  // steps of 128 bytes
+    int* partials;           // (split_k, M, N)
+    const int* m_indptr;     // ragged: (E + 1); else null
+    int E;
+};
+// any sizes and addresses
+int64_t int8_simple_threads(const Int8GemmParams& p);
+hipError_t run_int8_simple(const Int8GemmParams& p, hipStream_t s);
+
+// A row's int8 codes and its scale (int8_quant.hip)
+struct Int8QuantParams {
+    const void* x;           // (rows, K), or with silu_mul (rows, 2 K): gate, then up
+    int8_t* q;               // (rows, K), or with `place` (places, K)
+    float* scales;
+    int64_t rows;
+    int K;
+    int silu_mul;
+    const int* place;        // (rows, copies): where each row's copies go (below zero: zeros to -1 - place); null: where the row is
+    int copies;
+    int64_t places;
+};
+int64_t int8_quant_threads(const Int8QuantParams& p);
+hipError_t run_int8_quant(const Int8QuantParams& p, int x_type, hipStream_t s);
+
+// Tokens sorted by expert and back (moe_route.hip)
+constexpr int kSortMaxExperts = 512;
+hipError_t run_moe_sort(const void* ids, bool ids_are_i64, int n, int E, int* indptr, int* rows, int* slots, hipStream_t s);
+struct MoeRouteParams {
+    const void* x;           // permute, gradient: (tokens, H); unpermute: (tokens * top_k, H)
+    const void* made;        // gradient: what was weighted, (tokens * top_k, H)
+    void* out;
+    const int* rows;         // (tokens, top_k): the row of each slot; below zero, -1 - row, where it has no expert here
+    const void* weights;     // (tokens, top_k) or null
+    void* grad_weights;
+    int weights_type;
+    int64_t tokens;
+    int top_k, H;
+    int vec;                 // H and the addresses allow 16-byte vectors
+};
+int64_t moe_route_threads(const MoeRouteParams& p);
+hipError_t run_moe_permute(const MoeRouteParams& p, int type, hipStream_t s);
+hipError_t run_moe_unpermute(const MoeRouteParams& p, int type, hipStream_t s);
+hipError_t run_moe_unpermute_backward(const MoeRouteParams& p, int type, hipStream_t s);
 // dst (cols, rows) <- transpose of src (rows, cols), one byte per element
 // dst (cols x ld) = transpose of src (rows x cols), zero beyond `rows` in every dst row
 hipError_t run_transpose_u8(const uint8_t* src, uint8_t* dst, int rows, int cols, int ld, hipStream_t s);

@@ -2238,6 +2238,240 @@ int32_t tg_fp8_kv_attention(const tg_tensor* out, const tg_tensor* q, const tg_t
     return TG_OK;
 }
 
+// ---------------------------------------------------------------------------- products in 8-bit integers
+constexpr int64_t kInt8MostK = 131071;  // 2^14 * K stays below 2^31
+
+// a scale per row of an operand, or one for all
+static int32_t check_int8_scale(const tg_tensor* t, const char* name, int64_t rows, int* step) {
+    int32_t rc;
+    if ((rc = check_tensor(t, name, -1))) return rc;
+    if (t->dtype != TG_F32) return fail(TG_ERR_DTYPE, "%s must be f32", name);
+    const int64_t n = numel(t);
+    if (n != rows && n != 1) return fail(TG_ERR_INVALID, "%s must have %lld elements, or one, got %lld", name, (long long)rows, (long long)n);
+    *step = n == rows && rows != 1 ? 1 : 0;
+    return TG_OK;
+}
+
+static int32_t int8_operands(tg::Int8GemmParams& p, const tg_tensor* c, const tg_tensor* a, const tg_tensor* b, const tg_tensor* scale_a, const tg_tensor* scale_b) {
+    int32_t rc;
+    const int64_t M = a->shape[0], K = a->shape[1], N = b->shape[b->ndim - 2], E = b->ndim == 3 ? b->shape[0] : 1;
+    if (a->dtype != TG_I8 || b->dtype != TG_I8) return fail(TG_ERR_DTYPE, "a and b must be int8 (dtype code 8), got %d and %d", a->dtype, b->dtype);
+    const int out_type = io_type_of(c->dtype);
+    if (out_type < 0) return fail(TG_ERR_DTYPE, "c must be bf16, f16 or f32, got dtype code %d", c->dtype);
+    if (b->shape[b->ndim - 1] != K)
+        return fail(TG_ERR_INVALID, "incompatible matrices: K of a is %lld, K of b is %lld", (long long)K, (long long)b->shape[b->ndim - 1]);
+    if (c->shape[0] != M || c->shape[1] != N)
+        return fail(TG_ERR_INVALID, "c must be (%lld, %lld), got (%lld, %lld)", (long long)M, (long long)N, (long long)c->shape[0], (long long)c->shape[1]);
+    if (K < 1 || K > kInt8MostK) return fail(TG_ERR_INVALID, "K must be 1 to %lld (sums in 32 bits), got %lld", (long long)kInt8MostK, (long long)K);
+    if (M > INT32_MAX - 1024 || N > INT32_MAX - 1024) return fail(TG_ERR_INVALID, "extent exceeds int32");
+    if ((rc = check_int8_scale(scale_a, "scale_a", M, &p.sa_step)) || (rc = check_int8_scale(scale_b, "scale_b", E * N, &p.sb_step))) return rc;
+    p.A = reinterpret_cast<const int8_t*>(a->ptr);
+    p.B = reinterpret_cast<const int8_t*>(b->ptr);
+    p.C = reinterpret_cast<void*>(c->ptr);
+    p.sa = reinterpret_cast<const float*>(scale_a->ptr);
+    p.sb = reinterpret_cast<const float*>(scale_b->ptr);
+    p.out_type = out_type;
+    p.M = (int)M, p.N = (int)N, p.K = (int)K, p.ldc = N, p.E = (int)E;
+    p.split_k = 1;
+    p.vec_store = N % 8 == 0 && aligned16(c->ptr);
+    return TG_OK;
+}
+
+int32_t tg_int8_gemm(const tg_tensor* c, const tg_tensor* a, const tg_tensor* b, const tg_tensor* scale_a, const tg_tensor* scale_b, const tg_tensor* bias,
+                     const tg_tensor* workspace, const int32_t* cfg, int32_t ncfg, int32_t device_id, uint64_t hip_stream) {
+    g_err[0] = 0;
+    int32_t rc;
+    if ((rc = check_tensor(a, "a", 2)) || (rc = check_tensor(b, "b", 2)) || (rc = check_tensor(c, "c", 2))) return rc;
+    tg::Int8GemmParams p{};
+    if ((rc = int8_operands(p, c, a, b, scale_a, scale_b))) return rc;
+    if (bias) {
+        if ((rc = check_tensor(bias, "bias", 1))) return rc;
+        p.bias_type = io_type_of(bias->dtype);
+        if (p.bias_type < 0) return fail(TG_ERR_DTYPE, "bias must be bf16, f16 or f32, got dtype code %d", bias->dtype);
+        if (bias->shape[0] != p.N) return fail(TG_ERR_INVALID, "bias must have %d elements, got %lld", p.N, (long long)bias->shape[0]);
+        p.bias = reinterpret_cast<const void*>(bias->ptr);
+    }
+    if (p.M == 0 || p.N == 0) return TG_OK;
+    if ((rc = check_threads(tg::int8_simple_threads(p), "int8_gemm"))) return rc;
+    DeviceGuard guard(device_id);
+    if (!guard.ok) return fail(TG_ERR_DEVICE, "cannot use HIP device %d", device_id);
+    const hipError_t e = tg::run_int8_simple(p, reinterpret_cast<hipStream_t>(hip_stream));
+    if (e != hipSuccess) return fail(TG_ERR_LAUNCH, "int8_gemm launch failed: %s", hipGetErrorString(e));
+    return TG_OK;
+}
+
+int64_t tg_int8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) { return 0; }
+
+int32_t tg_int8_ragged_gemm(const tg_tensor* c, const tg_tensor* a, const tg_tensor* b, const tg_tensor* scale_a, const tg_tensor* scale_b,
+                            const tg_tensor* m_indptr, const int32_t* cfg, int32_t ncfg, int32_t device_id, uint64_t hip_stream) {
+    g_err[0] = 0;
+    int32_t rc;
+    if ((rc = check_tensor(a, "a", 2)) || (rc = check_tensor(b, "b", 3)) || (rc = check_tensor(c, "c", 2)) || (rc = check_tensor(m_indptr, "m_indptr", 1))) return rc;
+    tg::Int8GemmParams p{};
+    if ((rc = int8_operands(p, c, a, b, scale_a, scale_b))) return rc;
+    if (m_indptr->dtype != TG_I32) return fail(TG_ERR_DTYPE, "m_indptr must be int32");
+    const int64_t E = b->shape[0];
+    if (E > INT32_MAX || m_indptr->shape[0] != E + 1) return fail(TG_ERR_INVALID, "m_indptr must have %lld elements, got %lld", (long long)(E + 1), (long long)m_indptr->shape[0]);
+    if (p.M == 0 || p.N == 0 || E == 0) return TG_OK;
+    p.m_indptr = reinterpret_cast<const int*>(m_indptr->ptr);
+    if ((rc = check_threads(tg::int8_simple_threads(p), "int8_ragged_gemm"))) return rc;
+    DeviceGuard guard(device_id);
+    if (!guard.ok) return fail(TG_ERR_DEVICE, "cannot use HIP device %d", device_id);
+    const hipError_t e = tg::run_int8_simple(p, reinterpret_cast<hipStream_t>(hip_stream));
+    if (e != hipSuccess) return fail(TG_ERR_LAUNCH, "int8_ragged_gemm launch failed: %s", hipGetErrorString(e));
+    return TG_OK;
+}
+
+// place (tokens, copies): null, or where a token's copies go
+static int32_t check_places(const tg_tensor* place, const char* name, int64_t tokens) {
+    int32_t rc;
+    if ((rc = check_tensor(place, name, 2))) return rc;
+    if (place->dtype != TG_I32) return fail(TG_ERR_DTYPE, "%s must be int32", name);
+    if (place->shape[0] != tokens) return fail(TG_ERR_INVALID, "%s must have a row for each of the %lld tokens, got %lld", name, (long long)tokens, (long long)place->shape[0]);
+    if (tokens > INT32_MAX || place->shape[1] > INT32_MAX || tokens * place->shape[1] > INT32_MAX) return fail(TG_ERR_INVALID, "too many rows");
+    return TG_OK;
+}
+
+int32_t tg_int8_quant(const tg_tensor* q, const tg_tensor* scales, const tg_tensor* x, const tg_tensor* place, int32_t silu_mul, int32_t device_id,
+                      uint64_t hip_stream) {
+    g_err[0] = 0;
+    int32_t rc;
+    if ((rc = check_tensor(x, "x", -1)) || (rc = check_tensor(q, "q", -1)) || (rc = check_tensor(scales, "scales", -1))) return rc;
+    const int x_type = io_type_of(x->dtype);
+    if (x_type < 0) return fail(TG_ERR_DTYPE, "x must be bf16, f16 or f32");
+    if (q->dtype != TG_I8) return fail(TG_ERR_DTYPE, "q must be int8 (dtype code 8)");
+    if (scales->dtype != TG_F32) return fail(TG_ERR_DTYPE, "scales must be f32");
+    if (x->ndim < 1) return fail(TG_ERR_INVALID, "x needs at least one dimension");
+    const int64_t width = x->shape[x->ndim - 1], K = silu_mul ? width / 2 : width;
+    if (silu_mul && width % 2 != 0) return fail(TG_ERR_INVALID, "the last dimension (%lld) must be even: gate, then up", (long long)width);
+    if (silu_mul && place) return fail(TG_ERR_INVALID, "silu_mul and place exclude each other");
+    int64_t rows = 1;
+    for (int i = 0; i + 1 < x->ndim; ++i) rows *= x->shape[i];
+    if (rows > 0 && (K < 1 || K > INT32_MAX / 4)) return fail(TG_ERR_INVALID, "rows of %lld elements cannot be quantized", (long long)K);
+    tg::Int8QuantParams p{};
+    int64_t places = rows;
+    if (place) {
+        if ((rc = check_places(place, "place", rows))) return rc;
+        places = rows * place->shape[1];
+        p.place = reinterpret_cast<const int*>(place->ptr), p.copies = (int)place->shape[1], p.places = places;
+    }
+    if (numel(q) != places * K || numel(scales) != places) return fail(TG_ERR_INVALID, "q must have %lld elements and scales %lld", (long long)(places * K), (long long)places);
+    if (places == 0) return TG_OK;
+    p.x = reinterpret_cast<const void*>(x->ptr), p.q = reinterpret_cast<int8_t*>(q->ptr), p.scales = reinterpret_cast<float*>(scales->ptr);
+    p.rows = rows, p.K = (int)K, p.silu_mul = silu_mul != 0;
+    if ((rc = check_threads(tg::int8_quant_threads(p), "int8_quant"))) return rc;
+    DeviceGuard guard(device_id);
+    if (!guard.ok) return fail(TG_ERR_DEVICE, "cannot use HIP device %d", device_id);
+    const hipError_t e = tg::run_int8_quant(p, x_type, reinterpret_cast<hipStream_t>(hip_stream));
+    if (e != hipSuccess) return fail(TG_ERR_LAUNCH, "int8_quant launch failed: %s", hipGetErrorString(e));
+    return TG_OK;
+}
+
+// ---------------------------------------------------------------------------- tokens sorted by expert and back
+int32_t tg_moe_sort(const tg_tensor* topk_ids, int32_t num_experts, const tg_tensor* indptr, const tg_tensor* rows, const tg_tensor* slots, int32_t device_id,
+                    uint64_t hip_stream) {
+    g_err[0] = 0;
+    int32_t rc;
+    if ((rc = check_tensor(topk_ids, "topk_ids", -1)) || (rc = check_tensor(indptr, "indptr", 1)) || (rc = check_tensor(rows, "rows", -1)) ||
+        (rc = check_tensor(slots, "slots", -1)))
+        return rc;
+    if (topk_ids->dtype != TG_I32 && topk_ids->dtype != TG_I64) return fail(TG_ERR_DTYPE, "topk_ids must be int32 or int64");
+    if (indptr->dtype != TG_I32 || rows->dtype != TG_I32 || slots->dtype != TG_I32) return fail(TG_ERR_DTYPE, "indptr, rows and slots must be int32");
+    if (num_experts < 1 || num_experts > tg::kSortMaxExperts) return fail(TG_ERR_INVALID, "num_experts must be 1 to %d, got %d", tg::kSortMaxExperts, num_experts);
+    const int64_t n = numel(topk_ids);
+    if (n > INT32_MAX) return fail(TG_ERR_INVALID, "too many slots");
+    if (indptr->shape[0] != num_experts + 1 || numel(rows) != n || numel(slots) != n)
+        return fail(TG_ERR_INVALID, "indptr must have %d elements, rows and slots %lld each", num_experts + 1, (long long)n);
+    DeviceGuard guard(device_id);
+    if (!guard.ok) return fail(TG_ERR_DEVICE, "cannot use HIP device %d", device_id);
+    const hipError_t e = tg::run_moe_sort(reinterpret_cast<const void*>(topk_ids->ptr), topk_ids->dtype == TG_I64, (int)n, num_experts, reinterpret_cast<int*>(indptr->ptr),
+                                          reinterpret_cast<int*>(rows->ptr), reinterpret_cast<int*>(slots->ptr), reinterpret_cast<hipStream_t>(hip_stream));
+    if (e != hipSuccess) return fail(TG_ERR_LAUNCH, "moe_sort launch failed: %s", hipGetErrorString(e));
+    return TG_OK;
+}
+
+// by_token (tokens, H), by_row (tokens * top_k, H), of one type; `made` like by_row or null
+static int32_t route_operands(tg::MoeRouteParams& p, int* type, const tg_tensor* by_token, const char* token_name, const tg_tensor* by_row, const char* row_name,
+                              const tg_tensor* made, const tg_tensor* rows) {
+    int32_t rc;
+    if ((rc = check_tensor(by_token, token_name, 2)) || (rc = check_tensor(by_row, row_name, 2)) || (rc = check_places(rows, "rows", by_token->shape[0]))) return rc;
+    *type = io_type_of(by_token->dtype);
+    if (*type < 0) return fail(TG_ERR_DTYPE, "%s must be bf16, f16 or f32", token_name);
+    if (by_row->dtype != by_token->dtype) return fail(TG_ERR_DTYPE, "%s and %s must have one dtype", token_name, row_name);
+    const int64_t T = by_token->shape[0], H = by_token->shape[1], k = rows->shape[1];
+    if (H > INT32_MAX / 4) return fail(TG_ERR_INVALID, "rows of %lld elements are too long", (long long)H);
+    if (by_row->shape[0] != T * k || by_row->shape[1] != H)
+        return fail(TG_ERR_INVALID, "%s must be (%lld, %lld), got (%lld, %lld)", row_name, (long long)(T * k), (long long)H, (long long)by_row->shape[0], (long long)by_row->shape[1]);
+    if (made) {
+        if ((rc = check_tensor(made, "x", 2))) return rc;
+        if (made->dtype != by_token->dtype) return fail(TG_ERR_DTYPE, "x and %s must have one dtype", token_name);
+        if (made->shape[0] != T * k || made->shape[1] != H) return fail(TG_ERR_INVALID, "x must be (%lld, %lld)", (long long)(T * k), (long long)H);
+        p.made = reinterpret_cast<const void*>(made->ptr);
+    }
+    p.rows = reinterpret_cast<const int*>(rows->ptr);
+    p.tokens = T, p.top_k = (int)k, p.H = (int)H;
+    p.vec = H % 8 == 0 && aligned16(by_token->ptr) && aligned16(by_row->ptr) && (!made || aligned16(made->ptr));
+    return TG_OK;
+}
+static int32_t route_weights(tg::MoeRouteParams& p, const tg_tensor* weights, const tg_tensor* grad_weights) {
+    int32_t rc;
+    if ((rc = check_tensor(weights, "weights", 2))) return rc;
+    p.weights_type = io_type_of(weights->dtype);
+    if (p.weights_type < 0) return fail(TG_ERR_DTYPE, "weights must be bf16, f16 or f32");
+    if (weights->shape[0] != p.tokens || weights->shape[1] != p.top_k) return fail(TG_ERR_INVALID, "weights must be (%lld, %d)", (long long)p.tokens, p.top_k);
+    p.weights = reinterpret_cast<const void*>(weights->ptr);
+    if (!grad_weights) return TG_OK;
+    if ((rc = check_tensor(grad_weights, "grad_weights", 2))) return rc;
+    if (grad_weights->dtype != weights->dtype) return fail(TG_ERR_DTYPE, "grad_weights must have the weights' dtype");
+    if (grad_weights->shape[0] != p.tokens || grad_weights->shape[1] != p.top_k) return fail(TG_ERR_INVALID, "grad_weights must be (%lld, %d)", (long long)p.tokens, p.top_k);
+    p.grad_weights = reinterpret_cast<void*>(grad_weights->ptr);
+    return TG_OK;
+}
+static int32_t route_launch(hipError_t (*run)(const tg::MoeRouteParams&, int, hipStream_t), const char* what, const tg::MoeRouteParams& p, int type, int32_t device_id,
+                            uint64_t hip_stream) {
+    if (const int32_t rc = check_threads(tg::moe_route_threads(p), what)) return rc;
+    DeviceGuard guard(device_id);
+    if (!guard.ok) return fail(TG_ERR_DEVICE, "cannot use HIP device %d", device_id);
+    const hipError_t e = run(p, type, reinterpret_cast<hipStream_t>(hip_stream));
+    if (e != hipSuccess) return fail(TG_ERR_LAUNCH, "%s launch failed: %s", what, hipGetErrorString(e));
+    return TG_OK;
+}
+
+int32_t tg_moe_permute(const tg_tensor* out, const tg_tensor* x, const tg_tensor* rows, int32_t device_id, uint64_t hip_stream) {
+    g_err[0] = 0;
+    tg::MoeRouteParams p{};
+    int type;
+    if (const int32_t rc = route_operands(p, &type, x, "x", out, "out", nullptr, rows)) return rc;
+    if (p.tokens == 0 || p.top_k == 0 || p.H == 0) return TG_OK;
+    p.x = reinterpret_cast<const void*>(x->ptr), p.out = reinterpret_cast<void*>(out->ptr);
+    return route_launch(tg::run_moe_permute, "moe_permute", p, type, device_id, hip_stream);
+}
+
+int32_t tg_moe_unpermute(const tg_tensor* out, const tg_tensor* x, const tg_tensor* rows, const tg_tensor* weights, int32_t device_id, uint64_t hip_stream) {
+    g_err[0] = 0;
+    tg::MoeRouteParams p{};
+    int type;
+    int32_t rc;
+    if ((rc = route_operands(p, &type, out, "out", x, "x", nullptr, rows)) || (weights && (rc = route_weights(p, weights, nullptr)))) return rc;
+    if (p.tokens == 0 || p.H == 0) return TG_OK;
+    p.x = reinterpret_cast<const void*>(x->ptr), p.out = reinterpret_cast<void*>(out->ptr);
+    return route_launch(tg::run_moe_unpermute, "moe_unpermute", p, type, device_id, hip_stream);
+}
+
+int32_t tg_moe_unpermute_backward(const tg_tensor* grad_x, const tg_tensor* grad_weights, const tg_tensor* grad_out, const tg_tensor* x, const tg_tensor* rows,
+                                  const tg_tensor* weights, int32_t device_id, uint64_t hip_stream) {
+    g_err[0] = 0;
+    tg::MoeRouteParams p{};
+    int type;
+    int32_t rc;
+    if (!x) return fail(TG_ERR_NULL, "x: null tensor descriptor");
+    if (!grad_weights) return fail(TG_ERR_NULL, "grad_weights: null tensor descriptor");
+    if ((rc = route_operands(p, &type, grad_out, "grad_out", grad_x, "grad_x", x, rows)) || (rc = route_weights(p, weights, grad_weights))) return rc;
+    if (p.tokens == 0 || p.top_k == 0) return TG_OK;
+    p.x = reinterpret_cast<const void*>(grad_out->ptr), p.out = reinterpret_cast<void*>(grad_x->ptr);
+    return route_launch(tg::run_moe_unpermute_backward, "moe_unpermute_backward", p, type, device_id, hip_stream);
+}
+
 int32_t tg_silu_mul_quant_1x128(const tg_tensor* q, const tg_tensor* scales, const tg_tensor* x,
                                 int32_t device_id, uint64_t hip_stream) {
     g_err[0] = 0;
