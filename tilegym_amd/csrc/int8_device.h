@@ -23,4 +23,92 @@ __device__ __forceinline__ float load_bias(const void* p, int type, int64_t i) {
     return type == OUT_F32 ? load_any<float>(p, i) : type == OUT_BF16 ? load_any<__bf16>(p, i) : load_any<_Float16>(p, i);
 }
 
+// Rows of expert e.  Rows outside the M that a and c have are nobody's, whatever m_indptr holds.
+__device__ __forceinline__ int ragged_rows(const Int8GemmParams& p, int e) {
+    const int lo = p.m_indptr[e], hi = min(p.m_indptr[e + 1], p.M);
+    return lo >= 0 && hi > lo ? hi - lo : 0;
+}
+
+// Workgroup `bid`'s tile of the experts' BM-row tiles x tiles_n columns of them; false: none is left for it.  An expert's row tiles come one after the
+// other over the same columns, so that they share its weight in their XCD's L2.  Every lane of a wave gets the same.
+template <int BM, bool SPREAD>
+__device__ __forceinline__ bool ragged_tile(const Int8GemmParams& p, int bid, int tiles_n, int lane, int& expert, int64_t& m0, int& rows_valid, int& tile_n) {
+    auto scan = [&](int e0, int& rows) {  // row tiles of the experts from e0 up to and with the lane's
+        rows = e0 + lane < p.E ? ragged_rows(p, e0 + lane) : 0;
+        int upto = (rows + BM - 1) / BM;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int t = __shfl_up(upto, d);
+            if (lane >= d) upto += t;
+        }
+        return upto;
+    };
+    int rows = 0, upto = scan(0, rows), total = __shfl(upto, 63);
+    for (int e0 = 64; e0 < p.E; e0 += 64) {
+        int more;
+        total += __shfl(scan(e0, more), 63);
+    }
+    total = __builtin_amdgcn_readfirstlane(total) * tiles_n;
+    if (bid >= total) return false;
+    const int pid = SPREAD ? xcd_remap(bid, total) : bid, row_tile = pid / tiles_n;
+    int base = 0, e0 = 0;
+    unsigned long long hit;
+    while (!(hit = __ballot(base + upto > row_tile))) {
+        base += __shfl(upto, 63);
+        e0 += 64;
+        upto = scan(e0, rows);
+    }
+    const int l = __ffsll((long long)hit) - 1;
+    expert = __builtin_amdgcn_readfirstlane(e0 + l);
+    rows = __builtin_amdgcn_readlane(rows, l);
+    const int mine = (rows + BM - 1) / BM, first = __builtin_amdgcn_readfirstlane(base) + __builtin_amdgcn_readlane(upto, l) - mine;
+    const int inside = pid - first * tiles_n;  // of this expert's mine * tiles_n tiles
+    const int at = (inside % mine) * BM;
+    tile_n = inside / mine;
+    m0 = (int64_t)p.m_indptr[expert] + at;
+    rows_valid = min(BM, rows - at);
+    return true;
+}
+
+// One output at element `to` of C.
+__device__ __forceinline__ void put1(const Int8GemmParams& p, int64_t to, float y) {
+    if (p.out_type == OUT_BF16) ((__bf16*)p.C)[to] = (__bf16)y;
+    else if (p.out_type == OUT_F16) ((_Float16*)p.C)[to] = (_Float16)y;
+    else ((float*)p.C)[to] = y;
+}
+
+__device__ __forceinline__ v4i lo4(v8i v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3); }
+__device__ __forceinline__ v4i hi4(v8i v) { return __builtin_shufflevector(v, v, 4, 5, 6, 7); }
+
+// Scales and biases of the eight columns from `col` on, a multiple of eight (vec_store).
+struct ColumnFactors {
+    float s[8], b[8];
+    __device__ __forceinline__ void load(const Int8GemmParams& p, const float* sb, int col) {
+        if (p.sb_step) {
+            const v4f x = *reinterpret_cast<const v4f*>(sb + col), y = *reinterpret_cast<const v4f*>(sb + col + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] = x[i], s[4 + i] = y[i];
+        } else {
+            const float x = *sb;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] = x;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b[i] = 0.f;
+        if (!p.bias) return;
+        if (p.bias_type == OUT_F32) {
+            const v4f x = *reinterpret_cast<const v4f*>((const float*)p.bias + col), y = *reinterpret_cast<const v4f*>((const float*)p.bias + col + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) b[i] = x[i], b[4 + i] = y[i];
+        } else {
+            typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+            typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+            const u16x8 x = *reinterpret_cast<const u16x8*>((const uint16_t*)p.bias + col);
+            const f16x8 h = __builtin_bit_cast(f16x8, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) b[i] = p.bias_type == OUT_BF16 ? __uint_as_float((uint32_t)x[i] << 16) : (float)h[i];
+        }
+    }
+};
+
 }  // namespace tg

@@ -32,20 +32,17 @@ __global__ void __launch_bounds__(256) int8_gemm_simple_kernel(const Int8GemmPar
     __shared__ __align__(16) int8_t sA[2][64 * kPitch], sB[2][64 * kPitch];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int tiles_n = (p.N + 63) / 64, row_tile = blockIdx.x / tiles_n, n0 = blockIdx.x % tiles_n * 64;
-    int64_t m0 = (int64_t)row_tile * 64, m_end = p.M;
-    int expert = 0;
+    const int tiles_n = (p.N + 63) / 64;
+    int expert = 0, n0 = blockIdx.x % tiles_n * 64, rows_valid;
+    int64_t m0 = (int64_t)(blockIdx.x / tiles_n) * 64;
     if constexpr (RAGGED) {
-        int tile = 0;
-        ragged_find(p.m_indptr, p.E, 64, lane, row_tile, expert, tile);
-        if (expert < 0) return;
-        expert = __builtin_amdgcn_readfirstlane(expert);
-        const int lo = p.m_indptr[expert];
-        if (lo < 0) return;
-        m0 = (int64_t)lo + (int64_t)__builtin_amdgcn_readfirstlane(tile) * 64;
-        m_end = min(p.m_indptr[expert + 1], p.M);
+        int tile_n;
+        if (!ragged_tile<64, false>(p, (int)blockIdx.x, tiles_n, lane, expert, m0, rows_valid, tile_n)) return;
+        n0 = tile_n * 64;
+    } else {
+        rows_valid = (int)min((int64_t)64, p.M - m0);
     }
-    if (m0 >= m_end) return;
+    const int64_t m_end = m0 + rows_valid;
     const int row = tid >> 2, at = (tid & 3) * 16;  // what this thread fetches
     const bool has_a = m0 + row < m_end, has_b = n0 + row < p.N;
     const int8_t* a = p.A + (m0 + row) * (int64_t)p.K + at;
@@ -87,11 +84,7 @@ __global__ void __launch_bounds__(256) int8_gemm_simple_kernel(const Int8GemmPar
             for (int r = 0; r < 4; ++r) {
                 const int n = n0 + wn * 32 + tn * 16 + lg * 4 + r;
                 if (n >= p.N) continue;
-                const float y = finish(acc[tn][tm][r], sa, p.sb[((int64_t)expert * p.N + n) * p.sb_step], load_bias(p.bias, p.bias_type, n));
-                const int64_t to = m * p.ldc + n;
-                if (p.out_type == OUT_BF16) ((__bf16*)p.C)[to] = (__bf16)y;
-                else if (p.out_type == OUT_F16) ((_Float16*)p.C)[to] = (_Float16)y;
-                else ((float*)p.C)[to] = y;
+                put1(p, m * p.ldc + n, finish(acc[tn][tm][r], sa, p.sb[((int64_t)expert * p.N + n) * p.sb_step], load_bias(p.bias, p.bias_type, n)));
             }
     }
 #endif

@@ -1,0 +1,14 @@
+// Instantiation of the 256 x 256 int8 tiles.
+#include "int8_gemm_tile256.h"
+
+namespace tg {
+
+hipError_t run_int8_tile256(const Int8GemmParams& p, hipStream_t s) {
+    if (p.K % kKBlock != 0 || p.K < 2 * kKBlock || (int64_t)p.M * p.K >= ((int64_t)1 << 31) || (int64_t)p.N * p.K >= ((int64_t)1 << 31)) return hipErrorInvalidValue;
+    const int64_t tiles = (((int64_t)p.M + 255) / 256) * ((p.N + 255) / 256);
+    const int units = compute_units();
+    hipLaunchKernelGGL(int8_gemm_tile256_kernel, dim3((unsigned)(tiles < units ? tiles : units)), dim3(256), 0, s, p);
+    return hipGetLastError();
+}
+
+}  // namespace tg

@@ -202,8 +202,9 @@ struct Int8GemmParams {
     int sa_step, sb_step, bias_type, out_type;
     int M, N, K;
     int64_t ldc;
-    int vec_store;           // 16-byte stores of 8 outputs are aligned
+    int vec_store;           // outputs in vectors of 8 (N a multiple of 8), C, sb and bias 16-byte aligned
     int split_k, ksteps_per_split;  // steps of 128 bytes
+    int wave_rows;           // streaming: weight rows of a wave
     int* partials;           // (split_k, M, N)
     const int* m_indptr;     // ragged: (E + 1); else null
     int E;
@@ -211,6 +212,15 @@ struct Int8GemmParams {
 // any sizes and addresses
 int64_t int8_simple_threads(const Int8GemmParams& p);
 hipError_t run_int8_simple(const Int8GemmParams& p, hipStream_t s);
+// The others need K % 16 == 0 and A and B at 16-byte addresses.
+// up to 32 rows (ragged: any, 16 at a time); ksteps_per_split a multiple of 4
+hipError_t run_int8_stream(const Int8GemmParams& p, hipStream_t s);
+bool int8_ring_exists(int bm, int bn);
+hipError_t run_int8_ring(int bm, int bn, const Int8GemmParams& p, hipStream_t s);
+// K % 128 == 0, K >= 256, vec_store, A and B below 2 GiB, dense rows, unsplit
+hipError_t run_int8_tile256(const Int8GemmParams& p, hipStream_t s);
+// behind run_int8_stream or run_int8_ring with split_k > 1
+hipError_t run_int8_splitk_reduce(const Int8GemmParams& p, hipStream_t s);
 
 // A row's int8 codes and its scale (int8_quant.hip)
 struct Int8QuantParams {

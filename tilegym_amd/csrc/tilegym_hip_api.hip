@@ -2273,7 +2273,67 @@ static int32_t int8_operands(tg::Int8GemmParams& p, const tg_tensor* c, const tg
     p.out_type = out_type;
     p.M = (int)M, p.N = (int)N, p.K = (int)K, p.ldc = N, p.E = (int)E;
     p.split_k = 1;
-    p.vec_store = N % 8 == 0 && aligned16(c->ptr);
+    p.vec_store = N % 8 == 0 && aligned16(c->ptr) && aligned16(scale_b->ptr);
+    return TG_OK;
+}
+
+// What the direct loads of the fast kernels take.
+static bool int8_fast_layout(const tg::Int8GemmParams& p) {
+    return p.K % 16 == 0 && aligned16(reinterpret_cast<uint64_t>(p.A)) && aligned16(reinterpret_cast<uint64_t>(p.B));
+}
+
+// kernel 0 simple, 1 tiles, 3 streaming, as in cfg[]
+struct Int8Schedule { int kernel, bm, bn, split; };
+
+static bool int8_takes(const tg::Int8GemmParams& p, const Int8Schedule& s) {
+    if (s.kernel == 0) return true;
+    if (!int8_fast_layout(p)) return false;
+    if (s.kernel == 3) return (p.m_indptr || p.M <= 32) && s.bn >= 4 && s.bn <= 64 && s.bn % 4 == 0;
+    if (s.bm == 256 && s.bn == 256)
+        return !p.m_indptr && p.K % 128 == 0 && p.K >= 256 && p.vec_store && s.split == 1 && (int64_t)p.M * p.K < kOffsetLimit && (int64_t)p.N * p.K < kOffsetLimit;
+    return tg::int8_ring_exists(s.bm, s.bn);
+}
+
+static Int8Schedule choose_int8(const tg::Int8GemmParams& p, int64_t partial_bytes, const int32_t* cfg, int32_t ncfg) {
+    Int8Schedule s{0, -1, -1, 1};
+    const int want = cfg_get(cfg, ncfg, TG_CFG_KERNEL);
+    const int want_bm = cfg_get(cfg, ncfg, TG_CFG_BLOCK_M), want_bn = cfg_get(cfg, ncfg, TG_CFG_BLOCK_N), want_split = cfg_get(cfg, ncfg, TG_CFG_SPLIT_K);
+    const int64_t steps = cdiv(p.K, 128);
+    if (want == 0) return s;
+    if (want == 3 || want == 1) {
+        const Int8Schedule forced{want, want_bm, want == 3 && want_bn <= 0 ? 64 : want_bn, 1};
+        if (int8_takes(p, forced)) {
+            s = forced;
+            if (!p.m_indptr && want_split > 1 && !(s.bm == 256 && s.bn == 256)) s.split = pick_split(1, 1, want == 3 ? cdiv(steps, 4) : steps, 1, p.M, p.N, partial_bytes, want_split);
+            return s;
+        }
+    }
+    if (!int8_fast_layout(p)) return s;
+    const Int8Schedule tile{1, 256, 256, 1}, ring{1, 128, 128, 1}, stream{3, -1, 64, 1};
+    if (p.M <= 16 && !p.m_indptr) return stream;
+    return int8_takes(p, tile) && p.M > 1024 ? tile : ring;
+}
+
+static int32_t run_int8(tg::Int8GemmParams p, Int8Schedule s, const tg_tensor* workspace, const char* what, uint64_t hip_stream) {
+    hipStream_t stream = reinterpret_cast<hipStream_t>(hip_stream);
+    Schedule done{s.kernel, s.bm, s.bn, s.split, -1, -1, s.kernel == 1 && !(s.bm == 256 && s.bn == 256) ? 8 : -1};
+    const int64_t steps = cdiv(p.K, 128);
+    p.split_k = s.split;
+    p.ksteps_per_split = (int)(s.kernel == 3 ? cdiv(cdiv(steps, 4), s.split) * 4 : cdiv(steps, s.split));
+    if (s.split > 1) p.partials = reinterpret_cast<int*>(workspace->ptr);
+    hipError_t e;
+    if (s.kernel == 0) {
+        if (const int32_t rc = check_threads(tg::int8_simple_threads(p), what)) return rc;
+        e = tg::run_int8_simple(p, stream);
+    } else if (s.kernel == 3) {
+        p.wave_rows = s.bn / 4;
+        e = tg::run_int8_stream(p, stream);
+    } else {
+        e = s.bm == 256 && s.bn == 256 ? tg::run_int8_tile256(p, stream) : tg::run_int8_ring(s.bm, s.bn, p, stream);
+    }
+    if (e == hipSuccess && s.split > 1) e = tg::run_int8_splitk_reduce(p, stream);
+    if (e != hipSuccess) return fail(TG_ERR_LAUNCH, "%s launch failed: %s", what, hipGetErrorString(e));
+    remember(done);
     return TG_OK;
 }
 
@@ -2291,16 +2351,24 @@ int32_t tg_int8_gemm(const tg_tensor* c, const tg_tensor* a, const tg_tensor* b,
         if (bias->shape[0] != p.N) return fail(TG_ERR_INVALID, "bias must have %d elements, got %lld", p.N, (long long)bias->shape[0]);
         p.bias = reinterpret_cast<const void*>(bias->ptr);
     }
+    int64_t partial_bytes = 0;
+    if (workspace) {
+        if ((rc = check_tensor(workspace, "workspace", -1))) return rc;
+        if (!aligned16(workspace->ptr)) return fail(TG_ERR_INVALID, "workspace must be 16-byte aligned");
+        partial_bytes = numel(workspace) * elem_size(workspace->dtype);
+    }
     if (p.M == 0 || p.N == 0) return TG_OK;
-    if ((rc = check_threads(tg::int8_simple_threads(p), "int8_gemm"))) return rc;
+    if (bias && !aligned16(bias->ptr)) p.vec_store = 0;
+    const Int8Schedule s = choose_int8(p, partial_bytes, cfg, ncfg);
     DeviceGuard guard(device_id);
     if (!guard.ok) return fail(TG_ERR_DEVICE, "cannot use HIP device %d", device_id);
-    const hipError_t e = tg::run_int8_simple(p, reinterpret_cast<hipStream_t>(hip_stream));
-    if (e != hipSuccess) return fail(TG_ERR_LAUNCH, "int8_gemm launch failed: %s", hipGetErrorString(e));
-    return TG_OK;
+    return run_int8(p, s, workspace, "int8_gemm", hip_stream);
 }
 
-int64_t tg_int8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) { return 0; }
+int64_t tg_int8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    if (M <= 0 || N <= 0 || K <= 0 || M > 512) return 0;
+    return std::min<int64_t>(8 * M * N * 4, kAutoPartialBytes);
+}
 
 int32_t tg_int8_ragged_gemm(const tg_tensor* c, const tg_tensor* a, const tg_tensor* b, const tg_tensor* scale_a, const tg_tensor* scale_b,
                             const tg_tensor* m_indptr, const int32_t* cfg, int32_t ncfg, int32_t device_id, uint64_t hip_stream) {
@@ -2314,12 +2382,10 @@ int32_t tg_int8_ragged_gemm(const tg_tensor* c, const tg_tensor* a, const tg_ten
     if (E > INT32_MAX || m_indptr->shape[0] != E + 1) return fail(TG_ERR_INVALID, "m_indptr must have %lld elements, got %lld", (long long)(E + 1), (long long)m_indptr->shape[0]);
     if (p.M == 0 || p.N == 0 || E == 0) return TG_OK;
     p.m_indptr = reinterpret_cast<const int*>(m_indptr->ptr);
-    if ((rc = check_threads(tg::int8_simple_threads(p), "int8_ragged_gemm"))) return rc;
+    const Int8Schedule s = choose_int8(p, 0, cfg, ncfg);
     DeviceGuard guard(device_id);
     if (!guard.ok) return fail(TG_ERR_DEVICE, "cannot use HIP device %d", device_id);
-    const hipError_t e = tg::run_int8_simple(p, reinterpret_cast<hipStream_t>(hip_stream));
-    if (e != hipSuccess) return fail(TG_ERR_LAUNCH, "int8_ragged_gemm launch failed: %s", hipGetErrorString(e));
-    return TG_OK;
+    return run_int8(p, s, nullptr, "int8_ragged_gemm", hip_stream);
 }
 
 // place (tokens, copies): null, or where a token's copies go
