@@ -12,6 +12,20 @@ namespace tg {
 // 16-byte chunks l / 16 and l / 16 + 4 of row l % 16.
 __device__ __forceinline__ v4i mfma_i8(v4i w, v4i x, v4i acc) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(w, x, acc, 0, 0, 0); }
 
+// A 32x32x32 int8 MFMA: lane l holds 16 bytes of row l % 32, those of K half l / 32; a lane gets column l % 32 and, in register 4 g + j, row
+// 8 g + 4 (l / 32) + j.  It issues at the matrix pipe's full rate, where two waves on a SIMD get 0.71 and one gets 0.58 of it out of 16x16x64 ones
+// (registers only, zeros: 4966, 3531, 2900 TOP/s; normally distributed codes, at the power limit: 3507, 3175, 2879).
+typedef int v16i __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ v16i mfma_i8_32(v4i w, v4i x, v16i acc) { return __builtin_amdgcn_mfma_i32_32x32x32_i8(w, x, acc, 0, 0, 0); }
+// The weight row (of 32) that is row r of such an MFMA: bits 2 and 3 change places, so that registers 0 ... 7 and 8 ... 15 of a lane are eight
+// consecutive columns of the output each, 8 (l / 32) and 16 + 8 (l / 32) on.
+__device__ __forceinline__ int weight_row_32(int r) { return (r & 19) | ((r & 4) << 1) | ((r & 8) >> 1); }
+
+// Chunk swizzle of a slab whose fragments are read 32 rows at a time: 16-byte chunk j of row r sits at position j ^ swz32(r).  A 16-byte read serves lanes
+// 0 - 3, 12 - 15 and 20 - 27 of each half wave together, then the others: the rows of one parity among them, which share 32 of the 64 banks, differ in
+// bits 1 to 3.
+__device__ __forceinline__ int swz32(int r) { return (r >> 1) & 7; }
+
 // One output from its integer sum.  Three roundings at most beside the store's: the sum's conversion (exact to 2^24), the product with the
 // token's scale, and one multiply-add with the channel's scale and the bias.
 __device__ __forceinline__ float finish(int sum, float sa, float sb, float bias) { return __builtin_fmaf((float)sum * sa, sb, bias); }
@@ -70,6 +84,31 @@ __device__ __forceinline__ bool ragged_tile(const Int8GemmParams& p, int bid, in
     return true;
 }
 
+// Stores of eight outputs at byte offsets from a tile's first row; those from kBeyond on are left out.
+constexpr uint32_t kBeyond = 0x80000000u;
+struct StoreTile {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __amdgpu_buffer_rsrc_t rsrc;
+    __device__ __forceinline__ StoreTile(void* base, int64_t offset) : rsrc(__builtin_amdgcn_make_buffer_rsrc((char*)base + offset, 0, 0x7FFFFFFF, 0x00020000)) {}
+    template <int OT>
+    __device__ __forceinline__ void put8(uint32_t at, v4f lo, v4f hi) const {
+        typedef float v8f __attribute__((ext_vector_type(8)));
+        typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+        const v8f v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        if constexpr (OT == OUT_F32) {
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, lo), rsrc, at, 0, 0);
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, hi), rsrc, at | 16, 0, 0);
+        } else if constexpr (OT == OUT_BF16) {
+            typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, __builtin_convertvector(v, bf16x8)), rsrc, at, 0, 0);
+        } else {
+            typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, __builtin_convertvector(v, f16x8)), rsrc, at, 0, 0);
+        }
+    }
+#endif
+};
+
 // One output at element `to` of C.
 __device__ __forceinline__ void put1(const Int8GemmParams& p, int64_t to, float y) {
     if (p.out_type == OUT_BF16) ((__bf16*)p.C)[to] = (__bf16)y;
@@ -80,9 +119,46 @@ __device__ __forceinline__ void put1(const Int8GemmParams& p, int64_t to, float 
 __device__ __forceinline__ v4i lo4(v8i v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3); }
 __device__ __forceinline__ v4i hi4(v8i v) { return __builtin_shufflevector(v, v, 4, 5, 6, 7); }
 
-// Scales and biases of the eight columns from `col` on, a multiple of eight (vec_store).
+// Scales and biases of the eight columns from `col` on, a multiple of eight (vec_store), without branches (StoreTile's reason).
+enum BiasKind { BIAS_NONE = 0, BIAS_F32 = 1, BIAS_16 = 2 };
+inline int bias_kind(const Int8GemmParams& p) { return !p.bias ? BIAS_NONE : p.bias_type == OUT_F32 ? BIAS_F32 : BIAS_16; }
+template <int BIAS>
 struct ColumnFactors {
+#if defined(__HIP_DEVICE_COMPILE__)
+    float s[8], b[BIAS ? 8 : 1];
+    // the output in column i of them from its integer sum
+    __device__ __forceinline__ float finished(int sum, float sa, int i) const { return finish(sum, sa, s[i], BIAS ? b[BIAS ? i : 0] : 0.f); }
+    __device__ __forceinline__ void load(const Int8GemmParams& p, const float* sb, int col) {
+        typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+        // one scale for all columns: the others lie beyond the range and come as zeros
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)sb, 0, p.sb_step ? 0x7FFFFFFF : 4, 0x00020000);
+        const uint32_t at = (uint32_t)(col * p.sb_step) * 4u;
+        const v4f x = __builtin_bit_cast(v4f, (v4u)__builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0)), y = __builtin_bit_cast(v4f, (v4u)__builtin_amdgcn_raw_buffer_load_b128(rsrc, at + 16, 0, 0));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            s[i] = p.sb_step ? x[i] : x[0];
+            s[4 + i] = p.sb_step ? y[i] : x[0];
+        }
+        if constexpr (BIAS == BIAS_F32) {
+            const v4f u = *reinterpret_cast<const v4f*>((const float*)p.bias + col), v = *reinterpret_cast<const v4f*>((const float*)p.bias + col + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) b[i] = u[i], b[4 + i] = v[i];
+        } else if constexpr (BIAS == BIAS_16) {
+            typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+            typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+            const u16x8 u = *reinterpret_cast<const u16x8*>((const uint16_t*)p.bias + col);
+            const f16x8 h = __builtin_bit_cast(f16x8, u);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) b[i] = p.bias_type == OUT_BF16 ? __uint_as_float((uint32_t)u[i] << 16) : (float)h[i];
+        }
+    }
+#endif
+};
+
+// The same with the kinds of bias told apart as they come, for kernels that have registers to spare.
+struct AnyColumnFactors {
     float s[8], b[8];
+    __device__ __forceinline__ float finished(int sum, float sa, int i) const { return finish(sum, sa, s[i], b[i]); }
     __device__ __forceinline__ void load(const Int8GemmParams& p, const float* sb, int col) {
         if (p.sb_step) {
             const v4f x = *reinterpret_cast<const v4f*>(sb + col), y = *reinterpret_cast<const v4f*>(sb + col + 4);

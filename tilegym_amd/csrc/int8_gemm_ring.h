@@ -3,7 +3,7 @@
 //
 // One workgroup per compute unit: four waves compute (2 x 2), four waves only request the next K steps' slabs by direct global->LDS loads; one
 // barrier per step, in front of its last column tiles.  The reasons stand in fp8_gemm_tile_ring.h.  What differs:
-//   * a K step of 128 bytes is two MFMAs of 64 per output; the two are issued a row group apart, so that none waits for the other;
+//   * the MFMAs are 32x32x32 ones, four to a K step of 128 bytes and output, or in tiles whose steps are loads rather than MFMAs two 16x16x64 ones;
 //   * a tile's descriptors start at its own first rows, so that operands may be of any size and a ragged tile's rows anywhere;
 //   * K is any multiple of 16: chunks of the last step behind a row's end are requested from beyond the descriptor's range, which makes them
 //     zeros in LDS;
@@ -14,18 +14,187 @@
 
 namespace tg {
 
+#define TG_FENCE() __builtin_amdgcn_sched_barrier(0)
+
+// A computing wave's part of a step: which MFMA, how its fragments lie in LDS, in which order they are multiplied and refilled, and which outputs an
+// accumulator register is.  Rows and columns of the part: 16 x 16 or 32 x 32 to an MFMA.
+
+// 16x16x64 MFMAs, two to a step and output: tiles of 32 rows or of up to 64 x 64, whose steps are loads, not MFMAs.
+template <int TM, int TN>
+struct Mma16 {
+    static constexpr int SIDE = 16, VECS = TN / 2;  // vectors of eight columns that a lane has of a row
+    static constexpr int WS = 4, LAST = TN == 4 ? 2 : 1;  // weight fragment sets, column tiles behind the barrier
+    static_assert(TN == 2 || TN == 4, "column tiles");
+    v4i acc[TN][TM];
+    v8i af[TM], wf[WS];
+    uint32_t frag0, wfrag0;
+    int li, lg;
+    __device__ __forceinline__ void init(int lane, int row0, int col0, int b_base) {
+        li = lane & 15, lg = lane >> 4;
+        frag0 = (row0 + li) * kKBlock + ((lg ^ swz16(li)) << 4);
+        const int wrow = ((li >> 2) << 3) | (li & 3);
+        wfrag0 = b_base + (col0 + wrow) * kKBlock + ((lg ^ swz_w(wrow)) << 4);
+#pragma unroll
+        for (int tn = 0; tn < TN; ++tn)
+#pragma unroll
+            for (int tm = 0; tm < TM; ++tm) acc[tn][tm] = v4i{0, 0, 0, 0};
+    }
+    static __device__ __forceinline__ int a_swizzle(int r) { return swz16(r); }
+    static __device__ __forceinline__ int b_swizzle(int r) { return swz_w(r); }
+    template <int WGM>
+    __device__ __forceinline__ void read_a(int tm, const uint8_t* base) {
+        const uint8_t* a = base + tm * (WGM * 16 * kKBlock);
+        af[tm] = join(*reinterpret_cast<const v4i*>(a + frag0), *reinterpret_cast<const v4i*>(a + (frag0 ^ 64)));
+    }
+    __device__ __forceinline__ void read_w(int tn, const uint8_t* base) {
+        const uint8_t* b = base + ((tn >> 1) * 32 + (tn & 1) * 4) * kKBlock;
+        wf[tn % WS] = join(*reinterpret_cast<const v4i*>(b + wfrag0), *reinterpret_cast<const v4i*>(b + (wfrag0 ^ 64)));
+    }
+    template <int WGM>
+    __device__ __forceinline__ void first(const uint8_t* base) {
+        read_w(0, base);
+        read_w(1, base);
+#pragma unroll
+        for (int tm = 0; tm < TM; ++tm) read_a<WGM>(tm, base);
+    }
+    // column tile by column tile: all row groups' first halves, then the second ones
+    __device__ __forceinline__ void before(const uint8_t* cur) {
+#pragma unroll
+        for (int tn = 0; tn < TN - LAST; ++tn) {
+#pragma unroll
+            for (int tm = 0; tm < TM; ++tm) {
+                acc[tn][tm] = mfma_i8(lo4(wf[tn % WS]), lo4(af[tm]), acc[tn][tm]);
+                if (tm == 0 && tn + 2 < TN) read_w(tn + 2, cur);
+                TG_FENCE();
+            }
+#pragma unroll
+            for (int tm = 0; tm < TM; ++tm) acc[tn][tm] = mfma_i8(hi4(wf[tn % WS]), hi4(af[tm]), acc[tn][tm]);
+            TG_FENCE();
+        }
+    }
+    // row group by row group: the last MFMA of one releases its fragment
+    template <int WGM>
+    __device__ __forceinline__ void behind(const uint8_t* nxt) {
+        read_w(0, nxt);
+        if constexpr (TN > 2) read_w(1, nxt);
+        TG_FENCE();
+#pragma unroll
+        for (int tm = 0; tm < TM; ++tm) {
+#pragma unroll
+            for (int tn = TN - LAST; tn < TN; ++tn) acc[tn][tm] = mfma_i8(lo4(wf[tn % WS]), lo4(af[tm]), acc[tn][tm]);
+#pragma unroll
+            for (int tn = TN - LAST; tn < TN; ++tn) acc[tn][tm] = mfma_i8(hi4(wf[tn % WS]), hi4(af[tm]), acc[tn][tm]);
+            TG_FENCE();
+            read_a<WGM>(tm, nxt);
+            TG_FENCE();
+        }
+        if constexpr (TN == 2) read_w(1, nxt);  // (its registers were the last MFMAs')
+    }
+    __device__ __forceinline__ void keep() {  // (the reads for the step behind the last one)
+#pragma unroll
+        for (int tm = 0; tm < TM; ++tm) asm volatile("" : : "v"(af[tm]));
+        asm volatile("" : : "v"(wf[0]), "v"(wf[1]));
+    }
+    __device__ __forceinline__ int row() const { return li; }
+    __device__ __forceinline__ int column(int v) const { return v * 32 + lg * 8; }
+    __device__ __forceinline__ int get(int v, int tm, int i) const { return acc[2 * v + (i >> 2)][tm][i & 3]; }
+};
+
+// 32x32x32 MFMAs, four to a step and output.
+template <int TM, int TN>
+struct Mma32 {
+    static constexpr int SIDE = 32, VECS = 2 * TN;
+    static_assert(TN == 2 || TN == 3, "column tiles");
+    v16i acc[TN][TM];
+    v4i af[TM][4], wf[2][4];
+    uint32_t frag[4], wfrag[4];
+    int li, half;
+    __device__ __forceinline__ void init(int lane, int row0, int col0, int b_base) {
+        li = lane & 31, half = lane >> 5;
+        const int wrow = weight_row_32(li);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            frag[q] = (row0 + li) * kKBlock + (((2 * q + half) ^ swz32(li)) << 4);
+            wfrag[q] = b_base + (col0 + wrow) * kKBlock + (((2 * q + half) ^ swz32(wrow)) << 4);
+        }
+#pragma unroll
+        for (int tn = 0; tn < TN; ++tn)
+#pragma unroll
+            for (int tm = 0; tm < TM; ++tm) acc[tn][tm] = 0;
+    }
+    static __device__ __forceinline__ int a_swizzle(int r) { return swz32(r); }
+    static __device__ __forceinline__ int b_swizzle(int r) { return swz32(r); }
+    template <int WGM>
+    __device__ __forceinline__ void read_a(int tm, int q, const uint8_t* base) { af[tm][q] = *reinterpret_cast<const v4i*>(base + tm * (WGM * 32 * kKBlock) + frag[q]); }
+    __device__ __forceinline__ void read_w(int set, int tn, int q, const uint8_t* base) { wf[set][q] = *reinterpret_cast<const v4i*>(base + tn * (32 * kKBlock) + wfrag[q]); }
+    template <int WGM>
+    __device__ __forceinline__ void first(const uint8_t* base) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            read_w(0, 0, q, base);
+#pragma unroll
+            for (int tm = 0; tm < TM; ++tm) read_a<WGM>(tm, q, base);
+        }
+    }
+    __device__ __forceinline__ void before(const uint8_t* cur) {
+#pragma unroll
+        for (int tn = 0; tn < TN - 1; ++tn)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+#pragma unroll
+                for (int tm = 0; tm < TM; ++tm) {
+                    acc[tn][tm] = mfma_i8_32(wf[tn & 1][q], af[tm][q], acc[tn][tm]);
+                    if (tm == 0) read_w((tn + 1) & 1, tn + 1, q, cur);
+                    TG_FENCE();
+                }
+            }
+    }
+    // quarter by quarter of the step: its MFMAs release the row groups' pieces, and with three column tiles the weight's
+    template <int WGM>
+    __device__ __forceinline__ void behind(const uint8_t* nxt) {
+        constexpr int set = (TN - 1) & 1;
+        if constexpr (set == 1) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) read_w(0, 0, q, nxt);
+            TG_FENCE();
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+#pragma unroll
+            for (int tm = 0; tm < TM; ++tm) acc[TN - 1][tm] = mfma_i8_32(wf[set][q], af[tm][q], acc[TN - 1][tm]);
+            TG_FENCE();
+            if constexpr (set == 0) read_w(0, 0, q, nxt);
+#pragma unroll
+            for (int tm = 0; tm < TM; ++tm) read_a<WGM>(tm, q, nxt);
+            TG_FENCE();
+        }
+    }
+    __device__ __forceinline__ void keep() {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+#pragma unroll
+            for (int tm = 0; tm < TM; ++tm) asm volatile("" : : "v"(af[tm][q]));
+            asm volatile("" : : "v"(wf[0][q]));
+        }
+    }
+    __device__ __forceinline__ int row() const { return li; }
+    __device__ __forceinline__ int column(int v) const { return v * 16 + half * 8; }
+    __device__ __forceinline__ int get(int v, int tm, int i) const { return acc[v >> 1][tm][8 * (v & 1) + i]; }
+};
+
 template <int BM, int BN, int STAGES, bool SPLIT, bool RAGGED>
 __global__ void __launch_bounds__(512, 1) int8_gemm_ring_kernel(const Int8GemmParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    constexpr int NL = 4, WGN = BN == 32 ? 1 : 2, WGM = 4 / WGN;
+    constexpr bool WIDE = BM >= 64 && BN >= 128;
+    constexpr int NL = 4, WGN = BN == 32 ? 1 : 2, WGM = 4 / WGN, SIDE = WIDE ? 32 : 16;
     constexpr int WTN = BN / WGN;
-    constexpr int TM = BM / (16 * WGM), TN = WTN / 16;
+    constexpr int TM = BM / (SIDE * WGM), TN = WTN / SIDE;
+    using Mma = std::conditional_t<WIDE, Mma32<TM, WIDE ? TN : 2>, Mma16<TM, WIDE ? 2 : TN>>;
+    constexpr int VECS = Mma::VECS;
     constexpr int A_IT = BM / (8 * NL), B_IT = BN / (8 * NL);
     constexpr int STAGE_BYTES = (BM + BN) * kKBlock;
     constexpr int PER_STEP = A_IT + B_IT;
-    constexpr int WS = TN == 6 ? 3 : 4;                 // weight fragment sets
-    constexpr int LAST = TN == 4 ? 2 : 1;               // column tiles behind the barrier
-    static_assert(BM % (16 * WGM) == 0 && (TN == 2 || TN == 4 || TN == 6) && STAGES >= 3 && STAGES * STAGE_BYTES <= 160 * 1024, "shape");
+    static_assert(BM % (SIDE * WGM) == 0 && STAGES >= 3 && STAGES * STAGE_BYTES <= 160 * 1024, "shape");
     static_assert(!(SPLIT && RAGGED), "K is split for dense rows only");
 
     __shared__ __align__(1024) uint8_t lds[STAGES * STAGE_BYTES];  // stage s: A slab, then B slab
@@ -65,14 +234,13 @@ __global__ void __launch_bounds__(512, 1) int8_gemm_ring_kernel(const Int8GemmPa
     constexpr int kWaitLoop = 0x0F70 | (kLoop & 15) | ((kLoop >> 4) << 14);
     constexpr int kWaitAll = 0x0F70;
     constexpr int kWaitLds = 0xC07F;
-#define TG_FENCE() __builtin_amdgcn_sched_barrier(0)
 
     if (wave >= 4) {
         // ------------------------------------------------------------ loading waves
         const int lw = wave - 4;
         const int lrow = lane >> 3;
-        const int lj = (lane & 7) ^ swz16(lrow);
-        const int ljb = (lane & 7) ^ swz_w(((lw & 1) << 3) | lrow);
+        const int lj = (lane & 7) ^ Mma::a_swizzle(((lw & 1) << 3) | lrow);
+        const int ljb = (lane & 7) ^ Mma::b_swizzle(((lw & 1) << 3) | lrow);
         constexpr uint32_t kOutOfRange = 0x80000000u;  // beyond the descriptor's 2^31 - 1 bytes
         uint32_t a_off[A_IT], b_off[B_IT];
 #pragma unroll
@@ -114,98 +282,51 @@ __global__ void __launch_bounds__(512, 1) int8_gemm_ring_kernel(const Int8GemmPa
 
     // ---------------------------------------------------------------- computing waves
     const int wm = wave % WGM, wn = wave / WGM;
-    const int li = lane & 15, lg = lane >> 4;
-    const uint32_t frag0 = wm * 16 * kKBlock + li * kKBlock + ((lg ^ swz16(li)) << 4), frag1 = frag0 ^ 64;
-    const int wrow = ((li >> 2) << 3) | (li & 3);
-    const uint32_t wfrag0 = BM * kKBlock + wn * WTN * kKBlock + wrow * kKBlock + ((lg ^ swz_w(wrow)) << 4), wfrag1 = wfrag0 ^ 64;
+    Mma mma;
+    mma.init(lane, wm * SIDE, wn * WTN, BM * kKBlock);
+    const int li = mma.row();
 
-    v4i acc[TN][TM];
-#pragma unroll
-    for (int tn = 0; tn < TN; ++tn)
-#pragma unroll
-        for (int tm = 0; tm < TM; ++tm) acc[tn][tm] = v4i{0, 0, 0, 0};
-
-    // the scales and biases of this lane's rows and columns, asked for in front of the K loop where there are registers for them
+    // the scales of this lane's rows, asked for in front of the K loop
     const float* sb = p.sb + (int64_t)expert * p.N * p.sb_step;
     float srow[TM];
 #pragma unroll
-    for (int tm = 0; tm < TM; ++tm) srow[tm] = p.sa[(m0 + min((tm * WGM + wm) * 16 + li, rows_valid - 1)) * p.sa_step];
+    for (int tm = 0; tm < TM; ++tm) srow[tm] = p.sa[(m0 + min((tm * WGM + wm) * SIDE + li, rows_valid - 1)) * p.sa_step];
 
-    v8i af[TM], wf[WS];
-    auto read_a = [&](int tm, const uint8_t* base) {
-        const uint8_t* a = base + tm * (WGM * 16 * kKBlock);
-        af[tm] = join(*reinterpret_cast<const v4i*>(a + frag0), *reinterpret_cast<const v4i*>(a + frag1));
-    };
-    auto read_w = [&](int tn, const uint8_t* base) {
-        const uint8_t* b = base + ((tn >> 1) * 32 + (tn & 1) * 4) * kKBlock;
-        wf[tn % WS] = join(*reinterpret_cast<const v4i*>(b + wfrag0), *reinterpret_cast<const v4i*>(b + wfrag1));
-    };
     __builtin_amdgcn_s_barrier();  // step 0 has landed
-    read_w(0, lds);
-    read_w(1, lds);
-#pragma unroll
-    for (int tm = 0; tm < TM; ++tm) read_a(tm, lds);
+    mma.template first<WGM>(lds);
     int stage = 0;
     for (int k = 0; k < nsteps; ++k) {
         const uint8_t* cur = lds + stage * STAGE_BYTES;
         stage = stage == STAGES - 1 ? 0 : stage + 1;
         const uint8_t* nxt = lds + stage * STAGE_BYTES;
         TG_FENCE();
-        // in front of the barrier column tile by column tile: all row groups' first halves, then the second ones
-#pragma unroll
-        for (int tn = 0; tn < TN - LAST; ++tn) {
-#pragma unroll
-            for (int tm = 0; tm < TM; ++tm) {
-                acc[tn][tm] = mfma_i8(lo4(wf[tn % WS]), lo4(af[tm]), acc[tn][tm]);
-                if (tm == 0 && tn + 2 < TN) read_w(tn + 2, cur);
-                TG_FENCE();
-            }
-#pragma unroll
-            for (int tm = 0; tm < TM; ++tm) acc[tn][tm] = mfma_i8(hi4(wf[tn % WS]), hi4(af[tm]), acc[tn][tm]);
-            TG_FENCE();
-        }
+        mma.before(cur);
         __builtin_amdgcn_s_waitcnt(kWaitLds);  // all my reads of step k are done
         __builtin_amdgcn_s_barrier();          // step k+1 is visible
         TG_FENCE();
-        read_w(0, nxt);
-        if constexpr (TN > 2) read_w(1, nxt);
-        TG_FENCE();
-        // behind it row group by row group: the last MFMA of one releases its fragment
-#pragma unroll
-        for (int tm = 0; tm < TM; ++tm) {
-#pragma unroll
-            for (int tn = TN - LAST; tn < TN; ++tn) acc[tn][tm] = mfma_i8(lo4(wf[tn % WS]), lo4(af[tm]), acc[tn][tm]);
-#pragma unroll
-            for (int tn = TN - LAST; tn < TN; ++tn) acc[tn][tm] = mfma_i8(hi4(wf[tn % WS]), hi4(af[tm]), acc[tn][tm]);
-            TG_FENCE();
-            read_a(tm, nxt);
-            TG_FENCE();
-        }
-        if constexpr (TN == 2) read_w(1, nxt);  // (its registers were the last MFMAs')
+        mma.template behind<WGM>(nxt);
     }
-#pragma unroll
-    for (int tm = 0; tm < TM; ++tm) asm volatile("" : : "v"(af[tm]));
-    asm volatile("" : : "v"(wf[0]), "v"(wf[1]));
-#undef TG_FENCE
+    mma.keep();
 
-    const int col0 = n0 + wn * WTN + lg * 8;
+    const int col0 = n0 + wn * WTN;
     if constexpr (SPLIT) {
         int* mine = p.partials + (int64_t)blockIdx.y * p.M * p.N;
 #pragma unroll
         for (int tm = 0; tm < TM; ++tm) {
-            const int rt = (tm * WGM + wm) * 16 + li;
+            const int rt = (tm * WGM + wm) * SIDE + li;
             if (rt >= rows_valid) continue;
-            const int64_t at = (m0 + rt) * p.N + col0;
 #pragma unroll
-            for (int tp = 0; tp < TN / 2; ++tp) {
+            for (int v = 0; v < VECS; ++v) {
+                const int col = col0 + mma.column(v);
+                int* to = mine + (m0 + rt) * p.N + col;
                 if (p.N % 8 == 0) {
-                    if (col0 + tp * 32 >= p.N) continue;
-                    *reinterpret_cast<v4i*>(mine + at + tp * 32) = acc[2 * tp][tm];
-                    *reinterpret_cast<v4i*>(mine + at + tp * 32 + 4) = acc[2 * tp + 1][tm];
+                    if (col >= p.N) continue;
+                    *reinterpret_cast<v4i*>(to) = v4i{mma.get(v, tm, 0), mma.get(v, tm, 1), mma.get(v, tm, 2), mma.get(v, tm, 3)};
+                    *reinterpret_cast<v4i*>(to + 4) = v4i{mma.get(v, tm, 4), mma.get(v, tm, 5), mma.get(v, tm, 6), mma.get(v, tm, 7)};
                 } else {
 #pragma unroll
-                    for (int q = 0; q < 8; ++q)
-                        if (col0 + tp * 32 + q < p.N) mine[at + tp * 32 + q] = acc[2 * tp + (q >> 2)][tm][q & 3];
+                    for (int i = 0; i < 8; ++i)
+                        if (col + i < p.N) to[i] = mma.get(v, tm, i);
                 }
             }
         }
@@ -213,23 +334,28 @@ __global__ void __launch_bounds__(512, 1) int8_gemm_ring_kernel(const Int8GemmPa
     }
     auto emit_whole = [&](auto type_tag) __attribute__((always_inline)) {
         constexpr int OT = decltype(type_tag)::value;
-        ColumnFactors f[TN / 2];
+        constexpr int FT = TM * VECS > 16 ? 2 : VECS;  // vectors whose factors are in registers at a time
 #pragma unroll
-        for (int tp = 0; tp < TN / 2; ++tp) f[tp].load(p, sb, min(col0 + tp * 32, p.N - 8));
+        for (int v0 = 0; v0 < VECS; v0 += FT) {
+            AnyColumnFactors f[FT];
 #pragma unroll
-        for (int tm = 0; tm < TM; ++tm) {
-            const int rt = (tm * WGM + wm) * 16 + li;
-            if (rt >= rows_valid) continue;
+            for (int v = 0; v < FT; ++v) f[v].load(p, sb, min(col0 + mma.column(v0 + v), p.N - 8));
 #pragma unroll
-            for (int tp = 0; tp < TN / 2; ++tp) {
-                if (col0 + tp * 32 >= p.N) continue;
-                v4f x, y;
+            for (int tm = 0; tm < TM; ++tm) {
+                const int rt = (tm * WGM + wm) * SIDE + li;
+                if (rt >= rows_valid) continue;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    x[r] = finish(acc[2 * tp][tm][r], srow[tm], f[tp].s[r], f[tp].b[r]);
-                    y[r] = finish(acc[2 * tp + 1][tm][r], srow[tm], f[tp].s[4 + r], f[tp].b[4 + r]);
+                for (int v = 0; v < FT; ++v) {
+                    const int col = col0 + mma.column(v0 + v);
+                    if (col >= p.N) continue;
+                    v4f x, y;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        x[r] = f[v].finished(mma.get(v0 + v, tm, r), srow[tm], r);
+                        y[r] = f[v].finished(mma.get(v0 + v, tm, 4 + r), srow[tm], 4 + r);
+                    }
+                    put8<OT>(p.C, (m0 + rt) * p.ldc + col, x, y);
                 }
-                put8<OT>(p.C, (m0 + rt) * p.ldc + col0 + tp * 32, x, y);
             }
         }
     };
@@ -241,16 +367,16 @@ __global__ void __launch_bounds__(512, 1) int8_gemm_ring_kernel(const Int8GemmPa
     }
     // rows of outputs that are no whole vectors: element by element
 #pragma unroll
-    for (int tp = 0; tp < TN / 2; ++tp)
+    for (int v = 0; v < VECS; ++v)
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            const int col = col0 + tp * 32 + q;
+        for (int i = 0; i < 8; ++i) {
+            const int col = col0 + mma.column(v) + i;
             if (col >= p.N) continue;
             const float s = sb[(int64_t)col * p.sb_step], b = load_bias(p.bias, p.bias_type, col);
 #pragma unroll
             for (int tm = 0; tm < TM; ++tm) {
-                const int rt = (tm * WGM + wm) * 16 + li;
-                if (rt < rows_valid) put1(p, (m0 + rt) * p.ldc + col, finish(acc[2 * tp + (q >> 2)][tm][q & 3], srow[tm], s, b));
+                const int rt = (tm * WGM + wm) * SIDE + li;
+                if (rt < rows_valid) put1(p, (m0 + rt) * p.ldc + col, finish(mma.get(v, tm, i), srow[tm], s, b));
             }
         }
 #endif
@@ -268,5 +394,7 @@ inline hipError_t launch_int8_ring(const Int8GemmParams& p, hipStream_t stream) 
     else hipLaunchKernelGGL((int8_gemm_ring_kernel<BM, BN, STAGES, false, false>), grid, block, 0, stream, p);
     return hipGetLastError();
 }
+
+#undef TG_FENCE
 
 }  // namespace tg

@@ -35,26 +35,20 @@ __global__ void __launch_bounds__(256) int8_splitk_reduce_kernel(const Int8GemmP
 
 }  // namespace
 
+// Stages: as many as 160 KiB hold, up to twelve.
+#define TG_RING_TILES(X) X(64, 32, 12) X(32, 64, 12) X(64, 64, 9) X(32, 128, 7) X(64, 128, 6) X(128, 128, 4) X(192, 128, 4) X(128, 192, 4) X(192, 192, 3) X(256, 128, 3)
+
 bool int8_ring_exists(int bm, int bn) {
-    return (bn == 128 && (bm == 32 || bm == 64 || bm == 96 || bm == 128 || bm == 160 || bm == 256)) || (bn == 192 && (bm == 160 || bm == 192)) ||
-           (bn == 64 && (bm == 32 || bm == 64)) || (bn == 32 && bm == 64);
+#define TG_IS(BM, BN, STAGES) || (bm == BM && bn == BN)
+    return false TG_RING_TILES(TG_IS);
+#undef TG_IS
 }
 
 hipError_t run_int8_ring(int bm, int bn, const Int8GemmParams& p, hipStream_t s) {
     if (p.K % 16 != 0) return hipErrorInvalidValue;
 #define TG_CASE(BM, BN, STAGES) \
     if (bm == BM && bn == BN) return launch_int8_ring<BM, BN, STAGES>(p, s);
-    TG_CASE(64, 32, 12)
-    TG_CASE(32, 64, 12)
-    TG_CASE(64, 64, 9)
-    TG_CASE(32, 128, 7)
-    TG_CASE(64, 128, 5)
-    TG_CASE(96, 128, 4)
-    TG_CASE(128, 128, 4)
-    TG_CASE(160, 128, 4)
-    TG_CASE(160, 192, 3)
-    TG_CASE(192, 192, 3)
-    TG_CASE(256, 128, 3)
+    TG_RING_TILES(TG_CASE)
 #undef TG_CASE
     return hipErrorInvalidConfiguration;
 }

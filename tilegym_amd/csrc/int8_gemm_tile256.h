@@ -3,8 +3,8 @@
 //
 // Four waves, one per SIMD, each with a 128 x 128 part of the tile, one workgroup per compute unit that walks tiles b, b + grid, ... of the rastered
 // sequence; two activation slabs and three weight slabs (160 KiB, all of LDS); requests two steps ahead, running on into the next tile; one barrier per
-// step in front of its last sixteen outputs.  The reasons stand in fp8_gemm_tile256.h.  What differs: a K step of 128 bytes is two MFMAs of 64 per
-// output, issued four outputs apart so that none waits for the other, and the epilogue has a scale per row and per column and a bias.
+// step in front of its last sixteen MFMAs.  The reasons stand in fp8_gemm_tile256.h.  What differs: 32x32x32 MFMAs, four to a K step and output tile, and an
+// epilogue with a scale per row and per column and a bias.
 // K must be a multiple of 128 and at least 256, the operands below 2 GiB each, the outputs in whole vectors (vec_store).
 #pragma once
 
@@ -12,15 +12,26 @@
 
 namespace tg {
 
+// One element of an accumulator, out of the accumulation register it is in: left to itself the compiler copies whole accumulators out of them at the end
+// of the K loop, more than the other registers hold.  The caller sees to the wait states behind the MFMA that wrote it.
+__device__ __forceinline__ int read_acc(int x) {
+    int y;
+    asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(y) : "a"(x));
+    return y;
+}
+
+// A kernel per output type and kind of bias: with all in one the compiler reads every
+// accumulator out in front of the choice, spills, and waits for the reload in every K step (855 -> 1006 us).
+template <int OT, int BIAS>
 __global__ void __launch_bounds__(256, 1) int8_gemm_tile256_kernel(const Int8GemmParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int BM = 256, BN = 256, WGM = 2, WGN = 2, NW = 4;
     constexpr int WTN = BN / WGN;
-    constexpr int TM = 8, TN = WTN / 16;
+    constexpr int TM = 4, TN = WTN / 32;          // 4 row groups x 4 column tiles of 32 x 32 per wave
     constexpr int SLAB = 256 * kKBlock;
     constexpr int A_STAGES = 2, B_STAGES = 3;
     constexpr int IT = 256 / (8 * NW);
-    static_assert(TN == 8 && IT == 8, "schedule below is written for 8 x 8 MFMA tiles and 8 + 8 loads per wave");
+    static_assert(TN == 4 && IT == 8, "schedule below is written for 4 x 4 MFMA tiles and 8 + 8 loads per wave");
 
     __shared__ __align__(1024) uint8_t sA[A_STAGES * SLAB];
     __shared__ __align__(1024) uint8_t sB[B_STAGES * SLAB];
@@ -46,8 +57,7 @@ __global__ void __launch_bounds__(256, 1) int8_gemm_tile256_kernel(const Int8Gem
     const int nsteps = K / kKBlock, last = nsteps - 1;
 
     const int lrow = lane >> 3;
-    const int lj = (lane & 7) ^ swz16(lrow);
-    const int ljb = (lane & 7) ^ swz_w(((wave & 1) << 3) | lrow);
+    const int lj = (lane & 7) ^ swz32(((wave & 1) << 3) | lrow);
     uint32_t a_off[IT], b_off[IT];
     auto set_offsets = [&](int om0, int on0) {
         const int rv = min(BM, p.M - om0);
@@ -55,7 +65,7 @@ __global__ void __launch_bounds__(256, 1) int8_gemm_tile256_kernel(const Int8Gem
         for (int i = 0; i < IT; ++i) {
             const int r = (i * NW + wave) * 8 + lrow;
             a_off[i] = (uint32_t)(om0 + min(r, rv - 1)) * (uint32_t)K + lj * 16;
-            b_off[i] = (uint32_t)min(on0 + r, p.N - 1) * (uint32_t)K + ljb * 16;
+            b_off[i] = (uint32_t)min(on0 + r, p.N - 1) * (uint32_t)K + lj * 16;
         }
     };
     set_offsets(m0, n0);
@@ -68,24 +78,23 @@ __global__ void __launch_bounds__(256, 1) int8_gemm_tile256_kernel(const Int8Gem
         direct_load_b128_settled(rsrc_b, ldsB + stage * SLAB + i * NW * 1024, b_off[i], kstep * kKBlock);
     };
 
-    const int li = lane & 15, lg = lane >> 4;
-    const uint32_t frag0 = wm * 16 * kKBlock + li * kKBlock + ((lg ^ swz16(li)) << 4), frag1 = frag0 ^ 64;
-    const int wrow = ((li >> 2) << 3) | (li & 3);
-    const uint32_t wfrag0 = wn * WTN * kKBlock + wrow * kKBlock + ((lg ^ swz_w(wrow)) << 4), wfrag1 = wfrag0 ^ 64;
-    auto read_a = [&](int tm, const uint8_t* cA) {
-        const uint8_t* base = cA + tm * (WGM * 16 * kKBlock);
-        return join(*reinterpret_cast<const v4i*>(base + frag0), *reinterpret_cast<const v4i*>(base + frag1));
-    };
-    auto read_w = [&](int tn, const uint8_t* cB) {
-        const uint8_t* base = cB + ((tn >> 1) * 32 + (tn & 1) * 4) * kKBlock;
-        return join(*reinterpret_cast<const v4i*>(base + wfrag0), *reinterpret_cast<const v4i*>(base + wfrag1));
-    };
+    // chunk 2 q + half of a row is the lane's share of the K step's q-th 32 bytes
+    const int li = lane & 31, half = lane >> 5;
+    const int wrow = weight_row_32(li);
+    uint32_t frag[4], wfrag[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        frag[q] = (wm * 32 + li) * kKBlock + (((2 * q + half) ^ swz32(li)) << 4);
+        wfrag[q] = (wn * WTN + wrow) * kKBlock + (((2 * q + half) ^ swz32(wrow)) << 4);
+    }
+    auto read_a = [&](int tm, int q, const uint8_t* cA) { return *reinterpret_cast<const v4i*>(cA + tm * (WGM * 32 * kKBlock) + frag[q]); };
+    auto read_w = [&](int tn, int q, const uint8_t* cB) { return *reinterpret_cast<const v4i*>(cB + tn * (32 * kKBlock) + wfrag[q]); };
 
-    v4i acc[TN][TM];
+    v16i acc[TN][TM];
 #pragma unroll
     for (int tn = 0; tn < TN; ++tn)
 #pragma unroll
-        for (int tm = 0; tm < TM; ++tm) acc[tn][tm] = v4i{0, 0, 0, 0};
+        for (int tm = 0; tm < TM; ++tm) acc[tn][tm] = 0;
 
     constexpr int kWaitBut16 = 0x4F70 | 0, kWaitBut8 = 0x0F70 | 8, kWaitAll = 0x0F70;
     constexpr int kWaitLds = 0xC07F;
@@ -101,11 +110,13 @@ __global__ void __launch_bounds__(256, 1) int8_gemm_tile256_kernel(const Int8Gem
     for (int i = 0; i < IT; ++i) load_a(i, min(1, last), 1);
     __builtin_amdgcn_s_waitcnt(kWaitBut16);
     __builtin_amdgcn_s_barrier();
-    v8i af[TM], wf[4];
-    wf[0] = read_w(0, sB);
-    wf[1] = read_w(1, sB);
+    v4i af[TM][4], wf[2][4];
 #pragma unroll
-    for (int tm = 0; tm < TM; ++tm) af[tm] = read_a(tm, sA);
+    for (int q = 0; q < 4; ++q) {
+        wf[0][q] = read_w(0, q, sB);
+#pragma unroll
+        for (int tm = 0; tm < TM; ++tm) af[tm][q] = read_a(tm, q, sA);
+    }
 
     int sa = 0, sb = 0;
     for (;;) {
@@ -127,19 +138,17 @@ __global__ void __launch_bounds__(256, 1) int8_gemm_tile256_kernel(const Int8Gem
             const int sb2 = sb1 == B_STAGES - 1 ? 0 : sb1 + 1;
             const uint8_t* cB = sB + sb * SLAB;
             TG_FENCE();
-            // column tiles 0 .. 5 in halves of four outputs (eight MFMAs); behind each half of the first four a direct load, behind each first
-            // half the weight fragment of the column tile after next
+            // column tiles 0 .. 2 in groups of four MFMAs, one per row group; behind each of the first eight groups a direct load, behind every
+            // group a piece of the next column tile's weight fragment
 #pragma unroll
-            for (int tn = 0; tn < 6; ++tn) {
+            for (int tn = 0; tn < TN - 1; ++tn) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int q = 0; q < 4; ++q) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[tn][4 * h + j] = mfma_i8(lo4(wf[tn & 3]), lo4(af[4 * h + j]), acc[tn][4 * h + j]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[tn][4 * h + j] = mfma_i8(hi4(wf[tn & 3]), hi4(af[4 * h + j]), acc[tn][4 * h + j]);
+                    for (int tm = 0; tm < TM; ++tm) acc[tn][tm] = mfma_i8_32(wf[tn & 1][q], af[tm][q], acc[tn][tm]);
                     TG_FENCE();
-                    if (2 * tn + h < IT) load_b(2 * tn + h, k2, sb2);
-                    if (h == 0) wf[(tn + 2) & 3] = read_w(tn + 2, cB);
+                    if (4 * tn + q < IT) load_b(4 * tn + q, k2, sb2);
+                    wf[(tn + 1) & 1][q] = read_w(tn + 1, q, cB);
                     TG_FENCE();
                 }
             }
@@ -147,82 +156,91 @@ __global__ void __launch_bounds__(256, 1) int8_gemm_tile256_kernel(const Int8Gem
             __builtin_amdgcn_s_waitcnt(kWaitLds);
             __builtin_amdgcn_s_barrier();
             TG_FENCE();
+            // column tile 3: each MFMA releases a piece of an activation fragment, which is refilled from A(k+1) at once
             const uint8_t* nA = sA + sa1 * SLAB;
             const uint8_t* nB = sB + sb1 * SLAB;
-            wf[0] = read_w(0, nB);
-            wf[1] = read_w(1, nB);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) wf[0][q] = read_w(0, q, nB);
             TG_FENCE();
 #pragma unroll
-            for (int tm = 0; tm < TM; ++tm) {
-                acc[6][tm] = mfma_i8(lo4(wf[2]), lo4(af[tm]), acc[6][tm]);
-                acc[7][tm] = mfma_i8(lo4(wf[3]), lo4(af[tm]), acc[7][tm]);
-                acc[6][tm] = mfma_i8(hi4(wf[2]), hi4(af[tm]), acc[6][tm]);
-                acc[7][tm] = mfma_i8(hi4(wf[3]), hi4(af[tm]), acc[7][tm]);
-                TG_FENCE();
-                af[tm] = read_a(tm, nA);
-                load_a(tm, k2, sa);
-                TG_FENCE();
-            }
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    acc[TN - 1][2 * t] = mfma_i8_32(wf[1][q], af[2 * t][q], acc[TN - 1][2 * t]);
+                    acc[TN - 1][2 * t + 1] = mfma_i8_32(wf[1][q], af[2 * t + 1][q], acc[TN - 1][2 * t + 1]);
+                    TG_FENCE();
+                    af[2 * t][q] = read_a(2 * t, q, nA);
+                    af[2 * t + 1][q] = read_a(2 * t + 1, q, nA);
+                    load_a(2 * q + t, k2, sa);
+                    TG_FENCE();
+                }
             sa = sa1;
             sb = sb1;
         }
 #pragma unroll
-        for (int tm = 0; tm < TM; ++tm) asm volatile("" : : "v"(af[tm]));
-        asm volatile("" : : "v"(wf[0]), "v"(wf[1]));
+        for (int q = 0; q < 4; ++q) {
+#pragma unroll
+            for (int tm = 0; tm < TM; ++tm) asm volatile("" : : "v"(af[tm][q]));
+            asm volatile("" : : "v"(wf[0][q]));
+        }
 
         // ---- epilogue, straight from the accumulators
         const int rows_valid = min(BM, p.M - cm0);
-        int dsts[TM];
+        // (stores without branches, those outside the matrix beyond the descriptor's range: around a branch the compiler copies whole accumulators out
+        // of the accumulation registers early, more than the others hold)
+        constexpr int SIZE = OT == OUT_F32 ? 4 : 2;
+        const StoreTile out(p.C, (int64_t)cm0 * p.ldc * SIZE);
+        uint32_t dsts[TM];
         float srow[TM];
 #pragma unroll
         for (int tm = 0; tm < TM; ++tm) {
-            const int rt = (tm * WGM + wm) * 16 + li;
-            dsts[tm] = rt < rows_valid ? cm0 + rt : -1;
+            const int rt = (tm * WGM + wm) * 32 + li;
+            dsts[tm] = rt < rows_valid ? (uint32_t)rt * (uint32_t)(p.ldc * SIZE) : kBeyond;
             srow[tm] = p.sa[(int64_t)(cm0 + min(rt, rows_valid - 1)) * p.sa_step];
         }
-        // two pairs of column tiles at a time: their 64 columns are whole lines of a 16-bit output, and their factors half of the registers
-        auto emit = [&](auto type_tag) __attribute__((always_inline)) {
-            constexpr int OT = decltype(type_tag)::value;
-            auto half = [&](auto half_tag) __attribute__((always_inline)) {
-                constexpr int first = decltype(half_tag)::value * 2;
-                ColumnFactors f[2];
-                int cols[2];
+        asm volatile("s_nop 15\n\ts_nop 15");  // (the last MFMAs' results, in front of read_acc: 18 wait states)
+        TG_FENCE();
+        // FT sixteens of columns at a time: without a bias two column tiles, whole lines of a 16-bit output
+        constexpr int FT = BIAS ? 2 : 4;
+        auto group = [&](auto group_tag) __attribute__((always_inline)) {
+            constexpr int first = decltype(group_tag)::value * FT;
+            if constexpr (first < 2 * TN) {
+                ColumnFactors<BIAS> f[FT];
+                int cols[FT];
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    cols[t] = cn0 + wn * WTN + (first + t) * 32 + lg * 8;
+                for (int t = 0; t < FT; ++t) {
+                    cols[t] = cn0 + wn * WTN + (first + t) * 16 + half * 8;
                     f[t].load(p, p.sb, min(cols[t], p.N - 8));
                 }
+                TG_FENCE();
                 // (one call per row group instead of a loop, see fp8_gemm_tile256.h)
                 auto rows = [&](auto tm_tag) __attribute__((always_inline)) {
                     constexpr int tm = decltype(tm_tag)::value;
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        if (dsts[tm] < 0 || cols[t] >= p.N) continue;
+                    for (int t = 0; t < FT; ++t) {
                         v4f x, y;
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            x[r] = finish(acc[2 * (first + t)][tm][r], srow[tm], f[t].s[r], f[t].b[r]);
-                            y[r] = finish(acc[2 * (first + t) + 1][tm][r], srow[tm], f[t].s[4 + r], f[t].b[4 + r]);
+                            x[r] = f[t].finished(read_acc(acc[(first + t) / 2][tm][8 * (t & 1) + r]), srow[tm], r);
+                            y[r] = f[t].finished(read_acc(acc[(first + t) / 2][tm][8 * (t & 1) + 4 + r]), srow[tm], 4 + r);
                         }
-                        put8<OT>(p.C, (int64_t)dsts[tm] * p.ldc + cols[t], x, y);
+                        out.template put8<OT>(cols[t] < p.N ? dsts[tm] + (uint32_t)cols[t] * SIZE : kBeyond, x, y);
+                        TG_FENCE();
                     }
                 };
                 rows(std::integral_constant<int, 0>{}); rows(std::integral_constant<int, 1>{});
                 rows(std::integral_constant<int, 2>{}); rows(std::integral_constant<int, 3>{});
-                rows(std::integral_constant<int, 4>{}); rows(std::integral_constant<int, 5>{});
-                rows(std::integral_constant<int, 6>{}); rows(std::integral_constant<int, 7>{});
-            };
-            half(std::integral_constant<int, 0>{});
-            half(std::integral_constant<int, 1>{});
+            }
         };
-        if (p.out_type == OUT_BF16) emit(std::integral_constant<int, OUT_BF16>{});
-        else if (p.out_type == OUT_F32) emit(std::integral_constant<int, OUT_F32>{});
-        else emit(std::integral_constant<int, OUT_F16>{});
+        group(std::integral_constant<int, 0>{});
+        group(std::integral_constant<int, 1>{});
+        group(std::integral_constant<int, 2>{});
+        group(std::integral_constant<int, 3>{});
         if (!more) break;
 #pragma unroll
         for (int tn = 0; tn < TN; ++tn)
 #pragma unroll
-            for (int tm = 0; tm < TM; ++tm) acc[tn][tm] = v4i{0, 0, 0, 0};
+            for (int tm = 0; tm < TM; ++tm) acc[tn][tm] = 0;
     }
 #undef TG_FENCE
     __builtin_amdgcn_s_waitcnt(kWaitAll);  // the re-fetches past the end must land before the workgroup's LDS is released
