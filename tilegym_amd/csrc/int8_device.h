@@ -119,7 +119,7 @@ __device__ __forceinline__ void put1(const Int8GemmParams& p, int64_t to, float 
 __device__ __forceinline__ v4i lo4(v8i v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3); }
 __device__ __forceinline__ v4i hi4(v8i v) { return __builtin_shufflevector(v, v, 4, 5, 6, 7); }
 
-// Scales and biases of the eight columns from `col` on, a multiple of eight (vec_store), without branches (StoreTile's reason).
+// Scales and biases of the eight columns from `col` on, a multiple of eight (vec_store).
 enum BiasKind { BIAS_NONE = 0, BIAS_F32 = 1, BIAS_16 = 2 };
 inline int bias_kind(const Int8GemmParams& p) { return !p.bias ? BIAS_NONE : p.bias_type == OUT_F32 ? BIAS_F32 : BIAS_16; }
 template <int BIAS>
@@ -128,17 +128,19 @@ struct ColumnFactors {
     float s[8], b[BIAS ? 8 : 1];
     // the output in column i of them from its integer sum
     __device__ __forceinline__ float finished(int sum, float sa, int i) const { return finish(sum, sa, s[i], BIAS ? b[BIAS ? i : 0] : 0.f); }
-    __device__ __forceinline__ void load(const Int8GemmParams& p, const float* sb, int col) {
-        typedef uint32_t v4u __attribute__((ext_vector_type(4)));
-        // one scale for all columns: the others lie beyond the range and come as zeros
-        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)sb, 0, p.sb_step ? 0x7FFFFFFF : 4, 0x00020000);
-        const uint32_t at = (uint32_t)(col * p.sb_step) * 4u;
-        const v4f x = __builtin_bit_cast(v4f, (v4u)__builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0)), y = __builtin_bit_cast(v4f, (v4u)__builtin_amdgcn_raw_buffer_load_b128(rsrc, at + 16, 0, 0));
+    __device__ __forceinline__ void load_scales(const Int8GemmParams& p, const float* sb, int col) {
+        if (p.sb_step) {
+            const v4f x = *reinterpret_cast<const v4f*>(sb + col), y = *reinterpret_cast<const v4f*>(sb + col + 4);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            s[i] = p.sb_step ? x[i] : x[0];
-            s[4 + i] = p.sb_step ? y[i] : x[0];
+            for (int i = 0; i < 4; ++i) s[i] = x[i], s[4 + i] = y[i];
+        } else {
+            const float x = *sb;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] = x;
         }
+    }
+    // (no branches: StoreTile's reason)
+    __device__ __forceinline__ void load_bias8(const Int8GemmParams& p, int col) {
         if constexpr (BIAS == BIAS_F32) {
             const v4f u = *reinterpret_cast<const v4f*>((const float*)p.bias + col), v = *reinterpret_cast<const v4f*>((const float*)p.bias + col + 4);
 #pragma unroll
@@ -153,38 +155,6 @@ struct ColumnFactors {
         }
     }
 #endif
-};
-
-// The same with the kinds of bias told apart as they come, for kernels that have registers to spare.
-struct AnyColumnFactors {
-    float s[8], b[8];
-    __device__ __forceinline__ float finished(int sum, float sa, int i) const { return finish(sum, sa, s[i], b[i]); }
-    __device__ __forceinline__ void load(const Int8GemmParams& p, const float* sb, int col) {
-        if (p.sb_step) {
-            const v4f x = *reinterpret_cast<const v4f*>(sb + col), y = *reinterpret_cast<const v4f*>(sb + col + 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[i] = x[i], s[4 + i] = y[i];
-        } else {
-            const float x = *sb;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s[i] = x;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) b[i] = 0.f;
-        if (!p.bias) return;
-        if (p.bias_type == OUT_F32) {
-            const v4f x = *reinterpret_cast<const v4f*>((const float*)p.bias + col), y = *reinterpret_cast<const v4f*>((const float*)p.bias + col + 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) b[i] = x[i], b[4 + i] = y[i];
-        } else {
-            typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-            typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
-            const u16x8 x = *reinterpret_cast<const u16x8*>((const uint16_t*)p.bias + col);
-            const f16x8 h = __builtin_bit_cast(f16x8, x);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) b[i] = p.bias_type == OUT_BF16 ? __uint_as_float((uint32_t)x[i] << 16) : (float)h[i];
-        }
-    }
 };
 
 }  // namespace tg

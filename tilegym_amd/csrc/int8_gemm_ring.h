@@ -3,7 +3,11 @@
 //
 // One workgroup per compute unit: four waves compute (2 x 2), four waves only request the next K steps' slabs by direct global->LDS loads; one
 // barrier per step, in front of its last column tiles.  The reasons stand in fp8_gemm_tile_ring.h.  What differs:
-//   * the MFMAs are 32x32x32 ones, four to a K step of 128 bytes and output, or in tiles whose steps are loads rather than MFMAs two 16x16x64 ones;
+//   * a K step of 128 bytes is two 16x16x64 MFMAs per output, issued a row group apart, so that none waits for the other.  (Four 32x32x32 ones, at a
+//     higher rate, are ahead by up to 10 % while few compute units work, as 256 x 4096 x 4096 in 192 x 128 tiles 19.8 -> 18.2 us, and behind by 5 to 7 % on a full chip,
+//     where power counts: 1400 x 12288 x 5120 in 192 x 192 tiles 80.0 -> 85.9, 2048 x 4096 x 4096 in 256 x 128 32.4 -> 35.5.  Where the chip is not full smaller
+//     tiles are chosen, whose steps are loads.)
+//   * the scales and biases of a tile come to LDS while its first steps are on their way;
 //   * a tile's descriptors start at its own first rows, so that operands may be of any size and a ragged tile's rows anywhere;
 //   * K is any multiple of 16: chunks of the last step behind a row's end are requested from beyond the descriptor's range, which makes them
 //     zeros in LDS;
@@ -16,15 +20,13 @@ namespace tg {
 
 #define TG_FENCE() __builtin_amdgcn_sched_barrier(0)
 
-// A computing wave's part of a step: which MFMA, how its fragments lie in LDS, in which order they are multiplied and refilled, and which outputs an
-// accumulator register is.  Rows and columns of the part: 16 x 16 or 32 x 32 to an MFMA.
-
-// 16x16x64 MFMAs, two to a step and output: tiles of 32 rows or of up to 64 x 64, whose steps are loads, not MFMAs.
+// A computing wave's part of a tile: its accumulators and fragments, in which order they are multiplied and refilled, and which outputs an accumulator
+// register is.
 template <int TM, int TN>
-struct Mma16 {
-    static constexpr int SIDE = 16, VECS = TN / 2;  // vectors of eight columns that a lane has of a row
-    static constexpr int WS = 4, LAST = TN == 4 ? 2 : 1;  // weight fragment sets, column tiles behind the barrier
-    static_assert(TN == 2 || TN == 4, "column tiles");
+struct RingPart {
+    static constexpr int VECS = TN / 2;  // vectors of eight columns that a lane has of a row
+    static constexpr int WS = TN == 6 ? 3 : 4, LAST = TN == 4 ? 2 : 1;  // weight fragment sets, column tiles behind the barrier
+    static_assert(TN == 2 || TN == 4 || TN == 6, "column tiles");
     v4i acc[TN][TM];
     v8i af[TM], wf[WS];
     uint32_t frag0, wfrag0;
@@ -39,8 +41,6 @@ struct Mma16 {
 #pragma unroll
             for (int tm = 0; tm < TM; ++tm) acc[tn][tm] = v4i{0, 0, 0, 0};
     }
-    static __device__ __forceinline__ int a_swizzle(int r) { return swz16(r); }
-    static __device__ __forceinline__ int b_swizzle(int r) { return swz_w(r); }
     template <int WGM>
     __device__ __forceinline__ void read_a(int tm, const uint8_t* base) {
         const uint8_t* a = base + tm * (WGM * 16 * kKBlock);
@@ -52,10 +52,16 @@ struct Mma16 {
     }
     template <int WGM>
     __device__ __forceinline__ void first(const uint8_t* base) {
+        // (in the K loop's order: the compiler waits at its top for what is needed on either way in)
         read_w(0, base);
-        read_w(1, base);
+        if constexpr (TN > 2) read_w(1, base);
+        TG_FENCE();
 #pragma unroll
-        for (int tm = 0; tm < TM; ++tm) read_a<WGM>(tm, base);
+        for (int tm = 0; tm < TM; ++tm) {
+            read_a<WGM>(tm, base);
+            TG_FENCE();
+        }
+        if constexpr (TN == 2) read_w(1, base);
     }
     // column tile by column tile: all row groups' first halves, then the second ones
     __device__ __forceinline__ void before(const uint8_t* cur) {
@@ -100,104 +106,24 @@ struct Mma16 {
     __device__ __forceinline__ int get(int v, int tm, int i) const { return acc[2 * v + (i >> 2)][tm][i & 3]; }
 };
 
-// 32x32x32 MFMAs, four to a step and output.
-template <int TM, int TN>
-struct Mma32 {
-    static constexpr int SIDE = 32, VECS = 2 * TN;
-    static_assert(TN == 2 || TN == 3, "column tiles");
-    v16i acc[TN][TM];
-    v4i af[TM][4], wf[2][4];
-    uint32_t frag[4], wfrag[4];
-    int li, half;
-    __device__ __forceinline__ void init(int lane, int row0, int col0, int b_base) {
-        li = lane & 31, half = lane >> 5;
-        const int wrow = weight_row_32(li);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            frag[q] = (row0 + li) * kKBlock + (((2 * q + half) ^ swz32(li)) << 4);
-            wfrag[q] = b_base + (col0 + wrow) * kKBlock + (((2 * q + half) ^ swz32(wrow)) << 4);
-        }
-#pragma unroll
-        for (int tn = 0; tn < TN; ++tn)
-#pragma unroll
-            for (int tm = 0; tm < TM; ++tm) acc[tn][tm] = 0;
-    }
-    static __device__ __forceinline__ int a_swizzle(int r) { return swz32(r); }
-    static __device__ __forceinline__ int b_swizzle(int r) { return swz32(r); }
-    template <int WGM>
-    __device__ __forceinline__ void read_a(int tm, int q, const uint8_t* base) { af[tm][q] = *reinterpret_cast<const v4i*>(base + tm * (WGM * 32 * kKBlock) + frag[q]); }
-    __device__ __forceinline__ void read_w(int set, int tn, int q, const uint8_t* base) { wf[set][q] = *reinterpret_cast<const v4i*>(base + tn * (32 * kKBlock) + wfrag[q]); }
-    template <int WGM>
-    __device__ __forceinline__ void first(const uint8_t* base) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            read_w(0, 0, q, base);
-#pragma unroll
-            for (int tm = 0; tm < TM; ++tm) read_a<WGM>(tm, q, base);
-        }
-    }
-    __device__ __forceinline__ void before(const uint8_t* cur) {
-#pragma unroll
-        for (int tn = 0; tn < TN - 1; ++tn)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-#pragma unroll
-                for (int tm = 0; tm < TM; ++tm) {
-                    acc[tn][tm] = mfma_i8_32(wf[tn & 1][q], af[tm][q], acc[tn][tm]);
-                    if (tm == 0) read_w((tn + 1) & 1, tn + 1, q, cur);
-                    TG_FENCE();
-                }
-            }
-    }
-    // quarter by quarter of the step: its MFMAs release the row groups' pieces, and with three column tiles the weight's
-    template <int WGM>
-    __device__ __forceinline__ void behind(const uint8_t* nxt) {
-        constexpr int set = (TN - 1) & 1;
-        if constexpr (set == 1) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) read_w(0, 0, q, nxt);
-            TG_FENCE();
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-#pragma unroll
-            for (int tm = 0; tm < TM; ++tm) acc[TN - 1][tm] = mfma_i8_32(wf[set][q], af[tm][q], acc[TN - 1][tm]);
-            TG_FENCE();
-            if constexpr (set == 0) read_w(0, 0, q, nxt);
-#pragma unroll
-            for (int tm = 0; tm < TM; ++tm) read_a<WGM>(tm, q, nxt);
-            TG_FENCE();
-        }
-    }
-    __device__ __forceinline__ void keep() {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-#pragma unroll
-            for (int tm = 0; tm < TM; ++tm) asm volatile("" : : "v"(af[tm][q]));
-            asm volatile("" : : "v"(wf[0][q]));
-        }
-    }
-    __device__ __forceinline__ int row() const { return li; }
-    __device__ __forceinline__ int column(int v) const { return v * 16 + half * 8; }
-    __device__ __forceinline__ int get(int v, int tm, int i) const { return acc[v >> 1][tm][8 * (v & 1) + i]; }
-};
-
 template <int BM, int BN, int STAGES, bool SPLIT, bool RAGGED>
 __global__ void __launch_bounds__(512, 1) int8_gemm_ring_kernel(const Int8GemmParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    constexpr bool WIDE = BM >= 64 && BN >= 128;
-    constexpr int NL = 4, WGN = BN == 32 ? 1 : 2, WGM = 4 / WGN, SIDE = WIDE ? 32 : 16;
+    constexpr int NL = 4, WGN = BN == 32 ? 1 : 2, WGM = 4 / WGN;
     constexpr int WTN = BN / WGN;
-    constexpr int TM = BM / (SIDE * WGM), TN = WTN / SIDE;
-    using Mma = std::conditional_t<WIDE, Mma32<TM, WIDE ? TN : 2>, Mma16<TM, WIDE ? 2 : TN>>;
-    constexpr int VECS = Mma::VECS;
+    constexpr int TM = BM / (16 * WGM), TN = WTN / 16;
+    using Part = RingPart<TM, TN>;
+    constexpr int VECS = Part::VECS;
     constexpr int A_IT = BM / (8 * NL), B_IT = BN / (8 * NL);
     constexpr int STAGE_BYTES = (BM + BN) * kKBlock;
     constexpr int PER_STEP = A_IT + B_IT;
-    static_assert(BM % (SIDE * WGM) == 0 && STAGES >= 3 && STAGES * STAGE_BYTES <= 160 * 1024, "shape");
+    constexpr int FACTORS = (BM + 2 * BN) * 4;
+    static_assert(BM % (16 * WGM) == 0 && STAGES >= 3 && STAGES * STAGE_BYTES + FACTORS <= 160 * 1024, "shape");
     static_assert(!(SPLIT && RAGGED), "K is split for dense rows only");
 
     __shared__ __align__(1024) uint8_t lds[STAGES * STAGE_BYTES];  // stage s: A slab, then B slab
+    // scales of the tile's rows, scales and biases of its columns: brought here while the first steps are on their way
+    __shared__ __align__(16) float s_row[BM], s_col[BN], s_bias[BN];
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -239,8 +165,8 @@ __global__ void __launch_bounds__(512, 1) int8_gemm_ring_kernel(const Int8GemmPa
         // ------------------------------------------------------------ loading waves
         const int lw = wave - 4;
         const int lrow = lane >> 3;
-        const int lj = (lane & 7) ^ Mma::a_swizzle(((lw & 1) << 3) | lrow);
-        const int ljb = (lane & 7) ^ Mma::b_swizzle(((lw & 1) << 3) | lrow);
+        const int lj = (lane & 7) ^ swz16(lrow);
+        const int ljb = (lane & 7) ^ swz_w(((lw & 1) << 3) | lrow);
         constexpr uint32_t kOutOfRange = 0x80000000u;  // beyond the descriptor's 2^31 - 1 bytes
         uint32_t a_off[A_IT], b_off[B_IT];
 #pragma unroll
@@ -282,51 +208,55 @@ __global__ void __launch_bounds__(512, 1) int8_gemm_ring_kernel(const Int8GemmPa
 
     // ---------------------------------------------------------------- computing waves
     const int wm = wave % WGM, wn = wave / WGM;
-    Mma mma;
-    mma.init(lane, wm * SIDE, wn * WTN, BM * kKBlock);
-    const int li = mma.row();
+    Part part;
+    part.init(lane, wm * 16, wn * WTN, BM * kKBlock);
+    const int li = part.row();
 
-    // the scales of this lane's rows, asked for in front of the K loop
-    const float* sb = p.sb + (int64_t)expert * p.N * p.sb_step;
-    float srow[TM];
-#pragma unroll
-    for (int tm = 0; tm < TM; ++tm) srow[tm] = p.sa[(m0 + min((tm * WGM + wm) * SIDE + li, rows_valid - 1)) * p.sa_step];
-
+    if constexpr (!SPLIT) {
+        const float* sb = p.sb + (int64_t)expert * p.N * p.sb_step;
+        for (int i = tid; i < BM; i += 256) s_row[i] = p.sa[(m0 + min(i, rows_valid - 1)) * p.sa_step];
+        for (int i = tid; i < BN; i += 256) {
+            const int col = min(n0 + i, p.N - 1);
+            s_col[i] = sb[(int64_t)col * p.sb_step];
+            s_bias[i] = load_bias(p.bias, p.bias_type, col);
+        }
+    }
+    __builtin_amdgcn_s_waitcnt(kWaitLds);  // (and no scalar load is under way in the K loop: the compiler would wait for all reads of LDS at its top)
     __builtin_amdgcn_s_barrier();  // step 0 has landed
-    mma.template first<WGM>(lds);
+    part.template first<WGM>(lds);
     int stage = 0;
     for (int k = 0; k < nsteps; ++k) {
         const uint8_t* cur = lds + stage * STAGE_BYTES;
         stage = stage == STAGES - 1 ? 0 : stage + 1;
         const uint8_t* nxt = lds + stage * STAGE_BYTES;
         TG_FENCE();
-        mma.before(cur);
+        part.before(cur);
         __builtin_amdgcn_s_waitcnt(kWaitLds);  // all my reads of step k are done
         __builtin_amdgcn_s_barrier();          // step k+1 is visible
         TG_FENCE();
-        mma.template behind<WGM>(nxt);
+        part.template behind<WGM>(nxt);
     }
-    mma.keep();
+    part.keep();
 
     const int col0 = n0 + wn * WTN;
     if constexpr (SPLIT) {
         int* mine = p.partials + (int64_t)blockIdx.y * p.M * p.N;
 #pragma unroll
         for (int tm = 0; tm < TM; ++tm) {
-            const int rt = (tm * WGM + wm) * SIDE + li;
+            const int rt = (tm * WGM + wm) * 16 + li;
             if (rt >= rows_valid) continue;
 #pragma unroll
             for (int v = 0; v < VECS; ++v) {
-                const int col = col0 + mma.column(v);
+                const int col = col0 + part.column(v);
                 int* to = mine + (m0 + rt) * p.N + col;
                 if (p.N % 8 == 0) {
                     if (col >= p.N) continue;
-                    *reinterpret_cast<v4i*>(to) = v4i{mma.get(v, tm, 0), mma.get(v, tm, 1), mma.get(v, tm, 2), mma.get(v, tm, 3)};
-                    *reinterpret_cast<v4i*>(to + 4) = v4i{mma.get(v, tm, 4), mma.get(v, tm, 5), mma.get(v, tm, 6), mma.get(v, tm, 7)};
+                    *reinterpret_cast<v4i*>(to) = v4i{part.get(v, tm, 0), part.get(v, tm, 1), part.get(v, tm, 2), part.get(v, tm, 3)};
+                    *reinterpret_cast<v4i*>(to + 4) = v4i{part.get(v, tm, 4), part.get(v, tm, 5), part.get(v, tm, 6), part.get(v, tm, 7)};
                 } else {
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        if (col + i < p.N) to[i] = mma.get(v, tm, i);
+                        if (col + i < p.N) to[i] = part.get(v, tm, i);
                 }
             }
         }
@@ -334,25 +264,33 @@ __global__ void __launch_bounds__(512, 1) int8_gemm_ring_kernel(const Int8GemmPa
     }
     auto emit_whole = [&](auto type_tag) __attribute__((always_inline)) {
         constexpr int OT = decltype(type_tag)::value;
-        constexpr int FT = TM * VECS > 16 ? 2 : VECS;  // vectors whose factors are in registers at a time
+        constexpr int FV = VECS % 2 == 0 ? 2 : VECS; // vectors whose factors are in registers at a time
+        static_assert(VECS % FV == 0, "whole groups of them");
 #pragma unroll
-        for (int v0 = 0; v0 < VECS; v0 += FT) {
-            AnyColumnFactors f[FT];
+        for (int v0 = 0; v0 < VECS; v0 += FV) {
+            float f[FV][8], b[FV][8];
 #pragma unroll
-            for (int v = 0; v < FT; ++v) f[v].load(p, sb, min(col0 + mma.column(v0 + v), p.N - 8));
+            for (int v = 0; v < FV; ++v)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int at = wn * WTN + part.column(v0 + v) + i;
+                    f[v][i] = s_col[at];
+                    b[v][i] = s_bias[at];
+                }
 #pragma unroll
             for (int tm = 0; tm < TM; ++tm) {
-                const int rt = (tm * WGM + wm) * SIDE + li;
+                const int rt = (tm * WGM + wm) * 16 + li;
                 if (rt >= rows_valid) continue;
+                const float sa = s_row[rt];
 #pragma unroll
-                for (int v = 0; v < FT; ++v) {
-                    const int col = col0 + mma.column(v0 + v);
+                for (int v = 0; v < FV; ++v) {
+                    const int col = col0 + part.column(v0 + v);
                     if (col >= p.N) continue;
                     v4f x, y;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        x[r] = f[v].finished(mma.get(v0 + v, tm, r), srow[tm], r);
-                        y[r] = f[v].finished(mma.get(v0 + v, tm, 4 + r), srow[tm], 4 + r);
+                        x[r] = finish(part.get(v0 + v, tm, r), sa, f[v][r], b[v][r]);
+                        y[r] = finish(part.get(v0 + v, tm, 4 + r), sa, f[v][4 + r], b[v][4 + r]);
                     }
                     put8<OT>(p.C, (m0 + rt) * p.ldc + col, x, y);
                 }
@@ -367,18 +305,18 @@ __global__ void __launch_bounds__(512, 1) int8_gemm_ring_kernel(const Int8GemmPa
     }
     // rows of outputs that are no whole vectors: element by element
 #pragma unroll
-    for (int v = 0; v < VECS; ++v)
+    for (int tm = 0; tm < TM; ++tm) {
+        const int rt = (tm * WGM + wm) * 16 + li;
+        if (rt >= rows_valid) continue;
+        const float sa = s_row[rt];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int col = col0 + mma.column(v) + i;
-            if (col >= p.N) continue;
-            const float s = sb[(int64_t)col * p.sb_step], b = load_bias(p.bias, p.bias_type, col);
+        for (int v = 0; v < VECS; ++v)
 #pragma unroll
-            for (int tm = 0; tm < TM; ++tm) {
-                const int rt = (tm * WGM + wm) * SIDE + li;
-                if (rt < rows_valid) put1(p, (m0 + rt) * p.ldc + col, finish(mma.get(v, tm, i), srow[tm], s, b));
+            for (int i = 0; i < 8; ++i) {
+                const int at = wn * WTN + part.column(v) + i;
+                if (n0 + at < p.N) put1(p, (m0 + rt) * p.ldc + n0 + at, finish(part.get(v, tm, i), sa, s_col[at], s_bias[at]));
             }
-        }
+    }
 #endif
 }
 

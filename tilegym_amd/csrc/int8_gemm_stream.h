@@ -113,6 +113,20 @@ __global__ void __launch_bounds__(256) int8_gemm_stream_kernel(const Int8GemmPar
         for (int i = 0; i < A_LOADS; ++i) direct_load_b128(rsrc_a, a_lds + buf * ABUF + (wave + i * NW) * 1024, a_off[i], k0);
     };
 
+    // a lane holds four consecutive weight rows' results; their scales, asked for in front of everything else
+    const int col = n_base + lg * 4;
+    const float* sb = p.sb + (int64_t)expert * N * p.sb_step;
+    float s[4], b[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int c = min(col + q, N - 1);
+        s[q] = sb[(int64_t)c * p.sb_step];
+        b[q] = load_bias(p.bias, p.bias_type, c);
+    }
+    float sa[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) sa[mt] = p.sa[(row0 + min(mt * 16 + li, rows_a - 1)) * p.sa_step];
+
     v4i acc[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) acc[mt] = v4i{0, 0, 0, 0};
@@ -158,18 +172,9 @@ __global__ void __launch_bounds__(256) int8_gemm_stream_kernel(const Int8GemmPar
             for (int mt = 0; mt < MT; ++mt) acc[mt] = mfma_i8(hi4(wf[s]), hi4(af[mt][s]), acc[mt]);
         }
     }
-    // a lane holds four consecutive weight rows' results; n_end cuts off those that are not the wave's
-    const int col = n_base + lg * 4;
+    // (n_end cuts off those of the four that are not the wave's)
     if (col >= n_end) return;
     const bool vec_ok = p.vec_store != 0 && (R & 3) == 0;
-    const float* sb = p.sb + (int64_t)expert * N * p.sb_step;
-    float s[4], b[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int c = min(col + q, N - 1);
-        s[q] = sb[(int64_t)c * p.sb_step];
-        b[q] = load_bias(p.bias, p.bias_type, c);
-    }
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         const int m = mt * 16 + li;
@@ -185,10 +190,9 @@ __global__ void __launch_bounds__(256) int8_gemm_stream_kernel(const Int8GemmPar
             }
             continue;
         }
-        const float sa = p.sa[(row0 + m) * p.sa_step];
         v4f y;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) y[q] = finish(acc[mt][q], sa, s[q], b[q]);
+        for (int q = 0; q < 4; ++q) y[q] = finish(acc[mt][q], sa[mt], s[q], b[q]);
         store4(p.C, p.out_type, row0 + m, col, n_end, (int)p.ldc, y, 0.f, vec_ok);
     }
 #endif

@@ -122,6 +122,14 @@ __global__ void __launch_bounds__(256, 1) int8_gemm_tile256_kernel(const Int8Gem
     for (;;) {
         const int cm0 = m0, cn0 = n0;
         bool more = false;
+        // the tile's scales, asked for here: a trip to memory in front of the stores would be time without MFMAs
+        const int rows_valid = min(BM, p.M - cm0);
+        float srow[TM];
+        ColumnFactors<BIAS> scale[2 * TN];
+#pragma unroll
+        for (int tm = 0; tm < TM; ++tm) srow[tm] = p.sa[(int64_t)(cm0 + min((tm * WGM + wm) * 32 + li, rows_valid - 1)) * p.sa_step];
+#pragma unroll
+        for (int t = 0; t < 2 * TN; ++t) scale[t].load_scales(p, p.sb, min(cn0 + wn * WTN + t * 16 + half * 8, p.N - 8));
         for (int k = 0; k < nsteps; ++k) {
             if (k == nsteps - 2) {
                 more = vt + stride < total;
@@ -138,8 +146,8 @@ __global__ void __launch_bounds__(256, 1) int8_gemm_tile256_kernel(const Int8Gem
             const int sb2 = sb1 == B_STAGES - 1 ? 0 : sb1 + 1;
             const uint8_t* cB = sB + sb * SLAB;
             TG_FENCE();
-            // column tiles 0 .. 2 in groups of four MFMAs, one per row group; behind each of the first eight groups a direct load, behind every
-            // group a piece of the next column tile's weight fragment
+            // column tiles 0 .. 2 in groups of four MFMAs, one per row group; behind each of the first eight groups a direct load, behind a tile's
+            // first two the next one's weight fragment, so that the barrier finds no read under way
 #pragma unroll
             for (int tn = 0; tn < TN - 1; ++tn) {
 #pragma unroll
@@ -148,7 +156,10 @@ __global__ void __launch_bounds__(256, 1) int8_gemm_tile256_kernel(const Int8Gem
                     for (int tm = 0; tm < TM; ++tm) acc[tn][tm] = mfma_i8_32(wf[tn & 1][q], af[tm][q], acc[tn][tm]);
                     TG_FENCE();
                     if (4 * tn + q < IT) load_b(4 * tn + q, k2, sb2);
-                    wf[(tn + 1) & 1][q] = read_w(tn + 1, q, cB);
+                    if (q < 2) {
+                        wf[(tn + 1) & 1][2 * q] = read_w(tn + 1, 2 * q, cB);
+                        wf[(tn + 1) & 1][2 * q + 1] = read_w(tn + 1, 2 * q + 1, cB);
+                    }
                     TG_FENCE();
                 }
             }
@@ -185,46 +196,40 @@ __global__ void __launch_bounds__(256, 1) int8_gemm_tile256_kernel(const Int8Gem
         }
 
         // ---- epilogue, straight from the accumulators
-        const int rows_valid = min(BM, p.M - cm0);
         // (stores without branches, those outside the matrix beyond the descriptor's range: around a branch the compiler copies whole accumulators out
         // of the accumulation registers early, more than the others hold)
         constexpr int SIZE = OT == OUT_F32 ? 4 : 2;
         const StoreTile out(p.C, (int64_t)cm0 * p.ldc * SIZE);
         uint32_t dsts[TM];
-        float srow[TM];
 #pragma unroll
         for (int tm = 0; tm < TM; ++tm) {
             const int rt = (tm * WGM + wm) * 32 + li;
             dsts[tm] = rt < rows_valid ? (uint32_t)rt * (uint32_t)(p.ldc * SIZE) : kBeyond;
-            srow[tm] = p.sa[(int64_t)(cm0 + min(rt, rows_valid - 1)) * p.sa_step];
         }
         asm volatile("s_nop 15\n\ts_nop 15");  // (the last MFMAs' results, in front of read_acc: 18 wait states)
         TG_FENCE();
-        // FT sixteens of columns at a time: without a bias two column tiles, whole lines of a 16-bit output
-        constexpr int FT = BIAS ? 2 : 4;
+        // row group by row group: the sixteens of columns that make a line follow one another.  Biases: a line's sixteens at a time
         auto group = [&](auto group_tag) __attribute__((always_inline)) {
-            constexpr int first = decltype(group_tag)::value * FT;
+            constexpr int FT = BIAS == BIAS_NONE ? 2 * TN : OT == OUT_F32 ? 2 : 4, first = decltype(group_tag)::value * FT;
             if constexpr (first < 2 * TN) {
-                ColumnFactors<BIAS> f[FT];
-                int cols[FT];
+                if constexpr (BIAS != BIAS_NONE) {
 #pragma unroll
-                for (int t = 0; t < FT; ++t) {
-                    cols[t] = cn0 + wn * WTN + (first + t) * 16 + half * 8;
-                    f[t].load(p, p.sb, min(cols[t], p.N - 8));
+                    for (int t = 0; t < FT; ++t) scale[first + t].load_bias8(p, min(cn0 + wn * WTN + (first + t) * 16 + half * 8, p.N - 8));
+                    TG_FENCE();
                 }
-                TG_FENCE();
                 // (one call per row group instead of a loop, see fp8_gemm_tile256.h)
                 auto rows = [&](auto tm_tag) __attribute__((always_inline)) {
                     constexpr int tm = decltype(tm_tag)::value;
 #pragma unroll
-                    for (int t = 0; t < FT; ++t) {
+                    for (int t = first; t < first + FT; ++t) {
+                        const int col = cn0 + wn * WTN + t * 16 + half * 8;
                         v4f x, y;
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            x[r] = f[t].finished(read_acc(acc[(first + t) / 2][tm][8 * (t & 1) + r]), srow[tm], r);
-                            y[r] = f[t].finished(read_acc(acc[(first + t) / 2][tm][8 * (t & 1) + 4 + r]), srow[tm], 4 + r);
+                            x[r] = scale[t].finished(read_acc(acc[t / 2][tm][8 * (t & 1) + r]), srow[tm], r);
+                            y[r] = scale[t].finished(read_acc(acc[t / 2][tm][8 * (t & 1) + 4 + r]), srow[tm], 4 + r);
                         }
-                        out.template put8<OT>(cols[t] < p.N ? dsts[tm] + (uint32_t)cols[t] * SIZE : kBeyond, x, y);
+                        out.template put8<OT>(col < p.N ? dsts[tm] + (uint32_t)col * SIZE : kBeyond, x, y);
                         TG_FENCE();
                     }
                 };
