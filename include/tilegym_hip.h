@@ -394,8 +394,8 @@ int32_t tg_fp8_kv_attention(const tg_tensor* out, const tg_tensor* q, const tg_t
  * rounded once to c's type.  Every kernel and every split returns the same bits.
  *   a (M, K), b (N, K) int8, contiguous; c (M, N) bf16 / f16 / f32, contiguous; scale_a f32, M elements or one; scale_b f32, N elements or one;
  *   bias (N) bf16 / f16 / f32, or NULL.  Rows of a multiple of 16 bytes on 16-byte addresses take the fast kernels.
- *   workspace: NULL, or a 16-byte aligned buffer of tg_int8_gemm_workspace_bytes() bytes, contents irrelevant: it holds the partial sums of split K
- *   (without it K is not split).  Calls that share one must not overlap in time.
+ *   workspace: NULL, or a 16-byte aligned buffer, contents irrelevant: it holds the partial sums where K is split, tg_int8_gemm_workspace_bytes() bytes (0 where
+ *   it is not; with less K is split less).  Calls that share one must not overlap in time.
  * cfg: TG_CFG_KERNEL (0, 1 or 3), TG_CFG_BLOCK_M, TG_CFG_BLOCK_N, TG_CFG_SPLIT_K as for tg_fp8_gemm; what does not exist is ignored.
  *
  * tg_int8_ragged_gemm: rows m_indptr[e] .. m_indptr[e + 1] of a with b[e] (E, N, K) and scale_b (E, N) (or one element); m_indptr (E + 1) int32 DEVICE
@@ -403,7 +403,7 @@ int32_t tg_fp8_kv_attention(const tg_tensor* out, const tg_tensor* q, const tg_t
  */
 int32_t tg_int8_gemm(const tg_tensor* c, const tg_tensor* a, const tg_tensor* b, const tg_tensor* scale_a, const tg_tensor* scale_b, const tg_tensor* bias,
                      const tg_tensor* workspace, const int32_t* cfg, int32_t ncfg, int32_t device_id, uint64_t hip_stream);
-int64_t tg_int8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int64_t tg_int8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, const int32_t* cfg, int32_t ncfg);
 int32_t tg_int8_ragged_gemm(const tg_tensor* c, const tg_tensor* a, const tg_tensor* b, const tg_tensor* scale_a, const tg_tensor* scale_b,
                             const tg_tensor* m_indptr, const int32_t* cfg, int32_t ncfg, int32_t device_id, uint64_t hip_stream);
 

@@ -8,7 +8,7 @@ from tilegym_amd import _lib, ops
 
 from .test_int8_ops import BF16, F16, F32, _check_matmul, _check_ragged, bits, codes, scales
 
-RING = [(64, 32), (32, 64), (64, 64), (32, 128), (64, 128), (96, 128), (128, 128), (160, 128), (160, 192), (192, 192), (256, 128)]
+RING = [(64, 32), (32, 64), (64, 64), (64, 128), (96, 128), (128, 128), (160, 128), (160, 192), (192, 192), (256, 128)]
 TILE = dict(KERNEL="tiled")
 
 

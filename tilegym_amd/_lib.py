@@ -142,7 +142,7 @@ def load():
     L.tg_int8_gemm.restype = ctypes.c_int32
     L.tg_int8_gemm.argtypes = [P] * 7 + [I32P, ctypes.c_int32, ctypes.c_int32, ctypes.c_uint64]
     L.tg_int8_gemm_workspace_bytes.restype = ctypes.c_int64
-    L.tg_int8_gemm_workspace_bytes.argtypes = [ctypes.c_int64] * 3
+    L.tg_int8_gemm_workspace_bytes.argtypes = [ctypes.c_int64] * 3 + [I32P, ctypes.c_int32]
     L.tg_int8_ragged_gemm.restype = ctypes.c_int32
     L.tg_int8_ragged_gemm.argtypes = [P] * 6 + [I32P, ctypes.c_int32, ctypes.c_int32, ctypes.c_uint64]
     L.tg_int8_quant.restype = ctypes.c_int32
@@ -642,7 +642,7 @@ def int8_gemm(c, a, b, scale_a, scale_b, bias=None, kernel_configs=None) -> None
     dev, ws = _device_index(a), None
     cfg, ncfg = _cfg(kernel_configs)
     if a.dim() == 2 and b.dim() == 2:
-        need = L.tg_int8_gemm_workspace_bytes(a.shape[0], b.shape[0], a.shape[1])
+        need = L.tg_int8_gemm_workspace_bytes(a.shape[0], b.shape[0], a.shape[1], cfg, ncfg)
         if need > 0:
             ws = torch.empty(need, dtype=torch.uint8, device=a.device)
     rc = L.tg_int8_gemm(_desc(c), _desc(a), _desc(b), _desc(scale_a), _desc(scale_b), _desc(bias), _desc(ws), cfg, ncfg, dev, _stream_handle(a))

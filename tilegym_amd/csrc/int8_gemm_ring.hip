@@ -37,7 +37,7 @@ __global__ void __launch_bounds__(256) int8_splitk_reduce_kernel(const Int8GemmP
 
 // Stages: as many as 160 KiB hold, up to twelve.
 #define TG_RING_TILES(X) \
-    X(64, 32, 12) X(32, 64, 12) X(64, 64, 9) X(32, 128, 7) X(64, 128, 5) X(96, 128, 4) X(128, 128, 4) X(160, 128, 4) X(160, 192, 3) X(192, 192, 3) X(256, 128, 3)
+    X(64, 32, 12) X(32, 64, 12) X(64, 64, 9) X(64, 128, 5) X(96, 128, 4) X(128, 128, 4) X(160, 128, 4) X(160, 192, 3) X(192, 192, 3) X(256, 128, 3)
 
 bool int8_ring_exists(int bm, int bn) {
 #define TG_IS(BM, BN, STAGES) || (bm == BM && bn == BN)

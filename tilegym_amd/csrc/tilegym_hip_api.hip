@@ -2282,7 +2282,7 @@ static bool int8_fast_layout(const tg::Int8GemmParams& p) {
     return p.K % 16 == 0 && aligned16(reinterpret_cast<uint64_t>(p.A)) && aligned16(reinterpret_cast<uint64_t>(p.B));
 }
 
-// kernel 0 simple, 1 tiles, 3 streaming, as in cfg[]
+// kernel 0 simple, 1 tiles, 3 streaming (bn: weight rows of a workgroup), as in cfg[]
 struct Int8Schedule { int kernel, bm, bn, split; };
 
 static bool int8_takes(const tg::Int8GemmParams& p, const Int8Schedule& s) {
@@ -2290,28 +2290,87 @@ static bool int8_takes(const tg::Int8GemmParams& p, const Int8Schedule& s) {
     if (!int8_fast_layout(p)) return false;
     if (s.kernel == 3) return (p.m_indptr || p.M <= 32) && s.bn >= 4 && s.bn <= 64 && s.bn % 4 == 0;
     if (s.bm == 256 && s.bn == 256)
-        return !p.m_indptr && p.K % 128 == 0 && p.K >= 256 && p.vec_store && s.split == 1 && (int64_t)p.M * p.K < kOffsetLimit && (int64_t)p.N * p.K < kOffsetLimit;
+        return !p.m_indptr && p.K % 128 == 0 && p.K >= 256 && p.vec_store && s.split == 1 && (int64_t)p.M * p.K < kOffsetLimit && (int64_t)p.N * p.K < kOffsetLimit &&
+               p.ldc * 1024 < kOffsetLimit;
     return tg::int8_ring_exists(s.bm, s.bn);
 }
 
+// Cost models of the dense int8 kernels, of the form of kPerTensorTiles: a launch takes rounds of 256 workgroups x (K steps x step + fixed), the step
+// growing with the share of the chip that is busy and with a weight that comes from memory.  Fitted to 3180 shapes (M = 1 ... 4096, weights of 1 to
+// 330 MB, every tile x 1 / 2 / 4 / 8 splits), each timed over three sets of operands and over 768 MB of them; the constants stand for the geometric mean.  The pick is
+// 0.4 % behind the best schedule on average above 64 rows (95 of 100 shapes within 3 %, at worst 1.23 x), 0.8 % at 17 to 64, and with the
+// streaming form 1.2 % at 17 to 32 and 2.1 % up to 16 (95 of 100 within 7 %, at worst 1.33 x).
+struct Int8Cost { int bm, bn; float first, full, fixed, memory; };
+struct Int8Model { const Int8Cost* tiles; int n; float reduce_us, reduce_us_per_mb; };
+constexpr Int8Cost kInt8Many[] = {{32, 64, 0.147f, 0.114f, 3.124f, 0.031f}, {64, 32, 0.143f, 0.126f, 3.050f, 0.014f}, {64, 64, 0.180f, 0.165f, 3.230f, 0.030f},
+                                  {64, 128, 0.259f, 0.251f, 3.518f, 0.058f}, {96, 128, 0.292f, 0.324f, 3.959f, 0.061f}, {128, 128, 0.324f, 0.395f, 4.556f, 0.065f},
+                                  {160, 128, 0.373f, 0.474f, 4.989f, 0.061f}, {160, 192, 0.514f, 0.670f, 5.833f, 0.048f}, {256, 128, 0.541f, 0.755f, 5.932f, 0.015f},
+                                  {192, 192, 0.593f, 0.803f, 6.366f, 0.021f}, {256, 256, 0.775f, 1.477f, 8.428f, 0.f}};
+constexpr Int8Cost kInt8Few[] = {{32, 64, 0.107f, 0.179f, 3.721f, 0.043f}, {64, 32, 0.112f, 0.169f, 3.594f, 0.007f}, {64, 64, 0.132f, 0.314f, 3.651f, 0.019f},
+                                 {64, 128, 0.202f, 0.588f, 3.728f, 0.047f}};
+constexpr Int8Cost kInt8Decode[] = {{32, 64, 0.100f, 0.292f, 3.537f, 0.009f}, {64, 32, 0.116f, 0.162f, 3.494f, 0.f}, {64, 64, 0.129f, 0.301f, 3.511f, 0.004f},
+                                    {64, 128, 0.197f, 0.565f, 3.560f, 0.023f}};
+constexpr Int8Model kInt8Models[] = {{kInt8Decode, 4, 2.34f, 1.29f}, {kInt8Few, 4, 2.67f, 0.47f}, {kInt8Many, 11, 3.33f, 0.47f}};
+// The streaming form: us per piece of 512 bytes and round, of which `row` per weight row of a workgroup (more with more of the chip busy, and from memory).
+struct Int8StreamCost { float fixed, piece, row, row_busy, row_memory, reduce_us, reduce_us_per_mb; };
+constexpr Int8StreamCost kInt8Stream[] = {{3.432f, 0.376f, 0.00306f, 0.00333f, 0.00109f, 2.22f, 0.60f}, {3.761f, 0.548f, 0.00235f, 0.00586f, 0.00012f, 1.93f, 0.81f}};
+constexpr float kInt8SplitMargin = 1.03f;  // a split is a launch more for the host, too
+
+static Int8Schedule cheapest_int8(const tg::Int8GemmParams& p, int64_t partial_bytes) {
+    const int64_t M = p.M, N = p.N, K = p.K, steps = cdiv(K, 128);
+    const float from_memory = std::min(std::max(((float)(N * K) - 8e6f) / 12e6f, 0.f), 1.f);
+    Int8Schedule best{0, -1, -1, 1};
+    float best_us = 0.f;
+    auto offer = [&](const Int8Schedule& s, float us) {
+        if (s.split > 1) us *= kInt8SplitMargin;
+        if (best.kernel == 0 || us < best_us) { best = s; best_us = us; }
+    };
+    auto splits = [&](int64_t split) { return split == 1 || (M <= 512 && steps / split >= 4 && split * M * N * 4 <= partial_bytes); };
+    const Int8Model& m = kInt8Models[M <= 16 ? 0 : M <= 64 ? 1 : 2];
+    for (int i = 0; i < m.n; ++i) {
+        const Int8Cost& t = m.tiles[i];
+        if (!int8_takes(p, Int8Schedule{1, t.bm, t.bn, 1})) continue;
+        for (int sp = 1; sp <= (t.bm == 256 && t.bn == 256 ? 1 : 8) && splits(sp); sp *= 2) {
+            const int64_t tiles = cdiv(M, t.bm) * cdiv(N, t.bn) * sp, rest = tiles % 256;
+            if (sp > 1 && tiles > 600) break;
+            const float k = (float)cdiv(steps, sp), memory = t.memory * from_memory;
+            float us = (float)(tiles / 256) * (k * (t.full + memory) + t.fixed);
+            if (rest) us += k * (t.first + (t.full - t.first) * (float)rest / 256.f + memory) + t.fixed;
+            if (sp > 1) us += m.reduce_us + m.reduce_us_per_mb * (float)(M * N * 4 * sp) * 1e-6f;
+            offer(Int8Schedule{1, t.bm, t.bn, sp}, us);
+        }
+    }
+    if (M <= 32) {
+        const Int8StreamCost& c = kInt8Stream[M <= 16 ? 0 : 1];
+        for (int rows : {64, 48, 32})
+            for (int sp = 1; sp <= 8 && splits(sp); sp *= 2) {
+                const int64_t groups = cdiv(N, rows) * sp;
+                if (sp > 1 && groups > 700) break;
+                const float busy = std::min((float)groups, 256.f) / 256.f;
+                float us = c.fixed + (float)(cdiv(groups, 256) * cdiv(cdiv(K, 512), sp)) * (c.piece + (c.row + c.row_busy * busy + c.row_memory * from_memory) * (float)rows);
+                if (sp > 1) us += c.reduce_us + c.reduce_us_per_mb * (float)(M * N * 4 * sp) * 1e-6f;
+                offer(Int8Schedule{3, -1, rows, sp}, us);
+            }
+    }
+    return best;
+}
+
 static Int8Schedule choose_int8(const tg::Int8GemmParams& p, int64_t partial_bytes, const int32_t* cfg, int32_t ncfg) {
-    Int8Schedule s{0, -1, -1, 1};
+    const Int8Schedule simple{0, -1, -1, 1};
     const int want = cfg_get(cfg, ncfg, TG_CFG_KERNEL);
     const int want_bm = cfg_get(cfg, ncfg, TG_CFG_BLOCK_M), want_bn = cfg_get(cfg, ncfg, TG_CFG_BLOCK_N), want_split = cfg_get(cfg, ncfg, TG_CFG_SPLIT_K);
     const int64_t steps = cdiv(p.K, 128);
-    if (want == 0) return s;
+    if (want == 0) return simple;
     if (want == 3 || want == 1) {
-        const Int8Schedule forced{want, want_bm, want == 3 && want_bn <= 0 ? 64 : want_bn, 1};
-        if (int8_takes(p, forced)) {
-            s = forced;
+        Int8Schedule s{want, want_bm, want == 3 && want_bn <= 0 ? 64 : want_bn, 1};
+        if (int8_takes(p, s)) {
             if (!p.m_indptr && want_split > 1 && !(s.bm == 256 && s.bn == 256)) s.split = pick_split(1, 1, want == 3 ? cdiv(steps, 4) : steps, 1, p.M, p.N, partial_bytes, want_split);
             return s;
         }
     }
-    if (!int8_fast_layout(p)) return s;
-    const Int8Schedule tile{1, 256, 256, 1}, ring{1, 128, 128, 1}, stream{3, -1, 64, 1};
-    if (p.M <= 16 && !p.m_indptr) return stream;
-    return int8_takes(p, tile) && p.M > 1024 ? tile : ring;
+    if (!int8_fast_layout(p)) return simple;
+    if (!p.m_indptr) return cheapest_int8(p, std::min(partial_bytes, kAutoPartialBytes));
+    return Int8Schedule{1, 128, 128, 1};
 }
 
 static int32_t run_int8(tg::Int8GemmParams p, Int8Schedule s, const tg_tensor* workspace, const char* what, uint64_t hip_stream) {
@@ -2365,9 +2424,12 @@ int32_t tg_int8_gemm(const tg_tensor* c, const tg_tensor* a, const tg_tensor* b,
     return run_int8(p, s, workspace, "int8_gemm", hip_stream);
 }
 
-int64_t tg_int8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-    if (M <= 0 || N <= 0 || K <= 0 || M > 512) return 0;
-    return std::min<int64_t>(8 * M * N * 4, kAutoPartialBytes);
+int64_t tg_int8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, const int32_t* cfg, int32_t ncfg) {
+    if (M <= 0 || N <= 0 || K <= 0 || K > kInt8MostK || M > INT32_MAX - 1024 || N > INT32_MAX - 1024) return 0;
+    tg::Int8GemmParams p{};  // (as if at aligned addresses: without them K is not split)
+    p.M = (int)M, p.N = (int)N, p.K = (int)K, p.ldc = N, p.vec_store = N % 8 == 0;
+    const Int8Schedule s = choose_int8(p, INT64_MAX, cfg, ncfg);
+    return s.split > 1 ? (int64_t)s.split * M * N * 4 : 0;
 }
 
 int32_t tg_int8_ragged_gemm(const tg_tensor* c, const tg_tensor* a, const tg_tensor* b, const tg_tensor* scale_a, const tg_tensor* scale_b,
