@@ -422,6 +422,7 @@ int32_t tg_int8_quant(const tg_tensor* q, const tg_tensor* scales, const tg_tens
  * tg_moe_sort: the (token, slot) pairs of topk_ids (int32 / int64, any shape, n pairs) in the order of their experts, stable; pairs whose id is outside
  *   [0, num_experts) behind the last expert.  indptr (num_experts + 1) int32: rows indptr[e] .. indptr[e + 1] are expert e's; rows (n) int32: the
  *   row of each pair, or -1 - row for the pairs behind the last expert; slots (n) int32: the pair of each row.  num_experts at most 512.
+ *   workspace: at 16-byte addresses, tg_moe_sort_workspace_bytes(n, num_experts) bytes (0 for few pairs: NULL will do), written anew by every call.
  * tg_moe_permute: out[rows[t][j]] = x[t]; zeros in the rows behind the last expert.  x (T, H), rows (T, k), out (T * k, H).
  * tg_moe_unpermute: out[t] = sum_j weights[t][j] * x[rows[t][j]] over the pairs that have an expert, in fp32, in the order of j, rounded once.
  *   weights (T, k) bf16 / f16 / f32, or NULL (ones).  Without weights it is the gradient of tg_moe_permute.
@@ -429,8 +430,9 @@ int32_t tg_int8_quant(const tg_tensor* q, const tg_tensor* scales, const tg_tens
  *   x[rows[t][j]]> in fp32, rounded to the weights' type (zero for pairs without an expert).
  * Rows of bf16 / f16 / f32 (one type per call), contiguous, any H.  What `rows` names outside the T * k rows is left out.
  */
-int32_t tg_moe_sort(const tg_tensor* topk_ids, int32_t num_experts, const tg_tensor* indptr, const tg_tensor* rows, const tg_tensor* slots, int32_t device_id,
-                    uint64_t hip_stream);
+int64_t tg_moe_sort_workspace_bytes(int64_t n, int32_t num_experts);
+int32_t tg_moe_sort(const tg_tensor* topk_ids, int32_t num_experts, const tg_tensor* indptr, const tg_tensor* rows, const tg_tensor* slots,
+                    const tg_tensor* workspace, int32_t device_id, uint64_t hip_stream);
 int32_t tg_moe_permute(const tg_tensor* out, const tg_tensor* x, const tg_tensor* rows, int32_t device_id, uint64_t hip_stream);
 int32_t tg_moe_unpermute(const tg_tensor* out, const tg_tensor* x, const tg_tensor* rows, const tg_tensor* weights, int32_t device_id, uint64_t hip_stream);
 int32_t tg_moe_unpermute_backward(const tg_tensor* grad_x, const tg_tensor* grad_weights, const tg_tensor* grad_out, const tg_tensor* x, const tg_tensor* rows,

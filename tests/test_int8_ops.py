@@ -140,7 +140,7 @@ def test_route_refusals():
     ids = torch.zeros(3, 2, dtype=i32)
 
     def sort(ids=ids, E=4, ptr=torch.zeros(5, dtype=i32), rows=torch.zeros(3, 2, dtype=i32), slots=torch.zeros(6, dtype=i32)):
-        return L.tg_moe_sort(d(ids), E, d(ptr), d(rows), d(slots), 9999, 0)
+        return L.tg_moe_sort(d(ids), E, d(ptr), d(rows), d(slots), None, 9999, 0)
 
     assert sort() == -4 and sort(ids=ids.long()) == -4
     assert sort(ids=ids.to(torch.uint8)) == -2

@@ -70,7 +70,8 @@ _lib = None
 native = None  # the extension module, once load() has run (still None where it cannot be imported)
 _NATIVE_ENTRY_POINTS = ("tg_fp8_gemm", "tg_fp8_gemm_workspace_bytes", "tg_fp8_ragged_gemm", "tg_fp8_quant_group", "tg_fp8_fused_moe",
                         "tg_fp8_fused_moe_block_m", "tg_fp8_fused_moe_workspace_bytes", "tg_fp8_rms_norm_quant", "tg_fp8_kv_append",
-                        "tg_fp8_kv_read", "tg_fp8_kv_attention", "tg_fp8_kv_attention_workspace_bytes")
+                        "tg_fp8_kv_read", "tg_fp8_kv_attention", "tg_fp8_kv_attention_workspace_bytes", "tg_int8_gemm", "tg_int8_gemm_workspace_bytes",
+                        "tg_int8_ragged_gemm", "tg_int8_quant", "tg_moe_sort", "tg_moe_sort_workspace_bytes", "tg_moe_permute", "tg_moe_unpermute", "tg_moe_unpermute_backward")
 
 
 def lib_path() -> str:
@@ -148,7 +149,9 @@ def load():
     L.tg_int8_quant.restype = ctypes.c_int32
     L.tg_int8_quant.argtypes = [P] * 4 + [ctypes.c_int32, ctypes.c_int32, ctypes.c_uint64]
     L.tg_moe_sort.restype = ctypes.c_int32
-    L.tg_moe_sort.argtypes = [P, ctypes.c_int32, P, P, P, ctypes.c_int32, ctypes.c_uint64]
+    L.tg_moe_sort.argtypes = [P, ctypes.c_int32, P, P, P, P, ctypes.c_int32, ctypes.c_uint64]
+    L.tg_moe_sort_workspace_bytes.restype = ctypes.c_int64
+    L.tg_moe_sort_workspace_bytes.argtypes = [ctypes.c_int64, ctypes.c_int32]
     L.tg_moe_permute.restype = ctypes.c_int32
     L.tg_moe_permute.argtypes = [P] * 3 + [ctypes.c_int32, ctypes.c_uint64]
     L.tg_moe_unpermute.restype = ctypes.c_int32
@@ -664,7 +667,9 @@ def int8_quant(q, scales, x, place=None, silu_mul: bool = False) -> None:
 
 def moe_sort(topk_ids, num_experts: int, indptr, rows, slots) -> None:
     L = _lib if _lib is not None else load()
-    rc = L.tg_moe_sort(_desc(topk_ids), int(num_experts), _desc(indptr), _desc(rows), _desc(slots), _device_index(topk_ids), _stream_handle(topk_ids))
+    need = L.tg_moe_sort_workspace_bytes(topk_ids.numel(), int(num_experts))
+    ws = torch.empty(need, dtype=torch.uint8, device=topk_ids.device) if need > 0 else None
+    rc = L.tg_moe_sort(_desc(topk_ids), int(num_experts), _desc(indptr), _desc(rows), _desc(slots), _desc(ws), _device_index(topk_ids), _stream_handle(topk_ids))
     check_rc(rc, "tg_moe_sort")
 
 

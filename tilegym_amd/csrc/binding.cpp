@@ -33,6 +33,15 @@ decltype(&tg_fp8_kv_append) g_kv_append = nullptr;
 decltype(&tg_fp8_kv_read) g_kv_read = nullptr;
 decltype(&tg_fp8_kv_attention) g_kv_attention = nullptr;
 decltype(&tg_fp8_kv_attention_workspace_bytes) g_kv_attention_workspace_bytes = nullptr;
+decltype(&tg_int8_gemm) g_int8_gemm = nullptr;
+decltype(&tg_int8_gemm_workspace_bytes) g_int8_gemm_workspace_bytes = nullptr;
+decltype(&tg_int8_ragged_gemm) g_int8_ragged_gemm = nullptr;
+decltype(&tg_int8_quant) g_int8_quant = nullptr;
+decltype(&tg_moe_sort) g_moe_sort = nullptr;
+decltype(&tg_moe_sort_workspace_bytes) g_moe_sort_workspace_bytes = nullptr;
+decltype(&tg_moe_permute) g_moe_permute = nullptr;
+decltype(&tg_moe_unpermute) g_moe_unpermute = nullptr;
+decltype(&tg_moe_unpermute_backward) g_moe_unpermute_backward = nullptr;
 PyObject* g_workspaces = nullptr;     // {(device, stream, under capture): [scratch tensors, newest last]}
 PyObject* g_workspace_for = nullptr;  // callable(device, bytes, index, stream) -> tensor, for a new or larger one
 PyObject* g_check_rc = nullptr;       // callable(rc, where): raises
@@ -525,6 +534,206 @@ PyObject* py_kv_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// Calls f(device, stream) without the interpreter's lock; false with an exception set.
+template <typename F>
+bool launched(const at::Tensor& like, const char* where, F f) {
+    const int index = like.get_device();
+    const uint64_t stream = (uint64_t)(uintptr_t)c10::hip::getCurrentHIPStream(index).stream();
+    int32_t rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = f(index, stream);
+    Py_END_ALLOW_THREADS
+    return succeeded(rc, where);
+}
+
+PyObject* tuple_of(std::initializer_list<at::Tensor*> tensors) {
+    PyObject* tuple = PyTuple_New((Py_ssize_t)tensors.size());
+    if (!tuple) return nullptr;
+    Py_ssize_t at = 0;
+    for (at::Tensor* t : tensors) PyTuple_SET_ITEM(tuple, at++, THPVariable_Wrap(std::move(*t)));
+    return tuple;
+}
+
+// The given `out` (contiguous, of these sizes and type), or a new tensor.  False: not plain.
+bool out_tensor(PyObject* given, at::IntArrayRef sizes, PyObject* dtype, const at::Tensor& like, at::Tensor* out) {
+    if (!THPDtype_Check(dtype)) return false;
+    const at::ScalarType type = reinterpret_cast<THPDtype*>(dtype)->scalar_type;
+    if (!io_type(type)) return false;
+    if (given == Py_None) {
+        *out = new_tensor(sizes, type, like);
+        return true;
+    }
+    const at::Tensor* t = tensor_of(given);
+    if (!on_gpu(t) || t->scalar_type() != type || t->sizes() != sizes || !t->is_contiguous() || t->device() != like.device()) return false;
+    *out = *t;
+    return true;
+}
+PyObject* out_or_given(PyObject* given, at::Tensor&& out) {
+    if (given == Py_None) return THPVariable_Wrap(std::move(out));
+    Py_INCREF(given);
+    return given;
+}
+
+// int8_matmul(a, b, scale_a, scale_b, bias, out_dtype, out) -> out, or None.  The scratch memory is the call's own
+PyObject* py_int8_matmul(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 7) { PyErr_SetString(PyExc_TypeError, "int8_matmul takes 7 arguments"); return nullptr; }
+    const at::Tensor *a = tensor_of(args[0]), *b = tensor_of(args[1]);
+    if (!on_gpu(a) || a->dim() < 1 || !plain(a, at::kChar, a->dim()) || !plain(b, at::kChar, 2) || a->device() != b->device()) Py_RETURN_NONE;
+    const int64_t K = a->size(a->dim() - 1), N = b->size(0);
+    if (b->size(1) != K || K == 0) Py_RETURN_NONE;
+    const int64_t M = a->numel() / K;
+    tg_tensor dsa, dsb, dbias, dws;
+    const tg_tensor *sa, *sb, *bias;
+    if (!optional_tensor(args[2], *a, &dsa, &sa) || !sa || !optional_tensor(args[3], *a, &dsb, &sb) || !sb || !optional_tensor(args[4], *a, &dbias, &bias))
+        Py_RETURN_NONE;
+    c10::SmallVector<int64_t, 4> sizes(a->sizes().begin(), a->sizes().end());
+    sizes.back() = N;
+    at::Tensor c, ws;
+    if (!out_tensor(args[6], sizes, args[5], *a, &c)) Py_RETURN_NONE;
+    const int64_t need = g_int8_gemm_workspace_bytes(M, N, K, nullptr, 0);
+    if (need > 0) {
+        ws = new_tensor({need}, at::kByte, *a);
+        dws = describe_rows(ws, 1, need);
+    }
+    const tg_tensor dc = describe_rows(c, M, N), da = describe_rows(*a, M, K), db = describe_rows(*b, N, K);
+    if (!launched(*a, "tg_int8_gemm", [&](int32_t device, uint64_t stream) {
+            return g_int8_gemm(&dc, &da, &db, sa, sb, bias, need > 0 ? &dws : nullptr, nullptr, 0, device, stream);
+        }))
+        return nullptr;
+    return out_or_given(args[6], std::move(c));
+    END_HANDLE_TH_ERRORS
+}
+
+// ragged_int8_matmul(a, b, scale_a, scale_b, m_indptr, out_dtype, out) -> out, or None
+PyObject* py_ragged_int8_matmul(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 7) { PyErr_SetString(PyExc_TypeError, "ragged_int8_matmul takes 7 arguments"); return nullptr; }
+    const at::Tensor *a = tensor_of(args[0]), *b = tensor_of(args[1]);
+    if (!plain(a, at::kChar, 2) || !plain(b, at::kChar, 3) || a->device() != b->device() || a->size(1) != b->size(2)) Py_RETURN_NONE;
+    tg_tensor dc, da, db, dsa, dsb, dptr;
+    const tg_tensor *sa, *sb, *ptr;
+    if (!optional_tensor(args[2], *a, &dsa, &sa) || !sa || !optional_tensor(args[3], *a, &dsb, &sb) || !sb || !optional_tensor(args[4], *a, &dptr, &ptr) || !ptr)
+        Py_RETURN_NONE;
+    at::Tensor c;
+    if (!out_tensor(args[6], {a->size(0), b->size(1)}, args[5], *a, &c) || !describe(c, &dc) || !describe(*a, &da) || !describe(*b, &db)) Py_RETURN_NONE;
+    if (!launched(*a, "tg_int8_ragged_gemm",
+                  [&](int32_t device, uint64_t stream) { return g_int8_ragged_gemm(&dc, &da, &db, sa, sb, ptr, nullptr, 0, device, stream); }))
+        return nullptr;
+    return out_or_given(args[6], std::move(c));
+    END_HANDLE_TH_ERRORS
+}
+
+// int8_quant(x, rows, silu_mul) -> (q, scales), or None: rows (T, k) carries each row of x (T, H) to its k places, None leaves them in order
+PyObject* py_int8_quant(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 3) { PyErr_SetString(PyExc_TypeError, "int8_quant takes 3 arguments"); return nullptr; }
+    const at::Tensor* x = tensor_of(args[0]);
+    if (!on_gpu(x) || !io_type(x->scalar_type()) || !x->is_contiguous() || x->dim() < 1 || x->dim() > TG_MAX_DIMS) Py_RETURN_NONE;
+    tg_tensor dq, ds, dx, dplace;
+    const tg_tensor* place;
+    if (!optional_tensor(args[1], *x, &dplace, &place)) Py_RETURN_NONE;
+    const bool silu_mul = args[2] == Py_True;
+    c10::SmallVector<int64_t, 4> sizes(x->sizes().begin(), x->sizes().end());
+    if (place) {
+        if (dplace.ndim != 2 || x->dim() != 2 || dplace.shape[0] != sizes[0]) Py_RETURN_NONE;
+        sizes[0] *= dplace.shape[1];
+    }
+    if (silu_mul) {
+        if (sizes.back() % 2 != 0) Py_RETURN_NONE;
+        sizes.back() /= 2;
+    }
+    at::Tensor q = new_tensor(sizes, at::kChar, *x), scales = new_tensor(at::IntArrayRef(sizes.data(), sizes.size() - 1), at::kFloat, *x);
+    if (!describe(q, &dq) || !describe(scales, &ds) || !describe(*x, &dx)) Py_RETURN_NONE;
+    if (!launched(*x, "tg_int8_quant", [&](int32_t device, uint64_t stream) { return g_int8_quant(&dq, &ds, &dx, place, silu_mul, device, stream); }))
+        return nullptr;
+    return tuple_of({&q, &scales});
+    END_HANDLE_TH_ERRORS
+}
+
+// moe_sort(ids, num_experts) -> (indptr, rows, slots), or None.  The scratch memory is the call's own
+PyObject* py_moe_sort(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 2) { PyErr_SetString(PyExc_TypeError, "moe_sort takes 2 arguments"); return nullptr; }
+    const at::Tensor* ids = tensor_of(args[0]);
+    const long experts = PyLong_AsLong(args[1]);
+    if (PyErr_Occurred()) return nullptr;
+    if (!on_gpu(ids) || ids->dim() != 2 || !ids->is_contiguous() || experts < 1 || experts > INT32_MAX - 1) Py_RETURN_NONE;
+    at::Tensor indptr = new_tensor({experts + 1}, at::kInt, *ids), rows = new_tensor(ids->sizes(), at::kInt, *ids), slots = new_tensor({ids->numel()}, at::kInt, *ids);
+    tg_tensor di, dp, dr, ds, dws;
+    at::Tensor ws;
+    const int64_t need = g_moe_sort_workspace_bytes(ids->numel(), (int32_t)experts);
+    if (need > 0) {
+        ws = new_tensor({need}, at::kByte, *ids);
+        dws = describe_rows(ws, 1, need);
+    }
+    if (!describe(*ids, &di) || !describe(indptr, &dp) || !describe(rows, &dr) || !describe(slots, &ds)) Py_RETURN_NONE;
+    if (!launched(*ids, "tg_moe_sort", [&](int32_t device, uint64_t stream) {
+            return g_moe_sort(&di, (int32_t)experts, &dp, &dr, &ds, need > 0 ? &dws : nullptr, device, stream);
+        }))
+        return nullptr;
+    return tuple_of({&indptr, &rows, &slots});
+    END_HANDLE_TH_ERRORS
+}
+
+// The x (rows, H) and the places (T, k) of the ways there and back; false: not plain.
+bool route_operands(PyObject* x, PyObject* rows, const at::Tensor** px, const at::Tensor** prows, tg_tensor* dx, tg_tensor* drows) {
+    const at::Tensor *tx = tensor_of(x), *tr = tensor_of(rows);
+    if (!on_gpu(tx) || !io_type(tx->scalar_type()) || tx->dim() != 2 || !plain(tr, at::kInt, 2) || tx->device() != tr->device()) return false;
+    *px = tx;
+    *prows = tr;
+    return describe(*tx, dx) && describe(*tr, drows);
+}
+
+// moe_permute(x, rows) -> tensor, or None
+PyObject* py_moe_permute(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 2) { PyErr_SetString(PyExc_TypeError, "moe_permute takes 2 arguments"); return nullptr; }
+    const at::Tensor *x, *rows;
+    tg_tensor dout, dx, drows;
+    if (!route_operands(args[0], args[1], &x, &rows, &dx, &drows) || x->size(0) != rows->size(0)) Py_RETURN_NONE;
+    at::Tensor out = new_tensor({rows->numel(), x->size(1)}, x->scalar_type(), *x);
+    if (!describe(out, &dout)) Py_RETURN_NONE;
+    if (!launched(*x, "tg_moe_permute", [&](int32_t device, uint64_t stream) { return g_moe_permute(&dout, &dx, &drows, device, stream); })) return nullptr;
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// moe_unpermute(x, rows, weights) -> tensor, or None
+PyObject* py_moe_unpermute(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 3) { PyErr_SetString(PyExc_TypeError, "moe_unpermute takes 3 arguments"); return nullptr; }
+    const at::Tensor *x, *rows;
+    tg_tensor dout, dx, drows, dw;
+    const tg_tensor* weights;
+    if (!route_operands(args[0], args[1], &x, &rows, &dx, &drows) || x->size(0) != rows->numel() || !optional_tensor(args[2], *x, &dw, &weights)) Py_RETURN_NONE;
+    at::Tensor out = new_tensor({rows->size(0), x->size(1)}, x->scalar_type(), *x);
+    if (!describe(out, &dout)) Py_RETURN_NONE;
+    if (!launched(*x, "tg_moe_unpermute", [&](int32_t device, uint64_t stream) { return g_moe_unpermute(&dout, &dx, &drows, weights, device, stream); }))
+        return nullptr;
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// moe_unpermute_backward(grad_out, x, rows, weights) -> (grad_x, grad_weights), or None
+PyObject* py_moe_unpermute_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 4) { PyErr_SetString(PyExc_TypeError, "moe_unpermute_backward takes 4 arguments"); return nullptr; }
+    const at::Tensor *x, *rows, *grad = tensor_of(args[0]), *weights = tensor_of(args[3]);
+    tg_tensor dgx, dgw, dgrad, dx, drows, dw;
+    if (!route_operands(args[1], args[2], &x, &rows, &dx, &drows) || !on_gpu(grad) || grad->device() != x->device() || !grad->is_contiguous() ||
+        !on_gpu(weights) || weights->device() != x->device() || !io_type(weights->scalar_type()) || !describe(*grad, &dgrad) || !describe(*weights, &dw))
+        Py_RETURN_NONE;
+    at::Tensor gx = new_tensor(x->sizes(), x->scalar_type(), *x), gw = new_tensor(weights->sizes(), weights->scalar_type(), *x);
+    if (!describe(gx, &dgx) || !describe(gw, &dgw)) Py_RETURN_NONE;
+    if (!launched(*x, "tg_moe_unpermute_backward", [&](int32_t device, uint64_t stream) {
+            return g_moe_unpermute_backward(&dgx, &dgw, &dgrad, &dx, &drows, &dw, device, stream);
+        }))
+        return nullptr;
+    return tuple_of({&gx, &gw});
+    END_HANDLE_TH_ERRORS
+}
+
 // set_up({name: address}, workspaces, workspace_for, check_rc)
 PyObject* py_set_up(PyObject*, PyObject* args) {
     PyObject *table, *workspaces, *workspace_for, *check_rc;
@@ -540,7 +749,12 @@ PyObject* py_set_up(PyObject*, PyObject* args) {
         !find("tg_fp8_quant_group", &g_quant_group) || !find("tg_fp8_fused_moe", &g_fused_moe) ||
         !find("tg_fp8_rms_norm_quant", &g_rms_norm_quant) || !find("tg_fp8_kv_append", &g_kv_append) || !find("tg_fp8_kv_read", &g_kv_read) ||
         !find("tg_fp8_kv_attention", &g_kv_attention) || !find("tg_fp8_kv_attention_workspace_bytes", &g_kv_attention_workspace_bytes) ||
-        !find("tg_fp8_fused_moe_block_m", &g_fused_moe_block_m) || !find("tg_fp8_fused_moe_workspace_bytes", &g_fused_moe_workspace_bytes))
+        !find("tg_fp8_fused_moe_block_m", &g_fused_moe_block_m) || !find("tg_fp8_fused_moe_workspace_bytes", &g_fused_moe_workspace_bytes) ||
+        !find("tg_int8_gemm", &g_int8_gemm) || !find("tg_int8_gemm_workspace_bytes", &g_int8_gemm_workspace_bytes) ||
+        !find("tg_int8_ragged_gemm", &g_int8_ragged_gemm) || !find("tg_int8_quant", &g_int8_quant) || !find("tg_moe_sort", &g_moe_sort) ||
+        !find("tg_moe_sort_workspace_bytes", &g_moe_sort_workspace_bytes) ||
+        !find("tg_moe_permute", &g_moe_permute) || !find("tg_moe_unpermute", &g_moe_unpermute) ||
+        !find("tg_moe_unpermute_backward", &g_moe_unpermute_backward))
         return nullptr;
     for (auto [slot, o] : {std::pair{&g_workspaces, workspaces}, std::pair{&g_workspace_for, workspace_for}, std::pair{&g_check_rc, check_rc}}) {
         Py_INCREF(o);
@@ -561,6 +775,13 @@ PyMethodDef kMethods[] = {TG_FAST("matmul", py_matmul),
                           TG_FAST("kv_append", py_kv_append),
                           TG_FAST("kv_read", py_kv_read),
                           TG_FAST("kv_attention", py_kv_attention),
+                          TG_FAST("int8_matmul", py_int8_matmul),
+                          TG_FAST("ragged_int8_matmul", py_ragged_int8_matmul),
+                          TG_FAST("int8_quant", py_int8_quant),
+                          TG_FAST("moe_sort", py_moe_sort),
+                          TG_FAST("moe_permute", py_moe_permute),
+                          TG_FAST("moe_unpermute", py_moe_unpermute),
+                          TG_FAST("moe_unpermute_backward", py_moe_unpermute_backward),
                           {"set_up", py_set_up, METH_VARARGS, nullptr},
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

@@ -1,8 +1,9 @@
 // Tokens sorted by expert, carried there and back with the router's weights, and the gradients of both ways.
 //
 // sort: a stable counting sort of the (token, slot) pairs by expert.  Pairs whose expert is not here (an id outside [0, E)) are sorted behind the
-// last expert: every pair has a row, and every row a pair.  Every workgroup counts all ids in LDS (those in front of its slice, those behind),
-// ranks its own slice in order, and needs nothing from the others: one launch, no workspace, no order that atomics could change.
+// last expert: every pair has a row, and every row a pair.  Few pairs: every workgroup counts all ids in LDS (those in front of its slice, those
+// behind) and ranks its own slice in order: one launch.  Many: a first launch counts each slice, and a workgroup of the second adds the
+// slices' counts up.  No order that atomics could change.
 //
 // permute, unpermute and their gradients go by tokens, not by rows: a token's element is read once and written to its top_k rows, or
 // gathered from them, summed in fp32 in the order of the slots and rounded once.  No atomics.  Bound by HBM.
@@ -26,8 +27,25 @@ __device__ __forceinline__ unsigned long long same_key(int key, bool in) {
 }
 
 template <typename IdT>
-__global__ void __launch_bounds__(64 * kSortWaves) moe_sort_kernel(const IdT* __restrict__ ids, int n, int E, int per_wave, int* __restrict__ indptr,
-                                                                   int* __restrict__ rows, int* __restrict__ slots) {
+__device__ __forceinline__ int expert_of(IdT id, int E) { return id >= 0 && id < E ? (int)id : E; }
+
+// counts[blockIdx][e]: the pairs of expert e in this workgroup's slice.
+template <typename IdT>
+__global__ void __launch_bounds__(64 * kSortWaves) moe_count_kernel(const IdT* __restrict__ ids, int n, int E, int per_wave, int* __restrict__ counts) {
+    extern __shared__ int lds[];
+    const int B = E + 1, tid = threadIdx.x;
+    constexpr int NT = 64 * kSortWaves;
+    for (int i = tid; i < B; i += NT) lds[i] = 0;
+    __syncthreads();
+    const int64_t lo = (int64_t)blockIdx.x * kSortWaves * per_wave, hi = min(lo + (int64_t)kSortWaves * per_wave, (int64_t)n);
+    for (int64_t i = lo + tid; i < hi; i += NT) atomicAdd(&lds[expert_of(ids[i], E)], 1);
+    __syncthreads();
+    for (int i = tid; i < B; i += NT) counts[(int64_t)blockIdx.x * B + i] = lds[i];
+}
+
+template <typename IdT, bool COUNTED>
+__global__ void __launch_bounds__(64 * kSortWaves) moe_sort_kernel(const IdT* __restrict__ ids, int n, int E, int per_wave, const int* __restrict__ counts,
+                                                                   int* __restrict__ indptr, int* __restrict__ rows, int* __restrict__ slots) {
     extern __shared__ int lds[];
     const int B = E + 1;                   // experts, and the pairs without one
     int* const mine = lds;                 // [kSortWaves][B]: counts of this workgroup's waves, then their next rows
@@ -39,22 +57,28 @@ __global__ void __launch_bounds__(64 * kSortWaves) moe_sort_kernel(const IdT* __
     for (int i = tid; i < (kSortWaves + 2) * B; i += NT) lds[i] = 0;
     __syncthreads();
     const int64_t lo = (int64_t)blockIdx.x * kSortWaves * per_wave, hi = min(lo + (int64_t)kSortWaves * per_wave, (int64_t)n);
-    auto key_of = [&](int64_t i) {
-        const IdT id = ids[i];
-        return id >= 0 && id < E ? (int)id : E;
-    };
-    constexpr int BATCH = 8;  // loads in flight together
-    for (int64_t i0 = tid; i0 < n; i0 += NT * BATCH) {
-        int key[BATCH];
-#pragma unroll
-        for (int u = 0; u < BATCH; ++u) key[u] = i0 + u * NT < n ? key_of(i0 + u * NT) : -1;
-#pragma unroll
-        for (int u = 0; u < BATCH; ++u) {
-            const int64_t i = i0 + u * NT;
-            if (key[u] < 0) continue;
-            if (i < lo) atomicAdd(&before[key[u]], 1);
-            else if (i >= hi) atomicAdd(&behind[key[u]], 1);
-            else atomicAdd(&mine[(int)((i - lo) / per_wave) * B + key[u]], 1);
+    auto key_of = [&](int64_t i) { return expert_of(ids[i], E); };
+    if constexpr (COUNTED) {
+        // the slices' counts, several slices at a time; then this workgroup's own, by wave
+        const int at_once = NT / B, slice0 = tid / B, e = tid - slice0 * B;
+        if (slice0 < at_once) {
+            int front = 0, back = 0;
+            for (int g = slice0; g < (int)gridDim.x; g += at_once) {
+                const int c = counts[(int64_t)g * B + e];
+                front += g < (int)blockIdx.x ? c : 0;
+                back += g > (int)blockIdx.x ? c : 0;
+            }
+            if (front) atomicAdd(&before[e], front);
+            if (back) atomicAdd(&behind[e], back);
+        }
+        const int64_t first = lo + (int64_t)wave * per_wave, last = min(first + per_wave, (int64_t)n);
+        for (int64_t i = first + lane; i < last; i += 64) atomicAdd(&mine[wave * B + key_of(i)], 1);
+    } else {
+        for (int64_t i = tid; i < n; i += NT) {
+            const int key = key_of(i);
+            if (i < lo) atomicAdd(&before[key], 1);
+            else if (i >= hi) atomicAdd(&behind[key], 1);
+            else atomicAdd(&mine[(int)(i - lo) / per_wave * B + key], 1);
         }
     }
     __syncthreads();
@@ -238,17 +262,39 @@ hipError_t launch_type(int which, const MoeRouteParams& p, int type, hipStream_t
 
 }  // namespace
 
-hipError_t run_moe_sort(const void* ids, bool ids_are_i64, int n, int E, int* indptr, int* rows, int* slots, hipStream_t s) {
-    if (E < 1 || E > kSortMaxExperts) return hipErrorInvalidValue;
-    // up to 32 workgroups; a wave's slice is a multiple of 64 pairs
-    int groups = (n + 1023) / 1024;
-    groups = groups < 1 ? 1 : groups > 32 ? 32 : groups;
-    const int64_t waves = (int64_t)groups * kSortWaves;
-    const int per_wave = (int)((((int64_t)n + waves - 1) / waves + 63) / 64 * 64);
+namespace {
+constexpr int kSortAlone = 4096;     // pairs
+constexpr int kSortGroups = 256;
+// A wave's slice is a multiple of 64 pairs, a workgroup's at least 1024.
+struct SortPlan { int groups, per_wave; };
+SortPlan sort_plan(int64_t n) {
+    int64_t groups = (n + 64 * kSortWaves - 1) / (64 * kSortWaves);
+    groups = groups < 1 ? 1 : groups > kSortGroups ? kSortGroups : groups;
+    const int64_t waves = groups * kSortWaves, per_wave = ((n + waves - 1) / waves + 63) / 64 * 64;
+    return {(int)groups, per_wave > 0 ? (int)per_wave : 64};
+}
+template <typename IdT>
+hipError_t launch_sort(const IdT* ids, int n, int E, int* counts, int* indptr, int* rows, int* slots, hipStream_t s) {
+    const SortPlan plan = sort_plan(n);
+    const dim3 grid(plan.groups), block(64 * kSortWaves);
     const int bytes = ((kSortWaves + 2) * (E + 1) + kSortWaves) * 4;
-    if (ids_are_i64) hipLaunchKernelGGL(moe_sort_kernel<int64_t>, dim3(groups), dim3(64 * kSortWaves), bytes, s, (const int64_t*)ids, n, E, per_wave > 0 ? per_wave : 64, indptr, rows, slots);
-    else hipLaunchKernelGGL(moe_sort_kernel<int>, dim3(groups), dim3(64 * kSortWaves), bytes, s, (const int*)ids, n, E, per_wave > 0 ? per_wave : 64, indptr, rows, slots);
+    if (n <= kSortAlone) {
+        hipLaunchKernelGGL((moe_sort_kernel<IdT, false>), grid, block, bytes, s, ids, n, E, plan.per_wave, nullptr, indptr, rows, slots);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL((moe_count_kernel<IdT>), grid, block, (E + 1) * 4, s, ids, n, E, plan.per_wave, counts);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((moe_sort_kernel<IdT, true>), grid, block, bytes, s, ids, n, E, plan.per_wave, counts, indptr, rows, slots);
     return hipGetLastError();
+}
+}  // namespace
+
+int64_t moe_sort_workspace_bytes(int64_t n, int E) { return n <= kSortAlone ? 0 : (int64_t)sort_plan(n).groups * (E + 1) * 4; }
+
+hipError_t run_moe_sort(const void* ids, bool ids_are_i64, int n, int E, int* counts, int* indptr, int* rows, int* slots, hipStream_t s) {
+    if (E < 1 || E > kSortMaxExperts) return hipErrorInvalidValue;
+    return ids_are_i64 ? launch_sort((const int64_t*)ids, n, E, counts, indptr, rows, slots, s) : launch_sort((const int*)ids, n, E, counts, indptr, rows, slots, s);
 }
 
 int64_t moe_route_threads(const MoeRouteParams& p) { return p.tokens * kRouteLanes; }

@@ -239,7 +239,8 @@ hipError_t run_int8_quant(const Int8QuantParams& p, int x_type, hipStream_t s);
 
 // Tokens sorted by expert and back (moe_route.hip)
 constexpr int kSortMaxExperts = 512;
-hipError_t run_moe_sort(const void* ids, bool ids_are_i64, int n, int E, int* indptr, int* rows, int* slots, hipStream_t s);
+int64_t moe_sort_workspace_bytes(int64_t n, int E);  // of counts; 0: none
+hipError_t run_moe_sort(const void* ids, bool ids_are_i64, int n, int E, int* counts, int* indptr, int* rows, int* slots, hipStream_t s);
 struct MoeRouteParams {
     const void* x;           // permute, gradient: (tokens, H); unpermute: (tokens * top_k, H)
     const void* made;        // gradient: what was weighted, (tokens * top_k, H)

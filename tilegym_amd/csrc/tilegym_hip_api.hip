@@ -2521,8 +2521,12 @@ int32_t tg_int8_quant(const tg_tensor* q, const tg_tensor* scales, const tg_tens
 }
 
 // ---------------------------------------------------------------------------- tokens sorted by expert and back
-int32_t tg_moe_sort(const tg_tensor* topk_ids, int32_t num_experts, const tg_tensor* indptr, const tg_tensor* rows, const tg_tensor* slots, int32_t device_id,
-                    uint64_t hip_stream) {
+int64_t tg_moe_sort_workspace_bytes(int64_t n, int32_t num_experts) {
+    return n < 0 || n > INT32_MAX || num_experts < 1 || num_experts > tg::kSortMaxExperts ? 0 : tg::moe_sort_workspace_bytes(n, num_experts);
+}
+
+int32_t tg_moe_sort(const tg_tensor* topk_ids, int32_t num_experts, const tg_tensor* indptr, const tg_tensor* rows, const tg_tensor* slots,
+                    const tg_tensor* workspace, int32_t device_id, uint64_t hip_stream) {
     g_err[0] = 0;
     int32_t rc;
     if ((rc = check_tensor(topk_ids, "topk_ids", -1)) || (rc = check_tensor(indptr, "indptr", 1)) || (rc = check_tensor(rows, "rows", -1)) ||
@@ -2535,9 +2539,17 @@ int32_t tg_moe_sort(const tg_tensor* topk_ids, int32_t num_experts, const tg_ten
     if (n > INT32_MAX) return fail(TG_ERR_INVALID, "too many slots");
     if (indptr->shape[0] != num_experts + 1 || numel(rows) != n || numel(slots) != n)
         return fail(TG_ERR_INVALID, "indptr must have %d elements, rows and slots %lld each", num_experts + 1, (long long)n);
+    const int64_t need = tg::moe_sort_workspace_bytes(n, num_experts);
+    if (need > 0) {
+        if (!workspace) return fail(TG_ERR_INVALID, "%lld slots need a workspace of %lld bytes", (long long)n, (long long)need);
+        if ((rc = check_tensor(workspace, "workspace", -1))) return rc;
+        if (numel(workspace) * elem_size(workspace->dtype) < need || !aligned16(workspace->ptr))
+            return fail(TG_ERR_INVALID, "workspace must be 16-byte aligned and hold %lld bytes", (long long)need);
+    }
     DeviceGuard guard(device_id);
     if (!guard.ok) return fail(TG_ERR_DEVICE, "cannot use HIP device %d", device_id);
-    const hipError_t e = tg::run_moe_sort(reinterpret_cast<const void*>(topk_ids->ptr), topk_ids->dtype == TG_I64, (int)n, num_experts, reinterpret_cast<int*>(indptr->ptr),
+    const hipError_t e = tg::run_moe_sort(reinterpret_cast<const void*>(topk_ids->ptr), topk_ids->dtype == TG_I64, (int)n, num_experts,
+                                          need > 0 ? reinterpret_cast<int*>(workspace->ptr) : nullptr, reinterpret_cast<int*>(indptr->ptr),
                                           reinterpret_cast<int*>(rows->ptr), reinterpret_cast<int*>(slots->ptr), reinterpret_cast<hipStream_t>(hip_stream));
     if (e != hipSuccess) return fail(TG_ERR_LAUNCH, "moe_sort launch failed: %s", hipGetErrorString(e));
     return TG_OK;

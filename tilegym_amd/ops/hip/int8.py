@@ -19,6 +19,10 @@ def _output(where, out, shape, dtype, device):
 
 @register_impl("int8_matmul", backend="hip")
 def int8_matmul(a, b, scale_a, scale_b, bias=None, out_dtype=torch.bfloat16, out=None, kernel_configs=None):
+    if kernel_configs is None and _lib.native_path():
+        c = _lib.native.int8_matmul(a, b, scale_a, scale_b, bias, out_dtype, out)
+        if c is not None:
+            return c
     _one_device("int8_matmul", a, b, scale_a, scale_b, bias, out)
     if a.dim() < 1 or b.dim() != 2:
         raise ValueError(f"int8_matmul: a must be (..., K) and b (N, K), got {tuple(a.shape)} and {tuple(b.shape)}")
@@ -36,6 +40,10 @@ def int8_matmul(a, b, scale_a, scale_b, bias=None, out_dtype=torch.bfloat16, out
 
 @register_impl("ragged_int8_matmul", backend="hip")
 def ragged_int8_matmul(a, b, scale_a, scale_b, m_indptr, out_dtype=torch.bfloat16, out=None, kernel_configs=None):
+    if kernel_configs is None and _lib.native_path():
+        c = _lib.native.ragged_int8_matmul(a, b, scale_a, scale_b, m_indptr, out_dtype, out)
+        if c is not None:
+            return c
     _one_device("ragged_int8_matmul", a, b, scale_a, scale_b, m_indptr, out)
     if a.dim() != 2 or b.dim() != 3:
         raise ValueError(f"ragged_int8_matmul: a must be (M, K) and b (E, N, K), got {tuple(a.shape)} and {tuple(b.shape)}")
@@ -46,6 +54,10 @@ def ragged_int8_matmul(a, b, scale_a, scale_b, m_indptr, out_dtype=torch.bfloat1
 
 @register_impl("quant_int8", backend="hip")
 def quant_int8(x):
+    if _lib.native_path():
+        done = _lib.native.int8_quant(x, None, False)
+        if done is not None:
+            return done
     _one_device("quant_int8", x)
     if x.dim() < 1:
         raise ValueError("quant_int8: x needs at least one dimension")
@@ -57,6 +69,10 @@ def quant_int8(x):
 
 @register_impl("silu_mul_quant_int8", backend="hip")
 def silu_mul_quant_int8(x):
+    if _lib.native_path():
+        done = _lib.native.int8_quant(x, None, True)
+        if done is not None:
+            return done
     _one_device("silu_mul_quant_int8", x)
     if x.dim() < 1 or x.shape[-1] % 2 != 0:
         raise ValueError(f"silu_mul_quant_int8: x must be (..., 2 I), got {tuple(x.shape)}")

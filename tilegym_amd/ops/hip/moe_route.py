@@ -18,6 +18,10 @@ def _pairs(where, order):
 
 
 def _permute(x, order):
+    if _lib.native_path():
+        done = _lib.native.moe_permute(x, order.rows)
+        if done is not None:
+            return done
     _one_device("moe_permute", x, order.rows)
     tokens, k = _pairs("moe_permute", order)
     if x.dim() != 2 or x.shape[0] != tokens:
@@ -28,6 +32,10 @@ def _permute(x, order):
 
 
 def _unpermute(x, order, weights, where="moe_unpermute"):
+    if _lib.native_path():
+        done = _lib.native.moe_unpermute(x, order.rows, weights)
+        if done is not None:
+            return done
     _one_device(where, x, order.rows, weights)
     tokens, k = _pairs(where, order)
     if x.dim() != 2 or x.shape[0] != tokens * k:
@@ -69,6 +77,10 @@ class _Unpermute(torch.autograd.Function):
 
 @register_impl("moe_sort", backend="hip")
 def moe_sort(topk_ids, num_experts):
+    if _lib.native_path():
+        done = _lib.native.moe_sort(topk_ids, num_experts)
+        if done is not None:
+            return MoeOrder(*done)
     _one_device("moe_sort", topk_ids)
     if topk_ids.dim() != 2:
         raise ValueError(f"moe_sort: topk_ids must be (T, k), got {tuple(topk_ids.shape)}")
@@ -87,6 +99,10 @@ def moe_permute(x, order):
 
 @register_impl("moe_permute_quant_int8", backend="hip")
 def moe_permute_quant_int8(x, order):
+    if _lib.native_path():
+        done = _lib.native.int8_quant(x, order.rows, False)
+        if done is not None:
+            return done
     _one_device("moe_permute_quant_int8", x, order.rows)
     tokens, k = _pairs("moe_permute_quant_int8", order)
     if x.dim() != 2 or x.shape[0] != tokens:
@@ -111,8 +127,12 @@ def moe_permute_backward(grad_rows, order):
 
 @register_impl("moe_unpermute_backward", backend="hip")
 def moe_unpermute_backward(grad_out, x, order, weights):
-    _one_device("moe_unpermute_backward", grad_out, x, order.rows, weights)
     grad_out = grad_out.contiguous()
+    if _lib.native_path():
+        done = _lib.native.moe_unpermute_backward(grad_out, x, order.rows, weights)
+        if done is not None:
+            return done
+    _one_device("moe_unpermute_backward", grad_out, x, order.rows, weights)
     grad_x, grad_weights = torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty(weights.shape, dtype=weights.dtype, device=x.device)
     _lib.moe_unpermute_backward(grad_x, grad_weights, grad_out, x, order.rows, weights)
     return grad_x, grad_weights

@@ -25,7 +25,8 @@ class MoeOrder(NamedTuple):
 
 @dispatch("moe_sort")
 def moe_sort(topk_ids: torch.Tensor, num_experts: int) -> MoeOrder:
-    """The order of topk_ids (T, k), int32 or int64, by expert; pairs of one expert keep their order.  One launch, nothing is read by the host.
+    """The order of topk_ids (T, k), int32 or int64, by expert; pairs of one expert keep their order.  One launch, or two for many pairs; nothing is
+    read by the host.
     At most 512 experts."""
     raise NotImplementedError(f"moe_sort is not implemented for this backend: {get_current_backend()}")
 
