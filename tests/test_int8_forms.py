@@ -97,6 +97,19 @@ def test_ragged_ring_tiles(device, bm, bn):
 
 
 @pytest.mark.gpu
+def test_ragged_tile256(device):
+    cfg = dict(KERNEL="tiled", BLOCK_M=256, BLOCK_N=256)
+    for counts in COUNTS + [[0] * 70, [300, 0, 257, 256, 255, 1] * 50]:  # (the last: several tiles for a workgroup, experts beyond its first 64 and 256)
+        for n, k in ((280, 640), (40, 256)):
+            for t in (BF16, F32, F16):
+                _check_ragged(device, counts, n, k, t, tail=9, start=3, kernel_configs=cfg)
+                ran(KERNEL=1, BLOCK_M=256, BLOCK_N=256)
+    _check_ragged(device, [0] * 63 + [600, 900] + [0] * 63 + [700] + [0] * 100 + [1], 3000, 384, BF16, tail=300, start=0, kernel_configs=cfg)
+    _check_ragged(device, [5, 513, 0, 3], 264, 272, F32, tail=1, kernel_configs=cfg)  # K in no whole steps: another form
+    assert _lib.last_config()["BLOCK_N"] != 256
+
+
+@pytest.mark.gpu
 def test_ragged_stream_and_simple(device):
     for counts in COUNTS:
         for n, k in ((200, 1024), (40, 400), (72, 16)):

@@ -84,6 +84,53 @@ __device__ __forceinline__ bool ragged_tile(const Int8GemmParams& p, int bid, in
     return true;
 }
 
+// The same for a workgroup that takes one tile after the other, in their order: 64 experts' row tiles stay in registers, so that finding the next
+// tile reads memory only where it belongs to a later 64.
+template <int BM>
+struct RaggedWalk {
+    int upto, rows, first;  // lane l: the row tiles of experts e0 ... e0 + l, expert e0 + l's rows and the first of them
+    int e0, base;           // base: row tiles of the experts in front of e0
+    __device__ __forceinline__ void scan(const Int8GemmParams& p, int lane) {
+        const int e = e0 + lane;
+        rows = e < p.E ? ragged_rows(p, e) : 0;
+        first = e < p.E ? p.m_indptr[e] : 0;
+        upto = (rows + BM - 1) / BM;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int t = __shfl_up(upto, d);
+            if (lane >= d) upto += t;
+        }
+    }
+    // All tiles there are.
+    __device__ __forceinline__ int start(const Int8GemmParams& p, int lane, int tiles_n) {
+        int total = 0;
+        for (e0 = (p.E - 1) / 64 * 64;; e0 -= 64) {
+            scan(p, lane);
+            total += __builtin_amdgcn_readlane(upto, 63);
+            if (e0 == 0) break;
+        }
+        base = 0;
+        return total * tiles_n;
+    }
+    // Tile pid, below that total and not below the last one asked for.
+    __device__ __forceinline__ void find(const Int8GemmParams& p, int lane, int pid, int tiles_n, int& expert, int& m0, int& rows_valid, int& tile_n) {
+        const int row_tile = pid / tiles_n;
+        unsigned long long hit;
+        while (!(hit = __ballot(base + upto > row_tile))) {
+            base += __builtin_amdgcn_readlane(upto, 63);
+            e0 += 64;
+            scan(p, lane);
+        }
+        const int l = __builtin_amdgcn_readfirstlane(__ffsll((long long)hit) - 1), has = __builtin_amdgcn_readlane(rows, l);
+        const int mine = (has + BM - 1) / BM, inside = pid - (base + __builtin_amdgcn_readlane(upto, l) - mine) * tiles_n;
+        const int at = inside % mine * BM;
+        expert = e0 + l;
+        tile_n = inside / mine;
+        m0 = __builtin_amdgcn_readlane(first, l) + at;
+        rows_valid = min(BM, has - at);
+    }
+};
+
 // Stores of eight outputs at byte offsets from a tile's first row; those from kBeyond on are left out.
 constexpr uint32_t kBeyond = 0x80000000u;
 struct StoreTile {

@@ -22,7 +22,7 @@ __device__ __forceinline__ int read_acc(int x) {
 
 // A kernel per output type and kind of bias: with all in one the compiler reads every
 // accumulator out in front of the choice, spills, and waits for the reload in every K step (855 -> 1006 us).
-template <int OT, int BIAS>
+template <int OT, int BIAS, bool RAGGED>
 __global__ void __launch_bounds__(256, 1) int8_gemm_tile256_kernel(const Int8GemmParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int BM = 256, BN = 256, WGM = 2, WGN = 2, NW = 4;
@@ -40,18 +40,30 @@ __global__ void __launch_bounds__(256, 1) int8_gemm_tile256_kernel(const Int8Gem
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave % WGM, wn = wave / WGM;
     const int K = p.K;
-    const int tiles_n = (p.N + BN - 1) / BN, tiles_m = (p.M + BM - 1) / BM;
-    const int total = tiles_m * tiles_n, stride = (int)gridDim.x;
+    const int tiles_n = (p.N + BN - 1) / BN, tiles_m = (p.M + BM - 1) / BM, stride = (int)gridDim.x;
+    RaggedWalk<BM> walk;
+    int total;
+    if constexpr (RAGGED) total = walk.start(p, lane, tiles_n);
+    else total = tiles_m * tiles_n;
+    int rows = BM, expert = 0;  // of the tile at (m0, n0)
     auto origin = [&](int v, int& om0, int& on0) {
         const int pid = xcd_remap(v, total);
+        if constexpr (RAGGED) {
+            int tile_n;
+            walk.find(p, lane, pid, tiles_n, expert, om0, rows, tile_n);
+            on0 = tile_n * BN;
+            return;
+        }
         constexpr int GM = 8;
         const int width = GM * tiles_n;
         const int group = pid / width, first_m = group * GM;
         const int gsz = min(tiles_m - first_m, GM);
         om0 = (first_m + (pid % width) % gsz) * BM;
         on0 = ((pid % width) / gsz) * BN;
+        rows = min(BM, p.M - om0);
     };
     int vt = (int)blockIdx.x;
+    if (RAGGED && vt >= total) return;
     int m0, n0;
     origin(vt, m0, n0);
     const int nsteps = K / kKBlock, last = nsteps - 1;
@@ -60,16 +72,16 @@ __global__ void __launch_bounds__(256, 1) int8_gemm_tile256_kernel(const Int8Gem
     const int lj = (lane & 7) ^ swz32(((wave & 1) << 3) | lrow);
     uint32_t a_off[IT], b_off[IT];
     auto set_offsets = [&](int om0, int on0) {
-        const int rv = min(BM, p.M - om0);
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
             const int r = (i * NW + wave) * 8 + lrow;
-            a_off[i] = (uint32_t)(om0 + min(r, rv - 1)) * (uint32_t)K + lj * 16;
+            a_off[i] = (uint32_t)(om0 + min(r, rows - 1)) * (uint32_t)K + lj * 16;
             b_off[i] = (uint32_t)min(on0 + r, p.N - 1) * (uint32_t)K + lj * 16;
         }
     };
     set_offsets(m0, n0);
-    const v4i rsrc_a = make_rsrc(p.A), rsrc_b = make_rsrc(p.B);
+    const v4i rsrc_a = make_rsrc(p.A);
+    v4i rsrc_b = make_rsrc(p.B + (int64_t)expert * p.N * K);
     const uint32_t ldsA = settle(lds_address(sA) + wave * 1024), ldsB = settle(lds_address(sB) + wave * 1024);
     auto load_a = [&](int i, int kstep, int stage) {
         direct_load_b128_settled(rsrc_a, ldsA + stage * SLAB + i * NW * 1024, a_off[i], kstep * kKBlock);
@@ -120,16 +132,16 @@ __global__ void __launch_bounds__(256, 1) int8_gemm_tile256_kernel(const Int8Gem
 
     int sa = 0, sb = 0;
     for (;;) {
-        const int cm0 = m0, cn0 = n0;
+        const int cm0 = m0, cn0 = n0, rows_valid = rows;
+        const float* const sb_tile = p.sb + (int64_t)expert * p.N * p.sb_step;
         bool more = false;
         // the tile's scales, asked for here: a trip to memory in front of the stores would be time without MFMAs
-        const int rows_valid = min(BM, p.M - cm0);
         float srow[TM];
         ColumnFactors<BIAS> scale[2 * TN];
 #pragma unroll
         for (int tm = 0; tm < TM; ++tm) srow[tm] = p.sa[(int64_t)(cm0 + min((tm * WGM + wm) * 32 + li, rows_valid - 1)) * p.sa_step];
 #pragma unroll
-        for (int t = 0; t < 2 * TN; ++t) scale[t].load_scales(p, p.sb, min(cn0 + wn * WTN + t * 16 + half * 8, p.N - 8));
+        for (int t = 0; t < 2 * TN; ++t) scale[t].load_scales(p, sb_tile, min(cn0 + wn * WTN + t * 16 + half * 8, p.N - 8));
         for (int k = 0; k < nsteps; ++k) {
             if (k == nsteps - 2) {
                 more = vt + stride < total;
@@ -137,6 +149,7 @@ __global__ void __launch_bounds__(256, 1) int8_gemm_tile256_kernel(const Int8Gem
                     vt += stride;
                     origin(vt, m0, n0);
                     set_offsets(m0, n0);
+                    if constexpr (RAGGED) rsrc_b = make_rsrc(p.B + (int64_t)expert * p.N * K);
                 }
             }
             int k2 = k + 2;

@@ -63,6 +63,7 @@ __global__ void __launch_bounds__(64 * kSortWaves) moe_sort_kernel(const IdT* __
         const int at_once = NT / B, slice0 = tid / B, e = tid - slice0 * B;
         if (slice0 < at_once) {
             int front = 0, back = 0;
+#pragma unroll 8
             for (int g = slice0; g < (int)gridDim.x; g += at_once) {
                 const int c = counts[(int64_t)g * B + e];
                 front += g < (int)blockIdx.x ? c : 0;
@@ -263,7 +264,9 @@ hipError_t launch_type(int which, const MoeRouteParams& p, int type, hipStream_t
 }  // namespace
 
 namespace {
-constexpr int kSortAlone = 4096;     // pairs
+// Pairs that are sorted in one launch (64 experts, int64, us, one launch / two): 4096 4.9 / 6.8, 16384 6.7 / 7.2, 24576 7.9 / 7.4, 262144 43 / 12; 8 experts
+// 16384 7.9 / 6.9, 256 experts 24576 8.3 / 9.4.
+constexpr int64_t kSortAlone = 16384;
 constexpr int kSortGroups = 256;
 // A wave's slice is a multiple of 64 pairs, a workgroup's at least 1024.
 struct SortPlan { int groups, per_wave; };

@@ -2290,7 +2290,7 @@ static bool int8_takes(const tg::Int8GemmParams& p, const Int8Schedule& s) {
     if (!int8_fast_layout(p)) return false;
     if (s.kernel == 3) return (p.m_indptr || p.M <= 32) && s.bn >= 4 && s.bn <= 64 && s.bn % 4 == 0;
     if (s.bm == 256 && s.bn == 256)
-        return !p.m_indptr && p.K % 128 == 0 && p.K >= 256 && p.vec_store && s.split == 1 && (int64_t)p.M * p.K < kOffsetLimit && (int64_t)p.N * p.K < kOffsetLimit &&
+        return p.K % 128 == 0 && p.K >= 256 && p.vec_store && s.split == 1 && (int64_t)p.M * p.K < kOffsetLimit && (int64_t)p.N * p.K < kOffsetLimit &&
                p.ldc * 1024 < kOffsetLimit;
     return tg::int8_ring_exists(s.bm, s.bn);
 }
