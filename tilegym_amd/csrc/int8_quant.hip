@@ -44,20 +44,24 @@ __device__ __forceinline__ uint32_t magnitude(v8f_q v) {
 }
 
 __device__ __forceinline__ v2i codes8(v8f_q v, const ScaleDivider& d) {
-    int c[8];
+    // 1.5 * 2^23 added to a number below 2^22 rounds it half to even, and leaves the integer in the low bits
+    uint32_t c[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
         float t;
-        if (d.fast) {
+        if (d.fast) {  // (|t| < 127.5: the scale is max|y| / 127 to three roundings)
             t = v[k] * d.r;
             t = __builtin_fmaf(-__builtin_fmaf(d.s, t, -v[k]), d.r, t);
             t = __builtin_fmaf(-__builtin_fmaf(d.s, t, -v[k]), d.r, t);
         } else {
-            t = v[k] / d.s;
+            t = __builtin_amdgcn_fmed3f(v[k] / d.s, -127.f, 127.f);
         }
-        c[k] = (int)__builtin_amdgcn_fmed3f(__builtin_rintf(t), -127.f, 127.f) & 255;
+        c[k] = __float_as_uint(t + 0x1.8p23f);
     }
-    return v2i{c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24};
+    auto low_bytes = [](uint32_t a, uint32_t b, uint32_t e, uint32_t f) {
+        return (int)(__builtin_amdgcn_perm(b, a, 0x0c0c0400u) | __builtin_amdgcn_perm(f, e, 0x04000c0cu));
+    };
+    return v2i{low_bytes(c[0], c[1], c[2], c[3]), low_bytes(c[4], c[5], c[6], c[7])};
 }
 
 template <bool VEC>
@@ -144,9 +148,13 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) int8_quant_kernel(const
     }
 }
 
-// As many lanes as a row has vectors, one each: a row's chain of load, maximum, exchange, store is shortest.
+// (rows from which a wave has one to itself, us with / without: 2048 x 1408 activated 7.6 / 8.5, 24576 x 1408 34.5 / 48, 65536 x 1024 36 / 51)
+constexpr int64_t kWaveRows = 2048;
+// As many lanes as a row has vectors, one each: a row's chain of load, maximum, exchange, store is shortest.  With many rows, a
+// wave for each of up to 256 vectors: no lanes without a vector but in the last sixty-four, and nothing is exchanged through LDS.
 int lanes_of(const Int8QuantParams& p) {
     const int vectors = (p.K + 7) / 8;
+    if (p.rows >= kWaveRows && vectors <= 256) return 64;
     return vectors <= 64 ? 64 : vectors <= 128 ? 128 : vectors <= 256 ? 256 : vectors <= 512 ? 512 : 1024;
 }
 int64_t blocks_of(const Int8QuantParams& p, int lanes) {
@@ -164,6 +172,9 @@ hipError_t launch(const Int8QuantParams& p, hipStream_t s) {
         return hipGetLastError();                                                                    \
     }
     TG_QUANT(64, 1)
+    TG_QUANT(64, 2)
+    TG_QUANT(64, 3)
+    TG_QUANT(64, 4)
     TG_QUANT(128, 1)
     TG_QUANT(256, 1)
     TG_QUANT(512, 1)

@@ -2357,11 +2357,12 @@ static Int8Schedule cheapest_int8(const tg::Int8GemmParams& p, int64_t partial_b
 
 // Rows of experts, which the host knows the number of, not how they are spread.  The streaming form up to 12 rows per expert on average (it reads the weights of
 // the experts that have rows once per 16 rows); above, the tiles by a model of the form above over the row tiles to be expected, fitted to 3600 problems
-// (1 to 30 000 rows over 4 to 128 experts, spread evenly to e^1.5 : 1): 3.9 % behind the best form on average, 95 of 100 within 1.26 x.
+// (1 to 30 000 rows over 4 to 128 experts, spread evenly to e^1.5 : 1), its 256 x 256 row to 3000 (500 to 60 000 rows): 3.9 % and 3.5 % behind the best form on
+// average, 95 of 100 within 1.26 and 1.22 x.
 constexpr Int8Cost kInt8Ragged[] = {{32, 64, 0.134f, 0.139f, 4.512f, 0.114f}, {64, 32, 0.137f, 0.121f, 4.458f, 0.068f}, {64, 64, 0.149f, 0.172f, 4.557f, 0.122f},
                                     {64, 128, 0.218f, 0.261f, 4.680f, 0.222f}, {96, 128, 0.345f, 0.378f, 4.506f, 0.169f}, {128, 128, 0.389f, 0.491f, 5.001f, 0.126f},
                                     {160, 128, 0.424f, 0.589f, 5.501f, 0.104f}, {160, 192, 0.516f, 0.735f, 6.785f, 0.174f}, {256, 128, 0.556f, 0.828f, 6.743f, 0.078f},
-                                    {192, 192, 0.586f, 0.841f, 7.512f, 0.156f}};
+                                    {192, 192, 0.586f, 0.841f, 7.512f, 0.156f}, {256, 256, 0.918f, 1.362f, 9.757f, 0.212f}};
 constexpr int64_t kInt8StreamRowsPerExpert = 12;
 
 static Int8Schedule cheapest_int8_ragged(const tg::Int8GemmParams& p) {
@@ -2372,6 +2373,7 @@ static Int8Schedule cheapest_int8_ragged(const tg::Int8GemmParams& p) {
     Int8Schedule best{0, -1, -1, 1};
     float best_us = 0.f;
     for (const Int8Cost& t : kInt8Ragged) {
+        if (!int8_takes(p, Int8Schedule{1, t.bm, t.bn, 1})) continue;
         const double tiles = (M / t.bm + std::min(M, E) * 0.5) * (double)cdiv(p.N, t.bn), rounds = tiles / 256;
         const double whole = rounds <= 2 ? std::ceil(rounds) : (rounds + std::ceil(rounds)) / 2;
         const float us = (float)whole * ((float)(K / 128) * (t.first + (t.full - t.first) * (float)std::min(1., rounds) + t.memory * from_memory) + t.fixed);
