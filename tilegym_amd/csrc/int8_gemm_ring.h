@@ -36,6 +36,9 @@ struct RingPart {
         frag0 = (row0 + li) * kKBlock + ((lg ^ swz16(li)) << 4);
         const int wrow = ((li >> 2) << 3) | (li & 3);
         wfrag0 = b_base + (col0 + wrow) * kKBlock + ((lg ^ swz_w(wrow)) << 4);
+        clear();
+    }
+    __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int tn = 0; tn < TN; ++tn)
 #pragma unroll
@@ -106,7 +109,109 @@ struct RingPart {
     __device__ __forceinline__ int get(int v, int tm, int i) const { return acc[2 * v + (i >> 2)][tm][i & 3]; }
 };
 
-template <int BM, int BN, int STAGES, bool SPLIT, bool RAGGED>
+// A loading wave's share of a tile's slabs, and its requests.
+template <int BM, int BN, int NL>
+struct RingLoader {
+    static constexpr int A_IT = BM / (8 * NL), B_IT = BN / (8 * NL), STAGE_BYTES = (BM + BN) * kKBlock;
+    static constexpr uint32_t kOutOfRange = 0x80000000u;  // beyond the descriptor's 2^31 - 1 bytes
+    uint32_t a_off[A_IT], b_off[B_IT], lds0;
+    v4i rsrc_a, rsrc_b;
+    int lw, lrow, lj, ljb;
+    __device__ __forceinline__ void init(int wave, int lane, uint32_t lds) {
+        lw = wave, lrow = lane >> 3;
+        lj = (lane & 7) ^ swz16(lrow);
+        ljb = (lane & 7) ^ swz_w(((lw & 1) << 3) | lrow);
+        lds0 = lds + lw * 1024;
+    }
+    __device__ __forceinline__ void set(const Int8GemmParams& p, int64_t m0, int n0, int rows_valid, int expert) {
+#pragma unroll
+        for (int i = 0; i < A_IT; ++i) a_off[i] = (uint32_t)min((i * NL + lw) * 8 + lrow, rows_valid - 1) * (uint32_t)p.K + lj * 16;
+#pragma unroll
+        for (int i = 0; i < B_IT; ++i) b_off[i] = (uint32_t)min((i * NL + lw) * 8 + lrow, p.N - 1 - n0) * (uint32_t)p.K + ljb * 16;
+        rsrc_a = make_rsrc(p.A + m0 * p.K), rsrc_b = make_rsrc(p.B + ((int64_t)expert * p.N + n0) * p.K);
+    }
+    __device__ __forceinline__ void issue(int K, int kstep, int stage) const {
+        const int k0 = kstep * kKBlock;
+        const uint32_t dst = lds0 + stage * STAGE_BYTES;
+        if (k0 + kKBlock <= K) {
+#pragma unroll
+            for (int i = 0; i < B_IT; ++i) direct_load_b128(rsrc_b, dst + BM * kKBlock + i * NL * 1024, b_off[i], k0);
+#pragma unroll
+            for (int i = 0; i < A_IT; ++i) direct_load_b128(rsrc_a, dst + i * NL * 1024, a_off[i], k0);
+        } else {  // the last step of a K that is no multiple of 128: as many loads
+            const bool a_in = k0 + lj * 16 < K, b_in = k0 + ljb * 16 < K;
+#pragma unroll
+            for (int i = 0; i < B_IT; ++i) direct_load_b128(rsrc_b, dst + BM * kKBlock + i * NL * 1024, b_in ? b_off[i] : kOutOfRange, k0);
+#pragma unroll
+            for (int i = 0; i < A_IT; ++i) direct_load_b128(rsrc_a, dst + i * NL * 1024, a_in ? a_off[i] : kOutOfRange, k0);
+        }
+    }
+};
+
+// The wave's part of the tile at (m0, n0), finished and stored: its columns from col_in on, its row groups interleaved with the other waves'.
+template <int TM, int TN, int WGM, bool BIAS>
+__device__ __forceinline__ void ring_store(const Int8GemmParams& p, const RingPart<TM, TN>& part, int64_t m0, int n0, int rows_valid, int wm, int col_in,
+                                           const float* s_row, const float* s_col, const float* s_bias) {
+    constexpr int VECS = RingPart<TM, TN>::VECS;
+    const int li = part.row();
+    auto emit_whole = [&](auto type_tag) __attribute__((always_inline)) {
+        constexpr int OT = decltype(type_tag)::value;
+        constexpr int FV = VECS % 2 == 0 ? 2 : VECS; // vectors whose factors are in registers at a time
+        static_assert(VECS % FV == 0, "whole groups of them");
+#pragma unroll
+        for (int v0 = 0; v0 < VECS; v0 += FV) {
+            float f[FV][8], b[FV][8];
+#pragma unroll
+            for (int v = 0; v < FV; ++v)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int at = col_in + part.column(v0 + v) + i;
+                    f[v][i] = s_col[at];
+                    b[v][i] = BIAS ? s_bias[at] : 0.f;
+                }
+#pragma unroll
+            for (int tm = 0; tm < TM; ++tm) {
+                const int rt = (tm * WGM + wm) * 16 + li;
+                if (rt >= rows_valid) continue;
+                const float sa = s_row[rt];
+#pragma unroll
+                for (int v = 0; v < FV; ++v) {
+                    const int col = n0 + col_in + part.column(v0 + v);
+                    if (col >= p.N) continue;
+                    v4f x, y;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        x[r] = finish(part.get(v0 + v, tm, r), sa, f[v][r], b[v][r]);
+                        y[r] = finish(part.get(v0 + v, tm, 4 + r), sa, f[v][4 + r], b[v][4 + r]);
+                    }
+                    put8<OT>(p.C, (m0 + rt) * p.ldc + col, x, y);
+                }
+            }
+        }
+    };
+    if (p.vec_store) {
+        if (p.out_type == OUT_BF16) emit_whole(std::integral_constant<int, OUT_BF16>{});
+        else if (p.out_type == OUT_F32) emit_whole(std::integral_constant<int, OUT_F32>{});
+        else emit_whole(std::integral_constant<int, OUT_F16>{});
+        return;
+    }
+    // rows of outputs that are no whole vectors: element by element
+#pragma unroll
+    for (int tm = 0; tm < TM; ++tm) {
+        const int rt = (tm * WGM + wm) * 16 + li;
+        if (rt >= rows_valid) continue;
+        const float sa = s_row[rt];
+#pragma unroll
+        for (int v = 0; v < VECS; ++v)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int at = col_in + part.column(v) + i;
+                if (n0 + at < p.N) put1(p, (m0 + rt) * p.ldc + n0 + at, finish(part.get(v, tm, i), sa, s_col[at], BIAS ? s_bias[at] : 0.f));
+            }
+    }
+}
+
+template <int BM, int BN, int STAGES, bool SPLIT>
 __global__ void __launch_bounds__(512, 1) int8_gemm_ring_kernel(const Int8GemmParams p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int NL = 4, WGN = BN == 32 ? 1 : 2, WGM = 4 / WGN;
@@ -119,7 +224,6 @@ __global__ void __launch_bounds__(512, 1) int8_gemm_ring_kernel(const Int8GemmPa
     constexpr int PER_STEP = A_IT + B_IT;
     constexpr int FACTORS = (BM + 2 * BN) * 4;
     static_assert(BM % (16 * WGM) == 0 && STAGES >= 3 && STAGES * STAGE_BYTES + FACTORS <= 160 * 1024, "shape");
-    static_assert(!(SPLIT && RAGGED), "K is split for dense rows only");
 
     __shared__ __align__(1024) uint8_t lds[STAGES * STAGE_BYTES];  // stage s: A slab, then B slab
     // scales of the tile's rows, scales and biases of its columns: brought here while the first steps are on their way
@@ -129,23 +233,15 @@ __global__ void __launch_bounds__(512, 1) int8_gemm_ring_kernel(const Int8GemmPa
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int K = p.K;
     const int tiles_n = (p.N + BN - 1) / BN;
-    int n0, rows_valid, expert = 0;
-    int64_t m0;
-    if constexpr (RAGGED) {
-        int tile_n;
-        if (!ragged_tile<BM, true>(p, (int)blockIdx.x, tiles_n, lane, expert, m0, rows_valid, tile_n)) return;
-        n0 = tile_n * BN;
-    } else {
-        const int tiles_m = (p.M + BM - 1) / BM;
-        const int pid = xcd_remap((int)blockIdx.x, tiles_m * tiles_n);
-        constexpr int GM = 8;
-        const int width = GM * tiles_n;
-        const int group = pid / width, first_m = group * GM;
-        const int gsz = min(tiles_m - first_m, GM);
-        m0 = (int64_t)(first_m + (pid % width) % gsz) * BM;
-        n0 = ((pid % width) / gsz) * BN;
-        rows_valid = (int)min((int64_t)BM, p.M - m0);
-    }
+    const int tiles_m = (p.M + BM - 1) / BM;
+    const int pid = xcd_remap((int)blockIdx.x, tiles_m * tiles_n);
+    constexpr int GM = 8;
+    const int width = GM * tiles_n;
+    const int group = pid / width, first_m = group * GM;
+    const int gsz = min(tiles_m - first_m, GM);
+    const int64_t m0 = (int64_t)(first_m + (pid % width) % gsz) * BM;
+    const int n0 = ((pid % width) / gsz) * BN;
+    const int rows_valid = (int)min((int64_t)BM, p.M - m0);
     int ks = 0, ks_end = (K + kKBlock - 1) / kKBlock;
     if constexpr (SPLIT) {
         ks = blockIdx.y * p.ksteps_per_split;
@@ -163,34 +259,10 @@ __global__ void __launch_bounds__(512, 1) int8_gemm_ring_kernel(const Int8GemmPa
 
     if (wave >= 4) {
         // ------------------------------------------------------------ loading waves
-        const int lw = wave - 4;
-        const int lrow = lane >> 3;
-        const int lj = (lane & 7) ^ swz16(lrow);
-        const int ljb = (lane & 7) ^ swz_w(((lw & 1) << 3) | lrow);
-        constexpr uint32_t kOutOfRange = 0x80000000u;  // beyond the descriptor's 2^31 - 1 bytes
-        uint32_t a_off[A_IT], b_off[B_IT];
-#pragma unroll
-        for (int i = 0; i < A_IT; ++i) a_off[i] = (uint32_t)min((i * NL + lw) * 8 + lrow, rows_valid - 1) * (uint32_t)K + lj * 16;
-#pragma unroll
-        for (int i = 0; i < B_IT; ++i) b_off[i] = (uint32_t)min((i * NL + lw) * 8 + lrow, p.N - 1 - n0) * (uint32_t)K + ljb * 16;
-        const v4i rsrc_a = make_rsrc(p.A + m0 * K), rsrc_b = make_rsrc(p.B + ((int64_t)expert * p.N + n0) * K);
-        const uint32_t lds0 = lds_address(lds) + lw * 1024;
-        auto issue = [&](int kstep, int stage) {
-            const int k0 = min(kstep, last) * kKBlock;
-            const uint32_t dst = lds0 + stage * STAGE_BYTES;
-            if (k0 + kKBlock <= K) {
-#pragma unroll
-                for (int i = 0; i < B_IT; ++i) direct_load_b128(rsrc_b, dst + BM * kKBlock + i * NL * 1024, b_off[i], k0);
-#pragma unroll
-                for (int i = 0; i < A_IT; ++i) direct_load_b128(rsrc_a, dst + i * NL * 1024, a_off[i], k0);
-            } else {  // the last step of a K that is no multiple of 128: as many loads
-                const bool a_in = k0 + lj * 16 < K, b_in = k0 + ljb * 16 < K;
-#pragma unroll
-                for (int i = 0; i < B_IT; ++i) direct_load_b128(rsrc_b, dst + BM * kKBlock + i * NL * 1024, b_in ? b_off[i] : kOutOfRange, k0);
-#pragma unroll
-                for (int i = 0; i < A_IT; ++i) direct_load_b128(rsrc_a, dst + i * NL * 1024, a_in ? a_off[i] : kOutOfRange, k0);
-            }
-        };
+        RingLoader<BM, BN, NL> loader;
+        loader.init(wave - 4, lane, lds_address(lds));
+        loader.set(p, m0, n0, rows_valid, 0);
+        auto issue = [&](int kstep, int stage) { loader.issue(K, min(kstep, last), stage); };
 #pragma unroll
         for (int s = 0; s < STAGES; ++s) issue(ks + s, s);
         __builtin_amdgcn_s_waitcnt(kWaitPro);
@@ -213,11 +285,10 @@ __global__ void __launch_bounds__(512, 1) int8_gemm_ring_kernel(const Int8GemmPa
     const int li = part.row();
 
     if constexpr (!SPLIT) {
-        const float* sb = p.sb + (int64_t)expert * p.N * p.sb_step;
         for (int i = tid; i < BM; i += 256) s_row[i] = p.sa[(m0 + min(i, rows_valid - 1)) * p.sa_step];
         for (int i = tid; i < BN; i += 256) {
             const int col = min(n0 + i, p.N - 1);
-            s_col[i] = sb[(int64_t)col * p.sb_step];
+            s_col[i] = p.sb[(int64_t)col * p.sb_step];
             s_bias[i] = load_bias(p.bias, p.bias_type, col);
         }
     }
@@ -262,60 +333,111 @@ __global__ void __launch_bounds__(512, 1) int8_gemm_ring_kernel(const Int8GemmPa
         }
         return;
     }
-    auto emit_whole = [&](auto type_tag) __attribute__((always_inline)) {
-        constexpr int OT = decltype(type_tag)::value;
-        constexpr int FV = VECS % 2 == 0 ? 2 : VECS; // vectors whose factors are in registers at a time
-        static_assert(VECS % FV == 0, "whole groups of them");
-#pragma unroll
-        for (int v0 = 0; v0 < VECS; v0 += FV) {
-            float f[FV][8], b[FV][8];
-#pragma unroll
-            for (int v = 0; v < FV; ++v)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int at = wn * WTN + part.column(v0 + v) + i;
-                    f[v][i] = s_col[at];
-                    b[v][i] = s_bias[at];
-                }
-#pragma unroll
-            for (int tm = 0; tm < TM; ++tm) {
-                const int rt = (tm * WGM + wm) * 16 + li;
-                if (rt >= rows_valid) continue;
-                const float sa = s_row[rt];
-#pragma unroll
-                for (int v = 0; v < FV; ++v) {
-                    const int col = col0 + part.column(v0 + v);
-                    if (col >= p.N) continue;
-                    v4f x, y;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        x[r] = finish(part.get(v0 + v, tm, r), sa, f[v][r], b[v][r]);
-                        y[r] = finish(part.get(v0 + v, tm, 4 + r), sa, f[v][4 + r], b[v][4 + r]);
-                    }
-                    put8<OT>(p.C, (m0 + rt) * p.ldc + col, x, y);
-                }
+    ring_store<TM, TN, WGM, true>(p, part, m0, n0, rows_valid, wm, wn * WTN, s_row, s_col, s_bias);
+#endif
+}
+
+// The same over the segments of rows that belong to experts, persistent: a workgroup walks tiles b, b + grid, ... of the experts' row tiles x column tiles, and
+// its loading waves run on into the next tile while the others store one (launched tile by tile 64 x 94 rows of (2816, 2048) took 100 us).
+template <int BM, int BN, int STAGES>
+__global__ void __launch_bounds__(512, 1) int8_gemm_ring_experts_kernel(const Int8GemmParams p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int NL = 4, WGN = BN == 32 ? 1 : 2, WGM = 4 / WGN;
+    constexpr int WTN = BN / WGN;
+    constexpr int TM = BM / (16 * WGM), TN = WTN / 16;
+    using Loader = RingLoader<BM, BN, NL>;
+    constexpr int PER_STEP = Loader::A_IT + Loader::B_IT, FACTORS = BM + BN;
+    static_assert(BM <= 256 && BN <= 256 && STAGES * Loader::STAGE_BYTES + 2 * FACTORS * 4 <= 160 * 1024, "shape");
+    constexpr int kPro = (STAGES - 1) * PER_STEP, kLoop = (STAGES - 2) * PER_STEP;  // loads that may stay in flight
+    constexpr int kWaitPro = 0x0F70 | (kPro & 15) | ((kPro >> 4) << 14);
+    constexpr int kWaitLoop = 0x0F70 | (kLoop & 15) | ((kLoop >> 4) << 14);
+    constexpr int kWaitAll = 0x0F70;
+    constexpr int kWaitLds = 0xC07F;
+
+    __shared__ __align__(1024) uint8_t lds[STAGES * Loader::STAGE_BYTES];
+    __shared__ __align__(16) float factors[2][FACTORS];  // scales of a tile's rows, then of its columns; the next tile's beside them
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tiles_n = (p.N + BN - 1) / BN, grid = (int)gridDim.x;
+    RaggedWalk<BM> walk;
+    const int total = walk.start(p, lane, tiles_n);
+    int v = (int)blockIdx.x;
+    if (v >= total) return;
+    const int tiles = (total - v + grid - 1) / grid, nsteps = (p.K + kKBlock - 1) / kKBlock;
+    int expert, m0, rows_valid, tile_n;
+
+    if (wave >= 4) {
+        Loader loader;
+        loader.init(wave - 4, lane, lds_address(lds));
+        int left = tiles, k = 0;
+        auto go = [&]() {
+            walk.find(p, lane, xcd_remap(v, total), tiles_n, expert, m0, rows_valid, tile_n);
+            loader.set(p, m0, tile_n * BN, rows_valid, expert);
+            v += grid;
+        };
+        go();
+        auto issue = [&](int stage) {
+            loader.issue(p.K, k, stage);
+            if (k + 1 < nsteps) {
+                ++k;
+            } else if (left > 1) {  // (behind the last tile's last step: that one again)
+                --left;
+                k = 0;
+                go();
             }
+        };
+#pragma unroll
+        for (int s = 0; s < STAGES; ++s) issue(s);
+        __builtin_amdgcn_s_waitcnt(kWaitPro);
+        __builtin_amdgcn_s_barrier();
+        int stage = 0;
+        for (int64_t s = 0; s < (int64_t)tiles * nsteps; ++s) {
+            __builtin_amdgcn_s_waitcnt(kWaitLoop);
+            __builtin_amdgcn_s_barrier();
+            issue(stage);
+            stage = stage == STAGES - 1 ? 0 : stage + 1;
         }
-    };
-    if (p.vec_store) {
-        if (p.out_type == OUT_BF16) emit_whole(std::integral_constant<int, OUT_BF16>{});
-        else if (p.out_type == OUT_F32) emit_whole(std::integral_constant<int, OUT_F32>{});
-        else emit_whole(std::integral_constant<int, OUT_F16>{});
+        __builtin_amdgcn_s_waitcnt(kWaitAll);
         return;
     }
-    // rows of outputs that are no whole vectors: element by element
-#pragma unroll
-    for (int tm = 0; tm < TM; ++tm) {
-        const int rt = (tm * WGM + wm) * 16 + li;
-        if (rt >= rows_valid) continue;
-        const float sa = s_row[rt];
-#pragma unroll
-        for (int v = 0; v < VECS; ++v)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int at = wn * WTN + part.column(v) + i;
-                if (n0 + at < p.N) put1(p, (m0 + rt) * p.ldc + n0 + at, finish(part.get(v, tm, i), sa, s_col[at], s_bias[at]));
+
+    const int wm = wave % WGM, wn = wave / WGM;
+    RingPart<TM, TN> part;
+    part.init(lane, wm * 16, wn * WTN, BM * kKBlock);
+    __builtin_amdgcn_s_waitcnt(kWaitLds);
+    __builtin_amdgcn_s_barrier();  // step 0 has landed
+    int stage = 0;
+    for (int t = 0; t < tiles; ++t) {
+        walk.find(p, lane, xcd_remap(v, total), tiles_n, expert, m0, rows_valid, tile_n);
+        v += grid;
+        const int n0 = tile_n * BN;
+        // asked for here, in LDS from the tile's last step on
+        const float row = p.sa[((int64_t)m0 + min(tid, rows_valid - 1)) * p.sa_step];
+        const float col = p.sb[((int64_t)expert * p.N + min(n0 + tid, p.N - 1)) * p.sb_step];
+        float* const scales = factors[t & 1];
+        // (again behind the first tile: fragments that lived through the stores would be more than the registers hold)
+        part.template first<WGM>(lds + stage * Loader::STAGE_BYTES);
+        for (int k = 0; k < nsteps; ++k) {
+            if (k == nsteps - 1) {
+                if (tid < BM) scales[tid] = row;
+                if (tid < BN) scales[BM + tid] = col;
             }
+            const uint8_t* cur = lds + stage * Loader::STAGE_BYTES;
+            stage = stage == STAGES - 1 ? 0 : stage + 1;
+            const uint8_t* nxt = lds + stage * Loader::STAGE_BYTES;
+            TG_FENCE();
+            part.before(cur);
+            __builtin_amdgcn_s_waitcnt(kWaitLds);
+            __builtin_amdgcn_s_barrier();
+            TG_FENCE();
+            part.template behind<WGM>(nxt);
+        }
+        part.keep();
+        // (as if written here: what the stores compute from them would be held through all K loops)
+        asm volatile("" : "+v"(part.li), "+v"(part.lg));
+        ring_store<TM, TN, WGM, false>(p, part, m0, n0, rows_valid, wm, wn * WTN, scales, scales + BM, nullptr);
+        part.clear();
     }
 #endif
 }
@@ -325,11 +447,16 @@ inline hipError_t launch_int8_ring(const Int8GemmParams& p, hipStream_t stream) 
     const int64_t cols = ((int64_t)p.N + BN - 1) / BN;
     // ragged: no more row tiles than M rows in E segments can have
     const int64_t tiles = cols * (p.m_indptr ? (int64_t)p.M / BM + (p.E < p.M ? p.E : p.M) : ((int64_t)p.M + BM - 1) / BM);
+    if (p.m_indptr) {
+        if (tiles > INT32_MAX / 2) return hipErrorInvalidValue;
+        const int units = compute_units();
+        hipLaunchKernelGGL((int8_gemm_ring_experts_kernel<BM, BN, STAGES>), dim3((unsigned)(tiles < units ? tiles : units)), dim3(512), 0, stream, p);
+        return hipGetLastError();
+    }
     if (tiles * p.split_k * 512 > kMostThreads) return hipErrorInvalidValue;
     const dim3 grid((unsigned)tiles, p.split_k), block(512);
-    if (p.m_indptr) hipLaunchKernelGGL((int8_gemm_ring_kernel<BM, BN, STAGES, false, true>), grid, block, 0, stream, p);
-    else if (p.split_k > 1) hipLaunchKernelGGL((int8_gemm_ring_kernel<BM, BN, STAGES, true, false>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((int8_gemm_ring_kernel<BM, BN, STAGES, false, false>), grid, block, 0, stream, p);
+    if (p.split_k > 1) hipLaunchKernelGGL((int8_gemm_ring_kernel<BM, BN, STAGES, true>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((int8_gemm_ring_kernel<BM, BN, STAGES, false>), grid, block, 0, stream, p);
     return hipGetLastError();
 }
 
