@@ -1,0 +1,269 @@
+"""The int8 products and the routing as programs call them: through torch's dispatcher, with gradients under capture, over operands past 32-bit offsets, from
+several graphs and streams, and over drawn sizes."""
+
+import gc
+import random
+
+import pytest
+import torch
+
+from tilegym_amd import _lib, ops
+
+from .test_int8_ops import BF16, F16, F32, bits, codes, gen, routing, scales
+
+
+def test_sort_refuses_a_workspace_that_is_too_small():
+    d, L, i32 = _lib._desc, _lib.load(), torch.int32
+    n, experts = 40000, 8
+    need = L.tg_moe_sort_workspace_bytes(n, experts)
+    assert need >= 4 * (experts + 1) and L.tg_moe_sort_workspace_bytes(100, experts) == 0 and L.tg_moe_sort_workspace_bytes(n, 0) == 0
+    ids, ptr, slots = torch.zeros(n, 1, dtype=i32), torch.zeros(experts + 1, dtype=i32), torch.zeros(n, dtype=i32)
+
+    def rc(ws):
+        return L.tg_moe_sort(d(ids), experts, d(ptr), d(slots), d(slots), d(ws), 9999, 0)
+
+    assert rc(None) == -6 and rc(torch.zeros(need - 1, dtype=torch.uint8)) == -6
+    assert rc(torch.zeros(need + 8, dtype=torch.uint8)[8:]) == -6  # not at a 16-byte address
+    assert rc(torch.zeros(need, dtype=torch.uint8)) == -4          # everything is in order up to the device
+
+
+def test_leaf_held():
+    """What a capture asks about a leaf: whether a graph that still lives adds to its gradient."""
+    _lib.load()
+    if _lib.native is None:
+        pytest.skip("needs the native module")
+    x = torch.zeros(3, requires_grad=True)
+    assert not _lib.native.leaf_held(x)
+    y = x * 2
+    assert _lib.native.leaf_held(x) and not _lib.native.leaf_held(torch.zeros(3))
+    del y
+    assert not _lib.native.leaf_held(x)
+
+
+# ---------------------------------------------------------------------------- torch's dispatcher
+def test_operators_infer_shapes_through_torchs_dispatcher():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    t = torch.ops.tilegym_hip
+    with FakeTensorMode():
+        e = lambda *s, dtype=BF16: torch.empty(*s, dtype=dtype, device="cuda")  # noqa: E731
+        i8, i32 = dict(dtype=torch.int8), dict(dtype=torch.int32)
+        c = t.int8_gemm(e(2, 5, 64, **i8), e(24, 64, **i8), e(2, 5, dtype=F32), e(24, dtype=F32), None, F16)
+        assert c.shape == (2, 5, 24) and c.dtype == F16
+        c = t.int8_ragged_gemm(e(10, 64, **i8), e(4, 24, 64, **i8), e(10, dtype=F32), e(4, 24, dtype=F32), e(5, **i32), BF16)
+        assert c.shape == (10, 24) and c.dtype == BF16
+        for got, q_shape in ((t.int8_quant(e(2, 5, 64)), (2, 5, 64)), (t.int8_silu_mul_quant(e(2, 5, 64)), (2, 5, 32))):
+            assert got[0].shape == q_shape and got[0].dtype == torch.int8 and got[1].shape == (2, 5) and got[1].dtype == F32
+        order = t.moe_sort(e(7, 3, dtype=torch.int64), 9)
+        assert [tuple(x.shape) for x in order] == [(10,), (7, 3), (21,)] and all(x.dtype == torch.int32 for x in order)
+        rows = order[1]
+        q, s = t.int8_permute_quant(e(7, 40), rows)
+        assert q.shape == (21, 40) and s.shape == (21,)
+        there = t.moe_permute(e(7, 40), rows)
+        assert there.shape == (21, 40) and t.moe_unpermute(there, rows, None).shape == (7, 40)
+        gx, gw = t.moe_unpermute_backward(e(7, 40), there, rows, e(7, 3, dtype=F32))
+        assert gx.shape == (21, 40) and gx.dtype == BF16 and gw.shape == (7, 3) and gw.dtype == F32
+        for bad in (lambda: t.int8_gemm(e(2, 64, **i8), e(24, 32, **i8), e(2, dtype=F32), e(24, dtype=F32), None, F16), lambda: t.int8_silu_mul_quant(e(2, 63)),
+                    lambda: t.moe_permute(e(6, 40), rows), lambda: t.moe_unpermute(e(7, 40), rows, None)):
+            with pytest.raises(ValueError):
+                bad()
+    with pytest.raises(NotImplementedError):
+        t.int8_quant(torch.zeros(2, 8))
+
+
+@pytest.mark.gpu
+def test_operators_through_torchs_dispatcher(device):
+    """The bits of the direct calls, and the same gradients."""
+    tokens, experts, k, h = 40, 8, 3, 256
+    t = torch.ops.tilegym_hip
+    ids, x = routing(tokens, experts, k, 1, absent=True).to(device), torch.randn(tokens, h, generator=gen(2)).to(BF16).to(device)
+    w, g = torch.rand(tokens, k, generator=gen(3)).to(device), torch.randn(tokens, h, generator=gen(4)).to(BF16).to(device)
+    b, sb = codes((experts, 64, h), 5).to(device), scales((experts, 64), 6).to(device)
+    order = ops.moe_sort(ids, experts)
+    assert all(torch.equal(a, o) for a, o in zip(t.moe_sort(ids, experts), order))
+    q, s = ops.moe_permute_quant_int8(x, order)
+    assert all(torch.equal(a, o) for a, o in zip(t.int8_permute_quant(x, order.rows), (q, s)))
+    live = int(order.indptr[-1])
+    y = t.int8_ragged_gemm(q, b, s, sb, order.indptr, BF16)
+    assert torch.equal(bits(y[:live]), bits(ops.ragged_int8_matmul(q, b, s, sb, order.indptr)[:live])) and not bool(y[live:].any())
+    assert torch.equal(t.int8_gemm(q, b[0], s, sb[0], None, F32), ops.int8_matmul(q, b[0], s, sb[0], out_dtype=F32))
+    for got, want in ((t.int8_quant(x), ops.quant_int8(x)), (t.int8_silu_mul_quant(x), ops.silu_mul_quant_int8(x))):
+        assert all(torch.equal(a, o) for a, o in zip(got, want))
+
+    grads = []
+    for permute, unpermute in ((lambda v: ops.moe_permute(v, order), lambda v, u: ops.moe_unpermute(v, order, u)),
+                               (lambda v: t.moe_permute(v, order.rows), lambda v, u: t.moe_unpermute(v, order.rows, u))):
+        xl, wl = x.clone().requires_grad_(), w.clone().requires_grad_()
+        out = unpermute(permute(xl), wl)
+        plain = unpermute(permute(xl), None)
+        grads.append((out.detach(), plain.detach(), *torch.autograd.grad((out, plain), (xl, wl), (g, g))))
+    assert all(torch.equal(a, o) for a, o in zip(*grads))
+    torch.library.opcheck(t.moe_permute.default, (x.clone().requires_grad_(), order.rows))
+    torch.library.opcheck(t.moe_unpermute.default, (ops.moe_permute(x, order).requires_grad_(), order.rows, w.clone().requires_grad_()))
+
+
+# ---------------------------------------------------------------------------- gradients under capture
+@pytest.mark.gpu
+def test_forward_and_backward_captured(device):
+    """A training step's forward and backward passes in one graph, replayed over new inputs with eager steps between; while an eager graph of a leaf
+    lives, the capture is refused."""
+    tokens, experts, k, h = 30, 8, 2, 128
+    order = ops.moe_sort(routing(tokens, experts, k, 1).to(device), experts)
+    x = torch.randn(tokens, h, generator=gen(1)).to(device).requires_grad_()
+    w = torch.rand(tokens, k, generator=gen(2)).to(device).requires_grad_()
+    g = torch.randn(tokens, h, generator=gen(3)).to(device)
+
+    def step():
+        return torch.autograd.grad(ops.moe_unpermute(ops.moe_permute(x, order) * 2, order, w), (x, w), g)
+
+    held = ops.moe_permute(x, order), ops.moe_unpermute(ops.moe_permute(x.detach(), order), order, w)
+    torch.cuda.synchronize()
+    for call in (lambda: ops.moe_permute(x, order), lambda: ops.moe_unpermute(ops.moe_permute(g, order), order, w)):
+        with pytest.raises(RuntimeError, match="eager graph of this leaf"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                torch.zeros(1, device=device)
+                call()
+    del held
+    gc.collect()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grads = step()
+    for seed in range(4, 8):
+        with torch.no_grad():
+            x.copy_(torch.randn(tokens, h, generator=gen(seed)))
+            w.copy_(torch.rand(tokens, k, generator=gen(seed + 1)))
+            g.copy_(torch.randn(tokens, h, generator=gen(seed + 2)))
+        graph.replay()
+        got = [t.clone() for t in grads]
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---------------------------------------------------------------------------- several graphs
+@pytest.mark.gpu
+def test_two_graphs_replayed_at_once(device):
+    """Graphs captured on one stream and replayed on two keep their scratch memory (a split K's partial sums, a long sort's counts) apart."""
+    a, b = [codes((20, 4096), s).to(device) for s in (1, 2)], codes((256, 4096), 3).to(device)
+    one = torch.full((1,), 0.01, device=device)
+    ids = [torch.randint(0, 16, (20000, 2), generator=gen(s), dtype=torch.int32).to(device) for s in (4, 5)]
+    cfg = dict(KERNEL="tiled", BLOCK_M=32, BLOCK_N=64, SPLIT_K=8)
+
+    def run(i):
+        return [(ops.int8_matmul(a[i], b, one, one, kernel_configs=cfg), *ops.moe_sort(ids[i], 16)) for _ in range(4)]
+
+    want = [[[t.clone() for t in r] for r in run(i)] for i in (0, 1)]
+    assert _lib.last_config() is not None and _lib.load().tg_moe_sort_workspace_bytes(40000, 16) > 0
+    graphs, held = [], []
+    for i in (0, 1):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held.append(run(i))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(10):
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for h, w in zip(held, want):
+            assert all(torch.equal(x, y) for r, s in zip(h, w) for x, y in zip(r, s))
+
+
+# ---------------------------------------------------------------------------- offsets past 32 bits
+@pytest.mark.gpu
+def test_rows_past_32_bit_offsets(device):
+    """2.3 GB of rows against a small weight, and outputs of as many bytes: the last rows are those of a call over them alone."""
+    k, n = 16384, 256
+    m = 140_000
+    a = torch.randint(-128, 128, (m, k), dtype=torch.int8, device=device)
+    b, sa, sb = codes((n, k), 2).to(device), scales(m, 3).to(device), scales(n, 4).to(device)
+    last = slice(m - 300, m)
+    want = ops.int8_matmul(a[last].contiguous(), b, sa[last].contiguous(), sb)
+    assert torch.equal(ops.int8_matmul(a, b, sa, sb)[last], want)
+    for cfg in (dict(KERNEL="tiled", BLOCK_M=256, BLOCK_N=128), dict(KERNEL="fallback")):
+        assert torch.equal(ops.int8_matmul(a, b, sa, sb, kernel_configs=cfg)[last], want)
+    indptr = torch.tensor([0, 100, m - 300, m], dtype=torch.int32, device=device)
+    b3, sb3 = torch.stack([b.flip(0), b.flip(1), b]), torch.stack([sb, sb, sb])
+    for cfg in (None, dict(KERNEL="tiled", BLOCK_M=192, BLOCK_N=192), dict(KERNEL="tiled", BLOCK_M=256, BLOCK_N=256)):
+        assert torch.equal(ops.ragged_int8_matmul(a, b3, sa, sb3, indptr, kernel_configs=cfg)[last], want)
+    del a, b3
+    # a weight of more bytes, its last rows
+    b = torch.randint(-128, 128, (m, k), dtype=torch.int8, device=device)
+    x, one = codes((40, k), 5).to(device), torch.full((1,), 0.01, device=device)
+    want = ops.int8_matmul(x, b[last].contiguous(), one, sa[last].contiguous())
+    assert torch.equal(ops.int8_matmul(x, b, one, sa)[:, last], want)
+    assert torch.equal(ops.int8_matmul(x[:9], b, one, sa)[:, last], want[:9])
+    # experts whose weights lie past them: rows of the last one
+    e = torch.tensor([0] * 140 + [40], dtype=torch.int32, device=device)
+    w = b.view(140, 1000, k)
+    want = ops.int8_matmul(x, w[-1].contiguous(), one, one)
+    for rows in (40, 7):
+        e[-1] = rows
+        assert torch.equal(ops.ragged_int8_matmul(x[:rows].contiguous(), w, one, one, e), want[:rows])
+
+
+@pytest.mark.gpu
+def test_routing_past_32_bit_offsets(device):
+    tokens, k, h = 70_000, 8, 4096  # 560 000 rows of 4096
+    ids = torch.randint(0, 64, (tokens, k), dtype=torch.int32, device=device)
+    order = ops.moe_sort(ids, 64)
+    x = torch.randint(0, 256, (tokens, 1), device=device).to(BF16).expand(tokens, h).contiguous()
+    there = ops.moe_permute(x, order)
+    slots = order.slots.long()
+    assert torch.equal(there[:, 0], x[slots // k, 0]) and torch.equal(there[:, -1], x[slots // k, -1])
+    q, s = ops.moe_permute_quant_int8(x, order)
+    want = ops.quant_int8(x)
+    assert torch.equal(q[:, -1], want[0][slots // k, -1]) and torch.equal(s, want[1][slots // k])
+    w = torch.ones(tokens, k, device=device)
+    assert torch.equal(ops.moe_unpermute(there, order, w), x * k)
+    gx, gw = ops.moe_unpermute_backward(x, there, order, w)
+    assert torch.equal(gx[:, -1], there[:, -1])
+    assert torch.equal(gw, (x[:, :1].float() ** 2 * h).expand(tokens, k))  # (sums of equal powers of 2 ** 12 products: exact)
+    q, s = ops.silu_mul_quant_int8(there)
+    assert torch.equal(q[-5:], ops.silu_mul_quant_int8(there[-5:].contiguous())[0])
+
+
+# ---------------------------------------------------------------------------- drawn sizes
+def _exact(a, b, sa, sb, t):
+    """The kernels' fp32 steps on the exact sum, on the GPU (sums of integers below 2^31 are exact in float64)."""
+    return ((a.double() @ b.double().t()).float() * sa[:, None] * sb).to(t)
+
+
+@pytest.mark.gpu
+def test_drawn_products(device):
+    rng = random.Random(3)
+    for i in range(60):
+        m = rng.choice((1, 2, 13, 16, 17, 31, 32, 33, 70, 150, 333, 700, 1500, 4000))
+        n, k = rng.choice((8, 64, 72, 500, 1000, 2000, 4104)), rng.choice((16, 144, 256, 1000, 1024, 2064, 4096))
+        t = rng.choice((BF16, F16, F32))
+        a, b = codes((m, k), i).to(device), codes((n, k), i + 1).to(device)
+        sa, sb = scales(m, i + 2).to(device), scales(n, i + 3).to(device)
+        got = ops.int8_matmul(a, b, sa, sb, out_dtype=t)
+        assert torch.equal(bits(got), bits(_exact(a, b, sa, sb, t))), (m, n, k, t, _lib.last_config())
+
+
+@pytest.mark.gpu
+def test_drawn_products_over_experts(device):
+    rng = random.Random(4)
+    for i in range(40):
+        experts, rows = rng.choice((1, 3, 8, 60, 130)), rng.choice((1, 10, 100, 500, 3000, 9000))
+        n, k = rng.choice((8, 64, 264, 500, 1408)), rng.choice((16, 256, 400, 1024, 1408))
+        ids = torch.randint(-1, experts, (rows, 1), generator=gen(i), dtype=torch.int32).to(device)
+        if rng.random() < 0.3:
+            ids[:rows // 2] = 0
+        order = ops.moe_sort(ids, experts)
+        a, b = codes((rows, k), i).to(device), codes((experts, n, k), i + 1).to(device)
+        sa, sb = scales(rows, i + 2).to(device), scales((experts, n), i + 3).to(device)
+        out = torch.full((rows, n), 5.0, dtype=BF16, device=device)
+        ops.ragged_int8_matmul(a, b, sa, sb, order.indptr, out=out)
+        ptr = order.indptr.tolist()
+        for e in range(experts):
+            part = slice(ptr[e], ptr[e + 1])
+            assert torch.equal(bits(out[part]), bits(_exact(a[part], b[e], sa[part], sb[e], BF16))), (experts, rows, n, k, e, _lib.last_config())
+        assert bool((out[ptr[-1]:] == 5).all())

@@ -15,7 +15,9 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include "../../include/tilegym_hip.h"
 
@@ -734,6 +736,19 @@ PyObject* py_moe_unpermute_backward(PyObject*, PyObject* const* args, Py_ssize_t
     END_HANDLE_TH_ERRORS
 }
 
+// leaf_held(t) -> whether a graph that still lives accumulates into the leaf t on another stream than the current one
+PyObject* py_leaf_held(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const at::Tensor* t = n == 1 ? tensor_of(args[0]) : nullptr;
+    if (!t) { PyErr_SetString(PyExc_TypeError, "leaf_held takes a tensor"); return nullptr; }
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    if (!node) Py_RETURN_FALSE;
+    const auto stream = node->stream();
+    if (t->is_cuda() && stream && *stream == c10::hip::getCurrentHIPStream(t->get_device()).unwrap()) Py_RETURN_FALSE;
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
 // set_up({name: address}, workspaces, workspace_for, check_rc)
 PyObject* py_set_up(PyObject*, PyObject* args) {
     PyObject *table, *workspaces, *workspace_for, *check_rc;
@@ -782,6 +797,7 @@ PyMethodDef kMethods[] = {TG_FAST("matmul", py_matmul),
                           TG_FAST("moe_permute", py_moe_permute),
                           TG_FAST("moe_unpermute", py_moe_unpermute),
                           TG_FAST("moe_unpermute_backward", py_moe_unpermute_backward),
+                          TG_FAST("leaf_held", py_leaf_held),
                           {"set_up", py_set_up, METH_VARARGS, nullptr},
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

@@ -2356,13 +2356,16 @@ static Int8Schedule cheapest_int8(const tg::Int8GemmParams& p, int64_t partial_b
 }
 
 // Rows of experts, which the host knows the number of, not how they are spread.  The streaming form up to 12 rows per expert on average (it reads the weights of
-// the experts that have rows once per 16 rows); above, the tiles by a model of the form above over the row tiles to be expected, fitted to 3600 problems
-// (1 to 30 000 rows over 4 to 128 experts, spread evenly to e^1.5 : 1), its 256 x 256 row to 3000 (500 to 60 000 rows): 3.9 % and 3.5 % behind the best form on
-// average, 95 of 100 within 1.26 and 1.22 x.
-constexpr Int8Cost kInt8Ragged[] = {{32, 64, 0.134f, 0.139f, 4.512f, 0.114f}, {64, 32, 0.137f, 0.121f, 4.458f, 0.068f}, {64, 64, 0.149f, 0.172f, 4.557f, 0.122f},
-                                    {64, 128, 0.218f, 0.261f, 4.680f, 0.222f}, {96, 128, 0.345f, 0.378f, 4.506f, 0.169f}, {128, 128, 0.389f, 0.491f, 5.001f, 0.126f},
-                                    {160, 128, 0.424f, 0.589f, 5.501f, 0.104f}, {160, 192, 0.516f, 0.735f, 6.785f, 0.174f}, {256, 128, 0.556f, 0.828f, 6.743f, 0.078f},
-                                    {192, 192, 0.586f, 0.841f, 7.512f, 0.156f}, {256, 256, 0.918f, 1.362f, 9.757f, 0.212f}};
+// the experts that have rows once per 16 rows); above, the tiles by a model of the form above over the row tiles to be expected, persistent: a launch costs `fixed`,
+// a round `round` more than its steps.  Fitted to 6500 problems (30 to 60 000 rows over 4 to 128 experts, spread evenly to e^1.5 : 1): 3.1 % behind the
+// best form on average, 95 of 100 within 1.21 x.
+struct Int8RaggedCost { int bm, bn; float first, full, round, fixed, memory; };
+constexpr Int8RaggedCost kInt8Ragged[] = {{32, 64, 0.069f, 0.125f, 1.265f, 4.544f, 0.162f}, {64, 32, 0.085f, 0.140f, 1.184f, 4.469f, 0.100f},
+                                          {64, 64, 0.097f, 0.159f, 1.610f, 4.206f, 0.171f}, {64, 128, 0.152f, 0.295f, 2.137f, 3.857f, 0.220f},
+                                          {96, 128, 0.228f, 0.409f, 1.919f, 3.993f, 0.119f}, {128, 128, 0.283f, 0.512f, 2.266f, 4.012f, 0.098f},
+                                          {160, 128, 0.328f, 0.613f, 2.621f, 3.971f, 0.066f}, {160, 192, 0.461f, 0.757f, 3.782f, 3.681f, 0.103f},
+                                          {256, 128, 0.496f, 0.894f, 3.750f, 3.684f, 0.000f}, {192, 192, 0.530f, 0.884f, 4.253f, 3.715f, 0.073f},
+                                          {256, 256, 0.702f, 1.420f, 7.589f, 2.512f, 0.100f}};
 constexpr int64_t kInt8StreamRowsPerExpert = 12;
 
 static Int8Schedule cheapest_int8_ragged(const tg::Int8GemmParams& p) {
@@ -2372,11 +2375,11 @@ static Int8Schedule cheapest_int8_ragged(const tg::Int8GemmParams& p) {
     const float from_memory = (float)std::min(std::max((used * N * K - 8e6) / 40e6, 0.), 1.);
     Int8Schedule best{0, -1, -1, 1};
     float best_us = 0.f;
-    for (const Int8Cost& t : kInt8Ragged) {
+    for (const Int8RaggedCost& t : kInt8Ragged) {
         if (!int8_takes(p, Int8Schedule{1, t.bm, t.bn, 1})) continue;
         const double tiles = (M / t.bm + std::min(M, E) * 0.5) * (double)cdiv(p.N, t.bn), rounds = tiles / 256;
         const double whole = rounds <= 2 ? std::ceil(rounds) : (rounds + std::ceil(rounds)) / 2;
-        const float us = (float)whole * ((float)(K / 128) * (t.first + (t.full - t.first) * (float)std::min(1., rounds) + t.memory * from_memory) + t.fixed);
+        const float us = t.fixed + (float)whole * ((float)(K / 128) * (t.first + (t.full - t.first) * (float)std::min(1., rounds) + t.memory * from_memory) + t.round);
         if (best.kernel == 0 || us < best_us) { best = Int8Schedule{1, t.bm, t.bn, 1}; best_us = us; }
     }
     return best;

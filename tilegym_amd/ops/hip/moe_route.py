@@ -45,6 +45,18 @@ def _unpermute(x, order, weights, where="moe_unpermute"):
     return out
 
 
+def _recordable(where, *leaves):
+    """Under capture a leaf's gradient is added to on the stream of the graph that first used it.  Where that is an eager graph which still lives, the backward
+    pass would wait for its stream from within the capture, an error that torch's backward threads do not survive: refused here instead."""
+    if not torch.cuda.is_current_stream_capturing():
+        return
+    for t in leaves:
+        if t is not None and t.requires_grad and t.is_leaf and (not _lib.native_path() or _lib.native.leaf_held(t)):
+            raise RuntimeError(f"{where}: an eager graph of this leaf is alive on another stream; release what it computed (its loss, its outputs) before "
+                               f"the leaf's forward and backward passes are captured" if _lib.native_path() else
+                               f"{where}: without tilegym_amd/_native.so no graph is captured whose leaves take gradients")
+
+
 class _Permute(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, indptr, rows, slots):
@@ -93,6 +105,7 @@ def moe_sort(topk_ids, num_experts):
 @register_impl("moe_permute", backend="hip")
 def moe_permute(x, order):
     if torch.is_grad_enabled() and x.requires_grad:
+        _recordable("moe_permute", x)
         return _Permute.apply(x, *order)
     return _permute(x, order)
 
@@ -116,6 +129,7 @@ def moe_permute_quant_int8(x, order):
 @register_impl("moe_unpermute", backend="hip")
 def moe_unpermute(x, order, weights=None):
     if torch.is_grad_enabled() and (x.requires_grad or (weights is not None and weights.requires_grad)):
+        _recordable("moe_unpermute", x, weights)
         return _Unpermute.apply(x, weights, *order)
     return _unpermute(x, order, weights)
 

@@ -22,7 +22,14 @@ They are registered for device tensors only: with CPU tensors the dispatcher rai
     fp8_kv_read(k_cache, v_cache, k_scale, v_scale, block_table, indptr, total_tokens, out_dtype) -> (k, v)    tg_fp8_kv_read
     fp8_kv_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, indptr, sm_scale, window, sink_tokens) -> out
                                                                                         tg_fp8_kv_attention
-What the last five take and leave unset is said at ``tilegym_amd.ops``.
+    int8_gemm(a, b, scale_a, scale_b, bias, out_dtype) -> c                             tg_int8_gemm
+    int8_ragged_gemm(a, b, scale_a, scale_b, m_indptr, out_dtype) -> c                  tg_int8_ragged_gemm, rows of no expert zero
+    int8_quant(x) -> (q, scales); int8_silu_mul_quant(x) -> (q, scales)                 tg_int8_quant
+    int8_permute_quant(x, rows) -> (q, scales)                                          tg_int8_quant, rows carried to their experts
+    moe_sort(topk_ids, num_experts) -> (indptr, rows, slots)                            tg_moe_sort
+    moe_permute(x, rows) -> out; moe_unpermute(x, rows, weights) -> out                 tg_moe_permute, tg_moe_unpermute; differentiable
+    moe_unpermute_backward(grad_out, x, rows, weights) -> (grad_x, grad_weights)        tg_moe_unpermute_backward
+What all but the first six take and leave unset is said at ``tilegym_amd.ops``.
 """
 
 from __future__ import annotations
@@ -35,7 +42,8 @@ from . import _lib
 
 NAMESPACE = "tilegym_hip"
 OP_NAMES = ("fp8_gemm", "fp8_gemm_out", "fp8_ragged_gemm", "fp8_moe_gemm_out", "fp8_quant_1x128", "fp8_fused_moe", "fp8_rms_norm_quant",
-            "fp8_kv_append", "fp8_kv_append_turn", "fp8_kv_read", "fp8_kv_attention")
+            "fp8_kv_append", "fp8_kv_append_turn", "fp8_kv_read", "fp8_kv_attention", "int8_gemm", "int8_ragged_gemm", "int8_quant", "int8_silu_mul_quant",
+            "int8_permute_quant", "moe_sort", "moe_permute", "moe_unpermute", "moe_unpermute_backward")
 _CACHE = ("k_cache", "v_cache", "k_scale", "v_scale")
 
 
@@ -218,6 +226,155 @@ def fp8_kv_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
 def _(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, indptr, sm_scale, window, sink_tokens):
     _check_heads(k_cache, q, "fp8_kv_attention")
     return q.new_empty(q.shape)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::int8_gemm", mutates_args=(), device_types="cuda")
+def int8_gemm(a: torch.Tensor, b: torch.Tensor, scale_a: torch.Tensor, scale_b: torch.Tensor, bias: Optional[torch.Tensor], out_dtype: torch.dtype) -> torch.Tensor:
+    from .ops import int8_matmul
+    return int8_matmul(a, b, scale_a, scale_b, bias=bias, out_dtype=out_dtype)
+
+
+@int8_gemm.register_fake
+def _(a, b, scale_a, scale_b, bias, out_dtype):
+    if a.dim() < 1 or b.dim() != 2 or a.shape[-1] != b.shape[1]:
+        raise ValueError("int8_gemm expects a (..., K) and b (N, K)")
+    return a.new_empty(a.shape[:-1] + b.shape[:1], dtype=out_dtype)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::int8_ragged_gemm", mutates_args=(), device_types="cuda")
+def int8_ragged_gemm(a: torch.Tensor, b: torch.Tensor, scale_a: torch.Tensor, scale_b: torch.Tensor, m_indptr: torch.Tensor,
+                     out_dtype: torch.dtype) -> torch.Tensor:
+    from .ops import ragged_int8_matmul
+    out = torch.zeros((a.shape[0], b.shape[1]), dtype=out_dtype, device=a.device)
+    return ragged_int8_matmul(a, b, scale_a, scale_b, m_indptr, out_dtype=out_dtype, out=out)
+
+
+@int8_ragged_gemm.register_fake
+def _(a, b, scale_a, scale_b, m_indptr, out_dtype):
+    if a.dim() != 2 or b.dim() != 3 or a.shape[1] != b.shape[2]:
+        raise ValueError("int8_ragged_gemm expects a (rows, K) and b (experts, N, K)")
+    return a.new_empty((a.shape[0], b.shape[1]), dtype=out_dtype)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::int8_quant", mutates_args=(), device_types="cuda")
+def int8_quant(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    from .ops import quant_int8
+    return quant_int8(x)
+
+
+@int8_quant.register_fake
+def _(x):
+    return x.new_empty(x.shape, dtype=torch.int8), x.new_empty(x.shape[:-1], dtype=torch.float32)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::int8_silu_mul_quant", mutates_args=(), device_types="cuda")
+def int8_silu_mul_quant(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    from .ops import silu_mul_quant_int8
+    return silu_mul_quant_int8(x)
+
+
+@int8_silu_mul_quant.register_fake
+def _(x):
+    if x.shape[-1] % 2 != 0:
+        raise ValueError("int8_silu_mul_quant expects x (..., 2 I)")
+    return x.new_empty(x.shape[:-1] + (x.shape[-1] // 2,), dtype=torch.int8), x.new_empty(x.shape[:-1], dtype=torch.float32)
+
+
+def _order_of(rows):
+    """The operators over a MoeOrder read its rows only."""
+    from .ops import MoeOrder
+    return MoeOrder(rows, rows, rows)
+
+
+def _check_rows(name: str, x: torch.Tensor, rows: torch.Tensor, n) -> None:
+    if x.dim() != 2 or rows.dim() != 2 or x.shape[0] != n:
+        raise ValueError(f"{name}: x {tuple(x.shape)} does not go with rows {tuple(rows.shape)}")
+
+
+@torch.library.custom_op(f"{NAMESPACE}::int8_permute_quant", mutates_args=(), device_types="cuda")
+def int8_permute_quant(x: torch.Tensor, rows: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    from .ops import moe_permute_quant_int8
+    return moe_permute_quant_int8(x, _order_of(rows))
+
+
+@int8_permute_quant.register_fake
+def _(x, rows):
+    _check_rows("int8_permute_quant", x, rows, rows.shape[0])
+    return x.new_empty((rows.numel(), x.shape[1]), dtype=torch.int8), x.new_empty((rows.numel(),), dtype=torch.float32)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::moe_sort", mutates_args=(), device_types="cuda")
+def moe_sort(topk_ids: torch.Tensor, num_experts: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    from .ops import moe_sort as sort
+    return tuple(sort(topk_ids, num_experts))
+
+
+@moe_sort.register_fake
+def _(topk_ids, num_experts):
+    i32 = dict(dtype=torch.int32)
+    return topk_ids.new_empty((num_experts + 1,), **i32), topk_ids.new_empty(topk_ids.shape, **i32), topk_ids.new_empty((topk_ids.numel(),), **i32)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::moe_permute", mutates_args=(), device_types="cuda")
+def moe_permute(x: torch.Tensor, rows: torch.Tensor) -> torch.Tensor:
+    from .ops import moe_permute as permute
+    return permute(x, _order_of(rows))
+
+
+@moe_permute.register_fake
+def _(x, rows):
+    _check_rows("moe_permute", x, rows, rows.shape[0])
+    return x.new_empty((rows.numel(), x.shape[1]))
+
+
+@torch.library.custom_op(f"{NAMESPACE}::moe_unpermute", mutates_args=(), device_types="cuda")
+def moe_unpermute(x: torch.Tensor, rows: torch.Tensor, weights: Optional[torch.Tensor]) -> torch.Tensor:
+    from .ops import moe_unpermute as unpermute
+    return unpermute(x, _order_of(rows), weights)
+
+
+@moe_unpermute.register_fake
+def _(x, rows, weights):
+    _check_rows("moe_unpermute", x, rows, rows.numel())
+    return x.new_empty((rows.shape[0], x.shape[1]))
+
+
+@torch.library.custom_op(f"{NAMESPACE}::moe_unpermute_backward", mutates_args=(), device_types="cuda")
+def moe_unpermute_backward(grad_out: torch.Tensor, x: torch.Tensor, rows: torch.Tensor, weights: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    from .ops import moe_unpermute_backward as backward
+    return backward(grad_out, x, _order_of(rows), weights)
+
+
+@moe_unpermute_backward.register_fake
+def _(grad_out, x, rows, weights):
+    _check_rows("moe_unpermute_backward", x, rows, rows.numel())
+    return x.new_empty(x.shape), weights.new_empty(weights.shape)
+
+
+def _save_permute(ctx, inputs, output):
+    ctx.save_for_backward(inputs[1])
+
+
+def _save_unpermute(ctx, inputs, output):
+    x, rows, weights = inputs
+    ctx.weighted = weights is not None
+    ctx.save_for_backward(rows, *([x, weights] if ctx.weighted else []))
+
+
+def _grad_permute(ctx, grad):
+    return torch.ops.tilegym_hip.moe_unpermute(grad.contiguous(), ctx.saved_tensors[0], None), None
+
+
+def _grad_unpermute(ctx, grad):
+    rows = ctx.saved_tensors[0]
+    if not ctx.weighted:
+        return torch.ops.tilegym_hip.moe_permute(grad.contiguous(), rows), None, None
+    grad_x, grad_weights = torch.ops.tilegym_hip.moe_unpermute_backward(grad, ctx.saved_tensors[1], rows, ctx.saved_tensors[2])
+    return grad_x, None, grad_weights
+
+
+moe_permute.register_autograd(_grad_permute, setup_context=_save_permute)
+moe_unpermute.register_autograd(_grad_unpermute, setup_context=_save_unpermute)
 
 
 def registered_ops():
