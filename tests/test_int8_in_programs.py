@@ -27,6 +27,14 @@ def test_sort_refuses_a_workspace_that_is_too_small():
     assert rc(torch.zeros(need, dtype=torch.uint8)) == -4          # everything is in order up to the device
 
 
+def test_tensors_without_elements_are_contiguous():
+    """Whatever their strides: an expanded gradient of no tokens, say."""
+    d = _lib._desc
+    x = torch.zeros(1, 1).expand(0, 16)
+    assert x.stride() == (0, 0) or x.is_contiguous()
+    assert _lib.load().tg_int8_quant(d(torch.zeros(0, 16, dtype=torch.int8)), d(torch.zeros(0)), d(x), None, 0, 9999, 0) == 0
+
+
 def test_leaf_held():
     """What a capture asks about a leaf: whether a graph that still lives adds to its gradient."""
     _lib.load()
@@ -227,6 +235,53 @@ def test_routing_past_32_bit_offsets(device):
     assert torch.equal(gw, (x[:, :1].float() ** 2 * h).expand(tokens, k))  # (sums of equal powers of 2 ** 12 products: exact)
     q, s = ops.silu_mul_quant_int8(there)
     assert torch.equal(q[-5:], ops.silu_mul_quant_int8(there[-5:].contiguous())[0])
+
+
+# ---------------------------------------------------------------------------- nothing to do
+@pytest.mark.gpu
+def test_empty_sizes(device):
+    f32 = lambda *s: torch.ones(*s, device=device)  # noqa: E731
+    i8 = lambda *s: torch.zeros(*s, dtype=torch.int8, device=device)  # noqa: E731
+    for tokens, k, h in ((0, 2, 64), (3, 0, 64), (3, 2, 0), (0, 0, 0)):
+        order = ops.moe_sort(torch.zeros(tokens, k, dtype=torch.int32, device=device), 4)
+        assert order.indptr.tolist() == [0] + [tokens * k] * 4
+        x, y, w = f32(tokens, h), f32(tokens * k, h), f32(tokens, k)
+        assert torch.equal(ops.moe_permute(x, order), y)
+        assert torch.equal(ops.moe_unpermute(y, order), x * k) and torch.equal(ops.moe_unpermute(y, order, w), x * k)
+        gx, gw = ops.moe_unpermute_backward(x, y, order, w)
+        assert torch.equal(gx, y) and torch.equal(gw, w * h)
+        if h:
+            q, s = ops.moe_permute_quant_int8(x, order)
+            assert q.shape == (tokens * k, h) and s.shape == (tokens * k,)
+            xl = x.clone().requires_grad_()
+            ops.moe_unpermute(ops.moe_permute(xl, order), order, w).sum().backward()
+            assert torch.equal(xl.grad, x * k)
+    assert ops.int8_matmul(i8(0, 64), i8(24, 64), f32(1), f32(24)).shape == (0, 24)
+    assert ops.int8_matmul(i8(5, 64), i8(0, 64), f32(5), f32(1)).shape == (5, 0)
+    assert ops.ragged_int8_matmul(i8(0, 64), i8(4, 24, 64), f32(0), f32(4, 24), torch.zeros(5, dtype=torch.int32, device=device)).shape == (0, 24)
+    out = torch.full((6, 24), 3.0, dtype=BF16, device=device)
+    ops.ragged_int8_matmul(i8(6, 64), i8(0, 24, 64), f32(6), f32(1), torch.zeros(1, dtype=torch.int32, device=device), out=out)
+    assert bool((out == 3).all())  # rows of no expert, as there is none
+    assert ops.quant_int8(f32(0, 64))[1].shape == (0,) and ops.silu_mul_quant_int8(f32(0, 64))[0].shape == (0, 32)
+    none = torch.zeros(0, 2, dtype=torch.int32, device=device)
+    assert ops.int8_moe(f32(0, 64).to(BF16), i8(4, 64, 64), i8(4, 64, 32), f32(4, 64), f32(4, 64), f32(0, 2), none).shape == (0, 64)
+    # a layer none of whose experts is here
+    ids = torch.full((5, 2), -1, dtype=torch.int32, device=device)
+    made = ops.int8_moe(f32(5, 64).to(BF16), i8(4, 64, 64), i8(4, 64, 32), f32(4, 64), f32(4, 64), f32(5, 2), ids)
+    assert not bool(made.any())
+
+
+@pytest.mark.gpu
+def test_forced_streaming_over_more_passes_than_a_grid_has(device):
+    """2^20 rows and more of few experts: the streaming form does not take them, the call still answers."""
+    rows = 65600 * 16
+    a, b = torch.randint(-128, 128, (rows, 16), dtype=torch.int8, device=device), codes((2, 8, 16), 1).to(device)
+    sa, sb = torch.rand(rows, device=device), scales((2, 8), 2).to(device)
+    ptr = torch.tensor([0, 100, rows], dtype=torch.int32, device=device)
+    got = ops.ragged_int8_matmul(a, b, sa, sb, ptr, kernel_configs=dict(KERNEL="stream"))
+    assert _lib.last_config()["KERNEL"] != 3
+    assert torch.equal(bits(got[:100]), bits(_exact(a[:100], b[0], sa[:100], sb[0], BF16)))
+    assert torch.equal(bits(got[100:]), bits(_exact(a[100:], b[1], sa[100:], sb[1], BF16)))
 
 
 # ---------------------------------------------------------------------------- drawn sizes

@@ -56,6 +56,7 @@ hipError_t run_int8_ring(int bm, int bn, const Int8GemmParams& p, hipStream_t s)
 
 hipError_t run_int8_splitk_reduce(const Int8GemmParams& p, hipStream_t s) {
     const int64_t threads = ((int64_t)p.N + 3) / 4 * p.M;
+    if (threads > kMostThreads) return hipErrorInvalidValue;
     hipLaunchKernelGGL(int8_splitk_reduce_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, p);
     return hipGetLastError();
 }

@@ -264,6 +264,7 @@ hipError_t launch(int which, const MoeRouteParams& p, hipStream_t s) {
     const int64_t pieces = ((int64_t)p.H + piece - 1) / piece;
     const int lanes = pieces <= 64 ? 64 : pieces <= 128 ? 128 : kRouteLanes;
     int64_t parts = which == 2 ? 1 : (pieces + lanes - 1) / lanes;
+    if (parts == 0) return hipSuccess;  // rows of no elements
     if (parts * p.tokens > kRouteParts) parts = kRouteParts / p.tokens > 0 ? kRouteParts / p.tokens : 1;
     const dim3 grid((unsigned)p.tokens, (unsigned)parts), block(lanes);
     if (which == 0) hipLaunchKernelGGL((moe_permute_kernel<T, VEC>), grid, block, 0, s, p);

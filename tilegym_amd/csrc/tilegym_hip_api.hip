@@ -36,7 +36,9 @@ int64_t numel(const tg_tensor* t) {
     return n;
 }
 
-bool contiguous(const tg_tensor* t) {
+bool contiguous(const tg_tensor* t) {  // (without elements: whatever the strides, as torch has it)
+    for (int i = 0; i < t->ndim; ++i)
+        if (t->shape[i] == 0) return true;
     int64_t expect = 1;
     for (int i = t->ndim - 1; i >= 0; --i) {
         if (t->shape[i] != 1 && t->strides[i] != expect) return false;
@@ -2288,7 +2290,7 @@ struct Int8Schedule { int kernel, bm, bn, split; };
 static bool int8_takes(const tg::Int8GemmParams& p, const Int8Schedule& s) {
     if (s.kernel == 0) return true;
     if (!int8_fast_layout(p)) return false;
-    if (s.kernel == 3) return (p.m_indptr || p.M <= 32) && s.bn >= 4 && s.bn <= 64 && s.bn % 4 == 0;
+    if (s.kernel == 3) return (p.m_indptr ? (int64_t)p.E + p.M / 16 <= 65535 : p.M <= 32) && s.bn >= 4 && s.bn <= 64 && s.bn % 4 == 0;
     if (s.bm == 256 && s.bn == 256)
         return p.K % 128 == 0 && p.K >= 256 && p.vec_store && s.split == 1 && (int64_t)p.M * p.K < kOffsetLimit && (int64_t)p.N * p.K < kOffsetLimit &&
                p.ldc * 1024 < kOffsetLimit;
@@ -2370,7 +2372,8 @@ constexpr int64_t kInt8StreamRowsPerExpert = 12;
 
 static Int8Schedule cheapest_int8_ragged(const tg::Int8GemmParams& p) {
     const double M = p.M, E = p.E, N = p.N, K = p.K;
-    if (p.M <= kInt8StreamRowsPerExpert * p.E && p.E + p.M / 16 <= 65535) return Int8Schedule{3, -1, 64, 1};
+    const Int8Schedule stream{3, -1, 64, 1};
+    if (p.M <= kInt8StreamRowsPerExpert * p.E && int8_takes(p, stream)) return stream;
     const double used = E * (1.0 - std::pow(1.0 - 1.0 / E, M));  // experts with rows, to be expected
     const float from_memory = (float)std::min(std::max((used * N * K - 8e6) / 40e6, 0.), 1.);
     Int8Schedule best{0, -1, -1, 1};
