@@ -4,7 +4,8 @@
 // A row that holds a NaN or an infinity gets the scale NaN and codes of zero, so that it shows in what is
 // multiplied with it.  With `place` a row's codes go to several rows: tokens on their way to the experts that each of them was sent to.
 //
-// Bound by HBM (a row is read once and stays in the registers of the lanes that share it, V vectors of 8 elements each), few rows by latency.
+// Bound by HBM (a row is read once and stays in the registers of the lanes that share it, V vectors of 8 elements each), few rows by latency: 5000 x 14336 f16 42 us (5.1 TB/s),
+// 24576 x 1408 activated bf16 31 (5.6), 4096 x 2048 to six places each 17 (4.0).
 // Rows longer than the registers of 1024 lanes are read twice.
 #include "quant_device.h"
 
