@@ -68,28 +68,45 @@ struct RingPart {
         if constexpr (TN == 2) read_w(1, base);
     }
     // column tile by column tile: all row groups' first halves, then the second ones
-    __device__ __forceinline__ void before(const uint8_t* cur) {
+    // (PARTIAL: the upper half of the row groups only where it holds rows, see the kernel over experts)
+    template <bool PARTIAL>
+    __device__ __forceinline__ void before(const uint8_t* cur, bool upper) {
 #pragma unroll
         for (int tn = 0; tn < TN - LAST; ++tn) {
+            constexpr int H = PARTIAL ? (TM + 1) / 2 : TM;
 #pragma unroll
-            for (int tm = 0; tm < TM; ++tm) {
+            for (int tm = 0; tm < H; ++tm) {
                 acc[tn][tm] = mfma_i8(lo4(wf[tn % WS]), lo4(af[tm]), acc[tn][tm]);
                 if (tm == 0 && tn + 2 < TN) read_w(tn + 2, cur);
                 TG_FENCE();
             }
 #pragma unroll
-            for (int tm = 0; tm < TM; ++tm) acc[tn][tm] = mfma_i8(hi4(wf[tn % WS]), hi4(af[tm]), acc[tn][tm]);
+            for (int tm = 0; tm < H; ++tm) acc[tn][tm] = mfma_i8(hi4(wf[tn % WS]), hi4(af[tm]), acc[tn][tm]);
             TG_FENCE();
+            if (H < TM && upper) {
+#pragma unroll
+                for (int tm = H; tm < TM; ++tm) acc[tn][tm] = mfma_i8(lo4(wf[tn % WS]), lo4(af[tm]), acc[tn][tm]);
+#pragma unroll
+                for (int tm = H; tm < TM; ++tm) acc[tn][tm] = mfma_i8(hi4(wf[tn % WS]), hi4(af[tm]), acc[tn][tm]);
+                TG_FENCE();
+            }
         }
     }
     // row group by row group: the last MFMA of one releases its fragment
-    template <int WGM>
-    __device__ __forceinline__ void behind(const uint8_t* nxt) {
+    template <int WGM, bool PARTIAL>
+    __device__ __forceinline__ void behind(const uint8_t* nxt, bool upper) {
+        constexpr int H = PARTIAL ? (TM + 1) / 2 : TM;
         read_w(0, nxt);
         if constexpr (TN > 2) read_w(1, nxt);
         TG_FENCE();
+        groups<WGM, 0, H>(nxt);
+        if (H < TM && upper) groups<WGM, H, TM>(nxt);
+        if constexpr (TN == 2) read_w(1, nxt);  // (its registers were the last MFMAs')
+    }
+    template <int WGM, int FROM, int TO>
+    __device__ __forceinline__ void groups(const uint8_t* nxt) {
 #pragma unroll
-        for (int tm = 0; tm < TM; ++tm) {
+        for (int tm = FROM; tm < TO; ++tm) {
 #pragma unroll
             for (int tn = TN - LAST; tn < TN; ++tn) acc[tn][tm] = mfma_i8(lo4(wf[tn % WS]), lo4(af[tm]), acc[tn][tm]);
 #pragma unroll
@@ -98,7 +115,6 @@ struct RingPart {
             read_a<WGM>(tm, nxt);
             TG_FENCE();
         }
-        if constexpr (TN == 2) read_w(1, nxt);  // (its registers were the last MFMAs')
     }
     __device__ __forceinline__ void keep() {  // (the reads for the step behind the last one)
 #pragma unroll
@@ -263,7 +279,13 @@ __global__ void __launch_bounds__(512, 1) int8_gemm_ring_kernel(const Int8GemmPa
         RingLoader<BM, BN, NL> loader;
         loader.init(wave - 4, lane, lds_address(lds));
         loader.set(p, m0, n0, rows_valid, 0);
-        auto issue = [&](int kstep, int stage) { loader.issue(K, min(kstep, last), stage); };
+        // Where a weight row is read once, workgroups start at different K steps and go round: rows a power of two apart would meet on few memory
+        // channels (128 x 28672 x 4096 in 128 x 128 tiles 32.8 -> 28.7 us; with eight row tiles, 1024 x 8192 x 8192 in 256 x 128, 57 -> 63).
+        const int rot = tiles_m == 1 ? (int)((blockIdx.x >> 3) % (unsigned)nsteps) : 0;
+        auto issue = [&](int kstep, int stage) {
+            const int at = min(kstep, last) + rot;
+            loader.issue(K, at < ks_end ? at : at - nsteps, stage);
+        };
 #pragma unroll
         for (int s = 0; s < STAGES; ++s) issue(ks + s, s);
         __builtin_amdgcn_s_waitcnt(kWaitPro);
@@ -302,11 +324,11 @@ __global__ void __launch_bounds__(512, 1) int8_gemm_ring_kernel(const Int8GemmPa
         stage = stage == STAGES - 1 ? 0 : stage + 1;
         const uint8_t* nxt = lds + stage * STAGE_BYTES;
         TG_FENCE();
-        part.before(cur);
+        part.template before<false>(cur, true);
         __builtin_amdgcn_s_waitcnt(kWaitLds);  // all my reads of step k are done
         __builtin_amdgcn_s_barrier();          // step k+1 is visible
         TG_FENCE();
-        part.template behind<WGM>(nxt);
+        part.template behind<WGM, false>(nxt, true);
     }
     part.keep();
 
@@ -418,6 +440,9 @@ __global__ void __launch_bounds__(512, 1) int8_gemm_ring_experts_kernel(const In
         const float row = p.sa[((int64_t)m0 + min(tid, rows_valid - 1)) * p.sa_step];
         const float col = p.sb[((int64_t)expert * p.N + min(n0 + tid, p.N - 1)) * p.sb_step];
         float* const scales = factors[t & 1];
+        // An expert's last rows may leave the upper half of the row groups empty: then its MFMAs and fragments are left out (6000 rows, 1 to 711 an expert, in 192 x 192 tiles
+        // 101 -> 99 us; in steps of two groups no better).
+        const bool upper = rows_valid > (TM + 1) / 2 * 16 * WGM;
         // (again behind the first tile: fragments that lived through the stores would be more than the registers hold)
         part.template first<WGM>(lds + stage * Loader::STAGE_BYTES);
         for (int k = 0; k < nsteps; ++k) {
@@ -429,11 +454,11 @@ __global__ void __launch_bounds__(512, 1) int8_gemm_ring_experts_kernel(const In
             stage = stage == STAGES - 1 ? 0 : stage + 1;
             const uint8_t* nxt = lds + stage * Loader::STAGE_BYTES;
             TG_FENCE();
-            part.before(cur);
+            part.template before<true>(cur, upper);
             __builtin_amdgcn_s_waitcnt(kWaitLds);
             __builtin_amdgcn_s_barrier();
             TG_FENCE();
-            part.template behind<WGM>(nxt);
+            part.template behind<WGM, true>(nxt, upper);
         }
         part.keep();
         // (as if written here: what the stores compute from them would be held through all K loops)
