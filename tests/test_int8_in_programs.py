@@ -7,6 +7,7 @@ import random
 import pytest
 import torch
 
+from oracle import int8_reference as R
 from tilegym_amd import _lib, ops
 
 from .test_int8_ops import BF16, F16, F32, bits, codes, gen, routing, scales
@@ -265,10 +266,10 @@ def test_empty_sizes(device):
     assert ops.quant_int8(f32(0, 64))[1].shape == (0,) and ops.silu_mul_quant_int8(f32(0, 64))[0].shape == (0, 32)
     none = torch.zeros(0, 2, dtype=torch.int32, device=device)
     assert ops.int8_moe(f32(0, 64).to(BF16), i8(4, 64, 64), i8(4, 64, 32), f32(4, 64), f32(4, 64), f32(0, 2), none).shape == (0, 64)
-    # a layer none of whose experts is here
+    # a layer none of whose experts is here; it has no gradient, in the router's weights either
     ids = torch.full((5, 2), -1, dtype=torch.int32, device=device)
-    made = ops.int8_moe(f32(5, 64).to(BF16), i8(4, 64, 64), i8(4, 64, 32), f32(4, 64), f32(4, 64), f32(5, 2), ids)
-    assert not bool(made.any())
+    made = ops.int8_moe(f32(5, 64).to(BF16), i8(4, 64, 64), i8(4, 64, 32), f32(4, 64), f32(4, 64), f32(5, 2).requires_grad_(), ids)
+    assert not bool(made.any()) and not made.requires_grad
 
 
 @pytest.mark.gpu
@@ -282,6 +283,32 @@ def test_forced_streaming_over_more_passes_than_a_grid_has(device):
     assert _lib.last_config()["KERNEL"] != 3
     assert torch.equal(bits(got[:100]), bits(_exact(a[:100], b[0], sa[:100], sb[0], BF16)))
     assert torch.equal(bits(got[100:]), bits(_exact(a[100:], b[1], sa[100:], sb[1], BF16)))
+
+
+# ---------------------------------------------------------------------------- many rows
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [8, 500, 512, 1000, 1024, 1408, 1536, 2041, 2048])
+@pytest.mark.parametrize("t", [BF16, F16, F32])
+def test_quantizers_of_many_rows(device, k, t):
+    """Rows enough for a wave each, of up to 256 vectors; the odd ones element by element."""
+    rows = 2051
+    x = torch.randn(rows, k, generator=gen(k)).to(t)
+    x[5], x[6, k // 3], x[7, 0] = 0, float("nan"), float("inf")
+    wq, ws = R.ref_quant(x)
+    q, s = ops.quant_int8(x.to(device))
+    assert torch.equal(q.cpu(), wq) and torch.equal(bits(s.nan_to_num(-1)), bits(ws.nan_to_num(-1)))
+    order = ops.moe_sort(routing(rows, 16, 3, k, absent=True).to(device), 16)
+    q, s = ops.moe_permute_quant_int8(x.to(device), order)
+    live, slots = int(order.indptr[-1]), order.slots.cpu().long()
+    token = slots[:live] // 3
+    assert torch.equal(q[:live].cpu(), wq[token]) and torch.equal(bits(s[:live].nan_to_num(-1)), bits(ws[token].nan_to_num(-1)))
+    assert not bool(q[live:].any()) and bool((s[live:] == 1).all())
+    # the activation: the codes of few rows are those of many
+    both = torch.randn(rows, 2 * k, generator=gen(k + 1)).to(t).to(device)
+    q, s = ops.silu_mul_quant_int8(both)
+    for part in (slice(0, 40), slice(1000, 1333), slice(rows - 1, rows)):
+        pq, ps = ops.silu_mul_quant_int8(both[part].contiguous())
+        assert torch.equal(q[part], pq) and torch.equal(bits(s[part]), bits(ps))
 
 
 # ---------------------------------------------------------------------------- drawn sizes

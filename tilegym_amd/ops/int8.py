@@ -1,4 +1,4 @@
-"""Products in 8-bit integers with a scale per token and per output channel, and the quantizers in front of them.
+"""Products in 8-bit integers with a scale per token and per output channel, and the quantizers in front of them.  None of them has a gradient.
 
 The reference's counterparts are the int8 forms of its MoE interface (``use_int8_w8a16``, src/tilegym/ops/moe_interface.py:116-322) and
 ``per_token_group_quant_8bit`` (src/tilegym/suites/flashinfer/ops.py), whose int8 codes no product of it takes."""
@@ -81,7 +81,7 @@ def int8_moe(
 
     hidden_states (T, H) bf16 / f16; w1 (E, 2 I, H), w2 (E, H, I) int8 with scales per output channel w1_scale (E, 2 I), w2_scale (E, H) fp32;
     topk_weights (T, k) fp32 / bf16 / f16; topk_ids (T, k) int32 / int64.  The products' outputs are of hidden_states' type.  A slot whose id is outside
-    [0, E) (an expert of another rank, say) adds nothing.  Returns (T, H)."""
+    [0, E) (an expert of another rank, say) adds nothing.  Returns (T, H), without a gradient, in the weights either."""
     from .moe_route import moe_permute_quant_int8, moe_sort, moe_unpermute
 
     if hidden_states.dtype not in (torch.bfloat16, torch.float16):
@@ -91,4 +91,4 @@ def int8_moe(
     h = ragged_int8_matmul(q, w1, scales, w1_scale, order.indptr, out_dtype=hidden_states.dtype)
     q, scales = silu_mul_quant_int8(h)
     y = ragged_int8_matmul(q, w2, scales, w2_scale, order.indptr, out_dtype=hidden_states.dtype)
-    return moe_unpermute(y, order, topk_weights)
+    return moe_unpermute(y, order, topk_weights.detach())

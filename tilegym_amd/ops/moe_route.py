@@ -1,6 +1,9 @@
 """Tokens sorted by expert, carried to the experts' rows and back with the router's weights, and the gradients of both ways: what makes the
 segments that ``ragged_block_scaled_bmm`` and ``ragged_int8_matmul`` multiply.
 
+Forward and backward passes can be captured into a graph.  What is refused while capturing is a leaf that an eager graph on another stream still holds: its gradient would be
+added there (``moe_permute_backward`` and ``moe_unpermute_backward`` take no part in autograd and can always be captured).
+
 The reference sorts inside ``moe_align_block_size`` (src/tilegym/ops/moe_interface.py:21-79), into blocks that its gather GEMM pads."""
 
 from __future__ import annotations
