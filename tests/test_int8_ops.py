@@ -420,7 +420,7 @@ WIDTHS = [1, 7, 8, 64, 100, 2048, 2056, 4100, 7168]
 @pytest.mark.parametrize("h", WIDTHS)
 @pytest.mark.parametrize("t", [BF16, F16, F32])
 def test_there_and_back(device, h, t):
-    for tokens, experts, k, absent in ((1, 4, 2, False), (37, 16, 3, True), (20, 64, 8, False), (9, 32, 11, True)):
+    for tokens, experts, k, absent in ((1, 4, 2, False), (37, 16, 3, True), (20, 64, 8, False), (9, 32, 11, True), (2101, 16, 4, True)):
         order = _order(device, routing(tokens, experts, k, h, absent), experts)
         rows = order.rows.cpu()
         x = torch.randn(tokens, h, generator=gen(h)).to(t)
