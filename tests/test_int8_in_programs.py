@@ -285,6 +285,17 @@ def test_forced_streaming_over_more_passes_than_a_grid_has(device):
     assert torch.equal(bits(got[100:]), bits(_exact(a[100:], b[1], sa[100:], sb[1], BF16)))
 
 
+@pytest.mark.gpu
+def test_experts_beyond_the_limit_are_refused(device):
+    """Without an allocation of their number."""
+    ids = torch.zeros(3, 2, dtype=torch.int32, device=device)
+    for experts in (513, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 4, 10 ** 12, -1):
+        before = torch.cuda.memory_allocated()
+        with pytest.raises((_lib.TileGymHipError, OverflowError)):
+            ops.moe_sort(ids, experts)
+        assert torch.cuda.memory_allocated() == before
+
+
 # ---------------------------------------------------------------------------- many rows
 @pytest.mark.gpu
 @pytest.mark.parametrize("k", [8, 500, 512, 1000, 1024, 1408, 1536, 2041, 2048])

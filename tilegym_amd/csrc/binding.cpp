@@ -660,7 +660,7 @@ PyObject* py_moe_sort(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor* ids = tensor_of(args[0]);
     const long experts = PyLong_AsLong(args[1]);
     if (PyErr_Occurred()) return nullptr;
-    if (!on_gpu(ids) || ids->dim() != 2 || !ids->is_contiguous() || experts < 1 || experts > INT32_MAX - 1) Py_RETURN_NONE;
+    if (!on_gpu(ids) || ids->dim() != 2 || !ids->is_contiguous() || experts < 1 || experts > 512) Py_RETURN_NONE;
     at::Tensor indptr = new_tensor({experts + 1}, at::kInt, *ids), rows = new_tensor(ids->sizes(), at::kInt, *ids), slots = new_tensor({ids->numel()}, at::kInt, *ids);
     tg_tensor di, dp, dr, ds, dws;
     at::Tensor ws;

@@ -97,7 +97,7 @@ def moe_sort(topk_ids, num_experts):
     if topk_ids.dim() != 2:
         raise ValueError(f"moe_sort: topk_ids must be (T, k), got {tuple(topk_ids.shape)}")
     i32 = dict(dtype=torch.int32, device=topk_ids.device)
-    order = MoeOrder(torch.empty(max(int(num_experts), 0) + 1, **i32), torch.empty(topk_ids.shape, **i32), torch.empty(topk_ids.numel(), **i32))
+    order = MoeOrder(torch.empty(min(max(int(num_experts), 0), 512) + 1, **i32), torch.empty(topk_ids.shape, **i32), torch.empty(topk_ids.numel(), **i32))
     _lib.moe_sort(topk_ids.contiguous(), num_experts, *order)
     return order
 
