@@ -342,6 +342,26 @@ def test_drawn_products(device):
 
 
 @pytest.mark.gpu
+def test_lengths_of_no_vectors_split(device):
+    """Few tiles of the kernel that takes any length: its K is split, in parts that end inside a row's last bytes."""
+    seen = set()
+    for m, n, k in ((1, 4478, 3250), (2, 70, 7822), (64, 65, 4001), (65, 130, 2047), (200, 60, 16001), (30, 501, 1027), (513, 100, 4097), (5, 1, 131071)):
+        a, b = codes((m, k), m).to(device), codes((n, k), n).to(device)
+        sa, sb = scales(m, 3).to(device), scales(n, 4).to(device)
+        for t in (BF16, F32):
+            assert torch.equal(bits(ops.int8_matmul(a, b, sa, sb, out_dtype=t)), bits(_exact(a, b, sa, sb, t))), (m, n, k)
+            got = _lib.last_config()
+            assert got["KERNEL"] == 0
+            seen.add(got["SPLIT_K"])
+        bias = torch.randn(n, generator=gen(5)).to(device)
+        exact = (a.double() @ b.double().t()) * sa.double()[:, None] * sb.double() + bias.double()
+        got = ops.int8_matmul(a, b, sa, sb, bias=bias, out_dtype=F32).double()
+        # the sum's conversion, its product with the token's scale, the multiply-add
+        assert bool(((got - exact).abs() <= 3.01 * 2.0 ** -24 * (exact.abs() + 2 * bias.double().abs())).all())
+    assert 1 in seen and max(seen) > 8
+
+
+@pytest.mark.gpu
 def test_drawn_products_over_experts(device):
     rng = random.Random(4)
     for i in range(40):

@@ -4,7 +4,7 @@
 // A workgroup of four waves makes 64 x 64 outputs.  Both operands go through registers to LDS, 64 bytes of K at a time: a thread fetches
 // 16 bytes of one row at any address (the tail of a row byte by byte, zeros beyond it), one step ahead of the MFMAs.  Rows of LDS are 80
 // bytes apart, so that the sixteen rows a fragment read touches start in different banks.  Bound by the latency of that one
-// step: 512 x 1001 x 1003 takes 12.7 us, 4096 x 4099 x 4095 306 (449 TOP/s).
+// step (0.6 us), so K is split where tiles are few: 512 x 1001 x 1003 takes 12.7 us, 4096 x 4099 x 4095 306 (449 TOP/s).
 #include "int8_device.h"
 
 namespace tg {
@@ -47,14 +47,18 @@ __global__ void __launch_bounds__(256) int8_gemm_simple_kernel(const Int8GemmPar
     const bool has_a = m0 + row < m_end, has_b = n0 + row < p.N;
     const int8_t* a = p.A + (m0 + row) * (int64_t)p.K + at;
     const int8_t* b = p.B + ((int64_t)expert * p.N + n0 + row) * (int64_t)p.K + at;
-    const int steps = (p.K + 63) / 64;
+    int steps = (p.K + 63) / 64, s0 = 0;
+    if (!RAGGED && p.split_k > 1) {
+        s0 = 2 * (int)blockIdx.y * p.ksteps_per_split;
+        steps = min(s0 + 2 * p.ksteps_per_split, steps);
+    }
     auto left = [&](bool has, int step) { return has ? (int64_t)p.K - (int64_t)step * 64 - at : (int64_t)0; };
-    v4i ra = fetch16(a, left(has_a, 0)), rb = fetch16(b, left(has_b, 0));
+    v4i ra = fetch16(a + (int64_t)s0 * 64, left(has_a, s0)), rb = fetch16(b + (int64_t)s0 * 64, left(has_b, s0));
     const int wm = wave & 1, wn = wave >> 1, li = lane & 15, lg = lane >> 4;
     v4i acc[2][2];
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] = v4i{0, 0, 0, 0};
-    for (int s = 0; s < steps; ++s) {
+    for (int s = s0; s < steps; ++s) {
         *reinterpret_cast<v4i*>(&sA[s & 1][row * kPitch + at]) = ra;
         *reinterpret_cast<v4i*>(&sB[s & 1][row * kPitch + at]) = rb;
         __syncthreads();  // (the other buffer's readers have passed the barrier of the step before)
@@ -77,6 +81,17 @@ __global__ void __launch_bounds__(256) int8_gemm_simple_kernel(const Int8GemmPar
     for (int tm = 0; tm < 2; ++tm) {
         const int64_t m = m0 + wm * 32 + tm * 16 + li;
         if (m >= m_end) continue;
+        if (!RAGGED && p.split_k > 1) {
+            int* const mine = p.partials + ((int64_t)blockIdx.y * p.M + m) * p.N;
+#pragma unroll
+            for (int tn = 0; tn < 2; ++tn)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int n = n0 + wn * 32 + tn * 16 + lg * 4 + r;
+                    if (n < p.N) mine[n] = acc[tn][tm][r];
+                }
+            continue;
+        }
         const float sa = p.sa[m * p.sa_step];
 #pragma unroll
         for (int tn = 0; tn < 2; ++tn)
@@ -94,11 +109,11 @@ __global__ void __launch_bounds__(256) int8_gemm_simple_kernel(const Int8GemmPar
 
 int64_t int8_simple_threads(const Int8GemmParams& p) {
     const int64_t row_tiles = p.m_indptr ? (int64_t)p.M / 64 + (p.E < p.M ? p.E : p.M) : ((int64_t)p.M + 63) / 64;
-    return row_tiles * (((int64_t)p.N + 63) / 64) * 256;
+    return row_tiles * (((int64_t)p.N + 63) / 64) * 256 * p.split_k;
 }
 
 hipError_t run_int8_simple(const Int8GemmParams& p, hipStream_t s) {
-    const dim3 grid((unsigned)(int8_simple_threads(p) / 256));
+    const dim3 grid((unsigned)(int8_simple_threads(p) / 256 / p.split_k), p.split_k);
     if (p.m_indptr) hipLaunchKernelGGL(int8_gemm_simple_kernel<true>, grid, dim3(256), 0, s, p);
     else hipLaunchKernelGGL(int8_gemm_simple_kernel<false>, grid, dim3(256), 0, s, p);
     return hipGetLastError();

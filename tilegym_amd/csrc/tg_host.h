@@ -219,7 +219,7 @@ bool int8_ring_exists(int bm, int bn);
 hipError_t run_int8_ring(int bm, int bn, const Int8GemmParams& p, hipStream_t s);
 // K % 128 == 0, K >= 256, vec_store, A and each weight below 2 GiB, unsplit, over experts without a bias
 hipError_t run_int8_tile256(const Int8GemmParams& p, hipStream_t s);
-// behind run_int8_stream or run_int8_ring with split_k > 1
+// behind any of the dense ones with split_k > 1
 hipError_t run_int8_splitk_reduce(const Int8GemmParams& p, hipStream_t s);
 
 // A row's int8 codes and its scale (int8_quant.hip)

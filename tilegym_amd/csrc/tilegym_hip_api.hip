@@ -2388,12 +2388,30 @@ static Int8Schedule cheapest_int8_ragged(const tg::Int8GemmParams& p) {
     return best;
 }
 
+// The kernel for any length and address, K split where its tiles are few: 64 bytes of K take a workgroup 0.6 us of latency, unless all of them together
+// are bound by what they fetch (4.2 TB/s, from memory 2.2) or there are more than eight to a compute unit; the sum of the parts costs 3 us and 0.6 per MB.  us, whole / split:
+// 1 x 4478 x 13250 157 / 31, 30 x 4001 x 4001 39 / 19, 200 x 600 x 16001 152 / 26, 2 x 16677 x 7822 101 / 51; 300 x 5001 x 3003 37 / 41, 64 x 28671 x 4095 63 / 70.
+static Int8Schedule simple_int8(const tg::Int8GemmParams& p, int64_t partial_bytes) {
+    Int8Schedule best{0, -1, -1, 1};
+    if (p.m_indptr) return best;
+    const double M = p.M, N = p.N, K = p.K, tiles = (double)(cdiv(p.M, 64) * cdiv(p.N, 64)), steps = (double)cdiv(p.K, 128);
+    const double fetch = std::max(tiles * K * (64 + std::min(M, 64.)) / 4.2e6, (M + N) * K / 2.2e6);
+    double best_us = 0;
+    for (int split : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+        if (split > 1 && (steps < 2 * split || M > 512 || split * M * N * 4 > (double)partial_bytes)) break;
+        double us = std::max(1.2 * std::ceil(steps / split) * std::max(1., tiles * split / 2048), fetch);
+        if (split > 1) us = (us + 3 + 0.6e-6 * split * M * N * 4) * kInt8SplitMargin;
+        if (split == 1 || us < best_us) { best.split = split; best_us = us; }
+    }
+    return best;
+}
+
 static Int8Schedule choose_int8(const tg::Int8GemmParams& p, int64_t partial_bytes, const int32_t* cfg, int32_t ncfg) {
-    const Int8Schedule simple{0, -1, -1, 1};
+    const int64_t auto_bytes = std::min(partial_bytes, kAutoPartialBytes);
     const int want = cfg_get(cfg, ncfg, TG_CFG_KERNEL);
     const int want_bm = cfg_get(cfg, ncfg, TG_CFG_BLOCK_M), want_bn = cfg_get(cfg, ncfg, TG_CFG_BLOCK_N), want_split = cfg_get(cfg, ncfg, TG_CFG_SPLIT_K);
     const int64_t steps = cdiv(p.K, 128);
-    if (want == 0) return simple;
+    if (want == 0) return simple_int8(p, auto_bytes);
     if (want == 3 || want == 1) {
         Int8Schedule s{want, want_bm, want == 3 && want_bn <= 0 ? 64 : want_bn, 1};
         if (int8_takes(p, s)) {
@@ -2401,8 +2419,8 @@ static Int8Schedule choose_int8(const tg::Int8GemmParams& p, int64_t partial_byt
             return s;
         }
     }
-    if (!int8_fast_layout(p)) return simple;
-    if (!p.m_indptr) return cheapest_int8(p, std::min(partial_bytes, kAutoPartialBytes));
+    if (!int8_fast_layout(p)) return simple_int8(p, auto_bytes);
+    if (!p.m_indptr) return cheapest_int8(p, auto_bytes);
     return cheapest_int8_ragged(p);
 }
 
