@@ -238,6 +238,30 @@ def test_routing_past_32_bit_offsets(device):
     assert torch.equal(q[-5:], ops.silu_mul_quant_int8(there[-5:].contiguous())[0])
 
 
+# ---------------------------------------------------------------------------- the layer in one call
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,experts,k,h,i,dtype", [(1, 4, 2, 64, 32, BF16), (9, 64, 6, 256, 100, F16), (33, 8, 2, 250, 64, BF16), (700, 16, 4, 512, 192, BF16), (5000, 8, 6, 64, 48, F16)])
+def test_layer_in_one_call_is_its_operators(device, monkeypatch, tokens, experts, k, h, i, dtype):
+    x = torch.randn(tokens, h, generator=gen(1)).to(dtype).to(device)
+    w1, w2 = codes((experts, 2 * i, h), 2).to(device), codes((experts, h, i), 3).to(device)
+    s1, s2 = scales((experts, 2 * i), 4).to(device) / 50, scales((experts, h), 5).to(device)
+    for absent, wt, it in ((False, F32, torch.int32), (True, BF16, torch.int64)):
+        ids, w = routing(tokens, experts, k, 6, absent, dtype=it).to(device), torch.rand(tokens, k, generator=gen(7)).to(wt).to(device)
+        got = ops.int8_moe(x, w1, w2, s1, s2, w, ids)
+        order = ops.moe_sort(ids, experts)
+        q, s = ops.moe_permute_quant_int8(x, order)
+        q, s = ops.silu_mul_quant_int8(ops.ragged_int8_matmul(q, w1, s, s1, order.indptr, out_dtype=dtype))
+        want = ops.moe_unpermute(ops.ragged_int8_matmul(q, w2, s, s2, order.indptr, out_dtype=dtype), order, w)
+        assert torch.equal(bits(got), bits(want))
+        with monkeypatch.context() as m:
+            m.setattr(_lib, "native_path", lambda: False)
+            assert torch.equal(bits(ops.int8_moe(x, w1, w2, s1, s2, w, ids)), bits(want))
+    for bad in (dict(w2=w2[:-1]), dict(w1_scale=s1[:1, :3].contiguous()), dict(topk_weights=w[:, :1].contiguous()), dict(w1=w1[:, :-2].contiguous())):
+        args = {**dict(hidden_states=x, w1=w1, w2=w2, w1_scale=s1, w2_scale=s2, topk_weights=w, topk_ids=ids), **bad}
+        with pytest.raises((ValueError, _lib.TileGymHipError)):
+            ops.int8_moe(**args)
+
+
 # ---------------------------------------------------------------------------- nothing to do
 @pytest.mark.gpu
 def test_empty_sizes(device):

@@ -736,6 +736,77 @@ PyObject* py_moe_unpermute_backward(PyObject*, PyObject* const* args, Py_ssize_t
     END_HANDLE_TH_ERRORS
 }
 
+// int8_moe(x, w1, w2, w1_scale, w2_scale, topk_weights, topk_ids) -> tensor, or None: the layer's six launches one after the other, what lies between
+// them in one allocation of the call's own
+PyObject* py_int8_moe(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 7) { PyErr_SetString(PyExc_TypeError, "int8_moe takes 7 arguments"); return nullptr; }
+    const at::Tensor *x = tensor_of(args[0]), *w1 = tensor_of(args[1]), *w2 = tensor_of(args[2]), *s1 = tensor_of(args[3]), *s2 = tensor_of(args[4]),
+                     *tw = tensor_of(args[5]), *ids = tensor_of(args[6]);
+    if (!on_gpu(x) || (x->scalar_type() != at::kBFloat16 && x->scalar_type() != at::kHalf) || x->dim() != 2 || !x->is_contiguous() || !plain(w1, at::kChar, 3) ||
+        !plain(w2, at::kChar, 3) || !on_gpu(s1) || !plain(s1, at::kFloat, s1->dim()) || !on_gpu(s2) || !plain(s2, at::kFloat, s2->dim()) || !on_gpu(tw) ||
+        tw->dim() != 2 || !io_type(tw->scalar_type()) || !tw->is_contiguous() || !on_gpu(ids) || ids->dim() != 2 || !ids->is_contiguous() ||
+        (ids->scalar_type() != at::kInt && ids->scalar_type() != at::kLong))
+        Py_RETURN_NONE;
+    for (const at::Tensor* t : {w1, w2, s1, s2, tw, ids})
+        if (t->device() != x->device()) Py_RETURN_NONE;
+    const int64_t T = x->size(0), H = x->size(1), E = w1->size(0), I = w2->size(2), k = ids->size(1), rows = T * k;
+    if (T < 1 || k < 1 || H < 1 || I < 1 || E < 1 || E > 512 || rows > INT32_MAX || ids->size(0) != T || tw->sizes() != ids->sizes() || w1->size(1) != 2 * I ||
+        w1->size(2) != H || w2->size(0) != E || w2->size(1) != H)
+        Py_RETURN_NONE;
+    tg_tensor dx, dw1, dw2, ds1, ds2, dtw, dids, dout;
+    at::Tensor out = new_tensor({T, H}, x->scalar_type(), *x);
+    if (!describe(*x, &dx) || !describe(*w1, &dw1) || !describe(*w2, &dw2) || !describe(*s1, &ds1) || !describe(*s2, &ds2) || !describe(*tw, &dtw) ||
+        !describe(*ids, &dids) || !describe(out, &dout))
+        Py_RETURN_NONE;
+    const int io = dtype_code(x->scalar_type());
+    const int64_t sort_bytes = g_moe_sort_workspace_bytes(rows, (int32_t)E);
+    // (at, shape, type) of what lies between; a buffer is used again once what it held has been read
+    int64_t bytes = 0;
+    auto room = [&](int64_t size) { const int64_t at = bytes; bytes += (size + 255) / 256 * 256; return at; };
+    auto matrix = [](int64_t at, int64_t r, int64_t c, int type) {
+        tg_tensor d{};
+        d.ptr = (uint64_t)at;
+        d.ndim = 2;
+        d.dtype = type;
+        d.shape[0] = r, d.shape[1] = c;
+        d.strides[0] = c, d.strides[1] = 1;
+        return d;
+    };
+    auto vector = [&](int64_t at, int64_t r, int type) {
+        tg_tensor d = matrix(at, r, 1, type);
+        d.ndim = 1;
+        d.strides[0] = 1, d.shape[1] = d.strides[1] = 0;
+        return d;
+    };
+    tg_tensor dptr = vector(room((E + 1) * 4), E + 1, TG_I32), drows = matrix(room(rows * 4), T, k, TG_I32), dslots = vector(room(rows * 4), rows, TG_I32);
+    tg_tensor dsort = vector(room(sort_bytes), sort_bytes, 6);
+    const int64_t codes = room(rows * std::max(H, I)), scales = room(rows * 4), wide = room(rows * std::max(2 * I, H) * 2);
+    tg_tensor dq = matrix(codes, rows, H, TG_I8), ds = vector(scales, rows, TG_F32), dh = matrix(wide, rows, 2 * I, io);
+    tg_tensor dq2 = matrix(codes, rows, I, TG_I8), dy = matrix(wide, rows, H, io);
+    at::Tensor scratch = new_tensor({bytes}, at::kByte, *x);
+    const uint64_t base = reinterpret_cast<uint64_t>(scratch.data_ptr());
+    for (tg_tensor* d : {&dptr, &drows, &dslots, &dsort, &dq, &ds, &dh, &dq2, &dy}) d->ptr += base;
+    const char* where = "";
+    const int index = x->get_device();
+    const uint64_t stream = (uint64_t)(uintptr_t)c10::hip::getCurrentHIPStream(index).stream();
+    int32_t rc = TG_OK;
+    Py_BEGIN_ALLOW_THREADS
+    auto step = [&](const char* name, auto f) {
+        if (rc == TG_OK) where = name, rc = f();
+    };
+    step("tg_moe_sort", [&] { return g_moe_sort(&dids, (int32_t)E, &dptr, &drows, &dslots, sort_bytes > 0 ? &dsort : nullptr, index, stream); });
+    step("tg_int8_quant", [&] { return g_int8_quant(&dq, &ds, &dx, &drows, 0, index, stream); });
+    step("tg_int8_ragged_gemm", [&] { return g_int8_ragged_gemm(&dh, &dq, &dw1, &ds, &ds1, &dptr, nullptr, 0, index, stream); });
+    step("tg_int8_quant", [&] { return g_int8_quant(&dq2, &ds, &dh, nullptr, 1, index, stream); });
+    step("tg_int8_ragged_gemm", [&] { return g_int8_ragged_gemm(&dy, &dq2, &dw2, &ds, &ds2, &dptr, nullptr, 0, index, stream); });
+    step("tg_moe_unpermute", [&] { return g_moe_unpermute(&dout, &dy, &drows, &dtw, index, stream); });
+    Py_END_ALLOW_THREADS
+    if (!succeeded(rc, where)) return nullptr;
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
 // leaf_held(t) -> whether a graph that still lives accumulates into the leaf t on another stream than the current one
 PyObject* py_leaf_held(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -797,6 +868,7 @@ PyMethodDef kMethods[] = {TG_FAST("matmul", py_matmul),
                           TG_FAST("moe_permute", py_moe_permute),
                           TG_FAST("moe_unpermute", py_moe_unpermute),
                           TG_FAST("moe_unpermute_backward", py_moe_unpermute_backward),
+                          TG_FAST("int8_moe", py_int8_moe),
                           TG_FAST("leaf_held", py_leaf_held),
                           {"set_up", py_set_up, METH_VARARGS, nullptr},
                           {nullptr, nullptr, 0, nullptr}};

@@ -82,8 +82,13 @@ def int8_moe(
     hidden_states (T, H) bf16 / f16; w1 (E, 2 I, H), w2 (E, H, I) int8 with scales per output channel w1_scale (E, 2 I), w2_scale (E, H) fp32;
     topk_weights (T, k) fp32 / bf16 / f16; topk_ids (T, k) int32 / int64.  The products' outputs are of hidden_states' type.  A slot whose id is outside
     [0, E) (an expert of another rank, say) adds nothing.  Returns (T, H), without a gradient, in the weights either."""
+    from .. import _lib
     from .moe_route import moe_permute_quant_int8, moe_sort, moe_unpermute
 
+    if _lib.native_path():  # the six launches below in one call
+        out = _lib.native.int8_moe(hidden_states, w1, w2, w1_scale, w2_scale, topk_weights, topk_ids)
+        if out is not None:
+            return out
     if hidden_states.dtype not in (torch.bfloat16, torch.float16):
         raise NotImplementedError(f"int8_moe: hidden_states must be bf16 or f16, got {hidden_states.dtype}")
     order = moe_sort(topk_ids, w1.shape[0])
