@@ -111,6 +111,58 @@ def test_operators_through_torchs_dispatcher(device):
     torch.library.opcheck(t.moe_unpermute.default, (ops.moe_permute(x, order).requires_grad_(), order.rows, w.clone().requires_grad_()))
 
 
+# ---------------------------------------------------------------------------- gradients
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("t", [BF16, F32])
+def test_autograd_is_the_backward_operators(device, monkeypatch, native, t):
+    """In native code and without it: the gradients' bits, expanded and strided gradients, each input alone, what a second derivative and a changed input do."""
+    if not native:
+        monkeypatch.setattr(_lib, "native_path", lambda: False)
+    tokens, experts, k, h = 37, 8, 3, 72
+    order = ops.moe_sort(routing(tokens, experts, k, 1, absent=True).to(device), experts)
+    x = torch.randn(tokens, h, generator=gen(2)).to(t).to(device).requires_grad_()
+    y = torch.randn(tokens * k, h, generator=gen(3)).to(t).to(device).requires_grad_()
+    w = torch.rand(tokens, k, generator=gen(4)).to(device).requires_grad_()
+    g = torch.randn(tokens, h, generator=gen(5)).to(t).to(device)
+    gr = torch.randn(tokens * k, h, generator=gen(6)).to(t).to(device)
+    with torch.no_grad():
+        want_y, want_w = ops.moe_unpermute_backward(g, y, order, w)
+        want_x, want_plain = ops.moe_permute_backward(gr, order), ops.moe_permute(g, order)
+    there, back = ops.moe_permute(x, order), ops.moe_unpermute(y, order, w)
+    assert there.requires_grad and back.requires_grad and there.grad_fn is not None
+    assert torch.equal(bits(there.detach()), bits(ops.moe_permute(x.detach(), order)))
+    assert torch.equal(torch.autograd.grad(there, x, gr, retain_graph=True)[0], want_x)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(back, (y, w), g, retain_graph=True), (want_y, want_w)))
+    assert torch.equal(torch.autograd.grad(ops.moe_unpermute(y, order), y, g)[0], want_plain)
+    assert torch.equal(torch.autograd.grad(ops.moe_unpermute(y.detach(), order, w), w, g)[0], want_w)
+    assert torch.equal(torch.autograd.grad(ops.moe_unpermute(y, order, w.detach()), y, g)[0], want_y)
+    strided = g.t().contiguous().t()
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(back, (y, w), strided, retain_graph=True), (want_y, want_w)))
+    one = torch.ones((), dtype=t, device=device)
+    assert torch.equal(torch.autograd.grad(there, x, one.expand_as(there), retain_graph=True)[0], ops.moe_permute_backward(torch.ones_like(gr), order))
+    with torch.no_grad():
+        assert not ops.moe_permute(x, order).requires_grad and not ops.moe_unpermute(y, order, w).requires_grad
+    # no second derivative: an error, not a wrong number
+    for out, leaf, grad in ((there, x, gr), (back, y, g), (back, w, g)):
+        (first,) = torch.autograd.grad(out, leaf, grad.clone().requires_grad_(), create_graph=True)
+        assert first.requires_grad
+        with pytest.raises(RuntimeError, match="differentiate"):
+            first.float().sum().backward()
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(first.float().sum(), leaf)
+    # what the backward pass reads has been changed
+    out = ops.moe_unpermute(y, order, w)
+    with torch.no_grad():
+        y.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+    for call in (lambda: ops.moe_permute(x[1:], order), lambda: ops.moe_permute(x.t().contiguous().t(), order), lambda: ops.moe_unpermute(y, order, w[:, :2]),
+                 lambda: ops.moe_unpermute(y[1:], order), lambda: ops.moe_unpermute(y, order, w.cpu())):
+        with pytest.raises((ValueError, _lib.TileGymHipError)):
+            call()
+
+
 # ---------------------------------------------------------------------------- gradients under capture
 @pytest.mark.gpu
 def test_forward_and_backward_captured(device):

@@ -71,7 +71,7 @@ native = None  # the extension module, once load() has run (still None where it 
 _NATIVE_ENTRY_POINTS = ("tg_fp8_gemm", "tg_fp8_gemm_workspace_bytes", "tg_fp8_ragged_gemm", "tg_fp8_quant_group", "tg_fp8_fused_moe",
                         "tg_fp8_fused_moe_block_m", "tg_fp8_fused_moe_workspace_bytes", "tg_fp8_rms_norm_quant", "tg_fp8_kv_append",
                         "tg_fp8_kv_read", "tg_fp8_kv_attention", "tg_fp8_kv_attention_workspace_bytes", "tg_int8_gemm", "tg_int8_gemm_workspace_bytes",
-                        "tg_int8_ragged_gemm", "tg_int8_quant", "tg_moe_sort", "tg_moe_sort_workspace_bytes", "tg_moe_permute", "tg_moe_unpermute", "tg_moe_unpermute_backward")
+                        "tg_int8_ragged_gemm", "tg_int8_quant", "tg_last_error", "tg_moe_sort", "tg_moe_sort_workspace_bytes", "tg_moe_permute", "tg_moe_unpermute", "tg_moe_unpermute_backward")
 
 
 def lib_path() -> str:

@@ -15,7 +15,9 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
 
@@ -39,6 +41,7 @@ decltype(&tg_int8_gemm) g_int8_gemm = nullptr;
 decltype(&tg_int8_gemm_workspace_bytes) g_int8_gemm_workspace_bytes = nullptr;
 decltype(&tg_int8_ragged_gemm) g_int8_ragged_gemm = nullptr;
 decltype(&tg_int8_quant) g_int8_quant = nullptr;
+decltype(&tg_last_error) g_last_error = nullptr;
 decltype(&tg_moe_sort) g_moe_sort = nullptr;
 decltype(&tg_moe_sort_workspace_bytes) g_moe_sort_workspace_bytes = nullptr;
 decltype(&tg_moe_permute) g_moe_permute = nullptr;
@@ -807,6 +810,96 @@ PyObject* py_int8_moe(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- the ways there and back with their gradients.  Their backward passes run in torch's threads, without the interpreter: nothing below calls into it
+uint64_t stream_of(const at::Tensor& t) { return (uint64_t)(uintptr_t)c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+tg_tensor described(const at::Tensor& t) {
+    tg_tensor d;
+    TORCH_CHECK(describe(t, &d), "not a tensor of the C ABI");
+    return d;
+}
+void check(int32_t rc, const char* where) { TORCH_CHECK(rc == TG_OK, where, ": rc=", rc, ": ", g_last_error()); }
+
+at::Tensor permuted(const at::Tensor& x, const at::Tensor& rows) {
+    at::Tensor out = new_tensor({rows.numel(), x.size(1)}, x.scalar_type(), x);
+    const tg_tensor dout = described(out), dx = described(x), drows = described(rows);
+    check(g_moe_permute(&dout, &dx, &drows, x.get_device(), stream_of(x)), "tg_moe_permute");
+    return out;
+}
+at::Tensor unpermuted(const at::Tensor& x, const at::Tensor& rows, const at::Tensor& weights) {
+    at::Tensor out = new_tensor({rows.size(0), x.size(1)}, x.scalar_type(), x);
+    const tg_tensor dout = described(out), dx = described(x), drows = described(rows), dw = weights.defined() ? described(weights) : tg_tensor{};
+    check(g_moe_unpermute(&dout, &dx, &drows, weights.defined() ? &dw : nullptr, x.get_device(), stream_of(x)), "tg_moe_unpermute");
+    return out;
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// A backward pass has no gradient of its own: where a graph of it is made, it ends in an error.
+variable_list once(variable_list made) {
+    if (!c10::GradMode::is_enabled()) return made;
+    variable_list ends;
+    for (at::Tensor& t : made)
+        if (t.defined()) ends.push_back(t.detach().requires_grad_());
+    auto error = std::make_shared<torch::autograd::DelayedError>("the gradients of moe_permute and moe_unpermute cannot be differentiated again", (int64_t)ends.size());
+    ends = (*error)(std::move(ends));
+    size_t at = 0;
+    for (at::Tensor& t : made)
+        if (t.defined()) t = ends[at++];
+    return made;
+}
+
+struct Permute : torch::autograd::Function<Permute> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& rows) {
+        ctx->save_for_backward({rows});
+        return permuted(x, rows);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        return once({unpermuted(grads[0].contiguous(), ctx->get_saved_variables()[0], at::Tensor()), at::Tensor()});
+    }
+};
+struct Unpermute : torch::autograd::Function<Unpermute> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& rows, const std::optional<at::Tensor>& weights) {
+        ctx->save_for_backward(weights ? variable_list{rows, x, *weights} : variable_list{rows});
+        return unpermuted(x, rows, weights ? *weights : at::Tensor());
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        const at::Tensor grad = grads[0].contiguous();
+        if (saved.size() == 1) return once({permuted(grad, saved[0]), at::Tensor(), at::Tensor()});
+        const at::Tensor &rows = saved[0], &x = saved[1], &weights = saved[2];
+        at::Tensor gx = new_tensor(x.sizes(), x.scalar_type(), x), gw = new_tensor(weights.sizes(), weights.scalar_type(), x);
+        const tg_tensor dgx = described(gx), dgw = described(gw), dgrad = described(grad), dx = described(x), drows = described(rows), dw = described(weights);
+        check(g_moe_unpermute_backward(&dgx, &dgw, &dgrad, &dx, &drows, &dw, x.get_device(), stream_of(x)), "tg_moe_unpermute_backward");
+        return once({gx, at::Tensor(), gw});
+    }
+};
+
+// moe_permute_grad(x, rows) -> tensor with a gradient, or None
+PyObject* py_moe_permute_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 2) { PyErr_SetString(PyExc_TypeError, "moe_permute_grad takes 2 arguments"); return nullptr; }
+    const at::Tensor *x, *rows;
+    tg_tensor dx, drows;
+    if (!route_operands(args[0], args[1], &x, &rows, &dx, &drows) || !x->is_contiguous() || x->size(0) != rows->size(0)) Py_RETURN_NONE;
+    return THPVariable_Wrap(Permute::apply(*x, *rows));
+    END_HANDLE_TH_ERRORS
+}
+
+// moe_unpermute_grad(x, rows, weights) -> tensor with a gradient, or None
+PyObject* py_moe_unpermute_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 3) { PyErr_SetString(PyExc_TypeError, "moe_unpermute_grad takes 3 arguments"); return nullptr; }
+    const at::Tensor *x, *rows, *weights = args[2] == Py_None ? nullptr : tensor_of(args[2]);
+    tg_tensor dx, drows;
+    if (!route_operands(args[0], args[1], &x, &rows, &dx, &drows) || !x->is_contiguous() || x->size(0) != rows->numel() ||
+        (args[2] != Py_None && (!on_gpu(weights) || weights->device() != x->device() || !io_type(weights->scalar_type()) || !weights->is_contiguous() ||
+                                weights->sizes() != rows->sizes())))
+        Py_RETURN_NONE;
+    return THPVariable_Wrap(Unpermute::apply(*x, *rows, weights ? std::optional<at::Tensor>(*weights) : std::nullopt));
+    END_HANDLE_TH_ERRORS
+}
+
 // leaf_held(t) -> whether a graph that still lives accumulates into the leaf t on another stream than the current one
 PyObject* py_leaf_held(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -838,7 +931,7 @@ PyObject* py_set_up(PyObject*, PyObject* args) {
         !find("tg_fp8_fused_moe_block_m", &g_fused_moe_block_m) || !find("tg_fp8_fused_moe_workspace_bytes", &g_fused_moe_workspace_bytes) ||
         !find("tg_int8_gemm", &g_int8_gemm) || !find("tg_int8_gemm_workspace_bytes", &g_int8_gemm_workspace_bytes) ||
         !find("tg_int8_ragged_gemm", &g_int8_ragged_gemm) || !find("tg_int8_quant", &g_int8_quant) || !find("tg_moe_sort", &g_moe_sort) ||
-        !find("tg_moe_sort_workspace_bytes", &g_moe_sort_workspace_bytes) ||
+        !find("tg_last_error", &g_last_error) || !find("tg_moe_sort_workspace_bytes", &g_moe_sort_workspace_bytes) ||
         !find("tg_moe_permute", &g_moe_permute) || !find("tg_moe_unpermute", &g_moe_unpermute) ||
         !find("tg_moe_unpermute_backward", &g_moe_unpermute_backward))
         return nullptr;
@@ -869,6 +962,8 @@ PyMethodDef kMethods[] = {TG_FAST("matmul", py_matmul),
                           TG_FAST("moe_unpermute", py_moe_unpermute),
                           TG_FAST("moe_unpermute_backward", py_moe_unpermute_backward),
                           TG_FAST("int8_moe", py_int8_moe),
+                          TG_FAST("moe_permute_grad", py_moe_permute_grad),
+                          TG_FAST("moe_unpermute_grad", py_moe_unpermute_grad),
                           TG_FAST("leaf_held", py_leaf_held),
                           {"set_up", py_set_up, METH_VARARGS, nullptr},
                           {nullptr, nullptr, 0, nullptr}};

@@ -106,6 +106,10 @@ def moe_sort(topk_ids, num_experts):
 def moe_permute(x, order):
     if torch.is_grad_enabled() and x.requires_grad:
         _recordable("moe_permute", x)
+        if _lib.native_path():
+            done = _lib.native.moe_permute_grad(x, order.rows)
+            if done is not None:
+                return done
         return _Permute.apply(x, *order)
     return _permute(x, order)
 
@@ -130,6 +134,10 @@ def moe_permute_quant_int8(x, order):
 def moe_unpermute(x, order, weights=None):
     if torch.is_grad_enabled() and (x.requires_grad or (weights is not None and weights.requires_grad)):
         _recordable("moe_unpermute", x, weights)
+        if _lib.native_path():
+            done = _lib.native.moe_unpermute_grad(x, order.rows, weights)
+            if done is not None:
+                return done
         return _Unpermute.apply(x, weights, *order)
     return _unpermute(x, order, weights)
 
