@@ -438,6 +438,23 @@ def test_lengths_of_no_vectors_split(device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("steps", [9, 10, 11, 17, 19, 20, 33, 34, 35, 41, 42, 49, 50, 57])
+def test_splits_that_do_not_divide_the_length(device, steps):
+    """Every part of a split K has a share of it, whatever the scratch memory held: lengths that eight parts, or four, would leave one of empty."""
+    k, seen = 128 * steps, set()
+    for m, n in ((1, 72), (8, 64), (17, 64), (20, 130), (33, 256), (65, 128), (100, 256), (256, 64), (400, 64)):
+        a, b = codes((m, k), m).to(device), codes((n, k), n).to(device)
+        sa, sb = scales(m, 3).to(device), scales(n, 4).to(device)
+        want = bits(_exact(a, b, sa, sb, BF16))
+        for cfg in (None, dict(KERNEL="fallback"), dict(KERNEL="tiled", BLOCK_M=64, BLOCK_N=64, SPLIT_K=8), dict(KERNEL="stream", SPLIT_K=4)):
+            dirty = [torch.full((16 << i,), 0x55, dtype=torch.uint8, device=device) for i in range(10, 18)]
+            del dirty  # (the allocator's free blocks, of the scratch memory's sizes too)
+            assert torch.equal(bits(ops.int8_matmul(a, b, sa, sb, kernel_configs=cfg)), want), (m, n, k, cfg, _lib.last_config())
+            seen.add(_lib.last_config()["SPLIT_K"])
+    assert max(seen) > 1
+
+
+@pytest.mark.gpu
 def test_drawn_products_over_experts(device):
     rng = random.Random(4)
     for i in range(40):

@@ -2406,7 +2406,7 @@ static Int8Schedule simple_int8(const tg::Int8GemmParams& p, int64_t partial_byt
     return best;
 }
 
-static Int8Schedule choose_int8(const tg::Int8GemmParams& p, int64_t partial_bytes, const int32_t* cfg, int32_t ncfg) {
+static Int8Schedule wanted_int8(const tg::Int8GemmParams& p, int64_t partial_bytes, const int32_t* cfg, int32_t ncfg) {
     const int64_t auto_bytes = std::min(partial_bytes, kAutoPartialBytes);
     const int want = cfg_get(cfg, ncfg, TG_CFG_KERNEL);
     const int want_bm = cfg_get(cfg, ncfg, TG_CFG_BLOCK_M), want_bn = cfg_get(cfg, ncfg, TG_CFG_BLOCK_N), want_split = cfg_get(cfg, ncfg, TG_CFG_SPLIT_K);
@@ -2422,6 +2422,15 @@ static Int8Schedule choose_int8(const tg::Int8GemmParams& p, int64_t partial_byt
     if (!int8_fast_layout(p)) return simple_int8(p, auto_bytes);
     if (!p.m_indptr) return cheapest_int8(p, auto_bytes);
     return cheapest_int8_ragged(p);
+}
+
+static Int8Schedule choose_int8(const tg::Int8GemmParams& p, int64_t partial_bytes, const int32_t* cfg, int32_t ncfg) {
+    Int8Schedule s = wanted_int8(p, partial_bytes, cfg, ncfg);
+    if (s.split > 1) {  // every part has a step: one without would leave its partial sums unwritten
+        const int64_t units = s.kernel == 3 ? cdiv(cdiv(p.K, 128), 4) : cdiv(p.K, 128);
+        s.split = (int)cdiv(units, cdiv(units, s.split));
+    }
+    return s;
 }
 
 static int32_t run_int8(tg::Int8GemmParams p, Int8Schedule s, const tg_tensor* workspace, const char* what, uint64_t hip_stream) {
