@@ -399,7 +399,7 @@ int32_t tg_fp8_kv_attention(const tg_tensor* out, const tg_tensor* q, const tg_t
  * cfg: TG_CFG_KERNEL (0, 1 or 3), TG_CFG_BLOCK_M, TG_CFG_BLOCK_N, TG_CFG_SPLIT_K as for tg_fp8_gemm; what does not exist is ignored.
  *
  * tg_int8_ragged_gemm: rows m_indptr[e] .. m_indptr[e + 1] of a with b[e] (E, N, K) and scale_b (E, N) (or one element); m_indptr (E + 1) int32 DEVICE
- * memory, non-decreasing.  Rows that belong to no expert are not written.
+ * memory, non-decreasing.  Rows that belong to no expert are not written.  M below 2^29.
  */
 int32_t tg_int8_gemm(const tg_tensor* c, const tg_tensor* a, const tg_tensor* b, const tg_tensor* scale_a, const tg_tensor* scale_b, const tg_tensor* bias,
                      const tg_tensor* workspace, const int32_t* cfg, int32_t ncfg, int32_t device_id, uint64_t hip_stream);

@@ -36,6 +36,26 @@ def test_tensors_without_elements_are_contiguous():
     assert _lib.load().tg_int8_quant(d(torch.zeros(0, 16, dtype=torch.int8)), d(torch.zeros(0)), d(x), None, 0, 9999, 0) == 0
 
 
+def test_more_rows_of_experts_than_are_counted_are_refused():
+    import ctypes
+    one, (cfg, n) = torch.zeros(1, dtype=torch.int8), _lib.make_cfg(None)
+
+    def rc(m):
+        def desc(t, *shape):
+            d = _lib.make_tensor_desc(t)
+            d.ndim = len(shape)
+            for i, size in enumerate(shape):
+                d.shape[i], d.strides[i] = size, 1
+                for other in shape[i + 1:]:
+                    d.strides[i] *= other
+            return ctypes.byref(d)
+        f32 = torch.zeros(1)
+        return _lib.load().tg_int8_ragged_gemm(desc(torch.zeros(1, dtype=BF16), m, 8), desc(one, m, 16), desc(one, 2, 8, 16), desc(f32, 1), desc(f32, 1),
+                                               desc(torch.zeros(1, dtype=torch.int32), 3), cfg, n, 9999, 0)
+
+    assert rc(2 ** 29 - 1) == -4 and rc(2 ** 29) == -6  # (nothing is read: the device is refused behind all sizes)
+
+
 def test_leaf_held():
     """What a capture asks about a leaf: whether a graph that still lives adds to its gradient."""
     _lib.load()

@@ -2500,6 +2500,8 @@ int32_t tg_int8_ragged_gemm(const tg_tensor* c, const tg_tensor* a, const tg_ten
     tg::Int8GemmParams p{};
     if ((rc = int8_operands(p, c, a, b, scale_a, scale_b))) return rc;
     if (m_indptr->dtype != TG_I32) return fail(TG_ERR_DTYPE, "m_indptr must be int32");
+    // (64 experts' row tiles of 32 are added up in 32 bits, whatever m_indptr holds)
+    if (p.M > INT32_MAX / 4) return fail(TG_ERR_INVALID, "at most %d rows, got %d", INT32_MAX / 4, p.M);
     const int64_t E = b->shape[0];
     if (E > INT32_MAX || m_indptr->shape[0] != E + 1) return fail(TG_ERR_INVALID, "m_indptr must have %lld elements, got %lld", (long long)(E + 1), (long long)m_indptr->shape[0]);
     if (p.M == 0 || p.N == 0 || E == 0) return TG_OK;

@@ -47,7 +47,7 @@ def ragged_int8_matmul(
 ) -> torch.Tensor:
     """``int8_matmul`` of each expert's rows with its weight: rows m_indptr[e] : m_indptr[e + 1] of a (M, K) with b[e] of b (E, N, K) and scale_b[e]
     of scale_b (E, N).  scale_a has M elements, or one; scale_b E * N, or one.  ``m_indptr`` (E + 1) int32 on the device, non-decreasing, is not read by
-    the host (``MoeOrder.indptr``).  Rows of no expert are left as they were in ``out``, and unset without it."""
+    the host (``MoeOrder.indptr``); M is below 2^29.  Rows of no expert are left as they were in ``out``, and unset without it."""
     raise NotImplementedError(f"ragged_int8_matmul is not implemented for this backend: {get_current_backend()}")
 
 
