@@ -10,7 +10,7 @@ import torch
 from oracle import int8_reference as R
 from tilegym_amd import _lib, ops
 
-from .test_int8_ops import BF16, F16, F32, bits, codes, gen, routing, scales
+from .test_int8_ops import BF16, F16, F32, bits, codes, gen, near, routing, scales
 
 
 def test_sort_refuses_a_workspace_that_is_too_small():
@@ -308,6 +308,41 @@ def test_routing_past_32_bit_offsets(device):
     assert torch.equal(gw, (x[:, :1].float() ** 2 * h).expand(tokens, k))  # (sums of equal powers of 2 ** 12 products: exact)
     q, s = ops.silu_mul_quant_int8(there)
     assert torch.equal(q[-5:], ops.silu_mul_quant_int8(there[-5:].contiguous())[0])
+
+
+# ---------------------------------------------------------------------------- routings a router can make
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [BF16, F32])
+def test_an_expert_twice_and_ids_past_32_bits(device, t):
+    """A token that is sent to one expert in several slots, with weights of zero, below zero and infinite; ids whose low 32 bits are an expert's."""
+    tokens, experts, k, h = 60, 6, 4, 136
+    ids = torch.randint(0, experts, (tokens, k), generator=gen(1))
+    ids[::3] = ids[::3, :1]                                        # four times the same
+    ids[5, 1], ids[6, 2], ids[7, 0], ids[8] = 2 ** 32 + 1, -2 ** 33 + 2, 2 ** 62, -2 ** 63
+    order = ops.moe_sort(ids.to(device), experts)
+    indptr, rows, slots = R.ref_sort(ids, experts)
+    assert order.indptr.tolist() == indptr and order.rows.flatten().tolist() == rows and order.slots.tolist() == slots
+    rows = order.rows.cpu()
+    assert [int((rows[i] < 0).sum()) for i in (5, 6, 7, 8)] == [1, 1, 1, 4]
+    x = torch.randn(tokens, h, generator=gen(2)).to(t)
+    there = ops.moe_permute(x.to(device), order)
+    assert torch.equal(bits(there), bits(R.ref_permute(x, rows).to(t)))
+    w = torch.randn(tokens, k, generator=gen(3))
+    w[::4] = 0
+    w[5, 1], w[8, 0] = float("nan"), float("inf")                  # of pairs without an expert
+    y = torch.randn(tokens * k, h, generator=gen(4)).to(t)
+    exact, size = R.ref_unpermute(y, rows, w)
+    near(ops.moe_unpermute(y.to(device), order, w.to(device)), exact, size, t, k)
+    assert not bool(ops.moe_unpermute(y.to(device), order, w.to(device))[8].any())
+    g = torch.randn(tokens, h, generator=gen(5)).to(t)
+    gx, gw = ops.moe_unpermute_backward(g.to(device), y.to(device), order, w.to(device))
+    ex, ew, size = R.ref_unpermute_backward(g, y, rows, w)
+    near(gx, ex, ex.abs(), t, 1)
+    near(gw, ew, size, F32, h / 64 + 16)
+    # an infinite weight of a pair that has an expert shows in its token, and there alone
+    w[3, 0] = float("inf")
+    out = ops.moe_unpermute(y.to(device), order, w.to(device))
+    assert not bool(out[3].isfinite().any()) and bool(out[:3].isfinite().all()) and bool(out[4:].isfinite().all())
 
 
 # ---------------------------------------------------------------------------- the layer in one call
