@@ -101,18 +101,19 @@ struct RaggedWalk {
             if (lane >= d) upto += t;
         }
     }
-    // All tiles there are.
+    // All tiles there are, as far as the host counted them: segments that overlap would have more, and their sum need not stay within 32 bits.
     __device__ __forceinline__ int start(const Int8GemmParams& p, int lane, int tiles_n) {
+        const int most = (int)most_row_tiles(p.M, p.E, BM);
         int total = 0;
         for (e0 = (p.E - 1) / 64 * 64;; e0 -= 64) {
             scan(p, lane);
-            total += __builtin_amdgcn_readlane(upto, 63);
+            total = min(total + __builtin_amdgcn_readlane(upto, 63), most);
             if (e0 == 0) break;
         }
         base = 0;
         return total * tiles_n;
     }
-    // Tile pid, below that total and not below the last one asked for.
+    // Tile pid, below that total and not below the last one asked for (see walking_grid).
     __device__ __forceinline__ void find(const Int8GemmParams& p, int lane, int pid, int tiles_n, int& expert, int& m0, int& rows_valid, int& tile_n) {
         const int row_tile = pid / tiles_n;
         unsigned long long hit;

@@ -472,12 +472,10 @@ __global__ void __launch_bounds__(512, 1) int8_gemm_ring_experts_kernel(const In
 template <int BM, int BN, int STAGES>
 inline hipError_t launch_int8_ring(const Int8GemmParams& p, hipStream_t stream) {
     const int64_t cols = ((int64_t)p.N + BN - 1) / BN;
-    // ragged: no more row tiles than M rows in E segments can have
-    const int64_t tiles = cols * (p.m_indptr ? (int64_t)p.M / BM + (p.E < p.M ? p.E : p.M) : ((int64_t)p.M + BM - 1) / BM);
+    const int64_t tiles = cols * (p.m_indptr ? most_row_tiles(p.M, p.E, BM) : ((int64_t)p.M + BM - 1) / BM);
     if (p.m_indptr) {
         if (tiles > INT32_MAX / 2) return hipErrorInvalidValue;
-        const int units = compute_units();
-        hipLaunchKernelGGL((int8_gemm_ring_experts_kernel<BM, BN, STAGES>), dim3((unsigned)(tiles < units ? tiles : units)), dim3(512), 0, stream, p);
+        hipLaunchKernelGGL((int8_gemm_ring_experts_kernel<BM, BN, STAGES>), dim3((unsigned)walking_grid(tiles, compute_units())), dim3(512), 0, stream, p);
         return hipGetLastError();
     }
     if (tiles * p.split_k * 512 > kMostThreads) return hipErrorInvalidValue;

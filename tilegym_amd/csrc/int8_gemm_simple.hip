@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(256) int8_gemm_simple_kernel(const Int8GemmPar
 }  // namespace
 
 int64_t int8_simple_threads(const Int8GemmParams& p) {
-    const int64_t row_tiles = p.m_indptr ? (int64_t)p.M / 64 + (p.E < p.M ? p.E : p.M) : ((int64_t)p.M + 63) / 64;
+    const int64_t row_tiles = p.m_indptr ? most_row_tiles(p.M, p.E, 64) : ((int64_t)p.M + 63) / 64;
     return row_tiles * (((int64_t)p.N + 63) / 64) * 256 * p.split_k;
 }
 

@@ -5,11 +5,10 @@ namespace tg {
 
 hipError_t run_int8_tile256(const Int8GemmParams& p, hipStream_t s) {
     if (p.K % kKBlock != 0 || p.K < 2 * kKBlock || (int64_t)p.M * p.K >= ((int64_t)1 << 31) || (int64_t)p.N * p.K >= ((int64_t)1 << 31)) return hipErrorInvalidValue;
-    // (ragged: no more row tiles than M rows in E segments can have)
-    const int64_t row_tiles = p.m_indptr ? (int64_t)p.M / 256 + (p.E < p.M ? p.E : p.M) : ((int64_t)p.M + 255) / 256, tiles = row_tiles * ((p.N + 255) / 256);
+    const int64_t row_tiles = p.m_indptr ? most_row_tiles(p.M, p.E, 256) : ((int64_t)p.M + 255) / 256, tiles = row_tiles * ((p.N + 255) / 256);
     if (tiles > INT32_MAX / 2) return hipErrorInvalidValue;
-    const int units = compute_units();
-    const dim3 grid((unsigned)(tiles < units ? tiles : units)), block(256);
+    const int64_t units = compute_units();
+    const dim3 grid((unsigned)(p.m_indptr ? walking_grid(tiles, units) : tiles < units ? tiles : units)), block(256);
     if (p.m_indptr && p.bias) return hipErrorInvalidValue;
 #define TG_LAUNCH(OT, BIAS, RAGGED)                                                                  \
     {                                                                                                \

@@ -209,6 +209,11 @@ struct Int8GemmParams {
     const int* m_indptr;     // ragged: (E + 1); else null
     int E;
 };
+// Row tiles of bm rows that M rows make at most in E segments that do not overlap: what grids are counted for, and no kernel takes more, whatever m_indptr holds.
+constexpr int64_t most_row_tiles(int64_t M, int64_t E, int64_t bm) { return M / bm + (E < M ? E : M); }
+// Workgroups for `tiles` tiles over experts, of which each walks tiles b, b + grid, ...: one to a compute unit.  RaggedWalk asks for tile numbers that do not fall, and xcd_remap's
+// numbers of b, b + grid, ... rise where the grid is a multiple of eight; a workgroup that gets one tile at most needs neither.
+constexpr int64_t walking_grid(int64_t tiles, int64_t units) { return tiles <= units ? tiles : units < 8 ? 8 : units / 8 * 8; }
 // any sizes and addresses
 int64_t int8_simple_threads(const Int8GemmParams& p);
 hipError_t run_int8_simple(const Int8GemmParams& p, hipStream_t s);
