@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from ... import _lib
 from ...backend import register_impl
@@ -43,6 +44,13 @@ def _unpermute(x, order, weights, where="moe_unpermute"):
     out = torch.empty((tokens, x.shape[1]), dtype=x.dtype, device=x.device)
     _lib.moe_unpermute(out, x, order.rows, weights)
     return out
+
+
+def _without_tangents(where, *inputs):
+    """A dual tensor need not require a gradient: without a look at it the result would come back without its tangent."""
+    for t in inputs:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{where}: there are no forward-mode derivatives; only reverse mode is implemented")
 
 
 def _recordable(where, *leaves):
@@ -104,6 +112,7 @@ def moe_sort(topk_ids, num_experts):
 
 @register_impl("moe_permute", backend="hip")
 def moe_permute(x, order):
+    _without_tangents("moe_permute", x)
     if torch.is_grad_enabled() and x.requires_grad:
         _recordable("moe_permute", x)
         if _lib.native_path():
@@ -132,6 +141,7 @@ def moe_permute_quant_int8(x, order):
 
 @register_impl("moe_unpermute", backend="hip")
 def moe_unpermute(x, order, weights=None):
+    _without_tangents("moe_unpermute", x, weights)
     if torch.is_grad_enabled() and (x.requires_grad or (weights is not None and weights.requires_grad)):
         _recordable("moe_unpermute", x, weights)
         if _lib.native_path():
