@@ -1,5 +1,7 @@
 """What the ways to the experts and back do with derivatives that they do not have."""
 
+import gc
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -51,3 +53,60 @@ def test_forward_mode_is_refused_on_a_device(device, monkeypatch, native):
         assert torch.equal(ops.moe_unpermute(ops.moe_permute(x, order), order), 2 * x)
     with pytest.raises(NotImplementedError):
         torch.func.jvp(lambda v: ops.moe_permute(v, order), (x,), (x,))
+
+
+# ---------------------------------------------------------------------------- leaves under capture
+@pytest.mark.gpu
+def test_leaf_held_by_stream(device):
+    """A leaf is held by a graph that lives on another stream than the current one, and not by one on the same."""
+    x, side = torch.zeros(3, device=device, requires_grad=True), torch.cuda.Stream()
+    held = _lib.native.leaf_held
+    assert not held(x)
+    y = x * 2
+    assert not held(x)
+    with torch.cuda.stream(side):
+        assert held(x)
+    del y
+    with torch.cuda.stream(side):
+        assert not held(x)
+        y = x * 2
+        assert not held(x)
+    assert held(x)
+
+
+def _captured(step, leaves, inputs):
+    """The step's gradients, captured and replayed over new inputs with eager steps between, against the eager ones."""
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grads = step()
+    for seed in range(4, 8):
+        with torch.no_grad():
+            for i, t in enumerate(leaves + inputs):
+                t.copy_(torch.rand(t.shape, generator=gen(10 * seed + i)))
+        graph.replay()
+        got = [v.clone() for v in grads]
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_a_leaf_used_twice_in_a_captured_step(device):
+    """A residual beside the experts, weights that two layers share: the second use finds the first one's graph, on the stream of the capture."""
+    tokens, experts, k, h = 30, 8, 2, 128
+    order = ops.moe_sort(routing(tokens, experts, k, 1).to(device), experts)
+    x = torch.randn(tokens, h, generator=gen(1)).to(device).requires_grad_()
+    w = torch.rand(tokens, k, generator=gen(2)).to(device).requires_grad_()
+    g = torch.randn(tokens, h, generator=gen(3)).to(device)
+
+    def step():
+        made = x * 2 + ops.moe_unpermute(ops.moe_permute(x, order) * 3, order, w)
+        made = made + ops.moe_unpermute(ops.moe_permute(made, order) * 2, order, w)
+        return torch.autograd.grad(made, (x, w), g)
+
+    _captured(step, [x, w], [g])

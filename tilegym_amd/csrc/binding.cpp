@@ -11,6 +11,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
@@ -908,7 +909,8 @@ PyObject* py_leaf_held(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
     if (!node) Py_RETURN_FALSE;
     const auto stream = node->stream();
-    if (t->is_cuda() && stream && *stream == c10::hip::getCurrentHIPStream(t->get_device()).unwrap()) Py_RETURN_FALSE;
+    // (the node's stream is one of the tensor's device type, and equal only to such a one: not to a HIPStream's own c10::Stream)
+    if (t->is_cuda() && stream && *stream == c10::impl::VirtualGuardImpl(t->device().type()).getStream(t->device())) Py_RETURN_FALSE;
     Py_RETURN_TRUE;
     END_HANDLE_TH_ERRORS
 }
