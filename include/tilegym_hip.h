@@ -390,8 +390,8 @@ int32_t tg_fp8_kv_attention(const tg_tensor* out, const tg_tensor* q, const tg_t
 /*
  * Products in 8-bit integers, a scale per token and per output channel:
  *   C[m,n] = scale_a[m] * scale_b[n] * sum_k A[m,k] * B[n,k] + bias[n]
- * The sums are int32 and exact (K at most 131071); the rest is fp32: float(sum) * scale_a[m], then one multiply-add with scale_b[n] and the bias,
- * rounded once to c's type.  Every kernel and every split returns the same bits.
+ * The sums are int32 and exact (K at most 131071); the rest is fp32: float(sum) * scale_a[m], then one multiply-add with scale_b[n] and the bias
+ * (without one the product alone, zeros with its sign), rounded once to c's type.  Every kernel and every split returns the same bits.
  *   a (M, K), b (N, K) int8, contiguous; c (M, N) bf16 / f16 / f32, contiguous; scale_a f32, M elements or one; scale_b f32, N elements or one;
  *   bias (N) bf16 / f16 / f32, or NULL.  Rows of a multiple of 16 bytes on 16-byte addresses take the fast kernels.
  *   workspace: NULL, or a 16-byte aligned buffer, contents irrelevant: it holds the partial sums where K is split, tg_int8_gemm_workspace_bytes() bytes (0 where

@@ -27,13 +27,15 @@ __device__ __forceinline__ int weight_row_32(int r) { return (r & 19) | ((r & 4)
 __device__ __forceinline__ int swz32(int r) { return (r >> 1) & 7; }
 
 // One output from its integer sum.  Three roundings at most beside the store's: the sum's conversion (exact to 2^24), the product with the
-// token's scale, and one multiply-add with the channel's scale and the bias.
+// token's scale, and one multiply-add with the channel's scale and the bias.  Where there is none, kNoBias makes it the product alone: a product of -0 stays
+// one, which + 0 would not leave it.
 __device__ __forceinline__ float finish(int sum, float sa, float sb, float bias) { return __builtin_fmaf((float)sum * sa, sb, bias); }
+[[maybe_unused]] constexpr float kNoBias = -0.f;
 
 template <typename T>
 __device__ __forceinline__ float load_any(const void* p, int64_t i) { return (float)((const T*)p)[i]; }
 __device__ __forceinline__ float load_bias(const void* p, int type, int64_t i) {
-    if (!p) return 0.f;
+    if (!p) return kNoBias;
     return type == OUT_F32 ? load_any<float>(p, i) : type == OUT_BF16 ? load_any<__bf16>(p, i) : load_any<_Float16>(p, i);
 }
 
@@ -175,7 +177,7 @@ struct ColumnFactors {
 #if defined(__HIP_DEVICE_COMPILE__)
     float s[8], b[BIAS ? 8 : 1];
     // the output in column i of them from its integer sum
-    __device__ __forceinline__ float finished(int sum, float sa, int i) const { return finish(sum, sa, s[i], BIAS ? b[BIAS ? i : 0] : 0.f); }
+    __device__ __forceinline__ float finished(int sum, float sa, int i) const { return finish(sum, sa, s[i], BIAS ? b[BIAS ? i : 0] : kNoBias); }
     __device__ __forceinline__ void load_scales(const Int8GemmParams& p, const float* sb, int col) {
         if (p.sb_step) {
             const v4f x = *reinterpret_cast<const v4f*>(sb + col), y = *reinterpret_cast<const v4f*>(sb + col + 4);

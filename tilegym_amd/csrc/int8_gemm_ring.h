@@ -184,7 +184,7 @@ __device__ __forceinline__ void ring_store(const Int8GemmParams& p, const RingPa
                 for (int i = 0; i < 8; ++i) {
                     const int at = col_in + part.column(v0 + v) + i;
                     f[v][i] = s_col[at];
-                    b[v][i] = BIAS ? s_bias[at] : 0.f;
+                    b[v][i] = BIAS ? s_bias[at] : kNoBias;
                 }
 #pragma unroll
             for (int tm = 0; tm < TM; ++tm) {
@@ -223,7 +223,7 @@ __device__ __forceinline__ void ring_store(const Int8GemmParams& p, const RingPa
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int at = col_in + part.column(v) + i;
-                if (n0 + at < p.N) put1(p, (m0 + rt) * p.ldc + n0 + at, finish(part.get(v, tm, i), sa, s_col[at], BIAS ? s_bias[at] : 0.f));
+                if (n0 + at < p.N) put1(p, (m0 + rt) * p.ldc + n0 + at, finish(part.get(v, tm, i), sa, s_col[at], BIAS ? s_bias[at] : kNoBias));
             }
     }
 }
