@@ -110,3 +110,30 @@ def test_a_leaf_used_twice_in_a_captured_step(device):
         return torch.autograd.grad(made, (x, w), g)
 
     _captured(step, [x, w], [g])
+
+
+@pytest.mark.gpu
+def test_captures_through_torchs_dispatcher(device):
+    """As the direct calls: while an eager graph of a leaf lives on another stream the capture is refused (the refused ones run no backward pass); without one a
+    step is captured."""
+    t = torch.ops.tilegym_hip
+    tokens, experts, k, h = 30, 8, 2, 128
+    rows = ops.moe_sort(routing(tokens, experts, k, 1).to(device), experts).rows
+    x = torch.randn(tokens, h, generator=gen(1)).to(device).requires_grad_()
+    w = torch.rand(tokens, k, generator=gen(2)).to(device).requires_grad_()
+    g = torch.randn(tokens, h, generator=gen(3)).to(device)
+    held = t.moe_permute(x, rows), t.moe_unpermute(t.moe_permute(g, rows), rows, w)
+    torch.cuda.synchronize()
+    for call in (lambda: t.moe_permute(x, rows), lambda: t.moe_unpermute(t.moe_permute(g, rows), rows, w)):
+        with pytest.raises(RuntimeError, match="eager graph of this leaf"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                torch.zeros(1, device=device)
+                call()
+    del held
+    gc.collect()
+
+    def step():
+        made = x * 2 + t.moe_unpermute(t.moe_permute(x, rows) * 3, rows, w)
+        return torch.autograd.grad(t.moe_unpermute(t.moe_permute(made, rows) * 2, rows, w), (x, w), g)
+
+    _captured(step, [x, w], [g])

@@ -351,12 +351,20 @@ def _(grad_out, x, rows, weights):
     return x.new_empty(x.shape), weights.new_empty(weights.shape)
 
 
+def _recordable(name: str, *leaves) -> None:
+    """The operators themselves run below autograd and see no gradients: what they refuse of a capture is looked for where a graph is recorded."""
+    from .ops.hip.moe_route import _recordable as check
+    check(name, *leaves)
+
+
 def _save_permute(ctx, inputs, output):
+    _recordable("moe_permute", inputs[0])
     ctx.save_for_backward(inputs[1])
 
 
 def _save_unpermute(ctx, inputs, output):
     x, rows, weights = inputs
+    _recordable("moe_unpermute", x, weights)
     ctx.weighted = weights is not None
     ctx.save_for_backward(rows, *([x, weights] if ctx.weighted else []))
 
