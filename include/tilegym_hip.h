@@ -395,7 +395,7 @@ int32_t tg_fp8_kv_attention(const tg_tensor* out, const tg_tensor* q, const tg_t
  *   a (M, K), b (N, K) int8, contiguous; c (M, N) bf16 / f16 / f32, contiguous; scale_a f32, M elements or one; scale_b f32, N elements or one;
  *   bias (N) bf16 / f16 / f32, or NULL.  Rows of a multiple of 16 bytes on 16-byte addresses take the fast kernels.
  *   workspace: NULL, or a 16-byte aligned buffer, contents irrelevant: it holds the partial sums where K is split, tg_int8_gemm_workspace_bytes() bytes (0 where
- *   it is not; with less K is split less).  Calls that share one must not overlap in time.
+ *   it is not, for operands at 16-byte addresses; with less K is split less).  Calls that share one must not overlap in time.
  * cfg: TG_CFG_KERNEL (0, 1 or 3), TG_CFG_BLOCK_M, TG_CFG_BLOCK_N, TG_CFG_SPLIT_K as for tg_fp8_gemm; what does not exist is ignored.
  *
  * tg_int8_ragged_gemm: rows m_indptr[e] .. m_indptr[e + 1] of a with b[e] (E, N, K) and scale_b (E, N) (or one element); m_indptr (E + 1) int32 DEVICE
@@ -474,6 +474,10 @@ int64_t tg_diag_moe_lds_bytes(int64_t tokens, int64_t top_k, int64_t experts, in
  * into (1: uncut, one launch).  The arguments are those of tg_fp8_kv_attention_workspace_bytes.  Host arithmetic, no GPU needed. */
 int32_t tg_diag_kv_attention_form(int64_t tokens, int64_t q_heads, int64_t batch, int64_t kv_heads, int64_t head_dim, int64_t page_size,
                                   int64_t max_pages, int32_t window, int32_t sink_tokens, int32_t* form);
+
+/* The form that tg_int8_gemm takes for these sizes, at aligned addresses and with a workspace of so many bytes: form[0] kernel, form[1] BLOCK_M, form[2] BLOCK_N
+ * (-1: has none), form[3] parts of K.  Host arithmetic, no GPU needed. */
+int32_t tg_diag_int8_gemm_form(int64_t M, int64_t N, int64_t K, int64_t workspace_bytes, const int32_t* cfg, int32_t ncfg, int32_t* form);
 
 #ifdef __cplusplus
 }

@@ -2287,6 +2287,13 @@ static bool int8_fast_layout(const tg::Int8GemmParams& p) {
 // kernel 0 simple, 1 tiles, 3 streaming (bn: weight rows of a workgroup), as in cfg[]
 struct Int8Schedule { int kernel, bm, bn, split; };
 
+// Parts that a K cut in `split` falls into: of whole steps each (the streaming form: pieces of four), and none without one, whose partial sums nothing would write.
+// The choices below weigh no others, so that a workspace of the bytes that they ask for lets them choose the same again.
+static int int8_parts(const tg::Int8GemmParams& p, int kernel, int64_t split) {
+    const int64_t units = cdiv(p.K, kernel == 3 ? 512 : 128);
+    return (int)cdiv(units, cdiv(units, split));
+}
+
 static bool int8_takes(const tg::Int8GemmParams& p, const Int8Schedule& s) {
     if (s.kernel == 0) return true;
     if (!int8_fast_layout(p)) return false;
@@ -2317,6 +2324,9 @@ constexpr Int8Model kInt8Models[] = {{kInt8Decode, 4, 2.34f, 1.29f}, {kInt8Few, 
 struct Int8StreamCost { float fixed, piece, row, row_busy, row_memory, reduce_us, reduce_us_per_mb; };
 constexpr Int8StreamCost kInt8Stream[] = {{3.432f, 0.376f, 0.00306f, 0.00333f, 0.00109f, 2.22f, 0.60f}, {3.761f, 0.548f, 0.00235f, 0.00586f, 0.00012f, 1.93f, 0.81f}};
 constexpr float kInt8SplitMargin = 1.03f;  // a split is a launch more for the host, too
+// Cuts into 2, 4 and 8 are weighed as far as that many parts come of them, as in the fit, and up to 32 rows in both forms: the model thinks too well of the others.  Against the best of
+// fewer parts: the five to seven that a cut into eight leaves, 94 shapes 1.06 times as long (1 x 2543 x 4480 whole 8.5 us, in five parts 9.8); tiles in eight where streaming has
+// fewer, 108 shapes 1.12 times (14 x 1086 x 9088 streaming in four 10.7, 32 x 64 in eight 13.1).
 
 static Int8Schedule cheapest_int8(const tg::Int8GemmParams& p, int64_t partial_bytes) {
     const int64_t M = p.M, N = p.N, K = p.K, steps = cdiv(K, 128);
@@ -2327,7 +2337,8 @@ static Int8Schedule cheapest_int8(const tg::Int8GemmParams& p, int64_t partial_b
         if (s.split > 1) us *= kInt8SplitMargin;
         if (best.kernel == 0 || us < best_us) { best = s; best_us = us; }
     };
-    auto splits = [&](int64_t split) { return split == 1 || (M <= 512 && steps / split >= 4 && split * M * N * 4 <= partial_bytes); };
+    auto whole = [&](int split) { return int8_parts(p, 1, split) == split && (M > 32 || int8_parts(p, 3, split) == split); };
+    auto splits = [&](int split) { return split == 1 || (whole(split) && M <= 512 && steps / split >= 4 && split * M * N * 4 <= partial_bytes); };
     const Int8Model& m = kInt8Models[M <= 16 ? 0 : M <= 64 ? 1 : 2];
     for (int i = 0; i < m.n; ++i) {
         const Int8Cost& t = m.tiles[i];
@@ -2398,16 +2409,17 @@ static Int8Schedule simple_int8(const tg::Int8GemmParams& p, int64_t partial_byt
     const double M = p.M, N = p.N, K = p.K, tiles = (double)(cdiv(p.M, 64) * cdiv(p.N, 64)), steps = (double)cdiv(p.K, 128);
     const double fetch = std::max(tiles * K * (64 + std::min(M, 64.)) / 4.2e6, (M + N) * K / 2.2e6);
     double best_us = 0;
-    for (int split : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
-        if (split > 1 && (steps < 2 * split || M > 512 || split * M * N * 4 > (double)partial_bytes)) break;
+    for (int want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+        const int split = int8_parts(p, 0, want);
+        if (want > 1 && (steps < 2 * want || M > 512 || split * M * N * 4 > (double)partial_bytes)) break;
         double us = std::max(1.2 * std::ceil(steps / split) * std::max(1., tiles * split / 2048), fetch);
         if (split > 1) us = (us + 3 + 0.6e-6 * split * M * N * 4) * kInt8SplitMargin;
-        if (split == 1 || us < best_us) { best.split = split; best_us = us; }
+        if (want == 1 || us < best_us) { best.split = split; best_us = us; }
     }
     return best;
 }
 
-static Int8Schedule wanted_int8(const tg::Int8GemmParams& p, int64_t partial_bytes, const int32_t* cfg, int32_t ncfg) {
+static Int8Schedule choose_int8(const tg::Int8GemmParams& p, int64_t partial_bytes, const int32_t* cfg, int32_t ncfg) {
     const int64_t auto_bytes = std::min(partial_bytes, kAutoPartialBytes);
     const int want = cfg_get(cfg, ncfg, TG_CFG_KERNEL);
     const int want_bm = cfg_get(cfg, ncfg, TG_CFG_BLOCK_M), want_bn = cfg_get(cfg, ncfg, TG_CFG_BLOCK_N), want_split = cfg_get(cfg, ncfg, TG_CFG_SPLIT_K);
@@ -2423,15 +2435,6 @@ static Int8Schedule wanted_int8(const tg::Int8GemmParams& p, int64_t partial_byt
     if (!int8_fast_layout(p)) return simple_int8(p, auto_bytes);
     if (!p.m_indptr) return cheapest_int8(p, auto_bytes);
     return cheapest_int8_ragged(p);
-}
-
-static Int8Schedule choose_int8(const tg::Int8GemmParams& p, int64_t partial_bytes, const int32_t* cfg, int32_t ncfg) {
-    Int8Schedule s = wanted_int8(p, partial_bytes, cfg, ncfg);
-    if (s.split > 1) {  // every part has a step: one without would leave its partial sums unwritten
-        const int64_t units = s.kernel == 3 ? cdiv(cdiv(p.K, 128), 4) : cdiv(p.K, 128);
-        s.split = (int)cdiv(units, cdiv(units, s.split));
-    }
-    return s;
 }
 
 static int32_t run_int8(tg::Int8GemmParams p, Int8Schedule s, const tg_tensor* workspace, const char* what, uint64_t hip_stream) {
@@ -2485,12 +2488,30 @@ int32_t tg_int8_gemm(const tg_tensor* c, const tg_tensor* a, const tg_tensor* b,
     return run_int8(p, s, workspace, "int8_gemm", hip_stream);
 }
 
+// A problem of these sizes at aligned addresses; false: there is none.
+static bool int8_sizes(tg::Int8GemmParams* p, int64_t M, int64_t N, int64_t K) {
+    if (M <= 0 || N <= 0 || K <= 0 || K > kInt8MostK || M > INT32_MAX - 1024 || N > INT32_MAX - 1024) return false;
+    *p = tg::Int8GemmParams{};
+    p->M = (int)M, p->N = (int)N, p->K = (int)K, p->ldc = N, p->vec_store = N % 8 == 0;
+    return true;
+}
+
+// (Planned for aligned addresses, which is all that sizes say: operands at others are taken by the kernel for any address, with its K split as far as these bytes go.)
 int64_t tg_int8_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, const int32_t* cfg, int32_t ncfg) {
-    if (M <= 0 || N <= 0 || K <= 0 || K > kInt8MostK || M > INT32_MAX - 1024 || N > INT32_MAX - 1024) return 0;
-    tg::Int8GemmParams p{};  // (as if at aligned addresses: without them K is not split)
-    p.M = (int)M, p.N = (int)N, p.K = (int)K, p.ldc = N, p.vec_store = N % 8 == 0;
+    tg::Int8GemmParams p;
+    if (!int8_sizes(&p, M, N, K)) return 0;
     const Int8Schedule s = choose_int8(p, INT64_MAX, cfg, ncfg);
     return s.split > 1 ? (int64_t)s.split * M * N * 4 : 0;
+}
+
+int32_t tg_diag_int8_gemm_form(int64_t M, int64_t N, int64_t K, int64_t workspace_bytes, const int32_t* cfg, int32_t ncfg, int32_t* form) {
+    g_err[0] = 0;
+    if (!form) return fail(TG_ERR_NULL, "form: null pointer");
+    tg::Int8GemmParams p;
+    if (!int8_sizes(&p, M, N, K)) return fail(TG_ERR_INVALID, "sizes out of range");
+    const Int8Schedule s = choose_int8(p, workspace_bytes, cfg, ncfg);
+    form[0] = s.kernel, form[1] = s.bm, form[2] = s.bn, form[3] = s.split;
+    return TG_OK;
 }
 
 int32_t tg_int8_ragged_gemm(const tg_tensor* c, const tg_tensor* a, const tg_tensor* b, const tg_tensor* scale_a, const tg_tensor* scale_b,
