@@ -36,9 +36,7 @@ int64_t numel(const tg_tensor* t) {
     return n;
 }
 
-bool contiguous(const tg_tensor* t) {  // (without elements: whatever the strides, as torch has it)
-    for (int i = 0; i < t->ndim; ++i)
-        if (t->shape[i] == 0) return true;
+bool contiguous(const tg_tensor* t) {
     int64_t expect = 1;
     for (int i = t->ndim - 1; i >= 0; --i) {
         if (t->shape[i] != 1 && t->strides[i] != expect) return false;
@@ -47,13 +45,14 @@ bool contiguous(const tg_tensor* t) {  // (without elements: whatever the stride
     return true;
 }
 
-int32_t check_tensor(const tg_tensor* t, const char* name, int ndim) {
+// `empty`: a tensor without elements counts as contiguous whatever its strides, as torch has it.
+int32_t check_tensor(const tg_tensor* t, const char* name, int ndim, bool empty = false) {
     if (!t) return fail(TG_ERR_NULL, "%s: null tensor descriptor", name);
     if (t->ndim < 0 || t->ndim > TG_MAX_DIMS) return fail(TG_ERR_INVALID, "%s: ndim %d out of range", name, t->ndim);
     if (ndim >= 0 && t->ndim != ndim) return fail(TG_ERR_INVALID, "%s: expected %d dims, got %d", name, ndim, t->ndim);
     for (int i = 0; i < t->ndim; ++i)
         if (t->shape[i] < 0) return fail(TG_ERR_INVALID, "%s: negative extent", name);
-    if (!contiguous(t)) return fail(TG_ERR_INVALID, "%s: must be contiguous", name);
+    if (!contiguous(t) && !(empty && numel(t) == 0)) return fail(TG_ERR_INVALID, "%s: must be contiguous", name);
     if (numel(t) > 0 && t->ptr == 0) return fail(TG_ERR_NULL, "%s: null data pointer", name);
     return TG_OK;
 }
@@ -2241,12 +2240,15 @@ int32_t tg_fp8_kv_attention(const tg_tensor* out, const tg_tensor* q, const tg_t
 }
 
 // ---------------------------------------------------------------------------- products in 8-bit integers
+// (the operators from here to the routing's take tensors without elements)
+static int32_t check_extents(const tg_tensor* t, const char* name, int ndim) { return check_tensor(t, name, ndim, true); }
+
 constexpr int64_t kInt8MostK = 131071;  // 2^14 * K stays below 2^31
 
 // a scale per row of an operand, or one for all
 static int32_t check_int8_scale(const tg_tensor* t, const char* name, int64_t rows, int* step) {
     int32_t rc;
-    if ((rc = check_tensor(t, name, -1))) return rc;
+    if ((rc = check_extents(t, name, -1))) return rc;
     if (t->dtype != TG_F32) return fail(TG_ERR_DTYPE, "%s must be f32", name);
     const int64_t n = numel(t);
     if (n != rows && n != 1) return fail(TG_ERR_INVALID, "%s must have %lld elements, or one, got %lld", name, (long long)rows, (long long)n);
@@ -2464,11 +2466,11 @@ int32_t tg_int8_gemm(const tg_tensor* c, const tg_tensor* a, const tg_tensor* b,
                      const tg_tensor* workspace, const int32_t* cfg, int32_t ncfg, int32_t device_id, uint64_t hip_stream) {
     g_err[0] = 0;
     int32_t rc;
-    if ((rc = check_tensor(a, "a", 2)) || (rc = check_tensor(b, "b", 2)) || (rc = check_tensor(c, "c", 2))) return rc;
+    if ((rc = check_extents(a, "a", 2)) || (rc = check_extents(b, "b", 2)) || (rc = check_extents(c, "c", 2))) return rc;
     tg::Int8GemmParams p{};
     if ((rc = int8_operands(p, c, a, b, scale_a, scale_b))) return rc;
     if (bias) {
-        if ((rc = check_tensor(bias, "bias", 1))) return rc;
+        if ((rc = check_extents(bias, "bias", 1))) return rc;
         p.bias_type = io_type_of(bias->dtype);
         if (p.bias_type < 0) return fail(TG_ERR_DTYPE, "bias must be bf16, f16 or f32, got dtype code %d", bias->dtype);
         if (bias->shape[0] != p.N) return fail(TG_ERR_INVALID, "bias must have %d elements, got %lld", p.N, (long long)bias->shape[0]);
@@ -2476,7 +2478,7 @@ int32_t tg_int8_gemm(const tg_tensor* c, const tg_tensor* a, const tg_tensor* b,
     }
     int64_t partial_bytes = 0;
     if (workspace) {
-        if ((rc = check_tensor(workspace, "workspace", -1))) return rc;
+        if ((rc = check_extents(workspace, "workspace", -1))) return rc;
         if (!aligned16(workspace->ptr)) return fail(TG_ERR_INVALID, "workspace must be 16-byte aligned");
         partial_bytes = numel(workspace) * elem_size(workspace->dtype);
     }
@@ -2518,7 +2520,7 @@ int32_t tg_int8_ragged_gemm(const tg_tensor* c, const tg_tensor* a, const tg_ten
                             const tg_tensor* m_indptr, const int32_t* cfg, int32_t ncfg, int32_t device_id, uint64_t hip_stream) {
     g_err[0] = 0;
     int32_t rc;
-    if ((rc = check_tensor(a, "a", 2)) || (rc = check_tensor(b, "b", 3)) || (rc = check_tensor(c, "c", 2)) || (rc = check_tensor(m_indptr, "m_indptr", 1))) return rc;
+    if ((rc = check_extents(a, "a", 2)) || (rc = check_extents(b, "b", 3)) || (rc = check_extents(c, "c", 2)) || (rc = check_extents(m_indptr, "m_indptr", 1))) return rc;
     tg::Int8GemmParams p{};
     if ((rc = int8_operands(p, c, a, b, scale_a, scale_b))) return rc;
     if (m_indptr->dtype != TG_I32) return fail(TG_ERR_DTYPE, "m_indptr must be int32");
@@ -2537,7 +2539,7 @@ int32_t tg_int8_ragged_gemm(const tg_tensor* c, const tg_tensor* a, const tg_ten
 // place (tokens, copies): null, or where a token's copies go
 static int32_t check_places(const tg_tensor* place, const char* name, int64_t tokens) {
     int32_t rc;
-    if ((rc = check_tensor(place, name, 2))) return rc;
+    if ((rc = check_extents(place, name, 2))) return rc;
     if (place->dtype != TG_I32) return fail(TG_ERR_DTYPE, "%s must be int32", name);
     if (place->shape[0] != tokens) return fail(TG_ERR_INVALID, "%s must have a row for each of the %lld tokens, got %lld", name, (long long)tokens, (long long)place->shape[0]);
     if (tokens > INT32_MAX || place->shape[1] > INT32_MAX || tokens * place->shape[1] > INT32_MAX) return fail(TG_ERR_INVALID, "too many rows");
@@ -2548,7 +2550,7 @@ int32_t tg_int8_quant(const tg_tensor* q, const tg_tensor* scales, const tg_tens
                       uint64_t hip_stream) {
     g_err[0] = 0;
     int32_t rc;
-    if ((rc = check_tensor(x, "x", -1)) || (rc = check_tensor(q, "q", -1)) || (rc = check_tensor(scales, "scales", -1))) return rc;
+    if ((rc = check_extents(x, "x", -1)) || (rc = check_extents(q, "q", -1)) || (rc = check_extents(scales, "scales", -1))) return rc;
     const int x_type = io_type_of(x->dtype);
     if (x_type < 0) return fail(TG_ERR_DTYPE, "x must be bf16, f16 or f32");
     if (q->dtype != TG_I8) return fail(TG_ERR_DTYPE, "q must be int8 (dtype code 8)");
@@ -2588,8 +2590,8 @@ int32_t tg_moe_sort(const tg_tensor* topk_ids, int32_t num_experts, const tg_ten
                     const tg_tensor* workspace, int32_t device_id, uint64_t hip_stream) {
     g_err[0] = 0;
     int32_t rc;
-    if ((rc = check_tensor(topk_ids, "topk_ids", -1)) || (rc = check_tensor(indptr, "indptr", 1)) || (rc = check_tensor(rows, "rows", -1)) ||
-        (rc = check_tensor(slots, "slots", -1)))
+    if ((rc = check_extents(topk_ids, "topk_ids", -1)) || (rc = check_extents(indptr, "indptr", 1)) || (rc = check_extents(rows, "rows", -1)) ||
+        (rc = check_extents(slots, "slots", -1)))
         return rc;
     if (topk_ids->dtype != TG_I32 && topk_ids->dtype != TG_I64) return fail(TG_ERR_DTYPE, "topk_ids must be int32 or int64");
     if (indptr->dtype != TG_I32 || rows->dtype != TG_I32 || slots->dtype != TG_I32) return fail(TG_ERR_DTYPE, "indptr, rows and slots must be int32");
@@ -2601,7 +2603,7 @@ int32_t tg_moe_sort(const tg_tensor* topk_ids, int32_t num_experts, const tg_ten
     const int64_t need = tg::moe_sort_workspace_bytes(n, num_experts);
     if (need > 0) {
         if (!workspace) return fail(TG_ERR_INVALID, "%lld slots need a workspace of %lld bytes", (long long)n, (long long)need);
-        if ((rc = check_tensor(workspace, "workspace", -1))) return rc;
+        if ((rc = check_extents(workspace, "workspace", -1))) return rc;
         if (numel(workspace) * elem_size(workspace->dtype) < need || !aligned16(workspace->ptr))
             return fail(TG_ERR_INVALID, "workspace must be 16-byte aligned and hold %lld bytes", (long long)need);
     }
@@ -2618,7 +2620,7 @@ int32_t tg_moe_sort(const tg_tensor* topk_ids, int32_t num_experts, const tg_ten
 static int32_t route_operands(tg::MoeRouteParams& p, int* type, const tg_tensor* by_token, const char* token_name, const tg_tensor* by_row, const char* row_name,
                               const tg_tensor* made, const tg_tensor* rows) {
     int32_t rc;
-    if ((rc = check_tensor(by_token, token_name, 2)) || (rc = check_tensor(by_row, row_name, 2)) || (rc = check_places(rows, "rows", by_token->shape[0]))) return rc;
+    if ((rc = check_extents(by_token, token_name, 2)) || (rc = check_extents(by_row, row_name, 2)) || (rc = check_places(rows, "rows", by_token->shape[0]))) return rc;
     *type = io_type_of(by_token->dtype);
     if (*type < 0) return fail(TG_ERR_DTYPE, "%s must be bf16, f16 or f32", token_name);
     if (by_row->dtype != by_token->dtype) return fail(TG_ERR_DTYPE, "%s and %s must have one dtype", token_name, row_name);
@@ -2627,7 +2629,7 @@ static int32_t route_operands(tg::MoeRouteParams& p, int* type, const tg_tensor*
     if (by_row->shape[0] != T * k || by_row->shape[1] != H)
         return fail(TG_ERR_INVALID, "%s must be (%lld, %lld), got (%lld, %lld)", row_name, (long long)(T * k), (long long)H, (long long)by_row->shape[0], (long long)by_row->shape[1]);
     if (made) {
-        if ((rc = check_tensor(made, "x", 2))) return rc;
+        if ((rc = check_extents(made, "x", 2))) return rc;
         if (made->dtype != by_token->dtype) return fail(TG_ERR_DTYPE, "x and %s must have one dtype", token_name);
         if (made->shape[0] != T * k || made->shape[1] != H) return fail(TG_ERR_INVALID, "x must be (%lld, %lld)", (long long)(T * k), (long long)H);
         p.made = reinterpret_cast<const void*>(made->ptr);
@@ -2639,13 +2641,13 @@ static int32_t route_operands(tg::MoeRouteParams& p, int* type, const tg_tensor*
 }
 static int32_t route_weights(tg::MoeRouteParams& p, const tg_tensor* weights, const tg_tensor* grad_weights) {
     int32_t rc;
-    if ((rc = check_tensor(weights, "weights", 2))) return rc;
+    if ((rc = check_extents(weights, "weights", 2))) return rc;
     p.weights_type = io_type_of(weights->dtype);
     if (p.weights_type < 0) return fail(TG_ERR_DTYPE, "weights must be bf16, f16 or f32");
     if (weights->shape[0] != p.tokens || weights->shape[1] != p.top_k) return fail(TG_ERR_INVALID, "weights must be (%lld, %d)", (long long)p.tokens, p.top_k);
     p.weights = reinterpret_cast<const void*>(weights->ptr);
     if (!grad_weights) return TG_OK;
-    if ((rc = check_tensor(grad_weights, "grad_weights", 2))) return rc;
+    if ((rc = check_extents(grad_weights, "grad_weights", 2))) return rc;
     if (grad_weights->dtype != weights->dtype) return fail(TG_ERR_DTYPE, "grad_weights must have the weights' dtype");
     if (grad_weights->shape[0] != p.tokens || grad_weights->shape[1] != p.top_k) return fail(TG_ERR_INVALID, "grad_weights must be (%lld, %d)", (long long)p.tokens, p.top_k);
     p.grad_weights = reinterpret_cast<void*>(grad_weights->ptr);
