@@ -4,6 +4,7 @@ destination before a vmcnt wait.  The checker on hand-written snippets, then on 
 with inline-assembly loads."""
 import importlib.util
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -88,6 +89,16 @@ def test_spilled_registers_above_the_recorded_count_are_found(tmp_path, kernel):
     assert len(check_hazards.scan_spills(str(path))) == 1
     path.write_text(meta.format(n=0))
     assert check_hazards.scan_spills(str(path)) == []
+
+
+@pytest.mark.parametrize("header", ["int8_gemm_stream.h", "int8_gemm_ring.h", "int8_gemm_tile256.h"])
+def test_every_hand_scheduled_int8_kernel_is_watched_for_spills(tmp_path, header):
+    kernels = re.findall(r"__global__ void [^;{]*?\b(\w+_kernel)\(", open(os.path.join(CSRC, header)).read())
+    assert kernels
+    path = tmp_path / "k.s"
+    for kernel in kernels:
+        path.write_text(f"    .name:           _ZN2tg{len(kernel)}{kernel}ILi1EEEvNS_14Int8GemmParamsE\n    .vgpr_spill_count: 1\n")
+        assert len(check_hazards.scan_spills(str(path))) == 1, kernel
 
 
 def test_static_lds_of_a_kernel_that_uses_all_of_it_dynamically_is_found(tmp_path):
