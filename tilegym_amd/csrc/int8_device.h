@@ -46,8 +46,8 @@ __device__ __forceinline__ int ragged_rows(const Int8GemmParams& p, int e) {
 }
 
 // Workgroup `bid`'s tile of the experts' BM-row tiles x tiles_n columns of them; false: none is left for it.  An expert's row tiles come one after the
-// other over the same columns, so that they share its weight in their XCD's L2.  Every lane of a wave gets the same.
-template <int BM, bool SPREAD>
+// other over the same columns, which they read the same weight rows for.  Every lane of a wave gets the same.
+template <int BM>
 __device__ __forceinline__ bool ragged_tile(const Int8GemmParams& p, int bid, int tiles_n, int lane, int& expert, int64_t& m0, int& rows_valid, int& tile_n) {
     auto scan = [&](int e0, int& rows) {  // row tiles of the experts from e0 up to and with the lane's
         rows = e0 + lane < p.E ? ragged_rows(p, e0 + lane) : 0;
@@ -66,7 +66,7 @@ __device__ __forceinline__ bool ragged_tile(const Int8GemmParams& p, int bid, in
     }
     total = __builtin_amdgcn_readfirstlane(total) * tiles_n;
     if (bid >= total) return false;
-    const int pid = SPREAD ? xcd_remap(bid, total) : bid, row_tile = pid / tiles_n;
+    const int row_tile = bid / tiles_n;
     int base = 0, e0 = 0;
     unsigned long long hit;
     while (!(hit = __ballot(base + upto > row_tile))) {
@@ -78,7 +78,7 @@ __device__ __forceinline__ bool ragged_tile(const Int8GemmParams& p, int bid, in
     expert = __builtin_amdgcn_readfirstlane(e0 + l);
     rows = __builtin_amdgcn_readlane(rows, l);
     const int mine = (rows + BM - 1) / BM, first = __builtin_amdgcn_readfirstlane(base) + __builtin_amdgcn_readlane(upto, l) - mine;
-    const int inside = pid - first * tiles_n;  // of this expert's mine * tiles_n tiles
+    const int inside = bid - first * tiles_n;  // of this expert's mine * tiles_n tiles
     const int at = (inside % mine) * BM;
     tile_n = inside / mine;
     m0 = (int64_t)p.m_indptr[expert] + at;

@@ -1,5 +1,5 @@
 // Products in 8-bit integers for operands that the kernels with direct loads do not take: rows whose length or address is no multiple of
-// 16 bytes, and problems too small to fill one of their tiles' K step.
+// 16 bytes.
 //
 // A workgroup of four waves makes 64 x 64 outputs.  Both operands go through registers to LDS, 64 bytes of K at a time: a thread fetches
 // 16 bytes of one row at any address (the tail of a row byte by byte, zeros beyond it), one step ahead of the MFMAs.  Rows of LDS are 80
@@ -37,7 +37,7 @@ __global__ void __launch_bounds__(256) int8_gemm_simple_kernel(const Int8GemmPar
     int64_t m0 = (int64_t)(blockIdx.x / tiles_n) * 64;
     if constexpr (RAGGED) {
         int tile_n;
-        if (!ragged_tile<64, false>(p, (int)blockIdx.x, tiles_n, lane, expert, m0, rows_valid, tile_n)) return;
+        if (!ragged_tile<64>(p, (int)blockIdx.x, tiles_n, lane, expert, m0, rows_valid, tile_n)) return;
         n0 = tile_n * 64;
     } else {
         rows_valid = (int)min((int64_t)64, p.M - m0);
