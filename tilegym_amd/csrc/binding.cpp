@@ -787,6 +787,7 @@ PyObject* py_int8_moe(PyObject*, PyObject* const* args, Py_ssize_t n) {
     tg_tensor dsort = vector(room(sort_bytes), sort_bytes, 6);
     const int64_t codes = room(rows * std::max(H, I)), scales = room(rows * 4), wide = room(rows * std::max(2 * I, H) * 2);
     tg_tensor dq = matrix(codes, rows, H, TG_I8), ds = vector(scales, rows, TG_F32), dh = matrix(wide, rows, 2 * I, io);
+    // (dy in x's type: one more rounding of each row for half the bytes of what is written and gathered; rows_dtype asks for them whole, one operator after the other)
     tg_tensor dq2 = matrix(codes, rows, I, TG_I8), dy = matrix(wide, rows, H, io);
     at::Tensor scratch = new_tensor({bytes}, at::kByte, *x);
     const uint64_t base = reinterpret_cast<uint64_t>(scratch.data_ptr());
