@@ -12,7 +12,8 @@
 //   * K is any multiple of 16: chunks of the last step behind a row's end are requested from beyond the descriptor's range, which makes them
 //     zeros in LDS;
 //   * partial sums of a split K are int32, and their sum is exact.
-// Bound by the slabs' way through L2 into LDS where tiles are small: 333 x 5120 x 12288 in 64 x 128 tiles 30 us (1.37 POP/s; 566 MB of slabs).
+// Small tiles are bound inside their compute unit: a step of 64 x 128 takes some 580 cycles with 240 workgroups and 680 with four, so it does not wait for a shared L2.
+// The MFMAs are busy 256 of them, fragment reads hold the LDS port for 195, and 24 KB are filled beside these.  333 x 5120 x 12288 takes 30 us (1.37 POP/s).
 #pragma once
 
 #include "int8_device.h"

@@ -4,7 +4,8 @@
 // A workgroup of four waves makes 64 x 64 outputs.  Both operands go through registers to LDS, 64 bytes of K at a time: a thread fetches
 // 16 bytes of one row at any address (the tail of a row byte by byte, zeros beyond it), one step ahead of the MFMAs.  Rows of LDS are 80
 // bytes apart, so that the sixteen rows a fragment read touches start in different banks.  Bound by the latency of that one
-// step (0.6 us), so K is split where tiles are few: 512 x 1001 x 1003 takes 12.7 us, 4096 x 4099 x 4095 306 (449 TOP/s).
+// step (0.6 us), so K is split where tiles are few: 512 x 1001 x 1003 takes 12.7 us, 4096 x 4099 x 4095 306 (449 TOP/s); 8 x 4096 x 4096 from an odd address, for which
+// the Python calls bring no scratch memory, 24 where an aligned call takes 6.6.
 #include "int8_device.h"
 
 namespace tg {

@@ -8,7 +8,7 @@
 // changes no bits.  What a wave does not have (rows behind its R, chunks of K behind a row's end) is requested from beyond the descriptor's
 // range: no memory request, zeros in LDS.
 //
-// Bound by HBM: 16 x 6144 x 4096 takes 8.0 us (3.1 TB/s; the launch and the first piece are half of it), 240 rows over 53 of 64 experts of (2816, 2048) 47 (6.5 TB/s, part of it
+// Bound by HBM: 16 x 6144 x 4096 takes 8.4 us (3.0 TB/s; the launch and the first piece are half of it), 240 rows over 53 of 64 experts of (2816, 2048) 47 to 50 (6.1 to 6.5 TB/s, part of it
 // from the cache behind the L2).
 //
 // Ragged: a grid row per expert for its first 16 rows, which leaves at once where the expert has none, and grid rows past the experts for

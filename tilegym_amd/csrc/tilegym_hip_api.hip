@@ -2404,7 +2404,7 @@ static Int8Schedule cheapest_int8_ragged(const tg::Int8GemmParams& p) {
 // The kernel for any length and address, K split where its tiles are few: 64 bytes of K take a workgroup 0.6 us of latency, unless all of them together
 // are bound by what they fetch (4.2 TB/s, from memory 2.2) or there are more than eight to a compute unit; the sum of the parts costs 3 us and 0.6 per MB.  us, whole / split:
 // 1 x 4478 x 13250 157 / 38 (in 14 parts 31), 30 x 4001 x 4001 39 / 18, 200 x 600 x 16001 152 / 30, 2 x 16677 x 7822 101 / 61 (in three 51); whole 300 x 5001 x 3003 37 / 41,
-// 64 x 28671 x 4095 63 / 70.
+// 64 x 28671 x 4095 63 / 70.  Up to 512 rows, the limit of the other kernels' splits, which was not measured for this one: 512 x 600 x 16001 46 us in four parts, 513 rows 145 in one.
 static Int8Schedule simple_int8(const tg::Int8GemmParams& p, int64_t partial_bytes) {
     Int8Schedule best{0, -1, -1, 1};
     if (p.m_indptr) return best;

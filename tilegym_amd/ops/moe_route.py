@@ -52,21 +52,21 @@ def moe_unpermute_backward(grad_out: torch.Tensor, x: torch.Tensor, order: MoeOr
 
 @dispatch("moe_permute")
 def moe_permute(x: torch.Tensor, order: MoeOrder) -> torch.Tensor:
-    """Each token's row of x (T, H), bf16 / f16 / fp32, in the rows of its pairs: (T * k, H), sorted by expert.  The rows of pairs without an expert,
+    """Each token's row of x (T, H), bf16 / f16 / fp32, contiguous, in the rows of its pairs: (T * k, H), sorted by expert.  The rows of pairs without an expert,
     behind indptr[E], are zeros.  Differentiable in x (by ``moe_permute_backward``)."""
     raise NotImplementedError(f"moe_permute is not implemented for this backend: {get_current_backend()}")
 
 
 @dispatch("moe_permute_quant_int8")
 def moe_permute_quant_int8(x: torch.Tensor, order: MoeOrder) -> Tuple[torch.Tensor, torch.Tensor]:
-    """``quant_int8`` of x (T, H), carried to the rows of each token's pairs: (q (T * k, H) int8, scales (T * k) fp32), in one launch.  The rows of pairs
+    """``quant_int8`` of x (T, H), contiguous, carried to the rows of each token's pairs: (q (T * k, H) int8, scales (T * k) fp32), in one launch.  The rows of pairs
     without an expert have codes of zero and a scale of 1."""
     raise NotImplementedError(f"moe_permute_quant_int8 is not implemented for this backend: {get_current_backend()}")
 
 
 @dispatch("moe_unpermute")
 def moe_unpermute(x: torch.Tensor, order: MoeOrder, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Back to the tokens: out[t] = sum_j weights[t, j] * x[row of (t, j)], x (T * k, H) bf16 / f16 / fp32, weights (T, k) fp32 / bf16 / f16, or ones.
+    """Back to the tokens: out[t] = sum_j weights[t, j] * x[row of (t, j)], x (T * k, H) bf16 / f16 / fp32, weights (T, k) fp32 / bf16 / f16, or ones; all contiguous.
     Summed in fp32, in the order of the slots, rounded once.  Pairs without an expert add nothing, whatever their rows and weights hold.
-    Differentiable in x and weights (by ``moe_unpermute_backward``)."""
+    Differentiable in x and weights (by ``moe_unpermute_backward``, which makes both gradients whichever is asked for)."""
     raise NotImplementedError(f"moe_unpermute is not implemented for this backend: {get_current_backend()}")
