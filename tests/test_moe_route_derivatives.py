@@ -20,6 +20,8 @@ def _refusals(order, x, y, w, dual):
     t = torch.ops.tilegym_hip
     calls = [lambda: ops.moe_permute(dual(x), order), lambda: ops.moe_unpermute(dual(y), order), lambda: ops.moe_unpermute(dual(y), order, w),
              lambda: ops.moe_unpermute(y, order, dual(w))]
+    calls += [lambda: ops.moe_permute_backward(dual(y), order), lambda: ops.moe_unpermute_backward(dual(x), y, order, w), lambda: ops.moe_unpermute_backward(x, dual(y), order, w),
+              lambda: ops.moe_unpermute_backward(x, y, order, dual(w))]
     if x.is_cuda:
         calls += [lambda: t.moe_permute(dual(x), order.rows), lambda: t.moe_unpermute(y, order.rows, dual(w))]
     for call in calls:

@@ -682,10 +682,13 @@ PyObject* py_moe_sort(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// A dual tensor of forward-mode differentiation: not plain, the Python implementation refuses it.
+bool dual(const at::Tensor* t) { return t && t->_fw_grad(0).defined(); }
+
 // The x (rows, H) and the places (T, k) of the ways there and back; false: not plain.
 bool route_operands(PyObject* x, PyObject* rows, const at::Tensor** px, const at::Tensor** prows, tg_tensor* dx, tg_tensor* drows) {
     const at::Tensor *tx = tensor_of(x), *tr = tensor_of(rows);
-    if (!on_gpu(tx) || !io_type(tx->scalar_type()) || tx->dim() != 2 || !plain(tr, at::kInt, 2) || tx->device() != tr->device()) return false;
+    if (!on_gpu(tx) || !io_type(tx->scalar_type()) || tx->dim() != 2 || !plain(tr, at::kInt, 2) || tx->device() != tr->device() || dual(tx)) return false;
     *px = tx;
     *prows = tr;
     return describe(*tx, dx) && describe(*tr, drows);
@@ -712,7 +715,8 @@ PyObject* py_moe_unpermute(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor *x, *rows;
     tg_tensor dout, dx, drows, dw;
     const tg_tensor* weights;
-    if (!route_operands(args[0], args[1], &x, &rows, &dx, &drows) || x->size(0) != rows->numel() || !optional_tensor(args[2], *x, &dw, &weights)) Py_RETURN_NONE;
+    if (!route_operands(args[0], args[1], &x, &rows, &dx, &drows) || x->size(0) != rows->numel() || !optional_tensor(args[2], *x, &dw, &weights) || dual(tensor_of(args[2])))
+        Py_RETURN_NONE;
     at::Tensor out = new_tensor({rows->size(0), x->size(1)}, x->scalar_type(), *x);
     if (!describe(out, &dout)) Py_RETURN_NONE;
     if (!launched(*x, "tg_moe_unpermute", [&](int32_t device, uint64_t stream) { return g_moe_unpermute(&dout, &dx, &drows, weights, device, stream); }))
@@ -728,7 +732,7 @@ PyObject* py_moe_unpermute_backward(PyObject*, PyObject* const* args, Py_ssize_t
     const at::Tensor *x, *rows, *grad = tensor_of(args[0]), *weights = tensor_of(args[3]);
     tg_tensor dgx, dgw, dgrad, dx, drows, dw;
     if (!route_operands(args[1], args[2], &x, &rows, &dx, &drows) || !on_gpu(grad) || grad->device() != x->device() || !grad->is_contiguous() ||
-        !on_gpu(weights) || weights->device() != x->device() || !io_type(weights->scalar_type()) || !describe(*grad, &dgrad) || !describe(*weights, &dw))
+        !on_gpu(weights) || weights->device() != x->device() || !io_type(weights->scalar_type()) || dual(grad) || dual(weights) || !describe(*grad, &dgrad) || !describe(*weights, &dw))
         Py_RETURN_NONE;
     at::Tensor gx = new_tensor(x->sizes(), x->scalar_type(), *x), gw = new_tensor(weights->sizes(), weights->scalar_type(), *x);
     if (!describe(gx, &dgx) || !describe(gw, &dgw)) Py_RETURN_NONE;
@@ -895,7 +899,7 @@ PyObject* py_moe_unpermute_grad(PyObject*, PyObject* const* args, Py_ssize_t n) 
     const at::Tensor *x, *rows, *weights = args[2] == Py_None ? nullptr : tensor_of(args[2]);
     tg_tensor dx, drows;
     if (!route_operands(args[0], args[1], &x, &rows, &dx, &drows) || !x->is_contiguous() || x->size(0) != rows->numel() ||
-        (args[2] != Py_None && (!on_gpu(weights) || weights->device() != x->device() || !io_type(weights->scalar_type()) || !weights->is_contiguous() ||
+        (args[2] != Py_None && (!on_gpu(weights) || dual(weights) || weights->device() != x->device() || !io_type(weights->scalar_type()) || !weights->is_contiguous() ||
                                 weights->sizes() != rows->sizes())))
         Py_RETURN_NONE;
     return THPVariable_Wrap(Unpermute::apply(*x, *rows, weights ? std::optional<at::Tensor>(*weights) : std::nullopt));

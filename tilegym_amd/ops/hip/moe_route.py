@@ -18,11 +18,19 @@ def _pairs(where, order):
     return rows.shape[0], rows.shape[1]
 
 
+def _without_tangents(where, *inputs):
+    """A dual tensor need not require a gradient: without a look at it the result would come back without its tangent.  (The native calls leave these to here.)"""
+    for t in inputs:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{where}: there are no forward-mode derivatives; only reverse mode is implemented")
+
+
 def _permute(x, order):
     if _lib.native_path():
         done = _lib.native.moe_permute(x, order.rows)
         if done is not None:
             return done
+    _without_tangents("moe_permute", x)
     _one_device("moe_permute", x, order.rows)
     tokens, k = _pairs("moe_permute", order)
     if x.dim() != 2 or x.shape[0] != tokens:
@@ -37,6 +45,7 @@ def _unpermute(x, order, weights, where="moe_unpermute"):
         done = _lib.native.moe_unpermute(x, order.rows, weights)
         if done is not None:
             return done
+    _without_tangents(where, x, weights)
     _one_device(where, x, order.rows, weights)
     tokens, k = _pairs(where, order)
     if x.dim() != 2 or x.shape[0] != tokens * k:
@@ -44,13 +53,6 @@ def _unpermute(x, order, weights, where="moe_unpermute"):
     out = torch.empty((tokens, x.shape[1]), dtype=x.dtype, device=x.device)
     _lib.moe_unpermute(out, x, order.rows, weights)
     return out
-
-
-def _without_tangents(where, *inputs):
-    """A dual tensor need not require a gradient: without a look at it the result would come back without its tangent."""
-    for t in inputs:
-        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-            raise NotImplementedError(f"{where}: there are no forward-mode derivatives; only reverse mode is implemented")
 
 
 def _recordable(where, *leaves):
@@ -112,8 +114,8 @@ def moe_sort(topk_ids, num_experts):
 
 @register_impl("moe_permute", backend="hip")
 def moe_permute(x, order):
-    _without_tangents("moe_permute", x)
     if torch.is_grad_enabled() and x.requires_grad:
+        _without_tangents("moe_permute", x)
         _recordable("moe_permute", x)
         if _lib.native_path():
             done = _lib.native.moe_permute_grad(x, order.rows)
@@ -141,8 +143,8 @@ def moe_permute_quant_int8(x, order):
 
 @register_impl("moe_unpermute", backend="hip")
 def moe_unpermute(x, order, weights=None):
-    _without_tangents("moe_unpermute", x, weights)
     if torch.is_grad_enabled() and (x.requires_grad or (weights is not None and weights.requires_grad)):
+        _without_tangents("moe_unpermute", x, weights)
         _recordable("moe_unpermute", x, weights)
         if _lib.native_path():
             done = _lib.native.moe_unpermute_grad(x, order.rows, weights)
@@ -164,6 +166,7 @@ def moe_unpermute_backward(grad_out, x, order, weights):
         done = _lib.native.moe_unpermute_backward(grad_out, x, order.rows, weights)
         if done is not None:
             return done
+    _without_tangents("moe_unpermute_backward", grad_out, x, weights)
     _one_device("moe_unpermute_backward", grad_out, x, order.rows, weights)
     grad_x, grad_weights = torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty(weights.shape, dtype=weights.dtype, device=x.device)
     _lib.moe_unpermute_backward(grad_x, grad_weights, grad_out, x, order.rows, weights)

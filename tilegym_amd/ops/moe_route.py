@@ -1,7 +1,7 @@
 """Tokens sorted by expert, carried to the experts' rows and back with the router's weights, and the gradients of both ways: what makes the
 segments that ``ragged_block_scaled_bmm`` and ``ragged_int8_matmul`` multiply.
 
-Gradients are those of reverse mode, and once: dual tensors are refused, and so are second derivatives.
+Gradients are those of reverse mode, and once: dual tensors are refused here and in the backward operators, and so are second derivatives.
 
 Forward and backward passes can be captured into a graph.  What is refused while capturing is a leaf that an eager graph on another stream still holds: its gradient would be
 added there (``moe_permute_backward`` and ``moe_unpermute_backward`` take no part in autograd and can always be captured).
