@@ -1,6 +1,7 @@
 """What the ways to the experts and back do with derivatives that they do not have."""
 
 import gc
+import os
 
 import pytest
 import torch
@@ -58,6 +59,34 @@ def test_forward_mode_is_refused_on_a_device(device, monkeypatch, native):
 
 
 # ---------------------------------------------------------------------------- leaves under capture
+def test_leaves_without_a_device():
+    """No capture is asked for where no device has been used: shapes of graphs are inferred, and tensors of the host are refused for what they are."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+from tilegym_amd import ops
+t = torch.ops.tilegym_hip
+with FakeTensorMode():
+    x, rows = torch.empty(7, 40, device="cuda", requires_grad=True), torch.empty(7, 3, dtype=torch.int32, device="cuda")
+    w = torch.empty(7, 3, device="cuda", requires_grad=True)
+    y = t.moe_unpermute(t.moe_permute(x, rows), rows, w)
+    assert y.shape == (7, 40) and y.requires_grad
+assert not torch.cuda.is_initialized()
+rows = torch.zeros(2, 1, dtype=torch.int32)
+try:
+    ops.moe_permute(torch.zeros(2, 8, requires_grad=True), ops.MoeOrder(rows, rows, rows))
+except RuntimeError as e:
+    assert "HIP device" in str(e), e
+else:
+    raise AssertionError
+"""
+    # (a process of its own: the others' may have used a device)
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=110, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
 @pytest.mark.gpu
 def test_leaf_held_by_stream(device):
     """A leaf is held by a graph that lives on another stream than the current one, and not by one on the same."""
@@ -139,3 +168,32 @@ def test_captures_through_torchs_dispatcher(device):
         return torch.autograd.grad(t.moe_unpermute(t.moe_permute(made, rows) * 2, rows, w), (x, w), g)
 
     _captured(step, [x, w], [g])
+
+
+@pytest.mark.gpu
+def test_an_eager_graph_on_the_capturing_stream(device):
+    """What is documented beside the refusal: a leaf whose eager graph lives on the stream that captures is taken, forwards and backwards."""
+    tokens, experts, k, h = 30, 8, 2, 128
+    order = ops.moe_sort(routing(tokens, experts, k, 1).to(device), experts)
+    x = torch.randn(tokens, h, generator=gen(1)).to(device).requires_grad_()
+    w = torch.rand(tokens, k, generator=gen(2)).to(device).requires_grad_()
+    g = torch.randn(tokens, h, generator=gen(3)).to(device)
+
+    def step():
+        return torch.autograd.grad(ops.moe_unpermute(ops.moe_permute(x, order) * 2, order, w), (x, w), g)
+
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        want = step()
+        held = ops.moe_permute(x, order), ops.moe_unpermute(ops.moe_permute(g, order), order, w)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        grads = step()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(grads, want))
+        for t in grads:
+            t.zero_()
+    assert held[0].requires_grad and held[1].requires_grad

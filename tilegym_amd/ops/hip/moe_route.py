@@ -58,7 +58,7 @@ def _unpermute(x, order, weights, where="moe_unpermute"):
 def _recordable(where, *leaves):
     """Under capture a leaf's gradient is added to on the stream of the graph that first used it.  Where that is an eager graph which still lives, the backward
     pass would wait for its stream from within the capture, an error that torch's backward threads do not survive: refused here instead."""
-    if not torch.cuda.is_current_stream_capturing():
+    if not torch.cuda.is_initialized() or not torch.cuda.is_current_stream_capturing():  # (shapes may be inferred where there is no device to ask)
         return
     for t in leaves:
         if t is not None and t.requires_grad and t.is_leaf and (not _lib.native_path() or _lib.native.leaf_held(t)):
